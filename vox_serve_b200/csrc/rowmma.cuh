@@ -1,0 +1,42 @@
+// What the operators share whose weights a row brings with it (lora.cu, moe_layer.cu): weights as the streamed operand of mma.sync, taken from HBM
+// straight into registers, a few rows of activations as the other operand.  Few rows make these products a stream of weights, which mma.sync
+// keeps up with (an m16n8k16 product takes 2 clocks of an SM for 512 bytes of weights that arrive in 22).
+#pragma once
+#include "common.cuh"
+
+namespace vb {
+
+// 16 bytes that are read once: past L1
+__device__ __forceinline__ uint4 ldg_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// An fp32 value as bf16 parts whose sum it is: the upper 8 bits of the significand, the next 8, the last 8 (cut off, not rounded, so that a part
+// never overflows and three of them lose nothing).  Two parts are off by at most 2^-15 of the value, three by nothing.  What is not finite
+// stays whole in the first part (inf - inf would make it NaN).
+__device__ __forceinline__ float bf16_cut(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
+__device__ __forceinline__ void bf16_parts(float v, float& hi, float& mid, float& lo) {
+  hi = bf16_cut(v);
+  if ((__float_as_uint(v) & 0x7f800000u) == 0x7f800000u) {
+    hi = __uint_as_float((__float_as_uint(v) & 0x7fffffffu) > 0x7f800000u ? 0x7fc00000u : __float_as_uint(v));
+    mid = lo = 0.f;
+    return;
+  }
+  const float r = v - hi;
+  mid = bf16_cut(r);
+  lo = r - mid;
+}
+// two neighbours' upper halves as one register (both hold bf16 values)
+__device__ __forceinline__ uint32_t pack_cut(float first, float second) {
+  return __byte_perm(__float_as_uint(first), __float_as_uint(second), 0x7632);
+}
+
+}  // namespace vb

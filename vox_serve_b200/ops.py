@@ -1880,3 +1880,291 @@ def gemm_grouped_glu(x: torch.Tensor, w: "PackedWeight", out: torch.Tensor, N: i
     call("vb_gemm_bf16_grouped_glu", out.data_ptr(), w.data.data_ptr(), tensor_map_2d(x, t_tile).ptr, x.shape[0], N, K, N // 2,
          w.tile_rows, N // 2, t_tile, _p(tile_group), int(group_bytes), float(limit), float(slope), _stream())
     return out
+
+
+# ----------------------------------------------------------------------------------------------
+# weights that a row brings with it: adapters of many requests (lora.cu), experts of a decode step (moe_layer.cu)
+# ----------------------------------------------------------------------------------------------
+def _need_here(who: str, *ts):
+    """tensors of the current device: a launch goes to its stream"""
+    here = None
+    for t in ts:
+        if t is None:
+            continue
+        if here is None and t.is_cuda:
+            here = _device_index()
+        if not t.is_cuda or t.device.index != here:
+            raise VoxB200Error(f"{who}: tensors on the current device are needed, not on {t.device}")
+
+
+def _refuse(cond: bool, msg: str) -> None:
+    if cond:
+        raise VoxB200Error(msg)
+
+
+class LoraBank:
+    """Low-rank adapters of ONE projection, ``slots`` of them on the device: columns in ``widths`` (q | k | v, gate | up, or one slice), each slice with
+    an A of its own.  ``load`` lays an adapter out as the kernels read it (vb_lora); ranks up to ``rank`` (at most 128), padded with zeros."""
+
+    def __init__(self, slots: int, K: int, widths, rank: int, device="cuda"):
+        widths = tuple(int(w) for w in widths)
+        _refuse(not 1 <= slots <= 1023, f"LoraBank: {slots} adapters; 1 to 1023")
+        _refuse(not 1 <= rank <= 128, f"LoraBank: rank {rank}; 1 to 128")
+        _refuse(not 1 <= len(widths) <= 4 or any(w < 8 or w % 8 for w in widths), f"LoraBank: slices {widths}; one to four, multiples of 8 columns")
+        _refuse(K < 8 or K % 8 != 0, f"LoraBank: inputs of {K}; a multiple of 8")
+        self.slots, self.K, self.widths, self.rank = int(slots), int(K), widths, int(rank)
+        self.N = sum(widths)
+        self.rank_pad = next(r for r in (16, 32, 64, 128) if rank <= r)
+        kb, blocks = (K + 31) // 32, sum((w + 31) // 32 for w in widths)
+        self.a = torch.zeros(slots, len(widths) * self.rank_pad * kb * 32, dtype=BF16, device=device)
+        self.b = torch.zeros(slots, blocks * 32 * self.rank_pad, dtype=BF16, device=device)
+        self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
+        self._widths = (ctypes.c_int32 * len(widths))(*widths)
+        self._ptrs = (self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(), self.slots, self.rank_pad)
+        self._ws_floats: Dict[int, int] = {}
+
+    def load(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
+        """a [slices, r, K] (or [r, K] of one slice), b [N, r], r <= rank; values become bf16.  Rows read the adapter from the next call on
+        this stream on; a call that runs on another stream meanwhile is the caller's to wait for."""
+        _refuse(not 0 <= slot < self.slots, f"LoraBank.load: slot {slot} of {self.slots}")
+        S, rp = len(self.widths), self.rank_pad
+        a = a[None] if a.dim() == 2 else a
+        r = a.shape[1] if a.dim() == 3 else -1
+        _refuse(tuple(a.shape) != (S, r, self.K) or not 1 <= r <= self.rank, f"LoraBank.load: A {tuple(a.shape)}; [{S}, r <= {self.rank}, {self.K}] is needed")
+        _refuse(tuple(b.shape) != (self.N, r), f"LoraBank.load: B {tuple(b.shape)}; [{self.N}, {r}] is needed")
+        dev = self.a.device
+        kb = (self.K + 31) // 32
+        ap = torch.zeros(S, rp, kb * 32, dtype=BF16, device=dev)
+        ap[:, :r, :self.K] = a.to(device=dev, dtype=BF16)
+        # rows as m16 tiles (halves h of 8 rows), k as 8 per lane in two product steps of two pairs
+        ap = ap.view(S * rp // 16, 2, 8, kb, 4, 2, 2, 2).permute(0, 3, 5, 2, 4, 6, 1, 7)
+        self.a[slot].copy_(ap.reshape(-1))
+        blocks, n0 = [], 0
+        for w in self.widths:
+            bp = torch.zeros((w + 31) // 32 * 32, rp, dtype=BF16, device=dev)
+            bp[:w, :r] = b[n0:n0 + w].to(device=dev, dtype=BF16)
+            # 32 columns as 4 lanes of 8 neighbours in four n8 tiles; k as pairs of two halves
+            blocks.append(bp.view(-1, 4, 2, 2, 2, rp // 16, 2, 4, 2).permute(0, 5, 2, 1, 4, 7, 3, 6, 8).reshape(-1))
+            n0 += w
+        self.b[slot].copy_(torch.cat(blocks))
+        self.scale[slot] = float(scale)
+
+    def clear(self, slot: int) -> None:
+        """the slot's adapter becomes zero"""
+        _refuse(not 0 <= slot < self.slots, f"LoraBank.clear: slot {slot} of {self.slots}")
+        self.a[slot].zero_()
+        self.b[slot].zero_()
+        self.scale[slot] = 0.0
+
+    def _workspace(self, T: int) -> torch.Tensor:
+        n = self._ws_floats.get(T)
+        if n is None:
+            n = self._ws_floats[T] = _lib.load().vb_lora_workspace_bytes(T, self.K, self.slots, self.rank_pad, len(self.widths)) // 4
+        return torch.empty(n, dtype=torch.float32, device=self.a.device)
+
+
+class LoraPlan:
+    """Rows of a step by adapter (``lora_plan``): made once per step, read by every projection of every layer."""
+
+    def __init__(self, max_rows: int, slots: int, device="cuda"):
+        _refuse(max_rows < 1 or not 1 <= slots <= 1023, f"LoraPlan: {max_rows} rows, {slots} adapters (1 to 1023)")
+        self.max_rows, self.slots, self.n_rows = int(max_rows), int(slots), 0
+        lib = _lib.load()
+        tiles = max(lib.vb_lora_max_tiles(min(max_rows, 64), slots), lib.vb_lora_max_tiles(max_rows, slots))
+        self.order = torch.zeros(max_rows, dtype=torch.int32, device=device)
+        self.tiles = torch.zeros(1 + tiles, 4, dtype=torch.int32, device=device)
+
+
+def lora_plan(plan: LoraPlan, ids: torch.Tensor) -> LoraPlan:
+    """ids int32 [T]: the adapter of every row; what is not 0 .. slots - 1 (-1) has none."""
+    _need_here("lora_plan", ids, plan.order)
+    _refuse(ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous(), "lora_plan: int32 ids in one dimension are needed")
+    T = ids.numel()
+    _refuse(T > plan.max_rows, f"lora_plan: {T} rows; the plan holds {plan.max_rows}")
+    if T:
+        call("vb_lora_plan", plan.order.data_ptr(), plan.tiles.data_ptr(), ids.data_ptr(), T, plan.slots, _stream())
+    plan.n_rows = T
+    return plan
+
+
+def _lora_check(who: str, x: torch.Tensor, bank: LoraBank, plan: LoraPlan) -> None:
+    _need_here(who, x, bank.a, plan.order)
+    _refuse(x.dtype != BF16 or x.dim() != 2 or x.shape[1] != bank.K or (x.stride(1) != 1 and x.shape[0] > 0), f"{who}: bf16 rows of {bank.K} are needed")
+    _refuse(plan.slots != bank.slots, f"{who}: the plan counts {plan.slots} adapters, the bank {bank.slots}")
+    _refuse(plan.n_rows != x.shape[0], f"{who}: {x.shape[0]} rows, the plan was made for {plan.n_rows}")
+
+
+def lora(x: torch.Tensor, bank: LoraBank, plan: LoraPlan, out: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """out[t] = base[t] + B_a (scale_a A_a x[t]) with the adapter a of row t in ``plan`` (none: base[t]).  x bf16 [T, K]; out fp32 [T, N] (one more split-K
+    plane of the projection: ``gemm`` mode 1) or bf16 (rounded once), by ``out``, else by ``base``, else fp32.  ``base``: of out's type, may be out
+    itself; None: zeros."""
+    _lora_check("lora", x, bank, plan)
+    T, N = x.shape[0], bank.N
+    if out is None:
+        out = torch.empty(T, N, dtype=torch.float32 if base is None else base.dtype, device=x.device)
+    f32 = out.dtype == torch.float32
+    for t in (out, base):
+        if t is not None:
+            _need_here("lora", t)
+            _refuse(t.dtype != out.dtype or not (f32 or t.dtype == BF16) or tuple(t.shape) != (T, N) or t.stride(1) != 1,
+                    f"lora: out and base are fp32 or bf16 rows [{T}, {N}] of one type")
+    if T == 0:
+        return out
+    ws = bank._workspace(T)
+    call("vb_lora", out.data_ptr(), out.stride(0) if T > 1 else N, _p(base), base.stride(0) if base is not None and T > 1 else N, int(f32), x.data_ptr(),
+         x.stride(0) if T > 1 else bank.K, *bank._ptrs, bank._widths, len(bank.widths), plan.order.data_ptr(), plan.tiles.data_ptr(), T, bank.K, ws.data_ptr(),
+         ws.numel() * 4, _stream())
+    return out
+
+
+def lora_gate_up(x: torch.Tensor, bank: LoraBank, plan: LoraPlan, planes: torch.Tensor, half: int, out=None):
+    """silu(gate) * up with the adapters' products added to both: planes fp32 [splits, T, 2 * ceil(ff / half) * half] are what ``gemm`` mode 1 left of
+    weights packed by ``interleave_gate_up(.., half)``; bank: two slices of ff columns.  out: bf16 [T, ff] (row-major, or a TiledAct)."""
+    _lora_check("lora_gate_up", x, bank, plan)
+    _refuse(len(bank.widths) != 2 or bank.widths[0] != bank.widths[1], f"lora_gate_up: a bank of gate | up is needed, not of slices {bank.widths}")
+    _refuse(half not in (16, 32, 48, 64), f"lora_gate_up: tiles of {half} gate rows (16, 32, 48 or 64)")
+    _need_here("lora_gate_up", planes)
+    T, ff = x.shape[0], bank.widths[0]
+    width = (ff + half - 1) // half * half * 2
+    _refuse(planes.dtype != torch.float32 or planes.dim() != 3 or planes.shape[0] < 1 or tuple(planes.shape[1:]) != (T, width) or not planes.is_contiguous(),
+            f"lora_gate_up: fp32 planes [splits, {T}, {width}] are needed")
+    tiled = isinstance(out, TiledAct)
+    if tiled:
+        _need_here("lora_gate_up", out.data)
+        _refuse(out.T != T or out.K != ff, f"lora_gate_up: tiled rows [{out.T}, {out.K}] are not [{T}, {ff}]")
+    elif out is None:
+        out = torch.empty(T, ff, dtype=BF16, device=x.device)
+    else:
+        _need_here("lora_gate_up", out)
+        _refuse(out.dtype != BF16 or tuple(out.shape) != (T, ff) or out.stride(1) != 1, f"lora_gate_up: out is bf16 [{T}, {ff}]")
+    if T == 0:
+        return out
+    ws = bank._workspace(T)
+    call("vb_lora_gate_up", out.data.data_ptr() if tiled else out.data_ptr(), ff if tiled or T == 1 else out.stride(0), out.t_tile if tiled else 0,
+         planes.data_ptr(), planes.shape[0], int(half), ff, x.data_ptr(), x.stride(0) if T > 1 else bank.K, *bank._ptrs, plan.order.data_ptr(),
+         plan.tiles.data_ptr(), T, bank.K, ws.data_ptr(), ws.numel() * 4, _stream())
+    return out
+
+
+MOE_LAYER_ACTS = {"silu_glu": 0, "clamped_glu": 1, "relu2": 2, "gelu": 3, "gelu_tanh": 4}
+MOE_LAYER_ROUTERS = {"softmax": 0, "sigmoid": 1, "softmax_all": 2, "table": 3}
+MOE_LAYER_MAX_ROWS = 64
+
+
+class MoeWeights:
+    """The matrices of a mixture's experts as ``moe_layer`` reads them: packed tiles (the buffers that the projections of larger steps multiply), every
+    expert's gate | up rows after the other's, the shared expert last; the down matrices side by side along k."""
+    __slots__ = ("up", "down", "experts", "width", "ff", "shared_ff", "act", "limit", "slope")
+
+    def __init__(self, up: PackedWeight, down: PackedWeight, experts: int, width: int, ff: int, shared_ff: int = 0, act: str = "silu_glu",
+                 limit: float = 0.0, slope: float = 1.702):
+        _refuse(act not in MOE_LAYER_ACTS, f"MoeWeights: activation {act!r}; one of {sorted(MOE_LAYER_ACTS)}")
+        _refuse(act == "clamped_glu" and not limit > 0.0, f"MoeWeights: the clamped gate needs a positive limit, not {limit}")
+        _refuse(not 1 <= experts <= 1024, f"MoeWeights: {experts} experts; 1 to 1024")
+        _refuse(width < 8 or width % 8 != 0, f"MoeWeights: width {width}; a multiple of 8")
+        _refuse(ff < 64 or ff % 64 != 0 or shared_ff < 0 or shared_ff % 64 != 0, f"MoeWeights: expert widths {ff} and {shared_ff}; multiples of 64 (pack pads)")
+        rows = 2 if act.endswith("glu") else 1
+        n_all = experts * ff + shared_ff
+        _refuse(tuple(up.shape) != (rows * n_all, width) or tuple(down.shape) != (width, n_all), f"MoeWeights: packed matrices {up.shape} and {down.shape} do not "
+                f"hold {experts} experts of {ff} and {shared_ff} shared columns")
+        _refuse(up.tile_rows % 32 != 0 or rows * ff % up.tile_rows != 0 or rows * shared_ff % up.tile_rows != 0 or down.tile_rows != 128,
+                f"MoeWeights: tiles of {up.tile_rows} and {down.tile_rows} rows")
+        self.up, self.down, self.experts, self.width, self.ff, self.shared_ff = up, down, int(experts), int(width), int(ff), int(shared_ff)
+        self.act, self.limit, self.slope = act, float(limit), float(slope)
+
+    @classmethod
+    def pack(cls, gate: Optional[torch.Tensor], up: torch.Tensor, down: torch.Tensor, shared=None, act: str = "silu_glu", limit: float = 0.0,
+             slope: float = 1.702) -> "MoeWeights":
+        """gate, up bf16 [experts, ff, width] (gate None: experts of the form down(act(up h))), down [experts, width, ff]; shared: (gate, up, down) of the
+        expert that every row takes.  Expert widths are padded to multiples of 64 with zeros, which every activation leaves without effect."""
+        gated = act.endswith("glu")
+        _refuse(gated != (gate is not None), f"MoeWeights.pack: activation {act!r} {'needs' if gated else 'has no'} gate matrices")
+        _need_here("MoeWeights.pack", gate, up, down, *(shared or ()))
+        _refuse(up.dim() != 3 or tuple(down.shape) != (up.shape[0], up.shape[2], up.shape[1]) or (gated and gate.shape != up.shape),
+                f"MoeWeights.pack: up {tuple(up.shape)} and down {tuple(down.shape)} do not match")
+        E, ff, W = up.shape
+        ffp, sff, sffp = (ff + 63) // 64 * 64, 0, 0
+        if shared is not None:
+            sg, su, sd = shared
+            sff = su.shape[0]
+            sffp = (sff + 63) // 64 * 64
+            _refuse((sg is not None) != gated or tuple(su.shape) != (sff, W) or tuple(sd.shape) != (W, sff) or (gated and sg.shape != su.shape),
+                    "MoeWeights.pack: the shared expert's matrices do not match")
+        n_all = E * ffp + sffp
+
+        def rows(routed, one):
+            m = torch.zeros(n_all, W, dtype=BF16, device=up.device)
+            m[:E * ffp].view(E, ffp, W)[:, :ff] = routed.to(BF16)
+            if one is not None:
+                m[E * ffp:E * ffp + sff] = one.to(BF16)
+            return m
+        if gated:
+            packed = pack_weight(interleave_gate_up(rows(gate, shared and shared[0]), rows(up, shared and shared[1]), 64), 128)
+        else:
+            packed = pack_weight(rows(up, shared and shared[1]), 64)
+        cols = torch.zeros(W, n_all, dtype=BF16, device=up.device)
+        cols[:, :E * ffp].view(W, E, ffp)[:, :, :ff] = down.to(BF16).transpose(0, 1)
+        if shared is not None:
+            cols[:, E * ffp:E * ffp + sff] = shared[2].to(BF16)
+        return cls(packed, pack_weight(cols, 128), E, W, ffp, sffp, act, limit, slope)
+
+
+class MoeRouter:
+    """How ``moe_layer`` picks a row's ``top`` experts and weighs them:
+      "softmax"      the largest logits weight h + bias, softmax over the chosen (``moe_route``)
+      "sigmoid"      sigmoid scores, chosen by score + bias within the ``keep`` best of ``groups`` groups, weights over their sum (``moe_route_sigmoid``)
+      "softmax_all"  softmax over all experts, chosen within the kept groups, weights as they are (``moe_route_groups``)
+      "table"        the row's token id picks them, each 1 / top (``moe_route_table``)
+    weight fp32 [experts, width]; shared_gate fp32 [width] ("sigmoid", "table"): the shared expert times sigmoid(shared_gate . h)."""
+    __slots__ = ("kind", "top", "weight", "bias", "groups", "keep", "shared_gate", "table")
+
+    def __init__(self, kind: str, top: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, groups: int = 0, keep: int = 0,
+                 shared_gate: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None):
+        _refuse(kind not in MOE_LAYER_ROUTERS, f"MoeRouter: kind {kind!r}")
+        _refuse(not 1 <= top <= 32, f"MoeRouter: top {top}; 1 to 32")
+        _refuse((kind == "table") != (table is not None) or (kind == "table") == (weight is not None), f"MoeRouter: {kind!r} takes a {'table' if kind == 'table' else 'weight'}")
+        _refuse(weight is not None and (weight.dtype != F32 or weight.dim() != 2 or not weight.is_contiguous() or weight.shape[0] < top),
+                "MoeRouter: weight is fp32 [experts >= top, width]")
+        _refuse(table is not None and (table.dtype != torch.int32 or table.dim() != 2 or table.shape[1] != top or not table.is_contiguous()),
+                f"MoeRouter: table is int32 [vocab, {top}]")
+        _refuse(bias is not None and (weight is None or kind == "softmax_all" or bias.dtype != F32 or bias.numel() != weight.shape[0] or not bias.is_contiguous()),
+                "MoeRouter: bias is fp32 [experts] of a softmax or sigmoid router")
+        _refuse(shared_gate is not None and (kind not in ("sigmoid", "table") or shared_gate.dtype != F32 or shared_gate.dim() != 1 or not shared_gate.is_contiguous()),
+                "MoeRouter: shared_gate is fp32 [width] of a sigmoid or table router")
+        if groups > 1:
+            E = weight.shape[0] if weight is not None and kind != "softmax" else 0
+            _refuse(E == 0 or E % groups != 0 or not 1 <= keep <= groups or keep * (E // groups) < top,
+                    f"MoeRouter: {groups} groups (keep {keep}) do not fit a {kind!r} router of {E} experts, top {top}")
+        self.kind, self.top, self.weight, self.bias, self.groups, self.keep = kind, int(top), weight, bias, int(groups), int(keep)
+        self.shared_gate, self.table = shared_gate, table
+
+
+def moe_layer(h: torch.Tensor, weights: MoeWeights, router: MoeRouter, ids: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """A whole mixture-of-experts layer for the rows of a decode step (at most MOE_LAYER_MAX_ROWS): router, the chosen experts, the shared expert, weighted
+    sum.  h bf16 [T, width]; ids int32 [T] (token ids) for a table router; out fp32 [T, width].  The matrices of experts that no row chose are not read; nothing
+    is rounded between the two products."""
+    T, W, top, E = h.shape[0], weights.width, router.top, weights.experts
+    _need_here("moe_layer", h, weights.up.data, router.weight, router.bias, router.table, router.shared_gate, ids, out)
+    _refuse(h.dtype != BF16 or h.dim() != 2 or h.shape[1] != W or not h.is_contiguous(), f"moe_layer: contiguous bf16 rows of {W} are needed")
+    _refuse(T > MOE_LAYER_MAX_ROWS, f"moe_layer: {T} rows; at most {MOE_LAYER_MAX_ROWS} (larger steps group the rows: moe_group_tiles, gemm_tiles)")
+    _refuse(top > E or (router.weight is not None and tuple(router.weight.shape) != (E, W)), f"moe_layer: the router does not match {E} experts of width {W}")
+    _refuse(router.shared_gate is not None and (not weights.shared_ff or router.shared_gate.numel() != W), "moe_layer: a gate without a shared expert of its width")
+    _refuse((router.kind == "table") != (ids is not None) or (ids is not None and (ids.dtype != torch.int32 or ids.numel() != T or not ids.is_contiguous())),
+            "moe_layer: a table router, and no other, takes int32 ids of every row")
+    if out is None:
+        out = torch.empty(T, W, dtype=F32, device=h.device)
+    _refuse(out.dtype != F32 or tuple(out.shape) != (T, W) or (T > 0 and out.stride(1) != 1), f"moe_layer: out is fp32 [{T}, {W}]")
+    if T == 0:
+        return out
+    P = T * top
+    head = (8 * P + 4 * T + 15) // 16 * 16
+    act_bytes = 6 * (P + T) * max(weights.ff, weights.shared_ff)
+    ws = torch.empty(head + act_bytes, dtype=torch.uint8, device=h.device)
+    idx = ws.data_ptr()
+    wts, sgate, act, s = idx + 4 * P, (idx + 8 * P if router.shared_gate is not None else None), idx + head, _stream()
+    hp = h.data_ptr()
+    call("vb_moe_layer_route", idx, wts, sgate, MOE_LAYER_ROUTERS[router.kind], hp, W, _p(router.weight), _p(router.bias), _p(router.shared_gate), _p(ids),
+         _p(router.table), T, W, E, top, router.groups, router.keep, router.table.shape[0] if ids is not None else 0, s)
+    call("vb_moe_layer_experts", out.data_ptr(), out.stride(0) if T > 1 else W, hp, W, weights.up.data.data_ptr(), weights.down.data.data_ptr(), idx, wts, sgate,
+         T, W, E, top, weights.ff, weights.shared_ff, weights.up.tile_rows, MOE_LAYER_ACTS[weights.act], weights.limit, weights.slope, act, act_bytes, s)
+    return out
