@@ -184,11 +184,12 @@ def test_layer_non_finite_rows_stay_among_themselves(bad, kind):
     from vox_serve_b200 import ops
     groups, keep = (0, 0) if kind == "softmax" else (4, 2)
     h, ex, sh, router, w, ids = _layer(12, 136, 64, 8, 2, 64, "silu_glu", kind, groups, keep, seed=4)
-    want = ops.moe_layer(h, w, router)
     h[5, 17] = bad
     got = ops.moe_layer(h, w, router)
     rest = torch.arange(12, device="cuda") != 5
-    assert torch.equal(got[rest], want[rest]) and bool(got[5].isnan().any())
+    # (not bit for bit: the row's experts change, and sums are grouped by the step's experts; the bound holds for any grouping)
+    _check(got[rest], h[rest], ex, sh, router, ids, "silu_glu")
+    assert bool(got[5].isnan().any())
 
 
 def test_layer_table_names_experts_twice_and_out_of_range():

@@ -11,9 +11,9 @@
 //         one row's experts from all of them
 //   up    block = (expert, 32 rows of its gate | up matrix: 16 gated or 32 plain columns), the eight warps divide k; sums meet in shared memory, the
 //         activation times the routing weight leaves as three bf16 parts (exact, rowmma.cuh), so nothing is rounded between the two products
-//   down  block = 32 columns of the result x a share of the (expert, piece of ff) units of the chosen experts, every warp adding its products to rows
-//         of its own in shared memory; up to eight blocks of a cluster share the units and add up through distributed shared memory.  No atomics:
-//         units, warps and blocks are added in a fixed order
+//   down  block = 32 columns of the result x an equal share of the chosen experts' k blocks, every warp adding its products to rows of its own in
+//         shared memory; up to eight blocks of a cluster divide the k blocks and add up through distributed shared memory.  No atomics: products,
+//         warps and blocks are added in a fixed order
 //
 // A table that names an expert twice for a row counts it once with both weights; an index that is no expert counts as none.
 #include "../../include/vb_api.h"
@@ -41,6 +41,7 @@ struct MoeLayerParams {
 // ---- router -----------------------------------------------------------------------------------------------------------------------
 enum MlRouter { ML_SOFTMAX = 0, ML_SIGMOID = 1, ML_SOFTMAX_ALL = 2, ML_TABLE = 3 };
 constexpr int ML_ROUTE_CLUSTER = 8;      // blocks, and rows, of a cluster
+constexpr int ML_ROUTE_THREADS = 512;
 struct MoeRouteParams {
   int32_t* idx;
   float *wts, *sgate;
@@ -48,7 +49,7 @@ struct MoeRouteParams {
   long long ldh;
   const float *w, *bias, *wsg;           // [E][W], [E], [W]
   const int32_t *ids, *table;
-  int T, W, E, top, kind, groups, keep, vocab, parts;
+  int T, W, E, top, kind, groups, keep, vocab;
 };
 // floats as integers of the same order; NaN above all (so a row that holds one still picks experts that exist), 0 below all: not to be picked
 __device__ __forceinline__ uint32_t ml_key(float v) {
@@ -65,54 +66,85 @@ __device__ __forceinline__ int ml_argmax(const uint32_t* keys, int n, int lane) 
   const uint32_t top = __reduce_max_sync(0xffffffffu, best);
   return __reduce_min_sync(0xffffffffu, best == top ? at : 0x7fffffff);
 }
-__global__ void __launch_bounds__(ML_THREADS) moe_layer_route_kernel(const MoeRouteParams p) {
+// A block's rows of the matrix (its share of the experts, 16 at a time) by the cluster's rows of h: the fp32 values as three bf16 parts (exact), the k
+// blocks of 32 divided by the warps.  What a warp needs first is asked for before the rows of h are there (the matrix is older than the kernel in front).
+__global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const MoeRouteParams p) {
   extern __shared__ __align__(16) int smem[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  constexpr int WARPS = ML_ROUTE_THREADS / 32, AHEAD = 2;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int rank = blockIdx.x % ML_ROUTE_CLUSTER, t0 = blockIdx.x / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER, rows = min(ML_ROUTE_CLUSTER, p.T - t0);
-  // the matrix's rows: the experts, then the shared expert's gate
+  // the matrix's rows: the experts, then the shared expert's gate; a block has every eighth
   const int E = p.kind == ML_TABLE ? 0 : p.E, all = E + (p.wsg ? 1 : 0), per = (all + ML_ROUTE_CLUSTER - 1) / ML_ROUTE_CLUSTER;
-  float* part = reinterpret_cast<float*>(smem);                   // [per][parts][8 rows]
-  float* mine = part + per * p.parts * ML_ROUTE_CLUSTER;          // [per][8]: this block's logits
+  float* part = reinterpret_cast<float*>(smem);                   // [16 warps][16 of the block's][8 rows]
+  float* mine = part + WARPS * 16 * ML_ROUTE_CLUSTER;             // [per][8]: this block's logits
   float* z = mine + per * ML_ROUTE_CLUSTER;                       // [E] the row's logits, then its scores
   uint32_t* keys = reinterpret_cast<uint32_t*>(z + p.E);          // [E]
   uint32_t* gkeys = keys + p.E;                                   // [groups]
+  const int kbs = (p.W + 31) / 32;
+  float4 w[AHEAD][2][2];                                          // two rows, eight values each
+  auto take = [&](int u, int i0, int kb) {
+    const int k = kb * 32 + t4 * 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = (i0 + g + h * 8) * ML_ROUTE_CLUSTER + rank;
+      const bool in = e < all && i0 + g + h * 8 < per && k < p.W;
+      const float* r = (e < E ? p.w + static_cast<long long>(e) * p.W : p.wsg) + k;
+      w[u][h][0] = in ? __ldg(reinterpret_cast<const float4*>(r)) : make_float4(0.f, 0.f, 0.f, 0.f);
+      w[u][h][1] = in ? __ldg(reinterpret_cast<const float4*>(r + 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  };
+  if (per > 0)
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) take(u, 0, warp + u * WARPS);
   pdl_sync();
-  // a row of the matrix per warp, or `parts` warps share it
-  const int slots = ML_WARPS / p.parts, q = warp % p.parts;
-  for (int i = warp / p.parts; i < per; i += slots) {
-    const int e = i * ML_ROUTE_CLUSTER + rank;
-    if (e >= all) break;
-    const float* w = e < E ? p.w + static_cast<long long>(e) * p.W : p.wsg;
-    float s[ML_ROUTE_CLUSTER] = {};
-    for (int k = (q * 32 + lane) * 8; k < p.W; k += p.parts * 256) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(w + k)), b = __ldg(reinterpret_cast<const float4*>(w + k + 4));
+  const __nv_bfloat16* hr = p.h + (t0 + min(g, rows - 1)) * p.ldh;
+  for (int i0 = 0; i0 < per; i0 += 16) {
+    float acc[4] = {};
+    for (int kb0 = warp; kb0 < kbs; kb0 += AHEAD * WARPS) {
+      uint4 x[AHEAD];
 #pragma unroll
-      for (int t = 0; t < ML_ROUTE_CLUSTER; ++t) {
-        if (t >= rows) break;
-        const uint4 x = *reinterpret_cast<const uint4*>(p.h + (t0 + t) * p.ldh + k);
-        float v = s[t];
-        v = fmaf(bf16_lo(x.x), a.x, v); v = fmaf(bf16_hi(x.x), a.y, v); v = fmaf(bf16_lo(x.y), a.z, v); v = fmaf(bf16_hi(x.y), a.w, v);
-        v = fmaf(bf16_lo(x.z), b.x, v); v = fmaf(bf16_hi(x.z), b.y, v); v = fmaf(bf16_lo(x.w), b.z, v); v = fmaf(bf16_hi(x.w), b.w, v);
-        s[t] = v;
+      for (int u = 0; u < AHEAD; ++u) {
+        const int kb = kb0 + u * WARPS, k = kb * 32 + t4 * 8;
+        if (i0 > 0 || kb0 != warp) take(u, i0, kb);
+        x[u] = k < p.W ? *reinterpret_cast<const uint4*>(hr + k) : make_uint4(0u, 0u, 0u, 0u);
       }
-    }
 #pragma unroll
-    for (int t = 0; t < ML_ROUTE_CLUSTER; ++t) {
-      if (t >= rows) break;
-      const float v = warp_sum(s[t]);
-      if (lane == 0) part[(i * p.parts + q) * ML_ROUTE_CLUSTER + t] = v;
+      for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          float v[2][4];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) { v[h][0] = w[u][h][s].x; v[h][1] = w[u][h][s].y; v[h][2] = w[u][h][s].z; v[h][3] = w[u][h][s].w; }
+          uint32_t f[3][4];              // part, {row g, row g + 8} x {first pair, second pair}
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float h0, m0, l0, h1, m1, l1;
+            bf16_parts(v[q & 1][(q >> 1) * 2], h0, m0, l0);
+            bf16_parts(v[q & 1][(q >> 1) * 2 + 1], h1, m1, l1);
+            f[0][q] = pack_cut(h0, h1);
+            f[1][q] = pack_cut(m0, m1);
+            f[2][q] = pack_cut(l0, l1);
+          }
+#pragma unroll
+          for (int q = 0; q < 3; ++q) mma_bf16(acc, f[q][0], f[q][1], f[q][2], f[q][3], s ? x[u].z : x[u].x, s ? x[u].w : x[u].y);
+        }
     }
-  }
-  __syncthreads();
-  for (int i = tid; i < per * ML_ROUTE_CLUSTER; i += ML_THREADS) {
-    float v = 0.f;
-    for (int k = 0; k < p.parts; ++k) v += part[(i / ML_ROUTE_CLUSTER * p.parts + k) * ML_ROUTE_CLUSTER + i % ML_ROUTE_CLUSTER];
-    mine[i] = v;                                     // (rows behind the last and experts that are none hold anything; nobody asks for them)
+    float* o = part + warp * 16 * ML_ROUTE_CLUSTER;
+    *reinterpret_cast<float2*>(o + g * ML_ROUTE_CLUSTER + t4 * 2) = make_float2(acc[0], acc[1]);
+    *reinterpret_cast<float2*>(o + (g + 8) * ML_ROUTE_CLUSTER + t4 * 2) = make_float2(acc[2], acc[3]);
+    __syncthreads();
+    if (tid < 16 * ML_ROUTE_CLUSTER && i0 + tid / ML_ROUTE_CLUSTER < per) {
+      float v = 0.f;
+#pragma unroll
+      for (int q = 0; q < WARPS; ++q) v += part[q * 16 * ML_ROUTE_CLUSTER + tid];
+      mine[i0 * ML_ROUTE_CLUSTER + tid] = v;                      // (rows behind the last repeat it; nobody asks for them)
+    }
+    __syncthreads();
   }
   cluster_sync_all();
   const bool has = rank < rows;
   if (has) {
-    for (int e = tid; e < E; e += ML_THREADS) {
+    for (int e = tid; e < E; e += ML_ROUTE_THREADS) {
       const float v = ld_dsmem_f32(mine + e / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER + rank, e % ML_ROUTE_CLUSTER);
       z[e] = p.kind == ML_SOFTMAX && p.bias ? v + p.bias[e] : v;
     }
@@ -215,6 +247,8 @@ __device__ __forceinline__ MoePlanView ml_view(int* s, int T, int E, int top) {
   return v;
 }
 
+// ROUNDS: pairs a thread looks after (a step of 8 rows has at most one a thread)
+template <int ROUNDS>
 __device__ __forceinline__ void ml_build(const MoePlanView& v, const MoeLayerParams& p) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, P = p.T * p.top;
   for (int e = tid; e < p.E; e += ML_THREADS) v.cur[e] = 0;
@@ -225,10 +259,10 @@ __device__ __forceinline__ void ml_build(const MoePlanView& v, const MoeLayerPar
   }
   __syncthreads();
   // an expert named twice for a row: the first place takes both weights.  (Found first, written behind a barrier: others still compare.)
-  int keep[(ML_MAX_ROWS * ML_MAX_TOP) / ML_THREADS];
-  float weight[(ML_MAX_ROWS * ML_MAX_TOP) / ML_THREADS];
+  int keep[ROUNDS];
+  float weight[ROUNDS];
 #pragma unroll
-  for (int k = 0; k < (ML_MAX_ROWS * ML_MAX_TOP) / ML_THREADS; ++k) {
+  for (int k = 0; k < ROUNDS; ++k) {
     const int i = tid + k * ML_THREADS;
     keep[k] = -1;
     if (i >= P) continue;
@@ -290,7 +324,7 @@ __device__ __forceinline__ void ml_build(const MoePlanView& v, const MoeLayerPar
   if (p.sff > 0 && tid < p.T) v.row[r_all + tid] = P + tid;
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < (ML_MAX_ROWS * ML_MAX_TOP) / ML_THREADS; ++k)
+  for (int k = 0; k < ROUNDS; ++k)
     if (keep[k] >= 0) {
       const int i = tid + k * ML_THREADS;
       v.row[atomicAdd(&v.cur[keep[k]], 1)] = i;
@@ -319,188 +353,237 @@ __device__ __forceinline__ float ml_act(int kind, float g, float u, float limit,
 
 // ---- gate | up ------------------------------------------------------------------------------------------------------------------
 // NT column tiles of 8 rows a pass over the weights (an expert with more rows takes further passes, its weights from L2 then).
-template <int NT, bool GATED>
-__global__ void __launch_bounds__(ML_THREADS) moe_up_kernel(const MoeLayerParams p) {
-  extern __shared__ __align__(16) int smem[];
-  constexpr int LD = NT * 8 + (NT > 1 ? 8 : 0);
-  float* red = reinterpret_cast<float*>(smem);           // [8 warps][32][LD]
-  const MoePlanView v = ml_view(smem + ML_WARPS * 32 * LD, p.T, p.E, p.top);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-  pdl_sync();
-  ml_build(v, p);
-  const int P = p.T * p.top, n_active = *v.n_active;
-  const int routed = p.sff > 0 ? n_active - 1 : n_active;
-  const int items = routed * p.up_units + p.shared_units;
-  // the four rows of weights that a lane takes of every k block: gate g, up g, gate g + 8, up g + 8 of 16 | 16 rows, or four of 32 plain ones
-  for (int it = blockIdx.x; it < items; it += gridDim.x) {
-    const int a = it < routed * p.up_units ? it / p.up_units : routed, unit = it - a * p.up_units, e = v.active[a];
-    const int row0 = unit * 32, tile = row0 / p.up_rows, r0 = row0 - tile * p.up_rows;
-    const uint8_t* wb = p.up + e * p.expert_bytes + (static_cast<long long>(tile) * p.kb * p.up_rows + r0) * 128;
-    const int first = v.off[e], n = v.off[e + 1] - first;
-    for (int n0 = 0; n0 < n; n0 += NT * 8) {
-      const __nv_bfloat16* hr[NT];
+// All loads of a k block come before its first product.  A column tile's unused columns repeat the first row (a product's columns do not touch one another).
+template <int NT>
+__device__ __forceinline__ void ml_up_product(float (&acc)[2][NT][4], const uint8_t* wb, const __nv_bfloat16* const (&hr)[NT], int k0, int step,
+                                              const MoeLayerParams& p, int g, int t4) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
+#pragma unroll 1
+  for (int kb = k0; kb < p.kb; kb += step) {
+    const uint8_t* wk = wb + static_cast<long long>(kb) * p.up_rows * 128;
+    uint4 w[4][2], x[NT][2];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) w[q][s] = ldg_stream(wk + (q * 8 + g) * 128 + (((s * 4 + t4) ^ g) << 4));
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const int k = kb * 64 + (s * 4 + t4) * 8;
+        x[j][s] = k < p.W ? *reinterpret_cast<const uint4*>(hr[j] + k) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int s = 0; s < 2; ++s)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const uint4 lo = w[i][s], hi = w[i + 2][s];
+          mma_bf16(acc[i][j], lo.x, hi.x, lo.y, hi.y, x[j][s].x, x[j][s].y);
+          mma_bf16(acc[i][j], lo.z, hi.z, lo.w, hi.w, x[j][s].z, x[j][s].w);
+        }
+  }
+}
+// one activation, times its row's routing weight, as parts
+__device__ __forceinline__ void ml_store(const MoeLayerParams& p, const MoePlanView& v, int place, int col, float g, float u) {
+  const int P = p.T * p.top, pr = v.row[place];
+  const float scale = pr < P ? v.w[pr] : (p.sgate ? p.sgate[pr - P] : 1.f);
+  float hi, mid, lo;
+  bf16_parts(ml_act(p.act_kind, g, u, p.limit, p.slope) * scale, hi, mid, lo);
+  __nv_bfloat16* o = p.act + static_cast<long long>(pr) * p.ld_act + col;
+  o[0] = __float2bfloat16_rn(hi);
+  o[p.part_stride] = __float2bfloat16_rn(mid);
+  o[2 * p.part_stride] = __float2bfloat16_rn(lo);
+}
+template <int NT>
+__device__ __forceinline__ void ml_rows(const __nv_bfloat16* (&r)[NT], const __nv_bfloat16* base, long long ld, const MoePlanView& v, int first, int cols, int g, int P,
+                                        int top, bool by_row) {
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int c = j * 8 + g, pr = v.row[first + (c < cols ? c : 0)];
+    r[j] = base + (by_row ? (pr < P ? pr / top : pr - P) : pr) * ld;
+  }
+}
+// sums of one pass over an item: complete in the lanes (share 1), or parts of them that `share` warps leave in shared memory
+template <int NT, int LD, bool GATED>
+__device__ __forceinline__ void ml_up_pass(const MoeLayerParams& p, const MoePlanView& v, const uint8_t* wb, float* mine, int first, int cols, int unit, int part,
+                                           int share, int g, int t4) {
+  float acc[2][NT][4];
+  const __nv_bfloat16* hr[NT];
+  ml_rows<NT>(hr, p.h, p.ldh, v, first, cols, g, p.T * p.top, p.top, true);
+  ml_up_product<NT>(acc, wb, hr, part, share, p, g, t4);
+  if (share > 1) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int j = 0; j < NT; ++j) {
-        const int c = n0 + j * 8 + g;
-        hr[j] = nullptr;
-        if (c < n) {
-          const int pr = v.row[first + c], t = pr < P ? pr / p.top : pr - P;
-          hr[j] = p.h + t * p.ldh;
-        }
+        *reinterpret_cast<float2*>(mine + (i * 8 + g) * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][0], acc[i][j][1]);
+        *reinterpret_cast<float2*>(mine + (16 + i * 8 + g) * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][2], acc[i][j][3]);
       }
-      float acc[2][NT][4];
+    return;
+  }
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-        for (int j = 0; j < NT; ++j)
+    for (int h = 0; h < 2; ++h) {
+      const int c = j * 8 + t4 * 2 + h;
+      if (c < cols)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
-#pragma unroll 2
-      for (int kb = warp; kb < p.kb; kb += ML_WARPS) {
-        const uint8_t* wk = wb + static_cast<long long>(kb) * p.up_rows * 128;
-        uint4 w[4][2];
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int s = 0; s < 2; ++s) w[q][s] = ldg_stream(wk + (q * 8 + g) * 128 + (((s * 4 + t4) ^ g) << 4));
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          if (j > 0 && n0 + j * 8 >= n) break;
-          uint4 x[2];
-#pragma unroll
-          for (int s = 0; s < 2; ++s) {
-            const int k = kb * 64 + (s * 4 + t4) * 8;
-            x[s] = hr[j] && k < p.W ? *reinterpret_cast<const uint4*>(hr[j] + k) : make_uint4(0u, 0u, 0u, 0u);
+        for (int i = 0; i < 2; ++i) {
+          if (GATED) ml_store(p, v, first + c, unit * 16 + i * 8 + g, acc[i][j][h], acc[i][j][2 + h]);
+          else {
+            ml_store(p, v, first + c, unit * 32 + i * 8 + g, 0.f, acc[i][j][h]);
+            ml_store(p, v, first + c, unit * 32 + 16 + i * 8 + g, 0.f, acc[i][j][2 + h]);
           }
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              // gated: rows 0-7 gate, 8-15 of the tile their up rows; the packed order has 16 gate rows, then their 16 up rows
-              const uint4 lo = w[GATED ? i : 2 * i][s], hi = w[GATED ? i + 2 : 2 * i + 1][s];
-              mma_bf16(acc[i][j], lo.x, hi.x, lo.y, hi.y, x[s].x, x[s].y);
-              mma_bf16(acc[i][j], lo.z, hi.z, lo.w, hi.w, x[s].z, x[s].w);
-            }
         }
-      }
-      __syncthreads();                   // (the sums of the item before have been read)
-      float* mine = red + warp * 32 * LD;
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          *reinterpret_cast<float2*>(mine + (i * 16 + g) * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][0], acc[i][j][1]);
-          *reinterpret_cast<float2*>(mine + (i * 16 + g + 8) * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][2], acc[i][j][3]);
-        }
+    }
+}
+// An item is 32 rows of an expert's matrix.  Where the step has items for all warps a warp takes one by itself, its sums complete in its registers (a gate
+// row and its up row in the same lane); where it has few, 2, 4 or 8 warps divide an item's k and meet in shared memory.
+template <int NT, bool GATED>
+__global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 3 : 2) moe_up_kernel(const MoeLayerParams p) {
+  extern __shared__ __align__(16) int smem[];
+  constexpr int LD = NT * 8 + (NT > 1 ? 8 : 0);
+  float* red = reinterpret_cast<float*>(smem);           // two times [8 warps][32][LD]: a round's sums are read while the next round's are made
+  const MoePlanView v = ml_view(smem + 2 * ML_WARPS * 32 * LD, p.T, p.E, p.top);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+  pdl_sync();
+  ml_build<NT == 1 ? 8 * ML_MAX_TOP / ML_THREADS : ML_MAX_ROWS * ML_MAX_TOP / ML_THREADS>(v, p);
+  const int n_active = *v.n_active, routed = p.sff > 0 ? n_active - 1 : n_active;
+  const int items = routed * p.up_units + p.shared_units;
+  int share = 1;                                         // warps of an item
+  while (share < ML_WARPS && items * share * 2 <= static_cast<int>(gridDim.x) * ML_WARPS) share *= 2;
+  const int groups = ML_WARPS / share, group = warp / share, part = warp % share;
+  const int rounds = (items + groups * gridDim.x - 1) / (groups * gridDim.x);
+  int turn = 0;
+  for (int round = 0; round < rounds; ++round) {
+    const int it = (round * groups + group) * gridDim.x + blockIdx.x;
+    const bool on = it < items;
+    const int a = it < routed * p.up_units ? it / p.up_units : routed, unit = it - a * p.up_units, e = on ? v.active[a] : 0;
+    const int row0 = unit * 32, tile = row0 / p.up_rows, r0 = row0 - tile * p.up_rows;
+    const uint8_t* wb = p.up + e * p.expert_bytes + (static_cast<long long>(tile) * p.kb * p.up_rows + r0) * 128;
+    const int first = on ? v.off[e] : 0, n = on ? v.off[e + 1] - first : 0;
+    int passes = (n + NT * 8 - 1) / (NT * 8);
+    if (share > 1 && p.T > NT * 8) passes = __syncthreads_or(passes > 1) ? (ML_MAX_ROWS + NT * 8 - 1) / (NT * 8) : 1;      // (all groups meet in every pass)
+    else if (share > 1) passes = 1;
+    for (int pass = 0; pass < passes; ++pass) {
+      const int n0 = pass * NT * 8, cols = n - n0;
+      float* sums = red + (turn++ & 1) * ML_WARPS * 32 * LD;
+      if (NT > 1 && cols > 0 && cols <= 8) ml_up_pass<1, LD, GATED>(p, v, wb, sums + warp * 32 * LD, first + n0, cols, unit, part, share, g, t4);
+      else if (cols > 0) ml_up_pass<NT, LD, GATED>(p, v, wb, sums + warp * 32 * LD, first + n0, cols, unit, part, share, g, t4);
+      if (share == 1) continue;
       __syncthreads();
       constexpr int COLS = GATED ? 16 : 32;
-      const int cols = min(NT * 8, n - n0);
-      for (int i = tid; i < COLS * cols; i += ML_THREADS) {
+      for (int i = part * 32 + lane; i < COLS * min(NT * 8, cols); i += share * 32) {
         const int col = i % COLS, c = i / COLS;
-        const int r1 = GATED ? (col >> 3) * 16 + (col & 7) : col;
         float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int q = 0; q < ML_WARPS; ++q) {
-          s1 += red[(q * 32 + r1) * LD + c];
-          if (GATED) s2 += red[(q * 32 + r1 + 8) * LD + c];
+        for (int q = 0; q < share; ++q) {
+          s1 += sums[((group * share + q) * 32 + col) * LD + c];
+          if (GATED) s2 += sums[((group * share + q) * 32 + 16 + col) * LD + c];
         }
-        const int pr = v.row[first + n0 + c];
-        const float scale = pr < P ? v.w[pr] : (p.sgate ? p.sgate[pr - P] : 1.f);
-        const float y = ml_act(p.act_kind, s1, GATED ? s2 : s1, p.limit, p.slope) * scale;
-        float hi, mid, lo;
-        bf16_parts(y, hi, mid, lo);
-        __nv_bfloat16* o = p.act + static_cast<long long>(pr) * p.ld_act + unit * COLS + col;
-        o[0] = __float2bfloat16_rn(hi);
-        o[p.part_stride] = __float2bfloat16_rn(mid);
-        o[2 * p.part_stride] = __float2bfloat16_rn(lo);
+        ml_store(p, v, first + n0 + c, unit * COLS + col, s1, GATED ? s2 : s1);
       }
     }
   }
 }
 
 // ---- down -------------------------------------------------------------------------------------------------------------------------
-constexpr int ML_UNIT_KB = 4;            // k blocks (64 each) of an expert that a warp takes at a time
+// Products of one expert's k blocks k0 .. k1 - 1 with NT column tiles, added to the warp's rows of sums.  All loads of a k block come before its first product.
+constexpr int ML_LD = 36;                // floats between rows of sums (32 columns)
 template <int NT>
-__global__ void __launch_bounds__(ML_THREADS) moe_down_kernel(const MoeLayerParams p) {
+__device__ __forceinline__ void ml_down_pass(const MoeLayerParams& p, const MoePlanView& v, const uint8_t* wb, float* mine, int first, int cols, int k0, int k1, int g,
+                                             int t4) {
+  const int P = p.T * p.top;
+  const __nv_bfloat16* ar[NT];
+  ml_rows<NT>(ar, p.act + t4 * 8, p.ld_act, v, first, cols, g, P, p.top, false);
+  float acc[2][NT][4];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
+#pragma unroll 1
+  for (int kb = k0; kb < k1; ++kb) {
+    const uint8_t* wk = wb + static_cast<long long>(kb) * 16384;
+    uint4 w[4][2];
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) w[q][s] = ldg_stream(wk + (q * 8 + g) * 128 + (((s * 4 + t4) ^ g) << 4));
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      uint4 x[3][2];
+#pragma unroll
+      for (int part = 0; part < 3; ++part)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) x[part][s] = *reinterpret_cast<const uint4*>(ar[j] + part * p.part_stride + kb * 64 + s * 32);
+#pragma unroll
+      for (int part = 0; part < 3; ++part)
+#pragma unroll
+        for (int s = 0; s < 2; ++s)
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {
+            const uint4 lo = w[2 * i][s], hi = w[2 * i + 1][s];
+            mma_bf16(acc[i][j], lo.x, hi.x, lo.y, hi.y, x[part][s].x, x[part][s].y);
+            mma_bf16(acc[i][j], lo.z, hi.z, lo.w, hi.w, x[part][s].z, x[part][s].w);
+          }
+    }
+  }
+  // (a row occurs once among an expert's, so no two lanes add to the same place)
+#pragma unroll
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int c = j * 8 + t4 * 2 + h;
+      if (c < cols) {
+        const int pr = v.row[first + c], t = pr < P ? pr / p.top : pr - P;
+        float* s = mine + t * ML_LD + g;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          s[i * 16] += acc[i][j][h];
+          s[i * 16 + 8] += acc[i][j][2 + h];
+        }
+      }
+    }
+  __syncwarp();
+}
+// The k blocks of all chosen experts stand in one line, of which every warp of the cluster takes an equal part.
+template <int NT>
+__global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 3 : 2) moe_down_kernel(const MoeLayerParams p) {
   extern __shared__ __align__(16) int smem[];
-  constexpr int LD = 36;                 // floats between rows of sums (32 columns)
+  constexpr int LD = ML_LD;
   float* sums = reinterpret_cast<float*>(smem);          // [8 warps][T][LD]
   const MoePlanView v = ml_view(smem + ML_WARPS * p.T * LD, p.T, p.E, p.top);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int rank = blockIdx.x % p.cluster, block = blockIdx.x / p.cluster;
   // (routing and weights are older than the up kernel, whose activations are all that has to be waited for)
-  ml_build(v, p);
+  ml_build<NT == 1 ? 8 * ML_MAX_TOP / ML_THREADS : ML_MAX_ROWS * ML_MAX_TOP / ML_THREADS>(v, p);
   float* mine = sums + warp * p.T * LD;
   for (int i = lane; i < p.T * LD; i += 32) mine[i] = 0.f;
   __syncwarp();
   pdl_sync();
-  const int P = p.T * p.top, n_active = *v.n_active;
+  const int n_active = *v.n_active;
   const int col0 = block * 32, tile = col0 >> 7;
   const uint8_t* wt = p.down + static_cast<long long>(tile) * p.down_kb * 16384 + (col0 & 127) * 128;
-  const int per = (p.ff / 64 + ML_UNIT_KB - 1) / ML_UNIT_KB, per_shared = (p.sff / 64 + ML_UNIT_KB - 1) / ML_UNIT_KB;
-  const int routed = p.sff > 0 ? n_active - 1 : n_active, units = routed * per + per_shared;
-  for (int u = rank * ML_WARPS + warp; u < units; u += p.cluster * ML_WARPS) {
-    const int a = u < routed * per ? u / per : routed, piece = u - a * per, e = v.active[a];
-    const int kbs = (e < p.E ? p.ff : p.sff) / 64, k0 = piece * ML_UNIT_KB, k1 = min(kbs, k0 + ML_UNIT_KB);
-    const uint8_t* wb = wt + static_cast<long long>(e) * (p.ff / 64) * 16384;
+  const int fkb = p.ff / 64, routed = p.sff > 0 ? n_active - 1 : n_active, line = routed * fkb + p.sff / 64;
+  const int share = rank * ML_WARPS + warp, shares = p.cluster * ML_WARPS;
+  const int end = static_cast<int>(static_cast<long long>(line) * (share + 1) / shares);
+  for (int at = static_cast<int>(static_cast<long long>(line) * share / shares); at < end;) {
+    const int a = at < routed * fkb ? at / fkb : routed, e = v.active[a], k0 = at - a * fkb, k1 = min(e < p.E ? fkb : p.sff / 64, k0 + end - at);
+    const uint8_t* wb = wt + static_cast<long long>(e) * fkb * 16384;
     const int first = v.off[e], n = v.off[e + 1] - first;
     for (int n0 = 0; n0 < n; n0 += NT * 8) {
-      const __nv_bfloat16* ar[NT];
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        const int c = n0 + j * 8 + g;
-        ar[j] = c < n ? p.act + static_cast<long long>(v.row[first + c]) * p.ld_act + t4 * 8 : nullptr;
-      }
-      float acc[2][NT][4];
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
-#pragma unroll 2
-      for (int kb = k0; kb < k1; ++kb) {
-        const uint8_t* wk = wb + static_cast<long long>(kb) * 16384;
-        uint4 w[4][2];
-#pragma unroll
-        for (int q = 0; q < 4; ++q)
-#pragma unroll
-          for (int s = 0; s < 2; ++s) w[q][s] = ldg_stream(wk + (q * 8 + g) * 128 + (((s * 4 + t4) ^ g) << 4));
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          if (j > 0 && n0 + j * 8 >= n) break;
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-#pragma unroll
-            for (int part = 0; part < 3; ++part) {
-              const uint4 x = ar[j] ? *reinterpret_cast<const uint4*>(ar[j] + part * p.part_stride + kb * 64 + s * 32) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                const uint4 lo = w[2 * i][s], hi = w[2 * i + 1][s];
-                mma_bf16(acc[i][j], lo.x, hi.x, lo.y, hi.y, x.x, x.y);
-                mma_bf16(acc[i][j], lo.z, hi.z, lo.w, hi.w, x.z, x.w);
-              }
-            }
-        }
-      }
-      // (a row occurs once among an expert's, so no two lanes add to the same place)
-#pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const int c = n0 + j * 8 + t4 * 2 + h;
-          if (c < n) {
-            const int pr = v.row[first + c], t = pr < P ? pr / p.top : pr - P;
-            float* s = mine + t * LD + g;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-              s[i * 16] += acc[i][j][h];
-              s[i * 16 + 8] += acc[i][j][2 + h];
-            }
-          }
-        }
-      __syncwarp();
+      if (NT > 1 && n - n0 <= 8) ml_down_pass<1>(p, v, wb, mine, first + n0, n - n0, k0, k1, g, t4);
+      else ml_down_pass<NT>(p, v, wb, mine, first + n0, n - n0, k0, k1, g, t4);
     }
+    at += k1 - k0;
   }
   __syncthreads();
   // the warps' sums, then the cluster's: each block adds up its share of the rows
@@ -574,9 +657,8 @@ int vb_moe_layer_route(int32_t* d_idx, float* d_wts, float* d_shared_gate, int k
   p.keep = keep;
   p.vocab = vocab;
   const int all = (kind == ML_TABLE ? 0 : experts) + (d_shared_gate_w ? 1 : 0), per = (all + ML_ROUTE_CLUSTER - 1) / ML_ROUTE_CLUSTER;
-  p.parts = per <= 1 ? 8 : per <= 2 ? 4 : per <= 4 ? 2 : 1;
-  const size_t smem = (static_cast<size_t>(per) * (p.parts + 1) * ML_ROUTE_CLUSTER + 2 * static_cast<size_t>(experts) + (groups > 1 ? groups : 0)) * 4;
-  VB_LAUNCH_PDL_CLUSTER(moe_layer_route_kernel, (T + ML_ROUTE_CLUSTER - 1) / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER, ML_THREADS, smem, stream, ML_ROUTE_CLUSTER, p);
+  const size_t smem = (static_cast<size_t>(ML_ROUTE_THREADS / 32 * 16 + per) * ML_ROUTE_CLUSTER + 2 * static_cast<size_t>(experts) + (groups > 1 ? groups : 0)) * 4;
+  VB_LAUNCH_PDL_CLUSTER(moe_layer_route_kernel, (T + ML_ROUTE_CLUSTER - 1) / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER, ML_ROUTE_THREADS, smem, stream, ML_ROUTE_CLUSTER, p);
   return 0;
 }
 
@@ -627,11 +709,12 @@ int vb_moe_layer_experts(float* d_y, long long ldy, const void* d_h, long long l
   p.slope = slope;
   p.up_units = (gated ? 2 * ff : ff) / 32;
   p.shared_units = (gated ? 2 * shared_ff : shared_ff) / 32;
-  const int sms = sm_count(), nt = T <= 8 ? 1 : T <= 16 ? 2 : 4;
+  // column tiles a pass: by the rows an expert has on average, so that most experts are read once
+  const int sms = sm_count(), nt = T <= 8 ? 1 : T <= 16 || T * top <= 8 * experts ? 2 : 4;
   const long long most = static_cast<long long>(experts < T * top ? experts : T * top) * p.up_units + p.shared_units;
-  const int grid_up = static_cast<int>(most < 2 * sms ? most : 2 * sms);
+  const int fit = (nt == 1 ? 3 : 2) * sms, grid_up = static_cast<int>(most < fit ? most : fit);
   const size_t plan_bytes = static_cast<size_t>(ml_plan_words(T, experts, top)) * 4;
-  const size_t smem_up = static_cast<size_t>(ML_WARPS) * 32 * (nt * 8 + (nt > 1 ? 8 : 0)) * 4 + plan_bytes;
+  const size_t smem_up = static_cast<size_t>(2 * ML_WARPS) * 32 * (nt * 8 + (nt > 1 ? 8 : 0)) * 4 + plan_bytes;
 #define ML_UP(NT, G)                                                              \
   do {                                                                            \
     VB_CHECK_CUDA(max_dyn_smem_once(moe_up_kernel<NT, G>));                       \
@@ -648,8 +731,8 @@ int vb_moe_layer_experts(float* d_y, long long ldy, const void* d_h, long long l
   }
 #undef ML_UP
   const int blocks = (W + 31) / 32;
-  int cluster = 1;
-  while (cluster < 8 && blocks * cluster < 2 * sms) cluster *= 2;
+  int cluster = 1;                       // one wave
+  while (cluster < 8 && blocks * cluster * 2 <= fit) cluster *= 2;
   p.cluster = cluster;
   const size_t smem_down = static_cast<size_t>(ML_WARPS) * T * 36 * 4 + plan_bytes;
 #define ML_DOWN(NT)                                                                                                 \
