@@ -20,6 +20,8 @@
 #define VB_PDL_FAMILY 4
 #include "rowmma.cuh"
 
+#include <type_traits>
+
 namespace vb {
 
 constexpr int ML_MAX_ROWS = 64, ML_MAX_EXPERTS = 1024, ML_MAX_TOP = 32, ML_THREADS = 256, ML_WARPS = 8;
@@ -36,6 +38,8 @@ struct MoeLayerParams {
   long long ldy, expert_bytes, part_stride;
   int T, W, E, top, ff, sff, ld_act, kb, up_rows, down_kb, act_kind, up_units, shared_units, cluster;
   float limit, slope;
+  unsigned char* wait_flag;
+  uint32_t top_inverse;                  // 2^32 / top, rounded up
 };
 
 // ---- router -----------------------------------------------------------------------------------------------------------------------
@@ -57,29 +61,29 @@ __device__ __forceinline__ uint32_t ml_key(float v) {
   if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
-// the largest key of keys[0 .. n) and its place (ties: the lowest), in every lane
-__device__ __forceinline__ int ml_argmax(const uint32_t* keys, int n, int lane) {
-  uint32_t best = 0u;
-  int at = 0x7fffffff;
-  for (int e = lane; e < n; e += 32)
-    if (at == 0x7fffffff || keys[e] > best) { best = keys[e]; at = e; }
-  const uint32_t top = __reduce_max_sync(0xffffffffu, best);
-  return __reduce_min_sync(0xffffffffu, best == top ? at : 0x7fffffff);
+__device__ __forceinline__ void st_dsmem_f32(const float* local_ptr, uint32_t cta_rank, float v) {
+  uint32_t raddr;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(raddr) : "r"(smem_u32(local_ptr)), "r"(cta_rank));
+  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(raddr), "f"(v) : "memory");
 }
-// A block's rows of the matrix (its share of the experts, 16 at a time) by the cluster's rows of h: the fp32 values as three bf16 parts (exact), the k
-// blocks of 32 divided by the warps.  What a warp needs first is asked for before the rows of h are there (the matrix is older than the kernel in front).
+// First the logits of the cluster's eight rows: a block's share of the experts, 16 at a time, by the rows of h on the matrix units, the fp32 matrix as three
+// bf16 parts (exact), the k blocks of 32 divided by the warps.  What a warp needs of the matrix is asked for before the rows of h are there (it is older than
+// the kernel in front).  Every logit goes into the shared memory of the block that its row belongs to.  Then each block picks one row's experts: an
+// expert's place is the number of those in front of it, which all threads count at once.
 __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const MoeRouteParams p) {
   extern __shared__ __align__(16) int smem[];
-  constexpr int WARPS = ML_ROUTE_THREADS / 32, AHEAD = 2;
+  constexpr int THREADS = ML_ROUTE_THREADS, WARPS = THREADS / 32, AHEAD = 4;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int rank = blockIdx.x % ML_ROUTE_CLUSTER, t0 = blockIdx.x / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER, rows = min(ML_ROUTE_CLUSTER, p.T - t0);
-  // the matrix's rows: the experts, then the shared expert's gate; a block has every eighth
-  const int E = p.kind == ML_TABLE ? 0 : p.E, all = E + (p.wsg ? 1 : 0), per = (all + ML_ROUTE_CLUSTER - 1) / ML_ROUTE_CLUSTER;
-  float* part = reinterpret_cast<float*>(smem);                   // [16 warps][16 of the block's][8 rows]
-  float* mine = part + WARPS * 16 * ML_ROUTE_CLUSTER;             // [per][8]: this block's logits
-  float* z = mine + per * ML_ROUTE_CLUSTER;                       // [E] the row's logits, then its scores
+  const int E = p.kind == ML_TABLE ? 0 : p.E, per = (E + ML_ROUTE_CLUSTER - 1) / ML_ROUTE_CLUSTER, t = t0 + rank;
+  const bool has = rank < rows;
+  float* part = reinterpret_cast<float*>(smem);                   // [16 warps][16 of the block's experts][8 rows]
+  float* z = part + WARPS * 16 * ML_ROUTE_CLUSTER;                // [E] the row's logits, then its scores
   uint32_t* keys = reinterpret_cast<uint32_t*>(z + p.E);          // [E]
   uint32_t* gkeys = keys + p.E;                                   // [groups]
+  float* chosen = reinterpret_cast<float*>(gkeys + p.groups);     // [32]
+  float* gate = chosen + 32;                                      // [16]
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");      // (every block has begun before another writes into it)
   const int kbs = (p.W + 31) / 32;
   float4 w[AHEAD][2][2];                                          // two rows, eight values each
   auto take = [&](int u, int i0, int kb) {
@@ -87,18 +91,32 @@ __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int e = (i0 + g + h * 8) * ML_ROUTE_CLUSTER + rank;
-      const bool in = e < all && i0 + g + h * 8 < per && k < p.W;
-      const float* r = (e < E ? p.w + static_cast<long long>(e) * p.W : p.wsg) + k;
+      const bool in = e < E && k < p.W;
+      const float* r = p.w + static_cast<long long>(e) * p.W + k;
       w[u][h][0] = in ? __ldg(reinterpret_cast<const float4*>(r)) : make_float4(0.f, 0.f, 0.f, 0.f);
       w[u][h][1] = in ? __ldg(reinterpret_cast<const float4*>(r + 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   };
-  if (per > 0)
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u) take(u, 0, warp + u * WARPS);
+  for (int u = 0; u < AHEAD; ++u) take(u, 0, warp + u * WARPS);
+  const float my_bias = p.bias && tid < E ? __ldg(p.bias + tid) : 0.f;
   pdl_sync();
   const __nv_bfloat16* hr = p.h + (t0 + min(g, rows - 1)) * p.ldh;
+  if (p.wsg && has) {                                             // the shared expert's gate
+    const __nv_bfloat16* hs = p.h + t * p.ldh;
+    float s = 0.f;
+    for (int k = tid * 8; k < p.W; k += THREADS * 8) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(p.wsg + k)), b = __ldg(reinterpret_cast<const float4*>(p.wsg + k + 4));
+      const uint4 x = *reinterpret_cast<const uint4*>(hs + k);
+      s = fmaf(bf16_lo(x.x), a.x, s); s = fmaf(bf16_hi(x.x), a.y, s); s = fmaf(bf16_lo(x.y), a.z, s); s = fmaf(bf16_hi(x.y), a.w, s);
+      s = fmaf(bf16_lo(x.z), b.x, s); s = fmaf(bf16_hi(x.z), b.y, s); s = fmaf(bf16_lo(x.w), b.z, s); s = fmaf(bf16_hi(x.w), b.w, s);
+    }
+    s = warp_sum(s);
+    if (lane == 0) gate[warp] = s;
+  }
+  bool begun = false;
   for (int i0 = 0; i0 < per; i0 += 16) {
+    const bool upper = per - i0 > 8;                              // (up to 64 experts: the lower half of a product's rows is not used)
     float acc[4] = {};
     for (int kb0 = warp; kb0 < kbs; kb0 += AHEAD * WARPS) {
       uint4 x[AHEAD];
@@ -109,7 +127,8 @@ __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const
         x[u] = k < p.W ? *reinterpret_cast<const uint4*>(hr + k) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
+      for (int u = 0; u < AHEAD; ++u) {
+        if (kb0 + u * WARPS >= kbs) break;
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           float v[2][4];
@@ -118,124 +137,147 @@ __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const
           uint32_t f[3][4];              // part, {row g, row g + 8} x {first pair, second pair}
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
-            float h0, m0, l0, h1, m1, l1;
-            bf16_parts(v[q & 1][(q >> 1) * 2], h0, m0, l0);
-            bf16_parts(v[q & 1][(q >> 1) * 2 + 1], h1, m1, l1);
-            f[0][q] = pack_cut(h0, h1);
-            f[1][q] = pack_cut(m0, m1);
-            f[2][q] = pack_cut(l0, l1);
+            f[0][q] = f[1][q] = f[2][q] = 0u;
+            if ((q & 1) && !upper) continue;
+            const float a = v[q & 1][(q >> 1) * 2], b = v[q & 1][(q >> 1) * 2 + 1];
+            const float ra = a - bf16_cut(a), rb = b - bf16_cut(b), sa = ra - bf16_cut(ra), sb = rb - bf16_cut(rb);
+            f[0][q] = pack_cut(a, b);
+            f[1][q] = pack_cut(ra, rb);
+            f[2][q] = pack_cut(sa, sb);
           }
 #pragma unroll
           for (int q = 0; q < 3; ++q) mma_bf16(acc, f[q][0], f[q][1], f[q][2], f[q][3], s ? x[u].z : x[u].x, s ? x[u].w : x[u].y);
         }
+      }
     }
+    if (i0 > 0) __syncthreads();                                  // (the sums before have been read)
     float* o = part + warp * 16 * ML_ROUTE_CLUSTER;
     *reinterpret_cast<float2*>(o + g * ML_ROUTE_CLUSTER + t4 * 2) = make_float2(acc[0], acc[1]);
     *reinterpret_cast<float2*>(o + (g + 8) * ML_ROUTE_CLUSTER + t4 * 2) = make_float2(acc[2], acc[3]);
     __syncthreads();
-    if (tid < 16 * ML_ROUTE_CLUSTER && i0 + tid / ML_ROUTE_CLUSTER < per) {
+    if (!begun) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
+    begun = true;
+    const int e = (i0 + tid / ML_ROUTE_CLUSTER) * ML_ROUTE_CLUSTER + rank, row = tid % ML_ROUTE_CLUSTER;
+    if (tid < 16 * ML_ROUTE_CLUSTER && e < E && row < rows) {
       float v = 0.f;
 #pragma unroll
       for (int q = 0; q < WARPS; ++q) v += part[q * 16 * ML_ROUTE_CLUSTER + tid];
-      mine[i0 * ML_ROUTE_CLUSTER + tid] = v;                      // (rows behind the last repeat it; nobody asks for them)
+      st_dsmem_f32(z + e, row, v);
     }
-    __syncthreads();
   }
+  if (!begun) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
   cluster_sync_all();
-  const bool has = rank < rows;
-  if (has) {
-    for (int e = tid; e < E; e += ML_ROUTE_THREADS) {
-      const float v = ld_dsmem_f32(mine + e / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER + rank, e % ML_ROUTE_CLUSTER);
-      z[e] = p.kind == ML_SOFTMAX && p.bias ? v + p.bias[e] : v;
-    }
-    if (p.wsg && tid == 0) {
-      const float v = ld_dsmem_f32(mine + E / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER + rank, E % ML_ROUTE_CLUSTER);
-      p.sgate[t0 + rank] = 1.f / (1.f + expf(-v));
-    }
-  }
-  cluster_sync_all();                                // (others' logits have been read; nobody leaves before)
-  if (!has || warp != 0) return;
-  const int t = t0 + rank;
+  if (!has) return;
   int32_t* idx = p.idx + t * p.top;
   float* wts = p.wts + t * p.top;
+  if (p.wsg && tid == 0) {
+    float s = 0.f;
+#pragma unroll
+    for (int q = 0; q < WARPS; ++q) s += gate[q];
+    p.sgate[t] = 1.f / (1.f + expf(-s));
+  }
   if (p.kind == ML_TABLE) {
     const int32_t* row = p.table + static_cast<long long>(min(max(p.ids[t], 0), p.vocab - 1)) * p.top;
-    if (lane < p.top) {
-      idx[lane] = row[lane];
-      wts[lane] = 1.f / p.top;
+    if (tid < p.top) {
+      idx[tid] = row[tid];
+      wts[tid] = 1.f / p.top;
     }
     return;
   }
   float mx = -INFINITY, sum = 0.f;
-  if (p.kind == ML_SOFTMAX_ALL) {
+  if (p.kind == ML_SOFTMAX_ALL && warp == 0) {
     for (int e = lane; e < E; e += 32) mx = fmaxf(mx, z[e]);
     mx = warp_max(mx);
     for (int e = lane; e < E; e += 32) sum += expf(z[e] - mx);
     sum = warp_sum(sum);
   }
-  for (int e = lane; e < E; e += 32) {
+  for (int e = tid; e < E; e += THREADS) {
+    const float bias = e == tid ? my_bias : p.bias ? p.bias[e] : 0.f;
     float v = z[e];
-    if (p.kind == ML_SIGMOID) {
-      z[e] = 1.f / (1.f + expf(-v));
-      v = z[e] + (p.bias ? p.bias[e] : 0.f);
+    if (p.kind == ML_SOFTMAX) {
+      v += bias;
+      z[e] = v;
+    } else if (p.kind == ML_SIGMOID) {
+      const float s = 1.f / (1.f + expf(-v));
+      z[e] = s;
+      v = s + bias;
     }
     keys[e] = ml_key(v);                             // (softmax scores rank as their logits do)
   }
-  __syncwarp();
+  __syncthreads();
   if (p.groups > 1 && p.keep < p.groups) {
     const int size = E / p.groups;
-    for (int g = lane; g < p.groups; g += 32) {
+    for (int gr = tid; gr < p.groups; gr += THREADS) {
       uint32_t a = 0u, b = 0u;                       // the two largest of the group
-      int ia = g * size, ib = g * size;
-      for (int e = g * size; e < (g + 1) * size; ++e) {
+      int ia = gr * size, ib = gr * size;
+      for (int e = gr * size; e < (gr + 1) * size; ++e) {
         const uint32_t k = keys[e];
         if (k > a) { b = a; ib = ia; a = k; ia = e; }
         else if (k > b) { b = k; ib = e; }
       }
       if (p.kind == ML_SIGMOID && size > 1) a = ml_key(z[ia] + (p.bias ? p.bias[ia] : 0.f) + (z[ib] + (p.bias ? p.bias[ib] : 0.f)));
-      gkeys[g] = a;
+      gkeys[gr] = a;
     }
-    __syncwarp();
-    for (int c = 0; c < p.keep; ++c) {
-      const int g = ml_argmax(gkeys, p.groups, lane);
-      __syncwarp();
-      if (lane == 0) gkeys[g] = 0u;                  // 0: kept (no score's key is 0)
-      __syncwarp();
+    __syncthreads();
+    for (int e = tid; e < E; e += THREADS) {
+      const int mine = e / size;
+      const uint32_t k = gkeys[mine];
+      int before = 0;
+      for (int o = 0; o < p.groups; ++o) before += gkeys[o] > k || (gkeys[o] == k && o < mine);
+      if (before >= p.keep) keys[e] = 0u;            // (no score's key is 0)
     }
-    for (int e = lane; e < E; e += 32)
-      if (gkeys[e / size] != 0u) keys[e] = 0u;
-    __syncwarp();
+    __syncthreads();
   }
-  float first = 0.f, denom = 0.f, my = 0.f;
-  for (int c = 0; c < p.top; ++c) {
-    const int e = ml_argmax(keys, E, lane);
-    const float v = z[e];
-    __syncwarp();
-    if (lane == 0) {
-      keys[e] = 0u;
-      idx[c] = e;
+  // up to 32 neighbouring threads count for an expert
+  int share = 1;
+  while (share < 32 && 2 * share * E <= THREADS) share *= 2;
+  for (int e0 = 0; e0 < E; e0 += THREADS / share) {
+    const int e = e0 + tid / share, q = tid % share;
+    const uint32_t k = e < E ? keys[e] : 0u;
+    int before = 0;
+    if (k != 0u)
+      for (int o = q; o < E; o += share) {
+        const uint32_t other = keys[o];
+        before += other > k || (other == k && o < e);
+      }
+    for (int o = share >> 1; o > 0; o >>= 1) before += __shfl_xor_sync(0xffffffffu, before, o);
+    if (k != 0u && q == 0 && before < p.top) {
+      idx[before] = e;
+      chosen[before] = z[e];
     }
-    if (c == 0) first = v;
-    const float s = p.kind == ML_SOFTMAX ? expf(v - first) : p.kind == ML_SOFTMAX_ALL ? expf(v - mx) : v;
-    denom += s;
-    if (lane == c) my = s;                           // (top <= 32)
-    __syncwarp();
   }
-  if (lane < p.top) wts[lane] = my / (p.kind == ML_SOFTMAX_ALL ? sum : p.kind == ML_SIGMOID ? denom + 1e-20f : denom);
+  __syncthreads();
+  if (warp != 0) return;
+  float s = 0.f;
+  if (lane < p.top) {                                // (top <= 32)
+    s = chosen[lane];
+    if (p.kind == ML_SOFTMAX) s = expf(s - chosen[0]);
+    else if (p.kind == ML_SOFTMAX_ALL) s = expf(s - mx);
+  }
+  const float denom = warp_sum(s);
+  if (lane < p.top) wts[lane] = s / (p.kind == ML_SOFTMAX_ALL ? sum : p.kind == ML_SIGMOID ? denom + 1e-20f : denom);
 }
 
+// row of a pair (no division: the step has at most 2^11 pairs)
+__device__ __forceinline__ int ml_row_of(const MoeLayerParams& p, int pair) { return p.top == 1 ? pair : static_cast<int>(__umulhi(static_cast<uint32_t>(pair), p.top_inverse)); }
+
 // The step's rows by expert, built by every block for itself (at most 64 x 32 pairs): `active` lists the experts that have rows, the shared one (number E) last.
-// Shared memory: counts and sums of the warps [20], idx[P], weight[P], row[P + T] (place of a pair's activations), off[E + 2], active[E + 2], cur[E].
-constexpr int ML_PLAN_HEAD = 20;
-__host__ __device__ inline int ml_plan_words(int T, int E, int top) { return ML_PLAN_HEAD + 3 * T * top + T + 3 * E + 4; }
+// Shared memory: counts and sums of the warps [32], idx[P], weight[P], row[P + T] (place of a pair's activations), off[E + 2], active[E + 2], line[E + 2], rows of
+// an expert as bits [2 E].
+// `line`: where an active expert's work starts when all of it stands in one line (the blocks take equal parts of it); a unit of work, 32 rows of weights or a
+// block of 64 k, costs what its columns take.
+constexpr int ML_PLAN_HEAD = 32;
+__host__ __device__ inline int ml_plan_words(int T, int E, int top) { return ML_PLAN_HEAD + 3 * T * top + T + 5 * E + 8; }
 struct MoePlanView {
-  int *n_active, *scan, *idx, *off, *active, *row, *cur;
+  int *n_active, *n_named, *scan, *idx, *off, *active, *row, *line;
+  uint32_t* bits;
   float* w;
 };
 __device__ __forceinline__ MoePlanView ml_view(int* s, int T, int E, int top) {
   MoePlanView v;
   const int P = T * top;
   v.n_active = s;
+  v.n_named = s + 1;
   v.scan = s + 4;
   s += ML_PLAN_HEAD;
   v.idx = s;
@@ -243,94 +285,170 @@ __device__ __forceinline__ MoePlanView ml_view(int* s, int T, int E, int top) {
   v.row = s + 2 * P;
   v.off = v.row + P + T;
   v.active = v.off + E + 2;
-  v.cur = v.active + E + 2;
+  v.line = v.active + E + 2;
+  v.bits = reinterpret_cast<uint32_t*>(v.line + E + 2);
   return v;
 }
 
-// ROUNDS: pairs a thread looks after (a step of 8 rows has at most one a thread)
+// ROUNDS: pairs a thread looks after (a step of 8 rows has at most one a thread).  An expert's rows are collected as bits, which sorts them and counts a
+// row once however often it names the expert.
+// Cost of a unit with n columns, in eighths of one with up to 8 (whose weights take longer to come than to multiply); measured as the times at which blocks of
+// such units end.
+__device__ __forceinline__ int ml_cost(int n, bool down) { return n <= 8 ? 8 : n <= 16 ? (down ? 12 : 10) : n <= 32 ? (down ? 24 : 18) : (down ? 56 : 38); }
 template <int ROUNDS>
-__device__ __forceinline__ void ml_build(const MoePlanView& v, const MoeLayerParams& p) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, P = p.T * p.top;
-  for (int e = tid; e < p.E; e += ML_THREADS) v.cur[e] = 0;
-  for (int i = tid; i < P; i += ML_THREADS) {
-    const int e = p.idx[i];
-    v.idx[i] = e >= 0 && e < p.E ? e : -1;
-    v.w[i] = p.wts[i];
-  }
-  __syncthreads();
-  // an expert named twice for a row: the first place takes both weights.  (Found first, written behind a barrier: others still compare.)
-  int keep[ROUNDS];
-  float weight[ROUNDS];
+__device__ __forceinline__ void ml_build(const MoePlanView& v, const MoeLayerParams& p, int units, int shared_units, bool down) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, P = p.T * p.top, rounds = (P + ML_THREADS - 1) / ML_THREADS;
+  int mine[ROUNDS] = {};
+  float weight[ROUNDS] = {};
 #pragma unroll
   for (int k = 0; k < ROUNDS; ++k) {
+    if (k >= rounds) break;
     const int i = tid + k * ML_THREADS;
-    keep[k] = -1;
-    if (i >= P) continue;
-    const int t = i / p.top, c = i - t * p.top, e = v.idx[i];
-    bool first = e >= 0;
-    float w = v.w[i];
-    for (int j = 0; j < p.top; ++j)
-      if (j != c && v.idx[t * p.top + j] == e) {
-        if (j < c) first = false;
-        else w += v.w[t * p.top + j];
-      }
-    if (first) {
-      keep[k] = e;
-      weight[k] = w;
-      atomicAdd(&v.cur[e], 1);
+    mine[k] = -1;
+    weight[k] = 0.f;
+    if (i < P) {
+      const int e = p.idx[i];
+      mine[k] = e >= 0 && e < p.E ? e : -1;
+      weight[k] = p.wts[i];
     }
+  }
+  for (int e = tid; e < 2 * p.E; e += ML_THREADS) v.bits[e] = 0u;
+  if (tid == 0) *v.n_named = 0;
+  int named = 0;
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
+    if (k >= rounds) break;
+    const int i = tid + k * ML_THREADS;
+    if (i < P) {
+      v.idx[i] = mine[k];
+      v.w[i] = weight[k];
+      named += mine[k] >= 0;
+    }
+  }
+  named = __reduce_add_sync(0xffffffffu, named);
+  __syncthreads();
+  if (lane == 0 && named) atomicAdd(v.n_named, named);
+#pragma unroll
+  for (int k = 0; k < ROUNDS; ++k) {
+    if (k >= rounds) break;
+    const int t = ml_row_of(p, tid + k * ML_THREADS);
+    if (mine[k] >= 0) atomicOr(v.bits + 2 * mine[k] + (t >> 5), 1u << (t & 31));
   }
   __syncthreads();
   // places of the experts' rows, and the list of those that have any: four neighbouring experts a thread
-  int n[4], rows = 0, some = 0;
+  int n[4], rows = 0, some = 0, cost = 0;
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int e = tid * 4 + k;
-    n[k] = e < p.E ? v.cur[e] : 0;
+    n[k] = e < p.E ? __popc(v.bits[2 * e]) + __popc(v.bits[2 * e + 1]) : 0;
     rows += n[k];
     some += n[k] > 0;
+    cost += n[k] > 0 ? ml_cost(n[k], down) * units : 0;
   }
-  int r = rows, m = some;
+  int r = rows, m = some, l = cost;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int rr = __shfl_up_sync(0xffffffffu, r, o), mm = __shfl_up_sync(0xffffffffu, m, o);
-    if (lane >= o) { r += rr; m += mm; }
+    const int rr = __shfl_up_sync(0xffffffffu, r, o), mm = __shfl_up_sync(0xffffffffu, m, o), ll = __shfl_up_sync(0xffffffffu, l, o);
+    if (lane >= o) { r += rr; m += mm; l += ll; }
   }
-  if (lane == 31) { v.scan[warp] = r; v.scan[ML_WARPS + warp] = m; }
+  if (lane == 31) { v.scan[warp] = r; v.scan[ML_WARPS + warp] = m; v.scan[2 * ML_WARPS + warp] = l; }
   __syncthreads();
-  int r0 = r - rows, m0 = m - some, r_all = 0, m_all = 0;
+  int r0 = r - rows, m0 = m - some, l0 = l - cost, r_all = 0, m_all = 0, l_all = 0;
 #pragma unroll
   for (int q = 0; q < ML_WARPS; ++q) {
-    if (q < warp) { r0 += v.scan[q]; m0 += v.scan[ML_WARPS + q]; }
+    if (q < warp) { r0 += v.scan[q]; m0 += v.scan[ML_WARPS + q]; l0 += v.scan[2 * ML_WARPS + q]; }
     r_all += v.scan[q];
     m_all += v.scan[ML_WARPS + q];
+    l_all += v.scan[2 * ML_WARPS + q];
   }
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     const int e = tid * 4 + k;
     if (e < p.E) {
       v.off[e] = r0;
-      v.cur[e] = r0;
-      if (n[k] > 0) v.active[m0++] = e;
+      if (n[k] > 0) {
+        v.line[m0] = l0;
+        v.active[m0++] = e;
+        l0 += ml_cost(n[k], down) * units;
+      }
       r0 += n[k];
     }
   }
   if (tid == 0) {
     v.off[p.E] = r_all;
     v.off[p.E + 1] = r_all + (p.sff > 0 ? p.T : 0);
-    if (p.sff > 0) v.active[m_all] = p.E;
+    v.line[m_all] = l_all;
+    if (p.sff > 0) {
+      v.active[m_all] = p.E;
+      v.line[m_all + 1] = l_all + ml_cost(p.T, down) * shared_units;
+    }
     *v.n_active = m_all + (p.sff > 0 ? 1 : 0);
   }
   if (p.sff > 0 && tid < p.T) v.row[r_all + tid] = P + tid;
+  const bool twice = *v.n_named != r_all;                // (the same in all threads) a row names an expert twice: the first place takes both weights
+  if (twice) {
+#pragma unroll
+    for (int k = 0; k < ROUNDS; ++k) {
+    if (k >= rounds) break;
+      const int i = tid + k * ML_THREADS, t = ml_row_of(p, i), c = i - t * p.top;
+      if (mine[k] < 0) continue;
+      const int e = mine[k];
+      for (int j = 0; j < p.top; ++j)
+        if (j != c && v.idx[t * p.top + j] == e) {
+          if (j < c) mine[k] = -1;
+          else weight[k] += v.w[t * p.top + j];
+        }
+    }
+  }
   __syncthreads();
 #pragma unroll
-  for (int k = 0; k < ROUNDS; ++k)
-    if (keep[k] >= 0) {
-      const int i = tid + k * ML_THREADS;
-      v.row[atomicAdd(&v.cur[keep[k]], 1)] = i;
+  for (int k = 0; k < ROUNDS; ++k) {
+    if (k >= rounds) break;
+    if (mine[k] >= 0) {
+      const int i = tid + k * ML_THREADS, t = ml_row_of(p, i);
+      const uint32_t b0 = v.bits[2 * mine[k]], b1 = v.bits[2 * mine[k] + 1], below = (1u << (t & 31)) - 1u;
+      v.row[v.off[mine[k]] + (t < 32 ? __popc(b0 & below) : __popc(b0) + __popc(b1 & below))] = i;
       v.w[i] = weight[k];
     }
+  }
   __syncthreads();
+}
+
+// A part of the line: units from (a, unit) on that start before `end`.
+struct MlWalk {
+  int a, unit, at, step, units;          // the active expert, its unit, where that starts, its cost, how many the expert has
+  bool down;
+};
+__device__ __forceinline__ void ml_expert(MlWalk& w, const MoePlanView& v, int E, int units, int shared_units) {
+  const int e = v.active[w.a];
+  w.units = e < E ? units : shared_units;
+  w.step = ml_cost(v.off[e + 1] - v.off[e], w.down);
+}
+__device__ __forceinline__ MlWalk ml_walk(const MoePlanView& v, int begin, int E, int units, int shared_units, bool down) {
+  MlWalk w;
+  w.down = down;
+  int lo = 0, hi = *v.n_active;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (v.line[mid] <= begin) lo = mid;
+    else hi = mid;
+  }
+  w.a = lo;
+  ml_expert(w, v, E, units, shared_units);
+  w.unit = (begin - v.line[lo] + w.step - 1) / w.step;
+  w.at = v.line[lo] + w.unit * w.step;
+  if (w.unit >= w.units && lo + 1 < *v.n_active) {       // (begins inside the expert's last unit)
+    ++w.a;
+    w.unit = 0;
+    ml_expert(w, v, E, units, shared_units);
+  }
+  return w;
+}
+__device__ __forceinline__ void ml_next(MlWalk& w, const MoePlanView& v, int E, int units, int shared_units) {
+  w.at += w.step;
+  if (++w.unit < w.units) return;
+  w.unit = 0;
+  if (++w.a < *v.n_active) ml_expert(w, v, E, units, shared_units);
 }
 
 __device__ __forceinline__ float ml_gelu_tanh(float x) { return 0.5f * x * (1.f + tanhf(0.7978845608028654f * (x + 0.044715f * x * x * x))); }
@@ -351,44 +469,95 @@ __device__ __forceinline__ float ml_act(int kind, float g, float u, float limit,
   }
 }
 
-// ---- gate | up ------------------------------------------------------------------------------------------------------------------
-// NT column tiles of 8 rows a pass over the weights (an expert with more rows takes further passes, its weights from L2 then).
-// All loads of a k block come before its first product.  A column tile's unused columns repeat the first row (a product's columns do not touch one another).
-template <int NT>
-__device__ __forceinline__ void ml_up_product(float (&acc)[2][NT][4], const uint8_t* wb, const __nv_bfloat16* const (&hr)[NT], int k0, int step,
-                                              const MoeLayerParams& p, int g, int t4) {
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
-#pragma unroll 1
-  for (int kb = k0; kb < p.kb; kb += step) {
-    const uint8_t* wk = wb + static_cast<long long>(kb) * p.up_rows * 128;
-    uint4 w[4][2], x[NT][2];
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) w[q][s] = ldg_stream(wk + (q * 8 + g) * 128 + (((s * 4 + t4) ^ g) << 4));
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        const int k = kb * 64 + (s * 4 + t4) * 8;
-        x[j][s] = k < p.W ? *reinterpret_cast<const uint4*>(hr[j] + k) : make_uint4(0u, 0u, 0u, 0u);
-      }
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int s = 0; s < 2; ++s)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const uint4 lo = w[i][s], hi = w[i + 2][s];
-          mma_bf16(acc[i][j], lo.x, hi.x, lo.y, hi.y, x[j][s].x, x[j][s].y);
-          mma_bf16(acc[i][j], lo.z, hi.z, lo.w, hi.w, x[j][s].z, x[j][s].w);
-        }
+// ---- weights on their way ---------------------------------------------------------------------------------------------------------
+// Every warp has a ring of its own in shared memory: places of 4 KB, a block of 64 k of 32 rows each (one run of the packed tiles), filled by bulk copies that
+// its first lane asks for as soon as the warp has read a place.  What is on its way neither holds registers nor stops at the end of an item, and no
+// warp waits for another's data: 96 KB an SM are always on their way (2.2 us at an SM's share of the memory's rate).
+constexpr int ML_SLOT_BYTES = 4096;
+__host__ __device__ constexpr int ml_ring_bytes(int slots) { return ML_WARPS * slots * (ML_SLOT_BYTES + 8); }
+template <int SLOTS>
+struct MlRing {
+  uint8_t* slots;
+  uint64_t* bars;
+  int put = 0, got = 0;
+  uint32_t parity = 0u;
+  __device__ __forceinline__ void ask(const uint8_t* src) {              // (one lane)
+    mbar_arrive_expect_tx(bars + put, ML_SLOT_BYTES);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(slots + put * ML_SLOT_BYTES)), "l"(src),
+                 "r"(ML_SLOT_BYTES), "r"(smem_u32(bars + put))
+                 : "memory");
   }
+  __device__ __forceinline__ void asked() { put = put + 1 == SLOTS ? 0 : put + 1; }
+  __device__ __forceinline__ const uint8_t* wait(BoundedWait& bw) {
+    bw.wait(bars + got, parity);
+    return slots + got * ML_SLOT_BYTES;
+  }
+  __device__ __forceinline__ void read() {
+    got = got + 1 == SLOTS ? 0 : got + 1;
+    parity ^= got == 0 ? 1u : 0u;
+  }
+};
+// shared memory of both kernels: the rings, their barriers, then the kernel's own
+template <int SLOTS>
+__device__ __forceinline__ MlRing<SLOTS> ml_ring(int* smem, int warp) {
+  MlRing<SLOTS> r;
+  r.slots = reinterpret_cast<uint8_t*>(smem) + warp * SLOTS * ML_SLOT_BYTES;
+  r.bars = reinterpret_cast<uint64_t*>(reinterpret_cast<uint8_t*>(smem) + ML_WARPS * SLOTS * ML_SLOT_BYTES) + warp * SLOTS;
+  if ((threadIdx.x & 31) == 0) {
+    for (int i = 0; i < SLOTS; ++i) mbar_init(r.bars + i, 1);
+    fence_barrier_init();
+    fence_proxy_async();
+  }
+  __syncwarp();
+  return r;
+}
+// The lane's place among 8 rows.  Lanes 0 to 7 of a 16-byte load read two rows of 128 swizzled bytes; rows four apart lie in different banks.
+__device__ __forceinline__ int ml_row(int g) { return (g >> 1) | ((g & 1) << 2); }
+__device__ __forceinline__ void ml_weights(uint4 (&w)[4][2], const uint8_t* slot, int r, int t4) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+#pragma unroll
+    for (int s = 0; s < 2; ++s) w[q][s] = *reinterpret_cast<const uint4*>(slot + (q * 8 + r) * 128 + (((s * 4 + t4) ^ r) << 4));
+}
+// row of the step that a place of activations belongs to (the shared expert's follow the pairs')
+__device__ __forceinline__ int ml_token(const MoeLayerParams& p, int place) {
+  const int P = p.T * p.top;
+  return place < P ? ml_row_of(p, place) : place - P;
+}
+// rows of a column tile: a tile's unused columns repeat the first row (a product's columns do not touch one another)
+template <int NT>
+__device__ __forceinline__ void ml_rows(const __nv_bfloat16* (&r)[NT], const __nv_bfloat16* base, long long ld, const MoePlanView& v, int first, int cols, int g,
+                                        const MoeLayerParams& p, bool by_row) {
+#pragma unroll
+  for (int j = 0; j < NT; ++j) {
+    const int c = j * 8 + g, pr = v.row[first + (c < cols ? c : 0)];
+    r[j] = base + (by_row ? ml_token(p, pr) : pr) * ld;
+  }
+}
+// calls f with 1, 2 or 4 column tiles, as `cols` columns need and the kernel has
+template <int NT, typename F>
+__device__ __forceinline__ void ml_by_columns(int cols, F&& f) {
+  if constexpr (NT == 1) f(std::integral_constant<int, 1>());
+  else if (cols <= 8) f(std::integral_constant<int, 1>());
+  else if (cols <= 16) f(std::integral_constant<int, 2>());
+  else f(std::integral_constant<int, 4>());
+}
+
+// ---- gate | up ------------------------------------------------------------------------------------------------------------------
+// A unit is 32 rows of an expert's matrix (NT * 8 of the expert's rows a pass; further passes take the weights from L2), k blocks w, w + 8, .. to warp w.
+struct MlUpUnit {
+  const uint8_t* w;
+  int first, n, passes;
+};
+template <int NT>
+__device__ __forceinline__ MlUpUnit ml_up_unit(const MoeLayerParams& p, const MoePlanView& v, const MlWalk& at) {
+  MlUpUnit m;
+  const int e = v.active[at.a], row0 = at.unit * 32, tile = row0 / p.up_rows, r0 = row0 - tile * p.up_rows;
+  m.w = p.up + e * p.expert_bytes + (static_cast<long long>(tile) * p.kb * p.up_rows + r0) * 128;
+  m.first = v.off[e];
+  m.n = v.off[e + 1] - m.first;
+  m.passes = (m.n + NT * 8 - 1) / (NT * 8);
+  return m;
 }
 // one activation, times its row's routing weight, as parts
 __device__ __forceinline__ void ml_store(const MoeLayerParams& p, const MoePlanView& v, int place, int col, float g, float u) {
@@ -401,207 +570,300 @@ __device__ __forceinline__ void ml_store(const MoeLayerParams& p, const MoePlanV
   o[p.part_stride] = __float2bfloat16_rn(mid);
   o[2 * p.part_stride] = __float2bfloat16_rn(lo);
 }
-template <int NT>
-__device__ __forceinline__ void ml_rows(const __nv_bfloat16* (&r)[NT], const __nv_bfloat16* base, long long ld, const MoePlanView& v, int first, int cols, int g, int P,
-                                        int top, bool by_row) {
-#pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int c = j * 8 + g, pr = v.row[first + (c < cols ? c : 0)];
-    r[j] = base + (by_row ? (pr < P ? pr / top : pr - P) : pr) * ld;
-  }
-}
-// sums of one pass over an item: complete in the lanes (share 1), or parts of them that `share` warps leave in shared memory
-template <int NT, int LD, bool GATED>
-__device__ __forceinline__ void ml_up_pass(const MoeLayerParams& p, const MoePlanView& v, const uint8_t* wb, float* mine, int first, int cols, int unit, int part,
-                                           int share, int g, int t4) {
-  float acc[2][NT][4];
-  const __nv_bfloat16* hr[NT];
-  ml_rows<NT>(hr, p.h, p.ldh, v, first, cols, g, p.T * p.top, p.top, true);
-  ml_up_product<NT>(acc, wb, hr, part, share, p, g, t4);
-  if (share > 1) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        *reinterpret_cast<float2*>(mine + (i * 8 + g) * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][0], acc[i][j][1]);
-        *reinterpret_cast<float2*>(mine + (16 + i * 8 + g) * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][2], acc[i][j][3]);
-      }
-    return;
-  }
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = j * 8 + t4 * 2 + h;
-      if (c < cols)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          if (GATED) ml_store(p, v, first + c, unit * 16 + i * 8 + g, acc[i][j][h], acc[i][j][2 + h]);
-          else {
-            ml_store(p, v, first + c, unit * 32 + i * 8 + g, 0.f, acc[i][j][h]);
-            ml_store(p, v, first + c, unit * 32 + 16 + i * 8 + g, 0.f, acc[i][j][2 + h]);
-          }
-        }
-    }
-}
-// An item is 32 rows of an expert's matrix.  Where the step has items for all warps a warp takes one by itself, its sums complete in its registers (a gate
-// row and its up row in the same lane); where it has few, 2, 4 or 8 warps divide an item's k and meet in shared memory.
-template <int NT, bool GATED>
-__global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 3 : 2) moe_up_kernel(const MoeLayerParams p) {
-  extern __shared__ __align__(16) int smem[];
-  constexpr int LD = NT * 8 + (NT > 1 ? 8 : 0);
-  float* red = reinterpret_cast<float*>(smem);           // two times [8 warps][32][LD]: a round's sums are read while the next round's are made
-  const MoePlanView v = ml_view(smem + 2 * ML_WARPS * 32 * LD, p.T, p.E, p.top);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+template <int NT, bool GATED, int SLOTS>
+__global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 2 : 1) moe_up_kernel(const MoeLayerParams p) {
+  extern __shared__ __align__(128) int smem[];
+  constexpr int LD_MAX = NT * 8 + (NT > 1 ? 8 : 0);
+  // two times [8 warps][32][LD_MAX]: a pass's sums are read while the next one's are made
+  float* red = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(smem) + ml_ring_bytes(SLOTS));
+  const MoePlanView v = ml_view(reinterpret_cast<int*>(red + 2 * ML_WARPS * 32 * LD_MAX), p.T, p.E, p.top);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3, r = ml_row(g);
+  MlRing<SLOTS> ring = ml_ring<SLOTS>(smem, warp);
+  BoundedWait bw{p.wait_flag};
   pdl_sync();
-  ml_build<NT == 1 ? 8 * ML_MAX_TOP / ML_THREADS : ML_MAX_ROWS * ML_MAX_TOP / ML_THREADS>(v, p);
-  const int n_active = *v.n_active, routed = p.sff > 0 ? n_active - 1 : n_active;
-  const int items = routed * p.up_units + p.shared_units;
-  int share = 1;                                         // warps of an item
-  while (share < ML_WARPS && items * share * 2 <= static_cast<int>(gridDim.x) * ML_WARPS) share *= 2;
-  const int groups = ML_WARPS / share, group = warp / share, part = warp % share;
-  const int rounds = (items + groups * gridDim.x - 1) / (groups * gridDim.x);
+  ml_build<NT == 1 ? 8 * ML_MAX_TOP / ML_THREADS : ML_MAX_ROWS * ML_MAX_TOP / ML_THREADS>(v, p, p.up_units, p.shared_units, false);
+  const int n_active = *v.n_active;
+  if (n_active == 0) return;
+  const int total = v.line[n_active], warps = min(ML_WARPS, p.kb);      // (a warp takes every eighth k block)
+  const int begin = static_cast<int>(static_cast<long long>(total) * blockIdx.x / gridDim.x),
+            end = static_cast<int>(static_cast<long long>(total) * (blockIdx.x + 1) / gridDim.x);
+  const MlWalk start = ml_walk(v, begin, p.E, p.up_units, p.shared_units, false);
+  // what is asked for next
+  MlWalk ask_at = start;
+  int ask_pass = 0, ask_kb = warp;
+  MlUpUnit ask_m = {};
+  if (warp >= warps) ask_at.at = end;
+  if (ask_at.at < end) ask_m = ml_up_unit<NT>(p, v, ask_at);
+  auto ask = [&]() {
+    if (ask_at.at >= end) return;
+    if (lane == 0 && !bw.dead) ring.ask(ask_m.w + static_cast<long long>(ask_kb) * p.up_rows * 128);
+    ring.asked();
+    ask_kb += ML_WARPS;
+    if (ask_kb < p.kb) return;
+    ask_kb = warp;
+    if (++ask_pass < ask_m.passes) return;
+    ask_pass = 0;
+    ml_next(ask_at, v, p.E, p.up_units, p.shared_units);
+    if (ask_at.at < end) ask_m = ml_up_unit<NT>(p, v, ask_at);
+  };
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) ask();
   int turn = 0;
-  for (int round = 0; round < rounds; ++round) {
-    const int it = (round * groups + group) * gridDim.x + blockIdx.x;
-    const bool on = it < items;
-    const int a = it < routed * p.up_units ? it / p.up_units : routed, unit = it - a * p.up_units, e = on ? v.active[a] : 0;
-    const int row0 = unit * 32, tile = row0 / p.up_rows, r0 = row0 - tile * p.up_rows;
-    const uint8_t* wb = p.up + e * p.expert_bytes + (static_cast<long long>(tile) * p.kb * p.up_rows + r0) * 128;
-    const int first = on ? v.off[e] : 0, n = on ? v.off[e + 1] - first : 0;
-    int passes = (n + NT * 8 - 1) / (NT * 8);
-    if (share > 1 && p.T > NT * 8) passes = __syncthreads_or(passes > 1) ? (ML_MAX_ROWS + NT * 8 - 1) / (NT * 8) : 1;      // (all groups meet in every pass)
-    else if (share > 1) passes = 1;
-    for (int pass = 0; pass < passes; ++pass) {
-      const int n0 = pass * NT * 8, cols = n - n0;
-      float* sums = red + (turn++ & 1) * ML_WARPS * 32 * LD;
-      if (NT > 1 && cols > 0 && cols <= 8) ml_up_pass<1, LD, GATED>(p, v, wb, sums + warp * 32 * LD, first + n0, cols, unit, part, share, g, t4);
-      else if (cols > 0) ml_up_pass<NT, LD, GATED>(p, v, wb, sums + warp * 32 * LD, first + n0, cols, unit, part, share, g, t4);
-      if (share == 1) continue;
-      __syncthreads();
-      constexpr int COLS = GATED ? 16 : 32;
-      for (int i = part * 32 + lane; i < COLS * min(NT * 8, cols); i += share * 32) {
-        const int col = i % COLS, c = i / COLS;
-        float s1 = 0.f, s2 = 0.f;
-        for (int q = 0; q < share; ++q) {
-          s1 += sums[((group * share + q) * 32 + col) * LD + c];
-          if (GATED) s2 += sums[((group * share + q) * 32 + 16 + col) * LD + c];
+  for (MlWalk at = start; at.at < end; ml_next(at, v, p.E, p.up_units, p.shared_units)) {
+    const MlUpUnit m = ml_up_unit<NT>(p, v, at);
+    for (int pass = 0; pass < m.passes; ++pass, ++turn) {
+      const int n0 = pass * NT * 8, cols = m.n - n0;
+      float* sums = red + (turn & 1) * ML_WARPS * 32 * LD_MAX;
+      ml_by_columns<NT>(cols, [&](auto tiles) {
+        constexpr int N = decltype(tiles)::value, LD = N * 8 + (N > 1 ? 8 : 0);
+        float acc[2][N][4] = {};
+        const __nv_bfloat16* hr[N];
+        ml_rows<N>(hr, p.h + t4 * 8, p.ldh, v, m.first + n0, cols, g, p, true);
+        uint4 next[N][2];
+        auto take = [&](int kb) {
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+              const int k = kb * 64 + s * 32;
+              next[j][s] = k + t4 * 8 < p.W ? *reinterpret_cast<const uint4*>(hr[j] + k) : make_uint4(0u, 0u, 0u, 0u);
+            }
+        };
+        take(warp);
+        for (int kb = warp; kb < p.kb; kb += ML_WARPS) {
+          uint4 x[N][2], w[4][2];
+#pragma unroll
+          for (int j = 0; j < N; ++j) { x[j][0] = next[j][0]; x[j][1] = next[j][1]; }
+          take(kb + ML_WARPS);
+          ml_weights(w, ring.wait(bw), r, t4);
+#pragma unroll
+          for (int j = 0; j < N; ++j)
+#pragma unroll
+            for (int s = 0; s < 2; ++s)
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                // gated: 16 gate rows, then their up rows; a product's upper half takes the one, its lower half the other
+                const uint4 lo = w[i][s], hi = w[i + 2][s];
+                mma_bf16(acc[i][j], lo.x, hi.x, lo.y, hi.y, x[j][s].x, x[j][s].y);
+                mma_bf16(acc[i][j], lo.z, hi.z, lo.w, hi.w, x[j][s].z, x[j][s].w);
+              }
+          __syncwarp();
+          ring.read();
+          ask();
         }
-        ml_store(p, v, first + n0 + c, unit * COLS + col, s1, GATED ? s2 : s1);
-      }
+        if (warp < warps) {
+          float* mine = sums + warp * 32 * LD;
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int j = 0; j < N; ++j) {
+              *reinterpret_cast<float2*>(mine + (i * 8 + r) * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][0], acc[i][j][1]);
+              *reinterpret_cast<float2*>(mine + (16 + i * 8 + r) * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][2], acc[i][j][3]);
+            }
+        }
+        __syncthreads();
+        // (another warp begins each time: a unit of few columns is one warp's work, and the others go on)
+        constexpr int COLS = GATED ? 16 : 32;
+        for (int i = (tid + 32 * turn) & (ML_THREADS - 1); i < COLS * min(N * 8, cols); i += ML_THREADS) {
+          const int col = i % COLS, c = i / COLS;
+          float s1 = 0.f, s2 = 0.f;
+          for (int q = 0; q < warps; ++q) {
+            s1 += sums[(q * 32 + col) * LD + c];
+            if (GATED) s2 += sums[(q * 32 + 16 + col) * LD + c];
+          }
+          ml_store(p, v, m.first + n0 + c, at.unit * COLS + col, s1, GATED ? s2 : s1);
+        }
+      });
     }
   }
 }
 
 // ---- down -------------------------------------------------------------------------------------------------------------------------
-// Products of one expert's k blocks k0 .. k1 - 1 with NT column tiles, added to the warp's rows of sums.  All loads of a k block come before its first product.
+// A unit is a block of 64 k of an expert; every warp of the cluster takes an equal part of the line, and what a part has of one expert is a piece.
 constexpr int ML_LD = 36;                // floats between rows of sums (32 columns)
+struct MlDownPiece {
+  const uint8_t* w;
+  int first, n, passes, k0, k1;
+};
 template <int NT>
-__device__ __forceinline__ void ml_down_pass(const MoeLayerParams& p, const MoePlanView& v, const uint8_t* wb, float* mine, int first, int cols, int k0, int k1, int g,
-                                             int t4) {
-  const int P = p.T * p.top;
-  const __nv_bfloat16* ar[NT];
-  ml_rows<NT>(ar, p.act + t4 * 8, p.ld_act, v, first, cols, g, P, p.top, false);
-  float acc[2][NT][4];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-#pragma unroll
-    for (int j = 0; j < NT; ++j)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
-#pragma unroll 1
-  for (int kb = k0; kb < k1; ++kb) {
-    const uint8_t* wk = wb + static_cast<long long>(kb) * 16384;
-    uint4 w[4][2];
-#pragma unroll
-    for (int q = 0; q < 4; ++q)
-#pragma unroll
-      for (int s = 0; s < 2; ++s) w[q][s] = ldg_stream(wk + (q * 8 + g) * 128 + (((s * 4 + t4) ^ g) << 4));
-#pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      uint4 x[3][2];
-#pragma unroll
-      for (int part = 0; part < 3; ++part)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) x[part][s] = *reinterpret_cast<const uint4*>(ar[j] + part * p.part_stride + kb * 64 + s * 32);
-#pragma unroll
-      for (int part = 0; part < 3; ++part)
-#pragma unroll
-        for (int s = 0; s < 2; ++s)
-#pragma unroll
-          for (int i = 0; i < 2; ++i) {
-            const uint4 lo = w[2 * i][s], hi = w[2 * i + 1][s];
-            mma_bf16(acc[i][j], lo.x, hi.x, lo.y, hi.y, x[part][s].x, x[part][s].y);
-            mma_bf16(acc[i][j], lo.z, hi.z, lo.w, hi.w, x[part][s].z, x[part][s].w);
-          }
-    }
-  }
-  // (a row occurs once among an expert's, so no two lanes add to the same place)
-#pragma unroll
-  for (int j = 0; j < NT; ++j)
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int c = j * 8 + t4 * 2 + h;
-      if (c < cols) {
-        const int pr = v.row[first + c], t = pr < P ? pr / p.top : pr - P;
-        float* s = mine + t * ML_LD + g;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          s[i * 16] += acc[i][j][h];
-          s[i * 16 + 8] += acc[i][j][2 + h];
-        }
-      }
-    }
-  __syncwarp();
+__device__ __forceinline__ MlDownPiece ml_down_piece(const MoeLayerParams& p, const MoePlanView& v, const uint8_t* wt, const MlWalk& at, int end) {
+  MlDownPiece m;
+  const int e = v.active[at.a];
+  m.k0 = at.unit;
+  m.k1 = min(at.units, at.unit + (end - at.at + at.step - 1) / at.step);
+  m.w = wt + static_cast<long long>(e) * (p.ff / 64) * 16384;
+  m.first = v.off[e];
+  m.n = v.off[e + 1] - m.first;
+  m.passes = (m.n + NT * 8 - 1) / (NT * 8);
+  return m;
 }
-// The k blocks of all chosen experts stand in one line, of which every warp of the cluster takes an equal part.
-template <int NT>
-__global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 3 : 2) moe_down_kernel(const MoeLayerParams p) {
-  extern __shared__ __align__(16) int smem[];
+__device__ __forceinline__ float4 ld_dsmem_f32x4(const float* local_ptr, uint32_t cta_rank) {
+  uint32_t raddr;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(raddr) : "r"(smem_u32(local_ptr)), "r"(cta_rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(raddr) : "memory");
+  return v;
+}
+// four neighbours of a row of the result (its rows may start anywhere)
+__device__ __forceinline__ void ml_result(const MoeLayerParams& p, int t, int col, const float4& s) {
+  float* y = p.y + t * p.ldy + col;
+  if (col + 4 <= p.W && (reinterpret_cast<uintptr_t>(y) & 15) == 0) {
+    *reinterpret_cast<float4*>(y) = s;
+    return;
+  }
+  if (col < p.W) y[0] = s.x;
+  if (col + 1 < p.W) y[1] = s.y;
+  if (col + 2 < p.W) y[2] = s.z;
+  if (col + 3 < p.W) y[3] = s.w;
+}
+template <int NT, int SLOTS>
+__global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 2 : 1) moe_down_kernel(const MoeLayerParams p) {
+  extern __shared__ __align__(128) int smem[];
   constexpr int LD = ML_LD;
-  float* sums = reinterpret_cast<float*>(smem);          // [8 warps][T][LD]
-  const MoePlanView v = ml_view(smem + ML_WARPS * p.T * LD, p.T, p.E, p.top);
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+  float* sums = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(smem) + ml_ring_bytes(SLOTS));          // [8 warps][T][LD]
+  const MoePlanView v = ml_view(reinterpret_cast<int*>(sums + ML_WARPS * p.T * LD), p.T, p.E, p.top);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3, r = ml_row(g);
   const int rank = blockIdx.x % p.cluster, block = blockIdx.x / p.cluster;
+  MlRing<SLOTS> ring = ml_ring<SLOTS>(smem, warp);
+  BoundedWait bw{p.wait_flag};
   // (routing and weights are older than the up kernel, whose activations are all that has to be waited for)
-  ml_build<NT == 1 ? 8 * ML_MAX_TOP / ML_THREADS : ML_MAX_ROWS * ML_MAX_TOP / ML_THREADS>(v, p);
-  float* mine = sums + warp * p.T * LD;
-  for (int i = lane; i < p.T * LD; i += 32) mine[i] = 0.f;
-  __syncwarp();
-  pdl_sync();
-  const int n_active = *v.n_active;
+  const int units = p.ff / 64, shared_units = p.sff / 64;
+  ml_build<NT == 1 ? 8 * ML_MAX_TOP / ML_THREADS : ML_MAX_ROWS * ML_MAX_TOP / ML_THREADS>(v, p, units, shared_units, true);
+  const int n_active = *v.n_active, total = n_active ? v.line[n_active] : 0;
   const int col0 = block * 32, tile = col0 >> 7;
   const uint8_t* wt = p.down + static_cast<long long>(tile) * p.down_kb * 16384 + (col0 & 127) * 128;
-  const int fkb = p.ff / 64, routed = p.sff > 0 ? n_active - 1 : n_active, line = routed * fkb + p.sff / 64;
   const int share = rank * ML_WARPS + warp, shares = p.cluster * ML_WARPS;
-  const int end = static_cast<int>(static_cast<long long>(line) * (share + 1) / shares);
-  for (int at = static_cast<int>(static_cast<long long>(line) * share / shares); at < end;) {
-    const int a = at < routed * fkb ? at / fkb : routed, e = v.active[a], k0 = at - a * fkb, k1 = min(e < p.E ? fkb : p.sff / 64, k0 + end - at);
-    const uint8_t* wb = wt + static_cast<long long>(e) * fkb * 16384;
-    const int first = v.off[e], n = v.off[e + 1] - first;
-    for (int n0 = 0; n0 < n; n0 += NT * 8) {
-      if (NT > 1 && n - n0 <= 8) ml_down_pass<1>(p, v, wb, mine, first + n0, n - n0, k0, k1, g, t4);
-      else ml_down_pass<NT>(p, v, wb, mine, first + n0, n - n0, k0, k1, g, t4);
+  const int begin = static_cast<int>(static_cast<long long>(total) * share / shares), end = static_cast<int>(static_cast<long long>(total) * (share + 1) / shares);
+  MlWalk start = {};
+  start.at = end;
+  if (begin < end) start = ml_walk(v, begin, p.E, units, shared_units, true);
+  // past a piece: the walk stands at the next expert, or at the end of the part
+  auto past = [&](MlWalk& w, const MlDownPiece& m) {
+    w.at += (m.k1 - m.k0) * w.step;
+    w.unit = m.k1;
+    if (w.unit < w.units) return;
+    w.unit = 0;
+    if (++w.a < n_active) ml_expert(w, v, p.E, units, shared_units);
+  };
+  MlWalk ask_at = start;
+  int ask_pass = 0, ask_kb = 0;
+  MlDownPiece ask_m = {};
+  if (ask_at.at < end) {
+    ask_m = ml_down_piece<NT>(p, v, wt, ask_at, end);
+    ask_kb = ask_m.k0;
+  }
+  auto ask = [&]() {
+    if (ask_at.at >= end) return;
+    if (lane == 0 && !bw.dead) ring.ask(ask_m.w + static_cast<long long>(ask_kb) * 16384);
+    ring.asked();
+    if (++ask_kb < ask_m.k1) return;
+    ask_kb = ask_m.k0;
+    if (++ask_pass < ask_m.passes) return;
+    ask_pass = 0;
+    past(ask_at, ask_m);
+    if (ask_at.at < end) {
+      ask_m = ml_down_piece<NT>(p, v, wt, ask_at, end);
+      ask_kb = ask_m.k0;
     }
-    at += k1 - k0;
+  };
+#pragma unroll
+  for (int i = 0; i < SLOTS; ++i) ask();
+  float* mine = sums + warp * p.T * LD;
+  for (int i = lane; i < p.T * (LD / 4); i += 32) reinterpret_cast<float4*>(mine)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  __syncwarp();
+  pdl_sync();
+  for (MlWalk at = start; at.at < end;) {
+    const MlDownPiece m = ml_down_piece<NT>(p, v, wt, at, end);
+    for (int pass = 0; pass < m.passes; ++pass) {
+      const int n0 = pass * NT * 8, cols = m.n - n0;
+      ml_by_columns<NT>(cols, [&](auto tiles) {
+        constexpr int N = decltype(tiles)::value, HALF = N > 2 ? 2 : N;            // (registers: activations of at most two column tiles at a time)
+        float acc[2][N][4] = {};
+        const __nv_bfloat16* ar[N];
+        ml_rows<N>(ar, p.act + t4 * 8, p.ld_act, v, m.first + n0, cols, g, p, false);
+        uint4 next[HALF][3][2];
+        auto take = [&](int j0, int kb) {
+#pragma unroll
+          for (int j = 0; j < HALF; ++j)
+#pragma unroll
+            for (int part = 0; part < 3; ++part)
+#pragma unroll
+              for (int s = 0; s < 2; ++s) next[j][part][s] = *reinterpret_cast<const uint4*>(ar[j0 + j] + part * p.part_stride + kb * 64 + s * 32);
+        };
+        take(0, m.k0);
+        for (int kb = m.k0; kb < m.k1; ++kb) {
+          uint4 w[4][2];
+#pragma unroll
+          for (int j0 = 0; j0 < N; j0 += HALF) {
+            uint4 x[HALF][3][2];
+#pragma unroll
+            for (int j = 0; j < HALF; ++j)
+#pragma unroll
+              for (int part = 0; part < 3; ++part) { x[j][part][0] = next[j][part][0]; x[j][part][1] = next[j][part][1]; }
+            if (j0 + HALF < N) take(j0 + HALF, kb);
+            else take(0, min(kb + 1, m.k1 - 1));
+            if (j0 == 0) ml_weights(w, ring.wait(bw), r, t4);
+#pragma unroll
+            for (int j = 0; j < HALF; ++j)
+#pragma unroll
+              for (int part = 0; part < 3; ++part)
+#pragma unroll
+                for (int s = 0; s < 2; ++s)
+#pragma unroll
+                  for (int i = 0; i < 2; ++i) {
+                    const uint4 lo = w[2 * i][s], hi = w[2 * i + 1][s];
+                    mma_bf16(acc[i][j0 + j], lo.x, hi.x, lo.y, hi.y, x[j][part][s].x, x[j][part][s].y);
+                    mma_bf16(acc[i][j0 + j], lo.z, hi.z, lo.w, hi.w, x[j][part][s].z, x[j][part][s].w);
+                  }
+          }
+          __syncwarp();
+          ring.read();
+          ask();
+        }
+        // (a row occurs once among an expert's, so no two lanes add to the same place)
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int c = j * 8 + t4 * 2 + h;
+            if (c < cols) {
+              const int t = ml_token(p, v.row[m.first + n0 + c]);
+              float* s = mine + t * LD + r;
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                s[i * 16] += acc[i][j][h];
+                s[i * 16 + 8] += acc[i][j][2 + h];
+              }
+            }
+          }
+        __syncwarp();
+      });
+    }
+    past(at, m);
   }
   __syncthreads();
   // the warps' sums, then the cluster's: each block adds up its share of the rows
-  for (int i = tid; i < p.T * 32; i += ML_THREADS) {
-    const int t = i >> 5, c = i & 31;
-    float s = 0.f;
+  for (int i = tid; i < p.T * 8; i += ML_THREADS) {
+    const int t = i >> 3, c = (i & 7) * 4;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int q = 0; q < ML_WARPS; ++q) s += sums[(q * p.T + t) * LD + c];
-    if (p.cluster > 1) sums[t * LD + c] = s;             // (warp 0's place; read before by this thread alone)
-    else if (col0 + c < p.W) p.y[t * p.ldy + col0 + c] = s;
+    for (int q = 0; q < ML_WARPS; ++q) {
+      const float4 a = *reinterpret_cast<const float4*>(sums + (q * p.T + t) * LD + c);
+      s.x += a.x; s.y += a.y; s.z += a.z; s.w += a.w;
+    }
+    if (p.cluster > 1) *reinterpret_cast<float4*>(sums + t * LD + c) = s;             // (warp 0's place; read before by this thread alone)
+    else ml_result(p, t, col0 + c, s);
   }
   if (p.cluster > 1) {
     cluster_sync_all();
-    for (int i = rank * ML_THREADS + tid; i < p.T * 32; i += p.cluster * ML_THREADS) {
-      const int t = i >> 5, c = i & 31;
-      float s = 0.f;
-      for (int q = 0; q < p.cluster; ++q) s += ld_dsmem_f32(sums + t * LD + c, q);
-      if (col0 + c < p.W) p.y[t * p.ldy + col0 + c] = s;
+    for (int i = rank * ML_THREADS + tid; i < p.T * 8; i += p.cluster * ML_THREADS) {
+      const int t = i >> 3, c = (i & 7) * 4;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int q = 0; q < p.cluster; ++q) {
+        const float4 a = ld_dsmem_f32x4(sums + t * LD + c, q);
+        s.x += a.x; s.y += a.y; s.z += a.z; s.w += a.w;
+      }
+      ml_result(p, t, col0 + c, s);
     }
     cluster_sync_all();                  // (nobody leaves while others read its sums)
   }
@@ -653,11 +915,10 @@ int vb_moe_layer_route(int32_t* d_idx, float* d_wts, float* d_shared_gate, int k
   p.E = experts;
   p.top = top;
   p.kind = kind;
-  p.groups = groups;
+  p.groups = groups > 0 ? groups : 0;
   p.keep = keep;
   p.vocab = vocab;
-  const int all = (kind == ML_TABLE ? 0 : experts) + (d_shared_gate_w ? 1 : 0), per = (all + ML_ROUTE_CLUSTER - 1) / ML_ROUTE_CLUSTER;
-  const size_t smem = (static_cast<size_t>(ML_ROUTE_THREADS / 32 * 16 + per) * ML_ROUTE_CLUSTER + 2 * static_cast<size_t>(experts) + (groups > 1 ? groups : 0)) * 4;
+  const size_t smem = (static_cast<size_t>(ML_ROUTE_THREADS / 32 * 16) * ML_ROUTE_CLUSTER + 2 * static_cast<size_t>(experts) + (groups > 0 ? groups : 0) + 48) * 4;
   VB_LAUNCH_PDL_CLUSTER(moe_layer_route_kernel, (T + ML_ROUTE_CLUSTER - 1) / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER, ML_ROUTE_THREADS, smem, stream, ML_ROUTE_CLUSTER, p);
   return 0;
 }
@@ -696,6 +957,7 @@ int vb_moe_layer_experts(float* d_y, long long ldy, const void* d_h, long long l
   p.W = W;
   p.E = experts;
   p.top = top;
+  p.top_inverse = static_cast<uint32_t>(((1ull << 32) + top - 1) / top);
   p.ff = ff;
   p.sff = shared_ff;
   p.ld_act = ff > shared_ff ? ff : shared_ff;
@@ -709,40 +971,39 @@ int vb_moe_layer_experts(float* d_y, long long ldy, const void* d_h, long long l
   p.slope = slope;
   p.up_units = (gated ? 2 * ff : ff) / 32;
   p.shared_units = (gated ? 2 * shared_ff : shared_ff) / 32;
-  // column tiles a pass: by the rows an expert has on average, so that most experts are read once
-  const int sms = sm_count(), nt = T <= 8 ? 1 : T <= 16 || T * top <= 8 * experts ? 2 : 4;
+  VB_CHECK_ARG(p.wait_flag = wait_flag(WK_MOE_LAYER), "vb_moe_layer_experts: no mapped host memory");
+  const int sms = sm_count();
   const long long most = static_cast<long long>(experts < T * top ? experts : T * top) * p.up_units + p.shared_units;
-  const int fit = (nt == 1 ? 3 : 2) * sms, grid_up = static_cast<int>(most < fit ? most : fit);
+  const int grid_up = static_cast<int>(most < sms ? most : sms), nt = T <= 8 ? 1 : 4;
   const size_t plan_bytes = static_cast<size_t>(ml_plan_words(T, experts, top)) * 4;
-  const size_t smem_up = static_cast<size_t>(2 * ML_WARPS) * 32 * (nt * 8 + (nt > 1 ? 8 : 0)) * 4 + plan_bytes;
-#define ML_UP(NT, G)                                                              \
-  do {                                                                            \
-    VB_CHECK_CUDA(max_dyn_smem_once(moe_up_kernel<NT, G>));                       \
-    VB_LAUNCH_PDL((moe_up_kernel<NT, G>), grid_up, ML_THREADS, smem_up, stream, p); \
+  // Ring places a warp: three where a block of the next kernel can then stand beside (steps of up to 8 rows: it has its first weights before this one ends).
+  constexpr int FEW = 3, MANY = 3;
+  const size_t smem_up = ml_ring_bytes(nt == 1 ? FEW : MANY) + static_cast<size_t>(2 * ML_WARPS) * 32 * (nt == 1 ? 8 : 40) * 4 + plan_bytes;
+#define ML_UP(NT, G, S)                                                              \
+  do {                                                                               \
+    VB_CHECK_CUDA(max_dyn_smem_once(moe_up_kernel<NT, G, S>));                       \
+    VB_LAUNCH_PDL((moe_up_kernel<NT, G, S>), grid_up, ML_THREADS, smem_up, stream, p); \
   } while (0)
   if (gated) {
-    if (nt == 1) ML_UP(1, true);
-    else if (nt == 2) ML_UP(2, true);
-    else ML_UP(4, true);
+    if (nt == 1) ML_UP(1, true, FEW);
+    else ML_UP(4, true, MANY);
   } else {
-    if (nt == 1) ML_UP(1, false);
-    else if (nt == 2) ML_UP(2, false);
-    else ML_UP(4, false);
+    if (nt == 1) ML_UP(1, false, FEW);
+    else ML_UP(4, false, MANY);
   }
 #undef ML_UP
-  const int blocks = (W + 31) / 32;
+  const size_t smem_down = ml_ring_bytes(nt == 1 ? FEW : MANY) + static_cast<size_t>(ML_WARPS) * T * ML_LD * 4 + plan_bytes;
+  const int blocks = (W + 31) / 32, fit = (nt == 1 && smem_down <= 112 * 1024 ? 2 : 1) * sms;
   int cluster = 1;                       // one wave
   while (cluster < 8 && blocks * cluster * 2 <= fit) cluster *= 2;
   p.cluster = cluster;
-  const size_t smem_down = static_cast<size_t>(ML_WARPS) * T * 36 * 4 + plan_bytes;
-#define ML_DOWN(NT)                                                                                                 \
-  do {                                                                                                              \
-    VB_CHECK_CUDA(max_dyn_smem_once(moe_down_kernel<NT>));                                                          \
-    VB_LAUNCH_PDL_CLUSTER(moe_down_kernel<NT>, blocks * cluster, ML_THREADS, smem_down, stream, cluster, p);        \
+#define ML_DOWN(NT, S)                                                                                                  \
+  do {                                                                                                                  \
+    VB_CHECK_CUDA(max_dyn_smem_once(moe_down_kernel<NT, S>));                                                           \
+    VB_LAUNCH_PDL_CLUSTER((moe_down_kernel<NT, S>), blocks * cluster, ML_THREADS, smem_down, stream, cluster, p);       \
   } while (0)
-  if (nt == 1) ML_DOWN(1);
-  else if (nt == 2) ML_DOWN(2);
-  else ML_DOWN(4);
+  if (nt == 1) ML_DOWN(1, FEW);
+  else ML_DOWN(4, MANY);
 #undef ML_DOWN
   return 0;
 }
