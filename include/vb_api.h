@@ -893,22 +893,22 @@ int vb_selective_scan_tiled(void* d_out, int ld_out, float* d_state, float* d_sc
 /* ---- weights that a row brings with it ----------------------------------------------------------------------------------------
  * Low-rank adapters of many requests beside a shared projection (csrc/lora.cu):
  *   out[t][n] = base[t][n] + sum_j B_a[n][j] (scale_a sum_k A_a,s[j][k] x[t][k]),   a = ids[t] (outside 0 .. slots-1: base alone), s = n's slice
- * vb_lora_plan: rows of a step by adapter, once per step for every projection of every layer: d_order int32 [T], d_tiles int4
- *   [1 + vb_lora_max_tiles(T, slots)].  slots 1 .. 1023.
+ * vb_lora_plan: rows of a step by adapter, once per step for every projection of every layer: d_tiles, vb_lora_plan_bytes(T, slots) bytes, 16-byte
+ *   aligned.  slots 1 .. 1023.
  * vb_lora: out and base fp32 (out_f32) or bf16, rows 16-byte aligned; d_base may be NULL (zeros) or d_out.  d_a / d_b: the adapters in the order that
  *   csrc/lora.cu states (ops.LoraBank writes it), rank padded to 16, 32, 64 or 128, d_scale fp32 [slots]; widths: columns of the
  *   1 .. 4 slices (HOST array, multiples of 8).  K a multiple of 8.  Every row 0 .. T-1 of out is written, nothing behind it.
  * vb_lora_gate_up: act[t][i] = silu(g) u (bf16, row-major with ld_act or, xt_rows > 0, tiled) from d_planes fp32 [splits][T][2 * tiles * half], gate and
  *   up rows interleaved as vb_gemm_bf16 mode 1 leaves them, plus both adapters' products (two slices of ff columns). */
-int vb_lora_max_tiles(int T, int slots);
-int vb_lora_plan(int32_t* d_order, void* d_tiles, const int32_t* d_ids, int T, int slots, void* stream);
-size_t vb_lora_workspace_bytes(int T, int K, int slots, int rank, int slices);
+size_t vb_lora_plan_bytes(int T, int slots);
+int vb_lora_plan(void* d_tiles, const int32_t* d_ids, int T, int slots, void* stream);
+size_t vb_lora_workspace_bytes(int T, int slots, int rank, int slices);
 int vb_lora(void* d_out, long long ld_out, const void* d_base, long long ld_base, int out_f32, const void* d_x, long long ldx, const void* d_a,
-            const void* d_b, const float* d_scale, int slots, int rank, const int32_t* widths, int slices, const int32_t* d_order,
-            const void* d_tiles, int T, int K, void* d_ws, size_t ws_bytes, void* stream);
+            const void* d_b, const float* d_scale, int slots, int rank, const int32_t* widths, int slices, const void* d_tiles, int T, int K,
+            void* d_ws, size_t ws_bytes, void* stream);
 int vb_lora_gate_up(void* d_act, long long ld_act, int xt_rows, const float* d_planes, int splits, int half, int ff, const void* d_x, long long ldx,
-                    const void* d_a, const void* d_b, const float* d_scale, int slots, int rank, const int32_t* d_order, const void* d_tiles,
-                    int T, int K, void* d_ws, size_t ws_bytes, void* stream);
+                    const void* d_a, const void* d_b, const float* d_scale, int slots, int rank, const void* d_tiles, int T, int K, void* d_ws,
+                    size_t ws_bytes, void* stream);
 /* A mixture-of-experts layer for at most vb_moe_layer_max_rows() rows (csrc/moe_layer.cu).
  * vb_moe_layer_route: kind 0 softmax over the chosen logits (+ d_bias), 1 sigmoid scores (chosen by score + d_bias within the kept groups, weights over
  *   their sum), 2 softmax over all experts (chosen within the kept groups, weights as they are), 3 d_table[d_ids[t]] (int32 [vocab][top]; weights 1 / top).

@@ -211,11 +211,11 @@ SIGNATURES = {
     "vb_pool_blocks": (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P]),
     "vb_sigmoid_attn": (c_int, [P, c_int, P, P, P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, P, c_int, c_int, c_int, c_int,
                                 c_int, c_int, c_int, c_int, c_float, c_float, c_float, P, C.c_longlong, c_int, c_int, P]),
-    "vb_lora_max_tiles": (c_int, [c_int, c_int]),
-    "vb_lora_plan": (c_int, [P, P, P, c_int, c_int, P]),
-    "vb_lora_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
-    "vb_lora": (c_int, [P, C.c_longlong, P, C.c_longlong, c_int, P, C.c_longlong, P, P, P, c_int, c_int, P, c_int, P, P, c_int, c_int, P, c_size_t, P]),
-    "vb_lora_gate_up": (c_int, [P, C.c_longlong, c_int, P, c_int, c_int, c_int, P, C.c_longlong, P, P, P, c_int, c_int, P, P, c_int, c_int, P, c_size_t, P]),
+    "vb_lora_plan_bytes": (c_size_t, [c_int, c_int]),
+    "vb_lora_plan": (c_int, [P, P, c_int, c_int, P]),
+    "vb_lora_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "vb_lora": (c_int, [P, C.c_longlong, P, C.c_longlong, c_int, P, C.c_longlong, P, P, P, c_int, c_int, P, c_int, P, c_int, c_int, P, c_size_t, P]),
+    "vb_lora_gate_up": (c_int, [P, C.c_longlong, c_int, P, c_int, c_int, c_int, P, C.c_longlong, P, P, P, c_int, c_int, P, c_int, c_int, P, c_size_t, P]),
     "vb_moe_layer_max_rows": (c_int, []),
     "vb_moe_layer_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
     "vb_moe_layer_route": (c_int, [P, P, P, c_int, P, C.c_longlong, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P]),

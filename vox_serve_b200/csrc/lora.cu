@@ -7,9 +7,13 @@
 //   vb_lora           out as fp32 (one more split-K plane of the projection: its consumer sums planes anyway) or as bf16 rows with a base
 //   vb_lora_gate_up   silu(gate) * up from the projection's fp32 planes with both adapters' products added
 //
-// A tile is up to 16 rows (steps of at most 64) or 64 rows of one adapter.  Two launches a call: the first product over pieces of K, its partial
-// sums left as planes; the second adds the planes and walks the columns.  The bank keeps A and B in the order in which lanes take them (one
-// 16-byte load per lane and product step, 512 bytes in a row per warp), so both are streamed once per tile without a detour through shared memory.
+// A tile is up to 16 rows (steps of at most 64) or 64 rows of one adapter.  The bank keeps A and B in the order in which lanes take them (one 16-byte load per
+// lane and product step, 512 bytes in a row per warp).  Three kernels:
+//
+//   few   steps of at most 64 rows whose adapters are small: one launch.  A cluster of eight blocks per tile divides K, adds up v through distributed
+//         shared memory and divides the columns
+//   down  v of any step: a tile x a piece of K a block, the blocks of a tile a cluster that adds up its parts
+//   up    a tile x some columns a block, all that it reads but v on its way before v is there
 //
 // Sums are fp32.  v is not rounded on its way into the second product: it enters as three bf16 parts (exact, rowmma.cuh) where the result is fp32, as
 // two (off by 2^-15 of v at most) where the result is rounded to bf16 anyway.
@@ -20,19 +24,17 @@
 namespace vb {
 
 constexpr int LORA_MAX_SLOTS = 1023;       // (a thread of the planning block each, and one for rows without an adapter)
-constexpr int LORA_MAX_RANK = 128;
 constexpr int LORA_MAX_SLICES = 4;
 constexpr int LORA_THREADS = 256;
 
 // ---- rows by adapter ------------------------------------------------------------------------------------------------------------
-// tiles[0].x = how many; tiles[1 + i] = {adapter or -1, first place in `order`, rows, 0}.  One block: a counting sort in shared memory.  The
+// A record per tile: adapter or -1, first place among the sorted rows, rows (0: no tile), 0, then the rows.  One block: a counting sort in shared memory.  The
 // order of an adapter's rows among themselves may differ from run to run; a row's result does not depend on its place.
-__global__ void __launch_bounds__(1024) lora_plan_kernel(int32_t* __restrict__ order, int4* __restrict__ tiles, const int32_t* __restrict__ ids, int T,
-                                                         int slots, int tile_rows) {
-  __shared__ int cnt[1024], first[1024];
+__global__ void __launch_bounds__(1024) lora_plan_kernel(int32_t* __restrict__ tiles, const int32_t* __restrict__ ids, int T, int slots, int tile_rows, int max_tiles) {
+  __shared__ int cnt[1024], first_tile[1024];
   __shared__ int warp_rows[32], warp_tiles[32];
   pdl_sync();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, stride = 4 + tile_rows;
   cnt[tid] = 0;
   __syncthreads();
   for (int t = tid; t < T; t += 1024) {
@@ -61,33 +63,35 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(int32_t* __restrict__ o
   }
   __syncthreads();
   if (warp > 0) { r += warp_rows[warp - 1]; m += warp_tiles[warp - 1]; }
-  const int row0 = r - rows, tile0 = m - n;
-  first[tid] = row0;
+  const int row0 = r - rows, tile0 = m - n, all = warp_tiles[31];
+  first_tile[tid] = tile0;
   for (int i = 0; i < n; ++i)
-    tiles[1 + tile0 + i] = make_int4(tid < slots ? tid : -1, row0 + i * tile_rows, min(tile_rows, rows - i * tile_rows), 0);
-  if (tid == 1023) tiles[0] = make_int4(m, T, tile_rows, 0);
+    *reinterpret_cast<int4*>(tiles + static_cast<long long>(tile0 + i) * stride) =
+        make_int4(tid < slots ? tid : -1, row0 + i * tile_rows, min(tile_rows, rows - i * tile_rows), 0);
+  for (int i = all + tid; i < max_tiles; i += 1024) *reinterpret_cast<int4*>(tiles + static_cast<long long>(i) * stride) = make_int4(-1, 0, 0, 0);
   __syncthreads();
   cnt[tid] = 0;
   __syncthreads();
   for (int t = tid; t < T; t += 1024) {
     int a = ids[t];
     a = a >= 0 && a < slots ? a : slots;
-    order[first[a] + atomicAdd(&cnt[a], 1)] = t;
+    const int at = atomicAdd(&cnt[a], 1), i = at / tile_rows;
+    tiles[static_cast<long long>(first_tile[a] + i) * stride + 4 + at - i * tile_rows] = t;
   }
 }
 
 struct LoraParams {
-  const int4* tiles;
-  const int32_t* order;
+  const int32_t* tiles;            // records of 4 + tile_rows words
+  int tile_rows;
   const __nv_bfloat16* x;
   long long ldx;
   const uint4 *a, *b;              // [slots][S][rank / 16][K / 32][2][32 lanes], [slots][column blocks of 32][rank / 16][2][32 lanes]
   long long a_slot, b_slot;        // 16-byte units
   const float* scale;
-  float* v;                        // [k_split][T][VR]
-  int T, K, kb32, rank_tiles, VR, k_split;      // VR = S * rank
+  uint32_t* v;                     // [tiles][tile_rows / 16][S][parts][rank / 16][32 lanes][4]: v as the second product takes it
+  int T, K, kb32, rank_tiles, VR, k_split, parts;      // VR = S * rank
   // second product
-  int blocks;                      // column blocks of 32 over all slices
+  int blocks, per_block;           // column blocks of 32 over all slices (of gate | up: of one), and how many a block of threads has
   int slices, block0[LORA_MAX_SLICES + 1], col0[LORA_MAX_SLICES + 1];
   void* out;
   const void* base;
@@ -97,307 +101,529 @@ struct LoraParams {
   int splits, half, width, ff, xt_rows, xt_kb;
 };
 
+// ---- v as the second product's A operand ------------------------------------------------------------------------------------------
+// In the order of the lanes: [m16 block][slice][part][rank tile][32 lanes][4 registers].
+__device__ __forceinline__ void lora_put(uint32_t* frags, int slices, int parts, int ks, int r, int k, float a, float b) {      // row r, v[k] and v[k + 1]
+  const int tile = k >> 4, s = tile / ks, t = tile - s * ks;
+  float h0, m0, l0, h1, m1, l1;
+  bf16_parts(a, h0, m0, l0);
+  bf16_parts(b, h1, m1, l1);
+  uint32_t* at = frags + ((((r >> 4) * slices + s) * parts * ks + t) * 32 + (r & 7) * 4 + (k & 7) / 2) * 4 + (r & 15) / 8 + (k & 15) / 8 * 2;
+  at[0] = pack_cut(h0, h1);
+  at[ks * 128] = pack_cut(m0, m1);
+  if (parts > 2) at[2 * ks * 128] = pack_cut(l0, l1);
+}
+
+// 16 bytes past the registers and L1; zeros where `in` is false (nothing is read then)
+__device__ __forceinline__ void cp_async16(uint32_t to, const void* from, bool in) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
 // ---- first product: v = scale A x -------------------------------------------------------------------------------------------------
-// Block: a tile x a piece of K, the warps taking turns of 64 k; RT rank tiles (16 each) at a time over NT column tiles of 8 rows.  Where rows have
-// more rank tiles than RT the block walks its piece again (x from L2 then).
-template <int NT, int RT>
-__global__ void __launch_bounds__(LORA_THREADS) lora_down_kernel(const LoraParams p) {
-  extern __shared__ float red[];            // [8 warps][16][NT * 8 + 4]
-  constexpr int LD = NT * 8 + 4;
-  __shared__ int rows_s[NT * 8];
-  pdl_sync();
-  const int tile = blockIdx.x;
-  if (tile >= p.tiles[0].x) return;
-  const int4 tl = p.tiles[1 + tile];
-  if (tl.x < 0) return;                     // no adapter: the second kernel does not look at v
+// Block: a tile x a piece of K, in stages of 128 k: 256 bytes of each row of x and RT rank tiles of A, copied 16 bytes at a time with three to five stages on
+// their way.  (Bulk copies of a row's 256 bytes took 79 us where this takes 16: 4096 rows of 8192, rank 64; they start one at a time.)  Rows are 320 bytes apart:
+// lanes 0 to 7 of a 16-byte load read two rows, which then lie in different banks.  Warps: four k blocks of 32 by two halves of the rows.  More than RT rank
+// tiles: x again.  The pieces of a tile are a cluster, which adds them up and leaves v in parts.
+constexpr int LORA_STAGE_K = 128, LORA_ROW_BYTES = 2 * LORA_STAGE_K + 64, LORA_X_BYTES = 64 * LORA_ROW_BYTES, LORA_RED_LD = 36;
+template <int RT>
+struct LoraDown {
+  static constexpr int STAGES = RT == 4 ? 5 : RT == 2 ? 3 : 4, BLOCKS = RT >= 4 ? 1 : 2;
+  static constexpr int STAGE_BYTES = LORA_X_BYTES + RT * 4096;
+  static constexpr size_t SMEM = static_cast<size_t>(STAGES) * STAGE_BYTES;
+  static_assert(8 * RT * 16 * LORA_RED_LD * 4 + 64 * RT * 16 * 4 <= STAGES * STAGE_BYTES, "the sums stand where the stages stood");
+};
+template <int RT>
+__global__ void __launch_bounds__(LORA_THREADS, LoraDown<RT>::BLOCKS) lora_down_kernel(const LoraParams p) {
+  extern __shared__ __align__(128) uint8_t smem8[];
+  constexpr int STAGES = LoraDown<RT>::STAGES, STAGE_BYTES = LoraDown<RT>::STAGE_BYTES, LD = LORA_RED_LD;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-  const int n = tl.z;
-  if (tid < NT * 8) rows_s[tid] = tid < n ? p.order[tl.y + tid] : -1;
-  __syncthreads();
-  const __nv_bfloat16* xr[NT];
+  pdl_sync();
+  const int32_t* rec = p.tiles + static_cast<long long>(blockIdx.x) * (4 + p.tile_rows);
+  const int4 tl = *reinterpret_cast<const int4*>(rec);
+  if (tl.z == 0 || tl.x < 0) return;        // (all blocks of the cluster) no tile; no adapter: the second kernel does not look at v
+  const int n = tl.z, rts = p.VR >> 4;
+  const int stages = (p.K + LORA_STAGE_K - 1) / LORA_STAGE_K, s0 = static_cast<int>(static_cast<long long>(stages) * blockIdx.y / p.k_split),
+            s1 = static_cast<int>(static_cast<long long>(stages) * (blockIdx.y + 1) / p.k_split);
+  // a thread's copies: 16 bytes of four rows, 16 bytes of every rank tile
+  const int chunk = tid & 15, row0 = tid >> 4;
+  const __nv_bfloat16* xr[4];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) {
-    const int row = rows_s[j * 8 + g];
-    xr[j] = row >= 0 ? p.x + row * p.ldx + t4 * 8 : nullptr;
-  }
-  const uint4* a = p.a + tl.x * p.a_slot + lane;
-  // pieces in units of 64 k
-  const int units = (p.kb32 + 1) >> 1, u0 = static_cast<int>(static_cast<long long>(units) * blockIdx.y / p.k_split),
-            u1 = static_cast<int>(static_cast<long long>(units) * (blockIdx.y + 1) / p.k_split);
+  for (int i = 0; i < 4; ++i) xr[i] = row0 + i * 16 < n ? p.x + rec[4 + row0 + i * 16] * p.ldx + chunk * 8 : nullptr;
+  const uint32_t ring = smem_u32(smem8), x_to = ring + row0 * LORA_ROW_BYTES + chunk * 16, a_to = ring + LORA_X_BYTES + tid * 16;
+  const uint4* a = p.a + tl.x * p.a_slot + tid;
   const float scale = p.scale[tl.x];
-  const int rts = p.VR >> 4;
+  const int kq = warp & 3, half = warp >> 2;
+  const int tiles_n = min(4, max(0, (n - half * 32 + 7) >> 3));           // column tiles of 8 rows that this warp has
   for (int rt0 = 0; rt0 < rts; rt0 += RT) {
-    float acc[RT][NT][4];
+    auto load = [&](int s, int slot) {
+      if (s < s1) {
+        const int k = s * LORA_STAGE_K;
+        const bool in = k + chunk * 8 < p.K, in_a = s * 4 + (tid >> 6) < p.kb32;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (xr[i]) cp_async16(x_to + slot * STAGE_BYTES + i * 16 * LORA_ROW_BYTES, in ? xr[i] + k : xr[i], in);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+          if (rt0 + i < rts) cp_async16(a_to + slot * STAGE_BYTES + i * 4096, in_a ? a + (static_cast<long long>(rt0 + i) * p.kb32 + s * 4) * 64 : a, in_a);
+      }
+      cp_async_commit();
+    };
+    float acc[RT][4][4] = {};
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) load(s0 + i, i);
+    int slot = 0;
+    for (int s = s0; s < s1; ++s) {
+      cp_async_wait<STAGES - 2>();
+      __syncthreads();
+      load(s + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
+      const uint8_t* st = smem8 + slot * STAGE_BYTES;
+      uint4 av[RT][2];
+#pragma unroll
+      for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) av[i][h] = *reinterpret_cast<const uint4*>(st + LORA_X_BYTES + i * 4096 + ((kq * 2 + h) * 32 + lane) * 16);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (j >= tiles_n) break;
+        const uint4 x = *reinterpret_cast<const uint4*>(st + (half * 32 + j * 8 + g) * LORA_ROW_BYTES + kq * 64 + t4 * 16);
+#pragma unroll
+        for (int i = 0; i < RT; ++i)
+          if (rt0 + i < rts) {
+            mma_bf16(acc[i][j], av[i][0].x, av[i][0].y, av[i][0].z, av[i][0].w, x.x, x.y);
+            mma_bf16(acc[i][j], av[i][1].x, av[i][1].y, av[i][1].z, av[i][1].w, x.z, x.w);
+          }
+      }
+      slot = slot + 1 == STAGES ? 0 : slot + 1;
+    }
+    cp_async_wait<0>();
+    __syncthreads();
+    float* red = reinterpret_cast<float*>(smem8);                  // [8 warps][RT * 16][LD]
+    float* mine = red + 8 * RT * 16 * LD;                          // [64 rows][RT * 16]
 #pragma unroll
     for (int i = 0; i < RT; ++i)
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) acc[i][j][c] = 0.f;
-    for (int u = u0 + warp; u < u1; u += LORA_THREADS / 32) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int kb = 2 * u + h;
-        if (kb >= p.kb32) break;
-        const bool in = kb * 32 + t4 * 8 < p.K;
-        uint4 xv[NT], av[RT][2];
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-#pragma unroll
-          for (int s = 0; s < 2; ++s)
-            av[i][s] = rt0 + i < rts ? __ldg(a + ((static_cast<long long>(rt0 + i) * p.kb32 + kb) * 2 + s) * 32) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-          xv[j] = in && xr[j] ? *reinterpret_cast<const uint4*>(xr[j] + kb * 32) : make_uint4(0u, 0u, 0u, 0u);
-#pragma unroll
-        for (int j = 0; j < NT; ++j) {
-          if (j > 0 && j * 8 >= n) break;
-#pragma unroll
-          for (int i = 0; i < RT; ++i) {
-            mma_bf16(acc[i][j], av[i][0].x, av[i][0].y, av[i][0].z, av[i][0].w, xv[j].x, xv[j].y);
-            mma_bf16(acc[i][j], av[i][1].x, av[i][1].y, av[i][1].z, av[i][1].w, xv[j].z, xv[j].w);
-          }
-        }
+      for (int j = 0; j < 4; ++j) {
+        float* w = red + (warp * RT + i) * 16 * LD + j * 8 + t4 * 2;
+        *reinterpret_cast<float2*>(w + g * LD) = make_float2(acc[i][j][0], acc[i][j][1]);
+        *reinterpret_cast<float2*>(w + (g + 8) * LD) = make_float2(acc[i][j][2], acc[i][j][3]);
       }
+    __syncthreads();
+    const int ranks = min(RT, rts - rt0) * 16;
+    for (int e = tid; e < n * ranks; e += LORA_THREADS) {
+      const int c = e / ranks, r = e - c * ranks;
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) s += red[(((c >> 5) * 4 + q) * RT * 16 + r) * LD + (c & 31)];
+      mine[c * RT * 16 + r] = scale * s;
     }
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      if (rt0 + i >= rts) break;
-      __syncthreads();
-      float* w = red + warp * 16 * LD;
-#pragma unroll
-      for (int j = 0; j < NT; ++j) {
-        *reinterpret_cast<float2*>(w + g * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][0], acc[i][j][1]);
-        *reinterpret_cast<float2*>(w + (g + 8) * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][2], acc[i][j][3]);
+    if (p.k_split > 1) cluster_sync_all();
+    else __syncthreads();
+    uint32_t* v = p.v + static_cast<long long>(blockIdx.x) * (p.tile_rows >> 4) * rts * p.parts * 128;
+    for (int e = blockIdx.y * LORA_THREADS + tid; e < n * (ranks >> 1); e += p.k_split * LORA_THREADS) {
+      const int c = e / (ranks >> 1), r = (e - c * (ranks >> 1)) * 2;
+      float s = 0.f, t = 0.f;
+      for (int z = 0; z < p.k_split; ++z) {
+        const float* from = mine + c * RT * 16 + r;
+        s += p.k_split > 1 ? ld_dsmem_f32(from, z) : from[0];
+        t += p.k_split > 1 ? ld_dsmem_f32(from + 1, z) : from[1];
       }
-      __syncthreads();
-      for (int e = tid; e < 16 * NT * 8; e += LORA_THREADS) {
-        const int r = e & 15, c = e >> 4;
-        if (c >= n) break;
-        float s = 0.f;
-#pragma unroll
-        for (int q = 0; q < LORA_THREADS / 32; ++q) s += red[(q * 16 + r) * LD + c];
-        p.v[(static_cast<long long>(blockIdx.y) * p.T + tl.y + c) * p.VR + (rt0 + i) * 16 + r] = scale * s;
-      }
+      lora_put(v, p.slices, p.parts, p.rank_tiles, c, rt0 * 16 + r, s, t);
     }
+    if (p.k_split > 1) cluster_sync_all();                         // (others' parts have been read: the next stages may come, or the block may leave)
+    else __syncthreads();
   }
 }
 
 // ---- second product ---------------------------------------------------------------------------------------------------------------
-// The rows of a tile's m16 block as the A operand, all rank tiles of a slice: PARTS parts of v, read from shared memory (fp32, rows of LDV).
 template <int KS, int PARTS>
-__device__ __forceinline__ void lora_rows(uint32_t (&f)[PARTS][KS][4], const float* v, int ldv, int g, int t4) {
-#pragma unroll
-  for (int k = 0; k < KS; ++k)
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const float2 w = *reinterpret_cast<const float2*>(v + (g + (q & 1) * 8) * ldv + k * 16 + t4 * 2 + (q >> 1) * 8);
-      float h0, m0, l0, h1, m1, l1;
-      bf16_parts(w.x, h0, m0, l0);
-      bf16_parts(w.y, h1, m1, l1);
-      f[0][k][q] = pack_cut(h0, h1);
-      if constexpr (PARTS > 1) f[1][k][q] = pack_cut(m0, m1);
-      if constexpr (PARTS > 2) f[2][k][q] = pack_cut(l0, l1);
-    }
-}
-template <int KS, int PARTS>
-__device__ __forceinline__ void lora_block(float (&d)[4][4], const uint32_t (&f)[PARTS][KS][4], const uint4* __restrict__ b) {
-  uint4 w[KS][2];
-#pragma unroll
-  for (int k = 0; k < KS; ++k) {
-    w[k][0] = __ldg(b + k * 64);
-    w[k][1] = __ldg(b + k * 64 + 32);
-  }
+__device__ __forceinline__ void lora_block(float (&d)[4][4], const uint4* frags, const uint4 (&w)[KS][2]) {
 #pragma unroll
   for (int k = 0; k < KS; ++k)
 #pragma unroll
     for (int q = 0; q < PARTS; ++q) {
-      mma_bf16(d[0], f[q][k][0], f[q][k][1], f[q][k][2], f[q][k][3], w[k][0].x, w[k][0].y);
-      mma_bf16(d[1], f[q][k][0], f[q][k][1], f[q][k][2], f[q][k][3], w[k][0].z, w[k][0].w);
-      mma_bf16(d[2], f[q][k][0], f[q][k][1], f[q][k][2], f[q][k][3], w[k][1].x, w[k][1].y);
-      mma_bf16(d[3], f[q][k][0], f[q][k][1], f[q][k][2], f[q][k][3], w[k][1].z, w[k][1].w);
+      const uint4 f = frags[(q * KS + k) * 32];
+      mma_bf16(d[0], f.x, f.y, f.z, f.w, w[k][0].x, w[k][0].y);
+      mma_bf16(d[1], f.x, f.y, f.z, f.w, w[k][0].z, w[k][0].w);
+      mma_bf16(d[2], f.x, f.y, f.z, f.w, w[k][1].x, w[k][1].y);
+      mma_bf16(d[3], f.x, f.y, f.z, f.w, w[k][1].z, w[k][1].w);
     }
+}
+// a column block's part of B: from the bank, or from shared memory
+template <int KS, bool BANK>
+__device__ __forceinline__ void lora_take(uint4 (&w)[KS][2], const uint4* b) {
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    w[k][0] = BANK ? __ldg(b + k * 64) : b[k * 64];
+    w[k][1] = BANK ? __ldg(b + k * 64 + 32) : b[k * 64 + 32];
+  }
 }
 
 enum LoraOut { LORA_F32 = 0, LORA_BF16 = 1, LORA_GLU = 2 };
+__device__ __forceinline__ void lora_add4(float* y, const float4& w) { y[0] += w.x; y[1] += w.y; y[2] += w.z; y[3] += w.w; }
+__device__ __forceinline__ void lora_add8(float* y, const uint4& w) {
+  y[0] += bf16_lo(w.x); y[1] += bf16_hi(w.x); y[2] += bf16_lo(w.y); y[3] += bf16_hi(w.y);
+  y[4] += bf16_lo(w.z); y[5] += bf16_hi(w.z); y[6] += bf16_lo(w.w); y[7] += bf16_hi(w.w);
+}
+__device__ __forceinline__ uint4 lora_round(const float* y) {
+  return make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+}
 
-// sums of the planes of v of a tile into shared memory; rows behind the tile's last as zeros
-__device__ __forceinline__ void lora_sum_v(float* vs, int ldv, const LoraParams& p, const int4& tl, int m_tiles) {
-  const int quads = p.VR >> 2;
-  for (int e = threadIdx.x; e < m_tiles * 16 * quads; e += LORA_THREADS) {
-    const int r = e / quads, q = e - r * quads;
-    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (r < tl.z) {
-      const float* src = p.v + (static_cast<long long>(tl.y) + r) * p.VR + q * 4;
-      for (int z = 0; z < p.k_split; ++z) {
-        const float4 w = *reinterpret_cast<const float4*>(src + static_cast<long long>(z) * p.T * p.VR);
-        s.x += w.x; s.y += w.y; s.z += w.z; s.w += w.w;
+// Results of a lane: eight neighbouring columns of row `row`.  y: the products; base, planes: what is added (nullptr: nothing), the gate's and the up's columns 16 apart.
+template <int OUT>
+__device__ __forceinline__ void lora_result(const LoraParams& p, long long row, int col, float (&y)[8], const void* base) {
+  if constexpr (OUT == LORA_F32) {
+    if (base) {
+      lora_add4(y, static_cast<const float4*>(base)[0]);
+      lora_add4(y + 4, static_cast<const float4*>(base)[1]);
+    }
+    float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.ldo + col);
+    o[0] = make_float4(y[0], y[1], y[2], y[3]);
+    o[1] = make_float4(y[4], y[5], y[6], y[7]);
+  } else {
+    if (base) lora_add8(y, *static_cast<const uint4*>(base));
+    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + col) = lora_round(y);
+  }
+}
+__device__ __forceinline__ void lora_gated(const LoraParams& p, long long row, int col, float (&gv)[8], float (&uv)[8], const float* first) {
+  lora_add4(gv, *reinterpret_cast<const float4*>(first));
+  lora_add4(gv + 4, *reinterpret_cast<const float4*>(first + 4));
+  lora_add4(uv, *reinterpret_cast<const float4*>(first + 16));
+  lora_add4(uv + 4, *reinterpret_cast<const float4*>(first + 20));
+  for (int z = 1; z < p.splits; ++z) {
+    const float* more = p.planes + (static_cast<long long>(z) * p.T + row) * p.width + (col >> 4) * 32 + (col & 15);
+    lora_add4(gv, *reinterpret_cast<const float4*>(more));
+    lora_add4(gv + 4, *reinterpret_cast<const float4*>(more + 4));
+    lora_add4(uv, *reinterpret_cast<const float4*>(more + 16));
+    lora_add4(uv + 4, *reinterpret_cast<const float4*>(more + 20));
+  }
+  float y[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) y[i] = gv[i] / (1.f + expf(-gv[i])) * uv[i];
+  const long long to = p.xt_rows ? static_cast<long long>(xt_index(static_cast<int>(row), col, p.xt_rows, p.xt_kb)) : row * p.ldo + col;
+  *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + to) = lora_round(y);
+}
+template <int OUT>
+__host__ __device__ constexpr int lora_parts() { return OUT == LORA_F32 ? 3 : 2; }
+
+// Block: a tile x per_block column blocks.  All but v is older than the first product and on its way into shared memory before that ends: the block's part of B, and
+// its rows' part of the base or of the planes.  The warps stand ceil(rows / 16) deep along the rows and divide the columns.
+template <int OUT>
+__host__ __device__ constexpr int lora_row_bytes() { return OUT == LORA_GLU ? 256 : OUT == LORA_F32 ? 128 : 64; }      // of a column block in base or planes
+template <int KS, int OUT>
+__global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_kernel(const LoraParams p) {
+  extern __shared__ __align__(128) uint8_t smem8[];
+  constexpr int PARTS = lora_parts<OUT>(), B_BYTES = KS * 1024 * (OUT == LORA_GLU ? 2 : 1), SEG = lora_row_bytes<OUT>();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+  const int32_t* rec = p.tiles + static_cast<long long>(blockIdx.x) * (4 + p.tile_rows);
+  const int4 tl = *reinterpret_cast<const int4*>(rec);
+  const int n = tl.z, need = (n + 15) >> 4, c0 = blockIdx.y * p.per_block, c1 = min(p.blocks, c0 + p.per_block), nb = c1 - c0;
+  const bool has = tl.x >= 0;
+  if (n == 0) {
+    pdl_sync();
+    return;
+  }
+  // shared memory: v [m16 blocks][slices][PARTS][KS] of 512 bytes, B, rows of base or planes
+  const int v_bytes = need * p.slices * PARTS * KS * 512, ld_rows = p.per_block * SEG + 16;
+  uint8_t* bs = smem8 + (p.tile_rows >> 4) * p.slices * PARTS * KS * 512;
+  uint8_t* rows = bs + p.per_block * B_BYTES;
+  if (has) {
+    const uint4* b = p.b + tl.x * p.b_slot + static_cast<long long>(c0) * KS * 64;
+    const int half = nb * KS * 64;
+    for (int i = tid; i < half; i += LORA_THREADS) {
+      cp_async16(smem_u32(bs) + i * 16, b + i, true);
+      if (OUT == LORA_GLU) cp_async16(smem_u32(bs) + (half + i) * 16, b + static_cast<long long>(p.blocks) * KS * 64 + i, true);       // (the up columns' blocks follow the gate's)
+    }
+  }
+  // (base and planes: columns of a block are neighbours, but blocks of different slices may not be)
+  if (OUT == LORA_GLU || p.base) {
+    constexpr int PER = SEG / 16;
+    for (int i = tid; i < n * nb * PER; i += LORA_THREADS) {
+      const int r = i / (nb * PER), k = i - r * nb * PER, c = c0 + k / PER, q = k % PER;
+      const long long row = rec[4 + r];
+      if constexpr (OUT == LORA_GLU) {
+        const bool in = c * 64 + q * 4 < 2 * ((p.ff + 15) & ~15);
+        cp_async16(smem_u32(rows) + r * ld_rows + k * 16, p.planes + row * p.width + (in ? c * 64 + q * 4 : 0), in);
+      } else {
+        int s = 0;
+        while (c >= p.block0[s + 1]) ++s;
+        const int col = p.col0[s] + (c - p.block0[s]) * 32 + q * (OUT == LORA_F32 ? 4 : 8);
+        const bool in = col < p.col0[s + 1];
+        cp_async16(smem_u32(rows) + r * ld_rows + k * 16, static_cast<const uint8_t*>(p.base) + (row * p.ld_base + (in ? col : 0)) * (OUT == LORA_F32 ? 4 : 2), in);
       }
     }
-    *reinterpret_cast<float4*>(vs + r * ldv + q * 4) = s;
+  }
+  const int m_tiles = need == 3 ? 4 : need, mt = warp & (m_tiles - 1), step = 8 / m_tiles;
+  const int ra = mt * 16 + g, rb = ra + 8;
+  const long long row_a = ra < n ? rec[4 + ra] : -1, row_b = rb < n ? rec[4 + rb] : -1;
+  pdl_sync();
+  if (has) {
+    const uint4* v = reinterpret_cast<const uint4*>(p.v) + static_cast<long long>(blockIdx.x) * (p.tile_rows >> 4) * p.slices * PARTS * KS * 32;
+    for (int i = tid; i < v_bytes / 16; i += LORA_THREADS) cp_async16(smem_u32(smem8) + i * 16, v + i, true);
+  }
+  cp_async_commit();
+  cp_async_wait<0>();
+  __syncthreads();
+  if (mt >= need) return;
+  const uint4* frags = reinterpret_cast<const uint4*>(smem8) + mt * p.slices * PARTS * KS * 32 + lane;
+  const uint4* bw = reinterpret_cast<const uint4*>(bs) + lane;
+  for (int c = c0 + warp / m_tiles; c < c1; c += step) {
+    int s = 0;
+    while (OUT != LORA_GLU && c >= p.block0[s + 1]) ++s;
+    float d[4][4] = {}, u[4][4] = {};
+    if (has) {
+      uint4 w[KS][2];
+      lora_take<KS, false>(w, bw + (c - c0) * KS * 64);
+      lora_block<KS, PARTS>(d, frags + s * PARTS * KS * 32, w);
+      if constexpr (OUT == LORA_GLU) {
+        lora_take<KS, false>(w, bw + (nb + c - c0) * KS * 64);
+        lora_block<KS, PARTS>(u, frags + PARTS * KS * 32, w);
+      }
+    }
+    const int col = p.col0[s] + (c - p.block0[s]) * 32 + t4 * 8;
+    if (col >= p.col0[s + 1]) continue;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long long row = h ? row_b : row_a;
+      if (row < 0) continue;
+      const uint8_t* from = rows + (h ? rb : ra) * ld_rows + (c - c0) * SEG;
+      float y[8], z[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[i] = d[i >> 1][h * 2 + (i & 1)];
+        z[i] = u[i >> 1][h * 2 + (i & 1)];
+      }
+      if constexpr (OUT == LORA_GLU) lora_gated(p, row, col, y, z, reinterpret_cast<const float*>(from) + (t4 >> 1) * 32 + (t4 & 1) * 8);
+      else lora_result<OUT>(p, row, col, y, p.base ? from + t4 * (SEG / 4) : nullptr);
+    }
   }
 }
 
-// Block: a tile x a range of column blocks (32 columns each).  The warps stand ceil(rows / 16) deep along the rows and divide the columns.
-template <int KS, int OUT>
-__global__ void __launch_bounds__(LORA_THREADS) lora_up_kernel(const LoraParams p) {
-  constexpr int PARTS = OUT == LORA_F32 ? 3 : 2;
-  extern __shared__ float vs[];             // [rows][VR + 4]
+// ---- both, for few rows -------------------------------------------------------------------------------------------------------------
+// A cluster of eight blocks per tile of up to 16 rows.  RT: rank tiles a pass over the block's share of K.
+constexpr int LORA_CLUSTER = 8, LORA_FEW_RANKS = 128;
+template <int KS, int OUT, int RT>
+__global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams p) {
+  extern __shared__ __align__(16) float sm[];
+  constexpr int LD = 20;
+  float* red = sm;                                   // [8 warps][16][LD]
+  float* mine = red + 8 * 16 * LD;                   // [16 rows][VR]: this block's part of v
+  uint32_t* frags = reinterpret_cast<uint32_t*>(mine + 16 * p.VR);      // the sum, as parts
+  constexpr int PARTS = lora_parts<OUT>();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-  // (the plan is older than the first product, whose results are all that has to be waited for)
-  const int tile = blockIdx.x;
-  const bool mine = tile < p.tiles[0].x;
-  int4 tl = make_int4(-1, 0, 0, 0);
-  if (mine) tl = p.tiles[1 + tile];
-  const int ldv = p.VR + 4;
+  const int rank = blockIdx.x % LORA_CLUSTER;
   pdl_sync();
-  if (!mine) return;
-  const int need = (tl.z + 15) >> 4, m_tiles = need == 3 ? 4 : need;
+  const int32_t* rec = p.tiles + (blockIdx.x / LORA_CLUSTER) * (4 + 16);
+  const int4 tl = *reinterpret_cast<const int4*>(rec);
+  const int row_a = rec[4 + g], row_b = rec[12 + g]; // (places behind the tile's last hold anything)
+  const int n = tl.z;
+  if (n == 0) return;                                // (all blocks of the cluster)
   const bool has = tl.x >= 0;
-  if (has) {
-    lora_sum_v(vs, ldv, p, tl, need);
-    __syncthreads();
-  }
-  const int mt = warp & (m_tiles - 1), lanes_n = 8 / m_tiles, wn = warp / m_tiles;
-  if (mt >= need) return;
-  const int ra = mt * 16 + g, rb = ra + 8;
-  const long long row_a = ra < tl.z ? p.order[tl.y + ra] : -1, row_b = rb < tl.z ? p.order[tl.y + rb] : -1;
-  const int c0 = static_cast<int>(static_cast<long long>(p.blocks) * blockIdx.y / gridDim.y),
-            c1 = static_cast<int>(static_cast<long long>(p.blocks) * (blockIdx.y + 1) / gridDim.y);
+  const int c1 = static_cast<int>(static_cast<long long>(p.blocks) * (rank + 1) / LORA_CLUSTER), first = static_cast<int>(static_cast<long long>(p.blocks) * rank / LORA_CLUSTER) + warp;
   const uint4* b = p.b + (has ? tl.x : 0) * p.b_slot + lane;
-  if constexpr (OUT == LORA_GLU) {
-    // the up columns' blocks follow the gate's
-    uint32_t fg[PARTS][KS][4], fu[PARTS][KS][4];
-    if (has) {
-      lora_rows<KS, PARTS>(fg, vs + mt * 16 * ldv, ldv, g, t4);
-      lora_rows<KS, PARTS>(fu, vs + mt * 16 * ldv + KS * 16, ldv, g, t4);
-    }
-    for (int c = c0 + wn; c < c1; c += lanes_n) {
-      const int col = c * 32 + t4 * 8;
-      float dg[4][4] = {}, du[4][4] = {};
-      if (has) {
-        lora_block<KS, PARTS>(dg, fg, b + static_cast<long long>(c) * KS * 64);
-        lora_block<KS, PARTS>(du, fu, b + static_cast<long long>(p.blocks + c) * KS * 64);
-      }
-      if (col >= p.ff) continue;
-      const int it = col / p.half, j = col - it * p.half;
-      const long long at = static_cast<long long>(it) * 2 * p.half + (j >> 4) * 32 + (j & 15);
+  const long long rows[2] = {g < n ? row_a : -1, g + 8 < n ? row_b : -1};
+  uint4 w[KS][2];
+  if (has) {
+    const uint4* a = p.a + tl.x * p.a_slot + lane;
+    const float scale = p.scale[tl.x];
+    const int rts = p.VR >> 4, k0 = static_cast<int>(static_cast<long long>(p.kb32) * rank / LORA_CLUSTER), k1 = static_cast<int>(static_cast<long long>(p.kb32) * (rank + 1) / LORA_CLUSTER);
+    const __nv_bfloat16 *xa = p.x + (g < n ? row_a : 0) * p.ldx + t4 * 8, *xb = p.x + (g + 8 < n ? row_b : 0) * p.ldx + t4 * 8;
+    for (int rt0 = 0; rt0 < rts; rt0 += RT) {
+      float acc[RT][2][4] = {};
+      for (int kb = k0 + warp; kb < k1; kb += 16) {
+        // two blocks of 32 k at a time
+        uint4 av[2][RT][2], xv[2][2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const long long row = h ? row_b : row_a;
-        if (row < 0) continue;
-        float gv[8], uv[8];
+        for (int u = 0; u < 2; ++u) {
+          const int k = kb + u * 8;
+          const bool in = k < k1 && k * 32 + t4 * 8 < p.K;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          gv[i] = dg[i >> 1][h * 2 + (i & 1)];
-          uv[i] = du[i >> 1][h * 2 + (i & 1)];
+          for (int i = 0; i < RT; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+              av[u][i][h] = rt0 + i < rts && k < k1 ? ldg_stream(a + ((static_cast<long long>(rt0 + i) * p.kb32 + k) * 2 + h) * 32) : make_uint4(0u, 0u, 0u, 0u);
+          xv[u][0] = in ? *reinterpret_cast<const uint4*>(xa + k * 32) : make_uint4(0u, 0u, 0u, 0u);
+          xv[u][1] = in && n > 8 ? *reinterpret_cast<const uint4*>(xb + k * 32) : make_uint4(0u, 0u, 0u, 0u);
         }
-        for (int z = 0; z < p.splits; ++z) {
-          const float* pl = p.planes + (static_cast<long long>(z) * p.T + row) * p.width + at;
 #pragma unroll
-          for (int q = 0; q < 2; ++q) {
-            const float4 a4 = *reinterpret_cast<const float4*>(pl + q * 4), b4 = *reinterpret_cast<const float4*>(pl + 16 + q * 4);
-            gv[q * 4] += a4.x; gv[q * 4 + 1] += a4.y; gv[q * 4 + 2] += a4.z; gv[q * 4 + 3] += a4.w;
-            uv[q * 4] += b4.x; uv[q * 4 + 1] += b4.y; uv[q * 4 + 2] += b4.z; uv[q * 4 + 3] += b4.w;
-          }
-        }
-        float y[8];
+        for (int u = 0; u < 2; ++u)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = gv[i] / (1.f + expf(-gv[i])) * uv[i];
-        const uint4 o = make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
-        __nv_bfloat16* out = static_cast<__nv_bfloat16*>(p.out);
-        const long long to = p.xt_rows ? static_cast<long long>(xt_index(static_cast<int>(row), col, p.xt_rows, p.xt_kb)) : row * p.ldo + col;
-        *reinterpret_cast<uint4*>(out + to) = o;
-      }
-    }
-  } else {
-    uint32_t f[PARTS][KS][4];
-    int slice = -1;
-    for (int c = c0 + wn; c < c1; c += lanes_n) {
-      int s = slice < 0 ? 0 : slice;
-      while (c >= p.block0[s + 1]) ++s;
-      if (s != slice) {
-        slice = s;
-        if (has) lora_rows<KS, PARTS>(f, vs + mt * 16 * ldv + s * KS * 16, ldv, g, t4);
-      }
-      const int col = p.col0[s] + (c - p.block0[s]) * 32 + t4 * 8;
-      float d[4][4] = {};
-      if (has) lora_block<KS, PARTS>(d, f, b + static_cast<long long>(c) * KS * 64);
-      if (col >= p.col0[s + 1]) continue;
+          for (int j = 0; j < 2; ++j) {
+            if (j > 0 && n <= 8) break;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const long long row = h ? row_b : row_a;
-        if (row < 0) continue;
-        float y[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] = d[i >> 1][h * 2 + (i & 1)];
-        if constexpr (OUT == LORA_F32) {
-          if (p.base) {
-            const float* s4 = static_cast<const float*>(p.base) + row * p.ld_base + col;
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-              const float4 w = *reinterpret_cast<const float4*>(s4 + q * 4);
-              y[q * 4] += w.x; y[q * 4 + 1] += w.y; y[q * 4 + 2] += w.z; y[q * 4 + 3] += w.w;
+            for (int i = 0; i < RT; ++i) {
+              mma_bf16(acc[i][j], av[u][i][0].x, av[u][i][0].y, av[u][i][0].z, av[u][i][0].w, xv[u][j].x, xv[u][j].y);
+              mma_bf16(acc[i][j], av[u][i][1].x, av[u][i][1].y, av[u][i][1].z, av[u][i][1].w, xv[u][j].z, xv[u][j].w);
             }
           }
-          float* o = static_cast<float*>(p.out) + row * p.ldo + col;
-          *reinterpret_cast<float4*>(o) = make_float4(y[0], y[1], y[2], y[3]);
-          *reinterpret_cast<float4*>(o + 4) = make_float4(y[4], y[5], y[6], y[7]);
-        } else {
-          if (p.base) {
-            const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.base) + row * p.ld_base + col);
-            y[0] += bf16_lo(w.x); y[1] += bf16_hi(w.x); y[2] += bf16_lo(w.y); y[3] += bf16_hi(w.y);
-            y[4] += bf16_lo(w.z); y[5] += bf16_hi(w.z); y[6] += bf16_lo(w.w); y[7] += bf16_hi(w.w);
-          }
-          *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + col) =
-              make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
+      }
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        if (rt0 + i >= rts) break;
+        __syncthreads();
+        float* w = red + warp * 16 * LD;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          *reinterpret_cast<float2*>(w + g * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][0], acc[i][j][1]);
+          *reinterpret_cast<float2*>(w + (g + 8) * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][2], acc[i][j][3]);
         }
+        __syncthreads();
+        const int r = tid & 15, c = tid >> 4;
+        float s = 0.f;
+#pragma unroll
+        for (int q = 0; q < 8; ++q) s += red[(q * 16 + r) * LD + c];
+        mine[c * p.VR + (rt0 + i) * 16 + r] = c < n ? scale * s : 0.f;
       }
     }
+    if (first < c1) lora_take<KS, true>(w, b + static_cast<long long>(first) * KS * 64);         // (on its way while the cluster meets)
+    cluster_sync_all();
+    const int quads = p.VR >> 2;
+    for (int e = tid; e < 16 * quads; e += LORA_THREADS) {
+      const int r = e / quads, q = e - r * quads;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int z = 0; z < LORA_CLUSTER; ++z) {
+        const float4 w = ld_dsmem_f32x4(mine + r * p.VR + q * 4, z);
+        s.x += w.x; s.y += w.y; s.z += w.z; s.w += w.w;
+      }
+      lora_put(frags, p.slices, PARTS, KS, r, q * 4, s.x, s.y);
+      lora_put(frags, p.slices, PARTS, KS, r, q * 4 + 2, s.z, s.w);
+    }
+    __syncthreads();
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
+  const uint4* fr = reinterpret_cast<const uint4*>(frags) + lane;
+  for (int c = first, s = 0; c < c1; c += 8) {
+    while (OUT != LORA_GLU && c >= p.block0[s + 1]) ++s;
+    const int col = p.col0[s] + (c - p.block0[s]) * 32 + t4 * 8;
+    const bool in = col < p.col0[s + 1];
+    // base or planes first: they come from farther away than B
+    float4 add[2][OUT == LORA_GLU ? 6 : 2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+      if (in && rows[h] >= 0) {
+        if constexpr (OUT == LORA_GLU) {
+          const float4* pl = reinterpret_cast<const float4*>(p.planes + rows[h] * p.width + (col >> 4) * 32 + (col & 15));
+          add[h][0] = pl[0];
+          add[h][1] = pl[1];
+          add[h][4] = pl[4];
+          add[h][5] = pl[5];
+        } else if (p.base) {
+          const float4* from = reinterpret_cast<const float4*>(static_cast<const uint8_t*>(p.base) + (rows[h] * p.ld_base + col) * (OUT == LORA_F32 ? 4 : 2));
+          add[h][0] = from[0];
+          if (OUT == LORA_F32) add[h][1] = from[1];
+        }
+      }
+    float d[4][4] = {}, u[4][4] = {};
+    if (has) {
+      lora_block<KS, PARTS>(d, fr + s * PARTS * KS * 32, w);
+      if constexpr (OUT == LORA_GLU) {
+        lora_take<KS, true>(w, b + static_cast<long long>(p.blocks + c) * KS * 64);
+        lora_block<KS, PARTS>(u, fr + PARTS * KS * 32, w);
+      }
+      if (c + 8 < c1) lora_take<KS, true>(w, b + static_cast<long long>(c + 8) * KS * 64);
+    }
+    if (!in) continue;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (rows[h] < 0) continue;
+      float y[8], z[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        y[i] = d[i >> 1][h * 2 + (i & 1)];
+        z[i] = u[i >> 1][h * 2 + (i & 1)];
+      }
+      if constexpr (OUT == LORA_GLU) lora_gated(p, rows[h], col, y, z, reinterpret_cast<const float*>(&add[h][0]));
+      else lora_result<OUT>(p, rows[h], col, y, p.base ? static_cast<const void*>(&add[h][0]) : nullptr);
+    }
+  }
+  __syncwarp();
+  if (has) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");       // (nobody leaves while others read its part)
 }
 
-// how many tiles a step can have at most, and about how many it has (adapters of prompts are few)
+// ---- host -------------------------------------------------------------------------------------------------------------------------
 static int lora_tile_rows(int T) { return T <= 64 ? 16 : 64; }
-static int lora_max_tiles(int T, int slots) {
-  const int tr = lora_tile_rows(T);
-  return T / tr + (T < slots + 1 ? T : slots + 1);
+// the most tiles a step can have
+static int lora_max_tiles(int T, int slots) { return T / lora_tile_rows(T) + (T < slots + 1 ? T : slots + 1); }
+// ... and about how many it has (prompts bring few adapters)
+static int lora_tiles(int T, int slots) {
+  const int adapters = T < slots + 1 ? T : slots + 1;
+  return T <= 64 ? adapters : (T + 63) / 64 + (adapters > 16 ? 8 : adapters / 2);
 }
-static int lora_k_split(int T, int K, int slots) {
-  const int tr = lora_tile_rows(T), units = (K + 63) / 64;
-  const int tiles = T <= 64 ? (T < slots + 1 ? T : slots + 1) : (T + tr - 1) / tr;
-  int split = (2 * 148 + tiles - 1) / tiles;                 // two blocks an SM
-  const int most = units / 8 > 1 ? units / 8 : 1;            // a turn for each of the eight warps
+static int lora_k_split(int T, int K, int slots, int VR) {
+  const int stages = (K + LORA_STAGE_K - 1) / LORA_STAGE_K, tiles = lora_tiles(T, slots);
+  int split = ((VR > 32 ? 1 : 2) * sm_count() + tiles / 2) / tiles;       // the blocks that fit at a time
+  const int most = stages > 2 ? stages / 2 : 1;                           // two stages a block
   if (split > most) split = most;
-  return split > 16 ? 16 : split;
+  return split < 1 ? 1 : split > 8 ? 8 : split;
 }
+// One launch for a step of at most 64 rows, where an adapter is what eight SMs take in good time.
+static bool lora_few(const LoraParams& p) { return p.T <= 64 && p.VR <= LORA_FEW_RANKS && p.rank_tiles <= 4 && (p.a_slot + p.b_slot) * 16 <= 2 << 20; }
 
+template <int KS, int OUT>
+static int lora_up_launch(LoraParams& p, int max_tiles, void* stream) {
+  VB_CHECK_CUDA(max_dyn_smem_once(lora_up_kernel<KS, OUT>));
+  const int v_bytes = (p.tile_rows >> 4) * p.slices * lora_parts<OUT>() * KS * 512;
+  const int block_bytes = KS * 1024 * (OUT == LORA_GLU ? 2 : 1) + p.tile_rows * (OUT == LORA_GLU || p.base ? lora_row_bytes<OUT>() : 0);
+  // columns a block: about 48 KB beside v (two warps deep in columns at least), so that several blocks share an SM
+  int per = (48 * 1024) / block_bytes;
+  const int least = p.tile_rows == 16 ? 8 : 2;
+  if (per < least) per = least;
+  if (per > 16) per = 16;
+  if (per > p.blocks) per = p.blocks;
+  size_t smem;
+  while ((smem = static_cast<size_t>(v_bytes) + static_cast<size_t>(per) * block_bytes + p.tile_rows * 16) > VB_MAX_DYN_SMEM && per > 1) --per;      // (one fits always)
+  p.per_block = per;
+  VB_LAUNCH_PDL((lora_up_kernel<KS, OUT>), dim3(max_tiles, (p.blocks + per - 1) / per), LORA_THREADS, smem, stream, p);
+  return 0;
+}
+template <int RT>
+static int lora_down_launch(const LoraParams& p, int max_tiles, void* stream) {
+  VB_CHECK_CUDA(max_dyn_smem_once(lora_down_kernel<RT>));
+  VB_CHECK_CUDA(launch_kernel_cluster3(lora_down_kernel<RT>, dim3(max_tiles, p.k_split), dim3(LORA_THREADS), LoraDown<RT>::SMEM, static_cast<cudaStream_t>(stream), true,
+                                       dim3(1, p.k_split, 1), p));
+  return 0;
+}
+template <int KS, int OUT>
+static int lora_few_launch(const LoraParams& p, int tiles, void* stream) {
+  const size_t smem = (8 * 16 * 20 + 16 * static_cast<size_t>(p.VR)) * sizeof(float) + static_cast<size_t>(p.VR >> 4) * lora_parts<OUT>() * 512;
+  if (p.VR == 16) VB_LAUNCH_PDL_CLUSTER((lora_few_kernel<KS, OUT, 1>), tiles * LORA_CLUSTER, LORA_THREADS, smem, stream, LORA_CLUSTER, p);
+  else VB_LAUNCH_PDL_CLUSTER((lora_few_kernel<KS, OUT, 4>), tiles * LORA_CLUSTER, LORA_THREADS, smem, stream, LORA_CLUSTER, p);
+  return 0;
+}
 template <int OUT>
-static int lora_up_launch(const LoraParams& p, dim3 grid, size_t smem, void* stream) {
+static int lora_launch(LoraParams& p, int slots, void* stream) {
+  const int max_tiles = lora_max_tiles(p.T, slots);
+  p.parts = lora_parts<OUT>();
+  if (OUT == LORA_GLU) p.blocks = p.block0[1];         // column blocks of one of the two
+  if (lora_few(p)) {
+    if (p.rank_tiles == 1) return lora_few_launch<1, OUT>(p, max_tiles, stream);
+    if (p.rank_tiles == 2) return lora_few_launch<2, OUT>(p, max_tiles, stream);
+    return lora_few_launch<4, OUT>(p, max_tiles, stream);
+  }
+  const int rc = p.VR <= 16   ? lora_down_launch<1>(p, max_tiles, stream)
+                 : p.VR <= 32 ? lora_down_launch<2>(p, max_tiles, stream)
+                 : p.VR <= 64 ? lora_down_launch<4>(p, max_tiles, stream)
+                              : lora_down_launch<8>(p, max_tiles, stream);
+  if (rc) return rc;
   switch (p.rank_tiles) {
-    case 1: VB_CHECK_CUDA(max_dyn_smem_once(lora_up_kernel<1, OUT>)); VB_LAUNCH_PDL((lora_up_kernel<1, OUT>), grid, LORA_THREADS, smem, stream, p); break;
-    case 2: VB_CHECK_CUDA(max_dyn_smem_once(lora_up_kernel<2, OUT>)); VB_LAUNCH_PDL((lora_up_kernel<2, OUT>), grid, LORA_THREADS, smem, stream, p); break;
-    case 4: VB_CHECK_CUDA(max_dyn_smem_once(lora_up_kernel<4, OUT>)); VB_LAUNCH_PDL((lora_up_kernel<4, OUT>), grid, LORA_THREADS, smem, stream, p); break;
-    default: VB_CHECK_CUDA(max_dyn_smem_once(lora_up_kernel<8, OUT>)); VB_LAUNCH_PDL((lora_up_kernel<8, OUT>), grid, LORA_THREADS, smem, stream, p); break;
+    case 1: return lora_up_launch<1, OUT>(p, max_tiles, stream);
+    case 2: return lora_up_launch<2, OUT>(p, max_tiles, stream);
+    case 4: return lora_up_launch<4, OUT>(p, max_tiles, stream);
+    default: return lora_up_launch<8, OUT>(p, max_tiles, stream);
   }
-  return 0;
 }
-
-static int lora_down_launch(const LoraParams& p, int tile_rows, dim3 grid, void* stream) {
-  if (tile_rows == 16) {
-    const size_t smem = 8 * 16 * (2 * 8 + 4) * sizeof(float);
-    VB_LAUNCH_PDL((lora_down_kernel<2, 2>), grid, LORA_THREADS, smem, stream, p);
-  } else {
-    const size_t smem = 8 * 16 * (8 * 8 + 4) * sizeof(float);
-    VB_LAUNCH_PDL((lora_down_kernel<8, 2>), grid, LORA_THREADS, smem, stream, p);
-  }
-  return 0;
+// v of every tile in three parts
+static size_t lora_ws_bytes(int T, int slots, int rank, int slices) {
+  return static_cast<size_t>(lora_max_tiles(T, slots)) * (lora_tile_rows(T) / 16) * slices * (rank / 16) * 3 * 512;
 }
 
 // checks and fills what both entry points share
 static int lora_setup(const char* who, LoraParams& p, const void* d_x, long long ldx, const void* d_a, const void* d_b, const float* d_scale, int slots,
-                      int rank, const int32_t* widths, int slices, const int32_t* d_order, const void* d_tiles, int T, int K, void* d_ws, size_t ws_bytes) {
-  VB_CHECK_ARG(d_x && d_a && d_b && d_scale && d_order && d_tiles && widths && d_ws, "%s: null pointer", who);
+                      int rank, const int32_t* widths, int slices, const void* d_tiles, int T, int K, void* d_ws, size_t ws_bytes) {
+  VB_CHECK_ARG(d_x && d_a && d_b && d_scale && d_tiles && widths && d_ws, "%s: null pointer", who);
   VB_CHECK_ARG(slots >= 1 && slots <= LORA_MAX_SLOTS, "%s: %d adapters; 1 to %d", who, slots, LORA_MAX_SLOTS);
   VB_CHECK_ARG(rank == 16 || rank == 32 || rank == 64 || rank == 128, "%s: padded rank %d must be 16, 32, 64 or 128", who, rank);
   VB_CHECK_ARG(slices >= 1 && slices <= LORA_MAX_SLICES, "%s: %d slices; 1 to %d", who, slices, LORA_MAX_SLICES);
@@ -410,8 +636,8 @@ static int lora_setup(const char* who, LoraParams& p, const void* d_x, long long
     p.block0[s + 1] = p.block0[s] + (widths[s] + 31) / 32;
     p.col0[s + 1] = p.col0[s] + widths[s];
   }
-  p.tiles = static_cast<const int4*>(d_tiles);
-  p.order = d_order;
+  p.tiles = static_cast<const int32_t*>(d_tiles);
+  p.tile_rows = lora_tile_rows(T);
   p.x = static_cast<const __nv_bfloat16*>(d_x);
   p.ldx = ldx;
   p.a = static_cast<const uint4*>(d_a);
@@ -425,20 +651,12 @@ static int lora_setup(const char* who, LoraParams& p, const void* d_x, long long
   p.a_slot = static_cast<long long>(p.VR / 16) * p.kb32 * 64;
   p.b_slot = static_cast<long long>(p.block0[slices]) * p.rank_tiles * 64;
   p.blocks = p.block0[slices];
-  p.k_split = lora_k_split(T, K, slots);
-  p.v = static_cast<float*>(d_ws);
-  const size_t need = static_cast<size_t>(p.k_split) * T * p.VR * sizeof(float);
+  p.k_split = lora_k_split(T, K, slots, p.VR);
+  p.v = static_cast<uint32_t*>(d_ws);
+  const size_t need = lora_ws_bytes(T, slots, rank, slices);
   VB_CHECK_ARG(ws_bytes >= need && reinterpret_cast<uintptr_t>(d_ws) % 16 == 0, "%s: workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", who, need,
                ws_bytes);
   return 0;
-}
-
-static dim3 lora_up_grid(const LoraParams& p, int slots) {
-  const int tr = lora_tile_rows(p.T), tiles = p.T <= 64 ? (p.T < slots + 1 ? p.T : slots + 1) : (p.T + tr - 1) / tr;
-  int split = (4 * 148 + tiles - 1) / tiles;                // four blocks an SM, at least a column block for every warp
-  const int most = (p.blocks + 7) / 8;
-  if (split > most) split = most;
-  return dim3(lora_max_tiles(p.T, slots), split < 1 ? 1 : split);
 }
 
 }  // namespace vb
@@ -447,28 +665,28 @@ using namespace vb;
 
 extern "C" {
 
-int vb_lora_max_tiles(int T, int slots) { return T < 1 || slots < 1 ? 0 : lora_max_tiles(T, slots); }
+size_t vb_lora_plan_bytes(int T, int slots) {
+  return T < 1 || slots < 1 ? 0 : static_cast<size_t>(lora_max_tiles(T, slots)) * (4 + lora_tile_rows(T)) * 4;
+}
 
-int vb_lora_plan(int32_t* d_order, void* d_tiles, const int32_t* d_ids, int T, int slots, void* stream) {
-  VB_CHECK_ARG(d_order && d_tiles && d_ids, "vb_lora_plan: null pointer");
+int vb_lora_plan(void* d_tiles, const int32_t* d_ids, int T, int slots, void* stream) {
+  VB_CHECK_ARG(d_tiles && d_ids, "vb_lora_plan: null pointer");
+  VB_CHECK_ARG(reinterpret_cast<uintptr_t>(d_tiles) % 16 == 0, "vb_lora_plan: the plan must be 16-byte aligned");
   VB_CHECK_ARG(slots >= 1 && slots <= LORA_MAX_SLOTS, "vb_lora_plan: %d adapters; 1 to %d", slots, LORA_MAX_SLOTS);
   VB_CHECK_ARG(T >= 1, "vb_lora_plan: no rows");
-  VB_LAUNCH_PDL(lora_plan_kernel, 1, 1024, 0, stream, d_order, static_cast<int4*>(d_tiles), d_ids, T, slots, lora_tile_rows(T));
+  VB_LAUNCH_PDL(lora_plan_kernel, 1, 1024, 0, stream, static_cast<int32_t*>(d_tiles), d_ids, T, slots, lora_tile_rows(T), lora_max_tiles(T, slots));
   return 0;
 }
 
-size_t vb_lora_workspace_bytes(int T, int K, int slots, int rank, int slices) {
-  if (T < 1 || K < 1 || slots < 1) return 0;
-  return static_cast<size_t>(lora_k_split(T, K, slots)) * T * slices * rank * sizeof(float);
-}
+size_t vb_lora_workspace_bytes(int T, int slots, int rank, int slices) { return T < 1 || slots < 1 ? 0 : lora_ws_bytes(T, slots, rank, slices); }
 
 int vb_lora(void* d_out, long long ld_out, const void* d_base, long long ld_base, int out_f32, const void* d_x, long long ldx, const void* d_a, const void* d_b,
-            const float* d_scale, int slots, int rank, const int32_t* widths, int slices, const int32_t* d_order, const void* d_tiles, int T, int K, void* d_ws,
-            size_t ws_bytes, void* stream) {
+            const float* d_scale, int slots, int rank, const int32_t* widths, int slices, const void* d_tiles, int T, int K, void* d_ws, size_t ws_bytes,
+            void* stream) {
   VB_CHECK_ARG(d_out, "vb_lora: null pointer");
   if (T <= 0) return 0;
   LoraParams p = {};
-  const int rc = lora_setup("vb_lora", p, d_x, ldx, d_a, d_b, d_scale, slots, rank, widths, slices, d_order, d_tiles, T, K, d_ws, ws_bytes);
+  const int rc = lora_setup("vb_lora", p, d_x, ldx, d_a, d_b, d_scale, slots, rank, widths, slices, d_tiles, T, K, d_ws, ws_bytes);
   if (rc) return rc;
   const int unit = out_f32 ? 4 : 8;
   VB_CHECK_ARG(ld_out % unit == 0 && ld_out >= p.col0[slices] && reinterpret_cast<uintptr_t>(d_out) % 16 == 0 &&
@@ -478,22 +696,18 @@ int vb_lora(void* d_out, long long ld_out, const void* d_base, long long ld_base
   p.ldo = ld_out;
   p.base = d_base;
   p.ld_base = ld_base;
-  const int tr = lora_tile_rows(T);
-  const int rc1 = lora_down_launch(p, tr, dim3(lora_max_tiles(T, slots), p.k_split), stream);
-  if (rc1) return rc1;
-  const size_t smem = static_cast<size_t>(tr) * (p.VR + 4) * sizeof(float);
-  return out_f32 ? lora_up_launch<LORA_F32>(p, lora_up_grid(p, slots), smem, stream) : lora_up_launch<LORA_BF16>(p, lora_up_grid(p, slots), smem, stream);
+  return out_f32 ? lora_launch<LORA_F32>(p, slots, stream) : lora_launch<LORA_BF16>(p, slots, stream);
 }
 
 int vb_lora_gate_up(void* d_act, long long ld_act, int xt_rows, const float* d_planes, int splits, int half, int ff, const void* d_x, long long ldx,
-                    const void* d_a, const void* d_b, const float* d_scale, int slots, int rank, const int32_t* d_order, const void* d_tiles, int T, int K,
-                    void* d_ws, size_t ws_bytes, void* stream) {
+                    const void* d_a, const void* d_b, const float* d_scale, int slots, int rank, const void* d_tiles, int T, int K, void* d_ws,
+                    size_t ws_bytes, void* stream) {
   VB_CHECK_ARG(d_act && d_planes, "vb_lora_gate_up: null pointer");
   VB_CHECK_ARG(splits >= 1 && half >= 16 && half % 16 == 0 && half <= 64, "vb_lora_gate_up: %d planes, tiles of %d gate rows (16, 32, 48 or 64)", splits, half);
   if (T <= 0) return 0;
   LoraParams p = {};
   const int32_t widths[2] = {ff, ff};
-  const int rc = lora_setup("vb_lora_gate_up", p, d_x, ldx, d_a, d_b, d_scale, slots, rank, widths, 2, d_order, d_tiles, T, K, d_ws, ws_bytes);
+  const int rc = lora_setup("vb_lora_gate_up", p, d_x, ldx, d_a, d_b, d_scale, slots, rank, widths, 2, d_tiles, T, K, d_ws, ws_bytes);
   if (rc) return rc;
   VB_CHECK_ARG(xt_rows >= 0 && reinterpret_cast<uintptr_t>(d_act) % 16 == 0 && reinterpret_cast<uintptr_t>(d_planes) % 16 == 0 &&
                    (xt_rows > 0 || (ld_act % 8 == 0 && ld_act >= ff)),
@@ -507,12 +721,7 @@ int vb_lora_gate_up(void* d_act, long long ld_act, int xt_rows, const float* d_p
   p.width = (ff + half - 1) / half * 2 * half;
   p.xt_rows = xt_rows;
   p.xt_kb = (ff + 63) / 64;
-  const int tr = lora_tile_rows(T);
-  const int rc1 = lora_down_launch(p, tr, dim3(lora_max_tiles(T, slots), p.k_split), stream);
-  if (rc1) return rc1;
-  p.blocks = p.block0[1];              // column blocks of one of the two
-  const size_t smem = static_cast<size_t>(tr) * (p.VR + 4) * sizeof(float);
-  return lora_up_launch<LORA_GLU>(p, lora_up_grid(p, slots), smem, stream);
+  return lora_launch<LORA_GLU>(p, slots, stream);
 }
 
 }  // extern "C"

@@ -697,13 +697,6 @@ __device__ __forceinline__ MlDownPiece ml_down_piece(const MoeLayerParams& p, co
   m.passes = (m.n + NT * 8 - 1) / (NT * 8);
   return m;
 }
-__device__ __forceinline__ float4 ld_dsmem_f32x4(const float* local_ptr, uint32_t cta_rank) {
-  uint32_t raddr;
-  float4 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(raddr) : "r"(smem_u32(local_ptr)), "r"(cta_rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(raddr) : "memory");
-  return v;
-}
 // four neighbours of a row of the result (its rows may start anywhere)
 __device__ __forceinline__ void ml_result(const MoeLayerParams& p, int t, int col, const float4& s) {
   float* y = p.y + t * p.ldy + col;

@@ -39,4 +39,13 @@ __device__ __forceinline__ uint32_t pack_cut(float first, float second) {
   return __byte_perm(__float_as_uint(first), __float_as_uint(second), 0x7632);
 }
 
+// (distributed shared memory: the same place in another block of the cluster)
+__device__ __forceinline__ float4 ld_dsmem_f32x4(const float* local_ptr, uint32_t cta_rank) {
+  uint32_t raddr;
+  float4 v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(raddr) : "r"(smem_u32(local_ptr)), "r"(cta_rank));
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(raddr) : "memory");
+  return v;
+}
+
 }  // namespace vb

@@ -1959,7 +1959,7 @@ class LoraBank:
     def _workspace(self, T: int) -> torch.Tensor:
         n = self._ws_floats.get(T)
         if n is None:
-            n = self._ws_floats[T] = _lib.load().vb_lora_workspace_bytes(T, self.K, self.slots, self.rank_pad, len(self.widths)) // 4
+            n = self._ws_floats[T] = _lib.load().vb_lora_workspace_bytes(T, self.slots, self.rank_pad, len(self.widths)) // 4
         return torch.empty(n, dtype=torch.float32, device=self.a.device)
 
 
@@ -1970,25 +1970,24 @@ class LoraPlan:
         _refuse(max_rows < 1 or not 1 <= slots <= 1023, f"LoraPlan: {max_rows} rows, {slots} adapters (1 to 1023)")
         self.max_rows, self.slots, self.n_rows = int(max_rows), int(slots), 0
         lib = _lib.load()
-        tiles = max(lib.vb_lora_max_tiles(min(max_rows, 64), slots), lib.vb_lora_max_tiles(max_rows, slots))
-        self.order = torch.zeros(max_rows, dtype=torch.int32, device=device)
-        self.tiles = torch.zeros(1 + tiles, 4, dtype=torch.int32, device=device)
+        n = max(lib.vb_lora_plan_bytes(min(max_rows, 64), slots), lib.vb_lora_plan_bytes(max_rows, slots))
+        self.tiles = torch.zeros(n // 4, dtype=torch.int32, device=device)
 
 
 def lora_plan(plan: LoraPlan, ids: torch.Tensor) -> LoraPlan:
     """ids int32 [T]: the adapter of every row; what is not 0 .. slots - 1 (-1) has none."""
-    _need_here("lora_plan", ids, plan.order)
+    _need_here("lora_plan", ids, plan.tiles)
     _refuse(ids.dtype != torch.int32 or ids.dim() != 1 or not ids.is_contiguous(), "lora_plan: int32 ids in one dimension are needed")
     T = ids.numel()
     _refuse(T > plan.max_rows, f"lora_plan: {T} rows; the plan holds {plan.max_rows}")
     if T:
-        call("vb_lora_plan", plan.order.data_ptr(), plan.tiles.data_ptr(), ids.data_ptr(), T, plan.slots, _stream())
+        call("vb_lora_plan", plan.tiles.data_ptr(), ids.data_ptr(), T, plan.slots, _stream())
     plan.n_rows = T
     return plan
 
 
 def _lora_check(who: str, x: torch.Tensor, bank: LoraBank, plan: LoraPlan) -> None:
-    _need_here(who, x, bank.a, plan.order)
+    _need_here(who, x, bank.a, plan.tiles)
     _refuse(x.dtype != BF16 or x.dim() != 2 or x.shape[1] != bank.K or (x.stride(1) != 1 and x.shape[0] > 0), f"{who}: bf16 rows of {bank.K} are needed")
     _refuse(plan.slots != bank.slots, f"{who}: the plan counts {plan.slots} adapters, the bank {bank.slots}")
     _refuse(plan.n_rows != x.shape[0], f"{who}: {x.shape[0]} rows, the plan was made for {plan.n_rows}")
@@ -2012,7 +2011,7 @@ def lora(x: torch.Tensor, bank: LoraBank, plan: LoraPlan, out: Optional[torch.Te
         return out
     ws = bank._workspace(T)
     call("vb_lora", out.data_ptr(), out.stride(0) if T > 1 else N, _p(base), base.stride(0) if base is not None and T > 1 else N, int(f32), x.data_ptr(),
-         x.stride(0) if T > 1 else bank.K, *bank._ptrs, bank._widths, len(bank.widths), plan.order.data_ptr(), plan.tiles.data_ptr(), T, bank.K, ws.data_ptr(),
+         x.stride(0) if T > 1 else bank.K, *bank._ptrs, bank._widths, len(bank.widths), plan.tiles.data_ptr(), T, bank.K, ws.data_ptr(),
          ws.numel() * 4, _stream())
     return out
 
@@ -2041,8 +2040,7 @@ def lora_gate_up(x: torch.Tensor, bank: LoraBank, plan: LoraPlan, planes: torch.
         return out
     ws = bank._workspace(T)
     call("vb_lora_gate_up", out.data.data_ptr() if tiled else out.data_ptr(), ff if tiled or T == 1 else out.stride(0), out.t_tile if tiled else 0,
-         planes.data_ptr(), planes.shape[0], int(half), ff, x.data_ptr(), x.stride(0) if T > 1 else bank.K, *bank._ptrs, plan.order.data_ptr(),
-         plan.tiles.data_ptr(), T, bank.K, ws.data_ptr(), ws.numel() * 4, _stream())
+         planes.data_ptr(), planes.shape[0], int(half), ff, x.data_ptr(), x.stride(0) if T > 1 else bank.K, *bank._ptrs, plan.tiles.data_ptr(), T, bank.K, ws.data_ptr(), ws.numel() * 4, _stream())
     return out
 
 
