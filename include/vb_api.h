@@ -893,38 +893,49 @@ int vb_selective_scan_tiled(void* d_out, int ld_out, float* d_state, float* d_sc
 /* ---- weights that a row brings with it ----------------------------------------------------------------------------------------
  * Low-rank adapters of many requests beside a shared projection (csrc/lora.cu):
  *   out[t][n] = base[t][n] + sum_j B_a[n][j] (scale_a sum_k A_a,s[j][k] x[t][k]),   a = ids[t] (outside 0 .. slots-1: base alone), s = n's slice
+ * VbLoraBank (HOST struct): the adapters in the order that csrc/lora.cu states (ops.LoraBank writes it).  slots 1 .. 1023, rank padded to 16, 32, 64 or
+ *   128, K and the widths of the 1 .. 4 slices multiples of 8.
  * vb_lora_plan: rows of a step by adapter, once per step for every projection of every layer: d_tiles, vb_lora_plan_bytes(T, slots) bytes, 16-byte
- *   aligned.  slots 1 .. 1023.
- * vb_lora: out and base fp32 (out_f32) or bf16, rows 16-byte aligned; d_base may be NULL (zeros) or d_out.  d_a / d_b: the adapters in the order that
- *   csrc/lora.cu states (ops.LoraBank writes it), rank padded to 16, 32, 64 or 128, d_scale fp32 [slots]; widths: columns of the
- *   1 .. 4 slices (HOST array, multiples of 8).  K a multiple of 8.  Every row 0 .. T-1 of out is written, nothing behind it.
+ *   aligned.
+ * vb_lora: out and base fp32 (out_f32) or bf16, rows 16-byte aligned; d_base may be NULL (zeros) or d_out.  Every row 0 .. T-1 of out is written, nothing
+ *   behind it.  vb_lora_workspace_bytes may be 0 (d_ws may be NULL then).
  * vb_lora_gate_up: act[t][i] = silu(g) u (bf16, row-major with ld_act or, xt_rows > 0, tiled) from d_planes fp32 [splits][T][2 * tiles * half], gate and
- *   up rows interleaved as vb_gemm_bf16 mode 1 leaves them, plus both adapters' products (two slices of ff columns). */
+ *   up rows interleaved as vb_gemm_bf16 mode 1 leaves them, plus both adapters' products (a bank of two slices of equal width). */
+typedef struct {
+  const void *d_a, *d_b;
+  const float* d_scale;
+  int32_t slots, rank, K, slices, widths[4];
+} VbLoraBank;
 size_t vb_lora_plan_bytes(int T, int slots);
 int vb_lora_plan(void* d_tiles, const int32_t* d_ids, int T, int slots, void* stream);
-size_t vb_lora_workspace_bytes(int T, int slots, int rank, int slices);
-int vb_lora(void* d_out, long long ld_out, const void* d_base, long long ld_base, int out_f32, const void* d_x, long long ldx, const void* d_a,
-            const void* d_b, const float* d_scale, int slots, int rank, const int32_t* widths, int slices, const void* d_tiles, int T, int K,
-            void* d_ws, size_t ws_bytes, void* stream);
-int vb_lora_gate_up(void* d_act, long long ld_act, int xt_rows, const float* d_planes, int splits, int half, int ff, const void* d_x, long long ldx,
-                    const void* d_a, const void* d_b, const float* d_scale, int slots, int rank, const void* d_tiles, int T, int K, void* d_ws,
-                    size_t ws_bytes, void* stream);
-/* A mixture-of-experts layer for at most vb_moe_layer_max_rows() rows (csrc/moe_layer.cu).
- * vb_moe_layer_route: kind 0 softmax over the chosen logits (+ d_bias), 1 sigmoid scores (chosen by score + d_bias within the kept groups, weights over
- *   their sum), 2 softmax over all experts (chosen within the kept groups, weights as they are), 3 d_table[d_ids[t]] (int32 [vocab][top]; weights 1 / top).
- *   Ties go to the lower expert; a NaN ranks above everything, so that idx always names experts.  d_shared_gate [T] = sigmoid(d_shared_gate_w . h).
- * vb_moe_layer_experts: reads the chosen experts' matrices only.  d_up: packed tiles (vb_pack_weight_tiles, up_rows rows each) of the experts' gate | up rows (interleaved; act 0 silu, 1
- * clamped) or up rows (act 2 relu^2, 3 gelu, 4 tanh gelu), one expert after the other, the shared one (shared_ff > 0) last; d_down: packed tiles of
- * 128 rows of [W][experts * ff + shared_ff].  d_idx int32 [T][top] (an index that is no expert counts as none, one named twice counts with both
- * weights), d_wts fp32 [T][top], d_shared_gate fp32 [T] or NULL (1).  d_y fp32 [T] rows of W, ldy apart. */
+size_t vb_lora_workspace_bytes(const VbLoraBank* bank, int T);
+int vb_lora(void* d_out, long long ld_out, const void* d_base, long long ld_base, int out_f32, const void* d_x, long long ldx, const VbLoraBank* bank,
+            const void* d_tiles, int T, void* d_ws, size_t ws_bytes, void* stream);
+int vb_lora_gate_up(void* d_act, long long ld_act, int xt_rows, const float* d_planes, int splits, int half, const void* d_x, long long ldx,
+                    const VbLoraBank* bank, const void* d_tiles, int T, void* d_ws, size_t ws_bytes, void* stream);
+/* A mixture-of-experts layer for at most vb_moe_layer_max_rows() rows (csrc/moe_layer.cu); of the experts' matrices it reads those that a row chose.
+ * VbMoeWeights (HOST struct): d_up: packed tiles (vb_pack_weight_tiles, up_rows rows each) of the experts' gate | up rows (interleaved; act 0 silu, 1 clamped) or up
+ *   rows (act 2 relu^2, 3 gelu, 4 tanh gelu), one expert after the other, the shared one (shared_ff > 0) last; d_down: packed tiles of 128 rows of [width][experts *
+ *   ff + shared_ff].  width a multiple of 8, ff and shared_ff of 64.
+ * VbMoeRouter (HOST struct): kind 0 softmax over the chosen logits (+ d_bias), 1 sigmoid scores (chosen by score + d_bias within the kept groups, weights over their
+ *   sum), 2 softmax over all experts (chosen within the kept groups, weights as they are), 3 d_table[d_ids[t]] (int32 [vocab][top]; weights 1 / top; an entry
+ *   that is no expert counts as none, one named twice with both weights).  Ties go to the lower expert; a NaN ranks above everything.  d_shared_gate: the
+ *   shared expert times sigmoid(d_shared_gate . h).
+ * d_y fp32 [T] rows of width, ldy apart; d_ids int32 [T] for kind 3. */
+typedef struct {
+  const void *d_up, *d_down;
+  int32_t width, experts, ff, shared_ff, up_rows, act;
+  float limit, slope;
+} VbMoeWeights;
+typedef struct {
+  const float *d_weight, *d_bias, *d_shared_gate;
+  const int32_t* d_table;
+  int32_t kind, top, groups, keep, vocab;
+} VbMoeRouter;
 int vb_moe_layer_max_rows(void);
-int vb_moe_layer_route(int32_t* d_idx, float* d_wts, float* d_shared_gate, int kind, const void* d_h, long long ldh, const float* d_router_w,
-                       const float* d_bias, const float* d_shared_gate_w, const int32_t* d_ids, const int32_t* d_table, int T, int W, int experts,
-                       int top, int groups, int keep, int vocab, void* stream);
-size_t vb_moe_layer_workspace_bytes(int T, int top, int ff, int shared_ff);
-int vb_moe_layer_experts(float* d_y, long long ldy, const void* d_h, long long ldh, const void* d_up, const void* d_down, const int32_t* d_idx,
-                         const float* d_wts, const float* d_shared_gate, int T, int W, int experts, int top, int ff, int shared_ff, int up_rows,
-                         int act, float limit, float slope, void* d_ws, size_t ws_bytes, void* stream);
+size_t vb_moe_layer_workspace_bytes(const VbMoeWeights* weights, const VbMoeRouter* router, int T);
+int vb_moe_layer(float* d_y, long long ldy, const void* d_h, long long ldh, const VbMoeWeights* weights, const VbMoeRouter* router, const int32_t* d_ids, int T,
+                 void* d_ws, size_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -213,14 +213,12 @@ SIGNATURES = {
                                 c_int, c_int, c_int, c_int, c_float, c_float, c_float, P, C.c_longlong, c_int, c_int, P]),
     "vb_lora_plan_bytes": (c_size_t, [c_int, c_int]),
     "vb_lora_plan": (c_int, [P, P, c_int, c_int, P]),
-    "vb_lora_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
-    "vb_lora": (c_int, [P, C.c_longlong, P, C.c_longlong, c_int, P, C.c_longlong, P, P, P, c_int, c_int, P, c_int, P, c_int, c_int, P, c_size_t, P]),
-    "vb_lora_gate_up": (c_int, [P, C.c_longlong, c_int, P, c_int, c_int, c_int, P, C.c_longlong, P, P, P, c_int, c_int, P, c_int, c_int, P, c_size_t, P]),
+    "vb_lora_workspace_bytes": (c_size_t, [P, c_int]),
+    "vb_lora": (c_int, [P, C.c_longlong, P, C.c_longlong, c_int, P, C.c_longlong, P, P, c_int, P, c_size_t, P]),
+    "vb_lora_gate_up": (c_int, [P, C.c_longlong, c_int, P, c_int, c_int, P, C.c_longlong, P, P, c_int, P, c_size_t, P]),
     "vb_moe_layer_max_rows": (c_int, []),
-    "vb_moe_layer_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
-    "vb_moe_layer_route": (c_int, [P, P, P, c_int, P, C.c_longlong, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, P]),
-    "vb_moe_layer_experts": (c_int, [P, C.c_longlong, P, C.c_longlong, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_float,
-                                     P, c_size_t, P]),
+    "vb_moe_layer_workspace_bytes": (c_size_t, [P, P, c_int]),
+    "vb_moe_layer": (c_int, [P, C.c_longlong, P, C.c_longlong, P, P, P, c_int, P, c_size_t, P]),
     "vb_selective_scan_piece_rows": (c_int, []),
     "vb_selective_scan_scratch_floats": (c_int, [c_int, c_int, c_int, c_int]),
     "vb_selective_scan": (c_int, [P, c_int, P, P, c_int, P, c_int, P, P, c_int, c_int, c_int, P, c_int, P, P, P, P, P, c_int,
@@ -228,6 +226,22 @@ SIGNATURES = {
     "vb_selective_scan_tiled": (c_int, [P, c_int, P, P, P, c_int, P, c_int, P, P, c_int, c_int, c_int, P, c_int, P, P, P, P, P,
                                         P, P, c_int, c_int, c_int, c_int, c_int, c_float, c_int, P]),
 }
+
+
+class LoraBankStruct(C.Structure):
+    """VbLoraBank"""
+    _fields_ = [("d_a", P), ("d_b", P), ("d_scale", P), ("slots", C.c_int32), ("rank", C.c_int32), ("K", C.c_int32), ("slices", C.c_int32), ("widths", C.c_int32 * 4)]
+
+
+class MoeWeightsStruct(C.Structure):
+    """VbMoeWeights"""
+    _fields_ = [("d_up", P), ("d_down", P)] + [(n, C.c_int32) for n in ("width", "experts", "ff", "shared_ff", "up_rows", "act")] + [("limit", c_float), ("slope", c_float)]
+
+
+class MoeRouterStruct(C.Structure):
+    """VbMoeRouter"""
+    _fields_ = [("d_weight", P), ("d_bias", P), ("d_shared_gate", P), ("d_table", P)] + [(n, C.c_int32) for n in ("kind", "top", "groups", "keep", "vocab")]
+
 
 _lock = threading.Lock()
 _lib = None
@@ -311,7 +325,7 @@ LAUNCHES = {"vb_set_pdl": 0, "vb_set_trace": 0, "vb_weight_tiles_bytes": 0, "vb_
             "vb_set_gemm_smem_kb": 0, "vb_window_attn_tile_rows": 0, "vb_decay_attn_tile_rows": 0, "vb_decay_attn_tiled": 3, "vb_window_attn": 2, "vb_mingru_tiled": 3, "vb_mingru_scratch_floats": 0,
             "vb_short_conv": 2, "vb_selective_scan_tiled": 3, "vb_selective_scan_piece_rows": 0,
             "vb_selective_scan_scratch_floats": 0, "vb_sigmoid_attn": 1, "vb_ssd_tiled": 3, "vb_ssd_tile_rows": 0,
-            "vb_ssd_scratch_floats": 0, "vb_lora": 2, "vb_lora_gate_up": 2, "vb_moe_layer_experts": 2}
+            "vb_ssd_scratch_floats": 0, "vb_lora": 2, "vb_lora_gate_up": 2, "vb_moe_layer": 3}
 launch_counter = [0]
 
 

@@ -98,7 +98,7 @@ struct LoraParams {
   long long ldo, ld_base;
   // gate | up
   const float* planes;
-  int splits, half, width, ff, xt_rows, xt_kb;
+  int splits, width, ff, xt_rows, xt_kb;
 };
 
 // ---- v as the second product's A operand ------------------------------------------------------------------------------------------
@@ -114,9 +114,14 @@ __device__ __forceinline__ void lora_put(uint32_t* frags, int slices, int parts,
   if (parts > 2) at[2 * ks * 128] = pack_cut(l0, l1);
 }
 
-// 16 bytes past the registers and L1; zeros where `in` is false (nothing is read then)
-__device__ __forceinline__ void cp_async16(uint32_t to, const void* from, bool in) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(in ? 16 : 0) : "memory");
+// 16 bytes past the registers and L1; zeros where `bytes` is 0 instead of 16 (nothing is read then)
+__device__ __forceinline__ void cp_async16(uint32_t to, const void* from, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ uint4 lds16(uint32_t at) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at));
+  return v;
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -124,13 +129,13 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 
 // ---- first product: v = scale A x -------------------------------------------------------------------------------------------------
 // Block: a tile x a piece of K, in stages of 128 k: 256 bytes of each row of x and RT rank tiles of A, copied 16 bytes at a time with three to five stages on
-// their way.  (Bulk copies of a row's 256 bytes took 79 us where this takes 16: 4096 rows of 8192, rank 64; they start one at a time.)  Rows are 320 bytes apart:
+// their way.  (Bulk copies of a row's 256 bytes start one at a time: 79 us for 4096 rows of 8192 at rank 64.)  Rows are 320 bytes apart:
 // lanes 0 to 7 of a 16-byte load read two rows, which then lie in different banks.  Warps: four k blocks of 32 by two halves of the rows.  More than RT rank
 // tiles: x again.  The pieces of a tile are a cluster, which adds them up and leaves v in parts.
 constexpr int LORA_STAGE_K = 128, LORA_ROW_BYTES = 2 * LORA_STAGE_K + 64, LORA_X_BYTES = 64 * LORA_ROW_BYTES, LORA_RED_LD = 36;
 template <int RT>
 struct LoraDown {
-  static constexpr int STAGES = RT == 4 ? 5 : RT == 2 ? 3 : 4, BLOCKS = RT >= 4 ? 1 : 2;
+  static constexpr int STAGES = RT == 8 || RT == 1 ? 4 : 3, BLOCKS = RT == 8 ? 1 : 2;
   static constexpr int STAGE_BYTES = LORA_X_BYTES + RT * 4096;
   static constexpr size_t SMEM = static_cast<size_t>(STAGES) * STAGE_BYTES;
   static_assert(8 * RT * 16 * LORA_RED_LD * 4 + 64 * RT * 16 * 4 <= STAGES * STAGE_BYTES, "the sums stand where the stages stood");
@@ -147,56 +152,73 @@ __global__ void __launch_bounds__(LORA_THREADS, LoraDown<RT>::BLOCKS) lora_down_
   const int n = tl.z, rts = p.VR >> 4;
   const int stages = (p.K + LORA_STAGE_K - 1) / LORA_STAGE_K, s0 = static_cast<int>(static_cast<long long>(stages) * blockIdx.y / p.k_split),
             s1 = static_cast<int>(static_cast<long long>(stages) * (blockIdx.y + 1) / p.k_split);
-  // a thread's copies: 16 bytes of four rows, 16 bytes of every rank tile
+  // a thread's copies: 16 bytes of four rows, 16 bytes of every rank tile.  What is not there (rows behind the last, k behind K, rank tiles) is filled with zeros.
   const int chunk = tid & 15, row0 = tid >> 4;
   const __nv_bfloat16* xr[4];
+  int x_bytes[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) xr[i] = row0 + i * 16 < n ? p.x + rec[4 + row0 + i * 16] * p.ldx + chunk * 8 : nullptr;
+  for (int i = 0; i < 4; ++i) {
+    const bool in = row0 + i * 16 < n;
+    xr[i] = p.x + (in ? rec[4 + row0 + i * 16] : 0) * p.ldx + chunk * 8;
+    x_bytes[i] = in ? 16 : 0;
+  }
   const uint32_t ring = smem_u32(smem8), x_to = ring + row0 * LORA_ROW_BYTES + chunk * 16, a_to = ring + LORA_X_BYTES + tid * 16;
-  const uint4* a = p.a + tl.x * p.a_slot + tid;
   const float scale = p.scale[tl.x];
   const int kq = warp & 3, half = warp >> 2;
   const int tiles_n = min(4, max(0, (n - half * 32 + 7) >> 3));           // column tiles of 8 rows that this warp has
+  const uint32_t a_from = ring + LORA_X_BYTES + (kq * 64 + lane) * 16, x_from = ring + (half * 32 + g) * LORA_ROW_BYTES + kq * 64 + t4 * 16;
   for (int rt0 = 0; rt0 < rts; rt0 += RT) {
-    auto load = [&](int s, int slot) {
+    const uint4* ar[RT];
+    int a_bytes[RT];
+#pragma unroll
+    for (int i = 0; i < RT; ++i) {
+      const bool in = rt0 + i < rts;
+      ar[i] = p.a + tl.x * p.a_slot + static_cast<long long>(in ? rt0 + i : 0) * p.kb32 * 64 + tid;
+      a_bytes[i] = in ? 16 : 0;
+    }
+    auto load = [&](int s, uint32_t to) {
       if (s < s1) {
-        const int k = s * LORA_STAGE_K;
-        const bool in = k + chunk * 8 < p.K, in_a = s * 4 + (tid >> 6) < p.kb32;
+        const bool all = (s + 1) * LORA_STAGE_K <= p.K, in = all || s * LORA_STAGE_K + chunk * 8 < p.K, in_a = all || s * 4 + (tid >> 6) < p.kb32;
+        const long long x_at = in ? static_cast<long long>(s) * LORA_STAGE_K : 0, a_at = in_a ? static_cast<long long>(s) * 256 : 0;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (xr[i]) cp_async16(x_to + slot * STAGE_BYTES + i * 16 * LORA_ROW_BYTES, in ? xr[i] + k : xr[i], in);
+        for (int i = 0; i < 4; ++i) cp_async16(x_to + to + i * 16 * LORA_ROW_BYTES, xr[i] + x_at, in ? x_bytes[i] : 0);
 #pragma unroll
-        for (int i = 0; i < RT; ++i)
-          if (rt0 + i < rts) cp_async16(a_to + slot * STAGE_BYTES + i * 4096, in_a ? a + (static_cast<long long>(rt0 + i) * p.kb32 + s * 4) * 64 : a, in_a);
+        for (int i = 0; i < RT; ++i) cp_async16(a_to + to + i * 4096, ar[i] + a_at, in_a ? a_bytes[i] : 0);
       }
       cp_async_commit();
     };
     float acc[RT][4][4] = {};
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) load(s0 + i, i);
-    int slot = 0;
+    for (int i = 0; i < STAGES - 1; ++i) load(s0 + i, i * STAGE_BYTES);
+    uint32_t at = 0, free_at = (STAGES - 1) * STAGE_BYTES;
+#pragma unroll 1
     for (int s = s0; s < s1; ++s) {
       cp_async_wait<STAGES - 2>();
       __syncthreads();
-      load(s + STAGES - 1, slot == 0 ? STAGES - 1 : slot - 1);
-      const uint8_t* st = smem8 + slot * STAGE_BYTES;
+      load(s + STAGES - 1, free_at);
       uint4 av[RT][2];
 #pragma unroll
-      for (int i = 0; i < RT; ++i)
-#pragma unroll
-        for (int h = 0; h < 2; ++h) av[i][h] = *reinterpret_cast<const uint4*>(st + LORA_X_BYTES + i * 4096 + ((kq * 2 + h) * 32 + lane) * 16);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        if (j >= tiles_n) break;
-        const uint4 x = *reinterpret_cast<const uint4*>(st + (half * 32 + j * 8 + g) * LORA_ROW_BYTES + kq * 64 + t4 * 16);
-#pragma unroll
-        for (int i = 0; i < RT; ++i)
-          if (rt0 + i < rts) {
-            mma_bf16(acc[i][j], av[i][0].x, av[i][0].y, av[i][0].z, av[i][0].w, x.x, x.y);
-            mma_bf16(acc[i][j], av[i][1].x, av[i][1].y, av[i][1].z, av[i][1].w, x.z, x.w);
-          }
+      for (int i = 0; i < RT; ++i) {
+        av[i][0] = lds16(a_from + at + i * 4096);
+        av[i][1] = lds16(a_from + at + i * 4096 + 512);
       }
-      slot = slot + 1 == STAGES ? 0 : slot + 1;
+      auto column = [&](int j) {
+        const uint4 x = lds16(x_from + at + j * 8 * LORA_ROW_BYTES);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) mma_bf16(acc[i][j], av[i][0].x, av[i][0].y, av[i][0].z, av[i][0].w, x.x, x.y);
+#pragma unroll
+        for (int i = 0; i < RT; ++i) mma_bf16(acc[i][j], av[i][1].x, av[i][1].y, av[i][1].z, av[i][1].w, x.z, x.w);
+      };
+      if (tiles_n == 4) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) column(j);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 3; ++j)
+          if (j < tiles_n) column(j);
+      }
+      free_at = at;
+      at = at == (STAGES - 1) * STAGE_BYTES ? 0 : at + STAGE_BYTES;
     }
     cp_async_wait<0>();
     __syncthreads();
@@ -251,13 +273,29 @@ __device__ __forceinline__ void lora_block(float (&d)[4][4], const uint4* frags,
       mma_bf16(d[3], f.x, f.y, f.z, f.w, w[k][1].z, w[k][1].w);
     }
 }
-// a column block's part of B: from the bank, or from shared memory
-template <int KS, bool BANK>
+// a column block's part of B from the bank
+template <int KS>
 __device__ __forceinline__ void lora_take(uint4 (&w)[KS][2], const uint4* b) {
 #pragma unroll
   for (int k = 0; k < KS; ++k) {
-    w[k][0] = BANK ? __ldg(b + k * 64) : b[k * 64];
-    w[k][1] = BANK ? __ldg(b + k * 64 + 32) : b[k * 64 + 32];
+    w[k][0] = __ldg(b + k * 64);
+    w[k][1] = __ldg(b + k * 64 + 32);
+  }
+}
+// ... both operands from shared memory
+template <int KS, int PARTS>
+__device__ __forceinline__ void lora_product(float (&d)[4][4], uint32_t frags, uint32_t b) {
+#pragma unroll
+  for (int k = 0; k < KS; ++k) {
+    const uint4 w0 = lds16(b + k * 1024), w1 = lds16(b + k * 1024 + 512);
+#pragma unroll
+    for (int q = 0; q < PARTS; ++q) {
+      const uint4 f = lds16(frags + (q * KS + k) * 512);
+      mma_bf16(d[0], f.x, f.y, f.z, f.w, w0.x, w0.y);
+      mma_bf16(d[1], f.x, f.y, f.z, f.w, w0.z, w0.w);
+      mma_bf16(d[2], f.x, f.y, f.z, f.w, w1.x, w1.y);
+      mma_bf16(d[3], f.x, f.y, f.z, f.w, w1.z, w1.w);
+    }
   }
 }
 
@@ -271,39 +309,47 @@ __device__ __forceinline__ uint4 lora_round(const float* y) {
   return make_uint4(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7]));
 }
 
-// Results of a lane: eight neighbouring columns of row `row`.  y: the products; base, planes: what is added (nullptr: nothing), the gate's and the up's columns 16 apart.
+// Results of a lane: eight neighbouring columns.  y: the products; base: what is added (nullptr: nothing).
 template <int OUT>
-__device__ __forceinline__ void lora_result(const LoraParams& p, long long row, int col, float (&y)[8], const void* base) {
+__device__ __forceinline__ void lora_result(void* out, float (&y)[8], const void* base) {
   if constexpr (OUT == LORA_F32) {
     if (base) {
       lora_add4(y, static_cast<const float4*>(base)[0]);
       lora_add4(y + 4, static_cast<const float4*>(base)[1]);
     }
-    float4* o = reinterpret_cast<float4*>(static_cast<float*>(p.out) + row * p.ldo + col);
-    o[0] = make_float4(y[0], y[1], y[2], y[3]);
-    o[1] = make_float4(y[4], y[5], y[6], y[7]);
+    static_cast<float4*>(out)[0] = make_float4(y[0], y[1], y[2], y[3]);
+    static_cast<float4*>(out)[1] = make_float4(y[4], y[5], y[6], y[7]);
   } else {
     if (base) lora_add8(y, *static_cast<const uint4*>(base));
-    *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + col) = lora_round(y);
+    *static_cast<uint4*>(out) = lora_round(y);
   }
 }
-__device__ __forceinline__ void lora_gated(const LoraParams& p, long long row, int col, float (&gv)[8], float (&uv)[8], const float* first) {
+// ... of gate | up: `first` has the first plane's eight gate columns and, 16 further, their up columns.  (The fast exponential is off by 2 + 1.2 |g| units of 2^-23 and
+// the fast quotient by two: far below half a step of bf16, 2^-9.)
+__device__ __forceinline__ void lora_gated(const LoraParams& p, void* out, long long row, int col, float (&gv)[8], float (&uv)[8], const float* first) {
   lora_add4(gv, *reinterpret_cast<const float4*>(first));
   lora_add4(gv + 4, *reinterpret_cast<const float4*>(first + 4));
   lora_add4(uv, *reinterpret_cast<const float4*>(first + 16));
   lora_add4(uv + 4, *reinterpret_cast<const float4*>(first + 20));
-  for (int z = 1; z < p.splits; ++z) {
-    const float* more = p.planes + (static_cast<long long>(z) * p.T + row) * p.width + (col >> 4) * 32 + (col & 15);
-    lora_add4(gv, *reinterpret_cast<const float4*>(more));
-    lora_add4(gv + 4, *reinterpret_cast<const float4*>(more + 4));
-    lora_add4(uv, *reinterpret_cast<const float4*>(more + 16));
-    lora_add4(uv + 4, *reinterpret_cast<const float4*>(more + 20));
-  }
-  float y[8];
+  if (p.splits > 1)
+#pragma unroll 1
+    for (int z = 1; z < p.splits; ++z) {
+      const float* more = p.planes + (static_cast<long long>(z) * p.T + row) * p.width + (col >> 4) * 32 + (col & 15);
+      lora_add4(gv, *reinterpret_cast<const float4*>(more));
+      lora_add4(gv + 4, *reinterpret_cast<const float4*>(more + 4));
+      lora_add4(uv, *reinterpret_cast<const float4*>(more + 16));
+      lora_add4(uv + 4, *reinterpret_cast<const float4*>(more + 20));
+    }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) y[i] = gv[i] / (1.f + expf(-gv[i])) * uv[i];
-  const long long to = p.xt_rows ? static_cast<long long>(xt_index(static_cast<int>(row), col, p.xt_rows, p.xt_kb)) : row * p.ldo + col;
-  *reinterpret_cast<uint4*>(static_cast<__nv_bfloat16*>(p.out) + to) = lora_round(y);
+  for (int i = 0; i < 8; ++i) gv[i] = __fdividef(gv[i], 1.f + __expf(-gv[i])) * uv[i];
+  *static_cast<uint4*>(out) = lora_round(gv);
+}
+// where column `col` of a row's results stands
+template <int OUT>
+__device__ __forceinline__ void* lora_place(const LoraParams& p, long long row, int col) {
+  if constexpr (OUT == LORA_F32) return static_cast<float*>(p.out) + row * p.ldo + col;
+  if (OUT == LORA_GLU && p.xt_rows) return static_cast<__nv_bfloat16*>(p.out) + xt_index(static_cast<int>(row), col, p.xt_rows, p.xt_kb);
+  return static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + col;
 }
 template <int OUT>
 __host__ __device__ constexpr int lora_parts() { return OUT == LORA_F32 ? 3 : 2; }
@@ -313,7 +359,7 @@ __host__ __device__ constexpr int lora_parts() { return OUT == LORA_F32 ? 3 : 2;
 template <int OUT>
 __host__ __device__ constexpr int lora_row_bytes() { return OUT == LORA_GLU ? 256 : OUT == LORA_F32 ? 128 : 64; }      // of a column block in base or planes
 template <int KS, int OUT>
-__global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_kernel(const LoraParams p) {
+__global__ void __launch_bounds__(LORA_THREADS, KS == 8 || OUT == LORA_GLU ? 2 : 3) lora_up_kernel(const LoraParams p) {
   extern __shared__ __align__(128) uint8_t smem8[];
   constexpr int PARTS = lora_parts<OUT>(), B_BYTES = KS * 1024 * (OUT == LORA_GLU ? 2 : 1), SEG = lora_row_bytes<OUT>();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
@@ -333,26 +379,32 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_kernel(const LoraPara
     const uint4* b = p.b + tl.x * p.b_slot + static_cast<long long>(c0) * KS * 64;
     const int half = nb * KS * 64;
     for (int i = tid; i < half; i += LORA_THREADS) {
-      cp_async16(smem_u32(bs) + i * 16, b + i, true);
-      if (OUT == LORA_GLU) cp_async16(smem_u32(bs) + (half + i) * 16, b + static_cast<long long>(p.blocks) * KS * 64 + i, true);       // (the up columns' blocks follow the gate's)
+      cp_async16(smem_u32(bs) + i * 16, b + i, 16);
+      if (OUT == LORA_GLU) cp_async16(smem_u32(bs) + (half + i) * 16, b + static_cast<long long>(p.blocks) * KS * 64 + i, 16);       // (the up columns' blocks follow the gate's)
     }
   }
   // (base and planes: columns of a block are neighbours, but blocks of different slices may not be)
   if (OUT == LORA_GLU || p.base) {
     constexpr int PER = SEG / 16;
-    for (int i = tid; i < n * nb * PER; i += LORA_THREADS) {
-      const int r = i / (nb * PER), k = i - r * nb * PER, c = c0 + k / PER, q = k % PER;
-      const long long row = rec[4 + r];
+    for (int k = lane; k < nb * PER; k += 32) {
+      const int c = c0 + k / PER, q = k % PER;
+      long long at;
+      bool in;
       if constexpr (OUT == LORA_GLU) {
-        const bool in = c * 64 + q * 4 < 2 * ((p.ff + 15) & ~15);
-        cp_async16(smem_u32(rows) + r * ld_rows + k * 16, p.planes + row * p.width + (in ? c * 64 + q * 4 : 0), in);
+        at = c * 64 + q * 4;
+        in = at < 2 * ((p.ff + 15) & ~15);
       } else {
         int s = 0;
         while (c >= p.block0[s + 1]) ++s;
-        const int col = p.col0[s] + (c - p.block0[s]) * 32 + q * (OUT == LORA_F32 ? 4 : 8);
-        const bool in = col < p.col0[s + 1];
-        cp_async16(smem_u32(rows) + r * ld_rows + k * 16, static_cast<const uint8_t*>(p.base) + (row * p.ld_base + (in ? col : 0)) * (OUT == LORA_F32 ? 4 : 2), in);
+        at = p.col0[s] + (c - p.block0[s]) * 32 + q * (OUT == LORA_F32 ? 4 : 8);
+        in = at < p.col0[s + 1];
       }
+      const uint8_t* from = static_cast<const uint8_t*>(OUT == LORA_GLU ? p.planes : p.base) + (in ? at : 0) * (OUT == LORA_BF16 ? 2 : 4);
+      const long long ld = (OUT == LORA_GLU ? p.width : p.ld_base) * (OUT == LORA_BF16 ? 2 : 4);
+      const uint32_t to = smem_u32(rows) + k * 16;
+      const int bytes = in ? 16 : 0;
+#pragma unroll 4
+      for (int r = warp; r < n; r += 8) cp_async16(to + r * ld_rows, from + rec[4 + r] * ld, bytes);
     }
   }
   const int m_tiles = need == 3 ? 4 : need, mt = warp & (m_tiles - 1), step = 8 / m_tiles;
@@ -361,42 +413,38 @@ __global__ void __launch_bounds__(LORA_THREADS, 2) lora_up_kernel(const LoraPara
   pdl_sync();
   if (has) {
     const uint4* v = reinterpret_cast<const uint4*>(p.v) + static_cast<long long>(blockIdx.x) * (p.tile_rows >> 4) * p.slices * PARTS * KS * 32;
-    for (int i = tid; i < v_bytes / 16; i += LORA_THREADS) cp_async16(smem_u32(smem8) + i * 16, v + i, true);
+    for (int i = tid; i < v_bytes / 16; i += LORA_THREADS) cp_async16(smem_u32(smem8) + i * 16, v + i, 16);
   }
   cp_async_commit();
   cp_async_wait<0>();
   __syncthreads();
   if (mt >= need) return;
-  const uint4* frags = reinterpret_cast<const uint4*>(smem8) + mt * p.slices * PARTS * KS * 32 + lane;
-  const uint4* bw = reinterpret_cast<const uint4*>(bs) + lane;
-  for (int c = c0 + warp / m_tiles; c < c1; c += step) {
-    int s = 0;
+  const uint32_t frags = smem_u32(smem8) + (mt * p.slices * PARTS * KS * 32 + lane) * 16, bw = smem_u32(bs) + lane * 16;
+  const uint8_t* from[2] = {rows + ra * ld_rows + (OUT == LORA_GLU ? (t4 >> 1) * 128 + (t4 & 1) * 32 : t4 * (SEG / 4)), nullptr};
+  from[1] = from[0] + 8 * ld_rows;
+  const long long row[2] = {row_a, row_b};
+  for (int c = c0 + warp / m_tiles, s = 0; c < c1; c += step) {
     while (OUT != LORA_GLU && c >= p.block0[s + 1]) ++s;
     float d[4][4] = {}, u[4][4] = {};
     if (has) {
-      uint4 w[KS][2];
-      lora_take<KS, false>(w, bw + (c - c0) * KS * 64);
-      lora_block<KS, PARTS>(d, frags + s * PARTS * KS * 32, w);
-      if constexpr (OUT == LORA_GLU) {
-        lora_take<KS, false>(w, bw + (nb + c - c0) * KS * 64);
-        lora_block<KS, PARTS>(u, frags + PARTS * KS * 32, w);
-      }
+      lora_product<KS, PARTS>(d, frags + s * PARTS * KS * 512, bw + (c - c0) * KS * 1024);
+      if constexpr (OUT == LORA_GLU) lora_product<KS, PARTS>(u, frags + PARTS * KS * 512, bw + (nb + c - c0) * KS * 1024);
     }
     const int col = p.col0[s] + (c - p.block0[s]) * 32 + t4 * 8;
     if (col >= p.col0[s + 1]) continue;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const long long row = h ? row_b : row_a;
-      if (row < 0) continue;
-      const uint8_t* from = rows + (h ? rb : ra) * ld_rows + (c - c0) * SEG;
+      if (row[h] < 0) continue;
       float y[8], z[8];
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         y[i] = d[i >> 1][h * 2 + (i & 1)];
         z[i] = u[i >> 1][h * 2 + (i & 1)];
       }
-      if constexpr (OUT == LORA_GLU) lora_gated(p, row, col, y, z, reinterpret_cast<const float*>(from) + (t4 >> 1) * 32 + (t4 & 1) * 8);
-      else lora_result<OUT>(p, row, col, y, p.base ? from + t4 * (SEG / 4) : nullptr);
+      void* out = lora_place<OUT>(p, row[h], col);
+      const uint8_t* add = from[h] + (c - c0) * SEG;
+      if constexpr (OUT == LORA_GLU) lora_gated(p, out, row[h], col, y, z, reinterpret_cast<const float*>(add));
+      else lora_result<OUT>(out, y, p.base ? add : nullptr);
     }
   }
 }
@@ -477,7 +525,7 @@ __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams
         mine[c * p.VR + (rt0 + i) * 16 + r] = c < n ? scale * s : 0.f;
       }
     }
-    if (first < c1) lora_take<KS, true>(w, b + static_cast<long long>(first) * KS * 64);         // (on its way while the cluster meets)
+    if (first < c1) lora_take<KS>(w, b + static_cast<long long>(first) * KS * 64);         // (on its way while the cluster meets)
     cluster_sync_all();
     const int quads = p.VR >> 2;
     for (int e = tid; e < 16 * quads; e += LORA_THREADS) {
@@ -520,10 +568,10 @@ __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams
     if (has) {
       lora_block<KS, PARTS>(d, fr + s * PARTS * KS * 32, w);
       if constexpr (OUT == LORA_GLU) {
-        lora_take<KS, true>(w, b + static_cast<long long>(p.blocks + c) * KS * 64);
+        lora_take<KS>(w, b + static_cast<long long>(p.blocks + c) * KS * 64);
         lora_block<KS, PARTS>(u, fr + PARTS * KS * 32, w);
       }
-      if (c + 8 < c1) lora_take<KS, true>(w, b + static_cast<long long>(c + 8) * KS * 64);
+      if (c + 8 < c1) lora_take<KS>(w, b + static_cast<long long>(c + 8) * KS * 64);
     }
     if (!in) continue;
 #pragma unroll
@@ -535,8 +583,9 @@ __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams
         y[i] = d[i >> 1][h * 2 + (i & 1)];
         z[i] = u[i >> 1][h * 2 + (i & 1)];
       }
-      if constexpr (OUT == LORA_GLU) lora_gated(p, rows[h], col, y, z, reinterpret_cast<const float*>(&add[h][0]));
-      else lora_result<OUT>(p, rows[h], col, y, p.base ? static_cast<const void*>(&add[h][0]) : nullptr);
+      void* out = lora_place<OUT>(p, rows[h], col);
+      if constexpr (OUT == LORA_GLU) lora_gated(p, out, rows[h], col, y, z, reinterpret_cast<const float*>(&add[h][0]));
+      else lora_result<OUT>(out, y, p.base ? static_cast<const void*>(&add[h][0]) : nullptr);
     }
   }
   __syncwarp();
@@ -554,7 +603,7 @@ static int lora_tiles(int T, int slots) {
 }
 static int lora_k_split(int T, int K, int slots, int VR) {
   const int stages = (K + LORA_STAGE_K - 1) / LORA_STAGE_K, tiles = lora_tiles(T, slots);
-  int split = ((VR > 32 ? 1 : 2) * sm_count() + tiles / 2) / tiles;       // the blocks that fit at a time
+  int split = ((VR > 64 ? 1 : 2) * sm_count() + tiles / 2) / tiles;       // the blocks that fit at a time
   const int most = stages > 2 ? stages / 2 : 1;                           // two stages a block
   if (split > most) split = most;
   return split < 1 ? 1 : split > 8 ? 8 : split;
@@ -563,15 +612,17 @@ static int lora_k_split(int T, int K, int slots, int VR) {
 static bool lora_few(const LoraParams& p) { return p.T <= 64 && p.VR <= LORA_FEW_RANKS && p.rank_tiles <= 4 && (p.a_slot + p.b_slot) * 16 <= 2 << 20; }
 
 template <int KS, int OUT>
-static int lora_up_launch(LoraParams& p, int max_tiles, void* stream) {
-  VB_CHECK_CUDA(max_dyn_smem_once(lora_up_kernel<KS, OUT>));
+static int lora_up_launch(LoraParams& p, int max_tiles, int tiles, void* stream) {
+  VB_CHECK_CUDA((rm_smem<lora_up_kernel<KS, OUT>>()));
   const int v_bytes = (p.tile_rows >> 4) * p.slices * lora_parts<OUT>() * KS * 512;
   const int block_bytes = KS * 1024 * (OUT == LORA_GLU ? 2 : 1) + p.tile_rows * (OUT == LORA_GLU || p.base ? lora_row_bytes<OUT>() : 0);
-  // columns a block: about 48 KB beside v (two warps deep in columns at least), so that several blocks share an SM
-  int per = (48 * 1024) / block_bytes;
-  const int least = p.tile_rows == 16 ? 8 : 2;
+  // columns a block: what three blocks an SM (of gate | up: two) hold beside v at a time, in even waves
+  const long long work = static_cast<long long>(tiles) * p.blocks, slots = (OUT == LORA_GLU ? 2 : 3) * sm_count(),
+                  share = (OUT == LORA_GLU ? 90 : 66) * 1024, room = share - v_bytes > 16 * 1024 ? share - v_bytes : 16 * 1024;
+  const long long waves = (work * block_bytes + slots * room - 1) / (slots * room);
+  int per = static_cast<int>((work + slots * waves - 1) / (slots * waves));
+  const int least = p.tile_rows == 16 ? 8 : 2;         // a column block for every warp
   if (per < least) per = least;
-  if (per > 16) per = 16;
   if (per > p.blocks) per = p.blocks;
   size_t smem;
   while ((smem = static_cast<size_t>(v_bytes) + static_cast<size_t>(per) * block_bytes + p.tile_rows * 16) > VB_MAX_DYN_SMEM && per > 1) --per;      // (one fits always)
@@ -581,7 +632,7 @@ static int lora_up_launch(LoraParams& p, int max_tiles, void* stream) {
 }
 template <int RT>
 static int lora_down_launch(const LoraParams& p, int max_tiles, void* stream) {
-  VB_CHECK_CUDA(max_dyn_smem_once(lora_down_kernel<RT>));
+  VB_CHECK_CUDA((rm_smem<lora_down_kernel<RT>>()));
   VB_CHECK_CUDA(launch_kernel_cluster3(lora_down_kernel<RT>, dim3(max_tiles, p.k_split), dim3(LORA_THREADS), LoraDown<RT>::SMEM, static_cast<cudaStream_t>(stream), true,
                                        dim3(1, p.k_split, 1), p));
   return 0;
@@ -609,53 +660,58 @@ static int lora_launch(LoraParams& p, int slots, void* stream) {
                               : lora_down_launch<8>(p, max_tiles, stream);
   if (rc) return rc;
   switch (p.rank_tiles) {
-    case 1: return lora_up_launch<1, OUT>(p, max_tiles, stream);
-    case 2: return lora_up_launch<2, OUT>(p, max_tiles, stream);
-    case 4: return lora_up_launch<4, OUT>(p, max_tiles, stream);
-    default: return lora_up_launch<8, OUT>(p, max_tiles, stream);
+    case 1: return lora_up_launch<1, OUT>(p, max_tiles, lora_tiles(p.T, slots), stream);
+    case 2: return lora_up_launch<2, OUT>(p, max_tiles, lora_tiles(p.T, slots), stream);
+    case 4: return lora_up_launch<4, OUT>(p, max_tiles, lora_tiles(p.T, slots), stream);
+    default: return lora_up_launch<8, OUT>(p, max_tiles, lora_tiles(p.T, slots), stream);
   }
 }
-// v of every tile in three parts
-static size_t lora_ws_bytes(int T, int slots, int rank, int slices) {
-  return static_cast<size_t>(lora_max_tiles(T, slots)) * (lora_tile_rows(T) / 16) * slices * (rank / 16) * 3 * 512;
-}
-
 // checks and fills what both entry points share
-static int lora_setup(const char* who, LoraParams& p, const void* d_x, long long ldx, const void* d_a, const void* d_b, const float* d_scale, int slots,
-                      int rank, const int32_t* widths, int slices, const void* d_tiles, int T, int K, void* d_ws, size_t ws_bytes) {
-  VB_CHECK_ARG(d_x && d_a && d_b && d_scale && d_tiles && widths && d_ws, "%s: null pointer", who);
-  VB_CHECK_ARG(slots >= 1 && slots <= LORA_MAX_SLOTS, "%s: %d adapters; 1 to %d", who, slots, LORA_MAX_SLOTS);
-  VB_CHECK_ARG(rank == 16 || rank == 32 || rank == 64 || rank == 128, "%s: padded rank %d must be 16, 32, 64 or 128", who, rank);
-  VB_CHECK_ARG(slices >= 1 && slices <= LORA_MAX_SLICES, "%s: %d slices; 1 to %d", who, slices, LORA_MAX_SLICES);
-  VB_CHECK_ARG(K >= 8 && K % 8 == 0 && ldx % 8 == 0 && ldx >= K && reinterpret_cast<uintptr_t>(d_x) % 16 == 0,
-               "%s: rows of x must be multiples of 8 elements, 16-byte aligned (K %d, row stride %lld)", who, K, ldx);
-  p.slices = slices;
+static int lora_bank(const char* who, LoraParams& p, const VbLoraBank* bank, int T) {
+  VB_CHECK_ARG(bank && bank->d_a && bank->d_b && bank->d_scale, "%s: null pointer", who);
+  VB_CHECK_ARG(bank->slots >= 1 && bank->slots <= LORA_MAX_SLOTS, "%s: %d adapters; 1 to %d", who, bank->slots, LORA_MAX_SLOTS);
+  VB_CHECK_ARG(bank->rank == 16 || bank->rank == 32 || bank->rank == 64 || bank->rank == 128, "%s: padded rank %d must be 16, 32, 64 or 128", who, bank->rank);
+  VB_CHECK_ARG(bank->slices >= 1 && bank->slices <= LORA_MAX_SLICES, "%s: %d slices; 1 to %d", who, bank->slices, LORA_MAX_SLICES);
+  VB_CHECK_ARG(bank->K >= 8 && bank->K % 8 == 0, "%s: inputs of %d; a multiple of 8", who, bank->K);
+  p.slices = bank->slices;
   p.block0[0] = p.col0[0] = 0;
-  for (int s = 0; s < slices; ++s) {
-    VB_CHECK_ARG(widths[s] >= 8 && widths[s] % 8 == 0 && widths[s] <= (1 << 24), "%s: slice of %d columns; a multiple of 8", who, widths[s]);
-    p.block0[s + 1] = p.block0[s] + (widths[s] + 31) / 32;
-    p.col0[s + 1] = p.col0[s] + widths[s];
+  for (int s = 0; s < p.slices; ++s) {
+    const int w = bank->widths[s];
+    VB_CHECK_ARG(w >= 8 && w % 8 == 0 && w <= (1 << 24), "%s: slice of %d columns; a multiple of 8", who, w);
+    p.block0[s + 1] = p.block0[s] + (w + 31) / 32;
+    p.col0[s + 1] = p.col0[s] + w;
   }
-  p.tiles = static_cast<const int32_t*>(d_tiles);
   p.tile_rows = lora_tile_rows(T);
+  p.a = static_cast<const uint4*>(bank->d_a);
+  p.b = static_cast<const uint4*>(bank->d_b);
+  p.scale = bank->d_scale;
+  p.T = T;
+  p.K = bank->K;
+  p.kb32 = (p.K + 31) / 32;
+  p.rank_tiles = bank->rank / 16;
+  p.VR = p.slices * bank->rank;
+  p.a_slot = static_cast<long long>(p.VR / 16) * p.kb32 * 64;
+  p.b_slot = static_cast<long long>(p.block0[p.slices]) * p.rank_tiles * 64;
+  p.blocks = p.block0[p.slices];
+  p.k_split = lora_k_split(T, p.K, bank->slots, p.VR);
+  return 0;
+}
+// v of every tile in three parts; none where one launch does both products
+static size_t lora_ws_bytes(const LoraParams& p, int slots) {
+  return lora_few(p) ? 0 : static_cast<size_t>(lora_max_tiles(p.T, slots)) * (p.tile_rows / 16) * (p.VR / 16) * 3 * 512;
+}
+static int lora_setup(const char* who, LoraParams& p, const void* d_x, long long ldx, const VbLoraBank* bank, const void* d_tiles, int T, void* d_ws, size_t ws_bytes) {
+  const int rc = lora_bank(who, p, bank, T);
+  if (rc) return rc;
+  VB_CHECK_ARG(d_x && d_tiles, "%s: null pointer", who);
+  VB_CHECK_ARG(ldx % 8 == 0 && ldx >= p.K && reinterpret_cast<uintptr_t>(d_x) % 16 == 0, "%s: rows of x must be 16-byte aligned (K %d, row stride %lld)", who, p.K, ldx);
+  p.tiles = static_cast<const int32_t*>(d_tiles);
   p.x = static_cast<const __nv_bfloat16*>(d_x);
   p.ldx = ldx;
-  p.a = static_cast<const uint4*>(d_a);
-  p.b = static_cast<const uint4*>(d_b);
-  p.scale = d_scale;
-  p.T = T;
-  p.K = K;
-  p.kb32 = (K + 31) / 32;
-  p.rank_tiles = rank / 16;
-  p.VR = slices * rank;
-  p.a_slot = static_cast<long long>(p.VR / 16) * p.kb32 * 64;
-  p.b_slot = static_cast<long long>(p.block0[slices]) * p.rank_tiles * 64;
-  p.blocks = p.block0[slices];
-  p.k_split = lora_k_split(T, K, slots, p.VR);
   p.v = static_cast<uint32_t*>(d_ws);
-  const size_t need = lora_ws_bytes(T, slots, rank, slices);
-  VB_CHECK_ARG(ws_bytes >= need && reinterpret_cast<uintptr_t>(d_ws) % 16 == 0, "%s: workspace of %zu bytes, 16-byte aligned, is needed (%zu given)", who, need,
-               ws_bytes);
+  const size_t need = lora_ws_bytes(p, bank->slots);
+  VB_CHECK_ARG(need == 0 || (d_ws && ws_bytes >= need && reinterpret_cast<uintptr_t>(d_ws) % 16 == 0), "%s: workspace of %zu bytes, 16-byte aligned, is needed (%zu given)",
+               who, need, ws_bytes);
   return 0;
 }
 
@@ -678,37 +734,39 @@ int vb_lora_plan(void* d_tiles, const int32_t* d_ids, int T, int slots, void* st
   return 0;
 }
 
-size_t vb_lora_workspace_bytes(int T, int slots, int rank, int slices) { return T < 1 || slots < 1 ? 0 : lora_ws_bytes(T, slots, rank, slices); }
+size_t vb_lora_workspace_bytes(const VbLoraBank* bank, int T) {
+  LoraParams p = {};
+  return T < 1 || lora_bank("vb_lora_workspace_bytes", p, bank, T) ? 0 : lora_ws_bytes(p, bank->slots);
+}
 
-int vb_lora(void* d_out, long long ld_out, const void* d_base, long long ld_base, int out_f32, const void* d_x, long long ldx, const void* d_a, const void* d_b,
-            const float* d_scale, int slots, int rank, const int32_t* widths, int slices, const void* d_tiles, int T, int K, void* d_ws, size_t ws_bytes,
-            void* stream) {
+int vb_lora(void* d_out, long long ld_out, const void* d_base, long long ld_base, int out_f32, const void* d_x, long long ldx, const VbLoraBank* bank,
+            const void* d_tiles, int T, void* d_ws, size_t ws_bytes, void* stream) {
   VB_CHECK_ARG(d_out, "vb_lora: null pointer");
   if (T <= 0) return 0;
   LoraParams p = {};
-  const int rc = lora_setup("vb_lora", p, d_x, ldx, d_a, d_b, d_scale, slots, rank, widths, slices, d_tiles, T, K, d_ws, ws_bytes);
+  const int rc = lora_setup("vb_lora", p, d_x, ldx, bank, d_tiles, T, d_ws, ws_bytes);
   if (rc) return rc;
-  const int unit = out_f32 ? 4 : 8;
-  VB_CHECK_ARG(ld_out % unit == 0 && ld_out >= p.col0[slices] && reinterpret_cast<uintptr_t>(d_out) % 16 == 0 &&
-                   (!d_base || (ld_base % unit == 0 && ld_base >= p.col0[slices] && reinterpret_cast<uintptr_t>(d_base) % 16 == 0)),
-               "vb_lora: rows of out and base must be 16-byte aligned and at least %d columns apart", p.col0[slices]);
+  const int unit = out_f32 ? 4 : 8, N = p.col0[p.slices];
+  VB_CHECK_ARG(ld_out % unit == 0 && ld_out >= N && reinterpret_cast<uintptr_t>(d_out) % 16 == 0 &&
+                   (!d_base || (ld_base % unit == 0 && ld_base >= N && reinterpret_cast<uintptr_t>(d_base) % 16 == 0)),
+               "vb_lora: rows of out and base must be 16-byte aligned and at least %d columns apart", N);
   p.out = d_out;
   p.ldo = ld_out;
   p.base = d_base;
   p.ld_base = ld_base;
-  return out_f32 ? lora_launch<LORA_F32>(p, slots, stream) : lora_launch<LORA_BF16>(p, slots, stream);
+  return out_f32 ? lora_launch<LORA_F32>(p, bank->slots, stream) : lora_launch<LORA_BF16>(p, bank->slots, stream);
 }
 
-int vb_lora_gate_up(void* d_act, long long ld_act, int xt_rows, const float* d_planes, int splits, int half, int ff, const void* d_x, long long ldx,
-                    const void* d_a, const void* d_b, const float* d_scale, int slots, int rank, const void* d_tiles, int T, int K, void* d_ws,
-                    size_t ws_bytes, void* stream) {
+int vb_lora_gate_up(void* d_act, long long ld_act, int xt_rows, const float* d_planes, int splits, int half, const void* d_x, long long ldx, const VbLoraBank* bank,
+                    const void* d_tiles, int T, void* d_ws, size_t ws_bytes, void* stream) {
   VB_CHECK_ARG(d_act && d_planes, "vb_lora_gate_up: null pointer");
   VB_CHECK_ARG(splits >= 1 && half >= 16 && half % 16 == 0 && half <= 64, "vb_lora_gate_up: %d planes, tiles of %d gate rows (16, 32, 48 or 64)", splits, half);
   if (T <= 0) return 0;
   LoraParams p = {};
-  const int32_t widths[2] = {ff, ff};
-  const int rc = lora_setup("vb_lora_gate_up", p, d_x, ldx, d_a, d_b, d_scale, slots, rank, widths, 2, d_tiles, T, K, d_ws, ws_bytes);
+  const int rc = lora_setup("vb_lora_gate_up", p, d_x, ldx, bank, d_tiles, T, d_ws, ws_bytes);
   if (rc) return rc;
+  const int ff = p.col0[1];
+  VB_CHECK_ARG(p.slices == 2 && p.col0[2] == 2 * ff, "vb_lora_gate_up: a bank of two slices of equal width is needed");
   VB_CHECK_ARG(xt_rows >= 0 && reinterpret_cast<uintptr_t>(d_act) % 16 == 0 && reinterpret_cast<uintptr_t>(d_planes) % 16 == 0 &&
                    (xt_rows > 0 || (ld_act % 8 == 0 && ld_act >= ff)),
                "vb_lora_gate_up: rows of act must be 16-byte aligned and at least %d columns apart", ff);
@@ -716,12 +774,11 @@ int vb_lora_gate_up(void* d_act, long long ld_act, int xt_rows, const float* d_p
   p.ldo = ld_act;
   p.planes = d_planes;
   p.splits = splits;
-  p.half = half;
   p.ff = ff;
   p.width = (ff + half - 1) / half * 2 * half;
   p.xt_rows = xt_rows;
   p.xt_kb = (ff + 63) / 64;
-  return lora_launch<LORA_GLU>(p, slots, stream);
+  return lora_launch<LORA_GLU>(p, bank->slots, stream);
 }
 
 }  // extern "C"

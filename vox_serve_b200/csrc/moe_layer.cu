@@ -71,7 +71,7 @@ __device__ __forceinline__ void st_dsmem_f32(const float* local_ptr, uint32_t ct
 // the kernel in front).  Every logit goes into the shared memory of the block that its row belongs to.  Then each block picks one row's experts: an
 // expert's place is the number of those in front of it, which all threads count at once.
 __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const MoeRouteParams p) {
-  extern __shared__ __align__(16) int smem[];
+  extern __shared__ __align__(128) int smem[];
   constexpr int THREADS = ML_ROUTE_THREADS, WARPS = THREADS / 32, AHEAD = 4;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int rank = blockIdx.x % ML_ROUTE_CLUSTER, t0 = blockIdx.x / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER, rows = min(ML_ROUTE_CLUSTER, p.T - t0);
@@ -872,78 +872,67 @@ extern "C" {
 
 int vb_moe_layer_max_rows(void) { return ML_MAX_ROWS; }
 
-size_t vb_moe_layer_workspace_bytes(int T, int top, int ff, int sff) {
-  if (T < 1 || top < 1 || ff < 1 || sff < 0) return 0;
-  return 3 * ml_act_elems(T, top, ff, sff) * sizeof(__nv_bfloat16);
+// idx, weights and the shared expert's gates of every row, then the activations
+static size_t ml_head_bytes(int T, int top) { return (static_cast<size_t>(T) * (2 * top + 1) * 4 + 15) / 16 * 16; }
+size_t vb_moe_layer_workspace_bytes(const VbMoeWeights* weights, const VbMoeRouter* router, int T) {
+  if (!weights || !router || T < 1 || router->top < 1 || weights->ff < 1 || weights->shared_ff < 0) return 0;
+  return ml_head_bytes(T, router->top) + 3 * ml_act_elems(T, router->top, weights->ff, weights->shared_ff) * sizeof(__nv_bfloat16);
 }
 
-int vb_moe_layer_route(int32_t* d_idx, float* d_wts, float* d_shared_gate, int kind, const void* d_h, long long ldh, const float* d_router_w, const float* d_bias,
-                       const float* d_shared_gate_w, const int32_t* d_ids, const int32_t* d_table, int T, int W, int experts, int top, int groups, int keep,
-                       int vocab, void* stream) {
-  VB_CHECK_ARG(kind >= 0 && kind <= 3, "vb_moe_layer_route: kind %d", kind);
-  VB_CHECK_ARG(d_idx && d_wts && d_h && (kind == ML_TABLE ? d_ids && d_table && vocab > 0 : d_router_w != nullptr), "vb_moe_layer_route: null pointer");
-  VB_CHECK_ARG(experts >= 1 && experts <= ML_MAX_EXPERTS && top >= 1 && top <= ML_MAX_TOP && top <= experts, "vb_moe_layer_route: %d experts (1 to %d), top %d (1 to %d)",
-               experts, ML_MAX_EXPERTS, top, ML_MAX_TOP);
-  VB_CHECK_ARG(W >= 8 && W % 8 == 0 && ldh % 8 == 0 && ldh >= W && reinterpret_cast<uintptr_t>(d_h) % 16 == 0 &&
-                   reinterpret_cast<uintptr_t>(d_router_w) % 16 == 0 && reinterpret_cast<uintptr_t>(d_shared_gate_w) % 16 == 0,
-               "vb_moe_layer_route: rows must be multiples of 8 elements, 16-byte aligned (width %d)", W);
-  VB_CHECK_ARG(groups <= 1 || ((kind == ML_SIGMOID || kind == ML_SOFTMAX_ALL) && experts % groups == 0 && keep >= 1 && keep <= groups && keep * (experts / groups) >= top),
-               "vb_moe_layer_route: %d groups (keep %d) do not fit %d experts, top %d", groups, keep, experts, top);
-  VB_CHECK_ARG(!d_shared_gate_w || d_shared_gate, "vb_moe_layer_route: the shared gate needs an output");
-  VB_CHECK_ARG(T <= ML_MAX_ROWS, "vb_moe_layer_route: %d rows; at most %d", T, ML_MAX_ROWS);
-  if (T <= 0) return 0;
-  MoeRouteParams p = {};
-  p.idx = d_idx;
-  p.wts = d_wts;
-  p.sgate = d_shared_gate;
-  p.h = static_cast<const __nv_bfloat16*>(d_h);
-  p.ldh = ldh;
-  p.w = d_router_w;
-  p.bias = d_bias;
-  p.wsg = d_shared_gate_w;
-  p.ids = d_ids;
-  p.table = d_table;
-  p.T = T;
-  p.W = W;
-  p.E = experts;
-  p.top = top;
-  p.kind = kind;
-  p.groups = groups > 0 ? groups : 0;
-  p.keep = keep;
-  p.vocab = vocab;
-  const size_t smem = (static_cast<size_t>(ML_ROUTE_THREADS / 32 * 16) * ML_ROUTE_CLUSTER + 2 * static_cast<size_t>(experts) + (groups > 0 ? groups : 0) + 48) * 4;
-  VB_LAUNCH_PDL_CLUSTER(moe_layer_route_kernel, (T + ML_ROUTE_CLUSTER - 1) / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER, ML_ROUTE_THREADS, smem, stream, ML_ROUTE_CLUSTER, p);
-  return 0;
-}
-
-int vb_moe_layer_experts(float* d_y, long long ldy, const void* d_h, long long ldh, const void* d_up, const void* d_down, const int32_t* d_idx, const float* d_wts,
-                         const float* d_shared_gate, int T, int W, int experts, int top, int ff, int shared_ff, int up_rows, int act, float limit, float slope,
-                         void* d_ws, size_t ws_bytes, void* stream) {
-  VB_CHECK_ARG(d_y && d_h && d_up && d_down && d_idx && d_wts && d_ws, "vb_moe_layer_experts: null pointer");
-  VB_CHECK_ARG(T <= ML_MAX_ROWS, "vb_moe_layer_experts: %d rows; at most %d", T, ML_MAX_ROWS);
-  VB_CHECK_ARG(experts >= 1 && experts <= ML_MAX_EXPERTS && top >= 1 && top <= ML_MAX_TOP, "vb_moe_layer_experts: %d experts (1 to %d), top %d (1 to %d)", experts,
+int vb_moe_layer(float* d_y, long long ldy, const void* d_h, long long ldh, const VbMoeWeights* weights, const VbMoeRouter* router, const int32_t* d_ids, int T,
+                 void* d_ws, size_t ws_bytes, void* stream) {
+  VB_CHECK_ARG(d_y && d_h && weights && router && weights->d_up && weights->d_down && d_ws, "vb_moe_layer: null pointer");
+  const int W = weights->width, experts = weights->experts, ff = weights->ff, shared_ff = weights->shared_ff, up_rows = weights->up_rows, act = weights->act;
+  const int kind = router->kind, top = router->top, groups = router->groups > 0 ? router->groups : 0, keep = router->keep;
+  VB_CHECK_ARG(T <= ML_MAX_ROWS, "vb_moe_layer: %d rows; at most %d", T, ML_MAX_ROWS);
+  VB_CHECK_ARG(experts >= 1 && experts <= ML_MAX_EXPERTS && top >= 1 && top <= ML_MAX_TOP && top <= experts, "vb_moe_layer: %d experts (1 to %d), top %d (1 to %d)", experts,
                ML_MAX_EXPERTS, top, ML_MAX_TOP);
-  VB_CHECK_ARG(W >= 8 && W % 8 == 0 && ldh % 8 == 0 && ldh >= W && ldy >= W && reinterpret_cast<uintptr_t>(d_h) % 16 == 0,
-               "vb_moe_layer_experts: rows of h must be multiples of 8 elements, 16-byte aligned (width %d)", W);
-  VB_CHECK_ARG(ff >= 64 && ff % 64 == 0 && shared_ff >= 0 && shared_ff % 64 == 0, "vb_moe_layer_experts: expert widths %d and %d must be multiples of 64", ff,
-               shared_ff);
-  VB_CHECK_ARG(act >= 0 && act <= 4 && (act != ML_CLAMPED_GLU || limit > 0.f), "vb_moe_layer_experts: activation %d, limit %f", act, limit);
+  VB_CHECK_ARG(kind >= 0 && kind <= 3, "vb_moe_layer: router %d", kind);
+  VB_CHECK_ARG(kind == ML_TABLE ? d_ids && router->d_table && router->vocab > 0 : router->d_weight != nullptr, "vb_moe_layer: the router lacks its matrix, or its table and ids");
+  VB_CHECK_ARG(W >= 8 && W % 8 == 0 && ldh % 8 == 0 && ldh >= W && ldy >= W && reinterpret_cast<uintptr_t>(d_h) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(router->d_weight) % 16 == 0 && reinterpret_cast<uintptr_t>(router->d_shared_gate) % 16 == 0,
+               "vb_moe_layer: rows must be multiples of 8 elements, 16-byte aligned (width %d)", W);
+  VB_CHECK_ARG(groups <= 1 || ((kind == ML_SIGMOID || kind == ML_SOFTMAX_ALL) && experts % groups == 0 && keep >= 1 && keep <= groups && keep * (experts / groups) >= top),
+               "vb_moe_layer: %d groups (keep %d) do not fit %d experts, top %d", groups, keep, experts, top);
+  VB_CHECK_ARG(ff >= 64 && ff % 64 == 0 && shared_ff >= 0 && shared_ff % 64 == 0, "vb_moe_layer: expert widths %d and %d must be multiples of 64", ff, shared_ff);
+  VB_CHECK_ARG(act >= 0 && act <= 4 && (act != ML_CLAMPED_GLU || weights->limit > 0.f), "vb_moe_layer: activation %d, limit %f", act, weights->limit);
   const bool gated = act <= ML_CLAMPED_GLU;
   VB_CHECK_ARG(up_rows >= 32 && up_rows <= 128 && up_rows % 32 == 0 && (gated ? 2 * ff : ff) % up_rows == 0 && (gated ? 2 * shared_ff : shared_ff) % up_rows == 0,
-               "vb_moe_layer_experts: tiles of %d rows do not divide the experts", up_rows);
-  VB_CHECK_ARG(!d_shared_gate || shared_ff > 0, "vb_moe_layer_experts: a gate without a shared expert");
-  VB_CHECK_ARG(ws_bytes >= vb_moe_layer_workspace_bytes(T < 1 ? 1 : T, top, ff, shared_ff) && reinterpret_cast<uintptr_t>(d_ws) % 16 == 0,
-               "vb_moe_layer_experts: workspace of %zu bytes is too small or not aligned", ws_bytes);
+               "vb_moe_layer: tiles of %d rows do not divide the experts", up_rows);
+  VB_CHECK_ARG(!router->d_shared_gate || shared_ff > 0, "vb_moe_layer: a gate without a shared expert");
   if (T <= 0) return 0;
+  VB_CHECK_ARG(ws_bytes >= vb_moe_layer_workspace_bytes(weights, router, T) && reinterpret_cast<uintptr_t>(d_ws) % 16 == 0,
+               "vb_moe_layer: workspace of %zu bytes is too small or not aligned", ws_bytes);
   MoeLayerParams p = {};
-  p.h = static_cast<const __nv_bfloat16*>(d_h);
+  int32_t* d_idx = static_cast<int32_t*>(d_ws);
+  float *d_wts = reinterpret_cast<float*>(d_idx + T * top), *d_gate = router->d_shared_gate ? d_wts + T * top : nullptr;
+  MoeRouteParams r = {};
+  r.idx = d_idx;
+  r.wts = d_wts;
+  r.sgate = d_gate;
+  r.h = static_cast<const __nv_bfloat16*>(d_h);
+  r.ldh = ldh;
+  r.w = router->d_weight;
+  r.bias = kind == ML_SOFTMAX || kind == ML_SIGMOID ? router->d_bias : nullptr;
+  r.wsg = router->d_shared_gate;
+  r.ids = d_ids;
+  r.table = router->d_table;
+  r.T = T;
+  r.W = W;
+  r.E = experts;
+  r.top = top;
+  r.kind = kind;
+  r.groups = groups;
+  r.keep = keep;
+  r.vocab = router->vocab;
+  p.h = r.h;
   p.ldh = ldh;
-  p.up = static_cast<const uint8_t*>(d_up);
-  p.down = static_cast<const uint8_t*>(d_down);
+  p.up = static_cast<const uint8_t*>(weights->d_up);
+  p.down = static_cast<const uint8_t*>(weights->d_down);
   p.idx = d_idx;
   p.wts = d_wts;
-  p.sgate = d_shared_gate;
-  p.act = static_cast<__nv_bfloat16*>(d_ws);
+  p.sgate = d_gate;
+  p.act = reinterpret_cast<__nv_bfloat16*>(static_cast<uint8_t*>(d_ws) + ml_head_bytes(T, top));
   p.y = d_y;
   p.ldy = ldy;
   p.T = T;
@@ -960,11 +949,13 @@ int vb_moe_layer_experts(float* d_y, long long ldy, const void* d_h, long long l
   p.expert_bytes = static_cast<long long>(gated ? 2 * ff : ff) * p.kb * 128;
   p.down_kb = (experts * ff + shared_ff) / 64;
   p.act_kind = act;
-  p.limit = limit;
-  p.slope = slope;
+  p.limit = weights->limit;
+  p.slope = weights->slope;
   p.up_units = (gated ? 2 * ff : ff) / 32;
   p.shared_units = (gated ? 2 * shared_ff : shared_ff) / 32;
-  VB_CHECK_ARG(p.wait_flag = wait_flag(WK_MOE_LAYER), "vb_moe_layer_experts: no mapped host memory");
+  VB_CHECK_ARG(p.wait_flag = wait_flag(WK_MOE_LAYER), "vb_moe_layer: no mapped host memory");
+  const size_t smem_route = (static_cast<size_t>(ML_ROUTE_THREADS / 32 * 16) * ML_ROUTE_CLUSTER + 2 * static_cast<size_t>(experts) + groups + 48) * 4;
+  VB_LAUNCH_PDL_CLUSTER(moe_layer_route_kernel, (T + ML_ROUTE_CLUSTER - 1) / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER, ML_ROUTE_THREADS, smem_route, stream, ML_ROUTE_CLUSTER, r);
   const int sms = sm_count();
   const long long most = static_cast<long long>(experts < T * top ? experts : T * top) * p.up_units + p.shared_units;
   const int grid_up = static_cast<int>(most < sms ? most : sms), nt = T <= 8 ? 1 : 4;
@@ -974,7 +965,7 @@ int vb_moe_layer_experts(float* d_y, long long ldy, const void* d_h, long long l
   const size_t smem_up = ml_ring_bytes(nt == 1 ? FEW : MANY) + static_cast<size_t>(2 * ML_WARPS) * 32 * (nt == 1 ? 8 : 40) * 4 + plan_bytes;
 #define ML_UP(NT, G, S)                                                              \
   do {                                                                               \
-    VB_CHECK_CUDA(max_dyn_smem_once(moe_up_kernel<NT, G, S>));                       \
+    VB_CHECK_CUDA((rm_smem<moe_up_kernel<NT, G, S>>()));                             \
     VB_LAUNCH_PDL((moe_up_kernel<NT, G, S>), grid_up, ML_THREADS, smem_up, stream, p); \
   } while (0)
   if (gated) {
@@ -992,7 +983,7 @@ int vb_moe_layer_experts(float* d_y, long long ldy, const void* d_h, long long l
   p.cluster = cluster;
 #define ML_DOWN(NT, S)                                                                                                  \
   do {                                                                                                                  \
-    VB_CHECK_CUDA(max_dyn_smem_once(moe_down_kernel<NT, S>));                                                           \
+    VB_CHECK_CUDA((rm_smem<moe_down_kernel<NT, S>>()));                                                                 \
     VB_LAUNCH_PDL_CLUSTER((moe_down_kernel<NT, S>), blocks * cluster, ML_THREADS, smem_down, stream, cluster, p);       \
   } while (0)
   if (nt == 1) ML_DOWN(1, FEW);

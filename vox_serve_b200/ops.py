@@ -1919,9 +1919,10 @@ class LoraBank:
         self.a = torch.zeros(slots, len(widths) * self.rank_pad * kb * 32, dtype=BF16, device=device)
         self.b = torch.zeros(slots, blocks * 32 * self.rank_pad, dtype=BF16, device=device)
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
-        self._widths = (ctypes.c_int32 * len(widths))(*widths)
-        self._ptrs = (self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(), self.slots, self.rank_pad)
-        self._ws_floats: Dict[int, int] = {}
+        self._struct = _lib.LoraBankStruct(self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(), self.slots, self.rank_pad, self.K, len(widths),
+                                           (ctypes.c_int32 * 4)(*widths))
+        self._ptr, self._device = ctypes.addressof(self._struct), self.a.get_device()
+        self._ws: Dict[int, int] = {}                  # bytes of workspace by rows
 
     def load(self, slot: int, a: torch.Tensor, b: torch.Tensor, scale: float = 1.0) -> None:
         """a [slices, r, K] (or [r, K] of one slice), b [N, r], r <= rank; values become bf16.  Rows read the adapter from the next call on
@@ -1956,11 +1957,15 @@ class LoraBank:
         self.b[slot].zero_()
         self.scale[slot] = 0.0
 
-    def _workspace(self, T: int) -> torch.Tensor:
-        n = self._ws_floats.get(T)
+    def _workspace(self, x: torch.Tensor, T: int) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
+        """(workspace, its address, bytes); steps of few rows have none"""
+        n = self._ws.get(T)
         if n is None:
-            n = self._ws_floats[T] = _lib.load().vb_lora_workspace_bytes(T, self.slots, self.rank_pad, len(self.widths)) // 4
-        return torch.empty(n, dtype=torch.float32, device=self.a.device)
+            n = self._ws[T] = _lib.load().vb_lora_workspace_bytes(self._ptr, T)
+        if n == 0:
+            return None, None, 0
+        ws = x.new_empty(n // 2)                       # (of the allocator's, so that calls on other streams and captured graphs have their own)
+        return ws, ws.data_ptr(), n
 
 
 class LoraPlan:
@@ -1972,6 +1977,7 @@ class LoraPlan:
         lib = _lib.load()
         n = max(lib.vb_lora_plan_bytes(min(max_rows, 64), slots), lib.vb_lora_plan_bytes(max_rows, slots))
         self.tiles = torch.zeros(n // 4, dtype=torch.int32, device=device)
+        self._ptr, self._device = self.tiles.data_ptr(), self.tiles.get_device()
 
 
 def lora_plan(plan: LoraPlan, ids: torch.Tensor) -> LoraPlan:
@@ -1981,14 +1987,18 @@ def lora_plan(plan: LoraPlan, ids: torch.Tensor) -> LoraPlan:
     T = ids.numel()
     _refuse(T > plan.max_rows, f"lora_plan: {T} rows; the plan holds {plan.max_rows}")
     if T:
-        call("vb_lora_plan", plan.tiles.data_ptr(), ids.data_ptr(), T, plan.slots, _stream())
+        call("vb_lora_plan", plan._ptr, ids.data_ptr(), T, plan.slots, _stream())
     plan.n_rows = T
     return plan
 
 
 def _lora_check(who: str, x: torch.Tensor, bank: LoraBank, plan: LoraPlan) -> None:
+    """raises if a call's rows, bank and plan do not go together (one comparison per fact when they do: every call passes here)"""
+    if (x.is_cuda and x.dtype is BF16 and x.dim() == 2 and x.shape[1] == bank.K and x.get_device() == bank._device == plan._device == _device_index()
+            and plan.slots == bank.slots and plan.n_rows == x.shape[0] and (x.stride(1) == 1 or x.shape[0] == 0)):
+        return
     _need_here(who, x, bank.a, plan.tiles)
-    _refuse(x.dtype != BF16 or x.dim() != 2 or x.shape[1] != bank.K or (x.stride(1) != 1 and x.shape[0] > 0), f"{who}: bf16 rows of {bank.K} are needed")
+    _refuse(x.dtype != BF16 or x.dim() != 2 or x.shape[1] != bank.K or x.stride(1) != 1, f"{who}: bf16 rows of {bank.K} are needed")
     _refuse(plan.slots != bank.slots, f"{who}: the plan counts {plan.slots} adapters, the bank {bank.slots}")
     _refuse(plan.n_rows != x.shape[0], f"{who}: {x.shape[0]} rows, the plan was made for {plan.n_rows}")
 
@@ -1999,20 +2009,24 @@ def lora(x: torch.Tensor, bank: LoraBank, plan: LoraPlan, out: Optional[torch.Te
     itself; None: zeros."""
     _lora_check("lora", x, bank, plan)
     T, N = x.shape[0], bank.N
+    f32, ld_out = True, N
+    if out is not None or base is not None:
+        like = base if out is None else out
+        f32 = like.dtype is F32
+        for t in (out, base):
+            if t is not None:
+                _need_here("lora", t)
+                _refuse(t.dtype != like.dtype or not (f32 or t.dtype == BF16) or tuple(t.shape) != (T, N) or (t.stride(1) != 1 and T > 0),
+                        f"lora: out and base are fp32 or bf16 rows [{T}, {N}] of one type")
+        if out is not None and T > 1:
+            ld_out = out.stride(0)
     if out is None:
-        out = torch.empty(T, N, dtype=torch.float32 if base is None else base.dtype, device=x.device)
-    f32 = out.dtype == torch.float32
-    for t in (out, base):
-        if t is not None:
-            _need_here("lora", t)
-            _refuse(t.dtype != out.dtype or not (f32 or t.dtype == BF16) or tuple(t.shape) != (T, N) or t.stride(1) != 1,
-                    f"lora: out and base are fp32 or bf16 rows [{T}, {N}] of one type")
+        out = torch.empty((T, N), dtype=F32 if f32 else BF16, device=x.device)
     if T == 0:
         return out
-    ws = bank._workspace(T)
-    call("vb_lora", out.data_ptr(), out.stride(0) if T > 1 else N, _p(base), base.stride(0) if base is not None and T > 1 else N, int(f32), x.data_ptr(),
-         x.stride(0) if T > 1 else bank.K, *bank._ptrs, bank._widths, len(bank.widths), plan.tiles.data_ptr(), T, bank.K, ws.data_ptr(),
-         ws.numel() * 4, _stream())
+    ws, ws_ptr, ws_bytes = bank._workspace(x, T)
+    call("vb_lora", out.data_ptr(), ld_out, None if base is None else base.data_ptr(), N if base is None or T == 1 else base.stride(0), int(f32), x.data_ptr(),
+         x.stride(0) if T > 1 else bank.K, bank._ptr, plan._ptr, T, ws_ptr, ws_bytes, _stream())
     return out
 
 
@@ -2022,25 +2036,29 @@ def lora_gate_up(x: torch.Tensor, bank: LoraBank, plan: LoraPlan, planes: torch.
     _lora_check("lora_gate_up", x, bank, plan)
     _refuse(len(bank.widths) != 2 or bank.widths[0] != bank.widths[1], f"lora_gate_up: a bank of gate | up is needed, not of slices {bank.widths}")
     _refuse(half not in (16, 32, 48, 64), f"lora_gate_up: tiles of {half} gate rows (16, 32, 48 or 64)")
-    _need_here("lora_gate_up", planes)
     T, ff = x.shape[0], bank.widths[0]
-    width = (ff + half - 1) // half * half * 2
-    _refuse(planes.dtype != torch.float32 or planes.dim() != 3 or planes.shape[0] < 1 or tuple(planes.shape[1:]) != (T, width) or not planes.is_contiguous(),
-            f"lora_gate_up: fp32 planes [splits, {T}, {width}] are needed")
-    tiled = isinstance(out, TiledAct)
-    if tiled:
-        _need_here("lora_gate_up", out.data)
+    splits = planes.shape[0]
+    if (not planes.is_cuda or planes.get_device() != bank._device or planes.dtype is not F32 or splits < 1
+            or tuple(planes.shape) != (splits, T, (ff + half - 1) // half * half * 2) or not planes.is_contiguous()):
+        _need_here("lora_gate_up", planes)
+        raise VoxB200Error(f"lora_gate_up: fp32 planes [splits, {T}, {(ff + half - 1) // half * half * 2}] are needed, not {tuple(planes.shape)}")
+    xt, ld = 0, ff
+    if out is None:
+        out = to = torch.empty((T, ff), dtype=BF16, device=x.device)
+    elif isinstance(out, TiledAct):
+        to, xt = out.data, out.t_tile
+        _need_here("lora_gate_up", to)
         _refuse(out.T != T or out.K != ff, f"lora_gate_up: tiled rows [{out.T}, {out.K}] are not [{T}, {ff}]")
-    elif out is None:
-        out = torch.empty(T, ff, dtype=BF16, device=x.device)
     else:
+        to = out
         _need_here("lora_gate_up", out)
-        _refuse(out.dtype != BF16 or tuple(out.shape) != (T, ff) or out.stride(1) != 1, f"lora_gate_up: out is bf16 [{T}, {ff}]")
+        _refuse(out.dtype != BF16 or tuple(out.shape) != (T, ff) or (out.stride(1) != 1 and T > 0), f"lora_gate_up: out is bf16 [{T}, {ff}]")
+        ld = out.stride(0) if T > 1 else ff
     if T == 0:
         return out
-    ws = bank._workspace(T)
-    call("vb_lora_gate_up", out.data.data_ptr() if tiled else out.data_ptr(), ff if tiled or T == 1 else out.stride(0), out.t_tile if tiled else 0,
-         planes.data_ptr(), planes.shape[0], int(half), ff, x.data_ptr(), x.stride(0) if T > 1 else bank.K, *bank._ptrs, plan.tiles.data_ptr(), T, bank.K, ws.data_ptr(), ws.numel() * 4, _stream())
+    ws, ws_ptr, ws_bytes = bank._workspace(x, T)
+    call("vb_lora_gate_up", to.data_ptr(), ld, xt, planes.data_ptr(), splits, half, x.data_ptr(), x.stride(0) if T > 1 else bank.K, bank._ptr, plan._ptr, T, ws_ptr,
+         ws_bytes, _stream())
     return out
 
 
@@ -2052,7 +2070,7 @@ MOE_LAYER_MAX_ROWS = 64
 class MoeWeights:
     """The matrices of a mixture's experts as ``moe_layer`` reads them: packed tiles (the buffers that the projections of larger steps multiply), every
     expert's gate | up rows after the other's, the shared expert last; the down matrices side by side along k."""
-    __slots__ = ("up", "down", "experts", "width", "ff", "shared_ff", "act", "limit", "slope")
+    __slots__ = ("up", "down", "experts", "width", "ff", "shared_ff", "act", "limit", "slope", "_struct", "_ptr", "_device")
 
     def __init__(self, up: PackedWeight, down: PackedWeight, experts: int, width: int, ff: int, shared_ff: int = 0, act: str = "silu_glu",
                  limit: float = 0.0, slope: float = 1.702):
@@ -2069,6 +2087,9 @@ class MoeWeights:
                 f"MoeWeights: tiles of {up.tile_rows} and {down.tile_rows} rows")
         self.up, self.down, self.experts, self.width, self.ff, self.shared_ff = up, down, int(experts), int(width), int(ff), int(shared_ff)
         self.act, self.limit, self.slope = act, float(limit), float(slope)
+        self._struct = _lib.MoeWeightsStruct(up.data.data_ptr(), down.data.data_ptr(), self.width, self.experts, self.ff, self.shared_ff, up.tile_rows, MOE_LAYER_ACTS[act],
+                                             self.limit, self.slope)
+        self._ptr, self._device = ctypes.addressof(self._struct), up.data.get_device()
 
     @classmethod
     def pack(cls, gate: Optional[torch.Tensor], up: torch.Tensor, down: torch.Tensor, shared=None, act: str = "silu_glu", limit: float = 0.0,
@@ -2114,7 +2135,7 @@ class MoeRouter:
       "softmax_all"  softmax over all experts, chosen within the kept groups, weights as they are (``moe_route_groups``)
       "table"        the row's token id picks them, each 1 / top (``moe_route_table``)
     weight fp32 [experts, width]; shared_gate fp32 [width] ("sigmoid", "table"): the shared expert times sigmoid(shared_gate . h)."""
-    __slots__ = ("kind", "top", "weight", "bias", "groups", "keep", "shared_gate", "table")
+    __slots__ = ("kind", "top", "weight", "bias", "groups", "keep", "shared_gate", "table", "_struct", "_ptr", "_devices", "_weights")
 
     def __init__(self, kind: str, top: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, groups: int = 0, keep: int = 0,
                  shared_gate: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None):
@@ -2135,34 +2156,53 @@ class MoeRouter:
                     f"MoeRouter: {groups} groups (keep {keep}) do not fit a {kind!r} router of {E} experts, top {top}")
         self.kind, self.top, self.weight, self.bias, self.groups, self.keep = kind, int(top), weight, bias, int(groups), int(keep)
         self.shared_gate, self.table = shared_gate, table
+        self._struct = _lib.MoeRouterStruct(_p(weight), _p(bias), _p(shared_gate), _p(table), MOE_LAYER_ROUTERS[kind], self.top, self.groups, self.keep,
+                                            0 if table is None else table.shape[0])
+        self._ptr, self._devices = ctypes.addressof(self._struct), {t.get_device() for t in (weight, bias, shared_gate, table) if t is not None}
+        self._weights = None
+
+    def _goes_with(self, weights: MoeWeights) -> bool:
+        """whether the router's matrix has the weights' shape and device (remembered for the weights that it was asked about last)"""
+        if self._weights is not weights:
+            if (self.top > weights.experts or self._devices != {weights._device} or (self.weight is not None and tuple(self.weight.shape) != (weights.experts, weights.width))
+                    or (self.shared_gate is not None and (not weights.shared_ff or self.shared_gate.numel() != weights.width))):
+                return False
+            self._weights = weights
+        return True
+
+
+def _moe_layer_check(h: torch.Tensor, weights: MoeWeights, router: MoeRouter, ids: Optional[torch.Tensor]) -> None:
+    W, E, T = weights.width, weights.experts, h.shape[0]
+    _need_here("moe_layer", h, weights.up.data, weights.down.data, router.weight, router.bias, router.table, router.shared_gate, ids)
+    _refuse(h.dtype != BF16 or h.dim() != 2 or h.shape[1] != W or not h.is_contiguous(), f"moe_layer: contiguous bf16 rows of {W} are needed")
+    _refuse(T > MOE_LAYER_MAX_ROWS, f"moe_layer: {T} rows; at most {MOE_LAYER_MAX_ROWS} (larger steps group the rows: moe_group_tiles, gemm_tiles)")
+    _refuse(router.top > E or (router.weight is not None and tuple(router.weight.shape) != (E, W)), f"moe_layer: the router does not match {E} experts of width {W}")
+    _refuse(router.shared_gate is not None and (not weights.shared_ff or router.shared_gate.numel() != W), "moe_layer: a gate without a shared expert of its width")
+    _refuse((router.kind == "table") != (ids is not None) or (ids is not None and (ids.dtype != torch.int32 or ids.numel() != T or not ids.is_contiguous())),
+            "moe_layer: a table router, and no other, takes int32 ids of every row")
 
 
 def moe_layer(h: torch.Tensor, weights: MoeWeights, router: MoeRouter, ids: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A whole mixture-of-experts layer for the rows of a decode step (at most MOE_LAYER_MAX_ROWS): router, the chosen experts, the shared expert, weighted
     sum.  h bf16 [T, width]; ids int32 [T] (token ids) for a table router; out fp32 [T, width].  The matrices of experts that no row chose are not read; nothing
     is rounded between the two products."""
-    T, W, top, E = h.shape[0], weights.width, router.top, weights.experts
-    _need_here("moe_layer", h, weights.up.data, router.weight, router.bias, router.table, router.shared_gate, ids, out)
-    _refuse(h.dtype != BF16 or h.dim() != 2 or h.shape[1] != W or not h.is_contiguous(), f"moe_layer: contiguous bf16 rows of {W} are needed")
-    _refuse(T > MOE_LAYER_MAX_ROWS, f"moe_layer: {T} rows; at most {MOE_LAYER_MAX_ROWS} (larger steps group the rows: moe_group_tiles, gemm_tiles)")
-    _refuse(top > E or (router.weight is not None and tuple(router.weight.shape) != (E, W)), f"moe_layer: the router does not match {E} experts of width {W}")
-    _refuse(router.shared_gate is not None and (not weights.shared_ff or router.shared_gate.numel() != W), "moe_layer: a gate without a shared expert of its width")
-    _refuse((router.kind == "table") != (ids is not None) or (ids is not None and (ids.dtype != torch.int32 or ids.numel() != T or not ids.is_contiguous())),
-            "moe_layer: a table router, and no other, takes int32 ids of every row")
+    T, W = h.shape[0], weights.width
+    # (one comparison per fact when all goes together: every call passes here; what matches has been compared before)
+    if not (h.is_cuda and h.dtype is BF16 and h.dim() == 2 and h.shape[1] == W and T <= MOE_LAYER_MAX_ROWS and h.get_device() == weights._device == _device_index()
+            and router._goes_with(weights) and h.is_contiguous() and (ids is None) == (router.table is None)
+            and (ids is None or (ids.dtype is torch.int32 and ids.numel() == T and ids.get_device() == weights._device and ids.is_contiguous()))):
+        _moe_layer_check(h, weights, router, ids)
     if out is None:
-        out = torch.empty(T, W, dtype=F32, device=h.device)
-    _refuse(out.dtype != F32 or tuple(out.shape) != (T, W) or (T > 0 and out.stride(1) != 1), f"moe_layer: out is fp32 [{T}, {W}]")
+        out = torch.empty((T, W), dtype=F32, device=h.device)
+        ld = W
+    else:
+        _need_here("moe_layer", out)
+        _refuse(out.dtype != F32 or tuple(out.shape) != (T, W) or (T > 0 and out.stride(1) != 1), f"moe_layer: out is fp32 [{T}, {W}]")
+        ld = out.stride(0) if T > 1 else W
     if T == 0:
         return out
-    P = T * top
-    head = (8 * P + 4 * T + 15) // 16 * 16
-    act_bytes = 6 * (P + T) * max(weights.ff, weights.shared_ff)
-    ws = torch.empty(head + act_bytes, dtype=torch.uint8, device=h.device)
-    idx = ws.data_ptr()
-    wts, sgate, act, s = idx + 4 * P, (idx + 8 * P if router.shared_gate is not None else None), idx + head, _stream()
-    hp = h.data_ptr()
-    call("vb_moe_layer_route", idx, wts, sgate, MOE_LAYER_ROUTERS[router.kind], hp, W, _p(router.weight), _p(router.bias), _p(router.shared_gate), _p(ids),
-         _p(router.table), T, W, E, top, router.groups, router.keep, router.table.shape[0] if ids is not None else 0, s)
-    call("vb_moe_layer_experts", out.data_ptr(), out.stride(0) if T > 1 else W, hp, W, weights.up.data.data_ptr(), weights.down.data.data_ptr(), idx, wts, sgate,
-         T, W, E, top, weights.ff, weights.shared_ff, weights.up.tile_rows, MOE_LAYER_ACTS[weights.act], weights.limit, weights.slope, act, act_bytes, s)
+    P = T * router.top
+    n = (8 * P + 4 * T + 15) // 16 * 16 + 6 * (P + T) * max(weights.ff, weights.shared_ff)
+    ws = h.new_empty(n // 2)                           # (of the allocator's, so that calls on other streams and captured graphs have their own)
+    call("vb_moe_layer", out.data_ptr(), ld, h.data_ptr(), W, weights._ptr, router._ptr, None if ids is None else ids.data_ptr(), T, ws.data_ptr(), n, _stream())
     return out
