@@ -91,7 +91,8 @@ struct LoraParams {
   uint32_t* v;                     // [tiles][tile_rows / 16][S][parts][rank / 16][32 lanes][4]: v as the second product takes it
   int T, K, kb32, rank_tiles, VR, k_split, parts;      // VR = S * rank
   // second product
-  int blocks, per_block;           // column blocks of 32 over all slices (of gate | up: of one), and how many a block of threads has
+  int blocks;                      // column blocks of 32 over all slices (of gate | up: of one)
+  int ahead;                       // 1: a step's copies go out a step ahead
   int slices, block0[LORA_MAX_SLICES + 1], col0[LORA_MAX_SLICES + 1];
   void* out;
   const void* base;
@@ -150,8 +151,8 @@ __global__ void __launch_bounds__(LORA_THREADS, LoraDown<RT>::BLOCKS) lora_down_
   const int4 tl = *reinterpret_cast<const int4*>(rec);
   if (tl.z == 0 || tl.x < 0) return;        // (all blocks of the cluster) no tile; no adapter: the second kernel does not look at v
   const int n = tl.z, rts = p.VR >> 4;
-  const int stages = (p.K + LORA_STAGE_K - 1) / LORA_STAGE_K, s0 = static_cast<int>(static_cast<long long>(stages) * blockIdx.y / p.k_split),
-            s1 = static_cast<int>(static_cast<long long>(stages) * (blockIdx.y + 1) / p.k_split);
+  // (the blocks of a tile take stages in turn, so that at any time they read neighbouring pieces of the rows)
+  const int s1 = (p.K + LORA_STAGE_K - 1) / LORA_STAGE_K, s0 = blockIdx.y, hop = p.k_split;
   // a thread's copies: 16 bytes of four rows, 16 bytes of every rank tile.  What is not there (rows behind the last, k behind K, rank tiles) is filled with zeros.
   const int chunk = tid & 15, row0 = tid >> 4;
   const __nv_bfloat16* xr[4];
@@ -189,13 +190,13 @@ __global__ void __launch_bounds__(LORA_THREADS, LoraDown<RT>::BLOCKS) lora_down_
     };
     float acc[RT][4][4] = {};
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) load(s0 + i, i * STAGE_BYTES);
+    for (int i = 0; i < STAGES - 1; ++i) load(s0 + i * hop, i * STAGE_BYTES);
     uint32_t at = 0, free_at = (STAGES - 1) * STAGE_BYTES;
 #pragma unroll 1
-    for (int s = s0; s < s1; ++s) {
+    for (int s = s0; s < s1; s += hop) {
       cp_async_wait<STAGES - 2>();
       __syncthreads();
-      load(s + STAGES - 1, free_at);
+      load(s + (STAGES - 1) * hop, free_at);
       uint4 av[RT][2];
 #pragma unroll
       for (int i = 0; i < RT; ++i) {
@@ -354,98 +355,136 @@ __device__ __forceinline__ void* lora_place(const LoraParams& p, long long row, 
 template <int OUT>
 __host__ __device__ constexpr int lora_parts() { return OUT == LORA_F32 ? 3 : 2; }
 
-// Block: a tile x per_block column blocks.  All but v is older than the first product and on its way into shared memory before that ends: the block's part of B, and
-// its rows' part of the base or of the planes.  The warps stand ceil(rows / 16) deep along the rows and divide the columns.
+// Block: a tile x a range of column blocks, four warps, in steps: tiles of 64 rows, a warp per 16 rows, all warps the same one or two column blocks (so that of base and
+// results 128 bytes of a row at least move together); tiles of 16 rows, a warp per column block.  What a step reads, its part of B and the rows' part of base or
+// planes, is copied a step ahead; v is read once.  All but v is older than the first product, so the first steps' copies are on their way when that ends.
+constexpr int LORA_UP_THREADS = 128;
 template <int OUT>
 __host__ __device__ constexpr int lora_row_bytes() { return OUT == LORA_GLU ? 256 : OUT == LORA_F32 ? 128 : 64; }      // of a column block in base or planes
-template <int KS, int OUT>
-__global__ void __launch_bounds__(LORA_THREADS, KS == 8 || OUT == LORA_GLU ? 2 : 3) lora_up_kernel(const LoraParams p) {
+template <int OUT, bool TALL>
+struct LoraUp {
+  static constexpr int WIDE = TALL && OUT != LORA_GLU ? 2 : 1;           // column blocks of a warp
+  static constexpr int BLOCKS = TALL ? WIDE : 4;                         // ... of a step
+  static constexpr int ROW = lora_row_bytes<OUT>() * WIDE, LD = ROW + 16;
+  static constexpr int ROWS_BYTES = (TALL ? 64 : 4 * 16) * LD;
+};
+template <int KS, int OUT, bool TALL>
+__global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraParams p) {
   extern __shared__ __align__(128) uint8_t smem8[];
-  constexpr int PARTS = lora_parts<OUT>(), B_BYTES = KS * 1024 * (OUT == LORA_GLU ? 2 : 1), SEG = lora_row_bytes<OUT>();
+  using Up = LoraUp<OUT, TALL>;
+  constexpr int PARTS = lora_parts<OUT>(), B_BYTES = KS * 1024, SEG = lora_row_bytes<OUT>(), LD = Up::LD, WIDE = Up::WIDE, STEP = Up::BLOCKS, BOTH = OUT == LORA_GLU ? 2 : 1;
+  constexpr int TILE = TALL ? 64 : 16;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-  const int32_t* rec = p.tiles + static_cast<long long>(blockIdx.x) * (4 + p.tile_rows);
+  const int32_t* rec = p.tiles + static_cast<long long>(blockIdx.x) * (4 + TILE);
   const int4 tl = *reinterpret_cast<const int4*>(rec);
-  const int n = tl.z, need = (n + 15) >> 4, c0 = blockIdx.y * p.per_block, c1 = min(p.blocks, c0 + p.per_block), nb = c1 - c0;
+  // (ranges in whole steps)
+  const int n = tl.z, all = (p.blocks + STEP - 1) / STEP;
+  const int c0 = static_cast<int>(static_cast<long long>(all) * blockIdx.y / gridDim.y) * STEP, c1 = min(p.blocks, static_cast<int>(static_cast<long long>(all) * (blockIdx.y + 1) / gridDim.y) * STEP);
   const bool has = tl.x >= 0;
-  if (n == 0) {
+  if (n == 0 || c0 >= c1) {
     pdl_sync();
     return;
   }
-  // shared memory: v [m16 blocks][slices][PARTS][KS] of 512 bytes, B, rows of base or planes
-  const int v_bytes = need * p.slices * PARTS * KS * 512, ld_rows = p.per_block * SEG + 16;
-  uint8_t* bs = smem8 + (p.tile_rows >> 4) * p.slices * PARTS * KS * 512;
-  uint8_t* rows = bs + p.per_block * B_BYTES;
-  if (has) {
-    const uint4* b = p.b + tl.x * p.b_slot + static_cast<long long>(c0) * KS * 64;
-    const int half = nb * KS * 64;
-    for (int i = tid; i < half; i += LORA_THREADS) {
-      cp_async16(smem_u32(bs) + i * 16, b + i, 16);
-      if (OUT == LORA_GLU) cp_async16(smem_u32(bs) + (half + i) * 16, b + static_cast<long long>(p.blocks) * KS * 64 + i, 16);       // (the up columns' blocks follow the gate's)
+  // shared memory: v [m16 blocks][slices][PARTS][KS] of 512 bytes, then two steps: B of the column blocks (of gate, of up), rows of base or planes
+  const bool adds = OUT == LORA_GLU || p.base != nullptr;
+  const int v_bytes = ((n + 15) >> 4) * p.slices * PARTS * KS * 512, step_bytes = STEP * BOTH * B_BYTES + (adds ? Up::ROWS_BYTES : 0);
+  const uint32_t vs = smem_u32(smem8), steps = vs + (TILE / 16) * p.slices * PARTS * KS * 512;
+  // a lane's copies of base or planes: 16 bytes (q) of every ROWS-th row of its 16
+  constexpr int PER = Up::ROW / 16, ROWS = 32 / PER;
+  const int q = lane % PER, mt = TALL ? warp : 0, r0 = mt * 16 + lane / PER;
+  const uint8_t* src[16 / ROWS];
+  bool there[16 / ROWS];
+  if (adds) {
+    const long long ld = (OUT == LORA_GLU ? p.width : p.ld_base) * (OUT == LORA_BF16 ? 2 : 4);
+#pragma unroll
+    for (int i = 0; i < 16 / ROWS; ++i) {
+      there[i] = r0 + i * ROWS < n;
+      src[i] = static_cast<const uint8_t*>(OUT == LORA_GLU ? p.planes : p.base) + (there[i] ? rec[4 + r0 + i * ROWS] : 0) * ld;
     }
   }
-  // (base and planes: columns of a block are neighbours, but blocks of different slices may not be)
-  if (OUT == LORA_GLU || p.base) {
-    constexpr int PER = SEG / 16;
-    for (int k = lane; k < nb * PER; k += 32) {
-      const int c = c0 + k / PER, q = k % PER;
-      long long at;
-      bool in;
-      if constexpr (OUT == LORA_GLU) {
-        at = c * 64 + q * 4;
-        in = at < 2 * ((p.ff + 15) & ~15);
-      } else {
-        int s = 0;
-        while (c >= p.block0[s + 1]) ++s;
-        at = p.col0[s] + (c - p.block0[s]) * 32 + q * (OUT == LORA_F32 ? 4 : 8);
-        in = at < p.col0[s + 1];
+  const uint32_t rows_to = STEP * BOTH * B_BYTES + (TALL ? 0 : warp * 16 * LD);                // the warp's rows in a step (tall: all warps')
+  const uint4* b = p.b + (has ? tl.x : 0) * p.b_slot;
+  auto load = [&](int c, int turn) {
+    if (c < c1) {
+      const uint32_t to = steps + (turn & p.ahead) * step_bytes;
+      if (has) {
+        const int chunks = min(STEP, c1 - c) * KS * 64;
+        for (int i = tid; i < chunks; i += LORA_UP_THREADS) {
+          cp_async16(to + i * 16, b + static_cast<long long>(c) * KS * 64 + i, 16);
+          if (OUT == LORA_GLU) cp_async16(to + STEP * B_BYTES + i * 16, b + static_cast<long long>(p.blocks + c) * KS * 64 + i, 16);      // (the up columns' blocks follow the gate's)
+        }
       }
-      const uint8_t* from = static_cast<const uint8_t*>(OUT == LORA_GLU ? p.planes : p.base) + (in ? at : 0) * (OUT == LORA_BF16 ? 2 : 4);
-      const long long ld = (OUT == LORA_GLU ? p.width : p.ld_base) * (OUT == LORA_BF16 ? 2 : 4);
-      const uint32_t to = smem_u32(rows) + k * 16;
-      const int bytes = in ? 16 : 0;
-#pragma unroll 4
-      for (int r = warp; r < n; r += 8) cp_async16(to + r * ld_rows, from + rec[4 + r] * ld, bytes);
+      const int block = c + (TALL ? q / (SEG / 16) : warp), in_block = q % (SEG / 16);
+      if (adds && block < c1) {
+        long long at;
+        bool in;
+        if constexpr (OUT == LORA_GLU) {
+          at = block * 64 + in_block * 4;
+          in = at < 2 * ((p.ff + 15) & ~15);
+        } else {
+          int s = 0;
+          while (block >= p.block0[s + 1]) ++s;
+          at = p.col0[s] + (block - p.block0[s]) * 32 + in_block * (OUT == LORA_F32 ? 4 : 8);
+          in = at < p.col0[s + 1];
+        }
+        const uint32_t row_to = to + rows_to + r0 * LD + q * 16;
+        const long long bytes_at = (in ? at : 0) * (OUT == LORA_BF16 ? 2 : 4);
+#pragma unroll
+        for (int i = 0; i < 16 / ROWS; ++i)
+          if (there[i]) cp_async16(row_to + i * ROWS * LD, src[i] + bytes_at, in ? 16 : 0);
+      }
     }
-  }
-  const int m_tiles = need == 3 ? 4 : need, mt = warp & (m_tiles - 1), step = 8 / m_tiles;
+    cp_async_commit();
+  };
   const int ra = mt * 16 + g, rb = ra + 8;
-  const long long row_a = ra < n ? rec[4 + ra] : -1, row_b = rb < n ? rec[4 + rb] : -1;
+  const long long row[2] = {ra < n ? rec[4 + ra] : -1, rb < n ? rec[4 + rb] : -1};
+  load(c0, 0);
   pdl_sync();
   if (has) {
-    const uint4* v = reinterpret_cast<const uint4*>(p.v) + static_cast<long long>(blockIdx.x) * (p.tile_rows >> 4) * p.slices * PARTS * KS * 32;
-    for (int i = tid; i < v_bytes / 16; i += LORA_THREADS) cp_async16(smem_u32(smem8) + i * 16, v + i, 16);
+    const uint4* v = reinterpret_cast<const uint4*>(p.v) + static_cast<long long>(blockIdx.x) * (TILE / 16) * p.slices * PARTS * KS * 32;
+    for (int i = tid; i < v_bytes / 16; i += LORA_UP_THREADS) cp_async16(vs + i * 16, v + i, 16);
   }
   cp_async_commit();
-  cp_async_wait<0>();
-  __syncthreads();
-  if (mt >= need) return;
-  const uint32_t frags = smem_u32(smem8) + (mt * p.slices * PARTS * KS * 32 + lane) * 16, bw = smem_u32(bs) + lane * 16;
-  const uint8_t* from[2] = {rows + ra * ld_rows + (OUT == LORA_GLU ? (t4 >> 1) * 128 + (t4 & 1) * 32 : t4 * (SEG / 4)), nullptr};
-  from[1] = from[0] + 8 * ld_rows;
-  const long long row[2] = {row_a, row_b};
-  for (int c = c0 + warp / m_tiles, s = 0; c < c1; c += step) {
-    while (OUT != LORA_GLU && c >= p.block0[s + 1]) ++s;
-    float d[4][4] = {}, u[4][4] = {};
-    if (has) {
-      lora_product<KS, PARTS>(d, frags + s * PARTS * KS * 512, bw + (c - c0) * KS * 1024);
-      if constexpr (OUT == LORA_GLU) lora_product<KS, PARTS>(u, frags + PARTS * KS * 512, bw + (nb + c - c0) * KS * 1024);
+  const uint32_t frags = vs + (mt * p.slices * PARTS * KS * 32 + lane) * 16;
+  int turn = 0, s = 0;
+  for (int c = c0; c < c1; c += STEP, ++turn) {
+    if (p.ahead) {
+      load(c + STEP, turn + 1);
+      cp_async_wait<1>();                                     // (all but the step ahead; v came before it)
+    } else {
+      cp_async_wait<0>();
     }
-    const int col = p.col0[s] + (c - p.block0[s]) * 32 + t4 * 8;
-    if (col >= p.col0[s + 1]) continue;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      if (row[h] < 0) continue;
-      float y[8], z[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        y[i] = d[i >> 1][h * 2 + (i & 1)];
-        z[i] = u[i >> 1][h * 2 + (i & 1)];
+    __syncthreads();
+    const uint32_t from = steps + (turn & p.ahead) * step_bytes;
+#pragma unroll 1
+    for (int w = 0; w < WIDE; ++w) {
+      const int mine = TALL ? w : warp, block = c + mine;
+      if (mt * 16 >= n || block >= c1) break;
+      while (OUT != LORA_GLU && block >= p.block0[s + 1]) ++s;
+      float d[4][4] = {}, u[4][4] = {};
+      if (has) {
+        lora_product<KS, PARTS>(d, frags + s * PARTS * KS * 512, from + mine * B_BYTES + lane * 16);
+        if constexpr (OUT == LORA_GLU) lora_product<KS, PARTS>(u, frags + PARTS * KS * 512, from + (STEP + mine) * B_BYTES + lane * 16);
       }
-      void* out = lora_place<OUT>(p, row[h], col);
-      const uint8_t* add = from[h] + (c - c0) * SEG;
-      if constexpr (OUT == LORA_GLU) lora_gated(p, out, row[h], col, y, z, reinterpret_cast<const float*>(add));
-      else lora_result<OUT>(out, y, p.base ? add : nullptr);
+      const int col = p.col0[s] + (block - p.block0[s]) * 32 + t4 * 8;
+      if (col >= p.col0[s + 1]) continue;
+      const uint8_t* add = smem8 + (from - vs) + rows_to + ra * LD + (TALL ? w * SEG : 0) + (OUT == LORA_GLU ? (t4 >> 1) * 128 + (t4 & 1) * 32 : t4 * (SEG / 4));
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (row[h] < 0) continue;
+        float y[8], z[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          y[i] = d[i >> 1][h * 2 + (i & 1)];
+          z[i] = u[i >> 1][h * 2 + (i & 1)];
+        }
+        void* out = lora_place<OUT>(p, row[h], col);
+        if constexpr (OUT == LORA_GLU) lora_gated(p, out, row[h], col, y, z, reinterpret_cast<const float*>(add + h * 8 * LD));
+        else lora_result<OUT>(out, y, p.base ? add + h * 8 * LD : nullptr);
+      }
     }
+    __syncthreads();                                          // (the step has been read: the one after the next, or the next, may come into its place)
+    if (!p.ahead) load(c + STEP, 0);
   }
 }
 
@@ -596,10 +635,10 @@ __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams
 static int lora_tile_rows(int T) { return T <= 64 ? 16 : 64; }
 // the most tiles a step can have
 static int lora_max_tiles(int T, int slots) { return T / lora_tile_rows(T) + (T < slots + 1 ? T : slots + 1); }
-// ... and about how many it has (prompts bring few adapters)
+// ... and about how many it has (half of the adapters)
 static int lora_tiles(int T, int slots) {
   const int adapters = T < slots + 1 ? T : slots + 1;
-  return T <= 64 ? adapters : (T + 63) / 64 + (adapters > 16 ? 8 : adapters / 2);
+  return T <= 64 ? adapters : (T + 63) / 64 + adapters / 2;
 }
 static int lora_k_split(int T, int K, int slots, int VR) {
   const int stages = (K + LORA_STAGE_K - 1) / LORA_STAGE_K, tiles = lora_tiles(T, slots);
@@ -611,24 +650,26 @@ static int lora_k_split(int T, int K, int slots, int VR) {
 // One launch for a step of at most 64 rows, where an adapter is what eight SMs take in good time.
 static bool lora_few(const LoraParams& p) { return p.T <= 64 && p.VR <= LORA_FEW_RANKS && p.rank_tiles <= 4 && (p.a_slot + p.b_slot) * 16 <= 2 << 20; }
 
+template <int KS, int OUT, bool TALL>
+static int lora_up_tiles(LoraParams& p, int max_tiles, int tiles, void* stream) {
+  using Up = LoraUp<OUT, TALL>;
+  VB_CHECK_CUDA((rm_smem<lora_up_kernel<KS, OUT, TALL>>()));
+  const size_t v_bytes = static_cast<size_t>(p.tile_rows >> 4) * p.slices * lora_parts<OUT>() * KS * 512,
+               step = static_cast<size_t>(Up::BLOCKS) * KS * 1024 * (OUT == LORA_GLU ? 2 : 1) + (OUT == LORA_GLU || p.base ? Up::ROWS_BYTES : 0);
+  p.ahead = v_bytes + 2 * step <= VB_MAX_DYN_SMEM;     // (four slices of rank 128 beside a base leave room for one step only)
+  const size_t smem = v_bytes + (p.ahead + 1) * step;
+  // one wave of up to four blocks an SM (a wave and a few blocks take as long as two), a step each at least
+  const int fit = smem <= 56 * 1024 ? 4 : smem <= 75 * 1024 ? 3 : smem <= 113 * 1024 ? 2 : 1;
+  int split = fit * sm_count() / tiles;
+  const int most = (p.blocks + Up::BLOCKS - 1) / Up::BLOCKS;
+  if (split > most) split = most;
+  if (split < 1) split = 1;
+  VB_LAUNCH_PDL((lora_up_kernel<KS, OUT, TALL>), dim3(max_tiles, split), LORA_UP_THREADS, smem, stream, p);
+  return 0;
+}
 template <int KS, int OUT>
 static int lora_up_launch(LoraParams& p, int max_tiles, int tiles, void* stream) {
-  VB_CHECK_CUDA((rm_smem<lora_up_kernel<KS, OUT>>()));
-  const int v_bytes = (p.tile_rows >> 4) * p.slices * lora_parts<OUT>() * KS * 512;
-  const int block_bytes = KS * 1024 * (OUT == LORA_GLU ? 2 : 1) + p.tile_rows * (OUT == LORA_GLU || p.base ? lora_row_bytes<OUT>() : 0);
-  // columns a block: what three blocks an SM (of gate | up: two) hold beside v at a time, in even waves
-  const long long work = static_cast<long long>(tiles) * p.blocks, slots = (OUT == LORA_GLU ? 2 : 3) * sm_count(),
-                  share = (OUT == LORA_GLU ? 90 : 66) * 1024, room = share - v_bytes > 16 * 1024 ? share - v_bytes : 16 * 1024;
-  const long long waves = (work * block_bytes + slots * room - 1) / (slots * room);
-  int per = static_cast<int>((work + slots * waves - 1) / (slots * waves));
-  const int least = p.tile_rows == 16 ? 8 : 2;         // a column block for every warp
-  if (per < least) per = least;
-  if (per > p.blocks) per = p.blocks;
-  size_t smem;
-  while ((smem = static_cast<size_t>(v_bytes) + static_cast<size_t>(per) * block_bytes + p.tile_rows * 16) > VB_MAX_DYN_SMEM && per > 1) --per;      // (one fits always)
-  p.per_block = per;
-  VB_LAUNCH_PDL((lora_up_kernel<KS, OUT>), dim3(max_tiles, (p.blocks + per - 1) / per), LORA_THREADS, smem, stream, p);
-  return 0;
+  return p.tile_rows == 16 ? lora_up_tiles<KS, OUT, false>(p, max_tiles, tiles, stream) : lora_up_tiles<KS, OUT, true>(p, max_tiles, tiles, stream);
 }
 template <int RT>
 static int lora_down_launch(const LoraParams& p, int max_tiles, void* stream) {
