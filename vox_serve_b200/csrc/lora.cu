@@ -104,8 +104,8 @@ struct LoraParams {
 
 // ---- v as the second product's A operand ------------------------------------------------------------------------------------------
 // In the order of the lanes: [m16 block][slice][part][rank tile][32 lanes][4 registers].
-__device__ __forceinline__ void lora_put(uint32_t* frags, int slices, int parts, int ks, int r, int k, float a, float b) {      // row r, v[k] and v[k + 1]
-  const int tile = k >> 4, s = tile / ks, t = tile - s * ks;
+__device__ __forceinline__ void lora_put(uint32_t* frags, int slices, int parts, int log_ks, int r, int k, float a, float b) {      // row r, v[k] and v[k + 1]
+  const int tile = k >> 4, s = tile >> log_ks, ks = 1 << log_ks, t = tile & (ks - 1);
   float h0, m0, l0, h1, m1, l1;
   bf16_parts(a, h0, m0, l0);
   bf16_parts(b, h1, m1, l1);
@@ -226,34 +226,42 @@ __global__ void __launch_bounds__(LORA_THREADS, LoraDown<RT>::BLOCKS) lora_down_
     float* red = reinterpret_cast<float*>(smem8);                  // [8 warps][RT * 16][LD]
     float* mine = red + 8 * RT * 16 * LD;                          // [64 rows][RT * 16]
 #pragma unroll
-    for (int i = 0; i < RT; ++i)
+    for (int j = 0; j < 4; ++j) {
+      if (j >= tiles_n) break;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
+      for (int i = 0; i < RT; ++i) {
         float* w = red + (warp * RT + i) * 16 * LD + j * 8 + t4 * 2;
         *reinterpret_cast<float2*>(w + g * LD) = make_float2(acc[i][j][0], acc[i][j][1]);
         *reinterpret_cast<float2*>(w + (g + 8) * LD) = make_float2(acc[i][j][2], acc[i][j][3]);
       }
+    }
     __syncthreads();
-    const int ranks = min(RT, rts - rt0) * 16;
-    for (int e = tid; e < n * ranks; e += LORA_THREADS) {
-      const int c = e / ranks, r = e - c * ranks;
+    for (int e = tid; e < n * RT * 16; e += LORA_THREADS) {
+      const int c = e / (RT * 16), r = e % (RT * 16);
       float s = 0.f;
 #pragma unroll
       for (int q = 0; q < 4; ++q) s += red[(((c >> 5) * 4 + q) * RT * 16 + r) * LD + (c & 31)];
-      mine[c * RT * 16 + r] = scale * s;
+      mine[e] = scale * s;
     }
     if (p.k_split > 1) cluster_sync_all();
     else __syncthreads();
+    const int log_ks = 31 - __clz(p.rank_tiles);
     uint32_t* v = p.v + static_cast<long long>(blockIdx.x) * (p.tile_rows >> 4) * rts * p.parts * 128;
-    for (int e = blockIdx.y * LORA_THREADS + tid; e < n * (ranks >> 1); e += p.k_split * LORA_THREADS) {
-      const int c = e / (ranks >> 1), r = (e - c * (ranks >> 1)) * 2;
-      float s = 0.f, t = 0.f;
-      for (int z = 0; z < p.k_split; ++z) {
-        const float* from = mine + c * RT * 16 + r;
-        s += p.k_split > 1 ? ld_dsmem_f32(from, z) : from[0];
-        t += p.k_split > 1 ? ld_dsmem_f32(from + 1, z) : from[1];
+    for (int e = blockIdx.y * LORA_THREADS + tid; e < n * RT * 4; e += p.k_split * LORA_THREADS) {
+      const int c = e / (RT * 4), k = rt0 * 16 + e % (RT * 4) * 4;
+      if (k >= p.VR) continue;
+      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (p.k_split > 1) {
+#pragma unroll 4
+        for (int z = 0; z < p.k_split; ++z) {
+          const float4 w = ld_dsmem_f32x4(mine + e * 4, z);
+          s.x += w.x; s.y += w.y; s.z += w.z; s.w += w.w;
+        }
+      } else {
+        s = *reinterpret_cast<const float4*>(mine + e * 4);
       }
-      lora_put(v, p.slices, p.parts, p.rank_tiles, c, rt0 * 16 + r, s, t);
+      lora_put(v, p.slices, p.parts, log_ks, c, k, s.x, s.y);
+      lora_put(v, p.slices, p.parts, log_ks, c, k + 2, s.z, s.w);
     }
     if (p.k_split > 1) cluster_sync_all();                         // (others' parts have been read: the next stages may come, or the block may leave)
     else __syncthreads();
@@ -489,15 +497,15 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
 }
 
 // ---- both, for few rows -------------------------------------------------------------------------------------------------------------
-// A cluster of eight blocks per tile of up to 16 rows.  RT: rank tiles a pass over the block's share of K.
-constexpr int LORA_CLUSTER = 8, LORA_FEW_RANKS = 128;
+// A cluster of eight blocks per tile of up to 16 rows.  RT: rank tiles, all of them in one pass over the block's share of K.
+constexpr int LORA_CLUSTER = 8, LORA_FEW_RANKS = 128, LORA_FEW_LD = 20;
 template <int KS, int OUT, int RT>
 __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams p) {
-  extern __shared__ __align__(16) float sm[];
-  constexpr int LD = 20;
-  float* red = sm;                                   // [8 warps][16][LD]
-  float* mine = red + 8 * 16 * LD;                   // [16 rows][VR]: this block's part of v
-  uint32_t* frags = reinterpret_cast<uint32_t*>(mine + 16 * p.VR);      // the sum, as parts
+  extern __shared__ __align__(128) uint8_t smem8[];
+  constexpr int LD = LORA_FEW_LD, VR = RT * 16, U = RT > 2 ? 1 : 2;
+  float* red = reinterpret_cast<float*>(smem8);                         // [8 warps][VR][LD]
+  float* mine = red + 8 * VR * LD;                                      // [16 rows][VR]: this block's part of v
+  uint32_t* frags = reinterpret_cast<uint32_t*>(mine + 16 * VR);        // the sum, as parts
   constexpr int PARTS = lora_parts<OUT>();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int rank = blockIdx.x % LORA_CLUSTER;
@@ -517,66 +525,64 @@ __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams
     const float scale = p.scale[tl.x];
     const int rts = p.VR >> 4, k0 = static_cast<int>(static_cast<long long>(p.kb32) * rank / LORA_CLUSTER), k1 = static_cast<int>(static_cast<long long>(p.kb32) * (rank + 1) / LORA_CLUSTER);
     const __nv_bfloat16 *xa = p.x + (g < n ? row_a : 0) * p.ldx + t4 * 8, *xb = p.x + (g + 8 < n ? row_b : 0) * p.ldx + t4 * 8;
-    for (int rt0 = 0; rt0 < rts; rt0 += RT) {
-      float acc[RT][2][4] = {};
-      for (int kb = k0 + warp; kb < k1; kb += 16) {
-        // two blocks of 32 k at a time
-        uint4 av[2][RT][2], xv[2][2];
+    float acc[RT][2][4] = {};
+    for (int kb = k0 + warp; kb < k1; kb += 8 * U) {
+      uint4 av[U][RT][2], xv[U][2];
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const int k = kb + u * 8;
-          const bool in = k < k1 && k * 32 + t4 * 8 < p.K;
+      for (int u = 0; u < U; ++u) {
+        const int k = kb + u * 8;
+        const bool in = k < k1 && k * 32 + t4 * 8 < p.K;
 #pragma unroll
-          for (int i = 0; i < RT; ++i)
+        for (int i = 0; i < RT; ++i)
 #pragma unroll
-            for (int h = 0; h < 2; ++h)
-              av[u][i][h] = rt0 + i < rts && k < k1 ? ldg_stream(a + ((static_cast<long long>(rt0 + i) * p.kb32 + k) * 2 + h) * 32) : make_uint4(0u, 0u, 0u, 0u);
-          xv[u][0] = in ? *reinterpret_cast<const uint4*>(xa + k * 32) : make_uint4(0u, 0u, 0u, 0u);
-          xv[u][1] = in && n > 8 ? *reinterpret_cast<const uint4*>(xb + k * 32) : make_uint4(0u, 0u, 0u, 0u);
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            if (j > 0 && n <= 8) break;
-#pragma unroll
-            for (int i = 0; i < RT; ++i) {
-              mma_bf16(acc[i][j], av[u][i][0].x, av[u][i][0].y, av[u][i][0].z, av[u][i][0].w, xv[u][j].x, xv[u][j].y);
-              mma_bf16(acc[i][j], av[u][i][1].x, av[u][i][1].y, av[u][i][1].z, av[u][i][1].w, xv[u][j].z, xv[u][j].w);
-            }
-          }
+          for (int h = 0; h < 2; ++h)
+            av[u][i][h] = i < rts && k < k1 ? ldg_stream(a + ((static_cast<long long>(i) * p.kb32 + k) * 2 + h) * 32) : make_uint4(0u, 0u, 0u, 0u);
+        xv[u][0] = in ? *reinterpret_cast<const uint4*>(xa + k * 32) : make_uint4(0u, 0u, 0u, 0u);
+        xv[u][1] = in && n > 8 ? *reinterpret_cast<const uint4*>(xb + k * 32) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        if (rt0 + i >= rts) break;
-        __syncthreads();
-        float* w = red + warp * 16 * LD;
+      for (int u = 0; u < U; ++u)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          *reinterpret_cast<float2*>(w + g * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][0], acc[i][j][1]);
-          *reinterpret_cast<float2*>(w + (g + 8) * LD + j * 8 + t4 * 2) = make_float2(acc[i][j][2], acc[i][j][3]);
-        }
-        __syncthreads();
-        const int r = tid & 15, c = tid >> 4;
-        float s = 0.f;
+          if (j > 0 && n <= 8) break;
 #pragma unroll
-        for (int q = 0; q < 8; ++q) s += red[(q * 16 + r) * LD + c];
-        mine[c * p.VR + (rt0 + i) * 16 + r] = c < n ? scale * s : 0.f;
+          for (int i = 0; i < RT; ++i) mma_bf16(acc[i][j], av[u][i][0].x, av[u][i][0].y, av[u][i][0].z, av[u][i][0].w, xv[u][j].x, xv[u][j].y);
+#pragma unroll
+          for (int i = 0; i < RT; ++i) mma_bf16(acc[i][j], av[u][i][1].x, av[u][i][1].y, av[u][i][1].z, av[u][i][1].w, xv[u][j].z, xv[u][j].w);
+        }
+    }
+    if (first < c1) lora_take<KS>(w, b + static_cast<long long>(first) * KS * 64);         // (on its way while the warps and the cluster meet)
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      if (j > 0 && n <= 8) break;
+#pragma unroll
+      for (int i = 0; i < RT; ++i) {
+        float* to = red + (warp * VR + i * 16 + g) * LD + j * 8 + t4 * 2;
+        *reinterpret_cast<float2*>(to) = make_float2(acc[i][j][0], acc[i][j][1]);
+        *reinterpret_cast<float2*>(to + 8 * LD) = make_float2(acc[i][j][2], acc[i][j][3]);
       }
     }
-    if (first < c1) lora_take<KS>(w, b + static_cast<long long>(first) * KS * 64);         // (on its way while the cluster meets)
+    __syncthreads();
+    for (int e = tid; e < n * VR; e += LORA_THREADS) {
+      const int c = e / VR, r = e % VR;
+      float s = 0.f;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) s += red[(q * VR + r) * LD + c];
+      mine[e] = scale * s;
+    }
     cluster_sync_all();
-    const int quads = p.VR >> 2;
-    for (int e = tid; e < 16 * quads; e += LORA_THREADS) {
-      const int r = e / quads, q = e - r * quads;
+    constexpr int LOG = KS == 1 ? 0 : KS == 2 ? 1 : 2;
+    for (int e = tid; e < n * (VR / 4); e += LORA_THREADS) {             // (rows behind the last: a product's rows do not touch one another)
+      const int c = e / (VR / 4), k = e % (VR / 4) * 4;
+      if (k >= p.VR) continue;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
       for (int z = 0; z < LORA_CLUSTER; ++z) {
-        const float4 w = ld_dsmem_f32x4(mine + r * p.VR + q * 4, z);
-        s.x += w.x; s.y += w.y; s.z += w.z; s.w += w.w;
+        const float4 q = ld_dsmem_f32x4(mine + e * 4, z);
+        s.x += q.x; s.y += q.y; s.z += q.z; s.w += q.w;
       }
-      lora_put(frags, p.slices, PARTS, KS, r, q * 4, s.x, s.y);
-      lora_put(frags, p.slices, PARTS, KS, r, q * 4 + 2, s.z, s.w);
+      lora_put(frags, p.slices, PARTS, LOG, c, k, s.x, s.y);
+      lora_put(frags, p.slices, PARTS, LOG, c, k + 2, s.z, s.w);
     }
     __syncthreads();
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
@@ -678,12 +684,22 @@ static int lora_down_launch(const LoraParams& p, int max_tiles, void* stream) {
                                        dim3(1, p.k_split, 1), p));
   return 0;
 }
+template <int KS, int OUT, int RT>
+static int lora_few_tiles(const LoraParams& p, int tiles, void* stream) {
+  VB_CHECK_CUDA((rm_smem<lora_few_kernel<KS, OUT, RT>>()));
+  const size_t smem = (8 * RT * 16 * LORA_FEW_LD + 16 * RT * 16) * sizeof(float) + static_cast<size_t>(p.VR >> 4) * lora_parts<OUT>() * 512;
+  VB_LAUNCH_PDL_CLUSTER((lora_few_kernel<KS, OUT, RT>), tiles * LORA_CLUSTER, LORA_THREADS, smem, stream, LORA_CLUSTER, p);
+  return 0;
+}
 template <int KS, int OUT>
 static int lora_few_launch(const LoraParams& p, int tiles, void* stream) {
-  const size_t smem = (8 * 16 * 20 + 16 * static_cast<size_t>(p.VR)) * sizeof(float) + static_cast<size_t>(p.VR >> 4) * lora_parts<OUT>() * 512;
-  if (p.VR == 16) VB_LAUNCH_PDL_CLUSTER((lora_few_kernel<KS, OUT, 1>), tiles * LORA_CLUSTER, LORA_THREADS, smem, stream, LORA_CLUSTER, p);
-  else VB_LAUNCH_PDL_CLUSTER((lora_few_kernel<KS, OUT, 4>), tiles * LORA_CLUSTER, LORA_THREADS, smem, stream, LORA_CLUSTER, p);
-  return 0;
+  const int rts = p.VR >> 4;
+  if constexpr (KS == 1 && OUT != LORA_GLU)
+    if (rts == 1) return lora_few_tiles<KS, OUT, 1>(p, tiles, stream);
+  if constexpr (KS <= 2)
+    if (rts <= 2) return lora_few_tiles<KS, OUT, 2>(p, tiles, stream);
+  if (rts <= 4) return lora_few_tiles<KS, OUT, 4>(p, tiles, stream);
+  return lora_few_tiles<KS, OUT, 8>(p, tiles, stream);
 }
 template <int OUT>
 static int lora_launch(LoraParams& p, int slots, void* stream) {
