@@ -33,6 +33,9 @@ struct MoeLayerParams {
   const uint8_t *up, *down;             // packed: [expert][tile][k block][rows][128 B], [tile of 128][k block of all experts][128][128 B]
   const int32_t* idx;                   // [T][top]
   const float *wts, *sgate;
+  const int32_t *ids, *table;           // of a step without a router's launch (else nullptr): token ids, [vocab][top]
+  const float* wsg;                     // ... and its shared expert's gate row
+  int vocab;
   __nv_bfloat16* act;                   // [3 parts][T top + T][ld_act]
   float* y;
   long long ldy, expert_bytes, part_stride;
@@ -65,6 +68,14 @@ __device__ __forceinline__ void st_dsmem_f32(const float* local_ptr, uint32_t ct
   uint32_t raddr;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(raddr) : "r"(smem_u32(local_ptr)), "r"(cta_rank));
   asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(raddr), "f"(v) : "memory");
+}
+// eight values of a row times eight fp32 ones
+__device__ __forceinline__ float ml_dot8(const uint4& x, const float* w) {
+  const float4 a = __ldg(reinterpret_cast<const float4*>(w)), b = __ldg(reinterpret_cast<const float4*>(w + 4));
+  float s = bf16_lo(x.x) * a.x;
+  s = fmaf(bf16_hi(x.x), a.y, s); s = fmaf(bf16_lo(x.y), a.z, s); s = fmaf(bf16_hi(x.y), a.w, s);
+  s = fmaf(bf16_lo(x.z), b.x, s); s = fmaf(bf16_hi(x.z), b.y, s); s = fmaf(bf16_lo(x.w), b.z, s);
+  return fmaf(bf16_hi(x.w), b.w, s);
 }
 // First the logits of the cluster's eight rows: a block's share of the experts, 16 at a time, by the rows of h on the matrix units, the fp32 matrix as three
 // bf16 parts (exact), the k blocks of 32 divided by the warps.  What a warp needs of the matrix is asked for before the rows of h are there (it is older than
@@ -106,10 +117,7 @@ __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const
     const __nv_bfloat16* hs = p.h + t * p.ldh;
     float s = 0.f;
     for (int k = tid * 8; k < p.W; k += THREADS * 8) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(p.wsg + k)), b = __ldg(reinterpret_cast<const float4*>(p.wsg + k + 4));
-      const uint4 x = *reinterpret_cast<const uint4*>(hs + k);
-      s = fmaf(bf16_lo(x.x), a.x, s); s = fmaf(bf16_hi(x.x), a.y, s); s = fmaf(bf16_lo(x.y), a.z, s); s = fmaf(bf16_hi(x.y), a.w, s);
-      s = fmaf(bf16_lo(x.z), b.x, s); s = fmaf(bf16_hi(x.z), b.y, s); s = fmaf(bf16_lo(x.w), b.z, s); s = fmaf(bf16_hi(x.w), b.w, s);
+      s += ml_dot8(*reinterpret_cast<const uint4*>(hs + k), p.wsg + k);
     }
     s = warp_sum(s);
     if (lane == 0) gate[warp] = s;
@@ -181,6 +189,33 @@ __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const
     if (tid < p.top) {
       idx[tid] = row[tid];
       wts[tid] = 1.f / p.top;
+    }
+    return;
+  }
+  if (E <= 32 && !(p.groups > 1 && p.keep < p.groups)) {
+    // an expert a lane of one warp, which counts by looking at the others in turn
+    if (warp != 0) return;
+    const bool in = lane < E;
+    const float l = in ? z[lane] : -INFINITY;
+    const float logit = p.kind == ML_SOFTMAX ? l + my_bias : l, score = p.kind == ML_SIGMOID ? 1.f / (1.f + expf(-l)) : logit;
+    const uint32_t key = in ? ml_key(p.kind == ML_SIGMOID ? score + my_bias : logit) : 0u;
+    int before = 0;
+#pragma unroll 8
+    for (int o = 0; o < 32; ++o) {
+      const uint32_t other = __shfl_sync(0xffffffffu, key, o);
+      before += other > key || (other == key && o < lane);
+    }
+    const bool taken = in && before < p.top;
+    float s = score;
+    if (p.kind != ML_SIGMOID) {
+      // (relative to the chosen ones' largest logit, or to all: the same one, unless NaN, which then reaches every weight)
+      const float mx = __shfl_sync(0xffffffffu, logit, __ffs(__ballot_sync(0xffffffffu, in && before == 0)) - 1);
+      s = expf(logit - mx);
+    }
+    const float sum = warp_sum((p.kind == ML_SOFTMAX_ALL ? in : taken) ? s : 0.f);
+    if (taken) {
+      idx[before] = lane;
+      wts[before] = s / (p.kind == ML_SIGMOID ? sum + 1e-20f : sum);
     }
     return;
   }
@@ -262,16 +297,17 @@ __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const
 __device__ __forceinline__ int ml_row_of(const MoeLayerParams& p, int pair) { return p.top == 1 ? pair : static_cast<int>(__umulhi(static_cast<uint32_t>(pair), p.top_inverse)); }
 
 // The step's rows by expert, built by every block for itself (at most 64 x 32 pairs): `active` lists the experts that have rows, the shared one (number E) last.
-// Shared memory: counts and sums of the warps [32], idx[P], weight[P], row[P + T] (place of a pair's activations), off[E + 2], active[E + 2], line[E + 2], rows of
-// an expert as bits [2 E].
+// Shared memory: counts and sums of the warps [32], idx[P], weight[P], row[P + T] (place of a pair's activations), first[E + 2] (an active
+// expert's rows among them), active[E + 2], line[E + 2], an expert's first row [E], its
+// rows as bits [2 E], gates [8].
 // `line`: where an active expert's work starts when all of it stands in one line (the blocks take equal parts of it); a unit of work, 32 rows of weights or a
 // block of 64 k, costs what its columns take.
 constexpr int ML_PLAN_HEAD = 32;
-__host__ __device__ inline int ml_plan_words(int T, int E, int top) { return ML_PLAN_HEAD + 3 * T * top + T + 5 * E + 8; }
+__host__ __device__ inline int ml_plan_words(int T, int E, int top) { return ML_PLAN_HEAD + 3 * T * top + T + 6 * E + 16; }
 struct MoePlanView {
-  int *n_active, *n_named, *scan, *idx, *off, *active, *row, *line;
+  int *n_active, *n_named, *scan, *idx, *first, *active, *row, *line, *place;
   uint32_t* bits;
-  float* w;
+  float *w, *gates;
 };
 __device__ __forceinline__ MoePlanView ml_view(int* s, int T, int E, int top) {
   MoePlanView v;
@@ -283,21 +319,96 @@ __device__ __forceinline__ MoePlanView ml_view(int* s, int T, int E, int top) {
   v.idx = s;
   v.w = reinterpret_cast<float*>(s + P);
   v.row = s + 2 * P;
-  v.off = v.row + P + T;
-  v.active = v.off + E + 2;
+  v.first = v.row + P + T;
+  v.active = v.first + E + 2;
   v.line = v.active + E + 2;
-  v.bits = reinterpret_cast<uint32_t*>(v.line + E + 2);
+  v.place = v.line + E + 2;
+  v.bits = reinterpret_cast<uint32_t*>(v.place + E);
+  v.gates = reinterpret_cast<float*>(v.bits + 2 * E);
   return v;
+}
+
+// Cost of a unit with n columns, in eighths of one with up to 8 (whose weights take longer to come than to multiply); measured as the times at which blocks of
+// such units end.
+__device__ __forceinline__ int ml_cost(int n, bool down) { return n <= 8 ? 8 : n <= 16 ? (down ? 12 : 10) : n <= 32 ? (down ? 24 : 18) : (down ? 56 : 38); }
+// what the router (or, in steps without one, the table) says of a pair: its expert (-1: none) and its weight
+__device__ __forceinline__ void ml_pair(const MoeLayerParams& p, int i, int& e, float& w) {
+  if (p.table) {
+    const int t = ml_row_of(p, i);
+    e = p.table[static_cast<long long>(min(max(p.ids[t], 0), p.vocab - 1)) * p.top + i - t * p.top];
+    w = 1.f / p.top;
+  } else {
+    e = p.idx[i];
+    w = p.wts[i];
+  }
+  if (e < 0 || e >= p.E) e = -1;
+}
+// The same for steps of at most 32 pairs, by each warp for itself: pairs of an expert find one another by their values.  (The list stands in the order of the
+// pairs; 0.6 us where the other way takes 1.8.)
+__device__ __forceinline__ void ml_build_few(const MoePlanView& v, const MoeLayerParams& p, int units, int shared_units, bool down) {
+  const int tid = threadIdx.x, lane = tid & 31, P = p.T * p.top;
+  int e = -1;
+  float w = 0.f;
+  if (lane < P) ml_pair(p, lane, e, w);
+  const int t = ml_row_of(p, lane);
+  const uint32_t all = 0xffffffffu, below = (1u << lane) - 1u;
+  const uint32_t twins = __match_any_sync(all, e >= 0 ? e * 64 + t : -1 - lane);        // pairs of one row that name one expert: the first takes all weights
+  if (__any_sync(all, __popc(twins) > 1)) {
+    float sum = w;
+    for (int j = 0; j < 32; ++j) {
+      const float other = __shfl_sync(all, w, j);
+      if (j != lane && (twins >> j & 1u)) sum += other;
+    }
+    w = sum;
+  }
+  const bool kept = e >= 0 && (twins & below) == 0u;
+  const uint32_t group = __match_any_sync(all, kept ? e : -1 - lane);
+  const bool leader = kept && (group & below) == 0u;
+  const uint32_t leaders = __ballot_sync(all, leader);
+  const int n = __popc(group), first = __ffs(group) - 1;
+  int r = leader ? n : 0, l = leader ? ml_cost(n, down) * units : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int rr = __shfl_up_sync(all, r, o), ll = __shfl_up_sync(all, l, o);
+    if (lane >= o) { r += rr; l += ll; }
+  }
+  const int r_all = __shfl_sync(all, r, 31), l_all = __shfl_sync(all, l, 31), m_all = __popc(leaders);
+  const int r0 = __shfl_sync(all, r - n, first);                 // (a leader's own: the rows of those in front)
+  if (tid < 32) {
+    if (leader) {
+      const int a = __popc(leaders & below);
+      v.active[a] = e;
+      v.first[a] = r - n;
+      v.line[a] = l - ml_cost(n, down) * units;
+    }
+    if (kept) {
+      v.row[r0 + __popc(group & below)] = lane;
+      v.w[lane] = w;
+    }
+    if (lane == 0) {
+      v.first[m_all] = r_all;
+      v.line[m_all] = l_all;
+      if (p.sff > 0) {
+        v.first[m_all + 1] = r_all + p.T;
+        v.active[m_all] = p.E;
+        v.line[m_all + 1] = l_all + ml_cost(p.T, down) * shared_units;
+      }
+      *v.n_active = m_all + (p.sff > 0 ? 1 : 0);
+    }
+  }
+  if (p.sff > 0 && tid < p.T) v.row[r_all + tid] = P + tid;
+  __syncthreads();
 }
 
 // ROUNDS: pairs a thread looks after (a step of 8 rows has at most one a thread).  An expert's rows are collected as bits, which sorts them and counts a
 // row once however often it names the expert.
-// Cost of a unit with n columns, in eighths of one with up to 8 (whose weights take longer to come than to multiply); measured as the times at which blocks of
-// such units end.
-__device__ __forceinline__ int ml_cost(int n, bool down) { return n <= 8 ? 8 : n <= 16 ? (down ? 12 : 10) : n <= 32 ? (down ? 24 : 18) : (down ? 56 : 38); }
 template <int ROUNDS>
 __device__ __forceinline__ void ml_build(const MoePlanView& v, const MoeLayerParams& p, int units, int shared_units, bool down) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, P = p.T * p.top, rounds = (P + ML_THREADS - 1) / ML_THREADS;
+  if (P <= 32) {
+    ml_build_few(v, p, units, shared_units, down);
+    return;
+  }
   int mine[ROUNDS] = {};
   float weight[ROUNDS] = {};
 #pragma unroll
@@ -306,11 +417,7 @@ __device__ __forceinline__ void ml_build(const MoePlanView& v, const MoeLayerPar
     const int i = tid + k * ML_THREADS;
     mine[k] = -1;
     weight[k] = 0.f;
-    if (i < P) {
-      const int e = p.idx[i];
-      mine[k] = e >= 0 && e < p.E ? e : -1;
-      weight[k] = p.wts[i];
-    }
+    if (i < P) ml_pair(p, i, mine[k], weight[k]);
   }
   for (int e = tid; e < 2 * p.E; e += ML_THREADS) v.bits[e] = 0u;
   if (tid == 0) *v.n_named = 0;
@@ -365,8 +472,9 @@ __device__ __forceinline__ void ml_build(const MoePlanView& v, const MoeLayerPar
   for (int k = 0; k < 4; ++k) {
     const int e = tid * 4 + k;
     if (e < p.E) {
-      v.off[e] = r0;
+      v.place[e] = r0;
       if (n[k] > 0) {
+        v.first[m0] = r0;
         v.line[m0] = l0;
         v.active[m0++] = e;
         l0 += ml_cost(n[k], down) * units;
@@ -375,10 +483,10 @@ __device__ __forceinline__ void ml_build(const MoePlanView& v, const MoeLayerPar
     }
   }
   if (tid == 0) {
-    v.off[p.E] = r_all;
-    v.off[p.E + 1] = r_all + (p.sff > 0 ? p.T : 0);
+    v.first[m_all] = r_all;
     v.line[m_all] = l_all;
     if (p.sff > 0) {
+      v.first[m_all + 1] = r_all + p.T;
       v.active[m_all] = p.E;
       v.line[m_all + 1] = l_all + ml_cost(p.T, down) * shared_units;
     }
@@ -389,7 +497,7 @@ __device__ __forceinline__ void ml_build(const MoePlanView& v, const MoeLayerPar
   if (twice) {
 #pragma unroll
     for (int k = 0; k < ROUNDS; ++k) {
-    if (k >= rounds) break;
+      if (k >= rounds) break;
       const int i = tid + k * ML_THREADS, t = ml_row_of(p, i), c = i - t * p.top;
       if (mine[k] < 0) continue;
       const int e = mine[k];
@@ -407,7 +515,7 @@ __device__ __forceinline__ void ml_build(const MoePlanView& v, const MoeLayerPar
     if (mine[k] >= 0) {
       const int i = tid + k * ML_THREADS, t = ml_row_of(p, i);
       const uint32_t b0 = v.bits[2 * mine[k]], b1 = v.bits[2 * mine[k] + 1], below = (1u << (t & 31)) - 1u;
-      v.row[v.off[mine[k]] + (t < 32 ? __popc(b0 & below) : __popc(b0) + __popc(b1 & below))] = i;
+      v.row[v.place[mine[k]] + (t < 32 ? __popc(b0 & below) : __popc(b0) + __popc(b1 & below))] = i;
       v.w[i] = weight[k];
     }
   }
@@ -422,7 +530,7 @@ struct MlWalk {
 __device__ __forceinline__ void ml_expert(MlWalk& w, const MoePlanView& v, int E, int units, int shared_units) {
   const int e = v.active[w.a];
   w.units = e < E ? units : shared_units;
-  w.step = ml_cost(v.off[e + 1] - v.off[e], w.down);
+  w.step = ml_cost(v.first[w.a + 1] - v.first[w.a], w.down);
 }
 __device__ __forceinline__ MlWalk ml_walk(const MoePlanView& v, int begin, int E, int units, int shared_units, bool down) {
   MlWalk w;
@@ -554,15 +662,15 @@ __device__ __forceinline__ MlUpUnit ml_up_unit(const MoeLayerParams& p, const Mo
   MlUpUnit m;
   const int e = v.active[at.a], row0 = at.unit * 32, tile = row0 / p.up_rows, r0 = row0 - tile * p.up_rows;
   m.w = p.up + e * p.expert_bytes + (static_cast<long long>(tile) * p.kb * p.up_rows + r0) * 128;
-  m.first = v.off[e];
-  m.n = v.off[e + 1] - m.first;
+  m.first = v.first[at.a];
+  m.n = v.first[at.a + 1] - m.first;
   m.passes = (m.n + NT * 8 - 1) / (NT * 8);
   return m;
 }
 // one activation, times its row's routing weight, as parts
 __device__ __forceinline__ void ml_store(const MoeLayerParams& p, const MoePlanView& v, int place, int col, float g, float u) {
   const int P = p.T * p.top, pr = v.row[place];
-  const float scale = pr < P ? v.w[pr] : (p.sgate ? p.sgate[pr - P] : 1.f);
+  const float scale = pr < P ? v.w[pr] : p.wsg ? v.gates[pr - P] : p.sgate ? p.sgate[pr - P] : 1.f;
   float hi, mid, lo;
   bf16_parts(ml_act(p.act_kind, g, u, p.limit, p.slope) * scale, hi, mid, lo);
   __nv_bfloat16* o = p.act + static_cast<long long>(pr) * p.ld_act + col;
@@ -608,6 +716,13 @@ __global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 2 : 1) moe_up_kernel(con
   };
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i) ask();
+  if (NT == 1 && p.wsg && warp < p.T && end > v.line[n_active - 1]) {       // (the block has units of the shared expert: its rows' gates, a row a warp)
+    const __nv_bfloat16* hs = p.h + warp * p.ldh;
+    float s = 0.f;
+    for (int k = lane * 8; k < p.W; k += 256) s += ml_dot8(*reinterpret_cast<const uint4*>(hs + k), p.wsg + k);
+    s = warp_sum(s);
+    if (lane == 0) v.gates[warp] = 1.f / (1.f + expf(-s));                   // (read behind the next barrier)
+  }
   int turn = 0;
   for (MlWalk at = start; at.at < end; ml_next(at, v, p.E, p.up_units, p.shared_units)) {
     const MlUpUnit m = ml_up_unit<NT>(p, v, at);
@@ -692,8 +807,8 @@ __device__ __forceinline__ MlDownPiece ml_down_piece(const MoeLayerParams& p, co
   m.k0 = at.unit;
   m.k1 = min(at.units, at.unit + (end - at.at + at.step - 1) / at.step);
   m.w = wt + static_cast<long long>(e) * (p.ff / 64) * 16384;
-  m.first = v.off[e];
-  m.n = v.off[e + 1] - m.first;
+  m.first = v.first[at.a];
+  m.n = v.first[at.a + 1] - m.first;
   m.passes = (m.n + NT * 8 - 1) / (NT * 8);
   return m;
 }
@@ -954,8 +1069,16 @@ int vb_moe_layer(float* d_y, long long ldy, const void* d_h, long long ldh, cons
   p.up_units = (gated ? 2 * ff : ff) / 32;
   p.shared_units = (gated ? 2 * shared_ff : shared_ff) / 32;
   VB_CHECK_ARG(p.wait_flag = wait_flag(WK_MOE_LAYER), "vb_moe_layer: no mapped host memory");
-  const size_t smem_route = (static_cast<size_t>(ML_ROUTE_THREADS / 32 * 16) * ML_ROUTE_CLUSTER + 2 * static_cast<size_t>(experts) + groups + 48) * 4;
-  VB_LAUNCH_PDL_CLUSTER(moe_layer_route_kernel, (T + ML_ROUTE_CLUSTER - 1) / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER, ML_ROUTE_THREADS, smem_route, stream, ML_ROUTE_CLUSTER, r);
+  if (kind == ML_TABLE && T <= 8) {
+    // (every block looks the experts up by itself, and those of the shared expert form its gates: a launch less)
+    p.table = router->d_table;
+    p.ids = d_ids;
+    p.vocab = router->vocab;
+    p.wsg = router->d_shared_gate;
+  } else {
+    const size_t smem_route = (static_cast<size_t>(ML_ROUTE_THREADS / 32 * 16) * ML_ROUTE_CLUSTER + 2 * static_cast<size_t>(experts) + groups + 48) * 4;
+    VB_LAUNCH_PDL_CLUSTER(moe_layer_route_kernel, (T + ML_ROUTE_CLUSTER - 1) / ML_ROUTE_CLUSTER * ML_ROUTE_CLUSTER, ML_ROUTE_THREADS, smem_route, stream, ML_ROUTE_CLUSTER, r);
+  }
   const int sms = sm_count();
   const long long most = static_cast<long long>(experts < T * top ? experts : T * top) * p.up_units + p.shared_units;
   const int grid_up = static_cast<int>(most < sms ? most : sms), nt = T <= 8 ? 1 : 4;
