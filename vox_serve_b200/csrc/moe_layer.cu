@@ -43,6 +43,7 @@ struct MoeLayerParams {
   float limit, slope;
   unsigned char* wait_flag;
   uint32_t top_inverse;                  // 2^32 / top, rounded up
+  int tile_inverse;                      // 2^16 / (units of a tile of up_rows), rounded up: exact below 2^15 units
 };
 
 // ---- router -----------------------------------------------------------------------------------------------------------------------
@@ -645,10 +646,13 @@ __device__ __forceinline__ void ml_rows(const __nv_bfloat16* (&r)[NT], const __n
 // calls f with 1, 2 or 4 column tiles, as `cols` columns need and the kernel has
 template <int NT, typename F>
 __device__ __forceinline__ void ml_by_columns(int cols, F&& f) {
-  if constexpr (NT == 1) f(std::integral_constant<int, 1>());
-  else if (cols <= 8) f(std::integral_constant<int, 1>());
-  else if (cols <= 16) f(std::integral_constant<int, 2>());
-  else f(std::integral_constant<int, 4>());
+  if constexpr (NT == 1) {
+    f(std::integral_constant<int, 1>());
+  } else {
+    if (cols <= 8) f(std::integral_constant<int, 1>());
+    else if (NT == 2 || cols <= 16) f(std::integral_constant<int, 2>());
+    else if constexpr (NT == 4) f(std::integral_constant<int, 4>());
+  }
 }
 
 // ---- gate | up ------------------------------------------------------------------------------------------------------------------
@@ -660,7 +664,7 @@ struct MlUpUnit {
 template <int NT>
 __device__ __forceinline__ MlUpUnit ml_up_unit(const MoeLayerParams& p, const MoePlanView& v, const MlWalk& at) {
   MlUpUnit m;
-  const int e = v.active[at.a], row0 = at.unit * 32, tile = row0 / p.up_rows, r0 = row0 - tile * p.up_rows;
+  const int e = v.active[at.a], tile = at.unit * p.tile_inverse >> 16, r0 = at.unit * 32 - tile * p.up_rows;
   m.w = p.up + e * p.expert_bytes + (static_cast<long long>(tile) * p.kb * p.up_rows + r0) * 128;
   m.first = v.first[at.a];
   m.n = v.first[at.a + 1] - m.first;
@@ -714,11 +718,12 @@ __global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 2 : 1) moe_up_kernel(con
     ml_next(ask_at, v, p.E, p.up_units, p.shared_units);
     if (ask_at.at < end) ask_m = ml_up_unit<NT>(p, v, ask_at);
   };
-#pragma unroll
+#pragma unroll 1                         // (once a launch: its instructions have to come first)
   for (int i = 0; i < SLOTS; ++i) ask();
   if (NT == 1 && p.wsg && warp < p.T && end > v.line[n_active - 1]) {       // (the block has units of the shared expert: its rows' gates, a row a warp)
     const __nv_bfloat16* hs = p.h + warp * p.ldh;
     float s = 0.f;
+#pragma unroll 8
     for (int k = lane * 8; k < p.W; k += 256) s += ml_dot8(*reinterpret_cast<const uint4*>(hs + k), p.wsg + k);
     s = warp_sum(s);
     if (lane == 0) v.gates[warp] = 1.f / (1.f + expf(-s));                   // (read behind the next barrier)
@@ -825,7 +830,7 @@ __device__ __forceinline__ void ml_result(const MoeLayerParams& p, int t, int co
   if (col + 3 < p.W) y[3] = s.w;
 }
 template <int NT, int SLOTS>
-__global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 2 : 1) moe_down_kernel(const MoeLayerParams p) {
+__global__ void __launch_bounds__(ML_THREADS, NT <= 2 ? 2 : 1) moe_down_kernel(const MoeLayerParams p) {
   extern __shared__ __align__(128) int smem[];
   constexpr int LD = ML_LD;
   float* sums = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(smem) + ml_ring_bytes(SLOTS));          // [8 warps][T][LD]
@@ -874,7 +879,7 @@ __global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 2 : 1) moe_down_kernel(c
       ask_kb = ask_m.k0;
     }
   };
-#pragma unroll
+#pragma unroll 1                         // (once a launch: its instructions have to come first)
   for (int i = 0; i < SLOTS; ++i) ask();
   float* mine = sums + warp * p.T * LD;
   for (int i = lane; i < p.T * (LD / 4); i += 32) reinterpret_cast<float4*>(mine)[i] = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -885,7 +890,7 @@ __global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 2 : 1) moe_down_kernel(c
     for (int pass = 0; pass < m.passes; ++pass) {
       const int n0 = pass * NT * 8, cols = m.n - n0;
       ml_by_columns<NT>(cols, [&](auto tiles) {
-        constexpr int N = decltype(tiles)::value, HALF = N > 2 ? 2 : N;            // (registers: activations of at most two column tiles at a time)
+        constexpr int N = decltype(tiles)::value, HALF = NT == 2 ? 1 : N > 2 ? 2 : N;      // (registers: activations of one or two column tiles at a time)
         float acc[2][N][4] = {};
         const __nv_bfloat16* ar[N];
         ml_rows<N>(ar, p.act + t4 * 8, p.ld_act, v, m.first + n0, cols, g, p, false);
@@ -1010,6 +1015,7 @@ int vb_moe_layer(float* d_y, long long ldy, const void* d_h, long long ldh, cons
   VB_CHECK_ARG(groups <= 1 || ((kind == ML_SIGMOID || kind == ML_SOFTMAX_ALL) && experts % groups == 0 && keep >= 1 && keep <= groups && keep * (experts / groups) >= top),
                "vb_moe_layer: %d groups (keep %d) do not fit %d experts, top %d", groups, keep, experts, top);
   VB_CHECK_ARG(ff >= 64 && ff % 64 == 0 && shared_ff >= 0 && shared_ff % 64 == 0, "vb_moe_layer: expert widths %d and %d must be multiples of 64", ff, shared_ff);
+  VB_CHECK_ARG(ff <= (1 << 17) && shared_ff <= (1 << 17), "vb_moe_layer: expert widths %d and %d; at most %d", ff, shared_ff, 1 << 17);
   VB_CHECK_ARG(act >= 0 && act <= 4 && (act != ML_CLAMPED_GLU || weights->limit > 0.f), "vb_moe_layer: activation %d, limit %f", act, weights->limit);
   const bool gated = act <= ML_CLAMPED_GLU;
   VB_CHECK_ARG(up_rows >= 32 && up_rows <= 128 && up_rows % 32 == 0 && (gated ? 2 * ff : ff) % up_rows == 0 && (gated ? 2 * shared_ff : shared_ff) % up_rows == 0,
@@ -1061,6 +1067,7 @@ int vb_moe_layer(float* d_y, long long ldy, const void* d_h, long long ldh, cons
   p.part_stride = static_cast<long long>(ml_act_elems(T, top, ff, shared_ff));
   p.kb = (W + 63) / 64;
   p.up_rows = up_rows;
+  p.tile_inverse = (65536 + up_rows / 32 - 1) / (up_rows / 32);
   p.expert_bytes = static_cast<long long>(gated ? 2 * ff : ff) * p.kb * 128;
   p.down_kb = (experts * ff + shared_ff) / 64;
   p.act_kind = act;
@@ -1081,27 +1088,30 @@ int vb_moe_layer(float* d_y, long long ldy, const void* d_h, long long ldh, cons
   }
   const int sms = sm_count();
   const long long most = static_cast<long long>(experts < T * top ? experts : T * top) * p.up_units + p.shared_units;
-  const int grid_up = static_cast<int>(most < sms ? most : sms), nt = T <= 8 ? 1 : 4;
+  const int grid_up = static_cast<int>(most < sms ? most : sms), nt = T <= 8 ? 1 : T <= 16 ? 2 : 4;
   const size_t plan_bytes = static_cast<size_t>(ml_plan_words(T, experts, top)) * 4;
-  // Ring places a warp: three where a block of the next kernel can then stand beside (steps of up to 8 rows: it has its first weights before this one ends).
-  constexpr int FEW = 3, MANY = 3;
-  const size_t smem_up = ml_ring_bytes(nt == 1 ? FEW : MANY) + static_cast<size_t>(2 * ML_WARPS) * 32 * (nt == 1 ? 8 : 40) * 4 + plan_bytes;
-#define ML_UP(NT, G, S)                                                              \
-  do {                                                                               \
-    VB_CHECK_CUDA((rm_smem<moe_up_kernel<NT, G, S>>()));                             \
-    VB_LAUNCH_PDL((moe_up_kernel<NT, G, S>), grid_up, ML_THREADS, smem_up, stream, p); \
+  // Ring places a warp: three where one block an SM runs, and where a block of the next kernel stands beside (steps of up to 8 rows: it has its first weights before
+  // this one ends); two in the down kernel of up to 16 rows, of which an SM then holds two.
+  constexpr int PLACES = 3;
+  const size_t smem_up = ml_ring_bytes(PLACES) + static_cast<size_t>(2 * ML_WARPS) * 32 * (nt == 1 ? 8 : nt * 8 + 8) * 4 + plan_bytes;
+#define ML_UP(NT, G)                                                                      \
+  do {                                                                                    \
+    VB_CHECK_CUDA((rm_smem<moe_up_kernel<NT, G, PLACES>>()));                             \
+    VB_LAUNCH_PDL((moe_up_kernel<NT, G, PLACES>), grid_up, ML_THREADS, smem_up, stream, p); \
   } while (0)
   if (gated) {
-    if (nt == 1) ML_UP(1, true, FEW);
-    else ML_UP(4, true, MANY);
+    if (nt == 1) ML_UP(1, true);
+    else if (nt == 2) ML_UP(2, true);
+    else ML_UP(4, true);
   } else {
-    if (nt == 1) ML_UP(1, false, FEW);
-    else ML_UP(4, false, MANY);
+    if (nt == 1) ML_UP(1, false);
+    else if (nt == 2) ML_UP(2, false);
+    else ML_UP(4, false);
   }
 #undef ML_UP
-  const size_t smem_down = ml_ring_bytes(nt == 1 ? FEW : MANY) + static_cast<size_t>(ML_WARPS) * T * ML_LD * 4 + plan_bytes;
-  const int blocks = (W + 31) / 32, fit = (nt == 1 && smem_down <= 112 * 1024 ? 2 : 1) * sms;
-  int cluster = 1;                       // one wave
+  const size_t smem_down = ml_ring_bytes(nt == 2 ? 2 : PLACES) + static_cast<size_t>(ML_WARPS) * T * ML_LD * 4 + plan_bytes;
+  const int blocks = (W + 31) / 32, fit = (nt <= 2 && smem_down <= 112 * 1024 ? 2 : 1) * sms;
+  int cluster = 1;                       // one wave, in powers of two (clusters of three leave SMs out: 69 us where two take 58)
   while (cluster < 8 && blocks * cluster * 2 <= fit) cluster *= 2;
   p.cluster = cluster;
 #define ML_DOWN(NT, S)                                                                                                  \
@@ -1109,8 +1119,9 @@ int vb_moe_layer(float* d_y, long long ldy, const void* d_h, long long ldh, cons
     VB_CHECK_CUDA((rm_smem<moe_down_kernel<NT, S>>()));                                                                 \
     VB_LAUNCH_PDL_CLUSTER((moe_down_kernel<NT, S>), blocks * cluster, ML_THREADS, smem_down, stream, cluster, p);       \
   } while (0)
-  if (nt == 1) ML_DOWN(1, FEW);
-  else ML_DOWN(4, MANY);
+  if (nt == 1) ML_DOWN(1, PLACES);
+  else if (nt == 2) ML_DOWN(2, 2);
+  else ML_DOWN(4, PLACES);
 #undef ML_DOWN
   return 0;
 }
