@@ -165,6 +165,50 @@ class LlamaWeights:
         return self.nbytes() - (2 * self.embed.numel() if self.embed is not None else 0)
 
 
+class LlamaAdapters:
+    """Low-rank adapters of many voices beside one LlamaWeights: per layer a bank (ops.LoraBank) for q | k | v, o, gate | up and down, ``slots`` adapters
+    of rank up to ``rank`` each.  ``LlamaEngine.set_adapters`` takes them; a step names every row's adapter through an ops.LoraPlan."""
+
+    PROJECTIONS = {"qkv": ("self_attn.q_proj", "self_attn.k_proj", "self_attn.v_proj"), "o": ("self_attn.o_proj",), "gu": ("mlp.gate_proj", "mlp.up_proj"),
+                   "down": ("mlp.down_proj",)}
+
+    def __init__(self, dims: LlamaDims, slots: int, rank: int, device="cuda"):
+        H, I, D = dims.hidden_size, dims.intermediate_size, dims.head_dim
+        hq, hkv = dims.num_attention_heads * D, dims.num_key_value_heads * D
+        shapes = {"qkv": (H, (hq, hkv, hkv)), "o": (hq, (H,)), "gu": (H, (I, I)), "down": (I, (H,))}
+        self.dims, self.slots, self.rank = dims, slots, rank
+        self.layers = [{name: ops.LoraBank(slots, K, widths, rank, device) for name, (K, widths) in shapes.items()} for _ in range(dims.num_hidden_layers)]
+
+    def load(self, slot: int, state: Dict[str, torch.Tensor], scale: float, prefix: str = "model.") -> None:
+        """state: ``<prefix>layers.<i>.<module>.lora_A.weight`` [r, in] and ``.lora_B.weight`` [out, r] as adapter checkpoints name them; modules that it leaves
+        out are not adapted.  scale: alpha / r.  Names that fit no module raise."""
+        left = set(state)
+        for i, banks in enumerate(self.layers):
+            for name, modules in self.PROJECTIONS.items():
+                bank, n0 = banks[name], 0
+                keys = [(f"{prefix}layers.{i}.{m}.lora_A.weight", f"{prefix}layers.{i}.{m}.lora_B.weight") for m in modules]
+                if any((a in state) != (b in state) for a, b in keys):
+                    raise VoxB200Error(f"adapter: layer {i}, {name}: an A without its B")
+                if not any(a in state for a, _ in keys):
+                    bank.clear(slot)
+                    continue
+                r = max(state[a].shape[0] for a, _ in keys if a in state)
+                a = torch.zeros(len(modules), r, bank.K, dtype=BF16, device=bank.a.device)
+                b = torch.zeros(bank.N, r, dtype=BF16, device=bank.a.device)
+                for s, (ka, kb) in enumerate(keys):
+                    if ka in state:
+                        rs = state[ka].shape[0]
+                        if tuple(state[ka].shape) != (rs, bank.K) or tuple(state[kb].shape) != (bank.widths[s], rs):
+                            raise VoxB200Error(f"adapter: {ka} {tuple(state[ka].shape)} and its B {tuple(state[kb].shape)} do not fit [r, {bank.K}], [{bank.widths[s]}, r]")
+                        a[s, :rs] = state[ka].to(a)
+                        b[n0:n0 + bank.widths[s], :rs] = state[kb].to(b)
+                        left -= {ka, kb}
+                    n0 += bank.widths[s]
+                bank.load(slot, a, b, scale)
+        if left:
+            raise VoxB200Error(f"adapter: no such modules: {sorted(left)[:4]}")
+
+
 class LlamaEngine:
     def __init__(self, weights: LlamaWeights, kv_cache: torch.Tensor, page_size: int, max_rows: int,
                  max_seq_len: int = 2304):
@@ -229,11 +273,33 @@ class LlamaEngine:
         gu_tiles = (I + self.gu_half - 1) // self.gu_half
         self.ssq = torch.zeros(max(1, (H + 127) // 128) * self.FUSED_MAX_ROWS, dtype=torch.float32, device=dev)
         self.rope_cs = torch.zeros(self.FUSED_MAX_ROWS, 2, D, dtype=torch.float32, device=dev)
+        self.adapters: Optional[LlamaAdapters] = None
 
     FUSED_MAX_ROWS = 64
 
+    def set_adapters(self, adapters: LlamaAdapters) -> None:
+        """Adapters that a step may name (``forward(adapters=plan)``).  Their products are one more plane beside the split-K planes of a projection, which its
+        consumer sums anyway; the gate/up projection leaves planes too in such a step."""
+        d, R = self.dims, self.max_rows
+        if (adapters.dims.hidden_size, adapters.dims.intermediate_size, len(adapters.layers)) != (d.hidden_size, d.intermediate_size, d.num_hidden_layers):
+            raise VoxB200Error("set_adapters: adapters of another model")
+        small = (max(self.split_qkv, self.split_o, self.split_down) + 1) * min(R, self.FUSED_MAX_ROWS)
+        rows = max(small, ops.WIDE_SPLIT_ROWS + R, 2 * R) if R >= ops.WIDE_MIN_ROWS else small
+        self.adapters = adapters
+        self.adapter_planes = torch.zeros(rows * max(self.qkv_w, d.hidden_size), dtype=torch.float32, device=self.device)
+        self.adapter_gu = torch.zeros(R * self.w.layers[0]["gu"].N, dtype=torch.float32, device=self.device)
+
     def _partials(self, split: int, rows: int, width: int) -> torch.Tensor:
         return self.partials[: split * rows * width].view(split, rows, width)
+
+    def _adapted(self, layer: int, name: str, x: torch.Tensor, split: int, adapters: ops.LoraPlan, tile_rows: int = 128) -> torch.Tensor:
+        """the split-K planes of a projection and, behind them, the plane of its adapters"""
+        w, bank = self.w.layers[layer][name], self.adapters.layers[layer][name]
+        R = x.shape[0]
+        planes = self.adapter_planes[:(split + 1) * R * w.N].view(split + 1, R, w.N)
+        ops.gemm(x, w, mode=1, split_k=split, out=planes[:split], tile_rows=tile_rows)
+        ops.lora(x, bank, adapters, out=planes[split])
+        return planes
 
     def _splits(self, rows: int) -> Tuple[int, int, int]:
         """split-K of the QKV / O / down projections of a step with ``rows`` token rows.  Decode-sized steps use the tuned
@@ -253,7 +319,8 @@ class LlamaEngine:
 
     def forward(self, input_ids: Optional[torch.Tensor], position_ids: torch.Tensor, n_rows: int,
                 last_rows: Optional[torch.Tensor] = None, n_out: Optional[int] = None,
-                plan: Optional[ops.RowPlan] = None, last_rows_offset: int = 0, head=None, want_hidden: bool = False):
+                plan: Optional[ops.RowPlan] = None, last_rows_offset: int = 0, head=None, want_hidden: bool = False,
+                adapters: Optional[ops.LoraPlan] = None):
         """input_ids / position_ids int32 [n_rows] on the device; self.plan must hold the step's row plan
         (ops.plan_rows).  Returns logits [n_out or n_rows, vocab] bf16 (a view of the static buffer).
         last_rows (int32 [n_out]) selects the rows whose logits are needed (prefill: qo_indptr[1:] - 1).
@@ -261,13 +328,15 @@ class LlamaEngine:
         whose inputs are sums of several embeddings or projected features, csm.py:647-654).  ``head``: the packed
         output head to use instead of ``w.lm_head`` (per-position heads of a depth decoder).  ``want_hidden``: also
         return the final-normed rows [n_out or n_rows, hidden] bf16, row-major (the backbone state a depth decoder
-        starts from, csm.py:290-300)."""
+        starts from, csm.py:290-300).  ``adapters``: the plan of the rows' adapters (ops.lora_plan; ``set_adapters`` first)."""
         d, w, R = self.dims, self.w, n_rows
+        if adapters is not None and self.adapters is None:
+            raise VoxB200Error("forward: the engine has no adapters (set_adapters)")
         plan = self.plan if plan is None else plan
         if R > self.max_rows:
             raise VoxB200Error(f"{R} rows exceed the engine's max_rows {self.max_rows}")
         hidden, normed = self.hidden[:R], self.normed[:R]
-        fused = R <= self.FUSED_MAX_ROWS and self.fused_ok and not self.force_unfused
+        fused = R <= self.FUSED_MAX_ROWS and self.fused_ok and not self.force_unfused and adapters is None
         first = input_ids if input_ids is not None and not fused and input_ids.numel() == R else None      # (its rows come with their norm)
         if input_ids is not None and first is None:
             ops.embedding(w.embed, input_ids, out=hidden)
@@ -278,7 +347,7 @@ class LlamaEngine:
                 x_final = self.normed_t.view_rows(R)
             ops.rmsnorm(hidden, w.norm, d.rms_norm_eps, out=x_final)
         else:
-            x_final = self._layers_unfused(position_ids, R, plan, first)
+            x_final = self._layers_unfused(position_ids, R, plan, first, adapters)
         if last_rows is not None:
             n_out = last_rows.numel() if n_out is None else n_out
             if isinstance(x_final, ops.TiledAct):      # a gather needs rows: those of the stream, then their norm
@@ -336,14 +405,15 @@ class LlamaEngine:
             ops.proj_residual(act_x, L["down"], hidden, self.fsplit_down, hidden_out=hidden, ssq_out=ssq,
                               hidden_tiles_out=hidden_t)
 
-    def _layers_unfused(self, position_ids: torch.Tensor, R: int, plan: ops.RowPlan, input_ids: Optional[torch.Tensor] = None):
+    def _layers_unfused(self, position_ids: torch.Tensor, R: int, plan: ops.RowPlan, input_ids: Optional[torch.Tensor] = None,
+                         adapters: Optional[ops.LoraPlan] = None):
         """8 launches per layer.  Activations travel between kernels in the tiled layout (the attention output only in
         decode-sized steps and only with VB_ATTN_TILED=1); returns what holds the final normed rows (a TiledAct then,
         else self.normed[:R]).  input_ids: the embedding rows are still to be fetched."""
         d, w = self.dims, self.w
         hq, hkv, D, H, I = d.num_attention_heads, d.num_key_value_heads, d.head_dim, d.hidden_size, d.intermediate_size
         hidden = self.hidden[:R]
-        tiled = R <= self.tiled_max_rows and self.tiled_acts
+        tiled = R <= self.tiled_max_rows and self.tiled_acts and adapters is None        # (adapters read rows)
         normed = self.normed_t.view_rows(R) if tiled else self.normed[:R]
         attn_tiled = tiled and self.attn_tiled and R <= self.FUSED_MAX_ROWS
         attn_o = self.attn_t.view_rows(R) if attn_tiled else self.attn[:R]
@@ -356,17 +426,28 @@ class LlamaEngine:
         q = self.q[:R]
         n_layers = len(w.layers)
         for i, L in enumerate(w.layers):
-            p = ops.gemm(normed, L["qkv"], mode=1, split_k=s_qkv, out=self._partials(s_qkv, R, self.qkv_w), tile_rows=D)
+            if adapters is None:
+                p = ops.gemm(normed, L["qkv"], mode=1, split_k=s_qkv, out=self._partials(s_qkv, R, self.qkv_w), tile_rows=D)
+            else:
+                p = self._adapted(i, "qkv", normed, s_qkv, adapters, D)
             ops.qkv_rope_append(p, self.kv_cache[i], position_ids, self.freq, plan, hq, hkv, D, q_out=q,
                                 interleave=d.rope_interleave, q_norm=L.get("qn"), k_norm=L.get("kn"),
                                 norm_eps=d.rms_norm_eps, qkv_bias=L.get("qkv_b"))
             ops.paged_attn(q, self.kv_map, i * self.pages_per_layer, plan, R, hkv, self.page_size, self.chunk,
                            self.attn_ws, out=attn_o, grid_ctas=self.attn_grid)
-            p = ops.gemm(attn_o if attn_tiled else attn_o.view(R, hq * D), L["o"], mode=1, split_k=s_o,
-                         out=self._partials(s_o, R, H))
+            if adapters is None:
+                p = ops.gemm(attn_o if attn_tiled else attn_o.view(R, hq * D), L["o"], mode=1, split_k=s_o,
+                             out=self._partials(s_o, R, H))
+            else:
+                p = self._adapted(i, "o", attn_o.view(R, hq * D), s_o, adapters)
             ops.reduce_residual_rmsnorm(p, hidden, L["ln2"], d.rms_norm_eps, hidden_out=hidden, normed_out=normed)
-            ops.gemm(normed, L["gu"], mode=2, out=act, tile_rows=2 * self.gu_half, n_out=I)
-            p = ops.gemm(act, L["down"], mode=1, split_k=s_dn, out=self._partials(s_dn, R, H))
+            if adapters is None:
+                ops.gemm(normed, L["gu"], mode=2, out=act, tile_rows=2 * self.gu_half, n_out=I)
+                p = ops.gemm(act, L["down"], mode=1, split_k=s_dn, out=self._partials(s_dn, R, H))
+            else:
+                gu = ops.gemm(normed, L["gu"], mode=1, out=self.adapter_gu[:R * L["gu"].N].view(1, R, L["gu"].N), tile_rows=2 * self.gu_half)
+                ops.lora_gate_up(normed, self.adapters.layers[i]["gu"], adapters, gu, self.gu_half, out=act)
+                p = self._adapted(i, "down", act, s_dn, adapters)
             nxt = w.layers[i + 1]["ln1"] if i + 1 < n_layers else w.norm
             ops.reduce_residual_rmsnorm(p, hidden, nxt, d.rms_norm_eps, hidden_out=hidden, normed_out=normed)
         return normed

@@ -40,6 +40,7 @@ are fp32.  ``dtype`` float32 runs everything in fp32 (sequential FMA chains, no 
 from __future__ import annotations
 
 import math
+import os
 from dataclasses import dataclass, field
 from typing import Any, Dict, List, Optional, Tuple
 
@@ -562,6 +563,7 @@ class HybridWeights:
                 if f.shared_ff:
                     w["s_gu_view"] = ops.PackedWeight(w["gu_all"].data[f.experts * gb:], 2 * f.shared_ff, cfg.width,
                                                       2 * half)
+                self._few_experts(f, w, "gu_all")
         else:
             w["gu"] = torch.stack([mat(p + f"mlp.e{e}.gate", p + f"mlp.e{e}.up") for e in range(f.experts)]).contiguous()
             w["down"] = torch.stack([mat(p + f"mlp.e{e}.down") for e in range(f.experts)]).contiguous()
@@ -900,11 +902,23 @@ class HybridWeights:
                 w["grouped"] = {"group_bytes": gb, "kb_total": (n_all + 63) // 64, "group_kb": f.ff // 64}
                 if f.shared_ff:
                     w["s_up_view"] = ops.PackedWeight(w["up_all"].data[f.experts * gb:], f.shared_ff, W, tr)
+                self._few_experts(f, w, "up_all")
         else:
             w["up"] = torch.stack([mat(p + f"mlp.e{e}.up") for e in range(f.experts)]).contiguous()
             w["down"] = torch.stack([mat(p + f"mlp.e{e}.down") for e in range(f.experts)]).contiguous()
             if f.shared_ff:
                 w["s_up"], w["s_down"] = dense(mat(p + "mlp.shared.up")), dense(mat(p + "mlp.shared.down"))
+
+    def _few_experts(self, f: "MoEConfig", w: Dict[str, Any], up: str) -> None:
+        """The stacked matrices as ``ops.moe_layer`` reads them (the same buffers): for decode steps of engines that ask for it
+        (``HybridEngine.few_experts``)."""
+        W = self.cfg.width
+        if W % 8 or f.shared_ff % 64 or w[up].tile_rows % 32 or f.top > 32 or f.experts > 1024:
+            return
+        grouped = f.router in ("sigmoid", "softmax_all") and f.groups > 1
+        w["few"] = (ops.MoeWeights(w[up], w["down_all"], f.experts, W, f.ff, f.shared_ff, act=f.act, limit=f.limit, slope=f.slope),
+                    ops.MoeRouter(f.router, f.top, weight=w.get("router"), bias=w.get({"softmax": "router_b", "sigmoid": "correction"}.get(f.router, "")),
+                                  groups=f.groups if grouped else 0, keep=f.groups_keep if grouped else 0, shared_gate=w.get("sg"), table=w.get("table")))
 
     # the dense mixture-of-experts form runs experts / top times the FLOPs a token needs: taken up to this ratio
     DENSE_MOE_MAX_RATIO = 8
@@ -1224,6 +1238,11 @@ class HybridEngine:
         self.use_tiled_attention = True
         self.use_tiled_recurrence = True
 
+    # Steps of few rows run a mixture-of-experts layer as ops.moe_layer: the chosen experts' matrices only, nothing rounded between the two products (the
+    # stacked form reads every expert's and rounds the activations to bf16).  Off by default: results change in their last bits.  VB_MOE_LAYER=1, or the attribute
+    # before the first step (decode steps are captured), turns it on.
+    few_experts = os.environ.get("VB_MOE_LAYER", "0") != "0"
+
     GROUP_TILE = 128          # rows per tile of the grouped expert projections
     GROUPED_MIN_ROWS = 512    # steps with at least this many rows run the experts grouped; smaller ones in the dense form
 
@@ -1441,6 +1460,8 @@ class HybridEngine:
         T, W = s.T, self.cfg.width
         h = self.h[:T] if h is None else h
         out = self.y[:T] if out is None else out
+        if self.few_experts and T <= ops.MOE_LAYER_MAX_ROWS and "few" in w:
+            return ops.moe_layer(h, *w["few"], ids=s.ids if f.router == "table" else None, out=out)
         if f.act not in ("silu_glu", "clamped_glu"):
             return self._moe_plain(f, w, s, h, out)
         idx, wts = self.moe_idx[:T * f.top], self.moe_wts[:T * f.top]
