@@ -272,9 +272,9 @@ __global__ void __launch_bounds__(LORA_THREADS, LoraDown<RT>::BLOCKS) lora_down_
 template <int KS, int PARTS>
 __device__ __forceinline__ void lora_block(float (&d)[4][4], const uint4* frags, const uint4 (&w)[KS][2]) {
 #pragma unroll
-  for (int k = 0; k < KS; ++k)
+  for (int q = PARTS - 1; q >= 0; --q)               // (the smallest parts first)
 #pragma unroll
-    for (int q = 0; q < PARTS; ++q) {
+    for (int k = 0; k < KS; ++k) {
       const uint4 f = frags[(q * KS + k) * 32];
       mma_bf16(d[0], f.x, f.y, f.z, f.w, w[k][0].x, w[k][0].y);
       mma_bf16(d[1], f.x, f.y, f.z, f.w, w[k][0].z, w[k][0].w);
@@ -298,7 +298,7 @@ __device__ __forceinline__ void lora_product(float (&d)[4][4], uint32_t frags, u
   for (int k = 0; k < KS; ++k) {
     const uint4 w0 = lds16(b + k * 1024), w1 = lds16(b + k * 1024 + 512);
 #pragma unroll
-    for (int q = 0; q < PARTS; ++q) {
+    for (int q = PARTS - 1; q >= 0; --q) {
       const uint4 f = lds16(frags + (q * KS + k) * 512);
       mma_bf16(d[0], f.x, f.y, f.z, f.w, w0.x, w0.y);
       mma_bf16(d[1], f.x, f.y, f.z, f.w, w0.z, w0.w);

@@ -11,6 +11,7 @@
 //         one row's experts from all of them
 //   up    block = (expert, 32 rows of its gate | up matrix: 16 gated or 32 plain columns), the eight warps divide k; sums meet in shared memory, the
 //         activation times the routing weight leaves as three bf16 parts (exact, rowmma.cuh), so nothing is rounded between the two products
+//         (the matrix units cut a sum off instead of rounding it: they add up a k block of 64, ordinary additions the k blocks)
 //   down  block = 32 columns of the result x an equal share of the chosen experts' k blocks, every warp adding its products to rows of its own in
 //         shared memory; up to eight blocks of a cluster divide the k blocks and add up through distributed shared memory.  No atomics: products,
 //         warps and blocks are added in a fixed order
@@ -138,6 +139,7 @@ __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         if (kb0 + u * WARPS >= kbs) break;
+        float sum[4] = {};
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           float v[2][4];
@@ -155,8 +157,10 @@ __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const
             f[2][q] = pack_cut(sa, sb);
           }
 #pragma unroll
-          for (int q = 0; q < 3; ++q) mma_bf16(acc, f[q][0], f[q][1], f[q][2], f[q][3], s ? x[u].z : x[u].x, s ? x[u].w : x[u].y);
+          for (int q = 2; q >= 0; --q) mma_bf16(sum, f[q][0], f[q][1], f[q][2], f[q][3], s ? x[u].z : x[u].x, s ? x[u].w : x[u].y);
         }
+#pragma unroll
+        for (int c = 0; c < 4; ++c) acc[c] += sum[c];
       }
     }
     if (i0 > 0) __syncthreads();                                  // (the sums before have been read)
@@ -759,14 +763,18 @@ __global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 2 : 1) moe_up_kernel(con
 #pragma unroll
           for (int j = 0; j < N; ++j)
 #pragma unroll
-            for (int s = 0; s < 2; ++s)
+            for (int i = 0; i < 2; ++i) {
+              float sum[4] = {};
 #pragma unroll
-              for (int i = 0; i < 2; ++i) {
+              for (int s = 0; s < 2; ++s) {
                 // gated: 16 gate rows, then their up rows; a product's upper half takes the one, its lower half the other
                 const uint4 lo = w[i][s], hi = w[i + 2][s];
-                mma_bf16(acc[i][j], lo.x, hi.x, lo.y, hi.y, x[j][s].x, x[j][s].y);
-                mma_bf16(acc[i][j], lo.z, hi.z, lo.w, hi.w, x[j][s].z, x[j][s].w);
+                mma_bf16(sum, lo.x, hi.x, lo.y, hi.y, x[j][s].x, x[j][s].y);
+                mma_bf16(sum, lo.z, hi.z, lo.w, hi.w, x[j][s].z, x[j][s].w);
               }
+#pragma unroll
+              for (int c = 0; c < 4; ++c) acc[i][j][c] += sum[c];
+            }
           __syncwarp();
           ring.read();
           ask();
@@ -919,15 +927,19 @@ __global__ void __launch_bounds__(ML_THREADS, NT <= 2 ? 2 : 1) moe_down_kernel(c
 #pragma unroll
             for (int j = 0; j < HALF; ++j)
 #pragma unroll
-              for (int part = 0; part < 3; ++part)
+              for (int i = 0; i < 2; ++i) {
+                float sum[4] = {};
 #pragma unroll
-                for (int s = 0; s < 2; ++s)
+                for (int part = 2; part >= 0; --part)            // (the smallest first)
 #pragma unroll
-                  for (int i = 0; i < 2; ++i) {
+                  for (int s = 0; s < 2; ++s) {
                     const uint4 lo = w[2 * i][s], hi = w[2 * i + 1][s];
-                    mma_bf16(acc[i][j0 + j], lo.x, hi.x, lo.y, hi.y, x[j][part][s].x, x[j][part][s].y);
-                    mma_bf16(acc[i][j0 + j], lo.z, hi.z, lo.w, hi.w, x[j][part][s].z, x[j][part][s].w);
+                    mma_bf16(sum, lo.x, hi.x, lo.y, hi.y, x[j][part][s].x, x[j][part][s].y);
+                    mma_bf16(sum, lo.z, hi.z, lo.w, hi.w, x[j][part][s].z, x[j][part][s].w);
                   }
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[i][j0 + j][c] += sum[c];
+              }
           }
           __syncwarp();
           ring.read();
