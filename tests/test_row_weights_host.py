@@ -116,3 +116,27 @@ def test_layer_needs_the_device():
     w = ops.MoeWeights(_packed(2 * 4 * 64, 72, 128), _packed(72, 4 * 64, 128), 4, 72, 64)
     with pytest.raises(VoxB200Error, match="current device"):
         ops.moe_layer(torch.zeros(1, 72, dtype=BF16), w, ops.MoeRouter("softmax", 2, weight=torch.zeros(4, 72)))
+
+
+def test_refused_adapters_leave_their_slot_as_it_was():
+    from vox_serve_b200.engine import LlamaAdapters, LlamaDims
+
+    rnd = torch.Generator().manual_seed(5)
+    bank = LlamaAdapters(LlamaDims(128, 2, 2, 1, 64, 256, 100), 2, 8, device="cpu")
+    key = "model.layers.%d.self_attn.q_proj.lora_%s.weight"
+    good = {key % (0, "A"): torch.randn(4, 128, generator=rnd), key % (0, "B"): torch.randn(128, 4, generator=rnd)}
+    bank.load(1, good, 2.0)
+    banks = [b for layer in bank.layers for b in layer.values()]
+    before = [(b.a.clone(), b.b.clone(), b.scale.clone()) for b in banks]
+    assert any(a.any() for a, _, _ in before)
+    other = {k: v + 1 for k, v in good.items()}
+    for more in ({"model.layers.2.self_attn.q_proj.lora_A.weight": torch.zeros(4, 128)},                    # no such layer
+                 {key % (1, "A"): torch.zeros(4, 128)},                                                     # an A without its B
+                 {key % (1, "A"): torch.zeros(4, 64), key % (1, "B"): torch.zeros(128, 4)},
+                 {key % (1, "A"): torch.zeros(9, 128), key % (1, "B"): torch.zeros(128, 9)}):               # a rank too many
+        with pytest.raises(VoxB200Error):
+            bank.load(1, {**other, **more}, 1.0)
+        for b, (a0, b0, s0) in zip(banks, before):
+            assert torch.equal(b.a, a0) and torch.equal(b.b, b0) and torch.equal(b.scale, s0)
+    with pytest.raises(VoxB200Error):
+        bank.load(2, good, 1.0)

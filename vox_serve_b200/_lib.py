@@ -325,7 +325,8 @@ LAUNCHES = {"vb_set_pdl": 0, "vb_set_trace": 0, "vb_weight_tiles_bytes": 0, "vb_
             "vb_set_gemm_smem_kb": 0, "vb_window_attn_tile_rows": 0, "vb_decay_attn_tile_rows": 0, "vb_decay_attn_tiled": 3, "vb_window_attn": 2, "vb_mingru_tiled": 3, "vb_mingru_scratch_floats": 0,
             "vb_short_conv": 2, "vb_selective_scan_tiled": 3, "vb_selective_scan_piece_rows": 0,
             "vb_selective_scan_scratch_floats": 0, "vb_sigmoid_attn": 1, "vb_ssd_tiled": 3, "vb_ssd_tile_rows": 0,
-            "vb_ssd_scratch_floats": 0, "vb_lora": 2, "vb_lora_gate_up": 2, "vb_moe_layer": 3}
+            "vb_ssd_scratch_floats": 0, "vb_lora_plan_bytes": 0, "vb_lora_workspace_bytes": 0, "vb_moe_layer_max_rows": 0,
+            "vb_moe_layer_workspace_bytes": 0, "vb_moe_layer": 2}
 launch_counter = [0]
 
 

@@ -182,7 +182,7 @@ class LlamaAdapters:
     def load(self, slot: int, state: Dict[str, torch.Tensor], scale: float, prefix: str = "model.") -> None:
         """state: ``<prefix>layers.<i>.<module>.lora_A.weight`` [r, in] and ``.lora_B.weight`` [out, r] as adapter checkpoints name them; modules that it leaves
         out are not adapted.  scale: alpha / r.  Names that fit no module raise."""
-        left = set(state)
+        left, loads = set(state), []
         for i, banks in enumerate(self.layers):
             for name, modules in self.PROJECTIONS.items():
                 bank, n0 = banks[name], 0
@@ -190,9 +190,11 @@ class LlamaAdapters:
                 if any((a in state) != (b in state) for a, b in keys):
                     raise VoxB200Error(f"adapter: layer {i}, {name}: an A without its B")
                 if not any(a in state for a, _ in keys):
-                    bank.clear(slot)
+                    loads.append((bank,))
                     continue
                 r = max(state[a].shape[0] for a, _ in keys if a in state)
+                if not 1 <= r <= self.rank:
+                    raise VoxB200Error(f"adapter: layer {i}, {name}: rank {r}; 1 to {self.rank}")
                 a = torch.zeros(len(modules), r, bank.K, dtype=BF16, device=bank.a.device)
                 b = torch.zeros(bank.N, r, dtype=BF16, device=bank.a.device)
                 for s, (ka, kb) in enumerate(keys):
@@ -204,9 +206,14 @@ class LlamaAdapters:
                         b[n0:n0 + bank.widths[s], :rs] = state[kb].to(b)
                         left -= {ka, kb}
                     n0 += bank.widths[s]
-                bank.load(slot, a, b, scale)
+                loads.append((bank, a, b))
         if left:
             raise VoxB200Error(f"adapter: no such modules: {sorted(left)[:4]}")
+        for bank, *ab in loads:                    # (only now: what is refused leaves the slot as it was)
+            if ab:
+                bank.load(slot, *ab, scale)
+            else:
+                bank.clear(slot)
 
 
 class LlamaEngine:

@@ -913,7 +913,8 @@ class HybridWeights:
         """The stacked matrices as ``ops.moe_layer`` reads them (the same buffers): for decode steps of engines that ask for it
         (``HybridEngine.few_experts``)."""
         W = self.cfg.width
-        if W % 8 or f.shared_ff % 64 or w[up].tile_rows % 32 or f.top > 32 or f.experts > 1024:
+        if (W % 8 or f.shared_ff % 64 or w[up].tile_rows % 32 or f.top > 32 or f.experts > 1024 or f.act not in ops.MOE_LAYER_ACTS
+                or (w.get("sg") is not None and f.router not in ("sigmoid", "table"))):
             return
         grouped = f.router in ("sigmoid", "softmax_all") and f.groups > 1
         w["few"] = (ops.MoeWeights(w[up], w["down_all"], f.experts, W, f.ff, f.shared_ff, act=f.act, limit=f.limit, slope=f.slope),

@@ -2027,6 +2027,7 @@ def lora(x: torch.Tensor, bank: LoraBank, plan: LoraPlan, out: Optional[torch.Te
     ws, ws_ptr, ws_bytes = bank._workspace(x, T)
     call("vb_lora", out.data_ptr(), ld_out, None if base is None else base.data_ptr(), N if base is None or T == 1 else base.stride(0), int(f32), x.data_ptr(),
          x.stride(0) if T > 1 else bank.K, bank._ptr, plan._ptr, T, ws_ptr, ws_bytes, _stream())
+    _lib.launch_counter[0] += ws_ptr is not None       # (two launches then; ``call`` counts one)
     return out
 
 
@@ -2059,6 +2060,7 @@ def lora_gate_up(x: torch.Tensor, bank: LoraBank, plan: LoraPlan, planes: torch.
     ws, ws_ptr, ws_bytes = bank._workspace(x, T)
     call("vb_lora_gate_up", to.data_ptr(), ld, xt, planes.data_ptr(), splits, half, x.data_ptr(), x.stride(0) if T > 1 else bank.K, bank._ptr, plan._ptr, T, ws_ptr,
          ws_bytes, _stream())
+    _lib.launch_counter[0] += ws_ptr is not None
     return out
 
 
@@ -2205,4 +2207,5 @@ def moe_layer(h: torch.Tensor, weights: MoeWeights, router: MoeRouter, ids: Opti
     n = (8 * P + 4 * T + 15) // 16 * 16 + 6 * (P + T) * max(weights.ff, weights.shared_ff)
     ws = h.new_empty(n // 2)                           # (of the allocator's, so that calls on other streams and captured graphs have their own)
     call("vb_moe_layer", out.data_ptr(), ld, h.data_ptr(), W, weights._ptr, router._ptr, None if ids is None else ids.data_ptr(), T, ws.data_ptr(), n, _stream())
+    _lib.launch_counter[0] += ids is None or T > 8     # (the router's launch)
     return out
