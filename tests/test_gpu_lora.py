@@ -233,6 +233,8 @@ def test_lora_many_adapters_and_rows():
 @pytest.mark.parametrize("T,K,rank,launches", [(9, 256, 16, 1), (9, 1024, 128, 2), (70, 256, 16, 2)])
 def test_lora_counts_its_launches(T, K, rank, launches):
     """a step of few rows whose adapters are small is one launch, every other two (128 x 3 columns of v are more than the one launch takes)"""
+    from vox_serve_b200 import ops
+
     widths = (128, 64, 64) if rank == 128 else (256,)
     bank = ops.LoraBank(2, K, widths, rank)
     plan = ops.lora_plan(ops.LoraPlan(T, 2), torch.zeros(T, dtype=I32, device="cuda"))
