@@ -21,6 +21,8 @@
 #define VB_PDL_FAMILY 4
 #include "rowmma.cuh"
 
+#include <type_traits>
+
 namespace vb {
 
 constexpr int LORA_MAX_SLOTS = 1023;       // (a thread of the planning block each, and one for rows without an adapter)
@@ -155,36 +157,27 @@ __global__ void __launch_bounds__(LORA_THREADS, LoraDown<RT>::BLOCKS) lora_down_
   const int s1 = (p.K + LORA_STAGE_K - 1) / LORA_STAGE_K, s0 = blockIdx.y, hop = p.k_split;
   // a thread's copies: 16 bytes of four rows, 16 bytes of every rank tile.  What is not there (rows behind the last, k behind K, rank tiles) is filled with zeros.
   const int chunk = tid & 15, row0 = tid >> 4;
-  const __nv_bfloat16* xr[4];
-  int x_bytes[4];
+  int xr[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const bool in = row0 + i * 16 < n;
-    xr[i] = p.x + (in ? rec[4 + row0 + i * 16] : 0) * p.ldx + chunk * 8;
-    x_bytes[i] = in ? 16 : 0;
-  }
+  for (int i = 0; i < 4; ++i) xr[i] = row0 + i * 16 < n ? rec[4 + row0 + i * 16] : -1;
+  const __nv_bfloat16* xs = p.x + chunk * 8;
   const uint32_t ring = smem_u32(smem8), x_to = ring + row0 * LORA_ROW_BYTES + chunk * 16, a_to = ring + LORA_X_BYTES + tid * 16;
   const float scale = p.scale[tl.x];
   const int kq = warp & 3, half = warp >> 2;
   const int tiles_n = min(4, max(0, (n - half * 32 + 7) >> 3));           // column tiles of 8 rows that this warp has
   const uint32_t a_from = ring + LORA_X_BYTES + (kq * 64 + lane) * 16, x_from = ring + (half * 32 + g) * LORA_ROW_BYTES + kq * 64 + t4 * 16;
   for (int rt0 = 0; rt0 < rts; rt0 += RT) {
-    const uint4* ar[RT];
-    int a_bytes[RT];
-#pragma unroll
-    for (int i = 0; i < RT; ++i) {
-      const bool in = rt0 + i < rts;
-      ar[i] = p.a + tl.x * p.a_slot + static_cast<long long>(in ? rt0 + i : 0) * p.kb32 * 64 + tid;
-      a_bytes[i] = in ? 16 : 0;
-    }
+    const uint4* ar = p.a + tl.x * p.a_slot + static_cast<long long>(rt0) * p.kb32 * 64 + tid;
+    const int here = min(RT, rts - rt0);
     auto load = [&](int s, uint32_t to) {
       if (s < s1) {
         const bool all = (s + 1) * LORA_STAGE_K <= p.K, in = all || s * LORA_STAGE_K + chunk * 8 < p.K, in_a = all || s * 4 + (tid >> 6) < p.kb32;
-        const long long x_at = in ? static_cast<long long>(s) * LORA_STAGE_K : 0, a_at = in_a ? static_cast<long long>(s) * 256 : 0;
+        const __nv_bfloat16* x = xs + (in ? static_cast<long long>(s) * LORA_STAGE_K : 0);
+        const uint4* a = ar + (in_a ? static_cast<long long>(s) * 256 : 0);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) cp_async16(x_to + to + i * 16 * LORA_ROW_BYTES, xr[i] + x_at, in ? x_bytes[i] : 0);
+        for (int i = 0; i < 4; ++i) cp_async16(x_to + to + i * 16 * LORA_ROW_BYTES, x + max(xr[i], 0) * p.ldx, in && xr[i] >= 0 ? 16 : 0);
 #pragma unroll
-        for (int i = 0; i < RT; ++i) cp_async16(a_to + to + i * 4096, ar[i] + a_at, in_a ? a_bytes[i] : 0);
+        for (int i = 0; i < RT; ++i) cp_async16(a_to + to + i * 4096, a + (i < here ? static_cast<long long>(i) * p.kb32 * 64 : 0), in_a && i < here ? 16 : 0);
       }
       cp_async_commit();
     };
@@ -197,26 +190,24 @@ __global__ void __launch_bounds__(LORA_THREADS, LoraDown<RT>::BLOCKS) lora_down_
       cp_async_wait<STAGES - 2>();
       __syncthreads();
       load(s + (STAGES - 1) * hop, free_at);
-      uint4 av[RT][2];
+      uint4 x[4];
 #pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        av[i][0] = lds16(a_from + at + i * 4096);
-        av[i][1] = lds16(a_from + at + i * 4096 + 512);
-      }
-      auto column = [&](int j) {
-        const uint4 x = lds16(x_from + at + j * 8 * LORA_ROW_BYTES);
+      for (int j = 0; j < 4; ++j) x[j] = lds16(x_from + at + j * 8 * LORA_ROW_BYTES);
+      auto rank_tile = [&](int i, auto full) {
+        const uint4 a0 = lds16(a_from + at + i * 4096), a1 = lds16(a_from + at + i * 4096 + 512);
 #pragma unroll
-        for (int i = 0; i < RT; ++i) mma_bf16(acc[i][j], av[i][0].x, av[i][0].y, av[i][0].z, av[i][0].w, x.x, x.y);
+        for (int j = 0; j < 4; ++j)
+          if (decltype(full)::value || j < tiles_n) mma_bf16(acc[i][j], a0.x, a0.y, a0.z, a0.w, x[j].x, x[j].y);
 #pragma unroll
-        for (int i = 0; i < RT; ++i) mma_bf16(acc[i][j], av[i][1].x, av[i][1].y, av[i][1].z, av[i][1].w, x.z, x.w);
+        for (int j = 0; j < 4; ++j)
+          if (decltype(full)::value || j < tiles_n) mma_bf16(acc[i][j], a1.x, a1.y, a1.z, a1.w, x[j].z, x[j].w);
       };
       if (tiles_n == 4) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) column(j);
-      } else {
+        for (int i = 0; i < RT; ++i) rank_tile(i, std::true_type());
+      } else if (tiles_n > 0) {
 #pragma unroll
-        for (int j = 0; j < 3; ++j)
-          if (j < tiles_n) column(j);
+        for (int i = 0; i < RT; ++i) rank_tile(i, std::false_type());
       }
       free_at = at;
       at = at == (STAGES - 1) * STAGE_BYTES ? 0 : at + STAGE_BYTES;
@@ -236,12 +227,20 @@ __global__ void __launch_bounds__(LORA_THREADS, LoraDown<RT>::BLOCKS) lora_down_
       }
     }
     __syncthreads();
-    for (int e = tid; e < n * RT * 16; e += LORA_THREADS) {
-      const int c = e / (RT * 16), r = e % (RT * 16);
-      float s = 0.f;
+    // (four rows a thread: eight lanes' 16 bytes lie in different banks)
+    for (int e = tid; e < ((n + 3) >> 2) * RT * 16; e += LORA_THREADS) {
+      const int c = e / (RT * 16) * 4, r = e % (RT * 16);
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int q = 0; q < 4; ++q) s += red[(((c >> 5) * 4 + q) * RT * 16 + r) * LD + (c & 31)];
-      mine[e] = scale * s;
+      for (int q = 0; q < 4; ++q) {
+        const float4 w = *reinterpret_cast<const float4*>(red + (((c >> 5) * 4 + q) * RT * 16 + r) * LD + (c & 31));
+        sum.x += w.x; sum.y += w.y; sum.z += w.z; sum.w += w.w;
+      }
+      float* to = mine + c * RT * 16 + r;
+      to[0] = scale * sum.x;
+      to[RT * 16] = scale * sum.y;
+      to[2 * RT * 16] = scale * sum.z;
+      to[3 * RT * 16] = scale * sum.w;
     }
     if (p.k_split > 1) cluster_sync_all();
     else __syncthreads();
@@ -333,13 +332,14 @@ __device__ __forceinline__ void lora_result(void* out, float (&y)[8], const void
     *static_cast<uint4*>(out) = lora_round(y);
   }
 }
-// ... of gate | up: `first` has the first plane's eight gate columns and, 16 further, their up columns.  (The fast exponential is off by 2 + 1.2 |g| units of 2^-23 and
+// ... of gate | up: g0, g1, u0, u1 are the first plane's eight gate and eight up columns.  (The fast exponential is off by 2 + 1.2 |g| units of 2^-23 and
 // the fast quotient by two: far below half a step of bf16, 2^-9.)
-__device__ __forceinline__ void lora_gated(const LoraParams& p, void* out, long long row, int col, float (&gv)[8], float (&uv)[8], const float* first) {
-  lora_add4(gv, *reinterpret_cast<const float4*>(first));
-  lora_add4(gv + 4, *reinterpret_cast<const float4*>(first + 4));
-  lora_add4(uv, *reinterpret_cast<const float4*>(first + 16));
-  lora_add4(uv + 4, *reinterpret_cast<const float4*>(first + 20));
+__device__ __forceinline__ void lora_gated(const LoraParams& p, void* out, long long row, int col, float (&gv)[8], float (&uv)[8], const float4& g0, const float4& g1,
+                                           const float4& u0, const float4& u1) {
+  lora_add4(gv, g0);
+  lora_add4(gv + 4, g1);
+  lora_add4(uv, u0);
+  lora_add4(uv + 4, u1);
   if (p.splits > 1)
 #pragma unroll 1
     for (int z = 1; z < p.splits; ++z) {
@@ -373,9 +373,12 @@ template <int OUT, bool TALL>
 struct LoraUp {
   static constexpr int WIDE = TALL && OUT != LORA_GLU ? 2 : 1;           // column blocks of a warp
   static constexpr int BLOCKS = TALL ? WIDE : 4;                         // ... of a step
-  static constexpr int ROW = lora_row_bytes<OUT>() * WIDE, LD = ROW + 16;
+  // (rows of planes are not padded, so that four blocks fit; their 16-byte pieces change places instead: lora_swap)
+  static constexpr int ROW = lora_row_bytes<OUT>() * WIDE, LD = OUT == LORA_GLU ? ROW : ROW + 16;
   static constexpr int ROWS_BYTES = (TALL ? 64 : 4 * 16) * LD;
 };
+// where piece q of row r of planes stands: the eight lanes of a 16-byte load have two neighbouring rows and pieces c, c + 2, c + 8, c + 10
+__device__ __forceinline__ int lora_swap(int r, int q) { return q ^ (r & 1) ^ (q >> 3 << 2); }
 template <int KS, int OUT, bool TALL>
 __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraParams p) {
   extern __shared__ __align__(128) uint8_t smem8[];
@@ -435,7 +438,7 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
           at = p.col0[s] + (block - p.block0[s]) * 32 + in_block * (OUT == LORA_F32 ? 4 : 8);
           in = at < p.col0[s + 1];
         }
-        const uint32_t row_to = to + rows_to + r0 * LD + q * 16;
+        const uint32_t row_to = to + rows_to + r0 * LD + (OUT == LORA_GLU ? lora_swap(r0, q) : q) * 16;
         const long long bytes_at = (in ? at : 0) * (OUT == LORA_BF16 ? 2 : 4);
 #pragma unroll
         for (int i = 0; i < 16 / ROWS; ++i)
@@ -476,7 +479,7 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
       }
       const int col = p.col0[s] + (block - p.block0[s]) * 32 + t4 * 8;
       if (col >= p.col0[s + 1]) continue;
-      const uint8_t* add = smem8 + (from - vs) + rows_to + ra * LD + (TALL ? w * SEG : 0) + (OUT == LORA_GLU ? (t4 >> 1) * 128 + (t4 & 1) * 32 : t4 * (SEG / 4));
+      const uint8_t* add = smem8 + (from - vs) + rows_to + ra * LD + (OUT == LORA_GLU ? 0 : (TALL ? w * SEG : 0) + t4 * (SEG / 4));
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         if (row[h] < 0) continue;
@@ -487,7 +490,11 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
           z[i] = u[i >> 1][h * 2 + (i & 1)];
         }
         void* out = lora_place<OUT>(p, row[h], col);
-        if constexpr (OUT == LORA_GLU) lora_gated(p, out, row[h], col, y, z, reinterpret_cast<const float*>(add + h * 8 * LD));
+        if constexpr (OUT == LORA_GLU) {
+          const float4* pl = reinterpret_cast<const float4*>(add + h * 8 * LD);
+          const int c = lora_swap(g, (t4 >> 1) * 8 + (t4 & 1) * 2);               // (its neighbour, and the up columns', differ in one bit)
+          lora_gated(p, out, row[h], col, y, z, pl[c], pl[c ^ 1], pl[c ^ 4], pl[c ^ 5]);
+        }
         else lora_result<OUT>(out, y, p.base ? add + h * 8 * LD : nullptr);
       }
     }
@@ -629,7 +636,7 @@ __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams
         z[i] = u[i >> 1][h * 2 + (i & 1)];
       }
       void* out = lora_place<OUT>(p, rows[h], col);
-      if constexpr (OUT == LORA_GLU) lora_gated(p, out, rows[h], col, y, z, reinterpret_cast<const float*>(&add[h][0]));
+      if constexpr (OUT == LORA_GLU) lora_gated(p, out, rows[h], col, y, z, add[h][0], add[h][1], add[h][4], add[h][5]);
       else lora_result<OUT>(out, y, p.base ? static_cast<const void*>(&add[h][0]) : nullptr);
     }
   }
@@ -667,7 +674,7 @@ static int lora_up_tiles(LoraParams& p, int max_tiles, int tiles, void* stream) 
   p.ahead = v_bytes + 2 * step <= VB_MAX_DYN_SMEM;     // (four slices of rank 128 beside a base leave room for one step only)
   const size_t smem = v_bytes + (p.ahead + 1) * step;
   // one wave of up to four blocks an SM (a wave and a few blocks take as long as two), a step each at least
-  const int fit = smem <= 56 * 1024 ? 4 : smem <= 75 * 1024 ? 3 : smem <= 113 * 1024 ? 2 : 1;
+  const int fit = smem <= 56 * 1024 ? 4 : smem <= 75 * 1024 ? 3 : smem <= 113 * 1024 ? 2 : 1;       // (227 KB and 1 KB of the system's a block make 228)
   int split = fit * sm_count() / tiles;
   const int most = (p.blocks + Up::BLOCKS - 1) / Up::BLOCKS;
   if (split > most) split = most;
