@@ -610,6 +610,11 @@ struct MlRing {
     parity ^= got == 0 ? 1u : 0u;
   }
 };
+// a warp that gave up: the copies on their way land before the block may leave
+__device__ __noinline__ void ml_land() {
+  const unsigned long long t0 = gtimer();
+  while (gtimer() - t0 < 2000000ull) __nanosleep(1000);
+}
 // shared memory of both kernels: the rings, their barriers, then the kernel's own
 template <int SLOTS>
 __device__ __forceinline__ MlRing<SLOTS> ml_ring(int* smem, int warp) {
@@ -804,6 +809,7 @@ __global__ void __launch_bounds__(ML_THREADS, NT == 1 ? 2 : 1) moe_up_kernel(con
       });
     }
   }
+  if (bw.dead) ml_land();
 }
 
 // ---- down -------------------------------------------------------------------------------------------------------------------------
@@ -966,6 +972,7 @@ __global__ void __launch_bounds__(ML_THREADS, NT <= 2 ? 2 : 1) moe_down_kernel(c
     }
     past(at, m);
   }
+  if (bw.dead) ml_land();
   __syncthreads();
   // the warps' sums, then the cluster's: each block adds up its share of the rows
   for (int i = tid; i < p.T * 8; i += ML_THREADS) {
