@@ -242,3 +242,26 @@ def test_lora_counts_its_launches(T, K, rank, launches):
     before = ops.launch_count()
     ops.lora(x, bank, plan)
     assert ops.launch_count() - before == launches
+
+
+@pytest.mark.parametrize("K,widths,rank", [(200, (264,), 16), (72, (40, 72), 128), (1032, (136, 8, 24), 64), (320, (64,), 24)])
+@pytest.mark.parametrize("order", ["prompts", "turns", "both"])
+def test_lora_rows_in_a_row_and_apart(K, widths, rank, order):
+    """rows of an adapter that follow one another in x (fetched as boxes, which reach past the adapter's rows and, for the last, past x), rows that alternate, and
+    both; x as columns of a wider matrix whose others, and whose rows behind the step's, are NaN"""
+    from vox_serve_b200 import ops
+
+    T, slots = 333, 4
+    runs = [0] * 129 + [3] * 70 + [-1] * 3 + [1] * 131
+    ids = runs if order == "prompts" else [t % 5 - 1 for t in range(T)] if order == "turns" else runs[:202] + [t % 5 - 1 for t in range(T - 202)]
+    bank, a, b, scale, _, x = _inputs(T, K, widths, rank, slots, seed=K + rank)
+    ids = torch.tensor(ids, dtype=I32, device="cuda")
+    wide = torch.full((T + 40, K + 48), float("nan"), dtype=BF16, device="cuda")
+    wide[:T, 16:16 + K] = x
+    plan = _plan(ids, slots)
+    got = ops.lora(wide[:T, 16:16 + K], bank, plan)
+    want, err = _delta64(x, a, b, scale, widths, ids, 0.0)
+    assert bool(((got.double() - want).abs() <= err + want.abs() * 2.0 ** -23 + 1e-30).all())
+    assert bool((got[ids < 0] == 0).all())
+    again = ops.lora(x, bank, _plan(ids, slots))            # the order of a step's rows is kept: the same sums
+    assert torch.equal(got, again)

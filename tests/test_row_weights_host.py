@@ -34,16 +34,14 @@ def test_bank_order_of_values():
     a = torch.arange(1, 2 * r * K + 1).view(2, r, K) % 251 + 1
     b = torch.arange(1, 48 * r + 1).view(48, r) % 241 + 1
     bank.load(0, a.float(), b.float(), 2.0)
-    A, B, kb = bank.a[0].float(), bank.b[0].float(), (K + 31) // 32
+    A, B, kb = bank.a[0].float(), bank.b[0].float(), (K + 63) // 64
     rp = bank.rank_pad
     seen = torch.zeros_like(A)
     for s in range(2):
         for j in range(r):
             for k in range(K):
                 row = s * rp + j
-                tile, g, h = row // 16, row % 8, row % 16 // 8
-                lane, step, pair, e = g * 4 + k % 32 // 8, k % 8 // 4, k % 4 // 2, k % 2
-                at = (((tile * kb + k // 32) * 2 + step) * 32 + lane) * 8 + (pair * 2 + h) * 2 + e
+                at = (k // 64 * 2 * rp + row) * 64 + (k % 64 // 8 ^ row % 8) * 8 + k % 8
                 assert A[at] == a[s, j, k]
                 seen[at] = 1
     assert not bool(A[seen == 0].any())

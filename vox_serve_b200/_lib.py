@@ -247,7 +247,7 @@ _lock = threading.Lock()
 _lib = None
 # flags in mapped host memory, one byte per kind of kernel whose waits give up (csrc/common.cuh, BoundedWait)
 _wait_flags = None
-WAIT_KINDS = ("a projection of a prompt step", "a vocoder convolution", "prompt attention", "window attention of a prompt", "vb_wait_check", "experts of a decode step")
+WAIT_KINDS = ("a projection of a prompt step", "a vocoder convolution", "prompt attention", "window attention of a prompt", "vb_wait_check", "experts of a decode step", "adapters of a prompt step")
 
 
 class VoxB200Error(RuntimeError):

@@ -3,17 +3,17 @@
 //   v[t, s r + j] = scale_a sum_k A_a[s, j, k] x[t, k]            (a: the adapter of row t; s: slice of the projection's columns, q | k | v)
 //   out[t, n] = base[t, n] + sum_j B_a[n, j] v[t, s(n) r + j]
 //
-//   vb_lora_plan      rows of a step by adapter: a table of row tiles that every projection of every layer works through
+//   vb_lora_plan      rows of a step by adapter: a table of row tiles, and of groups of them, that every projection of every layer works through
 //   vb_lora           out as fp32 (one more split-K plane of the projection: its consumer sums planes anyway) or as bf16 rows with a base
 //   vb_lora_gate_up   silu(gate) * up from the projection's fp32 planes with both adapters' products added
 //
-// A tile is up to 16 rows (steps of at most 64) or 64 rows of one adapter.  The bank keeps A and B in the order in which lanes take them (one 16-byte load per
-// lane and product step, 512 bytes in a row per warp).  Three kernels:
+// A tile is up to 16 rows (steps of at most 64) or 64 rows of one adapter, a group up to 128.  The bank keeps A as swizzled tiles of 16 ranks x 64 k, which the
+// tensor cores take as they are and lanes of mma.sync by 16-byte pieces, and B in the order in which lanes take it (512 bytes in a row per warp).  Three kernels:
 //
 //   few   steps of at most 64 rows whose adapters are small: one launch.  A cluster of eight blocks per tile divides K, adds up v through distributed
 //         shared memory and divides the columns
-//   down  v of any step: a tile x a piece of K a block, the blocks of a tile a cluster that adds up its parts
-//   up    a tile x some columns a block, all that it reads but v on its way before v is there
+//   down  v of any step: a group x a piece of K a block (tcgen05), the blocks of a group a cluster that adds up its parts
+//   up    a tile x some columns a block (mma.sync: as many products as loads), all that it reads but v on its way before v is there
 //
 // Sums are fp32.  v is not rounded on its way into the second product: it enters as three bf16 parts (exact, rowmma.cuh) where the result is fp32, as
 // two (off by 2^-15 of v at most) where the result is rounded to bf16 anyway.
@@ -21,77 +21,113 @@
 #define VB_PDL_FAMILY 4
 #include "rowmma.cuh"
 
-#include <type_traits>
-
 namespace vb {
 
 constexpr int LORA_MAX_SLOTS = 1023;       // (a thread of the planning block each, and one for rows without an adapter)
 constexpr int LORA_MAX_SLICES = 4;
+constexpr int LORA_MAX_ROWS = 1 << 21;     // (tiles are a launch's second dimension)
 constexpr int LORA_THREADS = 256;
+constexpr int LORA_DOWN_ROWS = 128;        // rows of a block of the first product
+constexpr int LORA_PLAN_SMEM = 32 * (LORA_MAX_SLOTS + 1) * 4;
 
 // ---- rows by adapter ------------------------------------------------------------------------------------------------------------
-// A record per tile: adapter or -1, first place among the sorted rows, rows (0: no tile), 0, then the rows.  One block: a counting sort in shared memory.  The
-// order of an adapter's rows among themselves may differ from run to run; a row's result does not depend on its place.
-__global__ void __launch_bounds__(1024) lora_plan_kernel(int32_t* __restrict__ tiles, const int32_t* __restrict__ ids, int T, int slots, int tile_rows, int max_tiles) {
-  __shared__ int cnt[1024], first_tile[1024];
-  __shared__ int warp_rows[32], warp_tiles[32];
+// A record per tile: adapter or -1, first place among the sorted rows, rows (0: no tile), 0, then the rows.  Behind them a record per group, the up to 128 rows of an
+// adapter (neighbouring tiles) that a block of the first product takes: first tile (-1: no group), adapter, rows, the first row if they follow one another in x,
+// else -1.  One block: a counting sort in shared memory
+// that keeps an adapter's rows in their order (rows that follow one another in x are then fetched as boxes): a warp a piece of the rows, its counts per adapter [32 warps]
+// [slots + 1], which become the first places of the warps' rows.
+__global__ void __launch_bounds__(1024) lora_plan_kernel(int32_t* __restrict__ tiles, const int32_t* __restrict__ ids, int T, int slots, int tile_rows, int max_tiles,
+                                                         int max_groups) {
+  extern __shared__ __align__(128) int cnt[];
+  __shared__ int first_tile[1024];
+  __shared__ int warp_rows[32], warp_tiles[32], warp_groups[32];
   pdl_sync();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, stride = 4 + tile_rows;
-  cnt[tid] = 0;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, stride = 4 + tile_rows, counts = slots + 1;
+  for (int i = tid; i < 32 * counts; i += 1024) cnt[i] = 0;
   __syncthreads();
-  for (int t = tid; t < T; t += 1024) {
-    const int a = ids[t];
-    atomicAdd(&cnt[a >= 0 && a < slots ? a : slots], 1);
+  const int per = (T + 1023) / 1024 * 32, end = min(T, (warp + 1) * per);
+  int* mine = cnt + warp * counts;
+  for (int t0 = warp * per; t0 < end; t0 += 32) {
+    const int t = t0 + lane;
+    int a = t < end ? ids[t] : -1;
+    a = a >= 0 && a < slots ? a : slots;
+    const uint32_t same = __match_any_sync(0xffffffffu, t < end ? a : -1 - lane);
+    if (t < end && (same & ((1u << lane) - 1u)) == 0u) mine[a] += __popc(same);
+    __syncwarp();
   }
   __syncthreads();
-  const int rows = tid <= slots ? cnt[tid] : 0, n = (rows + tile_rows - 1) / tile_rows;
-  int r = rows, m = n;                      // inclusive sums over the threads
+  int rows = 0;
+  if (tid <= slots)
+    for (int w = 0; w < 32; ++w) {
+      const int c = cnt[w * counts + tid];
+      cnt[w * counts + tid] = rows;
+      rows += c;
+    }
+  const int n = (rows + tile_rows - 1) / tile_rows;
+  const int groups = tid < slots ? (rows + LORA_DOWN_ROWS - 1) / LORA_DOWN_ROWS : 0;
+  int r = rows, m = n, q = groups;          // inclusive sums over the threads
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int rr = __shfl_up_sync(0xffffffffu, r, o), mm = __shfl_up_sync(0xffffffffu, m, o);
-    if (lane >= o) { r += rr; m += mm; }
+    const int rr = __shfl_up_sync(0xffffffffu, r, o), mm = __shfl_up_sync(0xffffffffu, m, o), qq = __shfl_up_sync(0xffffffffu, q, o);
+    if (lane >= o) { r += rr; m += mm; q += qq; }
   }
-  if (lane == 31) { warp_rows[warp] = r; warp_tiles[warp] = m; }
+  if (lane == 31) { warp_rows[warp] = r; warp_tiles[warp] = m; warp_groups[warp] = q; }
   __syncthreads();
   if (warp == 0) {
-    int a = warp_rows[lane], b = warp_tiles[lane];
+    int a = warp_rows[lane], b = warp_tiles[lane], c = warp_groups[lane];
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int aa = __shfl_up_sync(0xffffffffu, a, o), bb = __shfl_up_sync(0xffffffffu, b, o);
-      if (lane >= o) { a += aa; b += bb; }
+      const int aa = __shfl_up_sync(0xffffffffu, a, o), bb = __shfl_up_sync(0xffffffffu, b, o), cc = __shfl_up_sync(0xffffffffu, c, o);
+      if (lane >= o) { a += aa; b += bb; c += cc; }
     }
     warp_rows[lane] = a;
     warp_tiles[lane] = b;
+    warp_groups[lane] = c;
   }
   __syncthreads();
-  if (warp > 0) { r += warp_rows[warp - 1]; m += warp_tiles[warp - 1]; }
-  const int row0 = r - rows, tile0 = m - n, all = warp_tiles[31];
+  if (warp > 0) { r += warp_rows[warp - 1]; m += warp_tiles[warp - 1]; q += warp_groups[warp - 1]; }
+  const int row0 = r - rows, tile0 = m - n, all = warp_tiles[31], all_groups = warp_groups[31];
+  int4* group = reinterpret_cast<int4*>(tiles + static_cast<long long>(max_tiles) * stride);
   first_tile[tid] = tile0;
   for (int i = 0; i < n; ++i)
-    *reinterpret_cast<int4*>(tiles + static_cast<long long>(tile0 + i) * stride) =
-        make_int4(tid < slots ? tid : -1, row0 + i * tile_rows, min(tile_rows, rows - i * tile_rows), 0);
+    *reinterpret_cast<int4*>(tiles + static_cast<long long>(tile0 + i) * stride) = make_int4(tid < slots ? tid : -1, row0 + i * tile_rows, min(tile_rows, rows - i * tile_rows), 0);
   for (int i = all + tid; i < max_tiles; i += 1024) *reinterpret_cast<int4*>(tiles + static_cast<long long>(i) * stride) = make_int4(-1, 0, 0, 0);
+  for (int i = all_groups + tid; i < max_groups; i += 1024) group[i] = make_int4(-1, 0, 0, 0);
   __syncthreads();
-  cnt[tid] = 0;
-  __syncthreads();
-  for (int t = tid; t < T; t += 1024) {
-    int a = ids[t];
+  for (int t0 = warp * per; t0 < end; t0 += 32) {
+    const int t = t0 + lane;
+    int a = t < end ? ids[t] : -1;
     a = a >= 0 && a < slots ? a : slots;
-    const int at = atomicAdd(&cnt[a], 1), i = at / tile_rows;
-    tiles[static_cast<long long>(first_tile[a] + i) * stride + 4 + at - i * tile_rows] = t;
+    const uint32_t same = __match_any_sync(0xffffffffu, t < end ? a : -1 - lane), below = same & ((1u << lane) - 1u);
+    if (t < end) {
+      const int at = mine[a] + __popc(below), i = at / tile_rows;
+      tiles[static_cast<long long>(first_tile[a] + i) * stride + 4 + at - i * tile_rows] = t;
+    }
+    __syncwarp();
+    if (t < end && below == 0u) mine[a] += __popc(same);
+    __syncwarp();
+  }
+  __syncthreads();
+  for (int i = 0; i < groups; ++i) {
+    const int first = i * LORA_DOWN_ROWS, last = min(rows, first + LORA_DOWN_ROWS) - 1;
+    auto row = [&](int k) { return tiles[static_cast<long long>(tile0 + k / tile_rows) * stride + 4 + k % tile_rows]; };
+    const int a = row(first);
+    group[q - groups + i] = make_int4(tile0 + first / tile_rows, tid, last - first + 1, row(last) - a == last - first ? a : -1);
   }
 }
 
 struct LoraParams {
   const int32_t* tiles;            // records of 4 + tile_rows words
+  const int4* groups;
   int tile_rows;
   const __nv_bfloat16* x;
   long long ldx;
-  const uint4 *a, *b;              // [slots][S][rank / 16][K / 32][2][32 lanes], [slots][column blocks of 32][rank / 16][2][32 lanes]
+  const uint4 *a, *b;              // [slots][K / 64][S][rank / 16][16 ranks][128 B, swizzled], [slots][column blocks of 32][rank / 16][2][32 lanes]
   long long a_slot, b_slot;        // 16-byte units
   const float* scale;
   uint32_t* v;                     // [tiles][tile_rows / 16][S][parts][rank / 16][32 lanes][4]: v as the second product takes it
-  int T, K, kb32, rank_tiles, VR, k_split, parts;      // VR = S * rank
+  int T, K, rank_tiles, VR, k_split, parts;      // VR = S * rank
+  unsigned char* wait_flag;
   // second product
   int blocks;                      // column blocks of 32 over all slices (of gate | up: of one)
   int ahead;                       // 1: a step's copies go out a step ahead
@@ -131,140 +167,191 @@ template <int N>
 __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 // ---- first product: v = scale A x -------------------------------------------------------------------------------------------------
-// Block: a tile x a piece of K, in stages of 128 k: 256 bytes of each row of x and RT rank tiles of A, copied 16 bytes at a time with three to five stages on
-// their way.  (Bulk copies of a row's 256 bytes start one at a time: 79 us for 4096 rows of 8192 at rank 64.)  Rows are 320 bytes apart:
-// lanes 0 to 7 of a 16-byte load read two rows, which then lie in different banks.  Warps: four k blocks of 32 by two halves of the rows.  More than RT rank
-// tiles: x again.  The pieces of a tile are a cluster, which adds them up and leaves v in parts.
-constexpr int LORA_STAGE_K = 128, LORA_ROW_BYTES = 2 * LORA_STAGE_K + 64, LORA_X_BYTES = 64 * LORA_ROW_BYTES, LORA_RED_LD = 36;
+// Block: a group of up to 128 rows of an adapter x a piece of K, in stages of 64 k on the tensor cores (tcgen05): D[row][rank] += x[row][k] A[rank][k].  A lies in the
+// bank as the tensor cores read it, one bulk copy a stage; rows that follow one another in x come as boxes of a tensor map, others by 16-byte copies of four
+// warps (some 16 clocks an instruction of 512 bytes: that rate bounded a form with copies alone, at 38 us for 4096 rows of 8192 at rank 64 and the second
+// product; mma.sync from such copies was bound by its shared-memory reads: 36 us, 69 at rank 128; this form takes 34 and 48).  A fifth warp multiplies.  Rows behind
+// the last are whatever stands there, in lanes that nobody reads.  Stages go to ACCS sums in turn: the tensor cores cut a sum off at every step, and chains of a
+// quarter lose a quarter.  More than RT rank tiles: x again.  The pieces of K are a cluster, which adds them up and leaves v in parts.
+constexpr int LORA_STAGE_K = 64, LORA_X_BYTES = LORA_DOWN_ROWS * 128, LORA_DOWN_THREADS = 160, LORA_LOADERS = 128, LORA_BOX_ROWS = 64;
 template <int RT>
 struct LoraDown {
-  static constexpr int STAGES = RT == 8 || RT == 1 ? 4 : 3, BLOCKS = RT == 8 ? 1 : 2;
-  static constexpr int STAGE_BYTES = LORA_X_BYTES + RT * 4096;
-  static constexpr size_t SMEM = static_cast<size_t>(STAGES) * STAGE_BYTES;
-  static_assert(8 * RT * 16 * LORA_RED_LD * 4 + 64 * RT * 16 * 4 <= STAGES * STAGE_BYTES, "the sums stand where the stages stood");
+  static constexpr int N = RT * 16, ACCS = RT == 8 ? 2 : 4, COLS = RT == 8 ? 256 : ACCS * N < 32 ? 32 : ACCS * N, STAGES = RT == 8 ? 3 : RT == 4 ? 4 : 5;
+  static constexpr int STAGE_BYTES = LORA_X_BYTES + RT * 2048, LD = N + 4;
+  static constexpr size_t SMEM = 1024 + static_cast<size_t>(STAGES) * STAGE_BYTES + 256;       // (1 KB to align; barriers)
+  static_assert(LORA_DOWN_ROWS * LD * 4 <= STAGES * STAGE_BYTES, "the sums stand where the stages stood");
 };
 template <int RT>
-__global__ void __launch_bounds__(LORA_THREADS, LoraDown<RT>::BLOCKS) lora_down_kernel(const LoraParams p) {
+__global__ void __launch_bounds__(LORA_DOWN_THREADS, 2) lora_down_kernel(const LoraParams p, const __grid_constant__ CUtensorMap x_map) {
   extern __shared__ __align__(128) uint8_t smem8[];
-  constexpr int STAGES = LoraDown<RT>::STAGES, STAGE_BYTES = LoraDown<RT>::STAGE_BYTES, LD = LORA_RED_LD;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+  using D = LoraDown<RT>;
+  constexpr int STAGES = D::STAGES, LD = D::LD, AHEAD = STAGES > 3 ? STAGES - 2 : 2;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  uint8_t* base = smem8 + ((1024u - (smem_u32(smem8) & 1023u)) & 1023u);
+  uint64_t* full = reinterpret_cast<uint64_t*>(base + STAGES * D::STAGE_BYTES);
+  uint64_t *empty = full + STAGES, *done = empty + STAGES;
+  uint32_t* tmem_at = reinterpret_cast<uint32_t*>(done + 1);
   pdl_sync();
-  const int32_t* rec = p.tiles + static_cast<long long>(blockIdx.x) * (4 + p.tile_rows);
-  const int4 tl = *reinterpret_cast<const int4*>(rec);
-  if (tl.z == 0 || tl.x < 0) return;        // (all blocks of the cluster) no tile; no adapter: the second kernel does not look at v
-  const int n = tl.z, rts = p.VR >> 4;
-  // (the blocks of a tile take stages in turn, so that at any time they read neighbouring pieces of the rows)
-  const int s1 = (p.K + LORA_STAGE_K - 1) / LORA_STAGE_K, s0 = blockIdx.y, hop = p.k_split;
-  // a thread's copies: 16 bytes of four rows, 16 bytes of every rank tile.  What is not there (rows behind the last, k behind K, rank tiles) is filled with zeros.
-  const int chunk = tid & 15, row0 = tid >> 4;
-  int xr[4];
+  const int4 gr = p.groups[blockIdx.y];
+  if (gr.x < 0) return;                     // (all blocks of the cluster)
+  const int n = gr.z, rts = p.VR >> 4;
+  const bool boxes = gr.w >= 0;
+  if (warp == 4) {
+    tmem_alloc(tmem_at, D::COLS);
+    tmem_relinquish();
+  }
+  // (the blocks of a group take stages in turn, so that at any time they read neighbouring pieces of the rows)
+  const int s1 = (p.K + LORA_STAGE_K - 1) / LORA_STAGE_K, s0 = blockIdx.x, hop = p.k_split, turns = (s1 - s0 + hop - 1) / hop;
+  const float scale = p.scale[gr.y];
+  // a thread's copies: 16 bytes of eight rows.  k behind K is filled with zeros; rows behind the last hold anything.
+  const int chunk = tid & 7, row0 = (tid >> 3) & 15, n_boxes = (n + LORA_BOX_ROWS - 1) / LORA_BOX_ROWS;
+  int xr[8];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) xr[i] = row0 + i * 16 < n ? rec[4 + row0 + i * 16] : -1;
+  for (int i = 0; i < 8; ++i) {             // (all tiles of a group but the last are full)
+    const int r = row0 + i * 16;
+    xr[i] = !boxes && r < n ? p.tiles[static_cast<long long>(gr.x + r / p.tile_rows) * (4 + p.tile_rows) + 4 + r % p.tile_rows] : -1;
+  }
+  if (tid == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(full + i, boxes ? 1 : 1 + LORA_LOADERS / 32);
+      mbar_init(empty + i, 1);
+    }
+    mbar_init(done, 1);
+    fence_barrier_init();
+  }
   const __nv_bfloat16* xs = p.x + chunk * 8;
-  const uint32_t ring = smem_u32(smem8), x_to = ring + row0 * LORA_ROW_BYTES + chunk * 16, a_to = ring + LORA_X_BYTES + tid * 16;
-  const float scale = p.scale[tl.x];
-  const int kq = warp & 3, half = warp >> 2;
-  const int tiles_n = min(4, max(0, (n - half * 32 + 7) >> 3));           // column tiles of 8 rows that this warp has
-  const uint32_t a_from = ring + LORA_X_BYTES + (kq * 64 + lane) * 16, x_from = ring + (half * 32 + g) * LORA_ROW_BYTES + kq * 64 + t4 * 16;
-  for (int rt0 = 0; rt0 < rts; rt0 += RT) {
-    const uint4* ar = p.a + tl.x * p.a_slot + static_cast<long long>(rt0) * p.kb32 * 64 + tid;
+  const uint32_t ring = smem_u32(base), x_to = ring + row0 * 128 + ((chunk ^ (row0 & 7)) << 4);
+  BoundedWait bw{p.wait_flag};
+  __syncthreads();                          // (barriers and TMEM are there)
+  tc_fence_after();
+  const uint32_t tmem = *tmem_at;
+  int slot = 0;                             // place and parity run on from one pass over x to the next
+  uint32_t parity = 0u;
+  auto next = [&]() {
+    slot = slot + 1 == STAGES ? 0 : slot + 1;
+    parity ^= slot == 0 ? 1u : 0u;
+  };
+  for (int rt0 = 0, pass = 0; rt0 < rts; rt0 += RT, ++pass) {
     const int here = min(RT, rts - rt0);
-    auto load = [&](int s, uint32_t to) {
-      if (s < s1) {
-        const bool all = (s + 1) * LORA_STAGE_K <= p.K, in = all || s * LORA_STAGE_K + chunk * 8 < p.K, in_a = all || s * 4 + (tid >> 6) < p.kb32;
-        const __nv_bfloat16* x = xs + (in ? static_cast<long long>(s) * LORA_STAGE_K : 0);
-        const uint4* a = ar + (in_a ? static_cast<long long>(s) * 256 : 0);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) cp_async16(x_to + to + i * 16 * LORA_ROW_BYTES, x + max(xr[i], 0) * p.ldx, in && xr[i] >= 0 ? 16 : 0);
-#pragma unroll
-        for (int i = 0; i < RT; ++i) cp_async16(a_to + to + i * 4096, a + (i < here ? static_cast<long long>(i) * p.kb32 * 64 : 0), in_a && i < here ? 16 : 0);
-      }
-      cp_async_commit();
+    // (one lane) A of a stage, all its rank tiles in a row, and how many bytes the stage waits for
+    auto ask = [&](int s, uint32_t x_bytes) {
+      mbar_arrive_expect_tx(full + slot, here * 2048 + x_bytes);
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring + slot * D::STAGE_BYTES + LORA_X_BYTES),
+                   "l"(p.a + gr.y * p.a_slot + (static_cast<long long>(s) * rts + rt0) * 128), "r"(here * 2048), "r"(smem_u32(full + slot))
+                   : "memory");
     };
-    float acc[RT][4][4] = {};
+    if (boxes && warp == 0) {
+      for (int i = 0; i < turns; ++i) {
+        bw.wait(empty + slot, parity ^ 1u);
+        if (!__all_sync(0xffffffffu, !bw.dead)) bw.dead = true;
+        if (bw.dead) break;
+        const int s = s0 + i * hop;
+        if (lane == 0) {
+          ask(s, n_boxes * LORA_BOX_ROWS * 128);
+          for (int b = 0; b < n_boxes; ++b)
+            tma_load_2d(base + slot * D::STAGE_BYTES + b * LORA_BOX_ROWS * 128, &x_map, full + slot, s * LORA_STAGE_K, gr.w + b * LORA_BOX_ROWS);
+        }
+        __syncwarp();
+        next();
+      }
+    } else if (!boxes && warp < 4) {
+      int told = slot;                      // the oldest stage that the multiplying warp has not been told of
+      for (int i = 0; i < turns + AHEAD; ++i) {
+        if (i < turns && !bw.dead) {
+          const int s = s0 + i * hop;
+          bw.wait(empty + slot, parity ^ 1u);
+          if (!__all_sync(0xffffffffu, !bw.dead)) bw.dead = true;
+          if (!bw.dead) {
+            if (tid == 0) ask(s, 0u);
+            const uint32_t to = slot * D::STAGE_BYTES;
+            const bool in = s * LORA_STAGE_K + chunk * 8 < p.K;
+            const __nv_bfloat16* x = xs + (in ? static_cast<long long>(s) * LORA_STAGE_K : 0);
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) load(s0 + i * hop, i * STAGE_BYTES);
-    uint32_t at = 0, free_at = (STAGES - 1) * STAGE_BYTES;
+            for (int j = 0; j < 8; ++j)
+              if (xr[j] >= 0) cp_async16(x_to + to + j * 2048, x + xr[j] * p.ldx, in ? 16 : 0);
+          }
+          next();
+        }
+        cp_async_commit();
+        if (i >= AHEAD) {
+          cp_async_wait<AHEAD>();
+          fence_proxy_async();              // (what the copies wrote, for the tensor cores' reads)
+          __syncwarp();
+          if (lane == 0 && !bw.dead) mbar_arrive(full + told);
+          told = told + 1 == STAGES ? 0 : told + 1;
+        }
+      }
+    } else if (warp == 4) {
+      const uint32_t idesc = umma_idesc(128, here * 16, 1u);
+      for (int i = 0; i < turns; ++i) {
+        bw.wait(full + slot, parity);
+        if (!__all_sync(0xffffffffu, !bw.dead)) bw.dead = true;
+        if (bw.dead) break;
+        tc_fence_after();
+        const uint64_t x_desc = umma_desc_sw128_kmajor(ring + slot * D::STAGE_BYTES), a_desc = umma_desc_sw128_kmajor(ring + slot * D::STAGE_BYTES + LORA_X_BYTES);
+        if (elect_one()) {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) umma_bf16(tmem + i % D::ACCS * D::N, x_desc + 2 * k, a_desc + 2 * k, idesc, i >= D::ACCS || k > 0);
+          umma_commit(empty + slot);
+          if (i + 1 == turns) umma_commit(done);
+        }
+        __syncwarp();
+        next();
+      }
+    }
+    // the products are through: rows of sums where the stages stood
+    float* mine = reinterpret_cast<float*>(base);                  // [128 rows][LD]
+    bw.wait(done, pass & 1);
+    tc_fence_after();
+    if (warp * 32 < n && warp < 4) {
 #pragma unroll 1
-    for (int s = s0; s < s1; s += hop) {
-      cp_async_wait<STAGES - 2>();
-      __syncthreads();
-      load(s + (STAGES - 1) * hop, free_at);
-      uint4 x[4];
+      for (int c0 = 0; c0 < here * 16; c0 += 16) {
+        float s[16];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) x[j] = lds16(x_from + at + j * 8 * LORA_ROW_BYTES);
-      auto rank_tile = [&](int i, auto full) {
-        const uint4 a0 = lds16(a_from + at + i * 4096), a1 = lds16(a_from + at + i * 4096 + 512);
+        for (int q = 0; q < D::ACCS; ++q) {
+          if (q > 0 && q >= turns) break;
+          uint32_t v[16];
+          tmem_ld_32x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + q * D::N + c0, v);
+          tmem_ld_wait();
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (decltype(full)::value || j < tiles_n) mma_bf16(acc[i][j], a0.x, a0.y, a0.z, a0.w, x[j].x, x[j].y);
+          for (int j = 0; j < 16; ++j) s[j] = q == 0 ? __uint_as_float(v[j]) : s[j] + __uint_as_float(v[j]);
+        }
+        float4* to = reinterpret_cast<float4*>(mine + (warp * 32 + lane) * LD + c0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (decltype(full)::value || j < tiles_n) mma_bf16(acc[i][j], a1.x, a1.y, a1.z, a1.w, x[j].z, x[j].w);
-      };
-      if (tiles_n == 4) {
-#pragma unroll
-        for (int i = 0; i < RT; ++i) rank_tile(i, std::true_type());
-      } else if (tiles_n > 0) {
-#pragma unroll
-        for (int i = 0; i < RT; ++i) rank_tile(i, std::false_type());
-      }
-      free_at = at;
-      at = at == (STAGES - 1) * STAGE_BYTES ? 0 : at + STAGE_BYTES;
-    }
-    cp_async_wait<0>();
-    __syncthreads();
-    float* red = reinterpret_cast<float*>(smem8);                  // [8 warps][RT * 16][LD]
-    float* mine = red + 8 * RT * 16 * LD;                          // [64 rows][RT * 16]
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j >= tiles_n) break;
-#pragma unroll
-      for (int i = 0; i < RT; ++i) {
-        float* w = red + (warp * RT + i) * 16 * LD + j * 8 + t4 * 2;
-        *reinterpret_cast<float2*>(w + g * LD) = make_float2(acc[i][j][0], acc[i][j][1]);
-        *reinterpret_cast<float2*>(w + (g + 8) * LD) = make_float2(acc[i][j][2], acc[i][j][3]);
+        for (int j = 0; j < 4; ++j) to[j] = make_float4(scale * s[4 * j], scale * s[4 * j + 1], scale * s[4 * j + 2], scale * s[4 * j + 3]);
       }
     }
-    __syncthreads();
-    // (four rows a thread: eight lanes' 16 bytes lie in different banks)
-    for (int e = tid; e < ((n + 3) >> 2) * RT * 16; e += LORA_THREADS) {
-      const int c = e / (RT * 16) * 4, r = e % (RT * 16);
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const float4 w = *reinterpret_cast<const float4*>(red + (((c >> 5) * 4 + q) * RT * 16 + r) * LD + (c & 31));
-        sum.x += w.x; sum.y += w.y; sum.z += w.z; sum.w += w.w;
-      }
-      float* to = mine + c * RT * 16 + r;
-      to[0] = scale * sum.x;
-      to[RT * 16] = scale * sum.y;
-      to[2 * RT * 16] = scale * sum.z;
-      to[3 * RT * 16] = scale * sum.w;
-    }
+    tc_fence_before();
     if (p.k_split > 1) cluster_sync_all();
     else __syncthreads();
     const int log_ks = 31 - __clz(p.rank_tiles);
-    uint32_t* v = p.v + static_cast<long long>(blockIdx.x) * (p.tile_rows >> 4) * rts * p.parts * 128;
-    for (int e = blockIdx.y * LORA_THREADS + tid; e < n * RT * 4; e += p.k_split * LORA_THREADS) {
-      const int c = e / (RT * 4), k = rt0 * 16 + e % (RT * 4) * 4;
-      if (k >= p.VR) continue;
+    uint32_t* v = p.v + static_cast<long long>(gr.x) * (p.tile_rows >> 4) * rts * p.parts * 128;
+    for (int e = blockIdx.x * LORA_DOWN_THREADS + tid; e < n * RT * 4; e += p.k_split * LORA_DOWN_THREADS) {
+      const int c = e / (RT * 4), k = e % (RT * 4) * 4;
+      if (rt0 * 16 + k >= p.VR) continue;
       float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
       if (p.k_split > 1) {
 #pragma unroll 4
         for (int z = 0; z < p.k_split; ++z) {
-          const float4 w = ld_dsmem_f32x4(mine + e * 4, z);
+          const float4 w = ld_dsmem_f32x4(mine + c * LD + k, z);
           s.x += w.x; s.y += w.y; s.z += w.z; s.w += w.w;
         }
       } else {
-        s = *reinterpret_cast<const float4*>(mine + e * 4);
+        s = *reinterpret_cast<const float4*>(mine + c * LD + k);
       }
-      lora_put(v, p.slices, p.parts, log_ks, c, k, s.x, s.y);
-      lora_put(v, p.slices, p.parts, log_ks, c, k + 2, s.z, s.w);
+      lora_put(v, p.slices, p.parts, log_ks, c, rt0 * 16 + k, s.x, s.y);
+      lora_put(v, p.slices, p.parts, log_ks, c, rt0 * 16 + k + 2, s.z, s.w);
     }
-    if (p.k_split > 1) cluster_sync_all();                         // (others' parts have been read: the next stages may come, or the block may leave)
+    fence_proxy_async();                                           // (others' parts have been read: the next stages may come, or the block may leave)
+    if (p.k_split > 1) cluster_sync_all();
     else __syncthreads();
+    tc_fence_after();
   }
+  if (bw.dead) {                            // let the copies in flight land before the block may leave
+    const unsigned long long t0 = gtimer();
+    while (gtimer() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  if (warp == 4) tmem_dealloc(tmem, D::COLS);
 }
 
 // ---- second product ---------------------------------------------------------------------------------------------------------------
@@ -386,11 +473,11 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
   constexpr int PARTS = lora_parts<OUT>(), B_BYTES = KS * 1024, SEG = lora_row_bytes<OUT>(), LD = Up::LD, WIDE = Up::WIDE, STEP = Up::BLOCKS, BOTH = OUT == LORA_GLU ? 2 : 1;
   constexpr int TILE = TALL ? 64 : 16;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
-  const int32_t* rec = p.tiles + static_cast<long long>(blockIdx.x) * (4 + TILE);
+  const int32_t* rec = p.tiles + static_cast<long long>(blockIdx.y) * (4 + TILE);
   const int4 tl = *reinterpret_cast<const int4*>(rec);
   // (ranges in whole steps)
   const int n = tl.z, all = (p.blocks + STEP - 1) / STEP;
-  const int c0 = static_cast<int>(static_cast<long long>(all) * blockIdx.y / gridDim.y) * STEP, c1 = min(p.blocks, static_cast<int>(static_cast<long long>(all) * (blockIdx.y + 1) / gridDim.y) * STEP);
+  const int c0 = static_cast<int>(static_cast<long long>(all) * blockIdx.x / gridDim.x) * STEP, c1 = min(p.blocks, static_cast<int>(static_cast<long long>(all) * (blockIdx.x + 1) / gridDim.x) * STEP);
   const bool has = tl.x >= 0;
   if (n == 0 || c0 >= c1) {
     pdl_sync();
@@ -452,7 +539,7 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
   load(c0, 0);
   pdl_sync();
   if (has) {
-    const uint4* v = reinterpret_cast<const uint4*>(p.v) + static_cast<long long>(blockIdx.x) * (TILE / 16) * p.slices * PARTS * KS * 32;
+    const uint4* v = reinterpret_cast<const uint4*>(p.v) + static_cast<long long>(blockIdx.y) * (TILE / 16) * p.slices * PARTS * KS * 32;
     for (int i = tid; i < v_bytes / 16; i += LORA_UP_THREADS) cp_async16(vs + i * 16, v + i, 16);
   }
   cp_async_commit();
@@ -528,9 +615,10 @@ __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams
   const long long rows[2] = {g < n ? row_a : -1, g + 8 < n ? row_b : -1};
   uint4 w[KS][2];
   if (has) {
-    const uint4* a = p.a + tl.x * p.a_slot + lane;
+    const uint4* a = p.a + tl.x * p.a_slot + g * 8;
+    const int even = t4 ^ g, odd = (4 + t4) ^ g;       // where this lane's eight k of 64 stand, of an even block of 32 and an odd one
     const float scale = p.scale[tl.x];
-    const int rts = p.VR >> 4, k0 = static_cast<int>(static_cast<long long>(p.kb32) * rank / LORA_CLUSTER), k1 = static_cast<int>(static_cast<long long>(p.kb32) * (rank + 1) / LORA_CLUSTER);
+    const int rts = p.VR >> 4, kb32 = (p.K + 31) / 32, k0 = kb32 * rank / LORA_CLUSTER, k1 = kb32 * (rank + 1) / LORA_CLUSTER;
     const __nv_bfloat16 *xa = p.x + (g < n ? row_a : 0) * p.ldx + t4 * 8, *xb = p.x + (g + 8 < n ? row_b : 0) * p.ldx + t4 * 8;
     float acc[RT][2][4] = {};
     for (int kb = k0 + warp; kb < k1; kb += 8 * U) {
@@ -543,7 +631,7 @@ __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams
         for (int i = 0; i < RT; ++i)
 #pragma unroll
           for (int h = 0; h < 2; ++h)
-            av[u][i][h] = i < rts && k < k1 ? ldg_stream(a + ((static_cast<long long>(i) * p.kb32 + k) * 2 + h) * 32) : make_uint4(0u, 0u, 0u, 0u);
+            av[u][i][h] = i < rts && k < k1 ? ldg_stream(a + (static_cast<long long>(k >> 1) * rts + i) * 128 + h * 64 + (k & 1 ? odd : even)) : make_uint4(0u, 0u, 0u, 0u);
         xv[u][0] = in ? *reinterpret_cast<const uint4*>(xa + k * 32) : make_uint4(0u, 0u, 0u, 0u);
         xv[u][1] = in && n > 8 ? *reinterpret_cast<const uint4*>(xb + k * 32) : make_uint4(0u, 0u, 0u, 0u);
       }
@@ -553,9 +641,9 @@ __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams
         for (int j = 0; j < 2; ++j) {
           if (j > 0 && n <= 8) break;
 #pragma unroll
-          for (int i = 0; i < RT; ++i) mma_bf16(acc[i][j], av[u][i][0].x, av[u][i][0].y, av[u][i][0].z, av[u][i][0].w, xv[u][j].x, xv[u][j].y);
+          for (int i = 0; i < RT; ++i) mma_bf16(acc[i][j], av[u][i][0].x, av[u][i][1].x, av[u][i][0].y, av[u][i][1].y, xv[u][j].x, xv[u][j].y);
 #pragma unroll
-          for (int i = 0; i < RT; ++i) mma_bf16(acc[i][j], av[u][i][1].x, av[u][i][1].y, av[u][i][1].z, av[u][i][1].w, xv[u][j].z, xv[u][j].w);
+          for (int i = 0; i < RT; ++i) mma_bf16(acc[i][j], av[u][i][0].z, av[u][i][1].z, av[u][i][0].w, av[u][i][1].w, xv[u][j].z, xv[u][j].w);
         }
     }
     if (first < c1) lora_take<KS>(w, b + static_cast<long long>(first) * KS * 64);         // (on its way while the warps and the cluster meet)
@@ -648,19 +736,26 @@ __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams
 static int lora_tile_rows(int T) { return T <= 64 ? 16 : 64; }
 // the most tiles a step can have
 static int lora_max_tiles(int T, int slots) { return T / lora_tile_rows(T) + (T < slots + 1 ? T : slots + 1); }
-// ... and about how many it has (half of the adapters)
+// ... groups
+static int lora_max_groups(int T, int slots) { return T / LORA_DOWN_ROWS + (T < slots ? T : slots); }
+// ... and about how many tiles it has (half of the adapters)
 static int lora_tiles(int T, int slots) {
   const int adapters = T < slots + 1 ? T : slots + 1;
   return T <= 64 ? adapters : (T + 63) / 64 + adapters / 2;
 }
 static int lora_k_split(const LoraParams& p, int slots) {
-  const int stages = (p.K + LORA_STAGE_K - 1) / LORA_STAGE_K, tiles = lora_tiles(p.T, slots);
-  int split = ((p.VR > 64 ? 1 : 2) * sm_count() + tiles / 2) / tiles;       // the blocks that fit at a time
-  const int most = stages > 2 ? stages / 2 : 1;                             // two stages a block
+  const int stages = (p.K + LORA_STAGE_K - 1) / LORA_STAGE_K, adapters = p.T < slots + 1 ? p.T : slots + 1;
+  const int groups = p.T <= 64 ? adapters : (p.T + LORA_DOWN_ROWS - 1) / LORA_DOWN_ROWS + adapters / 2;
+  // All clusters at once: one lives on the 18 SMs of a part of the chip, of which there are eight, two blocks an SM.  (4096 rows of 8192, some 35 clusters: of four
+  // 36.6 us, of seven 34.1, of eight, which do not all fit, 39.7; 1000 rows of 2048, some ten: of four 28.0, of eight 26.2.)
+  int split = 8;
+  while (split > 1 && groups > 8 * (36 / split)) --split;
+  const int most = stages > 4 ? stages / 4 : 1;          // four stages a block
   if (split > most) split = most;
-  // (results in fp32: at most 16 stages a block, since the matrix units cut a sum off at every step; 32 of them leave 1.2e-6 of the result where 16 leave 0.6e-6)
-  if (p.parts == 3 && split < (stages + 15) / 16) split = (stages + 15) / 16;
-  return split < 1 ? 1 : split > 8 ? 8 : split;
+  // (results in fp32: sums of at most eight stages, since the tensor cores cut a sum off at every step)
+  const int longest = 8 * (p.VR > 64 ? LoraDown<8>::ACCS : LoraDown<4>::ACCS), least = (stages + longest - 1) / longest;
+  if (p.parts == 3 && split < least) split = least < 8 ? least : 8;
+  return split;
 }
 // One launch for a step of at most 64 rows, where an adapter is what eight SMs take in good time.
 static bool lora_few(const LoraParams& p) { return p.T <= 64 && p.VR <= LORA_FEW_RANKS && p.rank_tiles <= 4 && (p.a_slot + p.b_slot) * 16 <= 2 << 20; }
@@ -679,7 +774,7 @@ static int lora_up_tiles(LoraParams& p, int max_tiles, int tiles, void* stream) 
   const int most = (p.blocks + Up::BLOCKS - 1) / Up::BLOCKS;
   if (split > most) split = most;
   if (split < 1) split = 1;
-  VB_LAUNCH_PDL((lora_up_kernel<KS, OUT, TALL>), dim3(max_tiles, split), LORA_UP_THREADS, smem, stream, p);
+  VB_LAUNCH_PDL((lora_up_kernel<KS, OUT, TALL>), dim3(split, max_tiles), LORA_UP_THREADS, smem, stream, p);
   return 0;
 }
 template <int KS, int OUT>
@@ -687,10 +782,13 @@ static int lora_up_launch(LoraParams& p, int max_tiles, int tiles, void* stream)
   return p.tile_rows == 16 ? lora_up_tiles<KS, OUT, false>(p, max_tiles, tiles, stream) : lora_up_tiles<KS, OUT, true>(p, max_tiles, tiles, stream);
 }
 template <int RT>
-static int lora_down_launch(const LoraParams& p, int max_tiles, void* stream) {
+static int lora_down_launch(const LoraParams& p, int slots, void* stream) {
   VB_CHECK_CUDA((rm_smem<lora_down_kernel<RT>>()));
-  VB_CHECK_CUDA(launch_kernel_cluster3(lora_down_kernel<RT>, dim3(max_tiles, p.k_split), dim3(LORA_THREADS), LoraDown<RT>::SMEM, static_cast<cudaStream_t>(stream), true,
-                                       dim3(1, p.k_split, 1), p));
+  CUtensorMap x_map;
+  const int rc = vb_tensor_map_2d_bf16(&x_map, p.x, p.T, p.K, p.ldx, LORA_BOX_ROWS);
+  if (rc) return rc;
+  VB_CHECK_CUDA(launch_kernel_cluster3(lora_down_kernel<RT>, dim3(p.k_split, lora_max_groups(p.T, slots)), dim3(LORA_DOWN_THREADS), LoraDown<RT>::SMEM, static_cast<cudaStream_t>(stream), true,
+                                       dim3(p.k_split, 1, 1), p, x_map));
   return 0;
 }
 template <int KS, int OUT, int RT>
@@ -721,10 +819,11 @@ static int lora_launch(LoraParams& p, int slots, void* stream) {
     if (p.rank_tiles == 2) return lora_few_launch<2, OUT>(p, max_tiles, stream);
     return lora_few_launch<4, OUT>(p, max_tiles, stream);
   }
-  const int rc = p.VR <= 16   ? lora_down_launch<1>(p, max_tiles, stream)
-                 : p.VR <= 32 ? lora_down_launch<2>(p, max_tiles, stream)
-                 : p.VR <= 64 ? lora_down_launch<4>(p, max_tiles, stream)
-                              : lora_down_launch<8>(p, max_tiles, stream);
+  VB_CHECK_ARG(p.wait_flag = wait_flag(WK_LORA), "vb_lora: no mapped host memory");
+  const int rc = p.VR <= 16   ? lora_down_launch<1>(p, slots, stream)
+                 : p.VR <= 32 ? lora_down_launch<2>(p, slots, stream)
+                 : p.VR <= 64 ? lora_down_launch<4>(p, slots, stream)
+                              : lora_down_launch<8>(p, slots, stream);
   if (rc) return rc;
   switch (p.rank_tiles) {
     case 1: return lora_up_launch<1, OUT>(p, max_tiles, lora_tiles(p.T, slots), stream);
@@ -754,10 +853,9 @@ static int lora_bank(const char* who, LoraParams& p, const VbLoraBank* bank, int
   p.scale = bank->d_scale;
   p.T = T;
   p.K = bank->K;
-  p.kb32 = (p.K + 31) / 32;
   p.rank_tiles = bank->rank / 16;
   p.VR = p.slices * bank->rank;
-  p.a_slot = static_cast<long long>(p.VR / 16) * p.kb32 * 64;
+  p.a_slot = static_cast<long long>(p.VR / 16) * ((p.K + 63) / 64) * 128;
   p.b_slot = static_cast<long long>(p.block0[p.slices]) * p.rank_tiles * 64;
   p.blocks = p.block0[p.slices];
   return 0;
@@ -770,8 +868,10 @@ static int lora_setup(const char* who, LoraParams& p, const void* d_x, long long
   const int rc = lora_bank(who, p, bank, T);
   if (rc) return rc;
   VB_CHECK_ARG(d_x && d_tiles, "%s: null pointer", who);
+  VB_CHECK_ARG(T <= LORA_MAX_ROWS, "%s: %d rows; at most %d", who, T, LORA_MAX_ROWS);
   VB_CHECK_ARG(ldx % 8 == 0 && ldx >= p.K && reinterpret_cast<uintptr_t>(d_x) % 16 == 0, "%s: rows of x must be 16-byte aligned (K %d, row stride %lld)", who, p.K, ldx);
   p.tiles = static_cast<const int32_t*>(d_tiles);
+  p.groups = reinterpret_cast<const int4*>(p.tiles + static_cast<long long>(lora_max_tiles(T, bank->slots)) * (4 + p.tile_rows));
   p.x = static_cast<const __nv_bfloat16*>(d_x);
   p.ldx = ldx;
   p.v = static_cast<uint32_t*>(d_ws);
@@ -788,15 +888,16 @@ using namespace vb;
 extern "C" {
 
 size_t vb_lora_plan_bytes(int T, int slots) {
-  return T < 1 || slots < 1 ? 0 : static_cast<size_t>(lora_max_tiles(T, slots)) * (4 + lora_tile_rows(T)) * 4;
+  return T < 1 || slots < 1 ? 0 : static_cast<size_t>(lora_max_tiles(T, slots)) * (4 + lora_tile_rows(T)) * 4 + static_cast<size_t>(lora_max_groups(T, slots)) * 16;
 }
 
 int vb_lora_plan(void* d_tiles, const int32_t* d_ids, int T, int slots, void* stream) {
   VB_CHECK_ARG(d_tiles && d_ids, "vb_lora_plan: null pointer");
   VB_CHECK_ARG(reinterpret_cast<uintptr_t>(d_tiles) % 16 == 0, "vb_lora_plan: the plan must be 16-byte aligned");
   VB_CHECK_ARG(slots >= 1 && slots <= LORA_MAX_SLOTS, "vb_lora_plan: %d adapters; 1 to %d", slots, LORA_MAX_SLOTS);
-  VB_CHECK_ARG(T >= 1, "vb_lora_plan: no rows");
-  VB_LAUNCH_PDL(lora_plan_kernel, 1, 1024, 0, stream, static_cast<int32_t*>(d_tiles), d_ids, T, slots, lora_tile_rows(T), lora_max_tiles(T, slots));
+  VB_CHECK_ARG(T >= 1 && T <= LORA_MAX_ROWS, "vb_lora_plan: %d rows; 1 to %d", T, LORA_MAX_ROWS);
+  VB_CHECK_CUDA((rm_smem<lora_plan_kernel>(LORA_PLAN_SMEM)));
+  VB_LAUNCH_PDL(lora_plan_kernel, 1, 1024, 32 * (slots + 1) * 4, stream, static_cast<int32_t*>(d_tiles), d_ids, T, slots, lora_tile_rows(T), lora_max_tiles(T, slots), lora_max_groups(T, slots));
   return 0;
 }
 

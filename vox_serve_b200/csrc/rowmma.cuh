@@ -50,13 +50,13 @@ __device__ __forceinline__ float4 ld_dsmem_f32x4(const float* local_ptr, uint32_
 
 // The opt-in shared memory of a kernel, once per device.  (A flag of its own for every kernel: max_dyn_smem_once keeps one per type, and these share theirs.)
 template <auto Kernel>
-inline cudaError_t rm_smem() {
+inline cudaError_t rm_smem(int bytes = VB_MAX_DYN_SMEM) {
   static std::atomic<unsigned long long> done{0ull};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
   if (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1ull)) return cudaSuccess;
-  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, VB_MAX_DYN_SMEM);
+  e = cudaFuncSetAttribute(Kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
   if (e == cudaSuccess && dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
   return e;
 }

@@ -1915,8 +1915,8 @@ class LoraBank:
         self.slots, self.K, self.widths, self.rank = int(slots), int(K), widths, int(rank)
         self.N = sum(widths)
         self.rank_pad = next(r for r in (16, 32, 64, 128) if rank <= r)
-        kb, blocks = (K + 31) // 32, sum((w + 31) // 32 for w in widths)
-        self.a = torch.zeros(slots, len(widths) * self.rank_pad * kb * 32, dtype=BF16, device=device)
+        kb, blocks = (K + 63) // 64, sum((w + 31) // 32 for w in widths)
+        self.a = torch.zeros(slots, len(widths) * self.rank_pad * kb * 64, dtype=BF16, device=device)
         self.b = torch.zeros(slots, blocks * 32 * self.rank_pad, dtype=BF16, device=device)
         self.scale = torch.zeros(slots, dtype=torch.float32, device=device)
         self._struct = _lib.LoraBankStruct(self.a.data_ptr(), self.b.data_ptr(), self.scale.data_ptr(), self.slots, self.rank_pad, self.K, len(widths),
@@ -1934,11 +1934,13 @@ class LoraBank:
         _refuse(tuple(a.shape) != (S, r, self.K) or not 1 <= r <= self.rank, f"LoraBank.load: A {tuple(a.shape)}; [{S}, r <= {self.rank}, {self.K}] is needed")
         _refuse(tuple(b.shape) != (self.N, r), f"LoraBank.load: B {tuple(b.shape)}; [{self.N}, {r}] is needed")
         dev = self.a.device
-        kb = (self.K + 31) // 32
-        ap = torch.zeros(S, rp, kb * 32, dtype=BF16, device=dev)
+        kb = (self.K + 63) // 64
+        ap = torch.zeros(S, rp, kb * 64, dtype=BF16, device=dev)
         ap[:, :r, :self.K] = a.to(device=dev, dtype=BF16)
-        # rows as m16 tiles (halves h of 8 rows), k as 8 per lane in two product steps of two pairs
-        ap = ap.view(S * rp // 16, 2, 8, kb, 4, 2, 2, 2).permute(0, 3, 5, 2, 4, 6, 1, 7)
+        # 64 k of 16 ranks after the other: rows of 128 bytes, 16-byte piece c of row r at c ^ (r & 7)
+        ap = ap.view(S * rp, kb, 8, 8).permute(1, 0, 2, 3)
+        swap = (torch.arange(8, device=dev)[None] ^ torch.arange(8, device=dev)[:, None]).repeat(S * rp // 8, 1)
+        ap = torch.gather(ap, 2, swap[None, :, :, None].expand(kb, S * rp, 8, 8))
         self.a[slot].copy_(ap.reshape(-1))
         blocks, n0 = [], 0
         for w in self.widths:
