@@ -377,19 +377,27 @@ __device__ __forceinline__ void lora_take(uint4 (&w)[KS][2], const uint4* b) {
     w[k][1] = __ldg(b + k * 64 + 32);
   }
 }
-// ... both operands from shared memory
-template <int KS, int PARTS>
-__device__ __forceinline__ void lora_product(float (&d)[4][4], uint32_t frags, uint32_t b) {
+// ... both operands from shared memory, NB neighbouring column blocks
+template <int KS, int PARTS, int NB>
+__device__ __forceinline__ void lora_product(float (*d)[4][4], uint32_t frags, uint32_t b) {
 #pragma unroll
   for (int k = 0; k < KS; ++k) {
-    const uint4 w0 = lds16(b + k * 1024), w1 = lds16(b + k * 1024 + 512);
+    uint4 w[NB][2];
+#pragma unroll
+    for (int i = 0; i < NB; ++i) {
+      w[i][0] = lds16(b + (i * KS + k) * 1024);
+      w[i][1] = lds16(b + (i * KS + k) * 1024 + 512);
+    }
 #pragma unroll
     for (int q = PARTS - 1; q >= 0; --q) {
       const uint4 f = lds16(frags + (q * KS + k) * 512);
-      mma_bf16(d[0], f.x, f.y, f.z, f.w, w0.x, w0.y);
-      mma_bf16(d[1], f.x, f.y, f.z, f.w, w0.z, w0.w);
-      mma_bf16(d[2], f.x, f.y, f.z, f.w, w1.x, w1.y);
-      mma_bf16(d[3], f.x, f.y, f.z, f.w, w1.z, w1.w);
+#pragma unroll
+      for (int i = 0; i < NB; ++i) {
+        mma_bf16(d[i][0], f.x, f.y, f.z, f.w, w[i][0].x, w[i][0].y);
+        mma_bf16(d[i][1], f.x, f.y, f.z, f.w, w[i][0].z, w[i][0].w);
+        mma_bf16(d[i][2], f.x, f.y, f.z, f.w, w[i][1].x, w[i][1].y);
+        mma_bf16(d[i][3], f.x, f.y, f.z, f.w, w[i][1].z, w[i][1].w);
+      }
     }
   }
 }
@@ -419,8 +427,16 @@ __device__ __forceinline__ void lora_result(void* out, float (&y)[8], const void
     *static_cast<uint4*>(out) = lora_round(y);
   }
 }
-// ... of gate | up: g0, g1, u0, u1 are the first plane's eight gate and eight up columns.  (The fast exponential is off by 2 + 1.2 |g| units of 2^-23 and
-// the fast quotient by two: far below half a step of bf16, 2^-9.)
+// g / (1 + exp(-g)) by the special function unit without its ranges below 2^-126 (1000 rows of gate | up: 26.3 us with the ranges, 25.8 without).  The power of
+// two is off by 2^-22, its argument's rounding by 1.2 |g| units of 2^-24, the reciprocal by 2^-23: far below half a step of bf16, 2^-9.  Below g = -87 the reciprocal is 0 (the
+// value 1e-36 at most).
+__device__ __forceinline__ float lora_silu(float g) {
+  float e, r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return g * r;
+}
+// ... of gate | up: g0, g1, u0, u1 are the first plane's eight gate and eight up columns
 __device__ __forceinline__ void lora_gated(const LoraParams& p, void* out, long long row, int col, float (&gv)[8], float (&uv)[8], const float4& g0, const float4& g1,
                                            const float4& u0, const float4& u1) {
   lora_add4(gv, g0);
@@ -437,7 +453,7 @@ __device__ __forceinline__ void lora_gated(const LoraParams& p, void* out, long 
       lora_add4(uv + 4, *reinterpret_cast<const float4*>(more + 20));
     }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) gv[i] = __fdividef(gv[i], 1.f + __expf(-gv[i])) * uv[i];
+  for (int i = 0; i < 8; ++i) gv[i] = lora_silu(gv[i]) * uv[i];
   *static_cast<uint4*>(out) = lora_round(gv);
 }
 // where column `col` of a row's results stands
@@ -554,15 +570,21 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
     }
     __syncthreads();
     const uint32_t from = steps + (turn & p.ahead) * step_bytes;
-#pragma unroll 1
+    float ds[WIDE][4][4] = {}, u[4][4] = {};
+    const int first = c + (TALL ? 0 : warp);
+    while (OUT != LORA_GLU && first < c1 && first >= p.block0[s + 1]) ++s;
+    // (two column blocks of one slice: v is read once for both.  34.0 -> 33.3 us for 4096 rows of bf16; fp32 results have no registers left for it: 79 -> 82)
+    const bool pair = WIDE == 2 && OUT == LORA_BF16 && first + 1 < c1 && first + 1 < p.block0[s + 1];
+    if (has && pair && mt * 16 < n) lora_product<KS, PARTS, OUT == LORA_BF16 ? WIDE : 1>(ds, frags + s * PARTS * KS * 512, from + lane * 16);
+#pragma unroll
     for (int w = 0; w < WIDE; ++w) {
       const int mine = TALL ? w : warp, block = c + mine;
       if (mt * 16 >= n || block >= c1) break;
       while (OUT != LORA_GLU && block >= p.block0[s + 1]) ++s;
-      float d[4][4] = {}, u[4][4] = {};
-      if (has) {
-        lora_product<KS, PARTS>(d, frags + s * PARTS * KS * 512, from + mine * B_BYTES + lane * 16);
-        if constexpr (OUT == LORA_GLU) lora_product<KS, PARTS>(u, frags + PARTS * KS * 512, from + (STEP + mine) * B_BYTES + lane * 16);
+      float (&d)[4][4] = ds[w];
+      if (has && !pair) {
+        lora_product<KS, PARTS, 1>(&d, frags + s * PARTS * KS * 512, from + mine * B_BYTES + lane * 16);
+        if constexpr (OUT == LORA_GLU) lora_product<KS, PARTS, 1>(&u, frags + PARTS * KS * 512, from + (STEP + mine) * B_BYTES + lane * 16);
       }
       const int col = p.col0[s] + (block - p.block0[s]) * 32 + t4 * 8;
       if (col >= p.col0[s + 1]) continue;
