@@ -132,6 +132,7 @@ struct LoraParams {
   int blocks;                      // column blocks of 32 over all slices (of gate | up: of one)
   int ahead;                       // 1: a step's copies go out a step ahead
   int slices, block0[LORA_MAX_SLICES + 1], col0[LORA_MAX_SLICES + 1];
+  int part0[LORA_MAX_SLICES + 1];  // the blocks of a tile by slice
   void* out;
   const void* base;
   long long ldo, ld_base;
@@ -172,7 +173,7 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 // warps (some 16 clocks an instruction of 512 bytes: that rate bounded a form with copies alone, at 38 us for 4096 rows of 8192 at rank 64 and the second
 // product; mma.sync from such copies was bound by its shared-memory reads: 36 us, 69 at rank 128; this form takes 34 and 48).  A fifth warp multiplies.  Rows behind
 // the last are whatever stands there, in lanes that nobody reads.  Stages go to ACCS sums in turn: the tensor cores cut a sum off at every step, and chains of a
-// quarter lose a quarter.  More than RT rank tiles: x again.  The pieces of K are a cluster, which adds them up and leaves v in parts.
+// quarter lose a quarter.  More than RT rank tiles: further blocks with x again.  The pieces of K are a cluster, which adds them up and leaves v in parts.
 constexpr int LORA_STAGE_K = 64, LORA_X_BYTES = LORA_DOWN_ROWS * 128, LORA_DOWN_THREADS = 160, LORA_LOADERS = 128, LORA_BOX_ROWS = 64;
 template <int RT>
 struct LoraDown {
@@ -225,128 +226,125 @@ __global__ void __launch_bounds__(LORA_DOWN_THREADS, 2) lora_down_kernel(const L
   __syncthreads();                          // (barriers and TMEM are there)
   tc_fence_after();
   const uint32_t tmem = *tmem_at;
-  int slot = 0;                             // place and parity run on from one pass over x to the next
+  int slot = 0;
   uint32_t parity = 0u;
   auto next = [&]() {
     slot = slot + 1 == STAGES ? 0 : slot + 1;
     parity ^= slot == 0 ? 1u : 0u;
   };
-  for (int rt0 = 0, pass = 0; rt0 < rts; rt0 += RT, ++pass) {
-    const int here = min(RT, rts - rt0);
-    // (one lane) A of a stage, all its rank tiles in a row, and how many bytes the stage waits for
-    auto ask = [&](int s, uint32_t x_bytes) {
-      mbar_arrive_expect_tx(full + slot, here * 2048 + x_bytes);
-      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring + slot * D::STAGE_BYTES + LORA_X_BYTES),
-                   "l"(p.a + gr.y * p.a_slot + (static_cast<long long>(s) * rts + rt0) * 128), "r"(here * 2048), "r"(smem_u32(full + slot))
-                   : "memory");
-    };
-    if (boxes && warp == 0) {
-      for (int i = 0; i < turns; ++i) {
+  const int rt0 = blockIdx.z * RT, here = min(RT, rts - rt0);
+  // (one lane) A of a stage, all its rank tiles in a row, and how many bytes the stage waits for
+  auto ask = [&](int s, uint32_t x_bytes) {
+    mbar_arrive_expect_tx(full + slot, here * 2048 + x_bytes);
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ring + slot * D::STAGE_BYTES + LORA_X_BYTES),
+                 "l"(p.a + gr.y * p.a_slot + (static_cast<long long>(s) * rts + rt0) * 128), "r"(here * 2048), "r"(smem_u32(full + slot))
+                 : "memory");
+  };
+  if (boxes && warp == 0) {
+    for (int i = 0; i < turns; ++i) {
+      bw.wait(empty + slot, parity ^ 1u);
+      if (!__all_sync(0xffffffffu, !bw.dead)) bw.dead = true;
+      if (bw.dead) break;
+      const int s = s0 + i * hop;
+      if (lane == 0) {
+        ask(s, n_boxes * LORA_BOX_ROWS * 128);
+        for (int b = 0; b < n_boxes; ++b)
+          tma_load_2d(base + slot * D::STAGE_BYTES + b * LORA_BOX_ROWS * 128, &x_map, full + slot, s * LORA_STAGE_K, gr.w + b * LORA_BOX_ROWS);
+      }
+      __syncwarp();
+      next();
+    }
+  } else if (!boxes && warp < 4) {
+    int told = slot;                      // the oldest stage that the multiplying warp has not been told of
+    for (int i = 0; i < turns + AHEAD; ++i) {
+      if (i < turns && !bw.dead) {
+        const int s = s0 + i * hop;
         bw.wait(empty + slot, parity ^ 1u);
         if (!__all_sync(0xffffffffu, !bw.dead)) bw.dead = true;
-        if (bw.dead) break;
-        const int s = s0 + i * hop;
-        if (lane == 0) {
-          ask(s, n_boxes * LORA_BOX_ROWS * 128);
-          for (int b = 0; b < n_boxes; ++b)
-            tma_load_2d(base + slot * D::STAGE_BYTES + b * LORA_BOX_ROWS * 128, &x_map, full + slot, s * LORA_STAGE_K, gr.w + b * LORA_BOX_ROWS);
+        if (!bw.dead) {
+          if (tid == 0) ask(s, 0u);
+          const uint32_t to = slot * D::STAGE_BYTES;
+          const bool in = s * LORA_STAGE_K + chunk * 8 < p.K;
+          const __nv_bfloat16* x = xs + (in ? static_cast<long long>(s) * LORA_STAGE_K : 0);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (xr[j] >= 0) cp_async16(x_to + to + j * 2048, x + xr[j] * p.ldx, in ? 16 : 0);
         }
-        __syncwarp();
         next();
       }
-    } else if (!boxes && warp < 4) {
-      int told = slot;                      // the oldest stage that the multiplying warp has not been told of
-      for (int i = 0; i < turns + AHEAD; ++i) {
-        if (i < turns && !bw.dead) {
-          const int s = s0 + i * hop;
-          bw.wait(empty + slot, parity ^ 1u);
-          if (!__all_sync(0xffffffffu, !bw.dead)) bw.dead = true;
-          if (!bw.dead) {
-            if (tid == 0) ask(s, 0u);
-            const uint32_t to = slot * D::STAGE_BYTES;
-            const bool in = s * LORA_STAGE_K + chunk * 8 < p.K;
-            const __nv_bfloat16* x = xs + (in ? static_cast<long long>(s) * LORA_STAGE_K : 0);
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-              if (xr[j] >= 0) cp_async16(x_to + to + j * 2048, x + xr[j] * p.ldx, in ? 16 : 0);
-          }
-          next();
-        }
-        cp_async_commit();
-        if (i >= AHEAD) {
-          cp_async_wait<AHEAD>();
-          fence_proxy_async();              // (what the copies wrote, for the tensor cores' reads)
-          __syncwarp();
-          if (lane == 0 && !bw.dead) mbar_arrive(full + told);
-          told = told + 1 == STAGES ? 0 : told + 1;
-        }
-      }
-    } else if (warp == 4) {
-      const uint32_t idesc = umma_idesc(128, here * 16, 1u);
-      for (int i = 0; i < turns; ++i) {
-        bw.wait(full + slot, parity);
-        if (!__all_sync(0xffffffffu, !bw.dead)) bw.dead = true;
-        if (bw.dead) break;
-        tc_fence_after();
-        const uint64_t x_desc = umma_desc_sw128_kmajor(ring + slot * D::STAGE_BYTES), a_desc = umma_desc_sw128_kmajor(ring + slot * D::STAGE_BYTES + LORA_X_BYTES);
-        if (elect_one()) {
-#pragma unroll
-          for (int k = 0; k < 4; ++k) umma_bf16(tmem + i % D::ACCS * D::N, x_desc + 2 * k, a_desc + 2 * k, idesc, i >= D::ACCS || k > 0);
-          umma_commit(empty + slot);
-          if (i + 1 == turns) umma_commit(done);
-        }
+      cp_async_commit();
+      if (i >= AHEAD) {
+        cp_async_wait<AHEAD>();
+        fence_proxy_async();              // (what the copies wrote, for the tensor cores' reads)
         __syncwarp();
-        next();
+        if (lane == 0 && !bw.dead) mbar_arrive(full + told);
+        told = told + 1 == STAGES ? 0 : told + 1;
       }
     }
-    // the products are through: rows of sums where the stages stood
-    float* mine = reinterpret_cast<float*>(base);                  // [128 rows][LD]
-    bw.wait(done, pass & 1);
-    tc_fence_after();
-    if (warp * 32 < n && warp < 4) {
-#pragma unroll 1
-      for (int c0 = 0; c0 < here * 16; c0 += 16) {
-        float s[16];
+  } else if (warp == 4) {
+    const uint32_t idesc = umma_idesc(128, here * 16, 1u);
+    for (int i = 0; i < turns; ++i) {
+      bw.wait(full + slot, parity);
+      if (!__all_sync(0xffffffffu, !bw.dead)) bw.dead = true;
+      if (bw.dead) break;
+      tc_fence_after();
+      const uint64_t x_desc = umma_desc_sw128_kmajor(ring + slot * D::STAGE_BYTES), a_desc = umma_desc_sw128_kmajor(ring + slot * D::STAGE_BYTES + LORA_X_BYTES);
+      if (elect_one()) {
 #pragma unroll
-        for (int q = 0; q < D::ACCS; ++q) {
-          if (q > 0 && q >= turns) break;
-          uint32_t v[16];
-          tmem_ld_32x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + q * D::N + c0, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int j = 0; j < 16; ++j) s[j] = q == 0 ? __uint_as_float(v[j]) : s[j] + __uint_as_float(v[j]);
-        }
-        float4* to = reinterpret_cast<float4*>(mine + (warp * 32 + lane) * LD + c0);
-#pragma unroll
-        for (int j = 0; j < 4; ++j) to[j] = make_float4(scale * s[4 * j], scale * s[4 * j + 1], scale * s[4 * j + 2], scale * s[4 * j + 3]);
+        for (int k = 0; k < 4; ++k) umma_bf16(tmem + i % D::ACCS * D::N, x_desc + 2 * k, a_desc + 2 * k, idesc, i >= D::ACCS || k > 0);
+        umma_commit(empty + slot);
+        if (i + 1 == turns) umma_commit(done);
       }
+      __syncwarp();
+      next();
     }
-    tc_fence_before();
-    if (p.k_split > 1) cluster_sync_all();
-    else __syncthreads();
-    const int log_ks = 31 - __clz(p.rank_tiles);
-    uint32_t* v = p.v + static_cast<long long>(gr.x) * (p.tile_rows >> 4) * rts * p.parts * 128;
-    for (int e = blockIdx.x * LORA_DOWN_THREADS + tid; e < n * RT * 4; e += p.k_split * LORA_DOWN_THREADS) {
-      const int c = e / (RT * 4), k = e % (RT * 4) * 4;
-      if (rt0 * 16 + k >= p.VR) continue;
-      float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (p.k_split > 1) {
-#pragma unroll 4
-        for (int z = 0; z < p.k_split; ++z) {
-          const float4 w = ld_dsmem_f32x4(mine + c * LD + k, z);
-          s.x += w.x; s.y += w.y; s.z += w.z; s.w += w.w;
-        }
-      } else {
-        s = *reinterpret_cast<const float4*>(mine + c * LD + k);
-      }
-      lora_put(v, p.slices, p.parts, log_ks, c, rt0 * 16 + k, s.x, s.y);
-      lora_put(v, p.slices, p.parts, log_ks, c, rt0 * 16 + k + 2, s.z, s.w);
-    }
-    fence_proxy_async();                                           // (others' parts have been read: the next stages may come, or the block may leave)
-    if (p.k_split > 1) cluster_sync_all();
-    else __syncthreads();
-    tc_fence_after();
   }
+  // the products are through: rows of sums where the stages stood
+  float* mine = reinterpret_cast<float*>(base);                  // [128 rows][LD]
+  bw.wait(done, 0);
+  tc_fence_after();
+  if (warp * 32 < n && warp < 4) {
+#pragma unroll 1
+    for (int c0 = 0; c0 < here * 16; c0 += 16) {
+      float s[16];
+#pragma unroll
+      for (int q = 0; q < D::ACCS; ++q) {
+        if (q > 0 && q >= turns) break;
+        uint32_t v[16];
+        tmem_ld_32x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + q * D::N + c0, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[j] = q == 0 ? __uint_as_float(v[j]) : s[j] + __uint_as_float(v[j]);
+      }
+      float4* to = reinterpret_cast<float4*>(mine + (warp * 32 + lane) * LD + c0);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) to[j] = make_float4(scale * s[4 * j], scale * s[4 * j + 1], scale * s[4 * j + 2], scale * s[4 * j + 3]);
+    }
+  }
+  tc_fence_before();
+  if (p.k_split > 1) cluster_sync_all();
+  else __syncthreads();
+  const int log_ks = 31 - __clz(p.rank_tiles);
+  uint32_t* v = p.v + static_cast<long long>(gr.x) * (p.tile_rows >> 4) * rts * p.parts * 128;
+  for (int e = blockIdx.x * LORA_DOWN_THREADS + tid; e < n * RT * 4; e += p.k_split * LORA_DOWN_THREADS) {
+    const int c = e / (RT * 4), k = e % (RT * 4) * 4;
+    if (rt0 * 16 + k >= p.VR) continue;
+    float4 s = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (p.k_split > 1) {
+#pragma unroll 4
+      for (int z = 0; z < p.k_split; ++z) {
+        const float4 w = ld_dsmem_f32x4(mine + c * LD + k, z);
+        s.x += w.x; s.y += w.y; s.z += w.z; s.w += w.w;
+      }
+    } else {
+      s = *reinterpret_cast<const float4*>(mine + c * LD + k);
+    }
+    lora_put(v, p.slices, p.parts, log_ks, c, rt0 * 16 + k, s.x, s.y);
+    lora_put(v, p.slices, p.parts, log_ks, c, rt0 * 16 + k + 2, s.z, s.w);
+  }
+  if (p.k_split > 1) cluster_sync_all();                         // (others' parts have been read: the block may leave)
+  else __syncthreads();
+  tc_fence_after();
   if (bw.dead) {                            // let the copies in flight land before the block may leave
     const unsigned long long t0 = gtimer();
     while (gtimer() - t0 < 2000000ull) __nanosleep(1000);
@@ -420,8 +418,13 @@ __device__ __forceinline__ void lora_result(void* out, float (&y)[8], const void
       lora_add4(y, static_cast<const float4*>(base)[0]);
       lora_add4(y + 4, static_cast<const float4*>(base)[1]);
     }
-    static_cast<float4*>(out)[0] = make_float4(y[0], y[1], y[2], y[3]);
-    static_cast<float4*>(out)[1] = make_float4(y[4], y[5], y[6], y[7]);
+    if ((reinterpret_cast<uintptr_t>(out) & 31) == 0) {
+      asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(out), "f"(y[0]), "f"(y[1]), "f"(y[2]), "f"(y[3]), "f"(y[4]), "f"(y[5]), "f"(y[6]), "f"(y[7])
+                   : "memory");
+    } else {
+      static_cast<float4*>(out)[0] = make_float4(y[0], y[1], y[2], y[3]);
+      static_cast<float4*>(out)[1] = make_float4(y[4], y[5], y[6], y[7]);
+    }
   } else {
     if (base) lora_add8(y, *static_cast<const uint4*>(base));
     *static_cast<uint4*>(out) = lora_round(y);
@@ -491,18 +494,25 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int32_t* rec = p.tiles + static_cast<long long>(blockIdx.y) * (4 + TILE);
   const int4 tl = *reinterpret_cast<const int4*>(rec);
-  // (ranges in whole steps)
-  const int n = tl.z, all = (p.blocks + STEP - 1) / STEP;
-  const int c0 = static_cast<int>(static_cast<long long>(all) * blockIdx.x / gridDim.x) * STEP, c1 = min(p.blocks, static_cast<int>(static_cast<long long>(all) * (blockIdx.x + 1) / gridDim.x) * STEP);
+  // (ranges of one slice, of gate | up of both, in whole steps)
+  int s = 0;
+  if (OUT != LORA_GLU)
+    while (static_cast<int>(blockIdx.x) >= p.part0[s + 1]) ++s;
+  const int n = tl.z, begin = OUT == LORA_GLU ? 0 : p.block0[s], blocks = OUT == LORA_GLU ? p.blocks : p.block0[s + 1] - begin, all = (blocks + STEP - 1) / STEP;
+  const int parts = OUT == LORA_GLU ? gridDim.x : p.part0[s + 1] - p.part0[s], part = blockIdx.x - (OUT == LORA_GLU ? 0 : p.part0[s]);
+  const int c0 = begin + static_cast<int>(static_cast<long long>(all) * part / parts) * STEP,
+            c1 = begin + min(blocks, static_cast<int>(static_cast<long long>(all) * (part + 1) / parts) * STEP);
   const bool has = tl.x >= 0;
   if (n == 0 || c0 >= c1) {
     pdl_sync();
     return;
   }
-  // shared memory: v [m16 blocks][slices][PARTS][KS] of 512 bytes, then two steps: B of the column blocks (of gate, of up), rows of base or planes
+  // shared memory: v [m16 blocks][the block's slice, or both][PARTS][KS] of 512 bytes, then one or two steps: B of the column blocks (of gate, of up), rows of base or planes
   const bool adds = OUT == LORA_GLU || p.base != nullptr;
-  const int v_bytes = ((n + 15) >> 4) * p.slices * PARTS * KS * 512, step_bytes = STEP * BOTH * B_BYTES + (adds ? Up::ROWS_BYTES : 0);
-  const uint32_t vs = smem_u32(smem8), steps = vs + (TILE / 16) * p.slices * PARTS * KS * 512;
+  constexpr bool PAIR = WIDE == 2 && (OUT == LORA_BF16 || KS >= 4);
+  constexpr int V_BLOCK = BOTH * PARTS * KS * 512;          // of 16 rows
+  const int step_bytes = STEP * BOTH * B_BYTES + (adds ? Up::ROWS_BYTES : 0);
+  const uint32_t vs = smem_u32(smem8), steps = vs + (TILE / 16) * V_BLOCK;
   // a lane's copies of base or planes: 16 bytes (q) of every ROWS-th row of its 16
   constexpr int PER = Up::ROW / 16, ROWS = 32 / PER;
   const int q = lane % PER, mt = TALL ? warp : 0, r0 = mt * 16 + lane / PER;
@@ -536,8 +546,6 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
           at = block * 64 + in_block * 4;
           in = at < 2 * ((p.ff + 15) & ~15);
         } else {
-          int s = 0;
-          while (block >= p.block0[s + 1]) ++s;
           at = p.col0[s] + (block - p.block0[s]) * 32 + in_block * (OUT == LORA_F32 ? 4 : 8);
           in = at < p.col0[s + 1];
         }
@@ -555,12 +563,13 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
   load(c0, 0);
   pdl_sync();
   if (has) {
-    const uint4* v = reinterpret_cast<const uint4*>(p.v) + static_cast<long long>(blockIdx.y) * (TILE / 16) * p.slices * PARTS * KS * 32;
-    for (int i = tid; i < v_bytes / 16; i += LORA_UP_THREADS) cp_async16(vs + i * 16, v + i, 16);
+    const uint4* v = reinterpret_cast<const uint4*>(p.v) + (static_cast<long long>(blockIdx.y) * (TILE / 16) * p.slices + s) * PARTS * KS * 32;
+    for (int m = 0; m < (n + 15) >> 4; ++m)
+      for (int i = tid; i < V_BLOCK / 16; i += LORA_UP_THREADS) cp_async16(vs + m * V_BLOCK + i * 16, v + m * p.slices * PARTS * KS * 32 + i, 16);
   }
   cp_async_commit();
-  const uint32_t frags = vs + (mt * p.slices * PARTS * KS * 32 + lane) * 16;
-  int turn = 0, s = 0;
+  const uint32_t frags = vs + mt * V_BLOCK + lane * 16;
+  int turn = 0;
   for (int c = c0; c < c1; c += STEP, ++turn) {
     if (p.ahead) {
       load(c + STEP, turn + 1);
@@ -572,18 +581,17 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
     const uint32_t from = steps + (turn & p.ahead) * step_bytes;
     float ds[WIDE][4][4] = {}, u[4][4] = {};
     const int first = c + (TALL ? 0 : warp);
-    while (OUT != LORA_GLU && first < c1 && first >= p.block0[s + 1]) ++s;
-    // (two column blocks of one slice: v is read once for both.  34.0 -> 33.3 us for 4096 rows of bf16; fp32 results have no registers left for it: 79 -> 82)
-    const bool pair = WIDE == 2 && OUT == LORA_BF16 && first + 1 < c1 && first + 1 < p.block0[s + 1];
-    if (has && pair && mt * 16 < n) lora_product<KS, PARTS, OUT == LORA_BF16 ? WIDE : 1>(ds, frags + s * PARTS * KS * 512, from + lane * 16);
+    // (two column blocks: v is read once for both.  4096 rows of bf16 at rank 64 34.0 -> 33.3 us, of q | k | v in fp32 82 -> 73; fp32 at rank 16 11.0 -> 11.7, too many
+    // registers for what it saves)
+    const bool pair = PAIR && first + 1 < c1;
+    if (has && pair && mt * 16 < n) lora_product<KS, PARTS, PAIR ? 2 : 1>(ds, frags, from + lane * 16);
 #pragma unroll
     for (int w = 0; w < WIDE; ++w) {
       const int mine = TALL ? w : warp, block = c + mine;
       if (mt * 16 >= n || block >= c1) break;
-      while (OUT != LORA_GLU && block >= p.block0[s + 1]) ++s;
       float (&d)[4][4] = ds[w];
       if (has && !pair) {
-        lora_product<KS, PARTS, 1>(&d, frags + s * PARTS * KS * 512, from + mine * B_BYTES + lane * 16);
+        lora_product<KS, PARTS, 1>(&d, frags, from + mine * B_BYTES + lane * 16);
         if constexpr (OUT == LORA_GLU) lora_product<KS, PARTS, 1>(&u, frags + PARTS * KS * 512, from + (STEP + mine) * B_BYTES + lane * 16);
       }
       const int col = p.col0[s] + (block - p.block0[s]) * 32 + t4 * 8;
@@ -770,8 +778,9 @@ static int lora_k_split(const LoraParams& p, int slots) {
   const int groups = p.T <= 64 ? adapters : (p.T + LORA_DOWN_ROWS - 1) / LORA_DOWN_ROWS + adapters / 2;
   // All clusters at once: one lives on the 18 SMs of a part of the chip, of which there are eight, two blocks an SM.  (4096 rows of 8192, some 35 clusters: of four
   // 36.6 us, of seven 34.1, of eight, which do not all fit, 39.7; 1000 rows of 2048, some ten: of four 28.0, of eight 26.2.)
+  const int passes = p.VR <= 64 ? 1 : (p.VR + LoraDown<8>::N - 1) / LoraDown<8>::N;
   int split = 8;
-  while (split > 1 && groups > 8 * (36 / split)) --split;
+  while (split > 1 && groups * passes > 8 * (36 / split)) --split;
   const int most = stages > 4 ? stages / 4 : 1;          // four stages a block
   if (split > most) split = most;
   // (results in fp32: sums of at most eight stages, since the tensor cores cut a sum off at every step)
@@ -786,9 +795,9 @@ template <int KS, int OUT, bool TALL>
 static int lora_up_tiles(LoraParams& p, int max_tiles, int tiles, void* stream) {
   using Up = LoraUp<OUT, TALL>;
   VB_CHECK_CUDA((rm_smem<lora_up_kernel<KS, OUT, TALL>>()));
-  const size_t v_bytes = static_cast<size_t>(p.tile_rows >> 4) * p.slices * lora_parts<OUT>() * KS * 512,
+  const size_t v_bytes = static_cast<size_t>(p.tile_rows >> 4) * (OUT == LORA_GLU ? 2 : 1) * lora_parts<OUT>() * KS * 512,
                step = static_cast<size_t>(Up::BLOCKS) * KS * 1024 * (OUT == LORA_GLU ? 2 : 1) + (OUT == LORA_GLU || p.base ? Up::ROWS_BYTES : 0);
-  p.ahead = v_bytes + 2 * step <= VB_MAX_DYN_SMEM;     // (four slices of rank 128 beside a base leave room for one step only)
+  p.ahead = v_bytes + 2 * step <= VB_MAX_DYN_SMEM;
   const size_t smem = v_bytes + (p.ahead + 1) * step;
   // one wave of up to four blocks an SM (a wave and a few blocks take as long as two), a step each at least
   const int fit = smem <= 56 * 1024 ? 4 : smem <= 75 * 1024 ? 3 : smem <= 113 * 1024 ? 2 : 1;       // (227 KB and 1 KB of the system's a block make 228)
@@ -796,6 +805,14 @@ static int lora_up_tiles(LoraParams& p, int max_tiles, int tiles, void* stream) 
   const int most = (p.blocks + Up::BLOCKS - 1) / Up::BLOCKS;
   if (split > most) split = most;
   if (split < 1) split = 1;
+  if (OUT != LORA_GLU) {                               // each slice its share of them
+    for (int s = 0; s < p.slices; ++s) {
+      const int blocks = p.block0[s + 1] - p.block0[s], steps = (blocks + Up::BLOCKS - 1) / Up::BLOCKS;
+      const int share = static_cast<int>(static_cast<long long>(split) * blocks / p.blocks);
+      p.part0[s + 1] = p.part0[s] + (share < 1 ? 1 : share > steps ? steps : share);
+    }
+    split = p.part0[p.slices];
+  }
   VB_LAUNCH_PDL((lora_up_kernel<KS, OUT, TALL>), dim3(split, max_tiles), LORA_UP_THREADS, smem, stream, p);
   return 0;
 }
@@ -809,7 +826,7 @@ static int lora_down_launch(const LoraParams& p, int slots, void* stream) {
   CUtensorMap x_map;
   const int rc = vb_tensor_map_2d_bf16(&x_map, p.x, p.T, p.K, p.ldx, LORA_BOX_ROWS);
   if (rc) return rc;
-  VB_CHECK_CUDA(launch_kernel_cluster3(lora_down_kernel<RT>, dim3(p.k_split, lora_max_groups(p.T, slots)), dim3(LORA_DOWN_THREADS), LoraDown<RT>::SMEM, static_cast<cudaStream_t>(stream), true,
+  VB_CHECK_CUDA(launch_kernel_cluster3(lora_down_kernel<RT>, dim3(p.k_split, lora_max_groups(p.T, slots), (p.VR / 16 + RT - 1) / RT), dim3(LORA_DOWN_THREADS), LoraDown<RT>::SMEM, static_cast<cudaStream_t>(stream), true,
                                        dim3(p.k_split, 1, 1), p, x_map));
   return 0;
 }
