@@ -773,18 +773,19 @@ static int lora_tiles(int T, int slots) {
   const int adapters = T < slots + 1 ? T : slots + 1;
   return T <= 64 ? adapters : (T + 63) / 64 + adapters / 2;
 }
+template <int RT>
 static int lora_k_split(const LoraParams& p, int slots) {
   const int stages = (p.K + LORA_STAGE_K - 1) / LORA_STAGE_K, adapters = p.T < slots + 1 ? p.T : slots + 1;
-  const int groups = p.T <= 64 ? adapters : (p.T + LORA_DOWN_ROWS - 1) / LORA_DOWN_ROWS + adapters / 2;
-  // All clusters at once: one lives on the 18 SMs of a part of the chip, of which there are eight, two blocks an SM.  (4096 rows of 8192, some 35 clusters: of four
-  // 36.6 us, of seven 34.1, of eight, which do not all fit, 39.7; 1000 rows of 2048, some ten: of four 28.0, of eight 26.2.)
-  const int passes = p.VR <= 64 ? 1 : (p.VR + LoraDown<8>::N - 1) / LoraDown<8>::N;
-  int split = 8;
-  while (split > 1 && groups * passes > 8 * (36 / split)) --split;
+  const int groups = p.T <= 64 ? adapters : (p.T + LORA_DOWN_ROWS - 1) / LORA_DOWN_ROWS + adapters / 4, passes = (p.VR / 16 + RT - 1) / RT;
+  // All clusters at once (4096 rows of 8192, some 35 clusters: of four 36.6 us, of seven, of which 37 fit, 34.1, of eight, of which 33 do, 39.7)
+  // (Of a kernel with tensor memory the runtime counts one block an SM; these take half of it at most, so another kernel stands in with their shared memory.)
+  constexpr auto like = lora_up_kernel<1, LORA_BF16, true>;
+  int split = rm_smem<like>() == cudaSuccess ? 8 : 1;
+  while (split > 1 && groups * passes > rm_clusters<like>(split, LORA_UP_THREADS, LoraDown<RT>::SMEM)) --split;
   const int most = stages > 4 ? stages / 4 : 1;          // four stages a block
   if (split > most) split = most;
   // (results in fp32: sums of at most eight stages, since the tensor cores cut a sum off at every step)
-  const int longest = 8 * (p.VR > 64 ? LoraDown<8>::ACCS : LoraDown<4>::ACCS), least = (stages + longest - 1) / longest;
+  const int longest = 8 * LoraDown<RT>::ACCS, least = (stages + longest - 1) / longest;
   if (p.parts == 3 && split < least) split = least < 8 ? least : 8;
   return split;
 }
@@ -821,8 +822,9 @@ static int lora_up_launch(LoraParams& p, int max_tiles, int tiles, void* stream)
   return p.tile_rows == 16 ? lora_up_tiles<KS, OUT, false>(p, max_tiles, tiles, stream) : lora_up_tiles<KS, OUT, true>(p, max_tiles, tiles, stream);
 }
 template <int RT>
-static int lora_down_launch(const LoraParams& p, int slots, void* stream) {
+static int lora_down_launch(LoraParams& p, int slots, void* stream) {
   VB_CHECK_CUDA((rm_smem<lora_down_kernel<RT>>()));
+  p.k_split = lora_k_split<RT>(p, slots);
   CUtensorMap x_map;
   const int rc = vb_tensor_map_2d_bf16(&x_map, p.x, p.T, p.K, p.ldx, LORA_BOX_ROWS);
   if (rc) return rc;
@@ -851,7 +853,6 @@ template <int OUT>
 static int lora_launch(LoraParams& p, int slots, void* stream) {
   const int max_tiles = lora_max_tiles(p.T, slots);
   p.parts = lora_parts<OUT>();
-  p.k_split = lora_k_split(p, slots);
   if (OUT == LORA_GLU) p.blocks = p.block0[1];         // column blocks of one of the two
   if (lora_few(p)) {
     if (p.rank_tiles == 1) return lora_few_launch<1, OUT>(p, max_tiles, stream);

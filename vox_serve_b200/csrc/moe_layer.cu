@@ -1129,14 +1129,14 @@ int vb_moe_layer(float* d_y, long long ldy, const void* d_h, long long ldh, cons
   }
 #undef ML_UP
   const size_t smem_down = ml_ring_bytes(nt == 2 ? 2 : PLACES) + static_cast<size_t>(ML_WARPS) * T * ML_LD * 4 + plan_bytes;
-  const int blocks = (W + 31) / 32, fit = (nt <= 2 && smem_down <= 112 * 1024 ? 2 : 1) * sms;
-  int cluster = 1;                       // one wave, in powers of two (clusters of three leave SMs out: 69 us where two take 58)
-  while (cluster < 8 && blocks * cluster * 2 <= fit) cluster *= 2;
-  p.cluster = cluster;
+  const int blocks = (W + 31) / 32;
+  // one wave of clusters (16 rows of 1536, 48 blocks of columns: of four 57.7 us, of five, of which 56 fit, 56.7, of six, of which 45 do, 70.9; 64 rows of 1280: of two 156, of three 138)
 #define ML_DOWN(NT, S)                                                                                                  \
   do {                                                                                                                  \
     VB_CHECK_CUDA((rm_smem<moe_down_kernel<NT, S>>()));                                                                 \
-    VB_LAUNCH_PDL_CLUSTER((moe_down_kernel<NT, S>), blocks * cluster, ML_THREADS, smem_down, stream, cluster, p);       \
+    p.cluster = 8;                                                                                                      \
+    while (p.cluster > 1 && blocks > rm_clusters<moe_down_kernel<NT, S>>(p.cluster, ML_THREADS, smem_down)) --p.cluster; \
+    VB_LAUNCH_PDL_CLUSTER((moe_down_kernel<NT, S>), blocks * p.cluster, ML_THREADS, smem_down, stream, p.cluster, p);   \
   } while (0)
   if (nt == 1) ML_DOWN(1, PLACES);
   else if (nt == 2) ML_DOWN(2, 2);

@@ -61,4 +61,34 @@ inline cudaError_t rm_smem(int bytes = VB_MAX_DYN_SMEM) {
   return e;
 }
 
+// How many clusters of `size` blocks run at a time (they live on one part of the chip each, so this is less than the blocks that fit divided by the size): asked for
+// once per device, size and number of blocks an SM holds.  rm_smem first.
+template <auto Kernel>
+inline int rm_clusters(int size, int threads, size_t smem) {
+  static std::atomic<int> known[16][5][9] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 1;
+  const size_t per_sm = 228 * 1024 / (smem + 1024);
+  std::atomic<int>& n = known[dev & 15][per_sm > 4 ? 4 : per_sm][size];
+  int clusters = dev < 16 ? n.load(std::memory_order_relaxed) : 0;
+  if (clusters > 0) return clusters;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&clusters, Kernel, &cfg) != cudaSuccess || clusters < 1) {
+    cudaGetLastError();
+    return 1;
+  }
+  if (dev < 16) n.store(clusters, std::memory_order_relaxed);
+  return clusters;
+}
+
 }  // namespace vb
