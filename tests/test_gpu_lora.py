@@ -265,3 +265,50 @@ def test_lora_rows_in_a_row_and_apart(K, widths, rank, order):
     assert bool((got[ids < 0] == 0).all())
     again = ops.lora(x, bank, _plan(ids, slots))            # the order of a step's rows is kept: the same sums
     assert torch.equal(got, again)
+
+
+@pytest.mark.parametrize("T,rank", [(150, 16), (150, 128), (64, 128)])
+def test_lora_two_launch_steps_captured_and_at_once(T, rank):
+    """steps of two launches: one graph of plan, plane and gate | up replayed over changing rows and adapters, the same calls on two streams at once: the same bits"""
+    from vox_serve_b200 import ops
+    K, ff, slots = 328, 136, 3
+    bank, a, b, scale, _, x = _inputs(T, K, (ff, ff), rank, slots, 11)
+    planes = torch.randn(1, T, 2 * 3 * 48, device="cuda")
+    sx, sid, plan = x.clone(), torch.zeros(T, dtype=I32, device="cuda"), ops.LoraPlan(T, slots)
+
+    def step(rows, ids, plan):
+        ops.lora_plan(plan, ids)
+        before = ops.launch_count()
+        out = ops.lora(rows, bank, plan), ops.lora_gate_up(rows, bank, plan, planes, 48)
+        assert ops.launch_count() - before == 4
+        return out
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    streams[0].wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(streams[0]):
+        step(sx, sid, plan)
+    torch.cuda.current_stream().wait_stream(streams[0])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        got = step(sx, sid, plan)
+    cases = []
+    for seed in range(4):
+        gen = torch.Generator(device="cuda").manual_seed(seed)
+        ids = torch.randint(-1, slots, (T,), generator=gen, device="cuda").to(I32)
+        cases.append((torch.randn(T, K, generator=gen, device="cuda").to(BF16), ids if seed % 2 else ids.sort().values.contiguous()))
+    want = [step(xs, ids, ops.LoraPlan(T, slots)) for xs, ids in cases]
+    torch.cuda.synchronize()
+    plans, at_once = [ops.LoraPlan(T, slots) for _ in cases], [None] * len(cases)
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(5):
+        for i, (xs, ids) in enumerate(cases):
+            with torch.cuda.stream(streams[i % 2]):
+                at_once[i] = step(xs, ids, plans[i])
+    torch.cuda.synchronize()
+    for (xs, ids), w, o in zip(cases, want, at_once):
+        assert torch.equal(w[0], o[0]) and torch.equal(w[1], o[1])
+        sx.copy_(xs)
+        sid.copy_(ids)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])
