@@ -35,7 +35,7 @@ constexpr int LORA_PLAN_SMEM = 32 * (LORA_MAX_SLOTS + 1) * 4;
 // adapter (neighbouring tiles) that a block of the first product takes: first tile (-1: no group), adapter, rows, the first row if they follow one another in x,
 // else -1.  One block: a counting sort in shared memory
 // that keeps an adapter's rows in their order (rows that follow one another in x are then fetched as boxes): a warp a piece of the rows, its counts per adapter [32 warps]
-// [slots + 1], which become the first places of the warps' rows.
+// [slots + 1], which become the first places of the warps' rows.  Two passes over the ids and three meetings: 5 us for 32 rows, 9 for 4096, once a step.
 __global__ void __launch_bounds__(1024) lora_plan_kernel(int32_t* __restrict__ tiles, const int32_t* __restrict__ ids, int T, int slots, int tile_rows, int max_tiles,
                                                          int max_groups) {
   extern __shared__ __align__(128) int cnt[];
@@ -471,7 +471,9 @@ __host__ __device__ constexpr int lora_parts() { return OUT == LORA_F32 ? 3 : 2;
 
 // Block: a tile x a range of column blocks, four warps, in steps: tiles of 64 rows, a warp per 16 rows, all warps the same one or two column blocks (so that of base and
 // results 128 bytes of a row at least move together); tiles of 16 rows, a warp per column block.  What a step reads, its part of B and the rows' part of base or
-// planes, is copied a step ahead; v is read once.  All but v is older than the first product, so the first steps' copies are on their way when that ends.
+// planes, is copied a step ahead; v is read once.  All but v is older than the first product, so the first steps' copies are on their way when that ends.  What bounds it are its
+// own instructions' latencies (16 warps an SM, 40 % of the issue slots): 4096 rows of 2048 columns at rank 64 in bf16 10 us for 34 MB, gate | up of 1000 rows of 2 x 8192 columns
+// 15 for 82 MB.  (Two steps ahead in half as many blocks: 38 us instead of 27 for the latter's whole call.)
 constexpr int LORA_UP_THREADS = 128;
 template <int OUT>
 __host__ __device__ constexpr int lora_row_bytes() { return OUT == LORA_GLU ? 256 : OUT == LORA_F32 ? 128 : 64; }      // of a column block in base or planes
@@ -621,7 +623,9 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
 }
 
 // ---- both, for few rows -------------------------------------------------------------------------------------------------------------
-// A cluster of eight blocks per tile of up to 16 rows.  RT: rank tiles, all of them in one pass over the block's share of K.
+// A cluster of eight blocks per tile of up to 16 rows.  RT: rank tiles, all of them in one pass over the block's share of K.  One chain: the tile's record, a round or two of
+// loads of x and A, the warps' and the cluster's meeting, the columns; each is latency.  32 rows with an adapter each, 2048 x 2048 at rank 16 (4.3 MB): 4.2 us a call in
+// a chain; 64 rows with 12 adapters, 4096 to 4608 columns at rank 32 (14 MB): 8.1.  In two launches 8.3 and 11.7.
 constexpr int LORA_CLUSTER = 8, LORA_FEW_RANKS = 128, LORA_FEW_LD = 20;
 template <int KS, int OUT, int RT>
 __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams p) {
@@ -789,8 +793,9 @@ static int lora_k_split(const LoraParams& p, int slots) {
   if (p.parts == 3 && split < least) split = least < 8 ? least : 8;
   return split;
 }
-// One launch for a step of at most 64 rows, where an adapter is what eight SMs take in good time.
-static bool lora_few(const LoraParams& p) { return p.T <= 64 && p.VR <= LORA_FEW_RANKS && p.rank_tiles <= 4 && (p.a_slot + p.b_slot) * 16 <= 2 << 20; }
+// One launch for a step of at most 64 rows, where an adapter is what eight SMs take in good time.  (Rank 64, one launch / two: 1 MB 5.7 / 7.5 us for a row, 8.6 / 11.1 for 64 rows
+// of 12 adapters; 3 MB 12.4 / 11.7 and 18.1 / 22.5; 4 MB 15.5 / 13.9 and 23.4 / 27.7.)
+static bool lora_few(const LoraParams& p) { return p.T <= 64 && p.VR <= LORA_FEW_RANKS && p.rank_tiles <= 4 && (p.a_slot + p.b_slot) * 16 <= 3 << 20; }
 
 template <int KS, int OUT, bool TALL>
 static int lora_up_tiles(LoraParams& p, int max_tiles, int tiles, void* stream) {

@@ -16,6 +16,9 @@
 //         shared memory; up to eight blocks of a cluster divide the k blocks and add up through distributed shared memory.  No atomics: products,
 //         warps and blocks are added in a fixed order
 //
+// What bounds it: HBM at 64 rows (8 of 128 experts of 2048 x 768: 1.2 GB in 191 us, 6.3 TB/s), below that starts (three of 2 to 3 us) and blocks that end in whole units (8 rows, 6 of
+// 64 experts of 2048 x 1024: 86 us for 440 MB; gate and up 5.6 TB/s, down 4.1; one row, 2 of 8 experts and the shared one of 1024 x 1024: 16 us for 19 MB).
+//
 // A table that names an expert twice for a row counts it once with both weights; an index that is no expert counts as none.
 #include "../../include/vb_api.h"
 #define VB_PDL_FAMILY 4
