@@ -2008,7 +2008,7 @@ def _lora_check(who: str, x: torch.Tensor, bank: LoraBank, plan: LoraPlan) -> No
 def lora(x: torch.Tensor, bank: LoraBank, plan: LoraPlan, out: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[t] = base[t] + B_a (scale_a A_a x[t]) with the adapter a of row t in ``plan`` (none: base[t]).  x bf16 [T, K]; out fp32 [T, N] (one more split-K
     plane of the projection: ``gemm`` mode 1) or bf16 (rounded once), by ``out``, else by ``base``, else fp32.  ``base``: of out's type, may be out
-    itself; None: zeros."""
+    itself; None: zeros.  K is divided by the number of rows and slots: the same rows in a step of another size agree to fp32 rounding, not to the bit."""
     _lora_check("lora", x, bank, plan)
     T, N = x.shape[0], bank.N
     f32, ld_out = True, N
