@@ -15,8 +15,10 @@
 //   down  v of any step: a group x a piece of K a block (tcgen05), the blocks of a group a cluster that adds up its parts
 //   up    a tile x some columns a block (mma.sync: as many products as loads), all that it reads but v on its way before v is there
 //
-// Sums are fp32.  v is not rounded on its way into the second product: it enters as three bf16 parts (exact, rowmma.cuh) where the result is fp32, as
-// two (off by 2^-15 of v at most) where the result is rounded to bf16 anyway.
+// Sums are fp32.  v is not rounded on its way into the second product: it enters as three bf16 parts (exact, rowmma.cuh).  But for large steps whose result is
+// rounded to bf16 anyway, by up to 2^-8 of itself: two parts there (rounded to nearest, off by 2^-17 of v at most).  A third of the second product's reads and
+// products less: 4096 rows of 2048 columns at rank 64 32.0 us a call instead of 36.2, gate | up of 1000 rows of 8192 at rank 32 25.5 instead of 28.7; in
+// steps of at most 64 rows the third part costs nothing that can be measured (17 rows of gate | up 5.5 us with it and without).
 #include "../../include/vb_api.h"
 #define VB_PDL_FAMILY 4
 #include "rowmma.cuh"
@@ -127,6 +129,7 @@ struct LoraParams {
   const float* scale;
   uint32_t* v;                     // [tiles][tile_rows / 16][S][parts][rank / 16][32 lanes][4]: v as the second product takes it
   int T, K, rank_tiles, VR, k_split, parts;      // VR = S * rank
+  bool f32;                        // the result is fp32
   unsigned char* wait_flag;
   // second product
   int blocks;                      // column blocks of 32 over all slices (of gate | up: of one)
@@ -145,13 +148,21 @@ struct LoraParams {
 // In the order of the lanes: [m16 block][slice][part][rank tile][32 lanes][4 registers].
 __device__ __forceinline__ void lora_put(uint32_t* frags, int slices, int parts, int log_ks, int r, int k, float a, float b) {      // row r, v[k] and v[k + 1]
   const int tile = k >> 4, s = tile >> log_ks, ks = 1 << log_ks, t = tile & (ks - 1);
-  float h0, m0, l0, h1, m1, l1;
-  bf16_parts(a, h0, m0, l0);
-  bf16_parts(b, h1, m1, l1);
   uint32_t* at = frags + ((((r >> 4) * slices + s) * parts * ks + t) * 32 + (r & 7) * 4 + (k & 7) / 2) * 4 + (r & 15) / 8 + (k & 15) / 8 * 2;
-  at[0] = pack_cut(h0, h1);
-  at[ks * 128] = pack_cut(m0, m1);
-  if (parts > 2) at[2 * ks * 128] = pack_cut(l0, l1);
+  if (parts > 2) {
+    float h0, m0, l0, h1, m1, l1;
+    bf16_parts(a, h0, m0, l0);
+    bf16_parts(b, h1, m1, l1);
+    at[0] = pack_cut(h0, h1);
+    at[ks * 128] = pack_cut(m0, m1);
+    at[2 * ks * 128] = pack_cut(l0, l1);
+  } else {
+    float h0, m0, h1, m1;
+    bf16_near(a, h0, m0);
+    bf16_near(b, h1, m1);
+    at[0] = pack_cut(h0, h1);
+    at[ks * 128] = pack_bf16(m0, m1);
+  }
 }
 
 // 16 bytes past the registers and L1; zeros where `bytes` is 0 instead of 16 (nothing is read then)
@@ -431,7 +442,7 @@ __device__ __forceinline__ void lora_result(void* out, float (&y)[8], const void
   }
 }
 // g / (1 + exp(-g)) by the special function unit without its ranges below 2^-126 (1000 rows of gate | up: 26.3 us with the ranges, 25.8 without).  The power of
-// two is off by 2^-22, its argument's rounding by 1.2 |g| units of 2^-24, the reciprocal by 2^-23: far below half a step of bf16, 2^-9.  Below g = -87 the reciprocal is 0 (the
+// two is off by 2^-22, its argument's rounding by 1.2 |g| units of 2^-24, the reciprocal by 2^-23: far below half a step of bf16, 2^-8.  Below g = -87 the reciprocal is 0 (the
 // value 1e-36 at most).
 __device__ __forceinline__ float lora_silu(float g) {
   float e, r;
@@ -466,8 +477,9 @@ __device__ __forceinline__ void* lora_place(const LoraParams& p, long long row, 
   if (OUT == LORA_GLU && p.xt_rows) return static_cast<__nv_bfloat16*>(p.out) + xt_index(static_cast<int>(row), col, p.xt_rows, p.xt_kb);
   return static_cast<__nv_bfloat16*>(p.out) + row * p.ldo + col;
 }
-template <int OUT>
-__host__ __device__ constexpr int lora_parts() { return OUT == LORA_F32 ? 3 : 2; }
+// bf16 parts of v; TALL: tiles of 64 rows
+template <int OUT, bool TALL>
+__host__ __device__ constexpr int lora_parts() { return OUT == LORA_F32 || !TALL ? 3 : 2; }
 
 // Block: a tile x a range of column blocks, four warps, in steps: tiles of 64 rows, a warp per 16 rows, all warps the same one or two column blocks (so that of base and
 // results 128 bytes of a row at least move together); tiles of 16 rows, a warp per column block.  What a step reads, its part of B and the rows' part of base or
@@ -491,7 +503,7 @@ template <int KS, int OUT, bool TALL>
 __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraParams p) {
   extern __shared__ __align__(128) uint8_t smem8[];
   using Up = LoraUp<OUT, TALL>;
-  constexpr int PARTS = lora_parts<OUT>(), B_BYTES = KS * 1024, SEG = lora_row_bytes<OUT>(), LD = Up::LD, WIDE = Up::WIDE, STEP = Up::BLOCKS, BOTH = OUT == LORA_GLU ? 2 : 1;
+  constexpr int PARTS = lora_parts<OUT, TALL>(), B_BYTES = KS * 1024, SEG = lora_row_bytes<OUT>(), LD = Up::LD, WIDE = Up::WIDE, STEP = Up::BLOCKS, BOTH = OUT == LORA_GLU ? 2 : 1;
   constexpr int TILE = TALL ? 64 : 16;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int32_t* rec = p.tiles + static_cast<long long>(blockIdx.y) * (4 + TILE);
@@ -634,7 +646,7 @@ __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams
   float* red = reinterpret_cast<float*>(smem8);                         // [8 warps][VR][LD]
   float* mine = red + 8 * VR * LD;                                      // [16 rows][VR]: this block's part of v
   uint32_t* frags = reinterpret_cast<uint32_t*>(mine + 16 * VR);        // the sum, as parts
-  constexpr int PARTS = lora_parts<OUT>();
+  constexpr int PARTS = lora_parts<OUT, false>();
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int rank = blockIdx.x % LORA_CLUSTER;
   pdl_sync();
@@ -790,7 +802,7 @@ static int lora_k_split(const LoraParams& p, int slots) {
   if (split > most) split = most;
   // (results in fp32: sums of at most eight stages, since the tensor cores cut a sum off at every step)
   const int longest = 8 * LoraDown<RT>::ACCS, least = (stages + longest - 1) / longest;
-  if (p.parts == 3 && split < least) split = least < 8 ? least : 8;
+  if (p.f32 && split < least) split = least < 8 ? least : 8;
   return split;
 }
 // One launch for a step of at most 64 rows, where an adapter is what eight SMs take in good time.  (Rank 64, one launch / two: 1 MB 5.7 / 7.5 us for a row, 8.6 / 11.1 for 64 rows
@@ -801,7 +813,7 @@ template <int KS, int OUT, bool TALL>
 static int lora_up_tiles(LoraParams& p, int max_tiles, int tiles, void* stream) {
   using Up = LoraUp<OUT, TALL>;
   VB_CHECK_CUDA((rm_smem<lora_up_kernel<KS, OUT, TALL>>()));
-  const size_t v_bytes = static_cast<size_t>(p.tile_rows >> 4) * (OUT == LORA_GLU ? 2 : 1) * lora_parts<OUT>() * KS * 512,
+  const size_t v_bytes = static_cast<size_t>(p.tile_rows >> 4) * (OUT == LORA_GLU ? 2 : 1) * lora_parts<OUT, TALL>() * KS * 512,
                step = static_cast<size_t>(Up::BLOCKS) * KS * 1024 * (OUT == LORA_GLU ? 2 : 1) + (OUT == LORA_GLU || p.base ? Up::ROWS_BYTES : 0);
   p.ahead = v_bytes + 2 * step <= VB_MAX_DYN_SMEM;
   const size_t smem = v_bytes + (p.ahead + 1) * step;
@@ -840,7 +852,7 @@ static int lora_down_launch(LoraParams& p, int slots, void* stream) {
 template <int KS, int OUT, int RT>
 static int lora_few_tiles(const LoraParams& p, int tiles, void* stream) {
   VB_CHECK_CUDA((rm_smem<lora_few_kernel<KS, OUT, RT>>()));
-  const size_t smem = (8 * RT * 16 * LORA_FEW_LD + 16 * RT * 16) * sizeof(float) + static_cast<size_t>(p.VR >> 4) * lora_parts<OUT>() * 512;
+  const size_t smem = (8 * RT * 16 * LORA_FEW_LD + 16 * RT * 16) * sizeof(float) + static_cast<size_t>(p.VR >> 4) * lora_parts<OUT, false>() * 512;
   VB_LAUNCH_PDL_CLUSTER((lora_few_kernel<KS, OUT, RT>), tiles * LORA_CLUSTER, LORA_THREADS, smem, stream, LORA_CLUSTER, p);
   return 0;
 }
@@ -857,7 +869,8 @@ static int lora_few_launch(const LoraParams& p, int tiles, void* stream) {
 template <int OUT>
 static int lora_launch(LoraParams& p, int slots, void* stream) {
   const int max_tiles = lora_max_tiles(p.T, slots);
-  p.parts = lora_parts<OUT>();
+  p.parts = p.tile_rows == 16 ? lora_parts<OUT, false>() : lora_parts<OUT, true>();
+  p.f32 = OUT == LORA_F32;
   if (OUT == LORA_GLU) p.blocks = p.block0[1];         // column blocks of one of the two
   if (lora_few(p)) {
     if (p.rank_tiles == 1) return lora_few_launch<1, OUT>(p, max_tiles, stream);

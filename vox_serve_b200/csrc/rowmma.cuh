@@ -19,9 +19,8 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// An fp32 value as bf16 parts whose sum it is: the upper 8 bits of the significand, the next 8, the last 8 (cut off, not rounded, so that a part
-// never overflows and three of them lose nothing).  Two parts are off by at most 2^-15 of the value, three by nothing.  What is not finite
-// stays whole in the first part (inf - inf would make it NaN).
+// An fp32 value as three bf16 parts whose sum it is: the upper 8 bits of the significand, the next 8, the last 8 (cut off, not rounded, so that a part
+// never overflows and nothing is lost).  What is not finite stays whole in the first part (inf - inf would make it NaN).
 __device__ __forceinline__ float bf16_cut(float v) { return __uint_as_float(__float_as_uint(v) & 0xffff0000u); }
 __device__ __forceinline__ void bf16_parts(float v, float& hi, float& mid, float& lo) {
   hi = bf16_cut(v);
@@ -33,6 +32,14 @@ __device__ __forceinline__ void bf16_parts(float v, float& hi, float& mid, float
   const float r = v - hi;
   mid = bf16_cut(r);
   lo = r - mid;
+}
+// ... as two: the nearest bf16 value (cut off instead where that is infinite), and what is left, which is exact in fp32 and rounded by whoever packs it: together
+// off by at most half a step of what 16 bits hold, 2^-17 of the value.
+__device__ __forceinline__ void bf16_near(float v, float& hi, float& rest) {
+  const bool finite = (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u;
+  hi = __bfloat162float(__float2bfloat16_rn(v));
+  if (finite && isinf(hi)) hi = bf16_cut(v);
+  rest = finite ? v - hi : 0.f;
 }
 // two neighbours' upper halves as one register (both hold bf16 values)
 __device__ __forceinline__ uint32_t pack_cut(float first, float second) {
