@@ -173,11 +173,15 @@ class LlamaAdapters:
                    "down": ("mlp.down_proj",)}
 
     def __init__(self, dims: LlamaDims, slots: int, rank: int, device="cuda"):
+        self.dims, self.slots, self.rank = dims, slots, rank
+        self.layers = [{name: ops.LoraBank(slots, K, widths, rank, device) for name, (K, widths) in self.shapes(dims).items()} for _ in range(dims.num_hidden_layers)]
+
+    @staticmethod
+    def shapes(dims: LlamaDims) -> Dict[str, Tuple[int, Tuple[int, ...]]]:
+        """inputs and widths of the slices of every projection"""
         H, I, D = dims.hidden_size, dims.intermediate_size, dims.head_dim
         hq, hkv = dims.num_attention_heads * D, dims.num_key_value_heads * D
-        shapes = {"qkv": (H, (hq, hkv, hkv)), "o": (hq, (H,)), "gu": (H, (I, I)), "down": (I, (H,))}
-        self.dims, self.slots, self.rank = dims, slots, rank
-        self.layers = [{name: ops.LoraBank(slots, K, widths, rank, device) for name, (K, widths) in shapes.items()} for _ in range(dims.num_hidden_layers)]
+        return {"qkv": (H, (hq, hkv, hkv)), "o": (hq, (H,)), "gu": (H, (I, I)), "down": (I, (H,))}
 
     def load(self, slot: int, state: Dict[str, torch.Tensor], scale: float, prefix: str = "model.") -> None:
         """state: ``<prefix>layers.<i>.<module>.lora_A.weight`` [r, in] and ``.lora_B.weight`` [out, r] as adapter checkpoints name them; modules that it leaves
@@ -286,10 +290,19 @@ class LlamaEngine:
 
     def set_adapters(self, adapters: LlamaAdapters) -> None:
         """Adapters that a step may name (``forward(adapters=plan)``).  Their products are one more plane beside the split-K planes of a projection, which its
-        consumer sums anyway; the gate/up projection leaves planes too in such a step."""
+        consumer sums anyway; the gate/up projection leaves planes too in such a step.
+        Once per engine: a captured step holds the addresses of the banks and of the planes.  Adapters come and go by ``LlamaAdapters.load`` and its slots;
+        another object is refused."""
         d, R = self.dims, self.max_rows
-        if (adapters.dims.hidden_size, adapters.dims.intermediate_size, len(adapters.layers)) != (d.hidden_size, d.intermediate_size, d.num_hidden_layers):
+        if adapters is self.adapters:
+            return
+        if self.adapters is not None:
+            raise VoxB200Error("set_adapters: the engine has adapters already, which captured steps may read (load others into their slots)")
+        if len(adapters.layers) != d.num_hidden_layers or adapters.shapes(adapters.dims) != adapters.shapes(d):
             raise VoxB200Error("set_adapters: adapters of another model")
+        on = adapters.layers[0]["qkv"].a.device
+        if on != self.hidden.device:
+            raise VoxB200Error(f"set_adapters: adapters on {on}, the engine is on {self.hidden.device}")
         small = (max(self.split_qkv, self.split_o, self.split_down) + 1) * min(R, self.FUSED_MAX_ROWS)
         rows = max(small, ops.WIDE_SPLIT_ROWS + R, 2 * R) if R >= ops.WIDE_MIN_ROWS else small
         self.adapters = adapters
@@ -337,8 +350,11 @@ class LlamaEngine:
         return the final-normed rows [n_out or n_rows, hidden] bf16, row-major (the backbone state a depth decoder
         starts from, csm.py:290-300).  ``adapters``: the plan of the rows' adapters (ops.lora_plan; ``set_adapters`` first)."""
         d, w, R = self.dims, self.w, n_rows
-        if adapters is not None and self.adapters is None:
-            raise VoxB200Error("forward: the engine has no adapters (set_adapters)")
+        if adapters is not None:                   # (before anything is written)
+            if self.adapters is None:
+                raise VoxB200Error("forward: the engine has no adapters (set_adapters)")
+            if (adapters.n_rows, adapters.slots) != (R, self.adapters.slots):
+                raise VoxB200Error(f"forward: the plan of adapters is of {adapters.n_rows} rows and {adapters.slots} slots, the step of {R} and {self.adapters.slots}")
         plan = self.plan if plan is None else plan
         if R > self.max_rows:
             raise VoxB200Error(f"{R} rows exceed the engine's max_rows {self.max_rows}")
