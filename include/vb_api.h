@@ -894,7 +894,7 @@ int vb_selective_scan_tiled(void* d_out, int ld_out, float* d_state, float* d_sc
  * Low-rank adapters of many requests beside a shared projection (csrc/lora.cu):
  *   out[t][n] = base[t][n] + sum_j B_a[n][j] (scale_a sum_k A_a,s[j][k] x[t][k]),   a = ids[t] (outside 0 .. slots-1: base alone), s = n's slice
  * VbLoraBank (HOST struct): the adapters in the order that csrc/lora.cu states (ops.LoraBank writes it).  slots 1 .. 1023, rank padded to 16, 32, 64 or
- *   128, K and the widths of the 1 .. 4 slices multiples of 8.
+ *   128, K and the widths of the 1 .. 4 slices multiples of 8 (at most 2^24); d_a and d_b 16-byte aligned.
  * vb_lora_plan: rows of a step by adapter, once per step for every projection of every layer: d_tiles, vb_lora_plan_bytes(T, slots) bytes, 16-byte
  *   aligned.
  * vb_lora: out and base fp32 (out_f32) or bf16, rows 16-byte aligned; d_base may be NULL (zeros) or d_out.  Every row 0 .. T-1 of out is written, nothing
@@ -916,7 +916,7 @@ int vb_lora_gate_up(void* d_act, long long ld_act, int xt_rows, const float* d_p
 /* A mixture-of-experts layer for at most vb_moe_layer_max_rows() rows (csrc/moe_layer.cu); of the experts' matrices it reads those that a row chose.
  * VbMoeWeights (HOST struct): d_up: packed tiles (vb_pack_weight_tiles, up_rows rows each) of the experts' gate | up rows (interleaved; act 0 silu, 1 clamped) or up
  *   rows (act 2 relu^2, 3 gelu, 4 tanh gelu), one expert after the other, the shared one (shared_ff > 0) last; d_down: packed tiles of 128 rows of [width][experts *
- *   ff + shared_ff].  width a multiple of 8, ff and shared_ff of 64.
+ *   ff + shared_ff], both 16-byte aligned.  width a multiple of 8 (at most 2^24), ff and shared_ff of 64 (at most 2^17).
  * VbMoeRouter (HOST struct): kind 0 softmax over the chosen logits (+ d_bias), 1 sigmoid scores (chosen by score + d_bias within the kept groups, weights over their
  *   sum), 2 softmax over all experts (chosen within the kept groups, weights as they are), 3 d_table[d_ids[t]] (int32 [vocab][top]; weights 1 / top; an entry
  *   that is no expert counts as none, one named twice with both weights).  Ties go to the lower expert; a NaN ranks above everything.  d_shared_gate: the

@@ -893,10 +893,12 @@ static int lora_launch(LoraParams& p, int slots, void* stream) {
 // checks and fills what both entry points share
 static int lora_bank(const char* who, LoraParams& p, const VbLoraBank* bank, int T) {
   VB_CHECK_ARG(bank && bank->d_a && bank->d_b && bank->d_scale, "%s: null pointer", who);
+  VB_CHECK_ARG(reinterpret_cast<uintptr_t>(bank->d_a) % 16 == 0 && reinterpret_cast<uintptr_t>(bank->d_b) % 16 == 0 && reinterpret_cast<uintptr_t>(bank->d_scale) % 4 == 0,
+               "%s: the bank must be 16-byte aligned", who);
   VB_CHECK_ARG(bank->slots >= 1 && bank->slots <= LORA_MAX_SLOTS, "%s: %d adapters; 1 to %d", who, bank->slots, LORA_MAX_SLOTS);
   VB_CHECK_ARG(bank->rank == 16 || bank->rank == 32 || bank->rank == 64 || bank->rank == 128, "%s: padded rank %d must be 16, 32, 64 or 128", who, bank->rank);
   VB_CHECK_ARG(bank->slices >= 1 && bank->slices <= LORA_MAX_SLICES, "%s: %d slices; 1 to %d", who, bank->slices, LORA_MAX_SLICES);
-  VB_CHECK_ARG(bank->K >= 8 && bank->K % 8 == 0, "%s: inputs of %d; a multiple of 8", who, bank->K);
+  VB_CHECK_ARG(bank->K >= 8 && bank->K % 8 == 0 && bank->K <= (1 << 24), "%s: inputs of %d; a multiple of 8", who, bank->K);
   p.slices = bank->slices;
   p.block0[0] = p.col0[0] = 0;
   for (int s = 0; s < p.slices; ++s) {
@@ -926,6 +928,7 @@ static int lora_setup(const char* who, LoraParams& p, const void* d_x, long long
   const int rc = lora_bank(who, p, bank, T);
   if (rc) return rc;
   VB_CHECK_ARG(d_x && d_tiles, "%s: null pointer", who);
+  VB_CHECK_ARG(reinterpret_cast<uintptr_t>(d_tiles) % 16 == 0, "%s: the plan must be 16-byte aligned", who);
   VB_CHECK_ARG(T <= LORA_MAX_ROWS, "%s: %d rows; at most %d", who, T, LORA_MAX_ROWS);
   VB_CHECK_ARG(ldx % 8 == 0 && ldx >= p.K && reinterpret_cast<uintptr_t>(d_x) % 16 == 0, "%s: rows of x must be 16-byte aligned (K %d, row stride %lld)", who, p.K, ldx);
   p.tiles = static_cast<const int32_t*>(d_tiles);
@@ -951,7 +954,7 @@ size_t vb_lora_plan_bytes(int T, int slots) {
 
 int vb_lora_plan(void* d_tiles, const int32_t* d_ids, int T, int slots, void* stream) {
   VB_CHECK_ARG(d_tiles && d_ids, "vb_lora_plan: null pointer");
-  VB_CHECK_ARG(reinterpret_cast<uintptr_t>(d_tiles) % 16 == 0, "vb_lora_plan: the plan must be 16-byte aligned");
+  VB_CHECK_ARG(reinterpret_cast<uintptr_t>(d_tiles) % 16 == 0 && reinterpret_cast<uintptr_t>(d_ids) % 4 == 0, "vb_lora_plan: the plan must be 16-byte aligned, ids 4-byte");
   VB_CHECK_ARG(slots >= 1 && slots <= LORA_MAX_SLOTS, "vb_lora_plan: %d adapters; 1 to %d", slots, LORA_MAX_SLOTS);
   VB_CHECK_ARG(T >= 1 && T <= LORA_MAX_ROWS, "vb_lora_plan: %d rows; 1 to %d", T, LORA_MAX_ROWS);
   VB_CHECK_CUDA((rm_smem<lora_plan_kernel>(LORA_PLAN_SMEM)));

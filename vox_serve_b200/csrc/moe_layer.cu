@@ -1031,7 +1031,10 @@ int vb_moe_layer(float* d_y, long long ldy, const void* d_h, long long ldh, cons
                ML_MAX_EXPERTS, top, ML_MAX_TOP);
   VB_CHECK_ARG(kind >= 0 && kind <= 3, "vb_moe_layer: router %d", kind);
   VB_CHECK_ARG(kind == ML_TABLE ? d_ids && router->d_table && router->vocab > 0 : router->d_weight != nullptr, "vb_moe_layer: the router lacks its matrix, or its table and ids");
-  VB_CHECK_ARG(W >= 8 && W % 8 == 0 && ldh % 8 == 0 && ldh >= W && ldy >= W && reinterpret_cast<uintptr_t>(d_h) % 16 == 0 &&
+  const auto off = [](const void* ptr, int align) { return reinterpret_cast<uintptr_t>(ptr) % align != 0; };
+  VB_CHECK_ARG(!off(weights->d_up, 16) && !off(weights->d_down, 16) && !off(d_y, 4) && !off(d_ids, 4) && !off(router->d_bias, 4) && !off(router->d_table, 4),
+               "vb_moe_layer: the experts' matrices must be 16-byte aligned, y, ids, bias and table 4-byte");
+  VB_CHECK_ARG(W >= 8 && W <= (1 << 24) && W % 8 == 0 && ldh % 8 == 0 && ldh >= W && ldy >= W && reinterpret_cast<uintptr_t>(d_h) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(router->d_weight) % 16 == 0 && reinterpret_cast<uintptr_t>(router->d_shared_gate) % 16 == 0,
                "vb_moe_layer: rows must be multiples of 8 elements, 16-byte aligned (width %d)", W);
   VB_CHECK_ARG(groups <= 1 || ((kind == ML_SIGMOID || kind == ML_SOFTMAX_ALL) && experts % groups == 0 && keep >= 1 && keep <= groups && keep * (experts / groups) >= top),

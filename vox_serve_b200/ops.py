@@ -1910,8 +1910,8 @@ class LoraBank:
         widths = tuple(int(w) for w in widths)
         _refuse(not 1 <= slots <= 1023, f"LoraBank: {slots} adapters; 1 to 1023")
         _refuse(not 1 <= rank <= 128, f"LoraBank: rank {rank}; 1 to 128")
-        _refuse(not 1 <= len(widths) <= 4 or any(w < 8 or w % 8 for w in widths), f"LoraBank: slices {widths}; one to four, multiples of 8 columns")
-        _refuse(K < 8 or K % 8 != 0, f"LoraBank: inputs of {K}; a multiple of 8")
+        _refuse(not 1 <= len(widths) <= 4 or any(not 8 <= w <= 1 << 24 or w % 8 for w in widths), f"LoraBank: slices {widths}; one to four, multiples of 8 columns (at most 2^24)")
+        _refuse(not 8 <= K <= 1 << 24 or K % 8 != 0, f"LoraBank: inputs of {K}; a multiple of 8 (at most 2^24)")
         self.slots, self.K, self.widths, self.rank = int(slots), int(K), widths, int(rank)
         self.N = sum(widths)
         self.rank_pad = next(r for r in (16, 32, 64, 128) if rank <= r)
@@ -1974,7 +1974,7 @@ class LoraPlan:
     """Rows of a step by adapter (``lora_plan``): made once per step, read by every projection of every layer."""
 
     def __init__(self, max_rows: int, slots: int, device="cuda"):
-        _refuse(max_rows < 1 or not 1 <= slots <= 1023, f"LoraPlan: {max_rows} rows, {slots} adapters (1 to 1023)")
+        _refuse(not 1 <= max_rows <= 1 << 21 or not 1 <= slots <= 1023, f"LoraPlan: {max_rows} rows (1 to 2^21), {slots} adapters (1 to 1023)")
         self.max_rows, self.slots, self.n_rows = int(max_rows), int(slots), 0
         lib = _lib.load()
         n = max(lib.vb_lora_plan_bytes(min(max_rows, 64), slots), lib.vb_lora_plan_bytes(max_rows, slots))
@@ -2081,8 +2081,9 @@ class MoeWeights:
         _refuse(act not in MOE_LAYER_ACTS, f"MoeWeights: activation {act!r}; one of {sorted(MOE_LAYER_ACTS)}")
         _refuse(act == "clamped_glu" and not limit > 0.0, f"MoeWeights: the clamped gate needs a positive limit, not {limit}")
         _refuse(not 1 <= experts <= 1024, f"MoeWeights: {experts} experts; 1 to 1024")
-        _refuse(width < 8 or width % 8 != 0, f"MoeWeights: width {width}; a multiple of 8")
-        _refuse(ff < 64 or ff % 64 != 0 or shared_ff < 0 or shared_ff % 64 != 0, f"MoeWeights: expert widths {ff} and {shared_ff}; multiples of 64 (pack pads)")
+        _refuse(not 8 <= width <= 1 << 24 or width % 8 != 0, f"MoeWeights: width {width}; a multiple of 8 (at most 2^24)")
+        _refuse(not 64 <= ff <= 1 << 17 or ff % 64 != 0 or not 0 <= shared_ff <= 1 << 17 or shared_ff % 64 != 0,
+                f"MoeWeights: expert widths {ff} and {shared_ff}; multiples of 64 (pack pads), at most 2^17")
         rows = 2 if act.endswith("glu") else 1
         n_all = experts * ff + shared_ff
         _refuse(tuple(up.shape) != (rows * n_all, width) or tuple(down.shape) != (width, n_all), f"MoeWeights: packed matrices {up.shape} and {down.shape} do not "
