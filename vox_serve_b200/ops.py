@@ -2140,7 +2140,7 @@ class MoeRouter:
       "softmax_all"  softmax over all experts, chosen within the kept groups, weights as they are (``moe_route_groups``)
       "table"        the row's token id picks them, each 1 / top (``moe_route_table``)
     weight fp32 [experts, width]; shared_gate fp32 [width] ("sigmoid", "table"): the shared expert times sigmoid(shared_gate . h)."""
-    __slots__ = ("kind", "top", "weight", "bias", "groups", "keep", "shared_gate", "table", "_struct", "_ptr", "_devices", "_weights")
+    __slots__ = ("kind", "top", "weight", "bias", "groups", "keep", "shared_gate", "table", "_struct", "_ptr", "_device", "_shape", "_gate")
 
     def __init__(self, kind: str, top: int, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, groups: int = 0, keep: int = 0,
                  shared_gate: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None):
@@ -2163,17 +2163,14 @@ class MoeRouter:
         self.shared_gate, self.table = shared_gate, table
         self._struct = _lib.MoeRouterStruct(_p(weight), _p(bias), _p(shared_gate), _p(table), MOE_LAYER_ROUTERS[kind], self.top, self.groups, self.keep,
                                             0 if table is None else table.shape[0])
-        self._ptr, self._devices = ctypes.addressof(self._struct), {t.get_device() for t in (weight, bias, shared_gate, table) if t is not None}
-        self._weights = None
+        on = {t.get_device() for t in (weight, bias, shared_gate, table) if t is not None}
+        self._ptr, self._device = ctypes.addressof(self._struct), on.pop() if len(on) == 1 else -2
+        self._shape, self._gate = None if weight is None else tuple(weight.shape), None if shared_gate is None else shared_gate.numel()
 
     def _goes_with(self, weights: MoeWeights) -> bool:
-        """whether the router's matrix has the weights' shape and device (remembered for the weights that it was asked about last)"""
-        if self._weights is not weights:
-            if (self.top > weights.experts or self._devices != {weights._device} or (self.weight is not None and tuple(self.weight.shape) != (weights.experts, weights.width))
-                    or (self.shared_gate is not None and (not weights.shared_ff or self.shared_gate.numel() != weights.width))):
-                return False
-            self._weights = weights
-        return True
+        """whether the router's matrix has the weights' shape and device"""
+        return (self.top <= weights.experts and self._device == weights._device and (self._shape is None or self._shape == (weights.experts, weights.width))
+                and (self._gate is None or (weights.shared_ff > 0 and self._gate == weights.width)))
 
 
 def _moe_layer_check(h: torch.Tensor, weights: MoeWeights, router: MoeRouter, ids: Optional[torch.Tensor]) -> None:
@@ -2192,7 +2189,7 @@ def moe_layer(h: torch.Tensor, weights: MoeWeights, router: MoeRouter, ids: Opti
     sum.  h bf16 [T, width]; ids int32 [T] (token ids) for a table router; out fp32 [T, width].  The matrices of experts that no row chose are not read; nothing
     is rounded between the two products."""
     T, W = h.shape[0], weights.width
-    # (one comparison per fact when all goes together: every call passes here; what matches has been compared before)
+    # (one comparison per fact when all goes together: every call passes here)
     if not (h.is_cuda and h.dtype is BF16 and h.dim() == 2 and h.shape[1] == W and T <= MOE_LAYER_MAX_ROWS and h.get_device() == weights._device == _device_index()
             and router._goes_with(weights) and h.is_contiguous() and (ids is None) == (router.table is None)
             and (ids is None or (ids.dtype is torch.int32 and ids.numel() == T and ids.get_device() == weights._device and ids.is_contiguous()))):
