@@ -54,3 +54,25 @@ def test_v_between_the_products(form, kind):
     assert ops.launch_count() - before == launches
     assert torch.equal(want.float().double(), want)
     assert torch.equal(got.float().cpu(), want.float().to(BF16).float())
+
+
+@pytest.mark.parametrize("T,K,rank", [(9, 65536, 128), (150, 65536, 128), (9, 65536, 16), (200, 65536, 16), (40, 28672, 64), (150, 28672, 64), (64, 14336, 128), (150, 14336, 128),
+                                      (9, 32768, 16), (9, 8192, 128)])
+def test_long_sums_of_fp32_results(T, K, rank):
+    """Products of one sign, where every step of the matrix units that cuts its sum off makes it smaller.  A chain of the first product has at most 32 steps, whose sums grow evenly:
+    cuts of 2^-22 of the sum so far (2^-23, twice that for the sums inside a step) are 33 / 2 of them at most.  Then up to 16 sums of a block and 8 blocks are added, each
+    rounded (2^-24).  Second product: rank / 16 steps over v's first parts (the sums over the others are below 2^-7 of it), then one rounding."""
+    from vox_serve_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(K + rank + T)
+    rnd = lambda *s: torch.rand(*s, generator=g, device="cuda")                       # noqa: E731
+    bank = ops.LoraBank(2, K, (64,), rank)
+    a, b = (rnd(1, rank, K) / K).to(BF16), rnd(64, rank).to(BF16)
+    bank.load(1, a, b, 0.75)
+    x = rnd(T, K).to(BF16)
+    ids = torch.ones(T, dtype=I32, device="cuda")
+    ids[T // 2] = -1
+    got = ops.lora(x, bank, ops.lora_plan(ops.LoraPlan(T, 2), ids))
+    want = 0.75 * (x.double() @ a[0].double().t()) @ b.double().t()
+    want[T // 2] = 0.0
+    bound = 33 / 2 * 2.0 ** -22 + 24 * 2.0 ** -24 + (rank // 16 + 1) / 2 * 1.02 * 2.0 ** -22 + 4 * 2.0 ** -24
+    assert bool(((got.double() - want).abs() <= bound * want).all()), float(((got.double() - want).abs() / want.clamp(min=1e-30)).max() / bound)

@@ -184,16 +184,17 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 // warps (some 16 clocks an instruction of 512 bytes: that rate bounded a form with copies alone, at 38 us for 4096 rows of 8192 at rank 64 and the second
 // product; mma.sync from such copies was bound by its shared-memory reads: 36 us, 69 at rank 128; this form takes 34 and 48).  A fifth warp multiplies.  Rows behind
 // the last are whatever stands there, in lanes that nobody reads.  Stages go to ACCS sums in turn: the tensor cores cut a sum off at every step, and chains of a
-// quarter lose a quarter.  More than RT rank tiles: further blocks with x again.  The pieces of K are a cluster, which adds them up and leaves v in parts.
+// quarter lose a quarter (lora_long: when they are more than four or two).  More than RT rank tiles: further blocks with x again.  The pieces of K are a cluster, which adds them
+// up and leaves v in parts.
 constexpr int LORA_STAGE_K = 64, LORA_X_BYTES = LORA_DOWN_ROWS * 128, LORA_DOWN_THREADS = 160, LORA_LOADERS = 128, LORA_BOX_ROWS = 64;
 template <int RT>
 struct LoraDown {
-  static constexpr int N = RT * 16, ACCS = RT == 8 ? 2 : 4, COLS = RT == 8 ? 256 : ACCS * N < 32 ? 32 : ACCS * N, STAGES = RT == 8 ? 3 : RT == 4 ? 4 : 5;
+  static constexpr int N = RT * 16, ACCS = RT == 8 ? 2 : 4, MOST_ACCS = 256 / N, STAGES = RT == 8 ? 3 : RT == 4 ? 4 : 5;      // (256 columns of tensor memory a block: two run on an SM)
   static constexpr int STAGE_BYTES = LORA_X_BYTES + RT * 2048, LD = N + 4;
   static constexpr size_t SMEM = 1024 + static_cast<size_t>(STAGES) * STAGE_BYTES + 256;       // (1 KB to align; barriers)
   static_assert(LORA_DOWN_ROWS * LD * 4 <= STAGES * STAGE_BYTES, "the sums stand where the stages stood");
 };
-template <int RT>
+template <int RT, int ACCS>
 __global__ void __launch_bounds__(LORA_DOWN_THREADS, 2) lora_down_kernel(const LoraParams p, const __grid_constant__ CUtensorMap x_map) {
   extern __shared__ __align__(128) uint8_t smem8[];
   using D = LoraDown<RT>;
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(LORA_DOWN_THREADS, 2) lora_down_kernel(const L
   const int n = gr.z, rts = p.VR >> 4;
   const bool boxes = gr.w >= 0;
   if (warp == 4) {
-    tmem_alloc(tmem_at, D::COLS);
+    tmem_alloc(tmem_at, ACCS * D::N);
     tmem_relinquish();
   }
   // (the blocks of a group take stages in turn, so that at any time they read neighbouring pieces of the rows)
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(LORA_DOWN_THREADS, 2) lora_down_kernel(const L
       const uint64_t x_desc = umma_desc_sw128_kmajor(ring + slot * D::STAGE_BYTES), a_desc = umma_desc_sw128_kmajor(ring + slot * D::STAGE_BYTES + LORA_X_BYTES);
       if (elect_one()) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) umma_bf16(tmem + i % D::ACCS * D::N, x_desc + 2 * k, a_desc + 2 * k, idesc, i >= D::ACCS || k > 0);
+        for (int k = 0; k < 4; ++k) umma_bf16(tmem + i % ACCS * D::N, x_desc + 2 * k, a_desc + 2 * k, idesc, i >= ACCS || k > 0);
         umma_commit(empty + slot);
         if (i + 1 == turns) umma_commit(done);
       }
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(LORA_DOWN_THREADS, 2) lora_down_kernel(const L
     for (int c0 = 0; c0 < here * 16; c0 += 16) {
       float s[16];
 #pragma unroll
-      for (int q = 0; q < D::ACCS; ++q) {
+      for (int q = 0; q < ACCS; ++q) {
         if (q > 0 && q >= turns) break;
         uint32_t v[16];
         tmem_ld_32x16(tmem + (static_cast<uint32_t>(warp * 32) << 16) + q * D::N + c0, v);
@@ -360,7 +361,7 @@ __global__ void __launch_bounds__(LORA_DOWN_THREADS, 2) lora_down_kernel(const L
     const unsigned long long t0 = gtimer();
     while (gtimer() - t0 < 2000000ull) __nanosleep(1000);
   }
-  if (warp == 4) tmem_dealloc(tmem, D::COLS);
+  if (warp == 4) tmem_dealloc(tmem, ACCS * D::N);
 }
 
 // ---- second product ---------------------------------------------------------------------------------------------------------------
@@ -789,6 +790,12 @@ static int lora_tiles(int T, int slots) {
   const int adapters = T < slots + 1 ? T : slots + 1;
   return T <= 64 ? adapters : (T + 63) / 64 + adapters / 2;
 }
+// Results in fp32: a sum takes at most eight stages, since the tensor cores cut it off at every step.  A cluster of eight with 256 columns of sums a block reaches
+// rank tiles of a block x K = 65536, to which lora_launch brings the rank tiles; beyond K = 65536 the chains grow.  (Products of one sign at rank 128, off by, of the
+// result: K = 14336 3.1e-6 with the usual sums, 2.1e-6 so; K = 65536 1.6e-5 and 2.2e-6.)
+constexpr int LORA_CHAIN = 8, LORA_CHAIN_K = LORA_STAGE_K * LORA_CHAIN * 8 * 16;
+template <int RT>
+static bool lora_long(const LoraParams& p) { return p.f32 && (p.K + LORA_STAGE_K - 1) / LORA_STAGE_K > 8 * LORA_CHAIN * LoraDown<RT>::ACCS; }
 template <int RT>
 static int lora_k_split(const LoraParams& p, int slots) {
   const int stages = (p.K + LORA_STAGE_K - 1) / LORA_STAGE_K, adapters = p.T < slots + 1 ? p.T : slots + 1;
@@ -800,14 +807,15 @@ static int lora_k_split(const LoraParams& p, int slots) {
   while (split > 1 && groups * passes > rm_clusters<like>(split, LORA_UP_THREADS, LoraDown<RT>::SMEM)) --split;
   const int most = stages > 4 ? stages / 4 : 1;          // four stages a block
   if (split > most) split = most;
-  // (results in fp32: sums of at most eight stages, since the tensor cores cut a sum off at every step)
-  const int longest = 8 * LoraDown<RT>::ACCS, least = (stages + longest - 1) / longest;
+  const int longest = LORA_CHAIN * (lora_long<RT>(p) ? LoraDown<RT>::MOST_ACCS : LoraDown<RT>::ACCS), least = (stages + longest - 1) / longest;
   if (p.f32 && split < least) split = least < 8 ? least : 8;
   return split;
 }
+// (its warps' chains: 32 steps of the matrix units, as many as eight stages have)
+constexpr int LORA_FEW_K = 32768;
 // One launch for a step of at most 64 rows, where an adapter is what eight SMs take in good time.  (Rank 64, one launch / two: 1 MB 5.7 / 7.5 us for a row, 8.6 / 11.1 for 64 rows
 // of 12 adapters; 3 MB 12.4 / 11.7 and 18.1 / 22.5; 4 MB 15.5 / 13.9 and 23.4 / 27.7.)
-static bool lora_few(const LoraParams& p) { return p.T <= 64 && p.VR <= LORA_FEW_RANKS && p.rank_tiles <= 4 && (p.a_slot + p.b_slot) * 16 <= 3 << 20; }
+static bool lora_few(const LoraParams& p) { return p.T <= 64 && p.VR <= LORA_FEW_RANKS && p.rank_tiles <= 4 && (p.a_slot + p.b_slot) * 16 <= 3 << 20 && p.K <= LORA_FEW_K; }
 
 template <int KS, int OUT, bool TALL>
 static int lora_up_tiles(LoraParams& p, int max_tiles, int tiles, void* stream) {
@@ -838,16 +846,22 @@ template <int KS, int OUT>
 static int lora_up_launch(LoraParams& p, int max_tiles, int tiles, void* stream) {
   return p.tile_rows == 16 ? lora_up_tiles<KS, OUT, false>(p, max_tiles, tiles, stream) : lora_up_tiles<KS, OUT, true>(p, max_tiles, tiles, stream);
 }
-template <int RT>
-static int lora_down_launch(LoraParams& p, int slots, void* stream) {
-  VB_CHECK_CUDA((rm_smem<lora_down_kernel<RT>>()));
+template <int RT, int ACCS>
+static int lora_down_sums(LoraParams& p, int slots, void* stream) {
+  VB_CHECK_CUDA((rm_smem<lora_down_kernel<RT, ACCS>>()));
   p.k_split = lora_k_split<RT>(p, slots);
   CUtensorMap x_map;
   const int rc = vb_tensor_map_2d_bf16(&x_map, p.x, p.T, p.K, p.ldx, LORA_BOX_ROWS);
   if (rc) return rc;
-  VB_CHECK_CUDA(launch_kernel_cluster3(lora_down_kernel<RT>, dim3(p.k_split, lora_max_groups(p.T, slots), (p.VR / 16 + RT - 1) / RT), dim3(LORA_DOWN_THREADS), LoraDown<RT>::SMEM, static_cast<cudaStream_t>(stream), true,
-                                       dim3(p.k_split, 1, 1), p, x_map));
+  VB_CHECK_CUDA(launch_kernel_cluster3(lora_down_kernel<RT, ACCS>, dim3(p.k_split, lora_max_groups(p.T, slots), (p.VR / 16 + RT - 1) / RT), dim3(LORA_DOWN_THREADS), LoraDown<RT>::SMEM,
+                                       static_cast<cudaStream_t>(stream), true, dim3(p.k_split, 1, 1), p, x_map));
   return 0;
+}
+template <int RT>
+static int lora_down_launch(LoraParams& p, int slots, void* stream) {
+  if constexpr (LoraDown<RT>::MOST_ACCS > LoraDown<RT>::ACCS)
+    if (lora_long<RT>(p)) return lora_down_sums<RT, LoraDown<RT>::MOST_ACCS>(p, slots, stream);
+  return lora_down_sums<RT, LoraDown<RT>::ACCS>(p, slots, stream);
 }
 template <int KS, int OUT, int RT>
 static int lora_few_tiles(const LoraParams& p, int tiles, void* stream) {
@@ -878,10 +892,12 @@ static int lora_launch(LoraParams& p, int slots, void* stream) {
     return lora_few_launch<4, OUT>(p, max_tiles, stream);
   }
   VB_CHECK_ARG(p.wait_flag = wait_flag(WK_LORA), "vb_lora: no mapped host memory");
-  const int rc = p.VR <= 16   ? lora_down_launch<1>(p, slots, stream)
-                 : p.VR <= 32 ? lora_down_launch<2>(p, slots, stream)
-                 : p.VR <= 64 ? lora_down_launch<4>(p, slots, stream)
-                              : lora_down_launch<8>(p, slots, stream);
+  int rt = p.VR <= 16 ? 1 : p.VR <= 32 ? 2 : p.VR <= 64 ? 4 : 8;
+  while (p.f32 && rt > 1 && static_cast<long long>(p.K) * rt > LORA_CHAIN_K) rt /= 2;
+  const int rc = rt == 1   ? lora_down_launch<1>(p, slots, stream)
+                 : rt == 2 ? lora_down_launch<2>(p, slots, stream)
+                 : rt == 4 ? lora_down_launch<4>(p, slots, stream)
+                           : lora_down_launch<8>(p, slots, stream);
   if (rc) return rc;
   switch (p.rank_tiles) {
     case 1: return lora_up_launch<1, OUT>(p, max_tiles, lora_tiles(p.T, slots), stream);
