@@ -76,3 +76,113 @@ def test_long_sums_of_fp32_results(T, K, rank):
     want[T // 2] = 0.0
     bound = 33 / 2 * 2.0 ** -22 + 24 * 2.0 ** -24 + (rank // 16 + 1) / 2 * 1.02 * 2.0 ** -22 + 4 * 2.0 ** -24
     assert bool(((got.double() - want).abs() <= bound * want).all()), float(((got.double() - want).abs() / want.clamp(min=1e-30)).max() / bound)
+
+
+def _delta64(x, a, b, scale, widths, ids, v_off):
+    """(value, bound of its error) of B (scale A x) in 64 bits.  fp32 chains: K / 16 steps of the first product and 40 sums of warps and blocks, 3 rank / 16 + 4 of the second,
+    2^-22 of the absolute sum a step (a step may cut off, 2^-23, twice that for the sums inside it); v_off: what v loses in between."""
+    T, K = x.shape
+    val = torch.zeros(T, sum(widths), dtype=F64, device="cuda")
+    err = torch.zeros_like(val)
+    for s in set(ids.tolist()):
+        if not 0 <= s < len(a):
+            continue
+        rows = ids == s
+        xs, n0 = x[rows].double(), 0
+        d1, d2 = (K / 16 + 40) * 2.0 ** -22, (3 * a[s].shape[1] / 16 + 4) * 2.0 ** -22 + v_off
+        out, bad = [], []
+        for i, w in enumerate(widths):
+            A, B = a[s][i].double(), b[s][n0:n0 + w].double()
+            v, av = xs @ A.t() * scale[s], xs.abs() @ A.abs().t() * scale[s]
+            out.append(v @ B.t())
+            bad.append((d1 * av + d2 * v.abs()) @ B.abs().t())
+            n0 += w
+        val[rows], err[rows] = torch.cat(out, 1), torch.cat(bad, 1)
+    return val, err
+
+
+def _order(T, slots, order):
+    if order == "runs":                                   # long runs, the last adapter's rows before those without one
+        ids = [min(slots - 1, t * (slots + 1) // T) for t in range(T - min(3, T // 4))] + [-1] * min(3, T // 4)
+    elif order == "turns":
+        ids = [t % (slots + 1) - 1 for t in range(T)]
+    else:                                                 # a run, then turns
+        ids = [0] * (T // 2) + [t % (slots + 1) - 1 for t in range(T - T // 2)]
+    return torch.tensor(ids, dtype=I32, device="cuda")
+
+
+# T, K, widths, rank, slots: two launches each, by more than 128 columns of v, ranks beyond 64 or adapters beyond 3 MB
+TWO = [(40, 264, (40, 72, 24), 64, 1), (64, 520, (136, 8, 40), 64, 2), (64, 40, (104,), 128, 3), (40, 8, (64,), 128, 1), (17, 72, (40, 200), 128, 2), (2, 264, (64, 64), 100, 1),
+       (64, 8, (264,), 65, 1), (33, 12296, (320,), 128, 2), (64, 24584, (328,), 64, 3)]
+
+
+def _case(T, K, widths, rank, slots, order):
+    from vox_serve_b200 import ops
+    g = torch.Generator(device="cuda").manual_seed(13 * T + K + rank)
+    rnd = lambda *s: torch.randn(*s, generator=g, device="cuda")                      # noqa: E731
+    bank = ops.LoraBank(slots, K, widths, rank)
+    a, b = [(rnd(len(widths), rank, K) / K ** 0.5).to(BF16) for _ in range(slots)], [rnd(sum(widths), rank).to(BF16) for _ in range(slots)]
+    scale = [0.5 + 0.375 * s for s in range(slots)]
+    for s in range(slots):
+        bank.load(s, a[s], b[s], scale[s])
+    ids = _order(T, slots, order)
+    return bank, a, b, scale, ids, rnd(T, K).to(BF16), ops.lora_plan(ops.LoraPlan(T, slots), ids), rnd
+
+
+@pytest.mark.parametrize("order", ["runs", "turns", "both"])
+@pytest.mark.parametrize("case", TWO, ids=lambda c: "-".join(map(str, c)).replace(" ", ""))
+@pytest.mark.parametrize("kind", ["plane", "plane_base", "rows", "rows_base"])
+def test_two_launches_of_few_rows_against_64_bits(case, kind, order):
+    """adapters of up to 64 rows, so of several tiles of 16, whose v the first launch leaves tile by tile"""
+    from vox_serve_b200 import ops
+    T, K, widths, rank, slots = case
+    bank, a, b, scale, ids, x, plan, rnd = _case(*case, order)
+    N, f32 = sum(widths), kind.startswith("plane")
+    base = rnd(T, N).to(F32 if f32 else BF16) if kind.endswith("base") else None
+    out = torch.full((T, N), float("nan"), dtype=F32 if f32 else BF16, device="cuda")
+    before = ops.launch_count()
+    got = ops.lora(x, bank, plan, out=out, base=base)
+    assert ops.launch_count() - before == 2
+    want, err = _delta64(x, a, b, scale, widths, ids, 0.0)
+    if base is not None:
+        want = want + base.double()
+    tol = err + want.abs() * (2.0 ** -23 if f32 else 2.0 ** -8) + 1e-30
+    assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("order", ["runs", "turns", "both"])
+@pytest.mark.parametrize("T,K,ff,rank,slots,half,splits", [(40, 264, 88, 128, 1, 16, 2), (64, 520, 264, 65, 2, 48, 1), (64, 40, 1000, 128, 3, 64, 1), (17, 8, 72, 128, 2, 32, 3)])
+def test_two_launches_of_few_rows_gate_up(T, K, ff, rank, slots, half, splits, order):
+    from vox_serve_b200 import ops
+    bank, a, b, scale, ids, x, plan, rnd = _case(T, K, (ff, ff), rank, slots, order)
+    tiles = (ff + half - 1) // half
+    planes = rnd(splits, T, 2 * tiles * half)
+    before = ops.launch_count()
+    got = ops.lora_gate_up(x, bank, plan, planes, half)
+    assert ops.launch_count() - before == 2
+    d, err = _delta64(x, a, b, scale, (ff, ff), ids, 0.0)
+    p = planes.double().view(splits, T, tiles, half // 16, 2, 16)
+    split = lambda v: (v[:, :, :, 0].reshape(T, -1)[:, :ff], v[:, :, :, 1].reshape(T, -1)[:, :ff])   # noqa: E731
+    (pg, pu), (ag, au) = split(p.sum(0)), split(p.abs().sum(0))
+    gate, up = pg + d[:, :ff], pu + d[:, ff:]
+    eg = err[:, :ff] + (splits + 1) * 2.0 ** -23 * (ag + d[:, :ff].abs())
+    eu = err[:, ff:] + (splits + 1) * 2.0 ** -23 * (au + d[:, ff:].abs())
+    silu = gate * torch.sigmoid(gate)
+    want = silu * up
+    # |silu'| < 1.1; the exponential of an argument that is rounded, 1.5 |g| 2^-24, itself, the reciprocal and two products: below 2^-20
+    tol = 1.1 * eg * (up.abs() + eu) + silu.abs() * eu + want.abs() * (2.0 ** -8 + 2.0 ** -20 + gate.abs() * 2.0 ** -23) + 1e-30
+    assert bool(((got.double() - want).abs() <= tol).all()), float(((got.double() - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("K", [8, 40])
+@pytest.mark.parametrize("order", ["runs", "turns", "both"])
+def test_inputs_narrower_than_a_box(K, order):
+    """large steps of fewer inputs than a box of x has columns; x as columns of a wider matrix whose others are NaN"""
+    from vox_serve_b200 import ops
+    T, widths, rank, slots = 200, (72, 40), 24, 2
+    bank, a, b, scale, ids, x, plan, rnd = _case(T, K, widths, rank, slots, order)
+    wide = torch.full((T + 70, K + 72), float("nan"), dtype=BF16, device="cuda")
+    wide[:T, 8:8 + K] = x
+    got = ops.lora(wide[:T, 8:8 + K], bank, plan)
+    want, err = _delta64(x, a, b, scale, widths, ids, 0.0)
+    assert bool(((got.double() - want).abs() <= err + want.abs() * 2.0 ** -23 + 1e-30).all())
