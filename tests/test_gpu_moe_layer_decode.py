@@ -60,3 +60,28 @@ def test_captured_decode_steps_are_the_eager_ones(name, monkeypatch):
         per = [mats(f"e{e}") for e in range(f.experts)]
         ex = [None if per[0][m] is None else torch.stack([p[m] for p in per]) for m in range(3)]
         L._check(torch.cat(out), torch.cat(h), ex, mats("shared") if f.shared_ff else None, router, None if ids[0] is None else torch.cat(ids), f.act)
+
+
+@pytest.mark.parametrize("E,T", [(8, 1), (64, 9), (300, 17)])
+def test_router_written_by_the_kernel_in_front(E, T):
+    """the router's matrix and bias are changed in place right before a call: the call reads what was written"""
+    from vox_serve_b200 import ops
+    h, ex, sh, router, w, _ = L._layer(T, 512, 64, E, 2, 0, "silu_glu", "softmax", 0, 0, seed=E)
+    rnd = L._rnd(E + 1)
+    kept = [(rnd(E, 512, std=0.07), rnd(E, std=0.2)) for _ in range(4)]
+    want = []
+    for weight, bias in kept:
+        torch.cuda.synchronize()
+        want.append(ops.moe_layer(h, w, ops.MoeRouter("softmax", 2, weight=weight, bias=bias)))
+    assert not torch.equal(want[0], want[1])
+    got = []
+    for turn in range(50):
+        weight, bias = kept[turn % 4]
+        router.bias.copy_(bias)
+        router.weight.copy_(weight)
+        got.append(ops.moe_layer(h, w, router))
+        router.weight.copy_(weight)
+        router.bias.copy_(bias)
+        got.append(ops.moe_layer(h, w, router))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want[i // 2 % 4]) for i, g in enumerate(got))

@@ -83,8 +83,7 @@ __device__ __forceinline__ float ml_dot8(const uint4& x, const float* w) {
   return fmaf(bf16_hi(x.w), b.w, s);
 }
 // First the logits of the cluster's eight rows: a block's share of the experts, 16 at a time, by the rows of h on the matrix units, the fp32 matrix as three
-// bf16 parts (exact), the k blocks of 32 divided by the warps.  What a warp needs of the matrix is asked for before the rows of h are there (it is older than
-// the kernel in front).  Every logit goes into the shared memory of the block that its row belongs to.  Then each block picks one row's experts: an
+// bf16 parts (exact), the k blocks of 32 divided by the warps.  What a warp needs of the matrix first is on its way to L2 before the rows of h are there.  Every logit goes into the shared memory of the block that its row belongs to.  Then each block picks one row's experts: an
 // expert's place is the number of those in front of it, which all threads count at once.
 __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const MoeRouteParams p) {
   extern __shared__ __align__(128) int smem[];
@@ -113,10 +112,18 @@ __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const
       w[u][h][1] = in ? __ldg(reinterpret_cast<const float4*>(r + 4)) : make_float4(0.f, 0.f, 0.f, 0.f);
     }
   };
+  // (into L2, not into registers: the kernel in front may be the one that writes the matrix)
 #pragma unroll
-  for (int u = 0; u < AHEAD; ++u) take(u, 0, warp + u * WARPS);
-  const float my_bias = p.bias && tid < E ? __ldg(p.bias + tid) : 0.f;
+  for (int u = 0; u < AHEAD; ++u) {
+    const int k = (warp + u * WARPS) * 32 + t4 * 8;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int e = (g + h * 8) * ML_ROUTE_CLUSTER + rank;
+      if (e < E && k < p.W) asm volatile("prefetch.global.L2 [%0];" ::"l"(p.w + static_cast<long long>(e) * p.W + k));
+    }
+  }
   pdl_sync();
+  const float my_bias = p.bias && tid < E ? __ldg(p.bias + tid) : 0.f;
   const __nv_bfloat16* hr = p.h + (t0 + min(g, rows - 1)) * p.ldh;
   if (p.wsg && has) {                                             // the shared expert's gate
     const __nv_bfloat16* hs = p.h + t * p.ldh;
@@ -136,7 +143,7 @@ __global__ void __launch_bounds__(ML_ROUTE_THREADS) moe_layer_route_kernel(const
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         const int kb = kb0 + u * WARPS, k = kb * 32 + t4 * 8;
-        if (i0 > 0 || kb0 != warp) take(u, i0, kb);
+        take(u, i0, kb);
         x[u] = k < p.W ? *reinterpret_cast<const uint4*>(hr + k) : make_uint4(0u, 0u, 0u, 0u);
       }
 #pragma unroll
