@@ -496,8 +496,8 @@ int vb_gemm_bf16_grouped_glu(void* d_y, const void* d_w_tiles, const void* x_map
  * vb_gemm_wide_timeouts: whether a wait of that kernel has run out since its flag was last cleared (0 unless something is wrong;
  * synchronises the device).
  * vb_wait_flags: eight bytes of host memory, one flag per kind of kernel whose waits give up after two seconds -- 0 prompt projections, 1
- * vocoder convolutions, 2 prompt attention, 3 window attention of prompts, 4 vb_wait_check.  A kernel whose wait ran out sets its
- * flag and leaves its output incomplete: look at them after synchronising, before results are used, and clear them (NULL: no device).
+ * vocoder convolutions, 2 prompt attention, 3 window attention of prompts, 4 vb_wait_check, 5 experts of a decode step, 6 adapters of a step.  A kernel whose
+ * wait ran out sets its flag and leaves its output incomplete (7 without a wait: adapters, a plan of other rows or slots than the call's): look at them after synchronising, before results are used, and clear them (NULL: no device).
  * vb_wait_check: one kernel that waits on a barrier at most limit_us from the moment a second warp opens it, pause_us after the start (both warps
  * then agree on whether it ran out: the flag is 3);
  * that warp then completes the barrier, or with complete = 0 does not (flag 4). */
@@ -896,7 +896,7 @@ int vb_selective_scan_tiled(void* d_out, int ld_out, float* d_state, float* d_sc
  * VbLoraBank (HOST struct): the adapters in the order that csrc/lora.cu states (ops.LoraBank writes it).  slots 1 .. 1023, rank padded to 16, 32, 64 or
  *   128, K and the widths of the 1 .. 4 slices multiples of 8 (at most 2^24); d_a and d_b 16-byte aligned.
  * vb_lora_plan: rows of a step by adapter, once per step for every projection of every layer: d_tiles, vb_lora_plan_bytes(T, slots) bytes, 16-byte
- *   aligned.
+ *   aligned.  A call of another T or of a bank of other slots (a captured one, say) writes nothing and sets flag 7 of vb_wait_flags.
  * vb_lora: out and base fp32 (out_f32) or bf16, rows 16-byte aligned; d_base may be NULL (zeros) or d_out.  Every row 0 .. T-1 of out is written, nothing
  *   behind it.  vb_lora_workspace_bytes may be 0 (d_ws may be NULL then).
  * vb_lora_gate_up: act[t][i] = silu(g) u (bf16, row-major with ld_act or, xt_rows > 0, tiled) from d_planes fp32 [splits][T][2 * tiles * half], gate and

@@ -186,3 +186,54 @@ def test_inputs_narrower_than_a_box(K, order):
     got = ops.lora(wide[:T, 8:8 + K], bank, plan)
     want, err = _delta64(x, a, b, scale, widths, ids, 0.0)
     assert bool(((got.double() - want).abs() <= err + want.abs() * 2.0 ** -23 + 1e-30).all())
+
+
+@pytest.mark.parametrize("T,rank,others", [(16, 16, (17, 40, 15, 200)), (16, 128, (17, 130, 9)), (130, 16, (129, 16, 300)), (130, 128, (64, 131))])
+def test_captured_steps_behind_another_step_s_plan(T, rank, others):
+    """A captured plane and gate | up, then the plan is made for a step of other rows: the replay writes nothing and the host learns of it; behind a plan of its own rows it
+    is as before.  So is a plan that was never made, and one of other slots."""
+    from vox_serve_b200 import ops
+    slots, K, ff = 4, 136, 72
+    bank, a, b, scale, ids, x, plan, rnd = _case(T, K, (ff, ff), rank, slots, "turns")
+    room = ops.LoraPlan(300, slots)
+    planes = rnd(1, T, 2 * 2 * 48)
+    outs = torch.zeros(T, 2 * ff, device="cuda"), torch.zeros(T, ff, dtype=BF16, device="cuda")
+    ops.check_waits()
+
+    def step():
+        ops.lora(x, bank, room, out=outs[0])
+        ops.lora_gate_up(x, bank, room, planes, 48, out=outs[1])
+    ops.lora_plan(room, ids)
+    step()
+    want = [o.clone() for o in outs]
+    g = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        step()
+
+    def replay(whole):
+        for o in outs:
+            o.fill_(7.0)
+        g.replay()
+        torch.cuda.synchronize()
+        if whole:
+            ops.check_waits()
+            assert all(torch.equal(o, w) for o, w in zip(outs, want))
+        else:
+            with pytest.raises(ops.VoxB200Error, match="a plan of adapters"):
+                ops.check_waits()
+            assert all(bool((o == 7.0).all()) for o in outs)
+    replay(True)
+    for n in others:
+        ops.lora_plan(room, _order(n, slots, "both"))
+        replay(False)
+        ops.lora_plan(room, ids)
+        replay(True)
+    room.tiles.zero_()
+    replay(False)
+    few = ops.LoraPlan(T, slots - 1)
+    ops.lora_plan(few, ids.clamp(max=slots - 2))
+    room.tiles[:few.tiles.numel()].copy_(few.tiles)
+    replay(False)
+    ops.lora_plan(room, ids)
+    replay(True)

@@ -245,9 +245,11 @@ class MoeRouterStruct(C.Structure):
 
 _lock = threading.Lock()
 _lib = None
-# flags in mapped host memory, one byte per kind of kernel whose waits give up (csrc/common.cuh, BoundedWait)
+# flags in mapped host memory, one byte per kind of kernel whose waits give up (csrc/common.cuh, BoundedWait); the last one: a kernel that met a table of
+# another step's (csrc/lora.cu)
 _wait_flags = None
-WAIT_KINDS = ("a projection of a prompt step", "a vocoder convolution", "prompt attention", "window attention of a prompt", "vb_wait_check", "experts of a decode step", "adapters of a prompt step")
+WAIT_KINDS = ("a projection of a prompt step", "a vocoder convolution", "prompt attention", "window attention of a prompt", "vb_wait_check", "experts of a decode step", "adapters of a step",
+              "a plan of adapters")
 
 
 class VoxB200Error(RuntimeError):
@@ -316,7 +318,12 @@ def check_waits():
     if bits:
         _wait_flags.value = 0
         kinds = [name for i, name in enumerate(WAIT_KINDS) if bits >> (8 * i) & 0xff] or ["a kernel"]
-        raise VoxB200Error(f"a wait inside {' and '.join(kinds)} ran out: results since then are incomplete")
+        why = []
+        if kinds[-1] == WAIT_KINDS[-1]:
+            why.append(f"{kinds.pop()} of other rows or slots than the step's was read (a captured step behind another step's plan?)")
+        if kinds:
+            why.append(f"a wait inside {' and '.join(kinds)} ran out")
+        raise VoxB200Error(f"{'; '.join(why)}: results since then are incomplete")
 
 
 # kernels (+ memset nodes) each entry point enqueues; everything not listed launches exactly one

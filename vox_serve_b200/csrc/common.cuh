@@ -307,7 +307,7 @@ __device__ __forceinline__ void mbar_wait(uint64_t* bar, uint32_t parity) {
 // every later wait of the thread returns at once, so that the block can stop issuing, let its copies land and leave with the
 // context usable.  `gate`: shared-memory word that the block sets once the kernels in front have completed (0: they have); the
 // clock starts there, or a predecessor's running time would count as the wait's own.
-enum WaitKind { WK_GEMM_WIDE = 0, WK_CL_CONV = 1, WK_PREFILL_ATTN = 2, WK_WINDOW_ATTN = 3, WK_CHECK = 4, WK_MOE_LAYER = 5, WK_LORA = 6, WK_KINDS = 8 };
+enum WaitKind { WK_GEMM_WIDE = 0, WK_CL_CONV = 1, WK_PREFILL_ATTN = 2, WK_WINDOW_ATTN = 3, WK_CHECK = 4, WK_MOE_LAYER = 5, WK_LORA = 6, WK_LORA_PLAN = 7, WK_KINDS = 8 };
 unsigned char* wait_flag(WaitKind kind);      // api.cu: its address on the device, nullptr if the flags could not be allocated
 int wait_ran_out(WaitKind kind);              // api.cu: after all work on the device
 struct BoundedWait {

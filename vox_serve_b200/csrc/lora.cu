@@ -30,10 +30,11 @@ constexpr int LORA_MAX_SLICES = 4;
 constexpr int LORA_MAX_ROWS = 1 << 21;     // (tiles are a launch's second dimension)
 constexpr int LORA_THREADS = 256;
 constexpr int LORA_DOWN_ROWS = 128;        // rows of a block of the first product
+constexpr int LORA_PLAN_HEAD = 4;          // words in front of the tiles
 constexpr int LORA_PLAN_SMEM = 32 * (LORA_MAX_SLOTS + 1) * 4;
 
 // ---- rows by adapter ------------------------------------------------------------------------------------------------------------
-// A record per tile: adapter or -1, first place among the sorted rows, rows (0: no tile), 0, then the rows.  Behind them a record per group, the up to 128 rows of an
+// Four words, rows and slots of the step in the first two (a call of another step does not read on), then a record per tile: adapter or -1, first place among the sorted rows, rows (0: no tile), 0, then the rows.  Behind them a record per group, the up to 128 rows of an
 // adapter (neighbouring tiles) that a block of the first product takes: first tile (-1: no group), adapter, rows, the first row if they follow one another in x,
 // else -1.  One block: a counting sort in shared memory
 // that keeps an adapter's rows in their order (rows that follow one another in x are then fetched as boxes): a warp a piece of the rows, its counts per adapter [32 warps]
@@ -46,6 +47,7 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(int32_t* __restrict__ t
   pdl_sync();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, stride = 4 + tile_rows, counts = slots + 1;
   for (int i = tid; i < 32 * counts; i += 1024) cnt[i] = 0;
+  if (tid == 0) *reinterpret_cast<int4*>(tiles - LORA_PLAN_HEAD) = make_int4(T, slots, 0, 0);
   __syncthreads();
   const int per = (T + 1023) / 1024 * 32, end = min(T, (warp + 1) * per);
   int* mine = cnt + warp * counts;
@@ -119,7 +121,9 @@ __global__ void __launch_bounds__(1024) lora_plan_kernel(int32_t* __restrict__ t
 }
 
 struct LoraParams {
-  const int32_t* tiles;            // records of 4 + tile_rows words
+  const int32_t* tiles;            // records of 4 + tile_rows words; in front of them (LORA_PLAN_HEAD) the step's rows and slots
+  unsigned char* plan_flag;
+  int slots;
   const int4* groups;
   int tile_rows;
   const __nv_bfloat16* x;
@@ -143,6 +147,18 @@ struct LoraParams {
   const float* planes;
   int splits, width, ff, xt_rows, xt_kb;
 };
+
+// What a plan was made for.  A captured call may meet one of another step, whose records it would take for rows and adapters: it raises a flag that the host reads and
+// writes nothing.
+__device__ __forceinline__ int2 lora_plan_of(const LoraParams& p) { return *reinterpret_cast<const int2*>(p.tiles - LORA_PLAN_HEAD); }
+__device__ __forceinline__ bool lora_other_plan(const LoraParams& p, const int2& made) {
+  if (made.x == p.T && made.y == p.slots) return false;
+  if (threadIdx.x == 0) {
+    *reinterpret_cast<volatile unsigned char*>(p.plan_flag) = 1;
+    __threadfence_system();
+  }
+  return true;
+}
 
 // ---- v as the second product's A operand ------------------------------------------------------------------------------------------
 // In the order of the lanes: [m16 block][slice][part][rank tile][32 lanes][4 registers].
@@ -205,8 +221,9 @@ __global__ void __launch_bounds__(LORA_DOWN_THREADS, 2) lora_down_kernel(const L
   uint64_t *empty = full + STAGES, *done = empty + STAGES;
   uint32_t* tmem_at = reinterpret_cast<uint32_t*>(done + 1);
   pdl_sync();
+  const int2 made = lora_plan_of(p);
   const int4 gr = p.groups[blockIdx.y];
-  if (gr.x < 0) return;                     // (all blocks of the cluster)
+  if (lora_other_plan(p, made) || gr.x < 0) return;        // (all blocks of the cluster)
   const int n = gr.z, rts = p.VR >> 4;
   const bool boxes = gr.w >= 0;
   if (warp == 4) {
@@ -509,6 +526,7 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int32_t* rec = p.tiles + static_cast<long long>(blockIdx.y) * (4 + TILE);
   const int4 tl = *reinterpret_cast<const int4*>(rec);
+  const int2 made = lora_plan_of(p);
   // (ranges of one slice, of gate | up of both, in whole steps)
   int s = 0;
   if (OUT != LORA_GLU)
@@ -518,7 +536,7 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
   const int c0 = begin + static_cast<int>(static_cast<long long>(all) * part / parts) * STEP,
             c1 = begin + min(blocks, static_cast<int>(static_cast<long long>(all) * (part + 1) / parts) * STEP);
   const bool has = tl.x >= 0;
-  if (n == 0 || c0 >= c1) {
+  if (lora_other_plan(p, made) || n == 0 || c0 >= c1) {
     pdl_sync();
     return;
   }
@@ -651,11 +669,12 @@ __global__ void __launch_bounds__(LORA_THREADS) lora_few_kernel(const LoraParams
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
   const int rank = blockIdx.x % LORA_CLUSTER;
   pdl_sync();
+  const int2 made = lora_plan_of(p);
   const int32_t* rec = p.tiles + (blockIdx.x / LORA_CLUSTER) * (4 + 16);
   const int4 tl = *reinterpret_cast<const int4*>(rec);
   const int row_a = rec[4 + g], row_b = rec[12 + g]; // (places behind the tile's last hold anything)
   const int n = tl.z;
-  if (n == 0) return;                                // (all blocks of the cluster)
+  if (lora_other_plan(p, made) || n == 0) return;    // (all blocks of the cluster)
   const bool has = tl.x >= 0;
   const int c1 = static_cast<int>(static_cast<long long>(p.blocks) * (rank + 1) / LORA_CLUSTER), first = static_cast<int>(static_cast<long long>(p.blocks) * rank / LORA_CLUSTER) + warp;
   const uint4* b = p.b + (has ? tl.x : 0) * p.b_slot + lane;
@@ -947,7 +966,9 @@ static int lora_setup(const char* who, LoraParams& p, const void* d_x, long long
   VB_CHECK_ARG(reinterpret_cast<uintptr_t>(d_tiles) % 16 == 0, "%s: the plan must be 16-byte aligned", who);
   VB_CHECK_ARG(T <= LORA_MAX_ROWS, "%s: %d rows; at most %d", who, T, LORA_MAX_ROWS);
   VB_CHECK_ARG(ldx % 8 == 0 && ldx >= p.K && reinterpret_cast<uintptr_t>(d_x) % 16 == 0, "%s: rows of x must be 16-byte aligned (K %d, row stride %lld)", who, p.K, ldx);
-  p.tiles = static_cast<const int32_t*>(d_tiles);
+  VB_CHECK_ARG(p.plan_flag = wait_flag(WK_LORA_PLAN), "%s: no mapped host memory", who);
+  p.slots = bank->slots;
+  p.tiles = static_cast<const int32_t*>(d_tiles) + LORA_PLAN_HEAD;
   p.groups = reinterpret_cast<const int4*>(p.tiles + static_cast<long long>(lora_max_tiles(T, bank->slots)) * (4 + p.tile_rows));
   p.x = static_cast<const __nv_bfloat16*>(d_x);
   p.ldx = ldx;
@@ -965,7 +986,7 @@ using namespace vb;
 extern "C" {
 
 size_t vb_lora_plan_bytes(int T, int slots) {
-  return T < 1 || slots < 1 ? 0 : static_cast<size_t>(lora_max_tiles(T, slots)) * (4 + lora_tile_rows(T)) * 4 + static_cast<size_t>(lora_max_groups(T, slots)) * 16;
+  return T < 1 || slots < 1 ? 0 : LORA_PLAN_HEAD * 4 + static_cast<size_t>(lora_max_tiles(T, slots)) * (4 + lora_tile_rows(T)) * 4 + static_cast<size_t>(lora_max_groups(T, slots)) * 16;
 }
 
 int vb_lora_plan(void* d_tiles, const int32_t* d_ids, int T, int slots, void* stream) {
@@ -974,7 +995,7 @@ int vb_lora_plan(void* d_tiles, const int32_t* d_ids, int T, int slots, void* st
   VB_CHECK_ARG(slots >= 1 && slots <= LORA_MAX_SLOTS, "vb_lora_plan: %d adapters; 1 to %d", slots, LORA_MAX_SLOTS);
   VB_CHECK_ARG(T >= 1 && T <= LORA_MAX_ROWS, "vb_lora_plan: %d rows; 1 to %d", T, LORA_MAX_ROWS);
   VB_CHECK_CUDA((rm_smem<lora_plan_kernel>(LORA_PLAN_SMEM)));
-  VB_LAUNCH_PDL(lora_plan_kernel, 1, 1024, 32 * (slots + 1) * 4, stream, static_cast<int32_t*>(d_tiles), d_ids, T, slots, lora_tile_rows(T), lora_max_tiles(T, slots), lora_max_groups(T, slots));
+  VB_LAUNCH_PDL(lora_plan_kernel, 1, 1024, 32 * (slots + 1) * 4, stream, static_cast<int32_t*>(d_tiles) + LORA_PLAN_HEAD, d_ids, T, slots, lora_tile_rows(T), lora_max_tiles(T, slots), lora_max_groups(T, slots));
   return 0;
 }
 

@@ -1971,7 +1971,8 @@ class LoraBank:
 
 
 class LoraPlan:
-    """Rows of a step by adapter (``lora_plan``): made once per step, read by every projection of every layer."""
+    """Rows of a step by adapter (``lora_plan``): made once per step, read by every projection of every layer.  A captured step that is replayed behind another
+    step's ``lora_plan`` writes nothing if that had other rows; ``check_waits`` raises."""
 
     def __init__(self, max_rows: int, slots: int, device="cuda"):
         _refuse(not 1 <= max_rows <= 1 << 21 or not 1 <= slots <= 1023, f"LoraPlan: {max_rows} rows (1 to 2^21), {slots} adapters (1 to 1023)")
