@@ -38,7 +38,8 @@ constexpr int LORA_PLAN_SMEM = 32 * (LORA_MAX_SLOTS + 1) * 4;
 // adapter (neighbouring tiles) that a block of the first product takes: first tile (-1: no group), adapter, rows, the first row if they follow one another in x,
 // else -1.  One block: a counting sort in shared memory
 // that keeps an adapter's rows in their order (rows that follow one another in x are then fetched as boxes): a warp a piece of the rows, its counts per adapter [32 warps]
-// [slots + 1], which become the first places of the warps' rows.  Two passes over the ids and three meetings: 5 us for 32 rows, 9 for 4096, once a step.
+// [slots + 1], which become the first places of the warps' rows.  Two passes over the ids; then a thread writes an adapter's records.  Once a step, in a chain of
+// captured calls: 3.5 us for 32 rows, 5.9 for 4096 of six adapters, 9.3 for 4096 of one, 29 for 16384 and 155 for 65536 of one (its thread's records: 2 us per 1024 rows).
 __global__ void __launch_bounds__(1024) lora_plan_kernel(int32_t* __restrict__ tiles, const int32_t* __restrict__ ids, int T, int slots, int tile_rows, int max_tiles,
                                                          int max_groups) {
   extern __shared__ __align__(128) int cnt[];
@@ -832,8 +833,13 @@ static int lora_k_split(const LoraParams& p, int slots) {
 }
 // (its warps' chains: 32 steps of the matrix units, as many as eight stages have)
 constexpr int LORA_FEW_K = 32768;
-// One launch for a step of at most 64 rows, where an adapter is what eight SMs take in good time.  (Rank 64, one launch / two: 1 MB 5.7 / 7.5 us for a row, 8.6 / 11.1 for 64 rows
-// of 12 adapters; 3 MB 12.4 / 11.7 and 18.1 / 22.5; 4 MB 15.5 / 13.9 and 23.4 / 27.7.)
+// One launch for a step of at most 64 rows, where an adapter is what eight SMs take in good time.  How many adapters the step's rows have the host does not know (the ids are on
+// the device), so the rule sees an adapter's bytes alone; 3 MB is where both forms take the same for one row and for a dozen adapters.  K = N at rank 64, us in
+// one launch / two:  1 row        1 MB 5.6 / 7.6   2 MB 8.6 / 9.6     3 MB 11.7 / 11.8   4 MB 14.5 / 14.0   6 MB 20.2 / 18.5
+//                    64, of 1     1 MB 7.9 / 8.4   2 MB 11.4 / 10.8   3 MB 14.6 / 13.3   4 MB 17.8 / 15.8
+//                    64, of 12    1 MB 8.0 / 10.8  2 MB 14.5 / 15.7   3 MB 18.2 / 19.7   4 MB 23.9 / 23.7   6 MB 30.7 / 32.2
+//                    64, of 32    1 MB 10.5 / 14.9 2 MB 16.6 / 21.3   3 MB 21.9 / 27.6   4 MB 27.8 / 34.1
+// (2 MB and more of one adapter for all rows lose 5 to 10 % by it, more than 3 MB of many up to 18 %; rank 16 to 1.5 MB: one launch takes half to 0.9 of two.)
 static bool lora_few(const LoraParams& p) { return p.T <= 64 && p.VR <= LORA_FEW_RANKS && p.rank_tiles <= 4 && (p.a_slot + p.b_slot) * 16 <= 3 << 20 && p.K <= LORA_FEW_K; }
 
 template <int KS, int OUT, bool TALL>

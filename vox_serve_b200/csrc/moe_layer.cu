@@ -4,17 +4,21 @@
 //
 // Two launches behind the router's.  A stream of weights: 3 x ff x W values for every expert that any row chose, a few
 // rows each, so the kernels are built around loads that never pause.  Weights go from the packed tiles (vb_pack_weight_tiles; the same buffers that the
-// projections of larger steps multiply) straight into the registers of the warp that multiplies them, 16 bytes a lane; a lane takes whole 16-byte chunks
-// of 8 k, and since a product's k may stand in any order as long as both operands agree, the rows of h are taken by the same chunks.
+// projections of larger steps multiply) by bulk copies into a ring of each warp's own in shared memory, and from there, 16 bytes a lane, into the registers
+// that it multiplies; a lane takes whole 16-byte chunks of 8 k, and since a product's k may stand in any order as long as both operands agree, the rows of h are
+// taken by the same chunks.
+//
+// Units of work (32 rows of an expert's gate | up matrix, 64 k of its down matrix) stand in one line, the active experts one behind the other, each as long as its
+// columns make it; blocks and warps take equal parts of the line.  Which experts the step chose therefore decides where a row's sums are cut: its last bits depend on
+// the step's other rows (the same step gives the same bits).
 //
 //   route eight blocks of a cluster share the experts' logits of eight rows (the router's fp32 matrix is read once per eight rows), then a block each picks
 //         one row's experts from all of them
-//   up    block = (expert, 32 rows of its gate | up matrix: 16 gated or 32 plain columns), the eight warps divide k; sums meet in shared memory, the
+//   up    a block takes a part of the line; the eight warps divide the k of a unit (16 gated or 32 plain columns), their sums meet in shared memory, the
 //         activation times the routing weight leaves as three bf16 parts (exact, rowmma.cuh), so nothing is rounded between the two products
 //         (the matrix units cut a sum off instead of rounding it: they add up a k block of 64, ordinary additions the k blocks)
-//   down  block = 32 columns of the result x an equal share of the chosen experts' k blocks, every warp adding its products to rows of its own in
-//         shared memory; up to eight blocks of a cluster divide the k blocks and add up through distributed shared memory.  No atomics: products,
-//         warps and blocks are added in a fixed order
+//   down  block = 32 columns of the result; the warps of up to eight blocks of a cluster take a part of the line each, every warp adding its products to rows of
+//         its own in shared memory, and the blocks add up through distributed shared memory.  No atomics: products, warps and blocks are added in a fixed order
 //
 // What bounds it: HBM at 64 rows (8 of 128 experts of 2048 x 768: 1.2 GB in 191 us, 6.3 TB/s), below that starts (three of 2 to 3 us) and blocks that end in whole units (8 rows, 6 of
 // 64 experts of 2048 x 1024: 86 us for 440 MB; gate and up 5.6 TB/s, down 4.1; one row, 2 of 8 experts and the shared one of 1024 x 1024: 16 us for 19 MB).

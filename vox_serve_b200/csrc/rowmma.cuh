@@ -1,6 +1,6 @@
-// What the operators share whose weights a row brings with it (lora.cu, moe_layer.cu): weights as the streamed operand of mma.sync, taken from HBM
-// straight into registers, a few rows of activations as the other operand.  Few rows make these products a stream of weights, which mma.sync
-// keeps up with (an m16n8k16 product takes 2 clocks of an SM for 512 bytes of weights that arrive in 22).
+// What the operators share whose weights a row brings with it (lora.cu, moe_layer.cu): weights as the streamed operand of mma.sync (straight into registers in
+// adapters' steps of few rows, else through shared memory), a few rows of activations as the other operand.  Few rows make these products a stream of weights,
+// which mma.sync keeps up with (an m16n8k16 product takes 2 clocks of an SM for 512 bytes of weights that arrive in 22).
 #pragma once
 #include "common.cuh"
 

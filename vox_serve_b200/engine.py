@@ -348,7 +348,9 @@ class LlamaEngine:
         whose inputs are sums of several embeddings or projected features, csm.py:647-654).  ``head``: the packed
         output head to use instead of ``w.lm_head`` (per-position heads of a depth decoder).  ``want_hidden``: also
         return the final-normed rows [n_out or n_rows, hidden] bf16, row-major (the backbone state a depth decoder
-        starts from, csm.py:290-300).  ``adapters``: the plan of the rows' adapters (ops.lora_plan; ``set_adapters`` first)."""
+        starts from, csm.py:290-300).  ``adapters``: the plan of the rows' adapters (ops.lora_plan; ``set_adapters`` first).  Such a
+        step runs every row, those without an adapter too, on row-major activations and planes of gate | up: their results are
+        those of a step without adapters up to bf16 rounding, not to the bit."""
         d, w, R = self.dims, self.w, n_rows
         if adapters is not None:                   # (before anything is written)
             if self.adapters is None:

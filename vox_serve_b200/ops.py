@@ -2009,7 +2009,8 @@ def _lora_check(who: str, x: torch.Tensor, bank: LoraBank, plan: LoraPlan) -> No
 def lora(x: torch.Tensor, bank: LoraBank, plan: LoraPlan, out: Optional[torch.Tensor] = None, base: Optional[torch.Tensor] = None) -> torch.Tensor:
     """out[t] = base[t] + B_a (scale_a A_a x[t]) with the adapter a of row t in ``plan`` (none: base[t]).  x bf16 [T, K]; out fp32 [T, N] (one more split-K
     plane of the projection: ``gemm`` mode 1) or bf16 (rounded once), by ``out``, else by ``base``, else fp32.  ``base``: of out's type, may be out
-    itself; None: zeros.  K is divided by the number of rows and slots: the same rows in a step of another size agree to fp32 rounding, not to the bit."""
+    itself; None: zeros.  K is divided by the number of rows and slots: the same rows in a step of another size agree to fp32 rounding, not to the bit.  A row, or an
+    adapter, that is not finite makes its rows not finite (infinities may become NaN: ranks are padded with zeros) and no others."""
     _lora_check("lora", x, bank, plan)
     T, N = x.shape[0], bank.N
     f32, ld_out = True, N
@@ -2188,7 +2189,8 @@ def _moe_layer_check(h: torch.Tensor, weights: MoeWeights, router: MoeRouter, id
 def moe_layer(h: torch.Tensor, weights: MoeWeights, router: MoeRouter, ids: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """A whole mixture-of-experts layer for the rows of a decode step (at most MOE_LAYER_MAX_ROWS): router, the chosen experts, the shared expert, weighted
     sum.  h bf16 [T, width]; ids int32 [T] (token ids) for a table router; out fp32 [T, width].  The matrices of experts that no row chose are not read; nothing
-    is rounded between the two products."""
+    is rounded between the two products.  Sums are divided by the experts that the step chose: the same step gives the same bits, but the same row in
+    other company agrees to fp32 rounding, not to the bit."""
     T, W = h.shape[0], weights.width
     # (one comparison per fact when all goes together: every call passes here)
     if not (h.is_cuda and h.dtype is BF16 and h.dim() == 2 and h.shape[1] == W and T <= MOE_LAYER_MAX_ROWS and h.get_device() == weights._device == _device_index()
