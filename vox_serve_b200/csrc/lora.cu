@@ -656,7 +656,7 @@ __global__ void __launch_bounds__(LORA_UP_THREADS, 4) lora_up_kernel(const LoraP
 
 // ---- both, for few rows -------------------------------------------------------------------------------------------------------------
 // A cluster of eight blocks per tile of up to 16 rows.  RT: rank tiles, all of them in one pass over the block's share of K.  One chain: the tile's record, a round or two of
-// loads of x and A, the warps' and the cluster's meeting, the columns; each is latency.  32 rows with an adapter each, 2048 x 2048 at rank 16 (4.3 MB): 4.2 us a call in
+// loads of x and A, the warps' and the cluster's meeting, the columns; each is latency.  32 rows with an adapter each, 2048 x 2048 at rank 16 (4.3 MB): 4.5 us a call in
 // a chain; 64 rows with 12 adapters, 4096 to 4608 columns at rank 32 (14 MB): 8.1.  In two launches 8.3 and 11.7.
 constexpr int LORA_CLUSTER = 8, LORA_FEW_RANKS = 128, LORA_FEW_LD = 20;
 template <int KS, int OUT, int RT>
