@@ -71,3 +71,11 @@ def test_unaligned_experts(which):
     weights = _lib.MoeWeightsStruct(at + by["up"], at + by["down"], 64, 4, 64, 0, 128, 0, 0.0, 1.0)
     router = _lib.MoeRouterStruct(at, at + by["bias"], None, at + by["table"], 3 if which in ("ids", "table") else 0, 2, 0, 0, 16)
     _refused(lib.vb_moe_layer(at + by["y"], 64, at, 64, ctypes.addressof(weights), ctypes.addressof(router), at + by["ids"], 2, at, 1 << 15, None), "aligned")
+
+
+def test_experts_on_two_devices():
+    """a call compares its rows with one of them"""
+    up, down = _packed(2 * 4 * 64, 72, 128), _packed(72, 4 * 64, 128)
+    ops.MoeWeights(up, down, 4, 72, 64)
+    with pytest.raises(VoxB200Error, match="meta"):
+        ops.MoeWeights(up, ops.PackedWeight(torch.zeros(8, dtype=torch.uint8, device="meta"), 72, 4 * 64, 128), 4, 72, 64)

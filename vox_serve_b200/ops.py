@@ -2092,6 +2092,7 @@ class MoeWeights:
                 f"hold {experts} experts of {ff} and {shared_ff} shared columns")
         _refuse(up.tile_rows % 32 != 0 or rows * ff % up.tile_rows != 0 or rows * shared_ff % up.tile_rows != 0 or down.tile_rows != 128,
                 f"MoeWeights: tiles of {up.tile_rows} and {down.tile_rows} rows")
+        _refuse(up.data.device != down.data.device, f"MoeWeights: matrices on {up.data.device} and {down.data.device}")
         self.up, self.down, self.experts, self.width, self.ff, self.shared_ff = up, down, int(experts), int(width), int(ff), int(shared_ff)
         self.act, self.limit, self.slope = act, float(limit), float(slope)
         self._struct = _lib.MoeWeightsStruct(up.data.data_ptr(), down.data.data_ptr(), self.width, self.experts, self.ff, self.shared_ff, up.tile_rows, MOE_LAYER_ACTS[act],
