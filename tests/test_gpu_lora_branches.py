@@ -237,3 +237,33 @@ def test_captured_steps_behind_another_step_s_plan(T, rank, others):
     replay(False)
     ops.lora_plan(room, ids)
     replay(True)
+
+
+def test_the_most_rows_and_offsets_past_32_bits():
+    """2^21 rows, the most that a plan takes, into results whose last rows stand past 2^31 elements; sampled rows against 64 bits, and rows without an adapter are their base"""
+    from vox_serve_b200 import ops
+    T, K, N, slots = 2 ** 21, 8, 64, 3
+    g = torch.Generator(device="cuda").manual_seed(4)
+    bank = ops.LoraBank(slots, K, (N,), 16)
+    a, b = [], []
+    for s in range(slots):
+        a.append(torch.randn(1, 16, K, generator=g, device="cuda").to(BF16))
+        b.append(torch.randn(N, 16, generator=g, device="cuda").to(BF16))
+        bank.load(s, a[s], b[s], 0.5)
+    ids = torch.randint(-1, slots, (T,), generator=g, device="cuda").to(I32)
+    ids[:T // 2] = 1                                      # half of the rows in a run
+    x = torch.randn(T, K, generator=g, device="cuda").to(BF16)
+    plan = ops.lora_plan(ops.LoraPlan(T, slots), ids)
+    wide = torch.zeros(T, 1032, dtype=BF16, device="cuda")[:, 512:512 + N]
+    assert T * wide.stride(0) > 2 ** 31
+    wide.copy_(torch.randn(T, N, generator=g, device="cuda"))
+    at = torch.cat([torch.randint(0, T, (3000,), generator=g, device="cuda"), torch.arange(T - 200, T, device="cuda"), torch.arange(T // 2 - 70, T // 2 + 70, device="cuda")])
+    base = wide[at].double()
+    assert ops.lora(x, bank, plan, out=wide, base=wide) is wide
+    d, err = _delta64(x[at], a, b, [0.5] * slots, (N,), ids[at], 2.0 ** -17)
+    want = base + d
+    got = wide[at].double()
+    assert bool(((got - want).abs() <= err + want.abs() * 2.0 ** -8 + 1e-30).all())
+    assert bool((got[ids[at] < 0] == base[ids[at] < 0]).all())
+    with pytest.raises(ops.VoxB200Error):
+        ops.LoraPlan(T + 1, slots)
