@@ -267,3 +267,28 @@ def test_the_most_rows_and_offsets_past_32_bits():
     assert bool((got[ids[at] < 0] == base[ids[at] < 0]).all())
     with pytest.raises(ops.VoxB200Error):
         ops.LoraPlan(T + 1, slots)
+
+
+@pytest.mark.parametrize("rank", [16, 128])
+def test_beside_a_vocoder_on_another_stream(rank):
+    """Large steps of adapters while a vocoder decodes on another stream, as a serving step has them: kernels of both keep tensor memory and meet in clusters, and a block
+    gives its own back before it waits for another.  Both streams' results are those of each alone, to the bit."""
+    from oracle import mimi as omimi
+    from tests.test_gpu_mimi import _decoder
+    from vox_serve_b200 import ops
+    cfg = omimi.MimiConfig()
+    dec, _ = _decoder(cfg, 5)
+    codes = torch.randint(0, cfg.bins, (2, 32, 10), generator=torch.Generator().manual_seed(1)).cuda()
+    bank, a, b, scale, ids, x, plan, rnd = _case(600, 2048, (512, 64), rank, 5, "runs")
+    wav, want = dec.decode(codes).clone(), ops.lora(x, bank, plan)
+    torch.cuda.synchronize()
+    side, main = torch.cuda.Stream(), torch.cuda.Stream()
+    got, heard = [], []
+    for _ in range(10):
+        with torch.cuda.stream(side):
+            heard.append(dec.decode(codes).clone())
+        with torch.cuda.stream(main):
+            got += [ops.lora(x, bank, plan) for _ in range(20)]
+    torch.cuda.synchronize()
+    ops.check_waits()
+    assert all(torch.equal(h, wav) for h in heard) and all(torch.equal(o, want) for o in got)

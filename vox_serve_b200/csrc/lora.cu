@@ -351,9 +351,23 @@ __global__ void __launch_bounds__(LORA_DOWN_THREADS, 2) lora_down_kernel(const L
       for (int j = 0; j < 4; ++j) to[j] = make_float4(scale * s[4 * j], scale * s[4 * j + 1], scale * s[4 * j + 2], scale * s[4 * j + 3]);
     }
   }
+  // Tensor memory goes back before the block waits for another: a block of another stream's cluster may wait for it on this SM while its neighbour holds what this cluster's
+  // other blocks wait for.
   tc_fence_before();
-  if (p.k_split > 1) cluster_sync_all();
-  else __syncthreads();
+  if (bw.dead) {                            // (copies and products in flight land first)
+    const unsigned long long t0 = gtimer();
+    while (gtimer() - t0 < 2000000ull) __nanosleep(1000);
+  }
+  __syncwarp();
+  if (warp < 4) {
+    asm volatile("barrier.cta.arrive 1, %0;" ::"n"(LORA_DOWN_THREADS) : "memory");
+  } else {
+    asm volatile("barrier.cta.sync 1, %0;" ::"n"(LORA_DOWN_THREADS) : "memory");
+    tc_fence_after();
+  }
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");       // (a cluster of one block meets itself)
+  if (warp == 4) tmem_dealloc(tmem, ACCS * D::N);
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
   const int log_ks = 31 - __clz(p.rank_tiles);
   uint32_t* v = p.v + static_cast<long long>(gr.x) * (p.tile_rows >> 4) * rts * p.parts * 128;
   for (int e = blockIdx.x * LORA_DOWN_THREADS + tid; e < n * RT * 4; e += p.k_split * LORA_DOWN_THREADS) {
@@ -373,13 +387,6 @@ __global__ void __launch_bounds__(LORA_DOWN_THREADS, 2) lora_down_kernel(const L
     lora_put(v, p.slices, p.parts, log_ks, c, rt0 * 16 + k + 2, s.z, s.w);
   }
   if (p.k_split > 1) cluster_sync_all();                         // (others' parts have been read: the block may leave)
-  else __syncthreads();
-  tc_fence_after();
-  if (bw.dead) {                            // let the copies in flight land before the block may leave
-    const unsigned long long t0 = gtimer();
-    while (gtimer() - t0 < 2000000ull) __nanosleep(1000);
-  }
-  if (warp == 4) tmem_dealloc(tmem, ACCS * D::N);
 }
 
 // ---- second product ---------------------------------------------------------------------------------------------------------------
