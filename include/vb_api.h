@@ -496,7 +496,7 @@ int vb_gemm_bf16_grouped_glu(void* d_y, const void* d_w_tiles, const void* x_map
  * vb_gemm_wide_timeouts: whether a wait of that kernel has run out since its flag was last cleared (0 unless something is wrong;
  * synchronises the device).
  * vb_wait_flags: eight bytes of host memory, one flag per kind of kernel whose waits give up after two seconds -- 0 prompt projections, 1
- * vocoder convolutions, 2 prompt attention, 3 window attention of prompts, 4 vb_wait_check, 5 experts of a decode step, 6 adapters of a step.  A kernel whose
+ * vocoder convolutions, 2 prompt attention and attention over shared pages, 3 window attention of prompts, 4 vb_wait_check, 5 experts of a decode step, 6 adapters of a step.  A kernel whose
  * wait ran out sets its flag and leaves its output incomplete (7 without a wait: adapters, a plan of other rows or slots than the call's): look at them after synchronising, before results are used, and clear them (NULL: no device).
  * vb_wait_check: one kernel that waits on a barrier at most limit_us from the moment a second warp opens it, pause_us after the start (both warps
  * then agree on whether it ran out: the flag is 3);
@@ -936,6 +936,58 @@ int vb_moe_layer_max_rows(void);
 size_t vb_moe_layer_workspace_bytes(const VbMoeWeights* weights, const VbMoeRouter* router, int T);
 int vb_moe_layer(float* d_y, long long ldy, const void* d_h, long long ldh, const VbMoeWeights* weights, const VbMoeRouter* router, const int32_t* d_ids, int T,
                  void* d_ws, size_t ws_bytes, void* stream);
+
+/* ---- a search over several continuations of a prompt --------------------------------------------------------------------------
+ * vb_beam_select (csrc/beam.cu): of the continuations of a request's `width` beams by every token the n best, in order.
+ *   total[w][v] = score[w] + x[w][v] - log sum_v exp x[w][v] over the v with a finite logit (others are masked), candidates ranked by weight[w] * total[w][v]
+ *   (d_weight NULL: 1), equal ones by (w, v).  A beam with d_ended[w] != 0 has one candidate, end_token at score[w]; one whose score is not finite or whose weight
+ *   is not a finite number > 0 has none.  Logits [requests * width] rows of vocab (1 .. 2^24), bf16 or fp32, row_stride elements apart, at any element.
+ *   Outputs [requests][n] (n 1 .. 64, width 1 .. 32): score fp32, parent int32 (beam of the request), token int64, d_out_ended (NULL: not wanted): the parent has
+ *   ended or the token is end_token.  Fewer than n candidates: -infinity, -1, -1, 1 behind them.  end_token < 0 where no beam ends (d_ended, d_out_ended NULL).
+ * vb_beam_reorder: row slot[b][i] of every state becomes what row slot[b][parent[b][i]] was, in place (d_slots NULL: b * width + i).  parent < 0, or one outside the
+ *   request: the row stays.  states / row_bytes: HOST arrays, n_states tensors of n_slots rows; a slot stands in d_slots once. */
+size_t vb_beam_select_workspace_bytes(int requests, int width, int vocab, int n);
+int vb_beam_select(float* d_score, int32_t* d_parent, int64_t* d_token, uint8_t* d_out_ended, const void* d_logits, int64_t row_stride, int logits_f32,
+                   const float* d_beam_score, const float* d_weight, const uint8_t* d_ended, int requests, int width, int vocab, int n, int64_t end_token,
+                   void* d_workspace, size_t workspace_bytes, void* stream);
+int vb_beam_reorder(void* const* states, const int64_t* row_bytes, int n_states, int n_slots, const int32_t* d_parent, const int32_t* d_slots, int requests, int width,
+                    void* stream);
+/* Page tables on the device (csrc/pages.cu).  VbPagePool (HOST struct): table [rows][columns] page numbers (-1 behind a row's last), tokens [rows], refs [pages] rows
+ *   that hold a page, status [4] {pages that were missing, rows that grew past their columns, copies, pages in use}, copies [max(rows, pages)][3] {page, page,
+ *   tokens}, moved [pages], scratch of vb_page_pool_scratch_bytes.  A page that is not full belongs to one row.
+ * VbPageCache (HOST struct): data [layers][pages][parts][slots][slot_bytes], 16-byte aligned, slot_bytes a multiple of 16.
+ * vb_fork_pages: row i of `out` continues row src[i] of `pool` (NULL: itself; < 0: none, its pages are given back; group > 0: counted within the row's group of so
+ *   many rows) and gets room for grow[i] (NULL: grow) more tokens.  Of the rows that take over a page that is not full the first keeps it, the others get copies
+ *   of its tokens in all caches.  Free pages: lowest number first, rows in order, a row's copy first.  If pages or columns run short, out = pool and status says how
+ *   many.  out may be pool.  A page that falls free in the step may be given out in it.
+ * vb_compact_pages: with U pages in use those numbered U and above move to the free ones below U, in order, contents and all; moved[page] is a page's new number, -1
+ *   where it was free. */
+typedef struct {
+  int32_t *d_table, *d_tokens, *d_refs, *d_status, *d_copies, *d_moved, *d_scratch;
+  int32_t pages, page_size, rows, columns;
+} VbPagePool;
+typedef struct {
+  void* data;
+  int64_t slot_bytes;
+  int32_t layers, parts, slots, pad;
+} VbPageCache;
+size_t vb_page_pool_scratch_bytes(int pages, int rows);
+int vb_fork_pages(const VbPagePool* pool, const VbPagePool* out, const int32_t* d_src, int group, const int32_t* d_grow, int grow, const VbPageCache* caches,
+                  int n_caches, void* stream);
+int vb_compact_pages(const VbPagePool* pool, const VbPagePool* out, const VbPageCache* caches, int n_caches, void* stream);
+/* Attention of one new token a row over pages that rows share (csrc/shared_attn.cu).  VbSharedPlan (HOST struct): rows in requests of `width`; a page that rows of a
+ *   request hold in the same column is read once for (up to 64 / (n_q / n_kv)) of them.  d_buffer: vb_shared_plan_bytes (0: sizes that are refused), 16-byte aligned,
+ *   written by vb_shared_plan once a step and by every vb_shared_attn (one stream at a time).  head_dim 64 or 128, page_size a multiple of 16, grid: blocks.
+ * vb_shared_plan: d_table [rows][columns], d_tokens [rows] (0: a row without tokens, its output is zero); entries that are no page are skipped.
+ * vb_shared_attn: q / out [rows][n_q][head_dim] bf16 (out_xt_tile > 0: the tiled layout), d_kv [slabs][2][page_size][n_kv][head_dim] bf16, slab_base = layer * pages. */
+typedef struct {
+  void* d_buffer;
+  int32_t rows, width, columns, page_size, n_q, n_kv, head_dim, grid;
+} VbSharedPlan;
+size_t vb_shared_plan_bytes(const VbSharedPlan* plan);
+int vb_shared_plan(const VbSharedPlan* plan, const int32_t* d_table, const int32_t* d_tokens, int pages, void* stream);
+int vb_shared_attn(void* d_out, const void* d_q, const void* d_kv, int64_t slabs, int64_t slab_base, const VbSharedPlan* plan, float sm_scale, int out_xt_tile,
+                   void* stream);
 
 #ifdef __cplusplus
 }

@@ -225,6 +225,15 @@ SIGNATURES = {
                                   c_int, c_int, c_float, c_int, c_int, c_int, P]),
     "vb_selective_scan_tiled": (c_int, [P, c_int, P, P, P, c_int, P, c_int, P, P, c_int, c_int, c_int, P, c_int, P, P, P, P, P,
                                         P, P, c_int, c_int, c_int, c_int, c_int, c_float, c_int, P]),
+    "vb_beam_select_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int]),
+    "vb_beam_select": (c_int, [P, P, P, P, P, c_int64, c_int, P, P, P, c_int, c_int, c_int, c_int, c_int64, P, c_size_t, P]),
+    "vb_beam_reorder": (c_int, [P, P, c_int, c_int, P, P, c_int, c_int, P]),
+    "vb_page_pool_scratch_bytes": (c_size_t, [c_int, c_int]),
+    "vb_fork_pages": (c_int, [P, P, P, c_int, P, c_int, P, c_int, P]),
+    "vb_compact_pages": (c_int, [P, P, P, c_int, P]),
+    "vb_shared_plan_bytes": (c_size_t, [P]),
+    "vb_shared_plan": (c_int, [P, P, P, c_int, P]),
+    "vb_shared_attn": (c_int, [P, P, P, c_int64, c_int64, P, c_float, c_int, P]),
 }
 
 
@@ -243,12 +252,27 @@ class MoeRouterStruct(C.Structure):
     _fields_ = [("d_weight", P), ("d_bias", P), ("d_shared_gate", P), ("d_table", P)] + [(n, C.c_int32) for n in ("kind", "top", "groups", "keep", "vocab")]
 
 
+class PagePoolStruct(C.Structure):
+    """VbPagePool"""
+    _fields_ = [(n, P) for n in ("d_table", "d_tokens", "d_refs", "d_status", "d_copies", "d_moved", "d_scratch")] + [(n, C.c_int32) for n in ("pages", "page_size", "rows", "columns")]
+
+
+class PageCacheStruct(C.Structure):
+    """VbPageCache"""
+    _fields_ = [("data", P), ("slot_bytes", C.c_int64)] + [(n, C.c_int32) for n in ("layers", "parts", "slots", "pad")]
+
+
+class SharedPlanStruct(C.Structure):
+    """VbSharedPlan"""
+    _fields_ = [("d_buffer", P)] + [(n, C.c_int32) for n in ("rows", "width", "columns", "page_size", "n_q", "n_kv", "head_dim", "grid")]
+
+
 _lock = threading.Lock()
 _lib = None
 # flags in mapped host memory, one byte per kind of kernel whose waits give up (csrc/common.cuh, BoundedWait); the last one: a kernel that met a table of
 # another step's (csrc/lora.cu)
 _wait_flags = None
-WAIT_KINDS = ("a projection of a prompt step", "a vocoder convolution", "prompt attention", "window attention of a prompt", "vb_wait_check", "experts of a decode step", "adapters of a step",
+WAIT_KINDS = ("a projection of a prompt step", "a vocoder convolution", "prompt attention or attention over shared pages", "window attention of a prompt", "vb_wait_check", "experts of a decode step", "adapters of a step",
               "a plan of adapters")
 
 
@@ -333,7 +357,8 @@ LAUNCHES = {"vb_set_pdl": 0, "vb_set_trace": 0, "vb_weight_tiles_bytes": 0, "vb_
             "vb_short_conv": 2, "vb_selective_scan_tiled": 3, "vb_selective_scan_piece_rows": 0,
             "vb_selective_scan_scratch_floats": 0, "vb_sigmoid_attn": 1, "vb_ssd_tiled": 3, "vb_ssd_tile_rows": 0,
             "vb_ssd_scratch_floats": 0, "vb_lora_plan_bytes": 0, "vb_lora_workspace_bytes": 0, "vb_moe_layer_max_rows": 0,
-            "vb_moe_layer_workspace_bytes": 0, "vb_moe_layer": 2}
+            "vb_moe_layer_workspace_bytes": 0, "vb_moe_layer": 2, "vb_beam_select_workspace_bytes": 0, "vb_beam_select": 2, "vb_page_pool_scratch_bytes": 0,
+            "vb_shared_plan_bytes": 0, "vb_shared_plan": 2, "vb_shared_attn": 2}
 launch_counter = [0]
 
 

@@ -1,0 +1,430 @@
+// Page tables of a paged cache on the device: rows that take over other rows' pages, room for further tokens, pages that fall free, and pages that move to
+// the front of the cache.  A page may be held by several rows; refs[page] counts them.  A page that is not full yet belongs to one row: when several rows
+// take it over, the first keeps it and the others get copies of the tokens in it.
+//
+// Two launches: one cluster that works the tables out (its blocks meet three times; atomics on integers only, so that nothing hangs on their order), and a
+// kernel that copies what it listed, in all layers of all caches.
+//
+// Free pages are given out lowest number first, to rows in their order, to a row first the page for a copy.  All or nothing: if pages or columns run short
+// nothing changes and the status says so.
+#include "../../include/vb_api.h"
+#define VB_PDL_FAMILY 4
+#include "rowmma.cuh"
+
+namespace vb {
+
+constexpr int PG_THREADS = 1024, PG_MAX_CLUSTER = 8, PG_MAX_ROWS = 4096, PG_STAGE = 8192;
+
+// words of a pool's status
+enum { PS_MISSING = 0, PS_LONG = 1, PS_COPIES = 2, PS_USED = 3 };
+
+__device__ __forceinline__ int ldcg(const int32_t* p) { return __ldcg(p); }
+
+// exclusive prefix over the block of one number a thread; total in all threads.  `sums`: 33 words
+__device__ __forceinline__ int block_prefix(int mine, int* sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  __syncthreads();                                   // (the last call's sums have been read)
+  if (lane == 31) sums[warp] = inc;
+  __syncthreads();
+  if (warp == 0) {
+    int s = sums[lane], t = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, t, o);
+      if (lane >= o) t += v;
+    }
+    sums[lane] = t - s;
+    if (lane == 31) sums[32] = t;
+  }
+  __syncthreads();
+  total = sums[32];
+  return sums[warp] + inc - mine;
+}
+
+struct ForkParams {
+  const int32_t *table, *tokens, *refs;              // the pool as it is
+  int32_t *out_table, *out_tokens, *out_refs;        // as it becomes (may be the same)
+  int32_t *status, *copies, *work, *first, *base;    // scratch of the pool that is written: copies [rows][3], work / first [pages], base [rows]
+  const int32_t *src, *grow;                         // row that every row continues (null: itself; < 0: none), tokens it gets room for (null: grow_all)
+  int rows, columns, pages, page_size, group, grow_all;
+};
+
+// the row that row i continues; -1: none
+__device__ __forceinline__ int fork_source(const ForkParams& p, int i) {
+  if (!p.src) return i;
+  int s = p.src[i];
+  if (s < 0) return -1;
+  if (p.group > 0) {
+    if (s >= p.group) return -1;
+    s += i / p.group * p.group;
+  }
+  return s < p.rows ? s : -1;
+}
+__device__ __forceinline__ int fork_tokens(const ForkParams& p, int row) {
+  const int n = ldcg(p.tokens + row);
+  return n < 0 ? 0 : n < p.columns * p.page_size ? n : p.columns * p.page_size;
+}
+// (a page number of the table, or -1 where it names none: the tables are the caller's memory)
+__device__ __forceinline__ int fork_page(const ForkParams& p, int row, int col) {
+  const int g = ldcg(p.table + static_cast<long long>(row) * p.columns + col);
+  return g >= 0 && g < p.pages ? g : -1;
+}
+
+__global__ void __launch_bounds__(PG_THREADS, 1) fork_pages_kernel(const __grid_constant__ ForkParams p) {
+  extern __shared__ int32_t pg_smem[];
+  int32_t* s_src = pg_smem;                          // [rows]
+  int32_t* s_tok = s_src + p.rows;                   // [rows] tokens of the row it continues
+  int32_t* stage = s_tok + p.rows;                   // PG_STAGE: new values of a block of columns
+  __shared__ int sums[33];
+  __shared__ int s_ok;
+  const int tid = threadIdx.x, rank = cluster_ctarank(), blocks = cluster_nctarank();
+  pdl_sync();
+  for (int i = tid; i < p.rows; i += PG_THREADS) {
+    const int s = fork_source(p, i);
+    s_src[i] = s;
+    s_tok[i] = s < 0 ? 0 : fork_tokens(p, s);
+  }
+  for (int g = rank * PG_THREADS + tid; g < p.pages; g += blocks * PG_THREADS) p.work[g] = p.refs[g], p.first[g] = 0x7fffffff;
+  __syncthreads();
+  cluster_sync_all();
+
+  // holders of every page after the step, from those before it: rows that go on where they are change nothing
+  const int P = p.page_size;
+  const long long cells = static_cast<long long>(p.rows) * p.columns;
+  for (long long e = static_cast<long long>(rank) * PG_THREADS + tid; e < cells; e += static_cast<long long>(blocks) * PG_THREADS) {
+    const int i = static_cast<int>(e / p.columns), c = static_cast<int>(e - static_cast<long long>(i) * p.columns), s = s_src[i];
+    if (s == i) continue;
+    if (c < (fork_tokens(p, i) + P - 1) / P) {
+      const int g = fork_page(p, i, c);
+      if (g >= 0) atomicSub(p.work + g, 1);
+    }
+    if (s >= 0 && c < (s_tok[i] + P - 1) / P) {
+      const int g = fork_page(p, s, c);
+      if (g >= 0) atomicAdd(p.work + g, 1);
+    }
+  }
+  // the first row that holds a page which is not full
+  for (int i = rank * PG_THREADS + tid; i < p.rows; i += blocks * PG_THREADS) {
+    if (s_src[i] < 0 || s_tok[i] % P == 0) continue;
+    const int g = fork_page(p, s_src[i], s_tok[i] / P);
+    if (g >= 0) atomicMin(p.first + g, i);
+  }
+  cluster_sync_all();
+
+  if (rank == 0) {
+    // pages that every row needs: one for a copy, the others for tokens
+    int need_all = 0, copies = 0, too_long = 0;
+    for (int i0 = 0; i0 < p.rows; i0 += PG_THREADS) {
+      const int i = i0 + tid;
+      int need = 0, copy = 0, longer = 0, tail = -1, part = 0;
+      if (i < p.rows && s_src[i] >= 0) {
+        const int n = s_tok[i], g = p.grow ? ldcg(p.grow + i) : p.grow_all;
+        const long long m = static_cast<long long>(n) + (g > 0 ? g : 0);
+        part = n % P;
+        if (part) tail = fork_page(p, s_src[i], n / P);
+        copy = tail >= 0 && ldcg(p.first + tail) != i;
+        const long long want = (m + P - 1) / P;
+        longer = want > p.columns;
+        need = longer ? 0 : copy + static_cast<int>(want) - (n + P - 1) / P;
+      }
+      int total, n_copies;
+      const int before = block_prefix(need, sums, total), place = block_prefix(copy, sums, n_copies);
+      if (i < p.rows) p.base[i] = (need_all + before) * 2 + copy;
+      if (copy) {
+        int32_t* c = p.copies + 3ll * (copies + place);
+        c[0] = tail, c[1] = need_all + before, c[2] = part;      // (c[1]: which of the free pages; its number follows)
+      }
+      too_long += __syncthreads_count(longer);
+      need_all += total;
+      copies += n_copies;
+    }
+    // the lowest free pages; `first` has done its work and takes their numbers
+    int have = 0;
+    for (int g0 = 0; g0 < p.pages && have < need_all; g0 += 4 * PG_THREADS) {
+      int free = 0, mine[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int g = g0 + 4 * tid + j;
+        mine[j] = g < p.pages && ldcg(p.work + g) == 0;
+        free += mine[j];
+      }
+      int total, at = have + block_prefix(free, sums, total);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (mine[j]) {
+          if (at < need_all) p.first[at] = g0 + 4 * tid + j;
+          ++at;
+        }
+      have += total;
+    }
+    const bool ok = have >= need_all && too_long == 0;
+    __syncthreads();
+    if (ok) {
+      for (int k = tid; k < need_all; k += PG_THREADS) p.work[p.first[k]] = 1;
+      for (int k = tid; k < copies; k += PG_THREADS) {
+        int32_t* c = p.copies + 3ll * k;
+        c[1] = p.first[c[1]];
+        atomicSub(p.work + c[0], 1);
+      }
+    }
+    if (tid == 0) {
+      p.status[PS_MISSING] = have >= need_all ? 0 : need_all - have;
+      p.status[PS_LONG] = too_long;
+      p.status[PS_COPIES] = ok ? copies : 0;
+    }
+  }
+  cluster_sync_all();
+
+  if (tid == 0) s_ok = ldcg(p.status + PS_MISSING) == 0 && ldcg(p.status + PS_LONG) == 0;
+  __syncthreads();
+  const bool ok = s_ok;
+  if (!ok && p.out_table == p.table) return;        // in place: nothing has been written
+  for (int g = rank * PG_THREADS + tid; g < p.pages; g += blocks * PG_THREADS) p.out_refs[g] = ok ? ldcg(p.work + g) : ldcg(p.refs + g);
+  // A block of columns in all rows at a time, read before it is written: rows may take over one another's pages in place
+  const int wide = min(p.columns, max(1, PG_STAGE / p.rows));
+  for (int c0 = rank * wide; c0 < p.columns; c0 += blocks * wide) {
+    const int w = min(wide, p.columns - c0);
+    for (int e = tid; e < p.rows * w; e += PG_THREADS) {
+      const int i = e / w, c = c0 + e - i * w;
+      int v = -1;
+      if (!ok) {
+        v = ldcg(p.table + static_cast<long long>(i) * p.columns + c);
+      } else if (s_src[i] >= 0) {
+        const int n = s_tok[i], b = ldcg(p.base + i), copy = b & 1, at = b >> 1, held = (n + P - 1) / P;
+        const int g = p.grow ? ldcg(p.grow + i) : p.grow_all, want = static_cast<int>((static_cast<long long>(n) + (g > 0 ? g : 0) + P - 1) / P);
+        if (copy && c == n / P) v = ldcg(p.first + at);
+        else if (c < held) v = ldcg(p.table + static_cast<long long>(s_src[i]) * p.columns + c);
+        else if (c < want) v = ldcg(p.first + at + copy + c - held);
+      }
+      stage[e] = v;
+    }
+    __syncthreads();
+    for (int e = tid; e < p.rows * w; e += PG_THREADS) {
+      const int i = e / w;
+      p.out_table[static_cast<long long>(i) * p.columns + c0 + e - i * w] = stage[e];
+    }
+    __syncthreads();
+  }
+  // (tokens last: every block has read what it needs of them only at the start)
+  for (int i = rank * PG_THREADS + tid; i < p.rows; i += blocks * PG_THREADS) {
+    const int g = p.grow ? ldcg(p.grow + i) : p.grow_all;
+    p.out_tokens[i] = !ok ? ldcg(p.tokens + i) : s_src[i] < 0 ? 0 : s_tok[i] + (g > 0 ? g : 0);
+  }
+}
+
+struct CompactParams {
+  const int32_t *table, *tokens, *refs;
+  int32_t *out_table, *out_tokens, *out_refs, *moved;        // moved [pages]: a page's new number, -1: not in use
+  int32_t *status, *copies;                                  // copies [pages][3]
+  int32_t *from, *to;                                        // scratch [pages]
+  long long cells;
+  int rows, pages, page_size;
+};
+
+// The pages in use that stand behind as many places as there are pages in use move into the holes in front, in their order.
+__global__ void __launch_bounds__(PG_THREADS, 1) compact_pages_kernel(const __grid_constant__ CompactParams p) {
+  __shared__ int sums[33];
+  const int tid = threadIdx.x, rank = cluster_ctarank(), blocks = cluster_nctarank();
+  pdl_sync();
+  if (rank == 0) {
+    int used = 0;
+    for (int g0 = 0; g0 < p.pages; g0 += 4 * PG_THREADS) {
+      int mine = 0;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int g = g0 + 4 * tid + j;
+        mine += g < p.pages && p.refs[g] > 0;
+      }
+      int total;
+      block_prefix(mine, sums, total);
+      used += total;
+    }
+    int holes = 0, movers = 0;
+    for (int g0 = 0; g0 < p.pages; g0 += 4 * PG_THREADS) {
+      int n[2] = {0, 0}, what[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int g = g0 + 4 * tid + j;
+        const bool in = g < p.pages && p.refs[g] > 0;
+        what[j] = g >= p.pages ? -1 : in ? (g >= used ? 1 : -1) : (g < used ? 0 : -1);
+        if (what[j] >= 0) ++n[what[j]];
+        if (g < p.pages) p.moved[g] = in && g < used ? g : -1;
+      }
+      int th, tm;
+      int h = holes + block_prefix(n[0], sums, th), m = movers + block_prefix(n[1], sums, tm);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (what[j] == 0) p.to[h++] = g0 + 4 * tid + j;
+        if (what[j] == 1) p.from[m++] = g0 + 4 * tid + j;
+      }
+      holes += th;
+      movers += tm;
+    }
+    __syncthreads();
+    for (int k = tid; k < movers; k += PG_THREADS) {      // (as many holes as movers)
+      const int from = p.from[k], to = p.to[k];
+      p.moved[from] = to;
+      int32_t* c = p.copies + 3ll * k;
+      c[0] = from, c[1] = to, c[2] = p.page_size;
+    }
+    if (tid == 0) p.status[PS_MISSING] = p.status[PS_LONG] = 0, p.status[PS_COPIES] = movers, p.status[PS_USED] = used;
+  }
+  cluster_sync_all();
+  const long long at = static_cast<long long>(rank) * PG_THREADS + tid, step = static_cast<long long>(blocks) * PG_THREADS;
+  for (long long e = at; e < p.cells; e += step) {
+    const int g = p.table[e];
+    p.out_table[e] = g >= 0 && g < p.pages ? ldcg(p.moved + g) : g;
+  }
+  for (long long i = at; i < p.rows; i += step) p.out_tokens[i] = p.tokens[i];
+  const int movers = ldcg(p.status + PS_COPIES), used = ldcg(p.status + PS_USED);
+  if (p.out_refs != p.refs)
+    for (long long g = at; g < p.pages; g += step)
+      if (g >= used || p.refs[g] > 0) p.out_refs[g] = g < used ? p.refs[g] : 0;
+  cluster_sync_all();                                     // (in place: what moves is read before it is cleared)
+  for (long long k = at; k < movers; k += step) {
+    const int from = ldcg(p.from + k), to = ldcg(p.to + k), n = p.refs[from];
+    p.out_refs[to] = n;
+    p.out_refs[from] = 0;
+  }
+}
+
+// ---- contents of pages ------------------------------------------------------------------------------------------------------------
+// A cache is [layers][pages][parts][slots][slot bytes] (keys | values: two parts).  copies[k] = (page, page, tokens): the first tokens of every part of the
+// one go to the other.  A unit of work is 16 KB of a part of a copy in a layer.
+constexpr int PC_CACHES = 32, PC_THREADS = 256, PC_UNIT = 1024;      // (vectors of a unit)
+struct CopyCaches {
+  uint4* at[PC_CACHES];
+  long long layer[PC_CACHES], page[PC_CACHES], part[PC_CACHES];      // strides in vectors
+  int layers[PC_CACHES], parts[PC_CACHES], slot[PC_CACHES], slots[PC_CACHES], units[PC_CACHES];      // vectors and slots of a part, units of a part
+  long long first[PC_CACHES + 1];                                    // units of a copy in front
+  int n, page_size;
+};
+
+__global__ void __launch_bounds__(PC_THREADS) copy_listed_pages_kernel(const __grid_constant__ CopyCaches t, const int32_t* copies, const int32_t* status) {
+  pdl_sync();
+  const int n = status[PS_COPIES];
+  const long long per = t.first[t.n], all = per * n;
+  for (long long u = blockIdx.x; u < all; u += gridDim.x) {
+    const int k = static_cast<int>(u / per);
+    long long r = u - k * per;
+    int c = 0;
+    while (c + 1 < t.n && t.first[c + 1] <= r) ++c;
+    r -= t.first[c];
+    const int chunk = static_cast<int>(r % t.units[c]);
+    r /= t.units[c];
+    const int part = static_cast<int>(r % t.parts[c]), layer = static_cast<int>(r / t.parts[c]);
+    const int32_t* e = copies + 3ll * k;
+    // (a part with other slots than a page's tokens -- blocks of tokens, say -- goes as a whole)
+    const int slots = t.slots[c] == t.page_size ? min(e[2], t.slots[c]) : t.slots[c];
+    const int end = min(slots * t.slot[c], (chunk + 1) * PC_UNIT);
+    const long long in_layer = layer * t.layer[c] + part * t.part[c];
+    const uint4* from = t.at[c] + in_layer + e[0] * t.page[c];
+    uint4* to = t.at[c] + in_layer + e[1] * t.page[c];
+    uint4 v[4];
+    const int i0 = chunk * PC_UNIT + threadIdx.x;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j * PC_THREADS < end) v[j] = from[i0 + j * PC_THREADS];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (i0 + j * PC_THREADS < end) to[i0 + j * PC_THREADS] = v[j];
+  }
+}
+
+static int copy_listed(const VbPageCache* caches, int n_caches, const VbPagePool* pool, const int32_t* copies, const int32_t* status, void* stream) {
+  for (int c0 = 0; c0 < n_caches; c0 += PC_CACHES) {
+    CopyCaches t = {};
+    t.n = n_caches - c0 < PC_CACHES ? n_caches - c0 : PC_CACHES;
+    t.page_size = pool->page_size;
+    for (int c = 0; c < t.n; ++c) {
+      const VbPageCache& s = caches[c0 + c];
+      t.at[c] = static_cast<uint4*>(s.data);
+      t.layers[c] = s.layers, t.parts[c] = s.parts, t.slots[c] = s.slots;
+      t.slot[c] = static_cast<int>(s.slot_bytes / 16);
+      t.part[c] = static_cast<long long>(s.slots) * t.slot[c];
+      t.page[c] = t.part[c] * s.parts;
+      t.layer[c] = t.page[c] * pool->pages;
+      t.units[c] = static_cast<int>((t.part[c] + PC_UNIT - 1) / PC_UNIT);
+      t.first[c + 1] = t.first[c] + static_cast<long long>(s.layers) * s.parts * t.units[c];
+    }
+    VB_LAUNCH_PDL(copy_listed_pages_kernel, sm_count() * 8, PC_THREADS, 0, stream, t, copies, status);
+  }
+  return 0;
+}
+
+static int check_pool(const char* who, const VbPagePool* a, const VbPagePool* out) {
+  VB_CHECK_ARG(a && out, "%s: null pool", who);
+  for (const VbPagePool* p : {a, out})
+    VB_CHECK_ARG(p->d_table && p->d_tokens && p->d_refs && p->d_status && p->d_copies && p->d_moved && p->d_scratch, "%s: null pointer in a pool", who);
+  VB_CHECK_ARG(a->pages > 0 && a->page_size > 0 && a->rows > 0 && a->rows <= PG_MAX_ROWS && a->columns > 0, "%s: a pool of %d pages of %d tokens, %d rows (1 to %d) of %d columns",
+               who, a->pages, a->page_size, a->rows, PG_MAX_ROWS, a->columns);
+  VB_CHECK_ARG(static_cast<int64_t>(a->columns) * a->page_size <= 0x3fffffff && static_cast<int64_t>(a->columns + 1) * a->rows <= 0x3fffffff,
+               "%s: %d rows of %d pages of %d tokens", who, a->rows, a->columns, a->page_size);
+  VB_CHECK_ARG(a->pages == out->pages && a->page_size == out->page_size && a->rows == out->rows && a->columns == out->columns,
+               "%s: the pool that is written is of another size", who);
+  VB_CHECK_ARG((a->d_table == out->d_table) == (a->d_refs == out->d_refs) && (a->d_table == out->d_table) == (a->d_tokens == out->d_tokens),
+               "%s: two pools that share some of their buffers", who);
+  return 0;
+}
+static int check_caches(const char* who, const VbPageCache* caches, int n) {
+  VB_CHECK_ARG(n >= 0 && (n == 0 || caches), "%s: %d caches", who, n);
+  for (int c = 0; c < n; ++c) {
+    const VbPageCache& s = caches[c];
+    VB_CHECK_ARG(s.data && s.layers > 0 && s.parts > 0 && s.slots > 0 && s.slot_bytes > 0, "%s: cache %d is empty", who, c);
+    VB_CHECK_ARG(s.slot_bytes % 16 == 0 && reinterpret_cast<uintptr_t>(s.data) % 16 == 0, "%s: cache %d: %lld bytes a slot (a multiple of 16, aligned to 16)", who, c,
+                 static_cast<long long>(s.slot_bytes));
+    VB_CHECK_ARG(s.slot_bytes / 16 * s.slots <= 0x3fffffff, "%s: cache %d: %d slots of %lld bytes", who, c, s.slots, static_cast<long long>(s.slot_bytes));
+  }
+  return 0;
+}
+
+}  // namespace vb
+
+using namespace vb;
+
+extern "C" size_t vb_page_pool_scratch_bytes(int pages, int rows) {
+  if (pages <= 0 || rows <= 0) return 0;
+  return 4ull * (2ull * pages + rows);
+}
+
+extern "C" int vb_fork_pages(const VbPagePool* pool, const VbPagePool* out, const int32_t* d_src, int group, const int32_t* d_grow, int grow, const VbPageCache* caches,
+                             int n_caches, void* stream) {
+  if (int rc = check_pool("vb_fork_pages", pool, out)) return rc;
+  if (int rc = check_caches("vb_fork_pages", caches, n_caches)) return rc;
+  VB_CHECK_ARG(group >= 0 && (group == 0 || pool->rows % group == 0), "vb_fork_pages: %d rows in groups of %d", pool->rows, group);
+  VB_CHECK_ARG(grow >= 0, "vb_fork_pages: room for %d more tokens", grow);
+  ForkParams p = {};
+  p.table = pool->d_table, p.tokens = pool->d_tokens, p.refs = pool->d_refs;
+  p.out_table = out->d_table, p.out_tokens = out->d_tokens, p.out_refs = out->d_refs;
+  p.status = out->d_status, p.copies = out->d_copies;
+  p.work = out->d_scratch, p.first = p.work + pool->pages, p.base = p.first + pool->pages;
+  p.src = d_src, p.grow = d_grow, p.grow_all = grow;
+  p.rows = pool->rows, p.columns = pool->columns, p.pages = pool->pages, p.page_size = pool->page_size, p.group = group;
+  const long long cells = static_cast<long long>(p.rows) * p.columns, share = (cells + 4 * PG_THREADS - 1) / (4 * PG_THREADS);
+  const int cluster = share >= PG_MAX_CLUSTER ? PG_MAX_CLUSTER : share > 2 ? 4 : static_cast<int>(share);
+  VB_CHECK_CUDA(rm_smem<fork_pages_kernel>((2 * PG_MAX_ROWS + PG_STAGE) * 4));
+  VB_LAUNCH_PDL_CLUSTER(fork_pages_kernel, cluster, PG_THREADS, (2 * p.rows + PG_STAGE) * 4, stream, cluster, p);
+  return copy_listed(caches, n_caches, pool, out->d_copies, out->d_status, stream);
+}
+
+extern "C" int vb_compact_pages(const VbPagePool* pool, const VbPagePool* out, const VbPageCache* caches, int n_caches, void* stream) {
+  if (int rc = check_pool("vb_compact_pages", pool, out)) return rc;
+  if (int rc = check_caches("vb_compact_pages", caches, n_caches)) return rc;
+  CompactParams p = {};
+  p.table = pool->d_table, p.tokens = pool->d_tokens, p.refs = pool->d_refs;
+  p.out_table = out->d_table, p.out_tokens = out->d_tokens, p.out_refs = out->d_refs, p.moved = out->d_moved;
+  p.status = out->d_status, p.copies = out->d_copies;
+  p.from = out->d_scratch, p.to = p.from + pool->pages;
+  p.rows = pool->rows, p.pages = pool->pages, p.page_size = pool->page_size;
+  p.cells = static_cast<long long>(pool->rows) * pool->columns;
+  const long long share = (p.cells + 4 * PG_THREADS - 1) / (4 * PG_THREADS);
+  const int cluster = share >= PG_MAX_CLUSTER ? PG_MAX_CLUSTER : share > 2 ? 4 : static_cast<int>(share);
+  VB_LAUNCH_PDL_CLUSTER(compact_pages_kernel, cluster, PG_THREADS, 0, stream, cluster, p);
+  return copy_listed(caches, n_caches, pool, out->d_copies, out->d_status, stream);
+}

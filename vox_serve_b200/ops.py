@@ -10,7 +10,7 @@ import ctypes
 import math
 import os
 from functools import lru_cache
-from typing import Dict, Optional, Tuple
+from typing import Dict, NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
@@ -2212,4 +2212,265 @@ def moe_layer(h: torch.Tensor, weights: MoeWeights, router: MoeRouter, ids: Opti
     ws = h.new_empty(n // 2)                           # (of the allocator's, so that calls on other streams and captured graphs have their own)
     call("vb_moe_layer", out.data_ptr(), ld, h.data_ptr(), W, weights._ptr, router._ptr, None if ids is None else ids.data_ptr(), T, ws.data_ptr(), n, _stream())
     _lib.launch_counter[0] += ids is None or T > 8     # (the router's launch)
+    return out
+
+
+# ----------------------------------------------------------------------------------------------
+# a search over several continuations of a prompt: selection (beam.cu), page tables (pages.cu), attention over shared pages (shared_attn.cu)
+# ----------------------------------------------------------------------------------------------
+BEAM_MAX_WIDTH, BEAM_MAX_N = 32, 64
+
+
+class BeamStep(NamedTuple):
+    """What ``beam_select`` chose, [requests, n] in order: totals (fp32), the beam of the request each came from (int32), its token (int64), and whether it has
+    ended (bool; None without an end token).  Where a request has fewer candidates: -inf, -1, -1, True."""
+    scores: torch.Tensor
+    parent: torch.Tensor
+    token: torch.Tensor
+    ended: Optional[torch.Tensor]
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, weight: Optional[torch.Tensor] = None, ended: Optional[torch.Tensor] = None,
+                end_token: Optional[int] = None) -> BeamStep:
+    """One step of a beam search.  logits [requests * width, vocab] bf16 or fp32 (rows apart by any stride), scores fp32 [requests, width]: the beams' log probabilities so
+    far.  Of all continuations of a request's beams, total[w, v] = scores[w] + log_softmax(logits[w])[v], the n best in order, equal ones by (w, v).
+
+    Logits that are not finite are masked: they are no candidates and have no part in the softmax.  A beam whose score is not finite (-inf: not alive yet, or dead), or that
+    has no logit left, has no candidates.  ``weight`` fp32 [requests, width]: candidates are ranked by weight * total (length to the power -alpha, say; totals come back
+    without it; a weight that is not a finite number above zero: no candidates).  ``ended`` bool [requests, width]: such a beam goes on as it is, as one candidate under
+    ``end_token``; its logits are not read.  width 1 .. 32, n 1 .. 64, vocab up to 2^24."""
+    _need_here("beam_select", logits, scores, weight, ended)
+    f32 = logits.dtype is F32
+    _refuse(not (f32 or logits.dtype is BF16) or logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1), "beam_select: bf16 or fp32 rows of logits are needed")
+    _refuse(scores.dtype is not F32 or scores.dim() != 2 or not scores.is_contiguous(), "beam_select: fp32 scores [requests, width] are needed")
+    B, W = scores.shape
+    R, V = logits.shape
+    _refuse(B < 1 or not 1 <= W <= BEAM_MAX_WIDTH or not 1 <= n <= BEAM_MAX_N, f"beam_select: {B} requests of {W} beams (1 to {BEAM_MAX_WIDTH}), the best {n} (1 to {BEAM_MAX_N})")
+    _refuse(R != B * W or not 1 <= V <= 1 << 24, f"beam_select: logits {tuple(logits.shape)} for {B} requests of {W} beams (a vocabulary of 1 to 2^24)")
+    if weight is not None:
+        _refuse(weight.dtype is not F32 or weight.shape != scores.shape or not weight.is_contiguous(), f"beam_select: fp32 weights [{B}, {W}] are needed")
+    if ended is not None:
+        _refuse(ended.dtype is not torch.bool or ended.shape != scores.shape or not ended.is_contiguous(), f"beam_select: ended beams are bool [{B}, {W}]")
+        _refuse(end_token is None, "beam_select: beams that have ended go on under an end token: end_token is needed")
+    _refuse(end_token is not None and not 0 <= end_token < V, f"beam_select: end token {end_token} outside the vocabulary of {V}")
+    lib = _lib._lib or _lib.load()
+    dev = logits.device
+    step = BeamStep(torch.empty((B, n), dtype=F32, device=dev), torch.empty((B, n), dtype=torch.int32, device=dev), torch.empty((B, n), dtype=torch.int64, device=dev),
+                    None if end_token is None else torch.empty((B, n), dtype=torch.bool, device=dev))
+    # (of the allocator's, so that calls on other streams and captured graphs have their own)
+    ws = torch.empty(lib.vb_beam_select_workspace_bytes(B, W, V, n) // 8, dtype=torch.int64, device=dev)
+    call("vb_beam_select", step.scores.data_ptr(), step.parent.data_ptr(), step.token.data_ptr(), _p(step.ended), logits.data_ptr(), logits.stride(0) if R > 1 else V,
+         int(f32), scores.data_ptr(), _p(weight), _p(ended), B, W, V, n, -1 if end_token is None else end_token, ws.data_ptr(), ws.numel() * 8, _stream())
+    return step
+
+
+def beam_reorder(states: Sequence[torch.Tensor], parent: torch.Tensor, slots: Optional[torch.Tensor] = None) -> Sequence[torch.Tensor]:
+    """Rows of recurrent states follow their beams, in place: with parent int32 [requests, width] row slots[b, i] of every state becomes what row
+    slots[b, parent[b, i]] was; parent -1 (or outside the request): the row stays as it is.  states: contiguous tensors [slots, ...] of any types, all of one number of slots
+    (of a stack of layers: one each).  slots int32 [requests, width] (None: b * width + i); a slot belongs to one beam: one that is named twice receives either row; one outside
+    the states is skipped.  Returns ``states``."""
+    _need_here("beam_reorder", parent, slots, *states)
+    _refuse(parent.dtype is not torch.int32 or parent.dim() != 2 or not parent.is_contiguous(), "beam_reorder: int32 parents [requests, width] are needed")
+    B, W = parent.shape
+    _refuse(B < 1 or B > 65535 or not 1 <= W <= BEAM_MAX_WIDTH, f"beam_reorder: {B} requests (1 to 65535) of {W} beams (1 to {BEAM_MAX_WIDTH})")
+    _refuse(slots is not None and (slots.dtype is not torch.int32 or slots.shape != parent.shape or not slots.is_contiguous()), f"beam_reorder: int32 slots [{B}, {W}] are needed")
+    if not states:
+        return states
+    n_slots, ptrs, sizes = states[0].shape[0] if states[0].dim() else 0, [], []
+    for t in states:
+        _refuse(t.dim() < 1 or t.shape[0] != n_slots or not t.is_contiguous() or t.numel() == 0, f"beam_reorder: contiguous states of {n_slots} slots are needed, not {tuple(t.shape)}")
+        ptrs.append(t.data_ptr())
+        sizes.append(t.numel() // n_slots * t.element_size())
+    _refuse(len(set(ptrs)) != len(ptrs), "beam_reorder: a state stands in the list twice")
+    _refuse(max(sizes) >= 1 << 32, "beam_reorder: a row of 4 GB or more")
+    _refuse(slots is None and B * W > n_slots, f"beam_reorder: {B} requests of {W} beams in {n_slots} rows")
+    k = len(ptrs)
+    call("vb_beam_reorder", (ctypes.c_void_p * k)(*ptrs), (ctypes.c_int64 * k)(*sizes), k, n_slots, parent.data_ptr(), _p(slots), B, W, _stream())
+    _lib.launch_counter[0] += (k + 63) // 64 - 1
+    return states
+
+
+class PagePool:
+    """Page tables of a paged cache on the device: ``table`` int32 [rows, columns] (-1 behind a row's last page), ``tokens`` int32 [rows], ``refs`` int32 [pages]: how many rows hold a
+    page, 0: free.  All rows are empty and all pages free at first.  ``fork_pages`` and ``compact_pages`` work on it without the host; ``check`` asks how the last one went.
+
+    For ``plan_rows`` a pool is a page table of ``columns`` pages a row: kv_indptr = ``indptr``, kv_indices = ``table`` in one dimension, kv_len = ``tokens``.  A
+    page that is not full belongs to one row; whoever writes the tables himself (``load``) keeps to that."""
+
+    def __init__(self, pages: int, page_size: int, rows: int, columns: int, device="cuda"):
+        _refuse(pages < 1 or page_size < 1 or not 1 <= rows <= 4096 or columns < 1 or columns * page_size > 0x3fffffff or (columns + 1) * rows > 0x3fffffff,
+                f"PagePool: {pages} pages of {page_size} tokens, {rows} rows (1 to 4096) of {columns} columns")
+        self.pages, self.page_size, self.rows, self.columns = int(pages), int(page_size), int(rows), int(columns)
+        n = [rows * columns, rows, pages, 4, 3 * max(rows, pages), pages, 2 * pages + rows]
+        self._buf = torch.zeros(sum((k + 3) // 4 * 4 for k in n), dtype=torch.int32, device=device)
+        parts, at = [], 0
+        for k in n:
+            parts.append(self._buf[at:at + k])
+            at += (k + 3) // 4 * 4
+        self.table, self.tokens, self.refs, self.status, self.copies, self.moved, scratch = parts
+        self.table = self.table.view(rows, columns)
+        self.table.fill_(-1)
+        self.indptr = torch.arange(0, (rows + 1) * columns, columns, dtype=torch.int32, device=device)
+        self._struct = _lib.PagePoolStruct(*(t.data_ptr() for t in (self.table, self.tokens, self.refs, self.status, self.copies, self.moved, scratch)),
+                                           self.pages, self.page_size, self.rows, self.columns)
+        self._ptr, self._device = ctypes.addressof(self._struct), self._buf.get_device()
+
+    def load(self, table: torch.Tensor, tokens: torch.Tensor) -> "PagePool":
+        """tables that exist already: int32 [rows, columns] and [rows]; ``refs`` is counted from them"""
+        _refuse(tuple(table.shape) != (self.rows, self.columns) or tuple(tokens.shape) != (self.rows,), f"PagePool.load: a table [{self.rows}, {self.columns}] is needed")
+        self.table.copy_(table)
+        self.tokens.copy_(tokens)
+        held = (self.tokens + self.page_size - 1) // self.page_size
+        on = (torch.arange(self.columns, device=self.table.device)[None] < held[:, None]) & (self.table >= 0) & (self.table < self.pages)
+        at = torch.where(on, self.table, torch.full_like(self.table, self.pages)).view(-1).long()
+        count = torch.zeros(self.pages + 1, dtype=torch.int32, device=self.table.device).index_add_(0, at, torch.ones_like(at, dtype=torch.int32))
+        self.refs.copy_(count[:self.pages])
+        self.table.masked_fill_(~on, -1)
+        return self
+
+    def check(self) -> None:
+        """Raises if the last ``fork_pages`` found too few pages or columns (it changed nothing then).  Waits for it."""
+        missing, longer = self.status[:2].tolist()
+        _refuse(missing > 0, f"fork_pages: {missing} pages are missing (of {self.pages})")
+        _refuse(longer > 0, f"fork_pages: {longer} rows grew past {self.columns} pages")
+
+
+def _page_caches(who: str, caches, pool: PagePool):
+    """VbPageCache of every cache: [layers, pages, 2, page, ...] or, of one layer, [pages, page, ...]; per page anything else [pages, n, ...] goes as a whole"""
+    out, seen = [], set()
+    for t in caches:
+        _need_here(who, t)
+        s, P, n = t.shape, pool.page_size, pool.pages
+        _refuse(not t.is_contiguous() or t.numel() == 0, f"{who}: contiguous caches are needed, not {tuple(s)}")
+        if t.data_ptr() in seen:                       # (a cache that is both keys and values is one)
+            continue
+        seen.add(t.data_ptr())
+        if t.dim() == 6 and s[1] == n and s[2] == 2 and s[3] == P:
+            layers, parts, slots = s[0], 2, P
+        elif t.dim() == 5 and s[0] == n and s[1] == 2 and s[2] == P:
+            layers, parts, slots = 1, 2, P
+        else:
+            _refuse(t.dim() < 2 or s[0] != n, f"{who}: a cache of {n} pages of {P} tokens is needed: [layers, pages, 2, page, ...], [pages, 2, page, ...] or [pages, n, ...], not {tuple(s)}")
+            layers, parts, slots = 1, 1, s[1]
+        slot = t.numel() // (layers * n * parts * slots) * t.element_size()
+        _refuse(slot % 16 != 0 or t.data_ptr() % 16 != 0, f"{who}: {slot} bytes a token of a cache (a multiple of 16, aligned to 16)")
+        out.append((t.data_ptr(), slot, layers, parts, slots, 0))
+    return (_lib.PageCacheStruct * max(1, len(out)))(*out), len(out)
+
+
+def _pool_check(who: str, pool: PagePool, out: Optional[PagePool]) -> PagePool:
+    out = pool if out is None else out
+    _refuse(pool._device < 0 or pool._device != _device_index() or out._device != pool._device, f"{who}: pools on the current device are needed")
+    _refuse((pool.pages, pool.page_size, pool.rows, pool.columns) != (out.pages, out.page_size, out.rows, out.columns), f"{who}: out is a pool of another size")
+    return out
+
+
+def fork_pages(pool: PagePool, src: Optional[torch.Tensor] = None, grow: Union[int, torch.Tensor] = 0, caches: Sequence[torch.Tensor] = (), group: Optional[int] = None,
+               out: Optional[PagePool] = None) -> PagePool:
+    """Rows of a pool take over other rows' pages, give pages back and get room for further tokens, all at once.
+
+    ``src`` int32: the row that every row continues, -1: none (its pages are given back); None: every row itself.  In one dimension [rows], or, [requests, width], counted within
+    the request (what ``beam_select`` leaves as ``parent``).  ``group``: the same for a ``src`` in one dimension.  ``grow``: how many more tokens a row gets room for and counts,
+    one number or int32 [rows].  So a decode step of a search is ``fork_pages(pool, parent, 1, [kv_cache])``; room for prompts is ``grow`` alone, several continuations of a
+    prompt are a ``src`` that names its row several times, and a request that leaves is a -1.
+
+    Pages are shared, not copied, but for one that is not full yet: of the rows that take it over the first keeps it, the others get copies of the tokens in it, in every one of
+    ``caches``: [layers, pages, 2, page, ...], [pages, 2, page, ...], or of one layer [pages, page, ...]; [pages, n, ...] with another n goes as a whole page.  A cache that is
+    left out loses those tokens for the copies.  Free pages are given out lowest number first.  If pages or columns run short nothing changes, and ``check`` of the pool
+    that was written raises.  ``out``: a pool of the same size that is written instead (it has tables of its own; the caches are one)."""
+    out = _pool_check("fork_pages", pool, out)
+    by, g_ptr, g_all = 0, None, 0
+    if src is not None:
+        _need_here("fork_pages", src)
+        _refuse(src.dtype is not torch.int32 or not src.is_contiguous() or src.numel() != pool.rows or src.dim() not in (1, 2), f"fork_pages: int32 sources of {pool.rows} rows are needed")
+        by = src.shape[1] if src.dim() == 2 else 0
+    if group is not None:
+        _refuse(group < 1 or pool.rows % group != 0 or by not in (0, group), f"fork_pages: {pool.rows} rows in groups of {group}")
+        by = group
+    if isinstance(grow, torch.Tensor):
+        _need_here("fork_pages", grow)
+        _refuse(grow.dtype is not torch.int32 or tuple(grow.shape) != (pool.rows,) or not grow.is_contiguous(), f"fork_pages: room is a number or int32 [{pool.rows}]")
+        g_ptr = grow.data_ptr()
+    else:
+        g_all = int(grow)
+        _refuse(not 0 <= g_all <= 0x3fffffff, f"fork_pages: room for {g_all} more tokens")
+    c, n = _page_caches("fork_pages", caches, pool)
+    call("vb_fork_pages", pool._ptr, out._ptr, _p(src), by, g_ptr, g_all, ctypes.addressof(c), n, _stream())
+    _lib.launch_counter[0] += (n + 31) // 32
+    return out
+
+
+def compact_pages(pool: PagePool, caches: Sequence[torch.Tensor] = (), out: Optional[PagePool] = None) -> PagePool:
+    """The pages in use move to the front of the cache: with U of them those numbered U and above go, in their order, to the free ones below U, contents (all of ``caches``, as for
+    ``fork_pages``), tables and counts.  ``moved`` int32 [pages] of the pool that is written: a page's new number, -1 where it was free; ``status[3]``: U."""
+    out = _pool_check("compact_pages", pool, out)
+    c, n = _page_caches("compact_pages", caches, pool)
+    call("vb_compact_pages", pool._ptr, out._ptr, ctypes.addressof(c), n, _stream())
+    _lib.launch_counter[0] += (n + 31) // 32
+    return out
+
+
+class SharedPlan:
+    """The different pages that the rows of a step hold (``shared_plan``): made once per step, read by ``shared_attn`` of every layer, which also keeps its partial results in it: a
+    plan belongs to one stream at a time, and captured steps that may run at once have one each.  rows: requests of ``width`` rows one after the other; columns: of the page table."""
+
+    def __init__(self, rows: int, width: int, columns: int, page_size: int, n_q: int, n_kv: int, head_dim: int, device="cuda"):
+        _refuse(rows < 1 or width < 1 or rows % width != 0, f"SharedPlan: {rows} rows in requests of {width}")
+        _refuse(n_kv < 1 or n_q < 1 or n_q % n_kv != 0 or n_q // n_kv > 64, f"SharedPlan: {n_q} query heads on {n_kv} key heads (at most 64 on one)")
+        _refuse(head_dim not in (64, 128), f"SharedPlan: heads of {head_dim} (64 or 128)")
+        _refuse(page_size < 16 or page_size % 16 != 0 or page_size > 4096, f"SharedPlan: pages of {page_size} tokens (a multiple of 16, at most 4096)")
+        _refuse(not 1 <= columns <= 16384, f"SharedPlan: {columns} pages a row (1 to 16384)")
+        self.rows, self.width, self.columns, self.page_size, self.n_q, self.n_kv, self.head_dim = (int(v) for v in (rows, width, columns, page_size, n_q, n_kv, head_dim))
+        self.pages = 0                                 # of the cache that the plan was made for
+        grid = attn_grid_ctas() if torch.device(device).type == "cuda" else 148
+        self._struct = _lib.SharedPlanStruct(None, self.rows, self.width, self.columns, self.page_size, self.n_q, self.n_kv, self.head_dim, grid)
+        self._ptr = ctypes.addressof(self._struct)
+        n = (_lib._lib or _lib.load()).vb_shared_plan_bytes(self._ptr)
+        _refuse(n == 0, f"SharedPlan: {rows} rows of {columns} pages on {n_kv} heads are too many")
+        self.buf = torch.zeros((n + 15) // 16 * 4, dtype=torch.int32, device=device)
+        self._struct.d_buffer = self.buf.data_ptr()
+        self._device = self.buf.get_device()
+
+
+def shared_plan(plan: SharedPlan, table: torch.Tensor, tokens: torch.Tensor, pages: int = 0) -> SharedPlan:
+    """table int32 [rows, columns], tokens int32 [rows]: what every row attends to, the new token's key and value among it; 0: nothing (zeros come out).  ``pages``: of the cache
+    (0: any); a number of the table outside it counts as no page."""
+    _need_here("shared_plan", plan.buf, table, tokens)
+    R = plan.rows
+    _refuse(table.dtype is not torch.int32 or tuple(table.shape) != (R, plan.columns) or not table.is_contiguous(), f"shared_plan: an int32 table [{R}, {plan.columns}] is needed")
+    _refuse(tokens.dtype is not torch.int32 or tuple(tokens.shape) != (R,) or not tokens.is_contiguous(), f"shared_plan: int32 tokens [{R}] are needed")
+    most = 0x7fffffff // plan.page_size
+    _refuse(not 0 <= pages <= most, f"shared_plan: {pages} pages of {plan.page_size} tokens")
+    call("vb_shared_plan", plan._ptr, table.data_ptr(), tokens.data_ptr(), pages or most, _stream())
+    plan.pages = int(pages)
+    return plan
+
+
+def shared_attn(q: torch.Tensor, kv_cache: torch.Tensor, slab_base: int, plan: SharedPlan, sm_scale: Optional[float] = None, out=None):
+    """Attention of one new token a row, every different page read once for the rows of a request that hold it: q bf16 [rows, Hq, D] -> [rows, Hq, D].  kv_cache: the whole cache
+    [layers, pages, 2, page, Hkv, D] (slab_base = layer * pages) or one layer [pages, 2, page, Hkv, D] bf16, as for ``paged_attn``, whose results it has up to rounding;
+    ``plan``: ``shared_plan`` of this step's tables.  out: bf16 like q, or a TiledAct.  What is not finite in a page reaches the rows that hold it and no others."""
+    R, Hq, D = plan.rows, plan.n_q, plan.head_dim
+    if not (q.is_cuda and q.get_device() == plan._device == kv_cache.get_device() == _device_index()):
+        _need_here("shared_attn", q, kv_cache, plan.buf)
+    _refuse(q.dtype is not BF16 or tuple(q.shape) != (R, Hq, D) or not q.is_contiguous(), f"shared_attn: bf16 queries [{R}, {Hq}, {D}] are needed")
+    s = kv_cache.shape
+    _refuse(kv_cache.dtype is not BF16 or not kv_cache.is_contiguous() or len(s) not in (5, 6) or tuple(s[-4:]) != (2, plan.page_size, plan.n_kv, D),
+            f"shared_attn: a bf16 cache [.., pages, 2, {plan.page_size}, {plan.n_kv}, {D}] is needed, not {tuple(s)}")
+    per, slabs = s[-5], s[0] * (s[1] if len(s) == 6 else 1)
+    _refuse(plan.pages > per, f"shared_attn: the plan is of {plan.pages} pages, the cache has {per} a layer")
+    _refuse(not 0 <= slab_base <= slabs - per or slab_base % per != 0, f"shared_attn: layer at page {slab_base} of {slabs}")
+    xt = 0
+    if isinstance(out, TiledAct):
+        _need_here("shared_attn", out.data)
+        _refuse(out.T != R or out.K != Hq * D, f"shared_attn: tiled rows [{out.T}, {out.K}] are not [{R}, {Hq * D}]")
+        to, xt = out.data, out.t_tile
+    elif out is None:
+        out = to = torch.empty_like(q)
+    else:
+        to = out
+        _need_here("shared_attn", out)
+        _refuse(out.dtype is not BF16 or out.shape != q.shape or not out.is_contiguous(), f"shared_attn: out is bf16 [{R}, {Hq}, {D}]")
+    call("vb_shared_attn", to.data_ptr(), q.data_ptr(), kv_cache.data_ptr(), slabs, int(slab_base), plan._ptr, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), xt,
+         _stream())
     return out
