@@ -946,7 +946,7 @@ int vb_moe_layer(float* d_y, long long ldy, const void* d_h, long long ldh, cons
  *   ended or the token is end_token.  Fewer than n candidates: -infinity, -1, -1, 1 behind them.  end_token < 0 where no beam ends (d_ended, d_out_ended NULL).
  * vb_beam_reorder: row slot[b][i] of every state becomes what row slot[b][parent[b][i]] was, in place (d_slots NULL: b * width + i).  parent < 0, or one outside the
  *   request: the row stays.  states / row_bytes: HOST arrays, n_states tensors of n_slots rows; a slot stands in d_slots once. */
-size_t vb_beam_select_workspace_bytes(int requests, int width, int vocab, int n);
+size_t vb_beam_select_workspace_bytes(int requests, int width, int vocab, int n, int logits_f32);
 int vb_beam_select(float* d_score, int32_t* d_parent, int64_t* d_token, uint8_t* d_out_ended, const void* d_logits, int64_t row_stride, int logits_f32,
                    const float* d_beam_score, const float* d_weight, const uint8_t* d_ended, int requests, int width, int vocab, int n, int64_t end_token,
                    void* d_workspace, size_t workspace_bytes, void* stream);

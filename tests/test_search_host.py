@@ -16,11 +16,13 @@ def launched(monkeypatch):
     monkeypatch.setattr(ops, "_need_here", lambda who, *ts: None)
     monkeypatch.setattr(ops, "_device_index", lambda: 0)
     monkeypatch.setattr(ops, "_stream", lambda: 0)
+    monkeypatch.setattr(ops, "_raw_stream", lambda dev: 0)
     monkeypatch.setattr(ops, "call", lambda name, *a: calls.append(name))
     return calls
 
 
-def test_cpu_tensors_are_refused():
+def test_cpu_tensors_are_refused(monkeypatch):
+    monkeypatch.setattr(ops, "_device_index", lambda: 0)
     with pytest.raises(VoxB200Error):
         ops.beam_select(torch.zeros(2, 8), torch.zeros(1, 2), 2)
     with pytest.raises(VoxB200Error):
@@ -192,7 +194,7 @@ def test_plan_cuts_requests_evenly():
 def test_entry_points_check_by_themselves():
     """the C ABI refuses without a device what it would not survive"""
     lib = _lib.load()
-    assert lib.vb_beam_select_workspace_bytes(2, 3, 8193, 4) == 2 * 3 * 2 * (8 + 32)
+    assert lib.vb_beam_select_workspace_bytes(2, 3, 8193, 4, 0) == 2 * 3 * 2 * (8 + 32)
     assert lib.vb_beam_select(None, None, None, None, None, 0, 0, None, None, None, 1, 1, 8, 1, -1, None, 0, None) != 0 and b"null" in lib.vb_last_error()
     buf = ctypes.create_string_buffer(4096)
     at = (ctypes.addressof(buf) + 15) // 16 * 16

@@ -4,19 +4,21 @@
 //   the n candidates of largest weight[w] * total[w][v]; equal ones in the order of (w, v)
 //   a beam that has ended has one candidate, its end token at its own score
 //
-// Two launches.  The first reads the logits once: a block takes 8192 of a row, keeps them in registers, and leaves their maximum, their sum of exponentials
-// and their n largest in order.  The second, a block a request, adds the sums up, ranks the n largest of every slice by their totals and writes the n best.
-// What orders candidates is computed in 64 bits from the slices' sums, so that it hangs on those alone; a sum's terms carry 2^-22 each and no common error.
+// Two launches.  The first reads the logits once: a block streams a part of a row through registers in chunks, the next one in flight, and leaves the part's
+// maximum, its sum of exponentials and its n largest in order.  The second, a block a request, adds the sums up, ranks the n largest of every part by their totals
+// and writes the n best.  What orders candidates is computed in 64 bits from the parts' sums; a sum's terms carry 2^-22 each and no common error.
 #include "../../include/vb_api.h"
 #define VB_PDL_FAMILY 16
-#include "common.cuh"
+#include "rowmma.cuh"
 
 namespace vb {
 
-constexpr int BS_THREADS = 256;
-constexpr int BS_SLICE = 8192;            // logits of a block: 32 a thread
-constexpr int BS_CAP = 512;               // candidates that a block ranks
+constexpr int BS_THREADS = 256, BS_VECS = 4, BS_STAGES = 2;     // a chunk: four vectors of 16 bytes a thread; chunks in shared memory
+constexpr int BS_CAP = 1024;                                   // candidates that a block keeps
+constexpr int BS_BLOCKS = 4;                                    // blocks an SM holds
 constexpr int BS_MAX_N = 64, BS_MAX_W = 32;
+constexpr int BJ_BINS = 1024;                                   // 16 to a doubling, from 2^-23 to 2^41
+constexpr int BJ_THREADS = 512, BJ_ALL = 8192;                  // candidates of a request: 128 KB of ranks and values
 
 struct BeamStats {
   float m, s;
@@ -26,6 +28,19 @@ __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
+}
+// two fp32 at a time
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\tfma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
 }
 constexpr float LOG2E = 1.44269502f, LOG2E_REST = 1.92596303e-8f;
 // e^d, d <= 0: log2 e in two parts, so that the product's rounding (2^-24 of the exponent) is the only error and has no common sign
@@ -42,6 +57,10 @@ __device__ __forceinline__ uint64_t order_f64(double x) {
   const uint64_t u = static_cast<uint64_t>(__double_as_longlong(x + 0.0));
   const uint64_t k = u ^ (static_cast<int64_t>(u) < 0 ? ~0ull : 0x8000000000000000ull);
   return (u & 0x7ff0000000000000ull) == 0x7ff0000000000000ull ? 0ull : k;
+}
+
+__device__ __forceinline__ double unorder_f64(uint64_t k) {
+  return __longlong_as_double(static_cast<long long>(k & 0x8000000000000000ull ? k ^ 0x8000000000000000ull : ~k));
 }
 
 // sum over the block of what its threads counted; `box`: three words, zero at first, used in turn
@@ -62,226 +81,358 @@ __device__ __forceinline__ bool beam_reads(const float* score, const float* weig
   return isfinite(s) && isfinite(by) && by > 0.f;
 }
 
-// 16 bytes from byte `by` of the 32 that two neighbouring vectors hold (by < 16, even)
-__device__ __forceinline__ uint4 realign(uint4 p, uint4 q, int by) {
-  uint32_t w[7] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z};
-  uint32_t last = q.w;
-  if (by & 8) {
+__device__ __forceinline__ void copy16_async(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+// Four words of shared memory at an address that is a multiple of ALIGN (two: the words that hold them are read)
+template <int ALIGN>
+__device__ __forceinline__ void read_words(uint32_t* w, uint32_t at) {
+  if (ALIGN == 16) {
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+  } else if (ALIGN == 8) {
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at) : "memory");
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[2]), "=r"(w[3]) : "r"(at + 8u) : "memory");
+  } else {
+    uint32_t v[5];
 #pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = w[i + 2];
-    w[5] = last;
-  }
-  if (by & 4) {
+    for (int j = 0; j < (ALIGN == 4 ? 4 : 5); ++j) asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v[j]) : "r"(at - (ALIGN == 2 ? 2u : 0u) + 4u * j) : "memory");
 #pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+    for (int j = 0; j < 4; ++j) w[j] = ALIGN == 4 ? v[j] : __funnelshift_r(v[j], v[j + 1], 16);
   }
-  if (by & 2) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = __funnelshift_r(w[i], w[i + 1], 16);
-  }
-  return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// The logits that a thread holds: 32, as they came
+// The logits of a chunk that a thread holds, as they came
 template <typename T>
-struct Held;
-template <>
-struct Held<float> {
-  uint32_t w[32];
-  __device__ __forceinline__ float at(int k) const { return __uint_as_float(w[k]); }
-  __device__ __forceinline__ void mask(int k) { w[k] = 0xff800000u; }
-};
-template <>
-struct Held<__nv_bfloat16> {
-  uint32_t w[16];
-  __device__ __forceinline__ float at(int k) const { return (k & 1) ? bf16_hi(w[k >> 1]) : bf16_lo(w[k >> 1]); }
-  __device__ __forceinline__ void mask(int k) { w[k >> 1] = (k & 1) ? (w[k >> 1] & 0xffffu) | 0xff800000u : (w[k >> 1] & 0xffff0000u) | 0xff80u; }
-};
-
-// One slice of one row.  T: bf16 or fp32 logits.  Rows may start at any element: a thread's vector is put together from the two aligned ones it lies in, so
-// that which thread adds what does not hang on the address, and equal rows have equal sums.  (A vector that holds a byte of the row lies in the same 16 bytes.)
-template <typename T>
-__global__ void __launch_bounds__(BS_THREADS, 4) beam_slice_kernel(BeamStats* __restrict__ stats, uint64_t* __restrict__ best, const T* __restrict__ logits,
-                                                                   long long stride, int V, int slices, const float* score, const float* weight,
-                                                                   const uint8_t* ended, int n) {
-  constexpr int EV = 16 / sizeof(T), NV = 32 / EV;
-  __shared__ uint64_t list[BS_CAP];
-  __shared__ uint32_t box[3], count;
-  __shared__ float groups[64], cut_s, part_m[8], part_s[8];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int row = blockIdx.x / slices, slice = blockIdx.x - row * slices;
-  if (tid == 0) box[0] = box[1] = box[2] = count = 0u;
-  pdl_sync();
-  if (!beam_reads(score, weight, ended, row)) return;       // (the second kernel does not look at this row either)
-  const uintptr_t at = reinterpret_cast<uintptr_t>(logits + static_cast<long long>(row) * stride);
-  const int by = static_cast<int>(at & 15);
-  const uint4* src = reinterpret_cast<const uint4*>(at - by);
-  const int vecs = (V + EV - 1) / EV, held = (V * static_cast<int>(sizeof(T)) + by + 15) / 16, v0 = slice * (BS_SLICE / EV);
-
-  Held<T> x;
-  {
-    uint4 q[NV];
-    const uint4 none = sizeof(T) == 4 ? make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u) : make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u);
+struct Held {
+  static constexpr int EV = 16 / sizeof(T), N = BS_VECS * EV;
+  uint32_t w[4 * BS_VECS];
+  __device__ __forceinline__ float at(int k) const {
+    if (sizeof(T) == 4) return __uint_as_float(w[k]);
+    return (k & 1) ? bf16_hi(w[k >> 1]) : bf16_lo(w[k >> 1]);
+  }
+  __device__ __forceinline__ void mask(int k) {
+    if (sizeof(T) == 4) w[k] = 0xff800000u;
+    else w[k >> 1] = (k & 1) ? (w[k >> 1] & 0xffffu) | 0xff800000u : (w[k >> 1] & 0xffff0000u) | 0xff80u;
+  }
+  __device__ __forceinline__ float max() const {            // (NaN only where there is nothing else)
+    if (sizeof(T) == 4) {
+      float m = at(0);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int vi = v0 + i * BS_THREADS + tid;
-      q[i] = vi < vecs ? __ldg(src + vi) : none;
+      for (int k = 1; k < N; ++k) m = fmaxf(m, at(k));
+      return m;
     }
-    if (by) {
+    __nv_bfloat162 m = *reinterpret_cast<const __nv_bfloat162*>(&w[0]);
 #pragma unroll
-      for (int i = 0; i < NV; ++i) {
-        const int vi = v0 + i * BS_THREADS + tid;
-        if (vi < vecs) q[i] = realign(q[i], vi + 1 < held ? __ldg(src + vi + 1) : none, by);
+    for (int j = 1; j < 4 * BS_VECS; ++j) m = __hmax2(m, *reinterpret_cast<const __nv_bfloat162*>(&w[j]));
+    return fmaxf(__low2float(m), __high2float(m));
+  }
+};
+
+// The n largest keys of the list's first c, in order, to its front.  (They differ: a key's place is the number of larger ones.)
+__device__ __forceinline__ void keep_largest(uint64_t* list, int c, int n) {
+  uint64_t key[BS_CAP / BS_THREADS];
+  int rank[BS_CAP / BS_THREADS];
+#pragma unroll
+  for (int e = 0; e < BS_CAP / BS_THREADS; ++e) {
+    const int i = threadIdx.x + e * BS_THREADS;
+    rank[e] = n;
+    if (i < c) {
+      key[e] = list[i];
+      int r = 0;
+#pragma unroll 8
+      for (int j = 0; j < c; ++j) r += list[j] > key[e] ? 1 : 0;
+      rank[e] = r;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < BS_CAP / BS_THREADS; ++e)
+    if (rank[e] < n) list[rank[e]] = key[e];
+  __syncthreads();
+}
+
+constexpr int BS_SPAN = 32 * BS_VECS, BS_SLOT = (BS_SPAN + 1) * 16;      // vectors of a chunk that a warp reads, and bytes of the aligned ones that hold them
+struct PartShared {
+  uint8_t ring[BS_STAGES][BS_THREADS / 32][BS_SLOT];
+  uint64_t list[BS_CAP];
+  uint32_t box[3], count, tops[8];
+  float part_m[8], part_s[8];
+};
+
+// One part of one row: every parts-th chunk, so that a masked stretch of the vocabulary is shared out.  T: bf16 or fp32 logits.  Rows may start at any
+// element: aligned vectors go to shared memory (each holds a byte of the row, and a vector lies within a page), the width of the reads there goes by the
+// row's address (ALIGN).  Which thread adds what does not, and equal rows have equal sums.  A warp's span is its own: no block waits for another warp's.
+template <typename T, int ALIGN>
+__device__ __forceinline__ void beam_part(PartShared& sh, BeamStats* stats, uint64_t* best, const uint8_t* at, int V, int part, int parts, int n) {
+  constexpr int EV = Held<T>::EV, N = Held<T>::N, CHUNK = BS_THREADS * BS_VECS;      // (vectors)
+  uint64_t* list = sh.list;
+  uint32_t *box = sh.box, &count = sh.count;
+  float *part_m = sh.part_m, *part_s = sh.part_s;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int by = ALIGN == 16 ? 0 : static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15);
+  const int vecs = (V + EV - 1) / EV, held = (V * static_cast<int>(sizeof(T)) + by + 15) / 16;
+  const int step = parts * CHUNK, first = part * CHUNK + warp * BS_SPAN;      // (this warp's vectors)
+  const uint8_t* src = at - by;
+  const uint32_t ring = smem_u32(sh.ring) + warp * BS_SLOT;
+  constexpr uint32_t STAGE = (BS_THREADS / 32) * BS_SLOT;
+  auto fetch = [&](int v0, int slot) {
+#pragma unroll
+    for (int j = 0; j < BS_VECS; ++j) {
+      const int vi = v0 + j * 32 + lane;
+      if (vi < held) copy16_async(ring + slot * STAGE + (j * 32 + lane) * 16, src + 16ll * vi);
+    }
+    if (ALIGN != 16 && lane == 0 && v0 + BS_SPAN < held) copy16_async(ring + slot * STAGE + BS_SPAN * 16, src + 16ll * (v0 + BS_SPAN));
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < BS_STAGES - 1; ++i) fetch(min(first + i * step, held), i);      // (held: nothing)
+  int slot = 0;
+  float m = -INFINITY, s = 0.f;
+  // Candidates are above this.  Once the list holds n that is the last one's value: of equal ones the lower tokens came first.
+  float above = -INFINITY;
+  bool low_cut = true;
+  for (int v0 = first; v0 - warp * BS_SPAN < vecs; v0 += step) {      // (as often in every warp: they meet)
+    asm volatile("cp.async.wait_group %0;" ::"n"(BS_STAGES - 2) : "memory");
+    __syncwarp();
+    Held<T> x;
+    const uint32_t mine_at = ring + slot * STAGE + lane * 16 + by;
+#pragma unroll
+    for (int j = 0; j < BS_VECS; ++j) read_words<ALIGN>(x.w + 4 * j, mine_at + j * 512);
+    // (the last chunk's slot: this warp is through with it)
+    fetch(min(v0 + (BS_STAGES - 1) * step, held), slot == 0 ? BS_STAGES - 1 : slot - 1);
+    slot = slot + 1 == BS_STAGES ? 0 : slot + 1;
+    const bool more = v0 - warp * BS_SPAN + step < vecs;
+    // the token of x.at(k)
+    auto token = [&](int k) { return static_cast<uint32_t>((v0 + (k / EV) * 32 + lane) * EV + (k % EV)); };
+    if (v0 + BS_SPAN > V / EV) {                     // behind the row's last token
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (token(k) >= static_cast<uint32_t>(V)) x.mask(k);
+    }
+    // Maximum and sum of exponentials of what the thread holds.  One product and sum an element: 2^(x log2 e - c) with c the rounded m log2 e, and what the
+    // rounding took is put back into the sum.  What is not finite shows up in the maximum or the sum and is masked then; huge values take the longer way.
+    float cm = x.max(), cs = 0.f;
+    if (!(cm >= -INFINITY)) cm = -INFINITY;                  // (NaN alone)
+    if (cm != -INFINITY) {
+      const float c = cm * LOG2E;
+      float2 t[2] = {{0.f, 0.f}, {0.f, 0.f}};
+#pragma unroll
+      for (int k = 0; k < N; k += 2) {
+        const float2 y = fma2(make_float2(x.at(k), x.at(k + 1)), make_float2(LOG2E, LOG2E), make_float2(-c, -c));
+        t[(k >> 1) & 1] = add2(t[(k >> 1) & 1], make_float2(ex2(y.x), ex2(y.y)));
+      }
+      cs = ((t[0].x + t[0].y) + (t[1].x + t[1].y)) * ex2(fmaf(-cm, LOG2E, c));
+      if (!(cs < INFINITY) || !(fabsf(cm) < 1e37f)) {
+#pragma unroll
+        for (int k = 0; k < N; ++k)
+          if (!isfinite(x.at(k))) x.mask(k);
+        cm = x.max();
+        cs = 0.f;
+        if (cm != -INFINITY) {
+#pragma unroll
+          for (int k = 0; k < N; ++k) cs += exp_down(x.at(k) - cm);
+        }
+      }
+      if (cm > m) {
+        s = (m != -INFINITY ? s * exp_down(m - cm) : 0.f) + cs;
+        m = cm;
+      } else if (cm != -INFINITY) {
+        s += cs * exp_down(cm - m);
       }
     }
+    if (low_cut) {
+      if (!__syncthreads_or(cm != -INFINITY)) continue;      // (a masked stretch)
+      // A cut of the chunk's own while the list is short of n: at least n threads' maxima are not below it, found from the largest one down by steps that
+      // double, then by halving.  Little more than n elements are above it.
+      const uint32_t key = order_f32(cm);
+      const uint32_t wtop = __reduce_max_sync(0xffffffffu, key);
+      if (lane == 0) sh.tops[warp] = wtop;
+      __syncthreads();
+      uint32_t lo = __reduce_max_sync(0xffffffffu, sh.tops[lane & 7]), hi = lo + 1u, step = 1u << 20;
+      int got;
+      for (;;) {
+        lo = lo > step ? lo - step : 1u;
+        step <<= 1;
+        got = __syncthreads_count(key >= lo);
+        if (got >= n || lo == 1u) break;
+        hi = lo;
+      }
+      while (got > n + n / 4 + 2 && hi - lo > 1u) {
+        const uint32_t mid = lo + ((hi - lo) >> 1);
+        const int c = __syncthreads_count(key >= mid);
+        if (c >= n) lo = mid, got = c;
+        else hi = mid;
+      }
+      const uint32_t under = lo - 1u;                       // (the next value below; 0x7fffffff would be -0, which is none)
+      above = lo <= 0x00800000u ? -INFINITY : unorder_f32(under - (under == 0x7fffffffu ? 1u : 0u));
+    }
+    // What few threads do they do one element after the other, from shared memory: unrolled it took registers from the stream.  An element as one number: its
+    // value, then the lower token first.
+    auto keyed = [&](int k) {
+      const uint32_t from = mine_at + (k / EV) * 512 + (k % EV) * sizeof(T);
+      uint32_t w;
+      if (sizeof(T) == 4) {
+        asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(from) : "memory");
+      } else {
+        uint16_t h;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(from) : "memory");
+        w = static_cast<uint32_t>(h) << 16;
+      }
+      const uint32_t o = order_f32(__uint_as_float(w));
+      return o && token(k) < static_cast<uint32_t>(V) ? (static_cast<uint64_t>(o) << 32 | (0xffffffffu - token(k))) : 0ull;
+    };
+    bool full = low_cut && more;
+    if (cm > above) {
+      uint32_t hits = 0u;
 #pragma unroll
-    for (int i = 0; i < NV; ++i) x.w[4 * i] = q[i].x, x.w[4 * i + 1] = q[i].y, x.w[4 * i + 2] = q[i].z, x.w[4 * i + 3] = q[i].w;
-  }
-  // the token of x.at(k)
-  auto token = [&](int k) { return static_cast<uint32_t>((v0 + (k / EV) * BS_THREADS + tid) * EV + (k % EV)); };
-  if (V % EV && v0 + BS_SLICE / EV >= vecs) {               // behind the row's last token
+      for (int k = 0; k < N; ++k) hits |= x.at(k) > above ? 1u << k : 0u;
+      uint32_t i = atomicAdd(&count, static_cast<uint32_t>(__popc(hits)));
+      for (; hits; hits &= hits - 1u, ++i) {
+        if (i < BS_CAP) list[i] = keyed(__ffs(hits) - 1);
+        full |= i >= BS_CAP / 4;
+      }
+    }
+    if (!__syncthreads_or(full)) continue;
+    int c = static_cast<int>(count);
+    if (c > BS_CAP) {      // many equal or rising values: of the list and this chunk together those above a cut that leaves at least n, found by halving
+      uint64_t mine_l[BS_CAP / BS_THREADS];
+      const uint32_t start = 0xffffffffu - static_cast<uint32_t>(v0 - warp * BS_SPAN) * EV;
 #pragma unroll
-    for (int k = 0; k < 32; ++k)
-      if (token(k) >= static_cast<uint32_t>(V)) x.mask(k);
+      for (int e = 0; e < BS_CAP / BS_THREADS; ++e) {
+        const uint64_t key = list[tid + e * BS_THREADS];
+        mine_l[e] = static_cast<uint32_t>(key) > start ? key : 0ull;      // (of earlier chunks)
+      }
+      int turn = 0, found = c;
+      // by values
+      uint32_t lo = above == -INFINITY ? 1u : order_f32(above) + 1u, hi = ~0u;      // at least n are >= lo, fewer than n are >= hi
+      while (found > BS_CAP / 4 && hi - lo > 1u) {
+        const uint32_t mid = lo + ((hi - lo) >> 1);
+        const float f = unorder_f32(mid);                      // (NaN and infinity above the largest value: none reaches them)
+        int mine = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) mine += x.at(k) >= f && x.at(k) != INFINITY ? 1 : 0;
+#pragma unroll
+        for (int e = 0; e < BS_CAP / BS_THREADS; ++e) mine += static_cast<uint32_t>(mine_l[e] >> 32) >= mid ? 1 : 0;
+        const int got = block_count(mine, box, turn);
+        if (got >= n) lo = mid, found = got;
+        else hi = mid;
+      }
+      // equal values by tokens
+      uint64_t cut = static_cast<uint64_t>(lo) << 32, end = static_cast<uint64_t>(lo + 1u) << 32;
+      while (found > BS_CAP / 4) {
+        const uint64_t mid = cut + ((end - cut) >> 1);
+        int mine = 0;
+#pragma unroll 4
+        for (int k = 0; k < N; ++k) mine += keyed(k) >= mid ? 1 : 0;
+#pragma unroll
+        for (int e = 0; e < BS_CAP / BS_THREADS; ++e) mine += mine_l[e] >= mid ? 1 : 0;
+        const int got = block_count(mine, box, turn);
+        if (got >= n) cut = mid, found = got;
+        else end = mid;
+      }
+      __syncthreads();
+      if (tid == 0) count = 0u;
+      __syncthreads();
+#pragma unroll 1
+      for (int k = 0; k < N; ++k) {
+        const uint64_t key = keyed(k);
+        if (key >= cut) list[atomicAdd(&count, 1u)] = key;
+      }
+#pragma unroll
+      for (int e = 0; e < BS_CAP / BS_THREADS; ++e)
+        if (mine_l[e] >= cut) list[atomicAdd(&count, 1u)] = mine_l[e];
+      if (tid < 3) box[tid] = 0u;
+      __syncthreads();
+      c = static_cast<int>(count);
+    }
+    keep_largest(list, c, n);
+    if (tid == 0) count = min(c, n);
+    if (c >= n) above = unorder_f32(static_cast<uint32_t>(list[n - 1] >> 32)), low_cut = false;
+    __syncthreads();
   }
 
-  // Maximum and sum of exponentials, each thread's own first.  One product and sum an element: 2^(x log2 e - c) with c the rounded m log2 e, and what the
-  // rounding took is put back into the sum.  What is not finite shows up in the maximum or the sum and is masked then; huge values take the longer way.
-  auto maximum = [&]() {
-    float m = x.at(0);
-#pragma unroll
-    for (int k = 1; k < 32; ++k) m = fmaxf(m, x.at(k));
-    return m;
-  };
-  float m = maximum(), s = 0.f;
-  if (m != -INFINITY) {
-    const float c = m * LOG2E;
-    float t[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int k = 0; k < 32; ++k) t[k & 3] += ex2(fmaf(x.at(k), LOG2E, -c));
-    s = (t[0] + t[1]) + (t[2] + t[3]);
-    s *= ex2(fmaf(-m, LOG2E, c));
-  }
-  bool odd = !(s < INFINITY) || !(fabsf(m) < 1e37f);
-  if (m == -INFINITY) {                                     // (masked all, or NaN)
-    odd = false;
-#pragma unroll
-    for (int k = 0; k < 32; ++k) odd |= x.at(k) != x.at(k);
-  }
-  if (odd) {
-#pragma unroll
-    for (int k = 0; k < 32; ++k)
-      if (!isfinite(x.at(k))) x.mask(k);
-    m = maximum();
-    s = 0.f;
-    if (m != -INFINITY) {
-#pragma unroll
-      for (int k = 0; k < 32; ++k) s += exp_down(x.at(k) - m);
-    }
-  }
+  asm volatile("cp.async.wait_all;" ::: "memory");          // (empty groups: nothing is on its way)
   const float wm = warp_max(m);
   const float ws = warp_sum(m != -INFINITY ? s * exp_down(m - wm) : 0.f);
   if (lane == 0) part_m[warp] = wm, part_s[warp] = ws;
-  // A first cut: of at least n groups of threads each has an element that is not below the smallest of the groups' maxima.  Groups of 256 / G
-  // neighbours, whose elements are spread over the whole slice.
-  const int G = n <= 8 ? 8 : n <= 16 ? 16 : n <= 32 ? 32 : 64;
-  float gm = m;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1)
-    if (o < BS_THREADS / G) gm = fmaxf(gm, __shfl_xor_sync(0xffffffffu, gm, o));
-  if ((tid & (BS_THREADS / G - 1)) == 0) groups[tid / (BS_THREADS / G)] = gm;
   __syncthreads();
   if (warp == 0) {
-    float low = lane < G ? groups[lane] : INFINITY;
-    if (G == 64) low = fminf(low, groups[lane + 32]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
-    if (lane == 0) cut_s = fmaxf(low, -3.4028235e38f);
-  }
-  if (warp == 1) {
     const float pm = lane < 8 ? part_m[lane] : -INFINITY;
     const float top = warp_max(pm);
     const float sum = warp_sum(pm != -INFINITY ? part_s[lane & 7] * exp_down(pm - top) : 0.f);
-    if (lane == 0) stats[blockIdx.x] = {top, top == -INFINITY ? 0.f : sum};
+    if (lane == 0) *stats = {top, top == -INFINITY ? 0.f : sum};
   }
-  __syncthreads();
-  // an element as one number: its value, then the lower token first
-  auto keyed = [&](int k) {
-    const uint32_t o = order_f32(x.at(k));
-    return o ? (static_cast<uint64_t>(o) << 32 | (0xffffffffu - token(k))) : 0ull;
-  };
-  const float cut_f = cut_s;
-  if (m >= cut_f) {
-#pragma unroll
-    for (int k = 0; k < 32; ++k)
-      if (x.at(k) >= cut_f) {
-        const uint32_t i = atomicAdd(&count, 1u);
-        if (i < BS_CAP) list[i] = keyed(k);
-      }
-  }
-  __syncthreads();
-  int found = static_cast<int>(count);
-  if (found > BS_CAP) {      // many equal or nearly equal values, or a group without any: halve the range until the list holds them
-    uint64_t lo = static_cast<uint64_t>(order_f32(cut_f)) << 32, hi = ~0ull;
-    int turn = 0;
-    while (found > BS_CAP) {                                  // at least n are >= lo, fewer than n are >= hi
-      const uint64_t mid = lo + ((hi - lo) >> 1);
-      int mine = 0;
-#pragma unroll
-      for (int k = 0; k < 32; ++k) mine += keyed(k) >= mid ? 1 : 0;
-      const int c = block_count(mine, box, turn);
-      if (c >= n) lo = mid, found = c;
-      else hi = mid;
-    }
-    if (tid == 0) count = 0u;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 32; ++k) {
-      const uint64_t key = keyed(k);
-      if (key >= lo) list[atomicAdd(&count, 1u)] = key;
-    }
-    __syncthreads();
-  }
-  // every key's place in the order is the number of larger ones (they differ)
-  uint64_t* out = best + static_cast<long long>(blockIdx.x) * n;
-  for (int i = tid; i < found; i += BS_THREADS) {
-    const uint64_t key = list[i];
-    int rank = 0;
-    for (int j = 0; j < found; ++j) rank += list[j] > key ? 1 : 0;
-    if (rank < n) out[rank] = key;
-  }
-  for (int i = found + tid; i < n; i += BS_THREADS) out[i] = 0ull;
+  const int c = static_cast<int>(count);
+  keep_largest(list, c, n);
+  if (tid < n) best[tid] = tid < c ? list[tid] : 0ull;
 }
 
-constexpr int BJ_THREADS = 512, BJ_CAP = 512;
+template <typename T>
+__global__ void __launch_bounds__(BS_THREADS, BS_BLOCKS) beam_part_kernel(BeamStats* __restrict__ stats, uint64_t* __restrict__ best, const T* __restrict__ logits,
+                                                                          long long stride, int V, int parts, const float* score, const float* weight,
+                                                                          const uint8_t* ended, int n) {
+  extern __shared__ __align__(16) uint8_t bs_raw[];
+  PartShared& sh = *reinterpret_cast<PartShared*>(bs_raw);
+  const int row = blockIdx.x / parts, part = blockIdx.x - row * parts;
+  if (threadIdx.x == 0) sh.box[0] = sh.box[1] = sh.box[2] = sh.count = 0u;
+  pdl_sync();
+  if (!beam_reads(score, weight, ended, row)) return;       // (the second kernel does not look at this row either)
+  __syncthreads();
+  const uint8_t* at = reinterpret_cast<const uint8_t*>(logits + static_cast<long long>(row) * stride);
+  const int by = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15);
+  BeamStats* st = stats + blockIdx.x;
+  uint64_t* out = best + static_cast<long long>(blockIdx.x) * n;
+  if (by == 0) beam_part<T, 16>(sh, st, out, at, V, part, parts, n);
+  else if (by == 8) beam_part<T, 8>(sh, st, out, at, V, part, parts, n);
+  else if (sizeof(T) == 4 || by % 4 == 0) beam_part<T, 4>(sh, st, out, at, V, part, parts, n);
+  else beam_part<T, sizeof(T)>(sh, st, out, at, V, part, parts, n);
+}
 
-// The n best of one request.  Candidate c of its W * slices * n: row, slice, place.
+// The n best of one request.  Candidate c of its W * parts * n: beam, part, place; its rank stands in shared memory (in registers, unrolled, the code took longer
+// to arrive than to run).
 __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(float* __restrict__ out_score, int32_t* __restrict__ out_parent, int64_t* __restrict__ out_token,
                                                                uint8_t* __restrict__ out_ended, const BeamStats* __restrict__ stats,
                                                                const uint64_t* __restrict__ best, const float* score, const float* weight,
-                                                               const uint8_t* ended, int W, int slices, int n, long long end_token) {
-  __shared__ double base[BS_MAX_W], tops[BS_MAX_W], by[BS_MAX_W];      // total = (x - top) + base: a row may hold nothing but lowest values; base of an ended beam: its score
+                                                               const uint8_t* ended, int W, int parts, int n, long long end_token) {
+  constexpr int CAP = BS_MAX_N + 32;
+  extern __shared__ uint64_t bj_key[];                 // [W * parts * n] ranks as ordered numbers, 0: none; behind them the candidates
+  // total = (x - top) + base: a row may hold nothing but lowest values; base of an ended beam: its score
+  __shared__ double base[BS_MAX_W], tops[BS_MAX_W];
   __shared__ uint8_t kind[BS_MAX_W];                   // 0: no candidates, 1: logits, 2: ended
-  __shared__ uint64_t list_key[BJ_CAP], list_at[BJ_CAP];      // rank, (beam, token)
-  __shared__ double list_total[BJ_CAP];
+  __shared__ uint64_t list_key[CAP], list_at[CAP], warp_most[BJ_THREADS / 32];      // rank, (beam, token)
+  __shared__ double list_total[CAP];
   __shared__ uint32_t box[3], count;
+  __shared__ int bins[BJ_BINS], warp_sum_s[BJ_THREADS / 32], box_bin, box_upto;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x;
+  const int per_row = parts * n, all = W * per_row;
+  uint64_t* bj_e = bj_key + all;
+  const uint64_t* mine_of = best + static_cast<long long>(b) * all;
   if (tid == 0) box[0] = box[1] = box[2] = count = 0u;
   pdl_sync();
-  for (int w = warp; w < W; w += BJ_THREADS / 32) {
+  auto total_of = [&](int w, uint64_t e) { return kind[w] == 2 ? base[w] : (static_cast<double>(unorder_f32(static_cast<uint32_t>(e >> 32))) - tops[w]) + base[w]; };
+  auto place_of = [&](int w, uint64_t e) {
+    return static_cast<uint64_t>(w) << 32 | (kind[w] == 2 ? static_cast<uint32_t>(end_token) : 0xffffffffu - static_cast<uint32_t>(e));
+  };
+  uint64_t most = 0ull;
+  int mine = 0;
+  for (int w = warp; w < W; w += BJ_THREADS / 32) {    // a warp a beam
     const int row = b * W + w;
     const float s = score[row], f = weight ? weight[row] : 1.f;
     const bool over = ended && ended[row];
-    int k = over ? 2 : 1;
-    if (!isfinite(s) || !isfinite(f) || !(f > 0.f)) k = 0;
+    const BeamStats t0 = lane < parts ? stats[row * parts + lane] : BeamStats{-INFINITY, 0.f};      // (of a row that was not read: anything)
+    int k = !isfinite(s) || !isfinite(f) || !(f > 0.f) ? 0 : over ? 2 : 1;
+    uint64_t e[4] = {0ull, 0ull, 0ull, 0ull};          // (the first of its candidates, on their way meanwhile)
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      if (lane + 32 * i < per_row) e[i] = mine_of[w * per_row + lane + 32 * i];
     double log_sum = 0.0, peak = 0.0;
     if (k == 1) {
-      float top = -INFINITY;
-      for (int i = lane; i < slices; i += 32) top = fmaxf(top, stats[row * slices + i].m);
+      float top = t0.m;
+      for (int i = lane + 32; i < parts; i += 32) top = fmaxf(top, stats[row * parts + i].m);
       top = warp_max(top);
-      double sum = 0.0;
-      for (int i = lane; i < slices; i += 32) {
-        const BeamStats t = stats[row * slices + i];
+      double sum = t0.m == -INFINITY ? 0.0 : static_cast<double>(t0.s) * exp(static_cast<double>(t0.m) - static_cast<double>(top));
+      for (int i = lane + 32; i < parts; i += 32) {
+        const BeamStats t = stats[row * parts + i];
         if (t.m != -INFINITY) sum += static_cast<double>(t.s) * exp(static_cast<double>(t.m) - static_cast<double>(top));
       }
 #pragma unroll
@@ -289,71 +440,117 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(float* __restrict
       if (top == -INFINITY) k = 0;                       // everything masked: nothing to go on with
       else peak = top, log_sum = log(sum);
     }
-    if (lane == 0) base[w] = static_cast<double>(s) - log_sum, tops[w] = peak, by[w] = f, kind[w] = k;
+    if (lane == 0) base[w] = static_cast<double>(s) - log_sum, tops[w] = peak, kind[w] = k;
+    __syncwarp();
+    for (int j = lane, i = 0; j < per_row; j += 32, ++i) {
+      uint64_t c = 0ull, key = 0ull;
+      if (k == 1) c = i == 0 ? e[0] : i == 1 ? e[1] : i == 2 ? e[2] : i == 3 ? e[3] : mine_of[w * per_row + j];
+      // (an ended beam's one candidate stands in its first place; what the memory holds there is not looked at)
+      if (k == 2 ? j == 0 : c != 0ull) key = order_f64(total_of(w, c) * static_cast<double>(f));
+      bj_key[w * per_row + j] = key;
+      bj_e[w * per_row + j] = c;
+      mine += key != 0ull;
+      most = max(most, key);
+    }
   }
-  __syncthreads();
-
-  const int per_row = slices * n, all = W * per_row;
-  auto key_of = [&](int c, uint64_t& at, double& total) -> uint64_t {
-    const int w = c / per_row;
-    if (kind[w] != 1) {
-      if (kind[w] == 0 || c != w * per_row) return 0ull;
-      at = static_cast<uint64_t>(w) << 32 | static_cast<uint64_t>(end_token);
-      total = base[w];
-    } else {
-      const uint64_t e = best[static_cast<long long>(b) * all + c];
-      if (!e) return 0ull;
-      at = static_cast<uint64_t>(w) << 32 | (0xffffffffu - static_cast<uint32_t>(e));
-      total = (static_cast<double>(unorder_f32(static_cast<uint32_t>(e >> 32))) - tops[w]) + base[w];
-    }
-    return order_f64(total * by[w]);
-  };
-  // All candidates if the list holds them, else those above a cut that leaves at least n: found by halving the range, first of ranks, then (equal ranks)
-  // of places.
-  int turn = 0;
-  auto count_from = [&](uint64_t cut, uint64_t tie) {
-    int mine = 0;
-    for (int c = tid; c < all; c += BJ_THREADS) {
-      uint64_t at;
-      double total;
-      const uint64_t key = key_of(c, at, total);
-      mine += key > cut || (key == cut && key && at <= tie) ? 1 : 0;
-    }
-    return block_count(mine, box, turn);
-  };
+  // All candidates if the list holds them, else those above a cut that leaves at least n.  Candidates are counted by their distance from the largest, 16 bins
+  // to every doubling of it; what a bin holds too much of (equal or nearly equal ranks) is found by halving, first of ranks, then of places.
+  int turn = 0, found = block_count(mine, box, turn);    // (its barrier: keys and totals are there)
   uint64_t cut = 1ull, tie = ~0ull;
-  int found = count_from(cut, tie);
-  if (found > BJ_CAP) {
-    uint64_t lo = 1ull, hi = ~0ull;
-    while (found > BJ_CAP && hi - lo > 1ull) {
+  const int room = n + 32;
+  if (found > room) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
+    if (lane == 0) warp_most[warp] = most;
+    for (int i = tid; i < BJ_BINS; i += BJ_THREADS) bins[i] = 0;
+    __syncthreads();
+    uint64_t top = 0ull;
+#pragma unroll
+    for (int i = 0; i < BJ_THREADS / 32; ++i) top = max(top, warp_most[i]);
+    const double best_rank = unorder_f64(top);
+    auto bin_of = [&](uint64_t key) {                       // (monotone: the same subtraction and conversion for all)
+      const int i = static_cast<int>(__float_as_uint(static_cast<float>(best_rank - unorder_f64(key))) >> 19) - (104 << 4);
+      return i < 0 ? 0 : i < BJ_BINS ? i : BJ_BINS - 1;
+    };
+#pragma unroll 2
+    for (int c = tid; c < all; c += BJ_THREADS)
+      if (bj_key[c]) atomicAdd(&bins[bin_of(bj_key[c])], 1);
+    __syncthreads();
+    // the bin in which the n-th is: two bins a thread
+    const int b0 = bins[2 * tid], b1 = bins[2 * tid + 1];
+    int upto = b0 + b1;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += v;
+    }
+    if (lane == 31) warp_sum_s[warp] = upto;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < BJ_THREADS / 32; ++i)
+      if (i < warp) upto += warp_sum_s[i];
+    if (upto >= n && upto - b0 - b1 < n) {                  // (one thread)
+      const bool second = upto - b1 < n;
+      box_bin = 2 * tid + second, box_upto = second ? upto : upto - b1;
+    }
+    __syncthreads();
+    const int last = box_bin;
+    found = box_upto;
+    if (found <= room) {
+      // the lowest rank of the bins that count: what is below stays out
+      uint64_t least = ~0ull;
+#pragma unroll 2
+      for (int c = tid; c < all; c += BJ_THREADS)
+        if (bj_key[c] && bin_of(bj_key[c]) <= last) least = min(least, bj_key[c]);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
+      if (lane == 0) warp_most[warp] = least;
+      __syncthreads();
+      cut = ~0ull;
+#pragma unroll
+      for (int i = 0; i < BJ_THREADS / 32; ++i) cut = min(cut, warp_most[i]);
+    }
+    auto count_from = [&](uint64_t from) {
+      int m = 0;
+#pragma unroll 4
+      for (int c = tid; c < all; c += BJ_THREADS) m += bj_key[c] >= from;
+      return block_count(m, box, turn);
+    };
+    uint64_t lo = cut, hi = top + 1ull;
+    while (found > room && hi - lo > 1ull) {
       const uint64_t mid = lo + ((hi - lo) >> 1);
-      const int c = count_from(mid, tie);
+      const int c = count_from(mid);
       if (c >= n) lo = mid, found = c;
       else hi = mid;
     }
     cut = lo;
     uint64_t below = 0ull;                                  // (places of equal ranks: the fewest of the first ones that are enough)
-    while (found > BJ_CAP) {
+    while (found > room) {
       const uint64_t mid = below + ((tie - below) >> 1);
-      const int c = count_from(cut, mid);
+      mine = 0;
+#pragma unroll 1
+      for (int c = tid; c < all; c += BJ_THREADS) mine += bj_key[c] > cut || (bj_key[c] == cut && place_of(c / per_row, bj_e[c]) <= mid);
+      const int c = block_count(mine, box, turn);
       if (c >= n) tie = mid, found = c;
       else below = mid + 1ull;
     }
   }
+#pragma unroll 1
   for (int c = tid; c < all; c += BJ_THREADS) {
-    uint64_t at;
-    double total;
-    const uint64_t key = key_of(c, at, total);
-    if (key > cut || (key == cut && at <= tie)) {
-      const uint32_t i = atomicAdd(&count, 1u);
-      list_key[i] = key, list_at[i] = at, list_total[i] = total;
-    }
+    const uint64_t key = bj_key[c];
+    if (key < cut) continue;
+    const int w = c / per_row;
+    const uint64_t e = bj_e[c], at = place_of(w, e);
+    if (key == cut && at > tie) continue;
+    const uint32_t o = atomicAdd(&count, 1u);
+    list_key[o] = key, list_at[o] = at, list_total[o] = total_of(w, e);
   }
   __syncthreads();
   for (int i = tid; i < found; i += BJ_THREADS) {
-    const uint64_t key = list_key[i], at = list_at[i];
+    const uint64_t k = list_key[i], at = list_at[i];
     int rank = 0;
-    for (int j = 0; j < found; ++j) rank += list_key[j] > key || (list_key[j] == key && list_at[j] < at) ? 1 : 0;
+#pragma unroll 8
+    for (int j = 0; j < found; ++j) rank += list_key[j] > k || (list_key[j] == k && list_at[j] < at) ? 1 : 0;
     if (rank < n) {
       const int w = static_cast<int>(at >> 32), o = b * n + rank;
       const uint32_t v = static_cast<uint32_t>(at);
@@ -432,15 +629,24 @@ __global__ void __launch_bounds__(BR_THREADS) beam_reorder_kernel(const __grid_c
   }
 }
 
-inline long long beam_slices(long long vocab) { return (vocab + BS_SLICE - 1) / BS_SLICE; }
+// Parts of a row: as many blocks as run at a time, of equally many chunks, and no more candidates of a request than the second kernel holds.
+static int beam_parts(int requests, int width, int vocab, int n, int elem) {
+  const int chunk = BS_THREADS * BS_VECS * 16 / elem, chunks = (vocab + chunk - 1) / chunk;
+  const long long rows = static_cast<long long>(requests) * width, blocks = static_cast<long long>(sm_count()) * BS_BLOCKS / rows;
+  int parts = static_cast<int>(blocks < 1 ? 1 : blocks < chunks ? blocks : chunks);
+  const int most = BJ_ALL / (width * n);
+  if (parts > most) parts = most;
+  const int each = (chunks + parts - 1) / parts;
+  return (chunks + each - 1) / each;
+}
 
 }  // namespace vb
 
 using namespace vb;
 
-extern "C" size_t vb_beam_select_workspace_bytes(int requests, int width, int vocab, int n) {
-  if (requests <= 0 || width <= 0 || vocab <= 0 || n <= 0) return 0;
-  return static_cast<size_t>(requests) * width * beam_slices(vocab) * (sizeof(BeamStats) + 8ull * n);
+extern "C" size_t vb_beam_select_workspace_bytes(int requests, int width, int vocab, int n, int logits_f32) {
+  if (requests <= 0 || width <= 0 || width > BS_MAX_W || vocab <= 0 || n <= 0 || n > BS_MAX_N) return 0;
+  return static_cast<size_t>(requests) * width * beam_parts(requests, width, vocab, n, logits_f32 ? 4 : 2) * (sizeof(BeamStats) + 8ull * n);
 }
 
 extern "C" int vb_beam_select(float* d_score, int32_t* d_parent, int64_t* d_token, uint8_t* d_out_ended, const void* d_logits, int64_t row_stride, int logits_f32,
@@ -454,20 +660,23 @@ extern "C" int vb_beam_select(float* d_score, int32_t* d_parent, int64_t* d_toke
   VB_CHECK_ARG(row_stride >= 0, "vb_beam_select: row stride %lld", static_cast<long long>(row_stride));
   VB_CHECK_ARG(!(d_ended || d_out_ended) || (end_token >= 0 && end_token < vocab), "vb_beam_select: end token %lld outside the vocabulary of %d",
                static_cast<long long>(end_token), vocab);
-  const long long slices = beam_slices(vocab), blocks = static_cast<long long>(requests) * width * slices;
-  VB_CHECK_ARG(blocks <= 0x7fffffffll && blocks * n / requests <= 0x7fffffffll, "vb_beam_select: %lld slices of rows", blocks);
-  VB_CHECK_ARG(workspace_bytes >= vb_beam_select_workspace_bytes(requests, width, vocab, n) && reinterpret_cast<uintptr_t>(d_workspace) % 8 == 0,
+  const int parts = beam_parts(requests, width, vocab, n, logits_f32 ? 4 : 2);
+  const long long blocks = static_cast<long long>(requests) * width * parts;
+  VB_CHECK_ARG(blocks <= 0x7fffffffll && static_cast<long long>(requests) * n <= 0x7fffffffll, "vb_beam_select: %lld parts of rows", blocks);
+  VB_CHECK_ARG(workspace_bytes >= vb_beam_select_workspace_bytes(requests, width, vocab, n, logits_f32) && reinterpret_cast<uintptr_t>(d_workspace) % 8 == 0,
                "vb_beam_select: workspace of %zu bytes", workspace_bytes);
   uint64_t* best = static_cast<uint64_t*>(d_workspace);
   BeamStats* stats = reinterpret_cast<BeamStats*>(best + blocks * n);
+  VB_CHECK_CUDA(logits_f32 ? rm_smem<beam_part_kernel<float>>(sizeof(PartShared)) : rm_smem<beam_part_kernel<__nv_bfloat16>>(sizeof(PartShared)));
   if (logits_f32)
-    VB_LAUNCH_PDL(beam_slice_kernel<float>, static_cast<unsigned>(blocks), BS_THREADS, 0, stream, stats, best, static_cast<const float*>(d_logits),
-                  static_cast<long long>(row_stride), vocab, static_cast<int>(slices), d_beam_score, d_weight, d_ended, n);
+    VB_LAUNCH_PDL(beam_part_kernel<float>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, stats, best, static_cast<const float*>(d_logits),
+                  static_cast<long long>(row_stride), vocab, parts, d_beam_score, d_weight, d_ended, n);
   else
-    VB_LAUNCH_PDL(beam_slice_kernel<__nv_bfloat16>, static_cast<unsigned>(blocks), BS_THREADS, 0, stream, stats, best, static_cast<const __nv_bfloat16*>(d_logits),
-                  static_cast<long long>(row_stride), vocab, static_cast<int>(slices), d_beam_score, d_weight, d_ended, n);
-  VB_LAUNCH_PDL(beam_join_kernel, static_cast<unsigned>(requests), BJ_THREADS, 0, stream, d_score, d_parent, d_token, d_out_ended, stats, best, d_beam_score, d_weight,
-                d_ended, width, static_cast<int>(slices), n, static_cast<long long>(end_token));
+    VB_LAUNCH_PDL(beam_part_kernel<__nv_bfloat16>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, stats, best, static_cast<const __nv_bfloat16*>(d_logits),
+                  static_cast<long long>(row_stride), vocab, parts, d_beam_score, d_weight, d_ended, n);
+  VB_CHECK_CUDA(rm_smem<beam_join_kernel>(BJ_ALL * 16));
+  VB_LAUNCH_PDL(beam_join_kernel, static_cast<unsigned>(requests), BJ_THREADS, static_cast<size_t>(width) * parts * n * 16, stream, d_score, d_parent, d_token, d_out_ended, stats, best, d_beam_score, d_weight,
+                d_ended, width, parts, n, static_cast<long long>(end_token));
   return 0;
 }
 

@@ -2221,6 +2221,11 @@ def moe_layer(h: torch.Tensor, weights: MoeWeights, router: MoeRouter, ids: Opti
 BEAM_MAX_WIDTH, BEAM_MAX_N = 32, 64
 
 
+@lru_cache(maxsize=1024)
+def _beam_ws(B: int, W: int, V: int, n: int, f32: bool) -> int:
+    return _lib.load().vb_beam_select_workspace_bytes(B, W, V, n, int(f32))
+
+
 class BeamStep(NamedTuple):
     """What ``beam_select`` chose, [requests, n] in order: totals (fp32), the beam of the request each came from (int32), its token (int64), and whether it has
     ended (bool; None without an end token).  Where a request has fewer candidates: -inf, -1, -1, True."""
@@ -2230,18 +2235,10 @@ class BeamStep(NamedTuple):
     ended: Optional[torch.Tensor]
 
 
-def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, weight: Optional[torch.Tensor] = None, ended: Optional[torch.Tensor] = None,
-                end_token: Optional[int] = None) -> BeamStep:
-    """One step of a beam search.  logits [requests * width, vocab] bf16 or fp32 (rows apart by any stride), scores fp32 [requests, width]: the beams' log probabilities so
-    far.  Of all continuations of a request's beams, total[w, v] = scores[w] + log_softmax(logits[w])[v], the n best in order, equal ones by (w, v).
-
-    Logits that are not finite are masked: they are no candidates and have no part in the softmax.  A beam whose score is not finite (-inf: not alive yet, or dead), or that
-    has no logit left, has no candidates.  ``weight`` fp32 [requests, width]: candidates are ranked by weight * total (length to the power -alpha, say; totals come back
-    without it; a weight that is not a finite number above zero: no candidates).  ``ended`` bool [requests, width]: such a beam goes on as it is, as one candidate under
-    ``end_token``; its logits are not read.  width 1 .. 32, n 1 .. 64, vocab up to 2^24."""
+def _beam_select_check(logits, scores, n, weight, ended, end_token) -> None:
+    """raises if something of a call does not fit"""
     _need_here("beam_select", logits, scores, weight, ended)
-    f32 = logits.dtype is F32
-    _refuse(not (f32 or logits.dtype is BF16) or logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1), "beam_select: bf16 or fp32 rows of logits are needed")
+    _refuse(logits.dtype not in (F32, BF16) or logits.dim() != 2 or (logits.stride(1) != 1 and logits.shape[1] > 1), "beam_select: bf16 or fp32 rows of logits are needed")
     _refuse(scores.dtype is not F32 or scores.dim() != 2 or not scores.is_contiguous(), "beam_select: fp32 scores [requests, width] are needed")
     B, W = scores.shape
     R, V = logits.shape
@@ -2253,15 +2250,48 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, weight: Opti
         _refuse(ended.dtype is not torch.bool or ended.shape != scores.shape or not ended.is_contiguous(), f"beam_select: ended beams are bool [{B}, {W}]")
         _refuse(end_token is None, "beam_select: beams that have ended go on under an end token: end_token is needed")
     _refuse(end_token is not None and not 0 <= end_token < V, f"beam_select: end token {end_token} outside the vocabulary of {V}")
-    lib = _lib._lib or _lib.load()
-    dev = logits.device
-    step = BeamStep(torch.empty((B, n), dtype=F32, device=dev), torch.empty((B, n), dtype=torch.int32, device=dev), torch.empty((B, n), dtype=torch.int64, device=dev),
-                    None if end_token is None else torch.empty((B, n), dtype=torch.bool, device=dev))
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, weight: Optional[torch.Tensor] = None, ended: Optional[torch.Tensor] = None,
+                end_token: Optional[int] = None) -> BeamStep:
+    """One step of a beam search.  logits [requests * width, vocab] bf16 or fp32 (rows apart by any stride), scores fp32 [requests, width]: the beams' log probabilities so
+    far.  Of all continuations of a request's beams, total[w, v] = scores[w] + log_softmax(logits[w])[v], the n best in order, equal ones by (w, v).
+
+    Logits that are not finite are masked: they are no candidates and have no part in the softmax.  A beam whose score is not finite (-inf: not alive yet, or dead), or that
+    has no logit left, has no candidates.  ``weight`` fp32 [requests, width]: candidates are ranked by weight * total (length to the power -alpha, say; totals come back
+    without it; a weight that is not a finite number above zero: no candidates).  ``ended`` bool [requests, width]: such a beam goes on as it is, as one candidate under
+    ``end_token``; its logits are not read.  width 1 .. 32, n 1 .. 64, vocab up to 2^24."""
+    dev, s, z = _device_index(), scores.shape, logits.shape
+    dtype = logits.dtype
+    # (one comparison per fact when all of them hold; what does not says so in the check)
+    if not (len(s) == len(z) == 2 and (dtype is BF16 or dtype is F32) and scores.dtype is F32 and logits.get_device() == scores.get_device() == dev and z[0] == s[0] * s[1] > 0
+            and s[1] <= BEAM_MAX_WIDTH and 1 <= n <= BEAM_MAX_N and 1 <= z[1] <= 1 << 24 and logits.stride(1) == 1 and scores.is_contiguous() and weight is None and ended is None
+            and (end_token is None or 0 <= end_token < z[1])):
+        _beam_select_check(logits, scores, n, weight, ended, end_token)
+    (B, W), (R, V), f32, on = s, z, dtype is F32, logits.device
+    step = BeamStep(torch.empty((B, n), dtype=F32, device=on), torch.empty((B, n), dtype=torch.int32, device=on), torch.empty((B, n), dtype=torch.int64, device=on),
+                    None if end_token is None else torch.empty((B, n), dtype=torch.bool, device=on))
     # (of the allocator's, so that calls on other streams and captured graphs have their own)
-    ws = torch.empty(lib.vb_beam_select_workspace_bytes(B, W, V, n) // 8, dtype=torch.int64, device=dev)
-    call("vb_beam_select", step.scores.data_ptr(), step.parent.data_ptr(), step.token.data_ptr(), _p(step.ended), logits.data_ptr(), logits.stride(0) if R > 1 else V,
-         int(f32), scores.data_ptr(), _p(weight), _p(ended), B, W, V, n, -1 if end_token is None else end_token, ws.data_ptr(), ws.numel() * 8, _stream())
+    n_ws = _beam_ws(B, W, V, n, f32)
+    ws = torch.empty(n_ws // 8, dtype=torch.int64, device=on)
+    call("vb_beam_select", step.scores.data_ptr(), step.parent.data_ptr(), step.token.data_ptr(), None if end_token is None else step.ended.data_ptr(), logits.data_ptr(),
+         logits.stride(0) if R > 1 else V, f32, scores.data_ptr(), _p(weight), _p(ended), B, W, V, n, -1 if end_token is None else end_token, ws.data_ptr(), n_ws, _raw_stream(dev))
     return step
+
+
+def _beam_reorder_check(states, parent, slots) -> None:
+    """raises if something of a call does not fit"""
+    _need_here("beam_reorder", parent, slots, *states)
+    _refuse(parent.dtype is not torch.int32 or parent.dim() != 2 or not parent.is_contiguous(), "beam_reorder: int32 parents [requests, width] are needed")
+    B, W = parent.shape
+    _refuse(B < 1 or B > 65535 or not 1 <= W <= BEAM_MAX_WIDTH, f"beam_reorder: {B} requests (1 to 65535) of {W} beams (1 to {BEAM_MAX_WIDTH})")
+    _refuse(slots is not None and (slots.dtype is not torch.int32 or slots.shape != parent.shape or not slots.is_contiguous()), f"beam_reorder: int32 slots [{B}, {W}] are needed")
+    n_slots = states[0].shape[0] if states and states[0].dim() else 0
+    for t in states:
+        _refuse(t.dim() < 1 or t.shape[0] != n_slots or not t.is_contiguous() or t.numel() == 0, f"beam_reorder: contiguous states of {n_slots} slots are needed, not {tuple(t.shape)}")
+        _refuse(t.nbytes // n_slots >= 1 << 32, "beam_reorder: a row of 4 GB or more")
+    _refuse(len({t.data_ptr() for t in states}) != len(states), "beam_reorder: a state stands in the list twice")
+    _refuse(bool(states) and slots is None and B * W > n_slots, f"beam_reorder: {B} requests of {W} beams in {n_slots} rows")
 
 
 def beam_reorder(states: Sequence[torch.Tensor], parent: torch.Tensor, slots: Optional[torch.Tensor] = None) -> Sequence[torch.Tensor]:
@@ -2269,24 +2299,21 @@ def beam_reorder(states: Sequence[torch.Tensor], parent: torch.Tensor, slots: Op
     slots[b, parent[b, i]] was; parent -1 (or outside the request): the row stays as it is.  states: contiguous tensors [slots, ...] of any types, all of one number of slots
     (of a stack of layers: one each).  slots int32 [requests, width] (None: b * width + i); a slot belongs to one beam: one that is named twice receives either row; one outside
     the states is skipped.  Returns ``states``."""
-    _need_here("beam_reorder", parent, slots, *states)
-    _refuse(parent.dtype is not torch.int32 or parent.dim() != 2 or not parent.is_contiguous(), "beam_reorder: int32 parents [requests, width] are needed")
-    B, W = parent.shape
-    _refuse(B < 1 or B > 65535 or not 1 <= W <= BEAM_MAX_WIDTH, f"beam_reorder: {B} requests (1 to 65535) of {W} beams (1 to {BEAM_MAX_WIDTH})")
-    _refuse(slots is not None and (slots.dtype is not torch.int32 or slots.shape != parent.shape or not slots.is_contiguous()), f"beam_reorder: int32 slots [{B}, {W}] are needed")
-    if not states:
+    dev, by, k = _device_index(), parent.shape, len(states)
+    ok = (parent.get_device() == dev and parent.dtype is torch.int32 and len(by) == 2 and parent.is_contiguous() and 0 < by[0] <= 65535 and 0 < by[1] <= BEAM_MAX_WIDTH
+          and (slots is None or (slots.get_device() == dev and slots.dtype is torch.int32 and slots.shape == by and slots.is_contiguous())))
+    ptrs, sizes, rows = [0] * k, [0] * k, states[0].shape[0] if k and states[0].dim() else 0
+    for i, t in enumerate(states):
+        n = t.nbytes
+        ok = ok and n > 0 and t.shape[0] == rows and t.get_device() == dev and t.is_contiguous()
+        ptrs[i], sizes[i] = t.data_ptr(), n // rows if rows else 0
+    if not ok or len(set(ptrs)) != k or (k and (max(sizes) >= 1 << 32 or (slots is None and by[0] * by[1] > rows))):
+        _beam_reorder_check(states, parent, slots)
+    if not k:
         return states
-    n_slots, ptrs, sizes = states[0].shape[0] if states[0].dim() else 0, [], []
-    for t in states:
-        _refuse(t.dim() < 1 or t.shape[0] != n_slots or not t.is_contiguous() or t.numel() == 0, f"beam_reorder: contiguous states of {n_slots} slots are needed, not {tuple(t.shape)}")
-        ptrs.append(t.data_ptr())
-        sizes.append(t.numel() // n_slots * t.element_size())
-    _refuse(len(set(ptrs)) != len(ptrs), "beam_reorder: a state stands in the list twice")
-    _refuse(max(sizes) >= 1 << 32, "beam_reorder: a row of 4 GB or more")
-    _refuse(slots is None and B * W > n_slots, f"beam_reorder: {B} requests of {W} beams in {n_slots} rows")
-    k = len(ptrs)
-    call("vb_beam_reorder", (ctypes.c_void_p * k)(*ptrs), (ctypes.c_int64 * k)(*sizes), k, n_slots, parent.data_ptr(), _p(slots), B, W, _stream())
-    _lib.launch_counter[0] += (k + 63) // 64 - 1
+    call("vb_beam_reorder", (ctypes.c_void_p * k)(*ptrs), (ctypes.c_int64 * k)(*sizes), k, rows, parent.data_ptr(), _p(slots), by[0], by[1], _raw_stream(dev))
+    if k > 64:
+        _lib.launch_counter[0] += (k - 1) // 64
     return states
 
 
