@@ -976,8 +976,8 @@ int vb_fork_pages(const VbPagePool* pool, const VbPagePool* out, const int32_t* 
                   int n_caches, void* stream);
 int vb_compact_pages(const VbPagePool* pool, const VbPagePool* out, const VbPageCache* caches, int n_caches, void* stream);
 /* Attention of one new token a row over pages that rows share (csrc/shared_attn.cu).  VbSharedPlan (HOST struct): rows in requests of `width`; a page that rows of a
- *   request hold in the same column is read once for (up to 64 / (n_q / n_kv)) of them.  d_buffer: vb_shared_plan_bytes (0: sizes that are refused), 16-byte aligned,
- *   written by vb_shared_plan once a step and by every vb_shared_attn (one stream at a time).  head_dim 64 or 128, page_size a multiple of 16, grid: blocks.
+ *   request hold in the same column is read once for (up to 32, and up to 128 / (n_q / n_kv)) of them.  d_buffer: vb_shared_plan_bytes (0: sizes that are refused), 16-byte aligned,
+ *   written by vb_shared_plan once a step and by every vb_shared_attn (one stream at a time).  head_dim 64 or 128, page_size a multiple of 16, grid: blocks that run at once (two an SM).
  * vb_shared_plan: d_table [rows][columns], d_tokens [rows] (0: a row without tokens, its output is zero); entries that are no page are skipped.
  * vb_shared_attn: q / out [rows][n_q][head_dim] bf16 (out_xt_tile > 0: the tiled layout), d_kv [slabs][2][page_size][n_kv][head_dim] bf16, slab_base = layer * pages. */
 typedef struct {

@@ -143,7 +143,7 @@ def test_caches_are_described(launched):
 
 
 @pytest.mark.parametrize("args", [(0, 1, 4, 16, 2, 1, 64), (6, 4, 4, 16, 2, 1, 64), (6, 3, 0, 16, 2, 1, 64), (6, 3, 16385, 16, 2, 1, 64), (6, 3, 4, 24, 2, 1, 64), (6, 3, 4, 0, 2, 1, 64),
-                                  (6, 3, 4, 4112, 2, 1, 64), (6, 3, 4, 16, 3, 2, 64), (6, 3, 4, 16, 65, 1, 64), (6, 3, 4, 16, 2, 1, 96), (6, 3, 4, 16, 2, 0, 64),
+                                  (6, 3, 4, 4112, 2, 1, 64), (6, 3, 4, 16, 3, 2, 64), (6, 3, 4, 16, 129, 1, 64), (6, 3, 4, 16, 2, 1, 96), (6, 3, 4, 16, 2, 0, 64),
                                   (30000, 3, 16384, 64, 8, 8, 64)])
 def test_plan_sizes(args):
     with pytest.raises(VoxB200Error):
@@ -173,7 +173,7 @@ def test_attn(launched):
 
 
 def test_plan_cuts_requests_evenly():
-    """rows times query heads of a key head: at most 64 to a group, which the buffer's size shows through its groups"""
+    """rows times query heads of a key head: at most 128 to a group, and 32 rows, which the buffer's size shows through its groups"""
     lib = _lib.load()
 
     def size(width, G):
@@ -181,14 +181,14 @@ def test_plan_cuts_requests_evenly():
         return lib.vb_shared_plan_bytes(ctypes.addressof(s))
 
     def expect(rows, sub, groups, mpad):
-        slots = 1 + groups
-        return 16 * groups * sub + 16 + slots * mpad * (64 * 4 + 8) + 4 * (2 * groups + 1 + rows + 2)
-    assert size(5, 16) == expect(5, 3, 2, 64)          # 4 rows would fit: 3 and 2
-    assert size(16, 4) == expect(16, 16, 1, 64)
-    assert size(17, 4) == expect(17, 9, 2, 64)
+        segments = 1 + groups
+        return 16 * groups * sub + 16 * segments + segments * mpad * (64 * 4 + 8) + 4 * (3 * groups + 1 + rows)
+    assert size(9, 16) == expect(9, 5, 2, 80)          # 8 rows would fit: 5 and 4
+    assert size(16, 8) == expect(16, 16, 1, 128)
+    assert size(17, 8) == expect(17, 9, 2, 80)
     assert size(33, 1) == expect(33, 17, 2, 32)
     assert size(8, 2) == expect(8, 8, 1, 16)
-    assert size(1, 64) == expect(1, 1, 1, 64)
+    assert size(1, 128) == expect(1, 1, 1, 128)
 
 
 def test_entry_points_check_by_themselves():

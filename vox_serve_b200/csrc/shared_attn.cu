@@ -3,44 +3,39 @@
 //   out[r] = sum_t softmax_t(q[r] . k[t] / sqrt d) v[t]     over row r's own tokens t
 //
 // What bounds it is the cache that is read.  Rows stand in groups (the rows of a request); of every column of their page table each DIFFERENT page is read
-// once, with the set of rows that hold it, instead of once for every row.  A group's rows times the query heads of a key head, up to 64, are the rows of a
-// matrix product: a tile of keys meets all of them while it is on chip.
+// once, with the set of rows that hold it, instead of once for every row.  A group's rows times the query heads of a key head, up to 128, are the accumulator
+// rows of the tcgen05 core (attn_tc.cuh): a tile of 64 keys meets all of them while it is on chip.
 //
-//   plan (once a step)   a block a group lists its different pages in pieces of 16 to 64 tokens: {place in the cache, position, rows, tokens}; a block deals
-//                        the tiles of all groups and key heads out to one block an SM in equal ranges
-//   attention            a warp fetches the pieces of a tile by TMA into a ring; eight warps, each with 16 rows and a share of a tile's tokens, keep their own
-//                        running maximum, sum and output in registers and meet at the end of a range only
-//   join                 the ranges of a group and head meet
+//   plan (once a step)   a cluster a group lists its different pages in pieces of 16 to 64 tokens {place in the cache, position, rows, tokens}: first the tiles
+//                        that all living rows see whole, then the rest; a block cuts the tiles of every group and key head into segments, two an SM in all
+//   attention            a block a segment: maximum, denominator and unnormalised output of its rows
+//   join                 the segments of a group and head meet, in their order
 //
-// Probabilities enter the second product as two bf16 parts (2^-17): what rounding them to one would add is as large as the rounding of the output.
-#include <cudaTypedefs.h>
-
+// Tiles that are seen whole need no masks.  In the others a row's probability is 0 where it does not see, and 0 times what is not finite is not 0.  So a block
+// whose results are not finite, and that had such tiles, walks its segment again: values that are not finite are taken out on the way, and the rows that see
+// them get them back at the end.  Finite caches never go there; what stands behind a row's last token is cleared in any case.
+// Probabilities enter the second product as two bf16 parts (2^-17).
 #include "../../include/vb_api.h"
 #define VB_PDL_FAMILY 1
+#include "attn_tc.cuh"
 #include "rowmma.cuh"
 
 namespace vb {
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
-
-constexpr int SA_MAX_ROWS = 64;                  // rows of a group times query heads of a key head
-constexpr int SA_WARPS = 8, SA_THREADS = 32 * (SA_WARPS + 1);
-constexpr int SA_RING = 192 * 1024;
-__host__ __device__ constexpr int sa_tile_tokens(int mt) { return mt == 1 ? 128 : 64; }
-inline int sa_row_tiles(int rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+constexpr int SA_MAX_ROWS = 128;                 // rows of a group times query heads of a key head
 inline int sa_piece(int page_size) { return page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : 16; }
 
 // ---- the plan -------------------------------------------------------------------------------------------------------------------
 struct SharedPlanParams {
-  int4* entries;                 // [groups][cap]: {token's place in a layer's pages, its position, rows that hold it, tokens | seen whole by all rows << 16}
-  int32_t *counts, *tile0, *len; // [groups], [groups + 1], [rows]
-  int4* parts;                   // [grid] {group, head, tile, tiles}
-  int32_t* head;                 // {tiles of a block, tiles of all groups}
+  int4* entries;                 // [groups][cap]: {token's place in a layer's pages, its position, rows that hold it, tokens}
+  int4* segments;                // [grid + units] {group, head, first tile, tiles}
+  int32_t *counts, *whole, *len; // [groups] pieces and tiles that are seen whole, [rows]
+  int32_t* seg0;                 // [units + 1] segments in front of a unit
   const int32_t *table, *tokens;
   int rows, width, sub, subs, groups, cap, columns, pages, page_size, piece, tile_pieces, heads, grid;
 };
 
-constexpr int SP_THREADS = 512, SP_MAX_COLUMNS = 16384;
+constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32, SP_MAX_COLUMNS = 16384, SP_CLUSTER = 8;
 
 __device__ __forceinline__ int shared_first_row(const SharedPlanParams& p, int g, int& n) {
   const int in = g % p.subs * p.sub;
@@ -48,18 +43,38 @@ __device__ __forceinline__ int shared_first_row(const SharedPlanParams& p, int g
   return g / p.subs * p.width + in;
 }
 
-// lane: row.  What its column c holds: the page (-1: none) and how many of the row's tokens stand there
-__device__ __forceinline__ int shared_page(const SharedPlanParams& p, const int32_t* row, int len, int c, int& tokens) {
-  tokens = min(p.page_size, len - c * p.page_size);
-  if (tokens <= 0) return -1;
-  const int g = row[c];
-  return g >= 0 && g < p.pages ? g : -1;
+// One column as a warp sees it, lane: row.  A class of lanes holds the same page; its first lane speaks for it: pieces that all living rows see whole,
+// pieces in all, tokens.
+struct SharedColumn {
+  int page, whole, pieces, tokens;
+  uint32_t same;
+};
+__device__ __forceinline__ SharedColumn shared_column(const SharedPlanParams& p, int page, int tokens, uint32_t alive) {
+  SharedColumn c;
+  c.page = tokens > 0 && page >= 0 && page < p.pages ? page : -1;
+  c.same = __match_any_sync(0xffffffffu, c.page);
+  int most = tokens, least = tokens;
+  if (!__all_sync(0xffffffffu, c.page < 0 || tokens >= p.page_size)) {      // (only a row's last column is not full)
+    most = 0, least = p.page_size;
+    for (uint32_t left = c.same; left; left &= left - 1) {
+      const int v = __shfl_sync(c.same, tokens, __ffs(left) - 1);
+      most = max(most, v), least = min(least, v);
+    }
+  }
+  const bool leads = c.page >= 0 && static_cast<int>(threadIdx.x & 31) == __ffs(c.same) - 1;
+  c.tokens = most = min(most, p.page_size);
+  c.pieces = leads ? (most + p.piece - 1) / p.piece : 0;
+  c.whole = leads && (c.same & alive) == alive ? min(least, p.page_size) / p.piece : 0;
+  return c;
 }
 
+// A cluster a group, its columns dealt out to the blocks in turn stretches.  Counted first, then written behind what stands in front.
 __global__ void __launch_bounds__(SP_THREADS) shared_list_kernel(const __grid_constant__ SharedPlanParams p) {
-  extern __shared__ int32_t sp_first[];                // [columns] pieces in front of a column
-  __shared__ int sums[SP_THREADS / 32], carry;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = blockIdx.x;
+  extern __shared__ int2 sp_first[];                   // whole pieces and others in front of a column, within the block
+  __shared__ int2 sums[SP_WARPS], carry;
+  __shared__ float totals[2];                          // (ints, read by the other blocks)
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = cluster_ctarank(), blocks = cluster_nctarank(), g = blockIdx.x / blocks;
   pdl_sync();
   int n;
   const int r0 = shared_first_row(p, g, n);
@@ -67,85 +82,128 @@ __global__ void __launch_bounds__(SP_THREADS) shared_list_kernel(const __grid_co
   if (lane < n) {
     len = p.tokens[r0 + lane];
     len = len < 0 ? 0 : min(len, p.columns * p.page_size);
-    if (warp == 0) p.len[r0 + lane] = len;
+    if (rank == 0 && warp == 0) p.len[r0 + lane] = len;
   }
   const int32_t* row = p.table + static_cast<long long>(r0 + (lane < n ? lane : 0)) * p.columns;
   const uint32_t alive = __ballot_sync(0xffffffffu, len > 0);
   const int longest = __reduce_max_sync(0xffffffffu, len), columns = (longest + p.page_size - 1) / p.page_size;
-  for (int c = warp; c < columns; c += SP_THREADS / 32) {
-    int t;
-    const int page = shared_page(p, row, len, c, t);
-    const uint32_t same = __match_any_sync(0xffffffffu, page);
-    int most = 0;
-    for (uint32_t left = same; left; left &= left - 1) most = max(most, __shfl_sync(same, t, __ffs(left) - 1));
-    const bool leads = page >= 0 && lane == __ffs(same) - 1;
-    const int pieces = __reduce_add_sync(0xffffffffu, leads ? (most + p.piece - 1) / p.piece : 0);
-    if (lane == 0) sp_first[c] = pieces;
+  const int each = (columns + blocks - 1) / blocks, c_lo = min(columns, rank * each), here = min(columns, c_lo + each) - c_lo;
+  auto page_at = [&](int c) { return c * p.page_size < len ? row[c] : -1; };
+  for (int c0 = warp * 4; c0 < here; c0 += SP_WARPS * 4) {
+    int page[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) page[j] = c0 + j < here ? page_at(c_lo + c0 + j) : -1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c0 + j < here) {
+        const SharedColumn c = shared_column(p, page[j], len - (c_lo + c0 + j) * p.page_size, alive);
+        const int all = __reduce_add_sync(0xffffffffu, c.pieces), whole = __reduce_add_sync(0xffffffffu, c.whole);
+        if (lane == 0) sp_first[c0 + j] = make_int2(whole, all - whole);
+      }
   }
-  if (tid == 0) carry = 0;
+  if (tid == 0) carry = make_int2(0, 0);
   __syncthreads();
-  for (int c0 = 0; c0 < columns; c0 += SP_THREADS) {       // exclusive prefix over the columns
-    const int c = c0 + tid, mine = c < columns ? sp_first[c] : 0;
-    int inc = mine;
+  for (int c0 = 0; c0 < here; c0 += SP_THREADS) {       // exclusive prefix over the block's columns
+    const int c = c0 + tid;
+    const int2 mine = c < here ? sp_first[c] : make_int2(0, 0);
+    int2 inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
+      const int x = __shfl_up_sync(0xffffffffu, inc.x, o), y = __shfl_up_sync(0xffffffffu, inc.y, o);
+      if (lane >= o) inc.x += x, inc.y += y;
     }
     if (lane == 31) sums[warp] = inc;
     __syncthreads();
-    int before = carry, all = carry;
-    for (int w = 0; w < SP_THREADS / 32; ++w) {
-      if (w < warp) before += sums[w];
-      all += sums[w];
+    int2 before = carry, all = carry;
+#pragma unroll
+    for (int w = 0; w < SP_WARPS; ++w) {
+      if (w < warp) before.x += sums[w].x, before.y += sums[w].y;
+      all.x += sums[w].x, all.y += sums[w].y;
     }
-    if (c < columns) sp_first[c] = before + inc - mine;
+    if (c < here) sp_first[c] = make_int2(before.x + inc.x - mine.x, before.y + inc.y - mine.y);
     __syncthreads();
     if (tid == 0) carry = all;
     __syncthreads();
   }
-  if (tid == 0) p.counts[g] = carry;
-  int4* out = p.entries + static_cast<long long>(g) * p.cap;
-  for (int c = warp; c < columns; c += SP_THREADS / 32) {
-    int t;
-    const int page = shared_page(p, row, len, c, t);
-    const uint32_t same = __match_any_sync(0xffffffffu, page);
-    int most = 0, least = p.page_size;
-    for (uint32_t left = same; left; left &= left - 1) {
-      const int v = __shfl_sync(same, t, __ffs(left) - 1);
-      most = max(most, v), least = min(least, v);
-    }
-    const bool leads = page >= 0 && lane == __ffs(same) - 1;
-    const int pieces = leads ? (most + p.piece - 1) / p.piece : 0;
-    int inc = pieces;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    int at = sp_first[c] + inc - pieces;
-    for (int i = 0; i < pieces; ++i) {
-      const int off = i * p.piece, here = min(p.piece, most - off);
-      const int whole = (same & alive) == alive && least >= off + p.piece;
-      out[at++] = make_int4(page * p.page_size + off, c * p.page_size + off, static_cast<int>(same), here | whole << 16);
-    }
+  if (tid == 0) totals[0] = __int_as_float(carry.x), totals[1] = __int_as_float(carry.y);
+  cluster_sync_all();
+  int w0 = 0, o0 = 0, all_w = 0, all_o = 0;             // pieces of the blocks in front, of all
+  for (int b = 0; b < blocks; ++b) {
+    const int w = __float_as_int(ld_dsmem_f32(&totals[0], b)), o = __float_as_int(ld_dsmem_f32(&totals[1], b));
+    if (b < rank) w0 += w, o0 += o;
+    all_w += w, all_o += o;
   }
+  const int tiles_w = all_w / p.tile_pieces;            // (what is left of the whole ones fills the first of the others)
+  if (rank == 0 && tid == 0) p.counts[g] = all_w + all_o, p.whole[g] = tiles_w;
+  int4* out = p.entries + static_cast<long long>(g) * p.cap;
+  for (int c0 = warp * 4; c0 < here; c0 += SP_WARPS * 4) {
+    int page[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) page[j] = c0 + j < here ? page_at(c_lo + c0 + j) : -1;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (c0 + j < here) {
+        const int col = c_lo + c0 + j;
+        const SharedColumn c = shared_column(p, page[j], len - col * p.page_size, alive);
+        int2 inc = make_int2(c.whole, c.pieces - c.whole);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const int x = __shfl_up_sync(0xffffffffu, inc.x, o), y = __shfl_up_sync(0xffffffffu, inc.y, o);
+          if (lane >= o) inc.x += x, inc.y += y;
+        }
+        const int2 first = sp_first[c0 + j];
+        int at_w = w0 + first.x + inc.x - c.whole, at_o = all_w + o0 + first.y + inc.y - (c.pieces - c.whole);
+        for (int i = 0; i < c.pieces; ++i) {
+          const int off = i * p.piece;
+          out[i < c.whole ? at_w++ : at_o++] = make_int4(c.page * p.page_size + off, col * p.page_size + off, static_cast<int>(c.same), min(p.piece, c.tokens - off));
+        }
+      }
+  }
+  cluster_sync_all();                                   // (totals have been read)
 }
 
 __global__ void __launch_bounds__(1024) shared_deal_kernel(const __grid_constant__ SharedPlanParams p) {
-  __shared__ int sums[32], carry;
+  __shared__ int sums[33];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  if (tid == 0) carry = 0;
   pdl_sync();
-  __syncthreads();
-  for (int g0 = 0; g0 < p.groups; g0 += 1024) {
-    const int g = g0 + tid, mine = g < p.groups ? (__ldcg(p.counts + g) + p.tile_pieces - 1) / p.tile_pieces : 0;
-    int inc = mine;
+  auto tiles_of = [&](int g) { return (__ldcg(p.counts + g) + p.tile_pieces - 1) / p.tile_pieces; };
+  // sum (op 0) or maximum over the block
+  auto meet = [&](int v, bool maximum) {
+    v = maximum ? __reduce_max_sync(0xffffffffu, v) : __reduce_add_sync(0xffffffffu, v);
+    __syncthreads();
+    if (lane == 0) sums[warp] = v;
+    __syncthreads();
+    v = sums[lane];
+    return maximum ? __reduce_max_sync(0xffffffffu, v) : __reduce_add_sync(0xffffffffu, v);
+  };
+  int mine = 0, longest = 0;
+  for (int g = tid; g < p.groups; g += 1024) {
+    const int t = tiles_of(g);
+    mine += t, longest = max(longest, t);
+  }
+  const int total = meet(mine, false) * p.heads, most = meet(longest, true);
+  // tiles of a segment: the fewest with which all segments run at once, where that is possible
+  int lo = max(1, (total + p.grid - 1) / p.grid), hi = max(lo, most);
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    mine = 0;
+    for (int g = tid; g < p.groups; g += 1024) mine += (tiles_of(g) + mid - 1) / mid;
+    if (meet(mine, false) * p.heads <= p.grid) hi = mid;
+    else lo = mid + 1;
+  }
+  const int units = p.groups * p.heads;
+  const int each = units <= p.grid ? lo : max(1, (total + p.grid - 1) / p.grid);
+  int carry = 0;
+  for (int u0 = 0; u0 < units; u0 += 1024) {
+    const int u = u0 + tid, g = u / p.heads, h = u - g * p.heads;
+    const int tiles = u < units ? tiles_of(g) : 0, n = (tiles + each - 1) / each;
+    int inc = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, inc, o);
       if (lane >= o) inc += v;
     }
+    __syncthreads();
     if (lane == 31) sums[warp] = inc;
     __syncthreads();
     int before = carry, all = carry;
@@ -153,41 +211,28 @@ __global__ void __launch_bounds__(1024) shared_deal_kernel(const __grid_constant
       if (w < warp) before += sums[w];
       all += sums[w];
     }
-    if (g < p.groups) p.tile0[g] = before + inc - mine;
-    __syncthreads();
-    if (tid == 0) carry = all;
-    __syncthreads();
-  }
-  const int total = carry, work = total * p.heads, each = max(1, (work + p.grid - 1) / p.grid);
-  if (tid == 0) p.tile0[p.groups] = total, p.head[0] = each, p.head[1] = total;
-  __syncthreads();
-  for (int i = tid; i < p.grid; i += 1024) {
-    const long long start = static_cast<long long>(i) * each;
-    int4 part = make_int4(0, 0, 0, 0);
-    if (start < work) {
-      int lo = 0, hi = p.groups - 1;                    // the last group that begins at or before the start (later ones of the same start are empty)
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (static_cast<long long>(p.tile0[mid]) * p.heads <= start) lo = mid;
-        else hi = mid - 1;
-      }
-      const int tiles = p.tile0[lo + 1] - p.tile0[lo], in = static_cast<int>(start - static_cast<long long>(p.tile0[lo]) * p.heads);
-      part = make_int4(lo, in / tiles, in % tiles, min(each, static_cast<int>(work - start)));
+    const int at = before + inc - n;
+    if (u < units) {
+      p.seg0[u] = at;
+      for (int i = 0; i < n; ++i) p.segments[at + i] = make_int4(g, h, i * each, min(each, tiles - i * each));
     }
-    p.parts[i] = part;
+    carry = all;
   }
+  if (tid == 0) p.seg0[units] = carry;
+  for (int i = carry + tid; i < p.grid + units; i += 1024) p.segments[i] = make_int4(0, 0, 0, 0);
 }
 
 // ---- attention -------------------------------------------------------------------------------------------------------------------
 struct SharedAttnParams {
-  const __nv_bfloat16* q;
+  const __nv_bfloat16 *q, *kv;
   __nv_bfloat16* out;
-  const int4 *entries, *parts;
-  const int32_t *counts, *tile0, *len, *head;
-  float *acc, *stat;             // [slots][row tiles * 16][D], [slots][row tiles * 16][2]
-  int64_t slab_base;
+  const int4 *entries, *segments;
+  const int32_t *counts, *whole, *len, *seg0;
+  float* acc;                    // [segments][mpad][D]
+  float2* stat;                  // [segments][mpad] maximum (base 2), denominator against it
+  long long slab_base;
   unsigned char* wait_flag;
-  int rows, width, sub, subs, groups, cap, page_size, piece, piece_log, n_q, heads, G, xt_tile;
+  int rows, width, sub, subs, groups, cap, page_size, piece, tile_pieces, n_q, heads, G, mpad, xt_tile;
   float scale_log2;
 };
 
@@ -196,368 +241,276 @@ __device__ __forceinline__ int shared_group(const SharedAttnParams& p, int g, in
   n = min(p.sub, p.width - in);
   return g / p.subs * p.width + in;
 }
-__device__ __forceinline__ float sa_ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 256;" ::: "memory"); }
 
-template <int D, int MT>
-struct SaShape {
-  static constexpr int TT = sa_tile_tokens(MT);                // tokens of a tile
-  static constexpr int HALF = TT * 128;                        // bytes of 64 dimensions of its keys
-  static constexpr int KV = HALF * (D / 64), STAGE = 2 * KV;
-  static constexpr int STAGES = SA_RING / STAGE;
-  static constexpr int WT = SA_WARPS / MT;                     // warps that share a tile's tokens
-  static constexpr int TOK = TT / WT, BLOCKS = TOK / 16;       // tokens of a warp, 16 at a time
-  static constexpr int MERGE = 4 * 16 * D * 4;                 // bytes: outputs of half the warps
-  static constexpr int SMEM = 1024 + SA_RING + MERGE;
+// what this thread's row sees of a segment, and where its part goes
+template <int D>
+struct SharedRows {
+  static constexpr bool HOLE = false, STAGED = false;
+  static constexpr int hole0 = 0, hole1 = 0;
+  const SharedAttnParams& p;
+  uint8_t* smem;
+  const int4 *entries, *meta;    // of the group; of the last four tiles with masks
+  int count, whole, t0, n_tiles; // pieces; tiles that need no mask; the segment
+  int row0, n_rows, head, group; // first row, rows, key head, query heads of it
+  int len, bit;
+  bool ok;
+  float scale_log2;
+  float2* stat;
+  bool careful;                  // values that are not finite have been taken out
+  mutable bool bad;              // a result that is not finite
+  mutable uint64_t seen;
+  __device__ __forceinline__ int tile(int it) const { return t0 + it; }
+  __device__ __forceinline__ int4 piece(int i) const { return i < count ? entries[i] : make_int4(0, 0, 0, 0); }
+  __device__ __forceinline__ uint64_t mask(const int4* pieces, int n_pieces) const {
+    uint64_t m = 0ull;
+    for (int i = 0; i < n_pieces; ++i) {
+      const int4 e = pieces[i];
+      const int n = (static_cast<uint32_t>(e.z) >> bit & 1u) ? min(len - e.y, e.w) : 0;
+      if (n > 0) m |= (n < 64 ? (1ull << n) - 1ull : ~0ull) << (i * p.piece);
+    }
+    return m;
+  }
+  __device__ __forceinline__ bool full(int tok0) const {
+    seen = ~0ull;
+    const int t = tok0 / PTC_KT;
+    if (t >= whole && ok) seen = mask(meta + (t - t0 & 3) * 4, p.tile_pieces);      // (a row that is none may have anything)
+    return seen == ~0ull;
+  }
+  __device__ __forceinline__ bool visible(int kj) const { return seen >> (kj & (PTC_KT - 1)) & 1ull; }
+  __device__ __forceinline__ const __nv_bfloat16* q_row(int t, int g) const {
+    return t < n_rows ? p.q + (static_cast<size_t>(row0 + t) * p.n_q + head * group + g) * D : nullptr;
+  }
+  __device__ __forceinline__ uint4* out_at(int, int, int) const { return nullptr; }
+  __device__ __forceinline__ float finish(float m_ref, float l) const {
+    if (ok) *stat = make_float2(m_ref, l);
+    return 1.f;
+  }
+  // a thread's row goes to the place of the keys and values (they have been multiplied): 16-byte chunk c of row r at chunk c ^ (r & 15) of its 16 or 32
+  __device__ __forceinline__ float4* staged(int r, int c) const { return reinterpret_cast<float4*>(smem + PtcLayout<D>::K) + r * (D / 4) + ((c & ~15) | ((c ^ r) & 15)); }
+  __device__ __forceinline__ void store(int c0, const uint32_t (&o)[32], float) const {
+    float v[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]);
+    if (careful && ok) give_back(c0, v);
+#pragma unroll
+    for (int i = 0; i < 32; ++i) bad |= !isfinite(v[i]);
+#pragma unroll
+    for (int c = 0; c < 8; ++c) *staged(threadIdx.x, (c0 >> 2) + c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+  }
+  // what is not finite among the values that the row sees, in tiles where it was taken out
+  __device__ __noinline__ void give_back(int c0, float (&v)[32]) const {
+    for (int t = max(t0, whole); t < t0 + n_tiles; ++t) {
+      const int first = t * p.tile_pieces;
+      const uint64_t m = mask(entries + first, min(p.tile_pieces, count - first));
+      for (int k = 0; k < PTC_KT; ++k) {
+        if (!(m >> k & 1ull)) continue;
+        const int4 e = piece(t * p.tile_pieces + k / p.piece);
+        const int tok = e.x + k % p.piece, page = tok / p.page_size, slot = tok - page * p.page_size;
+        const uint32_t* src = reinterpret_cast<const uint32_t*>(p.kv + ((((p.slab_base + page) * 2 + 1) * p.page_size + slot) * p.heads + head) * D + c0);
+        for (int i = 0; i < 16; ++i) {
+          const uint32_t w = src[i];
+          if ((w & 0x7f80u) == 0x7f80u) v[2 * i] += bf16_lo(w);
+          if ((w & 0x7f800000u) == 0x7f800000u) v[2 * i + 1] += bf16_hi(w);
+        }
+      }
+    }
+  }
 };
 
-template <int D, int MT>
-__global__ void __launch_bounds__(SA_THREADS, 1) shared_attn_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ SharedAttnParams p) {
-  using L = SaShape<D, MT>;
-  extern __shared__ uint8_t sa_raw[];
-  uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sa_raw) + 1023) & ~static_cast<uintptr_t>(1023));
-  float* merge = reinterpret_cast<float*>(ring + SA_RING);
-  __shared__ uint64_t full[L::STAGES], empty[L::STAGES];
-  __shared__ int4 meta[L::STAGES][8];
-  __shared__ float merge_ml[4][16][2];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  BoundedWait bw{p.wait_flag};
-  if (tid == 0) {
+// A lane a piece of the tile: its boxes, K or V
+template <int D>
+__device__ __forceinline__ void shared_fetch(const SharedAttnParams& p, const CUtensorMap* map, const int4& e, int part, int head, uint32_t dst, uint64_t* bar) {
+  const int lane = threadIdx.x & 31;
+  const bool has = e.w > 0;
+  const int n = __popc(__ballot_sync(0xffffffffu, has));
+  if (lane == 0) mbar_arrive_expect_tx(bar, n * p.piece * D * 2);
+  __syncwarp();
+  if (has) {
+    const int page = e.x / p.page_size, slot = e.x - page * p.page_size;
 #pragma unroll
-    for (int s = 0; s < L::STAGES; ++s) mbar_init(&full[s], 1), mbar_init(&empty[s], SA_WARPS);
-    fence_barrier_init();
-    prefetch_tmap(&map);
+    for (int kb = 0; kb < D / 64; ++kb)
+      ptc_tma_5d(dst + kb * (PTC_KT * 128) + lane * p.piece * 128, map, smem_u32(bar), kb * 64, slot, head, part, static_cast<int>(p.slab_base + page));
   }
-  __syncthreads();
-  pdl_sync();
-  int4 part = p.parts[blockIdx.x];
-  if (part.w == 0) return;
-  const int pieces = L::TT / p.piece;
-
-  if (warp == SA_WARPS) {
-    // ---- the warp that fetches: a lane a piece ----
-    int g = part.x, h = part.y, tile = part.z, count = p.counts[g], tiles = p.tile0[g + 1] - p.tile0[g];
-    auto entry = [&](int gg, int t, int n) {
-      const int i = t * pieces + lane;
-      return lane < pieces && i < n ? p.entries[static_cast<long long>(gg) * p.cap + i] : make_int4(0, 0, 0, 0);
-    };
-    int4 e = entry(g, tile, count);
-    int stage = 0, asked = 0;
-    uint32_t phase = 1;
-    for (; asked < part.w; ++asked) {
-      const int i = asked;
-      const int4 now = e;
-      const int head = h;
-      if (i + 1 < part.w) {                                       // the next tile's pieces, while this one's place is still in use
-        if (++tile == tiles) {
-          tile = 0;
-          if (++h == p.heads) {
-            h = 0;
-            do {
-              ++g;
-              tiles = p.tile0[g + 1] - p.tile0[g];
-            } while (tiles == 0);
-            count = p.counts[g];
-          }
-        }
-        e = entry(g, tile, count);
-      }
-      bw.wait(&empty[stage], phase);
-      if (__any_sync(0xffffffffu, bw.dead)) break;
-      const bool has = (now.w & 0xffff) != 0;
-      if (lane < pieces) meta[stage][lane] = now;
-      const int n = __popc(__ballot_sync(0xffffffffu, has));
-      __syncwarp();
-      if (lane == 0) mbar_arrive_expect_tx(&full[stage], n * p.piece * D * 4);
-      __syncwarp();
-      if (has) {
-        const int page = now.x / p.page_size, off = now.x - page * p.page_size, slab = static_cast<int>(p.slab_base + page);
-        uint8_t* at = ring + stage * L::STAGE + lane * p.piece * 128;
-#pragma unroll
-        for (int d = 0; d < D / 64; ++d) {
-          tma_load_5d(at + d * L::HALF, &map, &full[stage], d * 64, off, head, 0, slab);
-          tma_load_5d(at + L::KV + d * L::HALF, &map, &full[stage], d * 64, off, head, 1, slab);
-        }
-      }
-      if (++stage == L::STAGES) stage = 0, phase ^= 1;
-    }
-    // what has been asked for lands before the block leaves, whether or not the others waited for it
-    BoundedWait last{p.wait_flag};
-    for (int i = max(0, asked - L::STAGES); i < asked; ++i) last.wait(&full[i % L::STAGES], (i / L::STAGES) & 1);
-    return;
-  }
-
-  // ---- the warps that multiply: 16 rows (row tile mt), tokens tg * TOK and further of every tile ----
-  const int mt = warp % MT, tg = warp / MT;
-  const int m0 = mt * 16 + (lane >> 2), m1 = m0 + 8;             // this thread's rows of the group's products
-  int stage = 0;
-  uint32_t phase = 0;
-  int g = part.x, h = part.y, tile = part.z, left = part.w;
-  const uint32_t ring_at = smem_u32(ring);
-  while (left > 0) {
-    const int tiles = p.tile0[g + 1] - p.tile0[g];
-    if (tiles == 0) {
-      ++g, h = 0;
-      continue;
-    }
-    const int n_here = min(left, tiles - tile);
-    left -= n_here;
-    int n_rows;
-    const int r0 = shared_group(p, g, n_rows), n_m = n_rows * p.G;
-    const int i0 = m0 / p.G, i1 = m1 / p.G;                      // rows of the group
-    const int len0 = m0 < n_m ? p.len[r0 + i0] : 0, len1 = m1 < n_m ? p.len[r0 + i1] : 0;
-    const uint32_t bit0 = m0 < n_m ? 1u << i0 : 0u, bit1 = m1 < n_m ? 1u << i1 : 0u;
-    uint32_t qf[D / 16][4];
-    {
-      const uint32_t* q0 = reinterpret_cast<const uint32_t*>(p.q + (static_cast<long long>(r0 + i0) * p.n_q + h * p.G + m0 - i0 * p.G) * D) + (lane & 3);
-      const uint32_t* q1 = reinterpret_cast<const uint32_t*>(p.q + (static_cast<long long>(r0 + i1) * p.n_q + h * p.G + m1 - i1 * p.G) * D) + (lane & 3);
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        qf[k][0] = m0 < n_m ? q0[k * 8] : 0u;
-        qf[k][1] = m1 < n_m ? q1[k * 8] : 0u;
-        qf[k][2] = m0 < n_m ? q0[k * 8 + 4] : 0u;
-        qf[k][3] = m1 < n_m ? q1[k * 8 + 4] : 0u;
-      }
-    }
-    float o[D / 8][4];
-#pragma unroll
-    for (int n = 0; n < D / 8; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
-    float mx0 = -INFINITY, mx1 = -INFINITY, l0 = 0.f, l1 = 0.f;
-
-    for (int it = 0; it < n_here; ++it) {
-      bw.wait(&full[stage], phase);
-      const uint32_t k_at = ring_at + stage * L::STAGE, v_at = k_at + L::KV;
-      const int tok0 = tg * L::TOK;
-#pragma unroll
-      for (int blk = 0; blk < L::BLOCKS; ++blk) {
-        const int tb = tok0 + blk * 16;                          // 16 tokens of one piece
-        const int4 e = meta[stage][tb >> p.piece_log];
-        const int off = tb & (p.piece - 1), here = (e.w & 0xffff) - off;      // tokens of the piece from here on
-        if (here <= 0) continue;                                  // (uniform over the warp)
-        const bool whole = e.w >> 16;
-        float s[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
-        {
-          const int row = tb + ((lane >> 4) << 3) + (lane & 7), c = (lane >> 3) & 1;
-#pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            uint32_t b[4];
-            const int chunk = (k & 3) * 2 + c;
-            ldmatrix_x4(b, k_at + (k >> 2) * L::HALF + row * 128 + ((chunk ^ (row & 7)) << 4));
-            mma_bf16_16816(s[0], qf[k], b[0], b[1]);
-            mma_bf16_16816(s[1], qf[k], b[2], b[3]);
-          }
-        }
-        const int t0 = (lane & 3) * 2;
-        // what a row does not see: other rows' pages, tokens behind its last
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int pos = e.y + off + n * 8 + t0 + j;
-            s[n][j] = whole || ((e.z & bit0) && pos < len0) ? s[n][j] * p.scale_log2 : -INFINITY;
-            s[n][2 + j] = whole || ((e.z & bit1) && pos < len1) ? s[n][2 + j] * p.scale_log2 : -INFINITY;
-          }
-        float a = fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])), b = fmaxf(fmaxf(s[0][2], s[0][3]), fmaxf(s[1][2], s[1][3]));
-        a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 1)), b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, 1));
-        a = fmaxf(a, __shfl_xor_sync(0xffffffffu, a, 2)), b = fmaxf(b, __shfl_xor_sync(0xffffffffu, b, 2));
-        const bool up = a > mx0 || b > mx1;
-        if (__any_sync(0xffffffffu, up)) {
-          const float n0 = fmaxf(mx0, a), n1 = fmaxf(mx1, b);
-          const float c0 = n0 == -INFINITY ? 1.f : sa_ex2(mx0 - n0), c1 = n1 == -INFINITY ? 1.f : sa_ex2(mx1 - n1);
-          mx0 = n0, mx1 = n1, l0 *= c0, l1 *= c1;
-#pragma unroll
-          for (int n = 0; n < D / 8; ++n) o[n][0] *= c0, o[n][1] *= c0, o[n][2] *= c1, o[n][3] *= c1;
-        }
-        const float z0 = mx0 == -INFINITY ? 0.f : mx0, z1 = mx1 == -INFINITY ? 0.f : mx1;
-        bool seen[2][4];
-#pragma unroll
-        for (int n = 0; n < 2; ++n)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            seen[n][j] = !(s[n][j] == -INFINITY);
-            s[n][j] = sa_ex2(s[n][j] - (j < 2 ? z0 : z1));
-          }
-        l0 += (s[0][0] + s[0][1]) + (s[1][0] + s[1][1]);
-        l1 += (s[0][2] + s[0][3]) + (s[1][2] + s[1][3]);
-        uint32_t hi[4], lo[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float x = s[j >> 1][(j & 1) * 2], y = s[j >> 1][(j & 1) * 2 + 1];
-          hi[j] = pack_bf16(x, y);
-          lo[j] = pack_bf16(x - bf16_lo(hi[j]), y - bf16_hi(hi[j]));
-        }
-        const int vrow = tb + ((lane >> 3) & 1) * 8 + (lane & 7), vc = lane >> 4;
-        uint32_t keep0 = 0xffffffffu, keep1 = 0xffffffffu;       // tokens that are none: the page holds anything there
-        bool odd = false;
-        if (!whole) {
-          keep0 = (t0 < here ? 0xffffu : 0u) | (t0 + 1 < here ? 0xffff0000u : 0u);
-          keep1 = (t0 + 8 < here ? 0xffffu : 0u) | (t0 + 9 < here ? 0xffff0000u : 0u);
-          // a value that is not finite must not reach the rows that do not see it, through 0 times infinity
-          uint32_t any = 0u;
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d) {
-            uint32_t v[4];
-            const int chunk = (d & 3) * 2 + vc;
-            ldmatrix_x4_trans(v, v_at + (d >> 2) * L::HALF + vrow * 128 + ((chunk ^ (vrow & 7)) << 4));
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const uint32_t w = v[j] & ((j & 1) ? keep1 : keep0);
-              any |= (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
-            }
-          }
-          odd = __any_sync(0xffffffffu, any != 0u);
-        }
-        if (!odd) {
-#pragma unroll
-          for (int d = 0; d < D / 16; ++d) {
-            uint32_t v[4];
-            const int chunk = (d & 3) * 2 + vc;
-            ldmatrix_x4_trans(v, v_at + (d >> 2) * L::HALF + vrow * 128 + ((chunk ^ (vrow & 7)) << 4));
-            v[0] &= keep0, v[1] &= keep1, v[2] &= keep0, v[3] &= keep1;
-            mma_bf16_16816(o[2 * d], lo, v[0], v[1]);
-            mma_bf16_16816(o[2 * d + 1], lo, v[2], v[3]);
-            mma_bf16_16816(o[2 * d], hi, v[0], v[1]);
-            mma_bf16_16816(o[2 * d + 1], hi, v[2], v[3]);
-          }
-        } else {
-          // token by token, each row what it sees
-          for (int t = 0; t < 16; ++t) {
-            const int from = (lane & ~3) | ((t & 7) >> 1);
-            float pr[2];
-            bool sees[2];
-#pragma unroll
-            for (int r = 0; r < 2; ++r) {
-              const float even = t < 8 ? s[0][r * 2] : s[1][r * 2], other = t < 8 ? s[0][r * 2 + 1] : s[1][r * 2 + 1];
-              const bool se = t < 8 ? seen[0][r * 2] : seen[1][r * 2], so = t < 8 ? seen[0][r * 2 + 1] : seen[1][r * 2 + 1];
-              pr[r] = __shfl_sync(0xffffffffu, t & 1 ? other : even, from);
-              sees[r] = __shfl_sync(0xffffffffu, static_cast<int>(t & 1 ? so : se), from) != 0;
-            }
-            const int vr = tb + t;
-#pragma unroll
-            for (int n = 0; n < D / 8; ++n) {
-              uint32_t w;
-              asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w) : "r"(v_at + (n >> 3) * L::HALF + vr * 128 + (((n & 7) ^ (vr & 7)) << 4) + t0 * 2) : "memory");
-              if (sees[0]) o[n][0] += pr[0] * bf16_lo(w), o[n][1] += pr[0] * bf16_hi(w);
-              if (sees[1]) o[n][2] += pr[1] * bf16_lo(w), o[n][3] += pr[1] * bf16_hi(w);
-            }
-          }
-        }
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&empty[stage]);
-      if (++stage == L::STAGES) stage = 0, phase ^= 1;
-    }
-
-    // ---- the warps of a row tile meet: the upper half hands its part to the lower one, as often as it takes ----
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 1), l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
-    l0 += __shfl_xor_sync(0xffffffffu, l0, 2), l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-#pragma unroll
-    for (int half = SA_WARPS / 2; half >= MT; half >>= 1) {
-      consumers_sync();                                          // (the last part has been read)
-      if (warp >= half && warp < 2 * half) {
-        float* at = merge + (warp - half) * 16 * D;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          *reinterpret_cast<float2*>(at + (n * 64 + lane) * 2) = make_float2(o[n][0], o[n][1]);
-          *reinterpret_cast<float2*>(at + (n * 64 + 32 + lane) * 2) = make_float2(o[n][2], o[n][3]);
-        }
-        if ((lane & 3) == 0) {
-          merge_ml[warp - half][lane >> 2][0] = mx0, merge_ml[warp - half][lane >> 2][1] = l0;
-          merge_ml[warp - half][8 + (lane >> 2)][0] = mx1, merge_ml[warp - half][8 + (lane >> 2)][1] = l1;
-        }
-      }
-      consumers_sync();
-      if (warp < half) {
-        const float* at = merge + warp * 16 * D;
-        const float a = merge_ml[warp][lane >> 2][0], b = merge_ml[warp][8 + (lane >> 2)][0];
-        const float n0 = fmaxf(mx0, a), n1 = fmaxf(mx1, b);
-        const float c0 = n0 == -INFINITY ? 0.f : sa_ex2(mx0 - n0), c1 = n1 == -INFINITY ? 0.f : sa_ex2(mx1 - n1);
-        const float d0 = n0 == -INFINITY ? 0.f : sa_ex2(a - n0), d1 = n1 == -INFINITY ? 0.f : sa_ex2(b - n1);
-        l0 = l0 * c0 + merge_ml[warp][lane >> 2][1] * d0, l1 = l1 * c1 + merge_ml[warp][8 + (lane >> 2)][1] * d1;
-        mx0 = n0, mx1 = n1;
-#pragma unroll
-        for (int n = 0; n < D / 8; ++n) {
-          const float2 x = *reinterpret_cast<const float2*>(at + (n * 64 + lane) * 2), y = *reinterpret_cast<const float2*>(at + (n * 64 + 32 + lane) * 2);
-          o[n][0] = o[n][0] * c0 + x.x * d0, o[n][1] = o[n][1] * c0 + x.y * d0;
-          o[n][2] = o[n][2] * c1 + y.x * d1, o[n][3] = o[n][3] * c1 + y.y * d1;
-        }
-      }
-    }
-    if (warp < MT) {
-      const long long slot = blockIdx.x + static_cast<long long>(g) * p.heads + h;
-      float* acc = p.acc + slot * (MT * 16) * D;
-      float* st = p.stat + slot * (MT * 16) * 2;
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n) {
-        if (m0 < n_m) *reinterpret_cast<float2*>(acc + m0 * D + n * 8 + (lane & 3) * 2) = make_float2(o[n][0], o[n][1]);
-        if (m1 < n_m) *reinterpret_cast<float2*>(acc + m1 * D + n * 8 + (lane & 3) * 2) = make_float2(o[n][2], o[n][3]);
-      }
-      if ((lane & 3) == 0) {
-        if (m0 < n_m) *reinterpret_cast<float2*>(st + m0 * 2) = make_float2(mx0, l0);
-        if (m1 < n_m) *reinterpret_cast<float2*>(st + m1 * 2) = make_float2(mx1, l1);
-      }
-    }
-    tile = 0;
-    if (++h == p.heads) h = 0, ++g;
-  }
+  __syncwarp();
 }
 
-// A warp a row of a group and head: the parts that blocks left of it, in their order.
-constexpr int SJ_WARPS = 8;
 template <int D>
-__global__ void __launch_bounds__(32 * SJ_WARPS) shared_join_kernel(const __grid_constant__ SharedAttnParams p, int mpad) {
-  const int lane = threadIdx.x & 31, unit = blockIdx.x, g = unit / p.heads, h = unit - g * p.heads;
-  const int m = blockIdx.y * SJ_WARPS + (threadIdx.x >> 5);
+__global__ void __launch_bounds__(PTC_THREADS, 2) shared_attn_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ SharedAttnParams p) {
+  using L = PtcLayout<D>;
+  extern __shared__ uint8_t sa_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sa_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  static_assert(sizeof(PtcShared) <= 256, "two of them and four tiles' pieces behind the operands");
+  PtcShared *sh = reinterpret_cast<PtcShared*>(smem + L::BAR), *sh2 = reinterpret_cast<PtcShared*>(smem + L::BAR + 256);
+  int4* meta = reinterpret_cast<int4*>(smem + L::BAR + 512);
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  BoundedWait bw{p.wait_flag};
+  pdl_wait();
+  const int4 seg = p.segments[blockIdx.x];
+  pdl_trigger();
+  if (seg.w == 0) return;
+  if (tid == 0) {
+    ptc_init(sh, 1);
+    ptc_init(sh2, 1);
+    prefetch_tmap(&map);
+  }
+  if (warp == 4) {
+    tmem_alloc(&sh->tmem, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = sh->tmem;
+  if (tid == 0) sh2->tmem = tmem_base;
+
+  const int g = seg.x, head = seg.y, n_tiles = seg.w;
+  int n_rows;
+  const int row0 = shared_group(p, g, n_rows), t = tid / p.G;
+  const bool ok = warp < 4 && t < n_rows;
+  SharedRows<D> rows{p, smem, p.entries + static_cast<long long>(g) * p.cap, meta, p.counts[g], p.whole[g], seg.z, n_tiles, row0, n_rows, head, p.G,
+                     ok ? p.len[row0 + t] : 0, ok ? t : 0, ok, p.scale_log2, p.stat + static_cast<long long>(blockIdx.x) * p.mpad + tid, false, false, ~0ull};
+#pragma unroll 1
+  for (int pass = 0;; ++pass) {
+    rows.careful = pass != 0;
+    rows.bad = false;
+    if (warp < 4) {
+      ptc_softmax<D>(smem, sh, rows, bw);
+      fence_proxy_async();                                    // (results stand where keys and values may come again)
+    } else if (warp == 4) {
+      ptc_issue<D>(smem, sh, n_tiles, bw);
+    } else {
+      const bool values = warp == 6;
+      uint64_t *full = values ? sh->v_full : sh->k_full, *empty = values ? sh->v_empty : sh->k_empty;
+      const uint32_t ring = smem_u32(smem + (values ? L::V : L::K));
+      auto find = [&](int j) { return lane < p.tile_pieces && j < n_tiles ? rows.piece((seg.z + j) * p.tile_pieces + lane) : make_int4(0, 0, 0, 0); };
+      int4 next = find(0);
+      uint32_t turn = 0;                                      // bit s: parity of stage s's next tile that is changed
+      for (int j = 0; j < n_tiles; ++j) {
+        const int s = j & 1;
+        const int4 e = next;
+        next = find(j + 1);
+        bw.wait(&empty[s], ((j >> 1) & 1) ^ 1);
+        if (!__all_sync(0xffffffffu, !bw.dead)) {
+          bw.dead = true;
+          break;
+        }
+        const bool masked = seg.z + j >= rows.whole;
+        // (tile j + 4's stands where tile j's was: its stage was empty, so tile j + 2's scores have been multiplied, and tile j's output with them)
+        if (!values && masked && lane < p.tile_pieces) meta[(j & 3) * 4 + lane] = e;
+        const uint32_t short_ = __ballot_sync(0xffffffffu, lane < p.tile_pieces && e.w < p.piece);
+        const bool change = values && masked && (short_ || rows.careful);
+        shared_fetch<D>(p, &map, e, values ? 1 : 0, head, ring + s * L::TILE, change ? &sh->v_part[s] : &full[s]);
+        if (!change) continue;
+        bw.wait(&sh->v_part[s], turn >> s & 1u);
+        if (!__all_sync(0xffffffffu, !bw.dead)) {
+          bw.dead = true;
+          break;
+        }
+        turn ^= 1u << s;
+        uint4* v_tile = reinterpret_cast<uint4*>(smem + L::V + s * L::TILE);
+        for (uint32_t left = short_; left; left &= left - 1) {      // rows that are no tokens become zeros
+          const int i = __ffs(left) - 1, tokens = __shfl_sync(0xffffffffu, e.w, i), from = (i * p.piece + tokens) * 8, n = (p.piece - tokens) * 8;
+#pragma unroll
+          for (int kb = 0; kb < D / 64; ++kb)
+            for (int k = lane; k < n; k += 32) v_tile[kb * PTC_KT * 8 + from + k] = make_uint4(0u, 0u, 0u, 0u);
+        }
+        if (rows.careful) {
+          __syncwarp();
+          for (int i = lane; i < (D / 64) * PTC_KT * 8; i += 32) {
+            uint4 v = v_tile[i];
+            uint32_t* w = &v.x;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              if ((w[k] & 0x7f80u) == 0x7f80u) w[k] &= 0xffff0000u;
+              if ((w[k] & 0x7f800000u) == 0x7f800000u) w[k] &= 0xffffu;
+            }
+            v_tile[i] = v;
+          }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&full[s]);
+      }
+      ptc_let_land(bw.dead);
+      __syncwarp();
+    }
+    tc_fence_before();
+    const bool again = __syncthreads_or(rows.bad && rows.len > 0 && seg.z + n_tiles > rows.whole && !bw.dead);
+    tc_fence_after();
+    if (!again || pass) break;
+    sh = sh2;
+  }
+  if (warp < 4 && !bw.dead) {                                 // whole rows, 16 bytes a lane
+    float4* acc = reinterpret_cast<float4*>(p.acc + static_cast<long long>(blockIdx.x) * p.mpad * D);
+    const int n = n_rows * p.G * (D / 4);
+    for (int i = tid; i < n; i += 128) acc[i] = *rows.staged(i / (D / 4), i % (D / 4));
+  }
+  if (warp == 4) tmem_dealloc(tmem_base, 256);
+}
+
+// The segments of a group and head meet: WPR warps a row, each every WPR-th segment, a lane D / 32 neighbouring dimensions.
+constexpr int SJ_WARPS = 8;
+template <int D, int WPR>
+__global__ void __launch_bounds__(32 * SJ_WARPS) shared_join_kernel(const __grid_constant__ SharedAttnParams p) {
+  constexpr int E = D / 32;
+  __shared__ float part[SJ_WARPS][32][E + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, unit = blockIdx.x, g = unit / p.heads, h = unit - g * p.heads;
+  const int m = blockIdx.y * (SJ_WARPS / WPR) + warp / WPR, sub = warp % WPR;
   pdl_sync();
   int n_rows;
   const int r0 = shared_group(p, g, n_rows);
-  if (m >= n_rows * p.G) return;
-  const int row = r0 + m / p.G, head = h * p.G + m % p.G;
-  const int each = p.head[0], tiles = p.tile0[g + 1] - p.tile0[g];
-  float acc[D / 32];
+  const bool on = m < n_rows * p.G;
+  const int row = r0 + (on ? m / p.G : 0), k = (h * p.G + (on ? m % p.G : 0)) * D + lane * E;
+  float acc[E], total = 0.f;
 #pragma unroll
-  for (int d = 0; d < D / 32; ++d) acc[d] = 0.f;
-  float total = 0.f;
-  if (tiles > 0 && p.len[row] > 0) {
-    const long long first = static_cast<long long>(p.tile0[g]) * p.heads + static_cast<long long>(h) * tiles;
-    const int b0 = static_cast<int>(first / each), b1 = static_cast<int>((first + tiles - 1) / each);
+  for (int e = 0; e < E; ++e) acc[e] = 0.f;
+  if (on && p.len[row] > 0) {
+    const int s0 = p.seg0[unit], s1 = p.seg0[unit + 1];
     float top = -INFINITY;
-    for (int b = b0 + lane; b <= b1; b += 32) top = fmaxf(top, p.stat[((static_cast<long long>(b) + unit) * mpad + m) * 2]);
+    for (int s = s0 + lane; s < s1; s += 32) top = fmaxf(top, p.stat[static_cast<long long>(s) * p.mpad + m].x);
     top = warp_max(top);
-    if (top == -INFINITY) top = 0.f;                             // (scores that are all infinite or NaN: the sums below say so)
-#pragma unroll 4
-    for (int b = b0; b <= b1; ++b) {
-      const long long at = (static_cast<long long>(b) + unit) * mpad + m;
-      const float2 st = *reinterpret_cast<const float2*>(p.stat + at * 2);
-      const float f = st.x == -INFINITY ? (st.y == 0.f ? 0.f : 1.f) : sa_ex2(st.x - top);      // (nothing seen; scores that are NaN)
+    if (top == -INFINITY) top = 0.f;                            // (scores that are all NaN: the sums below say so)
+#pragma unroll 8
+    for (int s = s0 + sub; s < s1; s += WPR) {
+      const long long at = static_cast<long long>(s) * p.mpad + m;
+      const float2 st = p.stat[at];
+      const float f = st.x == -INFINITY ? (st.y == 0.f ? 0.f : 1.f) : ptc_ex2(st.x - top);      // (nothing seen; scores that are NaN)
+      float v[E];
+      if (E == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p.acc + at * D + lane * E);
+      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(p.acc + at * D + lane * E);
       total += st.y * f;
 #pragma unroll
-      for (int d = 0; d < D / 64; ++d) {
-        const float2 x = *reinterpret_cast<const float2*>(p.acc + at * D + d * 64 + lane * 2);
-        if (f != 0.f) acc[2 * d] += x.x * f, acc[2 * d + 1] += x.y * f;
+      for (int e = 0; e < E; ++e) acc[e] += v[e] * f;
+    }
+  }
+  if (WPR > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) part[warp][lane][e] = acc[e];
+    part[warp][lane][E] = total;
+    __syncthreads();
+    if (sub == 0) {
+#pragma unroll
+      for (int w = 1; w < WPR; ++w) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += part[warp + w][lane][e];
+        total += part[warp + w][lane][E];
       }
     }
   }
+  if (!on || sub != 0) return;
   const float by = total != 0.f ? 1.f / total : 0.f;
+  const size_t at = p.xt_tile ? xt_index(row, k, p.xt_tile, p.n_q * D / 64) : static_cast<size_t>(row) * p.n_q * D + k;
 #pragma unroll
-  for (int d = 0; d < D / 64; ++d) {
-    const int k = head * D + d * 64 + lane * 2;
-    const size_t at = p.xt_tile ? xt_index(row, k, p.xt_tile, p.n_q * D / 64) : static_cast<size_t>(row) * p.n_q * D + k;
-    *reinterpret_cast<uint32_t*>(p.out + at) = pack_bf16(acc[2 * d] * by, acc[2 * d + 1] * by);
-  }
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<uint32_t*>(p.out + at + e) = pack_bf16(acc[e] * by, acc[e + 1] * by);
 }
 
-template <int D, int MT>
+template <int D>
 static int launch_shared(const CUtensorMap& map, const SharedAttnParams& p, int grid, void* stream) {
-  VB_CHECK_CUDA((rm_smem<shared_attn_kernel<D, MT>>(SaShape<D, MT>::SMEM)));
-  VB_LAUNCH_PDL((shared_attn_kernel<D, MT>), grid, SA_THREADS, (SaShape<D, MT>::SMEM), stream, map, p);
-  VB_LAUNCH_PDL(shared_join_kernel<D>, dim3(p.groups * p.heads, (p.sub * p.G + SJ_WARPS - 1) / SJ_WARPS), 32 * SJ_WARPS, 0, stream, p, MT * 16);
+  const int units = p.groups * p.heads, m = p.sub * p.G;
+  VB_CHECK_CUDA(rm_smem<shared_attn_kernel<D>>(PtcLayout<D>::TOTAL + 512));
+  VB_LAUNCH_PDL(shared_attn_kernel<D>, grid + units, PTC_THREADS, PtcLayout<D>::TOTAL + 512, stream, map, p);
+  if (grid > 8 * units) VB_LAUNCH_PDL((shared_join_kernel<D, SJ_WARPS>), dim3(units, m), 32 * SJ_WARPS, 0, stream, p);
+  else VB_LAUNCH_PDL((shared_join_kernel<D, 1>), dim3(units, (m + SJ_WARPS - 1) / SJ_WARPS), 32 * SJ_WARPS, 0, stream, p);
   return 0;
 }
 
@@ -577,15 +530,14 @@ static int check_shared(const char* who, const VbSharedPlan* s) {
   VB_CHECK_ARG(s->columns > 0 && s->columns <= SP_MAX_COLUMNS && static_cast<int64_t>(s->columns) * s->page_size <= 0x3fffffff, "%s: %d pages a row (1 to %d)", who, s->columns,
                SP_MAX_COLUMNS);
   VB_CHECK_ARG(s->grid > 0 && s->grid <= 4096, "%s: %d blocks", who, s->grid);
-  const int sub = shared_sub(s->width, s->n_q / s->n_kv);
   const int64_t pieces = static_cast<int64_t>(s->rows) * s->columns * (s->page_size / sa_piece(s->page_size));
-  VB_CHECK_ARG(pieces * s->n_kv <= 0x3fffffff && sub > 0, "%s: %d rows of %d pages on %d heads", who, s->rows, s->columns, s->n_kv);
+  VB_CHECK_ARG(pieces * s->n_kv <= 0x3fffffff, "%s: %d rows of %d pages on %d heads", who, s->rows, s->columns, s->n_kv);
   return 0;
 }
 
 struct SharedLayout {
   int sub, subs, groups, cap, mpad;
-  size_t entries, parts, ints, stat, acc, bytes;
+  size_t segments, acc, stat, ints, bytes;      // entries first
 };
 static SharedLayout shared_layout(const VbSharedPlan* s) {
   SharedLayout l;
@@ -594,14 +546,13 @@ static SharedLayout shared_layout(const VbSharedPlan* s) {
   l.subs = (s->width + l.sub - 1) / l.sub;
   l.groups = s->rows / s->width * l.subs;
   l.cap = l.sub * s->columns * (s->page_size / sa_piece(s->page_size));
-  l.mpad = 16 * sa_row_tiles(l.sub * G);
-  const size_t slots = static_cast<size_t>(s->grid) + static_cast<size_t>(l.groups) * s->n_kv;
-  l.entries = 0;
-  l.parts = l.entries + 16ull * l.groups * l.cap;
-  l.acc = l.parts + 16ull * s->grid;
-  l.stat = l.acc + 4ull * slots * l.mpad * s->head_dim;
-  l.ints = l.stat + 8ull * slots * l.mpad;
-  l.bytes = l.ints + 4ull * (2ull * l.groups + 1 + s->rows + 2);
+  l.mpad = (l.sub * G + 15) / 16 * 16;
+  const size_t units = static_cast<size_t>(l.groups) * s->n_kv, segments = s->grid + units;
+  l.segments = 16ull * l.groups * l.cap;
+  l.acc = l.segments + 16ull * segments;
+  l.stat = l.acc + 4ull * segments * l.mpad * s->head_dim;
+  l.ints = l.stat + 8ull * segments * l.mpad;
+  l.bytes = l.ints + 4ull * (2ull * l.groups + units + 1 + s->rows);
   return l;
 }
 
@@ -622,16 +573,17 @@ extern "C" int vb_shared_plan(const VbSharedPlan* plan, const int32_t* d_table, 
   const SharedLayout l = shared_layout(plan);
   uint8_t* at = static_cast<uint8_t*>(plan->d_buffer);
   SharedPlanParams p = {};
-  p.entries = reinterpret_cast<int4*>(at + l.entries);
-  p.parts = reinterpret_cast<int4*>(at + l.parts);
-  int32_t* ints = reinterpret_cast<int32_t*>(at + l.ints);
-  p.head = ints, p.counts = ints + 2, p.tile0 = p.counts + l.groups, p.len = p.tile0 + l.groups + 1;
+  p.entries = reinterpret_cast<int4*>(at);
+  p.segments = reinterpret_cast<int4*>(at + l.segments);
+  p.counts = reinterpret_cast<int32_t*>(at + l.ints);
+  p.whole = p.counts + l.groups, p.seg0 = p.whole + l.groups, p.len = p.seg0 + l.groups * plan->n_kv + 1;
   p.table = d_table, p.tokens = d_tokens;
   p.rows = plan->rows, p.width = plan->width, p.sub = l.sub, p.subs = l.subs, p.groups = l.groups, p.cap = l.cap;
   p.columns = plan->columns, p.pages = pages, p.page_size = plan->page_size, p.piece = sa_piece(plan->page_size);
-  p.tile_pieces = sa_tile_tokens(l.mpad / 16) / p.piece, p.heads = plan->n_kv, p.grid = plan->grid;
-  VB_CHECK_CUDA(rm_smem<shared_list_kernel>(SP_MAX_COLUMNS * 4));
-  VB_LAUNCH_PDL(shared_list_kernel, l.groups, SP_THREADS, plan->columns * 4, stream, p);
+  p.tile_pieces = PTC_KT / p.piece, p.heads = plan->n_kv, p.grid = plan->grid;
+  const int cluster = plan->columns > 256 ? SP_CLUSTER : plan->columns > 64 ? 4 : plan->columns > 16 ? 2 : 1;
+  VB_CHECK_CUDA(rm_smem<shared_list_kernel>(SP_MAX_COLUMNS * 8));
+  VB_LAUNCH_PDL_CLUSTER(shared_list_kernel, l.groups * cluster, SP_THREADS, (plan->columns + cluster - 1) / cluster * 8, stream, cluster, p);
   VB_LAUNCH_PDL(shared_deal_kernel, 1, 1024, 0, stream, p);
   return 0;
 }
@@ -642,7 +594,7 @@ extern "C" int vb_shared_attn(void* d_out, const void* d_q, const void* d_kv, in
   VB_CHECK_ARG(d_out && d_q && d_kv, "vb_shared_attn: null pointer");
   VB_CHECK_ARG(slabs > 0 && slabs <= 0x7fffffff && slab_base >= 0 && slab_base < slabs, "vb_shared_attn: slab %lld of %lld", static_cast<long long>(slab_base),
                static_cast<long long>(slabs));
-  VB_CHECK_ARG(reinterpret_cast<uintptr_t>(d_kv) % 16 == 0 && reinterpret_cast<uintptr_t>(d_q) % 4 == 0 && reinterpret_cast<uintptr_t>(d_out) % 4 == 0,
+  VB_CHECK_ARG(reinterpret_cast<uintptr_t>(d_kv) % 16 == 0 && reinterpret_cast<uintptr_t>(d_q) % 16 == 0 && reinterpret_cast<uintptr_t>(d_out) % 16 == 0,
                "vb_shared_attn: unaligned tensors");
   const SharedLayout l = shared_layout(plan);
   const int D = plan->head_dim, H = plan->n_kv, P = plan->page_size, piece = sa_piece(P);
@@ -657,18 +609,16 @@ extern "C" int vb_shared_attn(void* d_out, const void* d_q, const void* d_kv, in
                         CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   VB_CHECK_ARG(r == CUDA_SUCCESS, "vb_shared_attn: cuTensorMapEncodeTiled failed: CUresult %d", static_cast<int>(r));
   uint8_t* at = static_cast<uint8_t*>(plan->d_buffer);
-  const int32_t* ints = reinterpret_cast<const int32_t*>(at + l.ints);
   SharedAttnParams p = {};
-  p.q = static_cast<const __nv_bfloat16*>(d_q), p.out = static_cast<__nv_bfloat16*>(d_out);
-  p.entries = reinterpret_cast<const int4*>(at + l.entries), p.parts = reinterpret_cast<const int4*>(at + l.parts);
-  p.head = ints, p.counts = ints + 2, p.tile0 = p.counts + l.groups, p.len = p.tile0 + l.groups + 1;
-  p.acc = reinterpret_cast<float*>(at + l.acc), p.stat = reinterpret_cast<float*>(at + l.stat);
+  p.q = static_cast<const __nv_bfloat16*>(d_q), p.out = static_cast<__nv_bfloat16*>(d_out), p.kv = static_cast<const __nv_bfloat16*>(d_kv);
+  p.entries = reinterpret_cast<const int4*>(at), p.segments = reinterpret_cast<const int4*>(at + l.segments);
+  p.counts = reinterpret_cast<const int32_t*>(at + l.ints);
+  p.whole = p.counts + l.groups, p.seg0 = p.whole + l.groups, p.len = p.seg0 + l.groups * H + 1;
+  p.acc = reinterpret_cast<float*>(at + l.acc), p.stat = reinterpret_cast<float2*>(at + l.stat);
   p.slab_base = slab_base;
   VB_CHECK_ARG(p.wait_flag = wait_flag(WK_PREFILL_ATTN), "vb_shared_attn: no mapped host memory");
-  p.rows = plan->rows, p.width = plan->width, p.sub = l.sub, p.subs = l.subs, p.groups = l.groups, p.cap = l.cap, p.page_size = P, p.piece = piece, p.piece_log = piece == 64 ? 6 : piece == 32 ? 5 : 4;
-  p.n_q = plan->n_q, p.heads = H, p.G = plan->n_q / H, p.xt_tile = out_xt_tile;
+  p.rows = plan->rows, p.width = plan->width, p.sub = l.sub, p.subs = l.subs, p.groups = l.groups, p.cap = l.cap, p.page_size = P, p.piece = piece;
+  p.tile_pieces = PTC_KT / piece, p.n_q = plan->n_q, p.heads = H, p.G = plan->n_q / H, p.mpad = l.mpad, p.xt_tile = out_xt_tile;
   p.scale_log2 = sm_scale * 1.44269504088896f;
-  const int mt = l.mpad / 16;
-  if (D == 64) return mt == 1 ? launch_shared<64, 1>(map, p, plan->grid, stream) : mt == 2 ? launch_shared<64, 2>(map, p, plan->grid, stream) : launch_shared<64, 4>(map, p, plan->grid, stream);
-  return mt == 1 ? launch_shared<128, 1>(map, p, plan->grid, stream) : mt == 2 ? launch_shared<128, 2>(map, p, plan->grid, stream) : launch_shared<128, 4>(map, p, plan->grid, stream);
+  return D == 64 ? launch_shared<64>(map, p, plan->grid, stream) : launch_shared<128>(map, p, plan->grid, stream);
 }

@@ -2443,13 +2443,13 @@ class SharedPlan:
 
     def __init__(self, rows: int, width: int, columns: int, page_size: int, n_q: int, n_kv: int, head_dim: int, device="cuda"):
         _refuse(rows < 1 or width < 1 or rows % width != 0, f"SharedPlan: {rows} rows in requests of {width}")
-        _refuse(n_kv < 1 or n_q < 1 or n_q % n_kv != 0 or n_q // n_kv > 64, f"SharedPlan: {n_q} query heads on {n_kv} key heads (at most 64 on one)")
+        _refuse(n_kv < 1 or n_q < 1 or n_q % n_kv != 0 or n_q // n_kv > 128, f"SharedPlan: {n_q} query heads on {n_kv} key heads (at most 128 on one)")
         _refuse(head_dim not in (64, 128), f"SharedPlan: heads of {head_dim} (64 or 128)")
         _refuse(page_size < 16 or page_size % 16 != 0 or page_size > 4096, f"SharedPlan: pages of {page_size} tokens (a multiple of 16, at most 4096)")
         _refuse(not 1 <= columns <= 16384, f"SharedPlan: {columns} pages a row (1 to 16384)")
         self.rows, self.width, self.columns, self.page_size, self.n_q, self.n_kv, self.head_dim = (int(v) for v in (rows, width, columns, page_size, n_q, n_kv, head_dim))
         self.pages = 0                                 # of the cache that the plan was made for
-        grid = attn_grid_ctas() if torch.device(device).type == "cuda" else 148
+        grid = 2 * (attn_grid_ctas() if torch.device(device).type == "cuda" else 148)      # two blocks an SM
         self._struct = _lib.SharedPlanStruct(None, self.rows, self.width, self.columns, self.page_size, self.n_q, self.n_kv, self.head_dim, grid)
         self._ptr = ctypes.addressof(self._struct)
         n = (_lib._lib or _lib.load()).vb_shared_plan_bytes(self._ptr)
