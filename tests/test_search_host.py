@@ -182,7 +182,7 @@ def test_plan_cuts_requests_evenly():
 
     def expect(rows, sub, groups, mpad):
         segments = 1 + groups
-        return 16 * groups * sub + 16 * segments + segments * mpad * (64 * 4 + 8) + 4 * (3 * groups + 1 + rows)
+        return 16 * groups * sub + 32 + segments * mpad * (64 * 4 + 8) + 8 * groups + 4 * (3 * groups + 1 + rows)
     assert size(9, 16) == expect(9, 5, 2, 80)          # 8 rows would fit: 5 and 4
     assert size(16, 8) == expect(16, 16, 1, 128)
     assert size(17, 8) == expect(17, 9, 2, 80)

@@ -11,6 +11,8 @@
 //   STAGED                   as bf16 through shared memory; out_at(t, g, c) is then where 16-byte chunk c of a row goes (nullptr: a padding
 //                            row)
 //   HOLE, hole0, hole1       keys [hole0, hole1) are seen by no row of the block: they are neither fetched nor multiplied
+//   CHAINED, next_q()        the block walks several row tiles one after the other: `base` tiles and `walk` walks lie behind this one, the stages and their
+//                            barriers go on from there, and next_q brings the next walk's query rows once this one's last scores have been multiplied
 // The running maximum, its rescale and the division at the end are the online softmax of M. Milakov and N. Gimelshein ("Online normalizer
 // calculation for softmax", 2018) as FlashAttention walks it over key tiles (T. Dao et al., 2022); the roles of the warps and scores
 // multiplied one tile ahead follow the published schedule of FlashAttention-3 (J. Shah et al., 2024).
@@ -220,37 +222,60 @@ __device__ __forceinline__ void ptc_finish_rows(uint8_t* smem, const Rows& rows,
   }
 }
 
-// ================= warps 0..3: softmax =================
+// ================= warps 0..3: query rows, softmax =================
 template <int D, class Rows>
-__device__ __forceinline__ void ptc_softmax(uint8_t* smem, PtcShared* sh, const Rows& rows, BoundedWait& bw) {
+__device__ __forceinline__ void ptc_load_q(uint8_t* smem, PtcShared* sh, const Rows& rows) {
   using L = PtcLayout<D>;
   constexpr int KBD = D / 64, CPR = D * 2 / 16;
-  const int tid = threadIdx.x, warp = tid >> 5, n_tiles = rows.n_tiles;
-  {
-    // CPR neighbouring threads take a row: a warp reads whole rows, four or two at a time.  (A row per thread, 16 bytes of 32 rows an
-    // instruction: the rows were there after 6 us instead of 2.)
-    __nv_bfloat16* sQ = reinterpret_cast<__nv_bfloat16*>(smem + L::Q);
-    constexpr int STEP = 128 / CPR;
-    const int c = tid % CPR, r0 = tid / CPR;
-    uint4 v[CPR];
-    PtcWalk<STEP> w(r0, rows.group);
+  const int tid = threadIdx.x;
+  // CPR neighbouring threads take a row: a warp reads whole rows, four or two at a time.  (A row per thread, 16 bytes of 32 rows an
+  // instruction: the rows were there after 6 us instead of 2.)
+  __nv_bfloat16* sQ = reinterpret_cast<__nv_bfloat16*>(smem + L::Q);
+  constexpr int STEP = 128 / CPR;
+  const int c = tid % CPR, r0 = tid / CPR;
+  uint4 v[CPR];
+  PtcWalk<STEP> w(r0, rows.group);
 #pragma unroll
-    for (int i = 0; i < CPR; ++i, w.next()) {
-      const __nv_bfloat16* src = rows.q_row(w.t, w.g);
-      v[i] = make_uint4(0u, 0u, 0u, 0u);
-      if (src) v[i] = *reinterpret_cast<const uint4*>(src + c * 8);
-    }
-#pragma unroll
-    for (int i = 0; i < CPR; ++i) *reinterpret_cast<uint4*>(sQ + xt_index(r0 + i * STEP, c * 8, 128, KBD)) = v[i];
-    fence_proxy_async();
-    mbar_arrive(&sh->q_full);
+  for (int i = 0; i < CPR; ++i, w.next()) {
+    const __nv_bfloat16* src = rows.q_row(w.t, w.g);
+    v[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (src) v[i] = *reinterpret_cast<const uint4*>(src + c * 8);
   }
+#pragma unroll
+  for (int i = 0; i < CPR; ++i) *reinterpret_cast<uint4*>(sQ + xt_index(r0 + i * STEP, c * 8, 128, KBD)) = v[i];
+  fence_proxy_async();
+  mbar_arrive(&sh->q_full);
+}
+// A warp whose rows are all padding: what it would compute nobody reads.  It keeps the others' pace only (its probabilities are whatever its scores were).
+template <class Rows>
+__device__ __forceinline__ void ptc_idle(PtcShared* sh, const Rows& rows, BoundedWait& bw, int base, int walk) {
+  for (int j = 0; j < rows.n_tiles; ++j) {
+    const int b = base + j;
+    bw.wait(&sh->s_full[b & 1], (b >> 1) & 1);
+    if (!__all_sync(0xffffffffu, !bw.dead)) {
+      bw.dead = true;
+      return;
+    }
+    tc_fence_after();
+    tc_fence_before();
+    mbar_arrive(&sh->p_full[b & 1]);
+  }
+  rows.next_q();
+  bw.wait(&sh->o_last, walk & 1);
+  if (!__all_sync(0xffffffffu, !bw.dead)) bw.dead = true;
+  tc_fence_after();
+}
+template <int D, class Rows>
+__device__ __forceinline__ void ptc_softmax(uint8_t* smem, PtcShared* sh, const Rows& rows, BoundedWait& bw, int base = 0, int walk = 0) {
+  const int tid = threadIdx.x, warp = tid >> 5, n_tiles = rows.n_tiles;
+  if constexpr (!Rows::CHAINED) ptc_load_q<D>(smem, sh, rows);
   const uint32_t t_lane = sh->tmem + (static_cast<uint32_t>(warp * 32) << 16);   // this warp's TMEM lane quarter
   const float scale = rows.scale_log2 > 0.f ? rows.scale_log2 : 1.f;
   float m_ref = -INFINITY, l_run = 0.f;            // the exponents' reference and the denominator against it
   for (int j = 0; j < n_tiles && !bw.dead; ++j) {
-    const uint32_t sc = t_lane + (j & 1) * 64;
-    bw.wait(&sh->s_full[j & 1], (j >> 1) & 1);
+    const int b = base + j;
+    const uint32_t sc = t_lane + (b & 1) * 64;
+    bw.wait(&sh->s_full[b & 1], (b >> 1) & 1);
     if (!__all_sync(0xffffffffu, !bw.dead)) { bw.dead = true; break; }
     tc_fence_after();
     uint32_t v[64];
@@ -287,7 +312,7 @@ __device__ __forceinline__ void ptc_softmax(uint8_t* smem, PtcShared* sh, const 
       if (move) m_ref = mx;
       l_run *= alpha;
       if (j > 0) {
-        bw.wait(&sh->o_done, (j - 1) & 1);                                   // tile j - 1 has been added
+        bw.wait(&sh->o_done, (b - 1) & 1);                                   // tile j - 1 has been added
         if (!__all_sync(0xffffffffu, !bw.dead)) { bw.dead = true; break; }
         tc_fence_after();
 #pragma unroll 1
@@ -320,11 +345,12 @@ __device__ __forceinline__ void ptc_softmax(uint8_t* smem, PtcShared* sh, const 
     ptc_tmem_st32(sc + 32, pl);
     ptc_tmem_st_wait();
     tc_fence_before();
-    mbar_arrive(&sh->p_full[j & 1]);
+    mbar_arrive(&sh->p_full[b & 1]);
   }
+  if constexpr (Rows::CHAINED) rows.next_q();
   // ---- normalise and store this thread's row ----
   if (n_tiles > 0 && !bw.dead) {
-    bw.wait(&sh->o_last, 0);
+    bw.wait(&sh->o_last, walk & 1);
     if (!__all_sync(0xffffffffu, !bw.dead)) bw.dead = true;
   }
   if (!bw.dead) ptc_finish_rows<D>(smem, rows, t_lane, n_tiles, m_ref, l_run);
@@ -333,7 +359,7 @@ __device__ __forceinline__ void ptc_softmax(uint8_t* smem, PtcShared* sh, const 
 
 // ================= warp 4: MMA issuer (the whole warp walks the loop, one elected lane issues: operands stay in uniform registers) =================
 template <int D>
-__device__ __forceinline__ void ptc_issue(uint8_t* smem, PtcShared* sh, int n_tiles, BoundedWait& bw) {
+__device__ __forceinline__ void ptc_issue(uint8_t* smem, PtcShared* sh, int n_tiles, BoundedWait& bw, int base = 0, int walk = 0) {
   using L = PtcLayout<D>;
   constexpr int KBD = D / 64;
   const uint32_t tmem = sh->tmem;
@@ -344,44 +370,47 @@ __device__ __forceinline__ void ptc_issue(uint8_t* smem, PtcShared* sh, int n_ti
     return !bw.dead;
   };
   auto scores = [&](int j) {
-    bw.wait(&sh->k_full[j & 1], (j >> 1) & 1);
+    const int b = base + j;
+    bw.wait(&sh->k_full[b & 1], (b >> 1) & 1);
     if (!alive()) return;
     tc_fence_after();
-    const uint64_t k_desc = umma_desc_sw128_kmajor(smem_u32(smem + L::K + (j & 1) * L::TILE));
+    const uint64_t k_desc = umma_desc_sw128_kmajor(smem_u32(smem + L::K + (b & 1) * L::TILE));
     if (elect_one()) {
 #pragma unroll
       for (int kb = 0; kb < KBD; ++kb)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
-          umma_bf16(tmem + (j & 1) * 64, q_desc + kb * (128 * 128 >> 4) + 2 * k, k_desc + kb * (PTC_KT * 128 >> 4) + 2 * k, idesc_s,
+          umma_bf16(tmem + (b & 1) * 64, q_desc + kb * (128 * 128 >> 4) + 2 * k, k_desc + kb * (PTC_KT * 128 >> 4) + 2 * k, idesc_s,
                     (kb > 0 || k > 0) ? 1u : 0u);
-      umma_commit(&sh->k_empty[j & 1]);
-      umma_commit(&sh->s_full[j & 1]);
+      umma_commit(&sh->k_empty[b & 1]);
+      umma_commit(&sh->s_full[b & 1]);
     }
     __syncwarp();
   };
   if (n_tiles > 0) {
-    bw.wait(&sh->q_full, 0);
+    bw.wait(&sh->q_full, walk & 1);
+    if (base > 0) bw.wait(&sh->o_done, (base - 1) & 1);      // (the walk in front: both score buffers are free)
     if (alive()) scores(0);
   }
   for (int j = 0; j < n_tiles && !bw.dead; ++j) {
+    const int b = base + j;
     if (j + 1 < n_tiles) {
       // the other score buffer holds the probabilities of tile j - 1 until they have been multiplied
-      if (j > 0) bw.wait(&sh->o_done, (j - 1) & 1);
+      if (j > 0) bw.wait(&sh->o_done, (b - 1) & 1);
       if (alive()) scores(j + 1);
     }
-    bw.wait(&sh->p_full[j & 1], (j >> 1) & 1);
-    bw.wait(&sh->v_full[j & 1], (j >> 1) & 1);
+    bw.wait(&sh->p_full[b & 1], (b >> 1) & 1);
+    bw.wait(&sh->v_full[b & 1], (b >> 1) & 1);
     if (!alive()) break;
     tc_fence_after();
-    const uint64_t v_desc = umma_desc_sw128_mnmajor(smem_u32(smem + L::V + (j & 1) * L::TILE), PTC_KT * 128);
+    const uint64_t v_desc = umma_desc_sw128_mnmajor(smem_u32(smem + L::V + (b & 1) * L::TILE), PTC_KT * 128);
     if (elect_one()) {
 #pragma unroll
       for (int k = 0; k < PTC_KT / 16; ++k) {        // 16 tokens: 8 columns of either term of the probabilities, two 8-row groups of V
-        umma_bf16_ta(tmem + 128, tmem + (j & 1) * 64 + 32 + 8 * k, v_desc + k * (2048 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
-        umma_bf16_ta(tmem + 128, tmem + (j & 1) * 64 + 8 * k, v_desc + k * (2048 >> 4), idesc_o, 1u);
+        umma_bf16_ta(tmem + 128, tmem + (b & 1) * 64 + 32 + 8 * k, v_desc + k * (2048 >> 4), idesc_o, (j > 0 || k > 0) ? 1u : 0u);
+        umma_bf16_ta(tmem + 128, tmem + (b & 1) * 64 + 8 * k, v_desc + k * (2048 >> 4), idesc_o, 1u);
       }
-      umma_commit(&sh->v_empty[j & 1]);
+      umma_commit(&sh->v_empty[b & 1]);
       umma_commit(&sh->o_done);
       if (j + 1 == n_tiles) umma_commit(&sh->o_last);
     }

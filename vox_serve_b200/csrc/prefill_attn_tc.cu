@@ -56,7 +56,7 @@ struct PrefillTcParams {
 
 // what this thread's row sees: the first kl keys of its request
 struct PagedRows {
-  static constexpr bool HOLE = false, STAGED = true;
+  static constexpr bool HOLE = false, STAGED = true, CHAINED = false;
   static constexpr int hole0 = 0, hole1 = 0;
   const PrefillTcParams& p;
   int n_tiles, kl, row0, nrows, head0, group, D;

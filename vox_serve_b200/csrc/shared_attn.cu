@@ -7,13 +7,14 @@
 // rows of the tcgen05 core (attn_tc.cuh): a tile of 64 keys meets all of them while it is on chip.
 //
 //   plan (once a step)   a cluster a group lists its different pages in pieces of 16 to 64 tokens {place in the cache, position, rows, tokens}: first the tiles
-//                        that all living rows see whole, then the rest; a block cuts the tiles of every group and key head into segments, two an SM in all
-//   attention            a block a segment: maximum, denominator and unnormalised output of its rows
+//                        that all living rows see whole, then the rest; the tiles of every group and key head are cut into equal segments, as many as there are
+//                        blocks (two an SM); where there are more groups and heads than blocks, a block gets an equal stretch of all of them
+//   attention            a block walks its segments: maximum, denominator and unnormalised output of each one's rows
 //   join                 the segments of a group and head meet, in their order
 //
 // Tiles that are seen whole need no masks.  In the others a row's probability is 0 where it does not see, and 0 times what is not finite is not 0.  So a block
-// whose results are not finite, and that had such tiles, walks its segment again: values that are not finite are taken out on the way, and the rows that see
-// them get them back at the end.  Finite caches never go there; what stands behind a row's last token is cleared in any case.
+// whose results are not finite, and that had such tiles, walks its segments again: values that are not finite are taken out on the way, and the rows that see
+// them get them back at the end.  Caches that hold finite numbers everywhere, behind a row's last token too, never go there.
 // Probabilities enter the second product as two bf16 parts (2^-17).
 #include "../../include/vb_api.h"
 #define VB_PDL_FAMILY 1
@@ -23,14 +24,20 @@
 namespace vb {
 
 constexpr int SA_MAX_ROWS = 128;                 // rows of a group times query heads of a key head
+// behind the operands: two sets of barriers, four tiles' pieces, results on their way out
+template <int D>
+constexpr int SA_OUT = PtcLayout<D>::BAR + 768;
+template <int D>
+constexpr int SA_SMEM = SA_OUT<D> + 128 * 64 + 1024;
 inline int sa_piece(int page_size) { return page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : 16; }
 
 // ---- the plan -------------------------------------------------------------------------------------------------------------------
 struct SharedPlanParams {
   int4* entries;                 // [groups][cap]: {token's place in a layer's pages, its position, rows that hold it, tokens}
-  int4* segments;                // [grid + units] {group, head, first tile, tiles}
+  int4* parts;                   // [grid][2] {group, head, first tile, tiles}, {pieces of the group, its tiles that are seen whole}
   int32_t *counts, *whole, *len; // [groups] pieces and tiles that are seen whole, [rows]
-  int32_t* seg0;                 // [units + 1] segments in front of a unit
+  int32_t* tile0;                // [groups + 1] tiles in front of a group
+  int2* blocks_of;               // [units] first and last block of a unit
   const int32_t *table, *tokens;
   int rows, width, sub, subs, groups, cap, columns, pages, page_size, piece, tile_pieces, heads, grid;
 };
@@ -163,41 +170,13 @@ __global__ void __launch_bounds__(SP_THREADS) shared_list_kernel(const __grid_co
 }
 
 __global__ void __launch_bounds__(1024) shared_deal_kernel(const __grid_constant__ SharedPlanParams p) {
-  __shared__ int sums[33];
+  __shared__ int sums[32];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_sync();
-  auto tiles_of = [&](int g) { return (__ldcg(p.counts + g) + p.tile_pieces - 1) / p.tile_pieces; };
-  // sum (op 0) or maximum over the block
-  auto meet = [&](int v, bool maximum) {
-    v = maximum ? __reduce_max_sync(0xffffffffu, v) : __reduce_add_sync(0xffffffffu, v);
-    __syncthreads();
-    if (lane == 0) sums[warp] = v;
-    __syncthreads();
-    v = sums[lane];
-    return maximum ? __reduce_max_sync(0xffffffffu, v) : __reduce_add_sync(0xffffffffu, v);
-  };
-  int mine = 0, longest = 0;
-  for (int g = tid; g < p.groups; g += 1024) {
-    const int t = tiles_of(g);
-    mine += t, longest = max(longest, t);
-  }
-  const int total = meet(mine, false) * p.heads, most = meet(longest, true);
-  // tiles of a segment: the fewest with which all segments run at once, where that is possible
-  int lo = max(1, (total + p.grid - 1) / p.grid), hi = max(lo, most);
-  while (lo < hi) {
-    const int mid = (lo + hi) >> 1;
-    mine = 0;
-    for (int g = tid; g < p.groups; g += 1024) mine += (tiles_of(g) + mid - 1) / mid;
-    if (meet(mine, false) * p.heads <= p.grid) hi = mid;
-    else lo = mid + 1;
-  }
-  const int units = p.groups * p.heads;
-  const int each = units <= p.grid ? lo : max(1, (total + p.grid - 1) / p.grid);
   int carry = 0;
-  for (int u0 = 0; u0 < units; u0 += 1024) {
-    const int u = u0 + tid, g = u / p.heads, h = u - g * p.heads;
-    const int tiles = u < units ? tiles_of(g) : 0, n = (tiles + each - 1) / each;
-    int inc = n;
+  for (int g0 = 0; g0 < p.groups; g0 += 1024) {
+    const int g = g0 + tid, mine = g < p.groups ? (__ldcg(p.counts + g) + p.tile_pieces - 1) / p.tile_pieces : 0;
+    int inc = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, inc, o);
@@ -206,30 +185,98 @@ __global__ void __launch_bounds__(1024) shared_deal_kernel(const __grid_constant
     __syncthreads();
     if (lane == 31) sums[warp] = inc;
     __syncthreads();
-    int before = carry, all = carry;
-    for (int w = 0; w < 32; ++w) {
-      if (w < warp) before += sums[w];
-      all += sums[w];
-    }
-    const int at = before + inc - n;
-    if (u < units) {
-      p.seg0[u] = at;
-      for (int i = 0; i < n; ++i) p.segments[at + i] = make_int4(g, h, i * each, min(each, tiles - i * each));
-    }
-    carry = all;
+    int all = sums[lane], before = lane < warp ? all : 0;
+    all = __reduce_add_sync(0xffffffffu, all), before = __reduce_add_sync(0xffffffffu, before);
+    if (g < p.groups) p.tile0[g] = carry + before + inc - mine;
+    carry += all;
   }
-  if (tid == 0) p.seg0[units] = carry;
-  for (int i = carry + tid; i < p.grid + units; i += 1024) p.segments[i] = make_int4(0, 0, 0, 0);
+  const int total = carry, units = p.groups * p.heads;
+  const long long work = static_cast<long long>(total) * p.heads;
+  if (tid == 0) p.tile0[p.groups] = total;
+  __syncthreads();
+  auto tile0 = [&](int g) { return __ldcg(p.tile0 + g); };
+  auto sum_of = [&](int v) {
+    v = __reduce_add_sync(0xffffffffu, v);
+    __syncthreads();
+    if (lane == 0) sums[warp] = v;
+    __syncthreads();
+    return __reduce_add_sync(0xffffffffu, sums[lane]);
+  };
+  if (units <= p.grid) {
+    // Blocks of their own for every unit (one that goes on to another unit waits for it: 5 us): equal segments of at most q tiles, q the smallest with which
+    // the blocks are enough.
+    int lo = static_cast<int>(max(1ll, (work + p.grid - 1) / p.grid)), hi = max(lo, total);
+    while (lo < hi) {
+      const int q = (lo + hi) >> 1;
+      int mine = 0;
+      for (int g = tid; g < p.groups; g += 1024) mine += (tile0(g + 1) - tile0(g) + q - 1) / q;
+      if (sum_of(mine) * p.heads <= p.grid) hi = q;
+      else lo = q + 1;
+    }
+    int used = 0;
+    for (int u0 = 0; u0 < units; u0 += 1024) {
+      const int u = u0 + tid, g = u / p.heads, tiles = u < units ? tile0(g + 1) - tile0(g) : 0, n = (tiles + lo - 1) / lo;
+      int inc = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, inc, o);
+        if (lane >= o) inc += v;
+      }
+      __syncthreads();
+      if (lane == 31) sums[warp] = inc;
+      __syncthreads();
+      int all = sums[lane], before = lane < warp ? all : 0;
+      all = __reduce_add_sync(0xffffffffu, all), before = __reduce_add_sync(0xffffffffu, before);
+      const int at = used + before + inc - n;
+      if (u < units) {
+        p.blocks_of[u] = make_int2(at, at + n - 1);
+        const int4 of = make_int4(__ldcg(p.counts + g), __ldcg(p.whole + g), 0, 0);
+        for (int i = 0; i < n; ++i) {
+          const int from = static_cast<int>(static_cast<long long>(tiles) * i / n), to = static_cast<int>(static_cast<long long>(tiles) * (i + 1) / n);
+          p.parts[2 * (at + i)] = make_int4(g, u - g * p.heads, from, to - from), p.parts[2 * (at + i) + 1] = of;
+        }
+      }
+      used += all;
+    }
+    for (int i = used + tid; i < p.grid; i += 1024) p.parts[2 * i] = make_int4(0, 0, 0, 0);
+    return;
+  }
+  // More units than blocks: equal stretches of all their tiles in a line
+  const long long blocks = min(work, static_cast<long long>(p.grid));      // (none without a tile: the join counts on it)
+  for (int i = tid; i < p.grid; i += 1024) {
+    int4 part = make_int4(0, 0, 0, 0), of = part;
+    if (i < blocks) {
+      const long long start = work * i / blocks;
+      int lo = 0, hi = p.groups - 1;                    // the last group that begins at or before the start (of several the others are empty)
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (static_cast<long long>(tile0(mid)) * p.heads <= start) lo = mid;
+        else hi = mid - 1;
+      }
+      const int t0 = tile0(lo), tiles = tile0(lo + 1) - t0, in = static_cast<int>(start - static_cast<long long>(t0) * p.heads);
+      part = make_int4(lo, in / tiles, in % tiles, static_cast<int>(work * (i + 1) / blocks - start));
+      of = make_int4(__ldcg(p.counts + lo), __ldcg(p.whole + lo), 0, 0);
+    }
+    p.parts[2 * i] = part, p.parts[2 * i + 1] = of;
+  }
+  for (int u = tid; u < units; u += 1024) {
+    const int g = u / p.heads, t0 = tile0(g), tiles = tile0(g + 1) - t0;
+    const long long first = static_cast<long long>(t0) * p.heads + static_cast<long long>(u - g * p.heads) * tiles;
+    // (whose stretch holds a tile)
+    if (tiles) p.blocks_of[u] = make_int2(static_cast<int>(((first + 1) * blocks - 1) / work), static_cast<int>(((first + tiles) * blocks - 1) / work));
+    else p.blocks_of[u] = make_int2(0, -1);
+  }
 }
 
 // ---- attention -------------------------------------------------------------------------------------------------------------------
 struct SharedAttnParams {
   const __nv_bfloat16 *q, *kv;
   __nv_bfloat16* out;
-  const int4 *entries, *segments;
-  const int32_t *counts, *whole, *len, *seg0;
-  float* acc;                    // [segments][mpad][D]
-  float2* stat;                  // [segments][mpad] maximum (base 2), denominator against it
+  const int4 *entries, *parts;
+  const int32_t *counts, *whole, *len;
+  const int2* blocks_of;         // [units]
+  float* acc;                    // [blocks + units][mpad][D]: the segment of block b on unit u stands at b + u
+  float2* stat;                  // [blocks + units][mpad] maximum (base 2), denominator against it
   long long slab_base;
   unsigned char* wait_flag;
   int rows, width, sub, subs, groups, cap, page_size, piece, tile_pieces, n_q, heads, G, mpad, xt_tile;
@@ -242,91 +289,151 @@ __device__ __forceinline__ int shared_group(const SharedAttnParams& p, int g, in
   return g / p.subs * p.width + in;
 }
 
+// A block's stretch, segment by segment
+struct SharedWalk {
+  const SharedAttnParams& p;
+  int g, h, t, left;             // group, key head, first tile; tiles of the stretch from here on
+  int count, whole, tiles;       // of the group
+  __device__ __forceinline__ SharedWalk(const SharedAttnParams& p_, const int4& part, const int4& of)
+      : p(p_), g(part.x), h(part.y), t(part.z), left(part.w), count(of.x), whole(of.y), tiles((of.x + p_.tile_pieces - 1) / p_.tile_pieces) {}
+  __device__ __forceinline__ int here() const { return min(left, tiles - t); }      // tiles of the segment
+  __device__ __forceinline__ void step(int n) {                                     // n tiles on, within the segment
+    t += n, left -= n;
+    if (t < tiles || left <= 0) return;
+    t = 0;
+    if (++h < p.heads) return;
+    h = 0;
+    do {
+      ++g;
+      count = p.counts[g];
+    } while (count == 0);        // (tiles are left, so there is one)
+    whole = p.whole[g], tiles = (count + p.tile_pieces - 1) / p.tile_pieces;
+  }
+};
+
+// Tokens of a tile that a row sees: it holds the page, and the token is not behind its last
+__device__ __forceinline__ uint64_t shared_mask(const int4* pieces, int n_pieces, int piece, int bit, int len) {
+  uint64_t m = 0ull;
+  for (int i = 0; i < n_pieces; ++i) {
+    const int4 e = pieces[i];
+    const int n = (static_cast<uint32_t>(e.z) >> bit & 1u) ? min(len - e.y, e.w) : 0;
+    if (n > 0) m |= (n < 64 ? (1ull << n) - 1ull : ~0ull) << (i * piece);
+  }
+  return m;
+}
+// What is not finite among the values that a row sees in the segment's tiles with masks, where it was taken out: 32 dimensions from c0.  (Not a member: an
+// object that is handed on lives in memory.)
+template <int D>
+__device__ __noinline__ void shared_give_back(const SharedAttnParams& p, const int4* entries, int count, int from, int to, int head, int bit, int len, int c0, float* v) {
+  for (int t = from; t < to; ++t) {
+    const int first = t * p.tile_pieces;
+    const uint64_t m = shared_mask(entries + first, min(p.tile_pieces, count - first), p.piece, bit, len);
+    for (int k = 0; k < PTC_KT; ++k) {
+      if (!(m >> k & 1ull)) continue;
+      const int tok = entries[first + k / p.piece].x + k % p.piece, page = tok / p.page_size, slot = tok - page * p.page_size;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(p.kv + ((((p.slab_base + page) * 2 + 1) * p.page_size + slot) * p.heads + head) * D + c0);
+      for (int i = 0; i < 16; ++i) {
+        const uint32_t w = src[i];
+        if ((w & 0x7f80u) == 0x7f80u) v[2 * i] += bf16_lo(w);
+        if ((w & 0x7f800000u) == 0x7f800000u) v[2 * i + 1] += bf16_hi(w);
+      }
+    }
+  }
+}
+
 // what this thread's row sees of a segment, and where its part goes
 template <int D>
 struct SharedRows {
-  static constexpr bool HOLE = false, STAGED = false;
+  static constexpr bool HOLE = false, STAGED = false, CHAINED = true;
   static constexpr int hole0 = 0, hole1 = 0;
   const SharedAttnParams& p;
   uint8_t* smem;
-  const int4 *entries, *meta;    // of the group; of the last four tiles with masks
+  PtcShared* sh;
+  const int4 *entries, *meta;    // of the group; of the block's last four tiles, as far as they have masks
+  int base;                      // tiles of the block in front of the segment
   int count, whole, t0, n_tiles; // pieces; tiles that need no mask; the segment
   int row0, n_rows, head, group; // first row, rows, key head, query heads of it
   int len, bit;
   bool ok;
   float scale_log2;
   float2* stat;
+  float* acc;                    // of the segment
+  int next_g, next_h;            // the segment behind this one; -1: none
   bool careful;                  // values that are not finite have been taken out
   mutable bool bad;              // a result that is not finite
   mutable uint64_t seen;
   __device__ __forceinline__ int tile(int it) const { return t0 + it; }
-  __device__ __forceinline__ int4 piece(int i) const { return i < count ? entries[i] : make_int4(0, 0, 0, 0); }
-  __device__ __forceinline__ uint64_t mask(const int4* pieces, int n_pieces) const {
-    uint64_t m = 0ull;
-    for (int i = 0; i < n_pieces; ++i) {
-      const int4 e = pieces[i];
-      const int n = (static_cast<uint32_t>(e.z) >> bit & 1u) ? min(len - e.y, e.w) : 0;
-      if (n > 0) m |= (n < 64 ? (1ull << n) - 1ull : ~0ull) << (i * p.piece);
-    }
-    return m;
-  }
   __device__ __forceinline__ bool full(int tok0) const {
     seen = ~0ull;
     const int t = tok0 / PTC_KT;
-    if (t >= whole && ok) seen = mask(meta + (t - t0 & 3) * 4, p.tile_pieces);      // (a row that is none may have anything)
+    if (t >= whole && ok) seen = shared_mask(meta + (base + t - t0 & 3) * 4, p.tile_pieces, p.piece, bit, len);      // (a row that is none may have anything)
     return seen == ~0ull;
   }
   __device__ __forceinline__ bool visible(int kj) const { return seen >> (kj & (PTC_KT - 1)) & 1ull; }
   __device__ __forceinline__ const __nv_bfloat16* q_row(int t, int g) const {
     return t < n_rows ? p.q + (static_cast<size_t>(row0 + t) * p.n_q + head * group + g) * D : nullptr;
   }
+  struct Query {                 // of the segment behind this one
+    const SharedAttnParams& p;
+    int row0, n_rows, head, group;
+    __device__ __forceinline__ const __nv_bfloat16* q_row(int t, int g) const {
+      return t < n_rows ? p.q + (static_cast<size_t>(row0 + t) * p.n_q + head * group + g) * D : nullptr;
+    }
+  };
+  __device__ __forceinline__ void next_q() const {
+    if (next_g < 0) return;
+    Query q{p, 0, 0, next_h, group};
+    q.row0 = shared_group(p, next_g, q.n_rows);
+    ptc_load_q<D>(smem, sh, q);
+  }
   __device__ __forceinline__ uint4* out_at(int, int, int) const { return nullptr; }
   __device__ __forceinline__ float finish(float m_ref, float l) const {
     if (ok) *stat = make_float2(m_ref, l);
     return 1.f;
   }
-  // a thread's row goes to the place of the keys and values (they have been multiplied): 16-byte chunk c of row r at chunk c ^ (r & 15) of its 16 or 32
-  __device__ __forceinline__ float4* staged(int r, int c) const { return reinterpret_cast<float4*>(smem + PtcLayout<D>::K) + r * (D / 4) + ((c & ~15) | ((c ^ r) & 15)); }
+  // 32 values of a warp's rows go out in whole sectors, 16 at a time through shared memory: 16-byte chunk c of row r at chunk c ^ (r / 2 & 3)
   __device__ __forceinline__ void store(int c0, const uint32_t (&o)[32], float) const {
     float v[32];
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(o[i]);
-    if (careful && ok) give_back(c0, v);
+    if (careful && ok) {                                      // (a copy: an array that is handed on lives in memory)
+      float w[32];
+#pragma unroll
+      for (int i = 0; i < 32; ++i) w[i] = v[i];
+      shared_give_back<D>(p, entries, count, max(t0, whole), t0 + n_tiles, head, bit, len, c0, w);
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = w[i];
+    }
 #pragma unroll
     for (int i = 0; i < 32; ++i) bad |= !isfinite(v[i]);
+    const int lane = threadIdx.x & 31, row = threadIdx.x - lane;
+    float4* mine = reinterpret_cast<float4*>(smem + SA_OUT<D>) + row * 4;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) *staged(threadIdx.x, (c0 >> 2) + c) = make_float4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
-  }
-  // what is not finite among the values that the row sees, in tiles where it was taken out
-  __device__ __noinline__ void give_back(int c0, float (&v)[32]) const {
-    for (int t = max(t0, whole); t < t0 + n_tiles; ++t) {
-      const int first = t * p.tile_pieces;
-      const uint64_t m = mask(entries + first, min(p.tile_pieces, count - first));
-      for (int k = 0; k < PTC_KT; ++k) {
-        if (!(m >> k & 1ull)) continue;
-        const int4 e = piece(t * p.tile_pieces + k / p.piece);
-        const int tok = e.x + k % p.piece, page = tok / p.page_size, slot = tok - page * p.page_size;
-        const uint32_t* src = reinterpret_cast<const uint32_t*>(p.kv + ((((p.slab_base + page) * 2 + 1) * p.page_size + slot) * p.heads + head) * D + c0);
-        for (int i = 0; i < 16; ++i) {
-          const uint32_t w = src[i];
-          if ((w & 0x7f80u) == 0x7f80u) v[2 * i] += bf16_lo(w);
-          if ((w & 0x7f800000u) == 0x7f800000u) v[2 * i + 1] += bf16_hi(w);
-        }
+    for (int half = 0; half < 2; ++half) {
+      __syncwarp();
+#pragma unroll
+      for (int c = 0; c < 4; ++c)
+        mine[lane * 4 + (c ^ (lane >> 1 & 3))] = make_float4(v[16 * half + 4 * c], v[16 * half + 4 * c + 1], v[16 * half + 4 * c + 2], v[16 * half + 4 * c + 3]);
+      __syncwarp();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = i * 8 + (lane >> 2), c = lane & 3;
+        if (row + r < n_rows * group) *reinterpret_cast<float4*>(acc + (row + r) * D + c0 + 16 * half + c * 4) = mine[r * 4 + (c ^ (r >> 1 & 3))];
       }
     }
   }
 };
 
-// A lane a piece of the tile: its boxes, K or V
+// A lane a piece of the tile: its boxes, K or V.  A place without a piece gets the first one again: what stands there is multiplied by probability 0, and what
+// an earlier kernel left in shared memory need not be finite.
 template <int D>
 __device__ __forceinline__ void shared_fetch(const SharedAttnParams& p, const CUtensorMap* map, const int4& e, int part, int head, uint32_t dst, uint64_t* bar) {
   const int lane = threadIdx.x & 31;
-  const bool has = e.w > 0;
-  const int n = __popc(__ballot_sync(0xffffffffu, has));
-  if (lane == 0) mbar_arrive_expect_tx(bar, n * p.piece * D * 2);
+  const int first = __shfl_sync(0xffffffffu, e.x, 0), at = e.w > 0 ? e.x : first;
+  if (lane == 0) mbar_arrive_expect_tx(bar, PTC_KT * D * 2);
   __syncwarp();
-  if (has) {
-    const int page = e.x / p.page_size, slot = e.x - page * p.page_size;
+  if (lane < p.tile_pieces) {
+    const int page = at / p.page_size, slot = at - page * p.page_size;
 #pragma unroll
     for (int kb = 0; kb < D / 64; ++kb)
       ptc_tma_5d(dst + kb * (PTC_KT * 128) + lane * p.piece * 128, map, smem_u32(bar), kb * 64, slot, head, part, static_cast<int>(p.slab_base + page));
@@ -344,10 +451,6 @@ __global__ void __launch_bounds__(PTC_THREADS, 2) shared_attn_kernel(const __gri
   int4* meta = reinterpret_cast<int4*>(smem + L::BAR + 512);
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   BoundedWait bw{p.wait_flag};
-  pdl_wait();
-  const int4 seg = p.segments[blockIdx.x];
-  pdl_trigger();
-  if (seg.w == 0) return;
   if (tid == 0) {
     ptc_init(sh, 1);
     ptc_init(sh2, 1);
@@ -362,90 +465,108 @@ __global__ void __launch_bounds__(PTC_THREADS, 2) shared_attn_kernel(const __gri
   tc_fence_after();
   const uint32_t tmem_base = sh->tmem;
   if (tid == 0) sh2->tmem = tmem_base;
-
-  const int g = seg.x, head = seg.y, n_tiles = seg.w;
-  int n_rows;
-  const int row0 = shared_group(p, g, n_rows), t = tid / p.G;
-  const bool ok = warp < 4 && t < n_rows;
-  SharedRows<D> rows{p, smem, p.entries + static_cast<long long>(g) * p.cap, meta, p.counts[g], p.whole[g], seg.z, n_tiles, row0, n_rows, head, p.G,
-                     ok ? p.len[row0 + t] : 0, ok ? t : 0, ok, p.scale_log2, p.stat + static_cast<long long>(blockIdx.x) * p.mpad + tid, false, false, ~0ull};
+  pdl_wait();
+  const int4 part = p.parts[2 * blockIdx.x], of = p.parts[2 * blockIdx.x + 1];
+  pdl_trigger();
 #pragma unroll 1
-  for (int pass = 0;; ++pass) {
-    rows.careful = pass != 0;
-    rows.bad = false;
+  for (int pass = 0; part.w > 0; ++pass) {
+    bool bad = false;
+    const bool careful = pass != 0;
+    SharedWalk w(p, part, of);
     if (warp < 4) {
-      ptc_softmax<D>(smem, sh, rows, bw);
-      fence_proxy_async();                                    // (results stand where keys and values may come again)
+      for (int base = 0, walk = 0; w.left > 0 && !bw.dead; ++walk) {
+        const int g = w.g, head = w.h, t0 = w.t, n_tiles = w.here(), whole = w.whole, count = w.count;
+        w.step(n_tiles);                                      // (the next segment)
+        int n_rows;
+        const int row0 = shared_group(p, g, n_rows), t = tid / p.G;
+        const bool ok = t < n_rows;
+        const long long slot = (blockIdx.x + static_cast<long long>(g) * p.heads + head) * p.mpad;
+        SharedRows<D> rows{p, smem, sh, p.entries + static_cast<long long>(g) * p.cap, meta, base, count, whole, t0, n_tiles, row0, n_rows, head, p.G,
+                           ok ? p.len[row0 + t] : 0, ok ? t : 0, ok, p.scale_log2, p.stat + slot + tid, p.acc + slot * D, w.left > 0 ? w.g : -1, w.h, careful, false, ~0ull};
+        if (walk == 0) ptc_load_q<D>(smem, sh, rows);
+        if (warp * 32 < n_rows * p.G) ptc_softmax<D>(smem, sh, rows, bw, base, walk);
+        else ptc_idle(sh, rows, bw, base, walk);
+        bad |= rows.bad && rows.len > 0 && t0 + n_tiles > whole;
+        base += n_tiles;
+      }
+      fence_proxy_async();                                    // (results passed through where keys may come again)
     } else if (warp == 4) {
-      ptc_issue<D>(smem, sh, n_tiles, bw);
+      for (int base = 0, walk = 0; w.left > 0 && !bw.dead; ++walk) {
+        const int n_tiles = w.here();
+        ptc_issue<D>(smem, sh, n_tiles, bw, base, walk);
+        base += n_tiles;
+        w.step(n_tiles);
+      }
     } else {
       const bool values = warp == 6;
       uint64_t *full = values ? sh->v_full : sh->k_full, *empty = values ? sh->v_empty : sh->k_empty;
       const uint32_t ring = smem_u32(smem + (values ? L::V : L::K));
-      auto find = [&](int j) { return lane < p.tile_pieces && j < n_tiles ? rows.piece((seg.z + j) * p.tile_pieces + lane) : make_int4(0, 0, 0, 0); };
-      int4 next = find(0);
+      auto find = [&]() {                                     // a lane a piece of the tile
+        const int i = w.t * p.tile_pieces + lane;
+        return lane < p.tile_pieces && w.left > 0 && i < w.count ? p.entries[static_cast<long long>(w.g) * p.cap + i] : make_int4(0, 0, 0, 0);
+      };
+      int4 next = find();
       uint32_t turn = 0;                                      // bit s: parity of stage s's next tile that is changed
-      for (int j = 0; j < n_tiles; ++j) {
+      bool pending = false;                                   // the tile in front, if its values are still to be changed
+      for (int j = 0; j <= part.w; ++j) {
         const int s = j & 1;
         const int4 e = next;
-        next = find(j + 1);
-        bw.wait(&empty[s], ((j >> 1) & 1) ^ 1);
-        if (!__all_sync(0xffffffffu, !bw.dead)) {
-          bw.dead = true;
-          break;
+        bool change = false;
+        if (j < part.w) {
+          const int head = w.h;
+          const bool masked = w.t >= w.whole;
+          w.step(1);
+          next = find();
+          bw.wait(&empty[s], ((j >> 1) & 1) ^ 1);
+          if (!__all_sync(0xffffffffu, !bw.dead)) {
+            bw.dead = true;
+            break;
+          }
+          // (tile j + 4's stands where tile j's was: its stage was empty, so tile j + 2's scores have been multiplied, and tile j's output with them)
+          if (!values && masked && lane < p.tile_pieces) meta[(j & 3) * 4 + lane] = e;
+          change = values && masked && careful;
+          shared_fetch<D>(p, &map, e, values ? 1 : 0, head, ring + s * L::TILE, change ? &sh->v_part[s] : &full[s]);
         }
-        const bool masked = seg.z + j >= rows.whole;
-        // (tile j + 4's stands where tile j's was: its stage was empty, so tile j + 2's scores have been multiplied, and tile j's output with them)
-        if (!values && masked && lane < p.tile_pieces) meta[(j & 3) * 4 + lane] = e;
-        const uint32_t short_ = __ballot_sync(0xffffffffu, lane < p.tile_pieces && e.w < p.piece);
-        const bool change = values && masked && (short_ || rows.careful);
-        shared_fetch<D>(p, &map, e, values ? 1 : 0, head, ring + s * L::TILE, change ? &sh->v_part[s] : &full[s]);
-        if (!change) continue;
-        bw.wait(&sh->v_part[s], turn >> s & 1u);
-        if (!__all_sync(0xffffffffu, !bw.dead)) {
-          bw.dead = true;
-          break;
-        }
-        turn ^= 1u << s;
-        uint4* v_tile = reinterpret_cast<uint4*>(smem + L::V + s * L::TILE);
-        for (uint32_t left = short_; left; left &= left - 1) {      // rows that are no tokens become zeros
-          const int i = __ffs(left) - 1, tokens = __shfl_sync(0xffffffffu, e.w, i), from = (i * p.piece + tokens) * 8, n = (p.piece - tokens) * 8;
-#pragma unroll
-          for (int kb = 0; kb < D / 64; ++kb)
-            for (int k = lane; k < n; k += 32) v_tile[kb * PTC_KT * 8 + from + k] = make_uint4(0u, 0u, 0u, 0u);
-        }
-        if (rows.careful) {
-          __syncwarp();
+        if (pending) {                                        // (behind the next tile's copies, which are on their way meanwhile)
+          const int o = s ^ 1;
+          bw.wait(&sh->v_part[o], turn >> o & 1u);
+          if (!__all_sync(0xffffffffu, !bw.dead)) {
+            bw.dead = true;
+            break;
+          }
+          turn ^= 1u << o;
+          uint4* v_tile = reinterpret_cast<uint4*>(smem + L::V + o * L::TILE);
           for (int i = lane; i < (D / 64) * PTC_KT * 8; i += 32) {
             uint4 v = v_tile[i];
-            uint32_t* w = &v.x;
+            uint32_t* x = &v.x;
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-              if ((w[k] & 0x7f80u) == 0x7f80u) w[k] &= 0xffff0000u;
-              if ((w[k] & 0x7f800000u) == 0x7f800000u) w[k] &= 0xffffu;
+              if ((x[k] & 0x7f80u) == 0x7f80u) x[k] &= 0xffff0000u;
+              if ((x[k] & 0x7f800000u) == 0x7f800000u) x[k] &= 0xffffu;
             }
             v_tile[i] = v;
           }
+          fence_proxy_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&full[o]);
         }
-        fence_proxy_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&full[s]);
+        pending = change;
       }
       ptc_let_land(bw.dead);
       __syncwarp();
     }
     tc_fence_before();
-    const bool again = __syncthreads_or(rows.bad && rows.len > 0 && seg.z + n_tiles > rows.whole && !bw.dead);
+    const bool again = __syncthreads_or(bad && !bw.dead);
     tc_fence_after();
     if (!again || pass) break;
     sh = sh2;
   }
-  if (warp < 4 && !bw.dead) {                                 // whole rows, 16 bytes a lane
-    float4* acc = reinterpret_cast<float4*>(p.acc + static_cast<long long>(blockIdx.x) * p.mpad * D);
-    const int n = n_rows * p.G * (D / 4);
-    for (int i = tid; i < n; i += 128) acc[i] = *rows.staged(i / (D / 4), i % (D / 4));
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, 256);
   }
-  if (warp == 4) tmem_dealloc(tmem_base, 256);
 }
 
 // The segments of a group and head meet: WPR warps a row, each every WPR-th segment, a lane D / 32 neighbouring dimensions.
@@ -465,7 +586,8 @@ __global__ void __launch_bounds__(32 * SJ_WARPS) shared_join_kernel(const __grid
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   if (on && p.len[row] > 0) {
-    const int s0 = p.seg0[unit], s1 = p.seg0[unit + 1];
+    const int2 blocks = p.blocks_of[unit];
+    const int s0 = blocks.x + unit, s1 = blocks.y + unit + 1;
     float top = -INFINITY;
     for (int s = s0 + lane; s < s1; s += 32) top = fmaxf(top, p.stat[static_cast<long long>(s) * p.mpad + m].x);
     top = warp_max(top);
@@ -507,8 +629,8 @@ __global__ void __launch_bounds__(32 * SJ_WARPS) shared_join_kernel(const __grid
 template <int D>
 static int launch_shared(const CUtensorMap& map, const SharedAttnParams& p, int grid, void* stream) {
   const int units = p.groups * p.heads, m = p.sub * p.G;
-  VB_CHECK_CUDA(rm_smem<shared_attn_kernel<D>>(PtcLayout<D>::TOTAL + 512));
-  VB_LAUNCH_PDL(shared_attn_kernel<D>, grid + units, PTC_THREADS, PtcLayout<D>::TOTAL + 512, stream, map, p);
+  VB_CHECK_CUDA(rm_smem<shared_attn_kernel<D>>(SA_SMEM<D>));
+  VB_LAUNCH_PDL(shared_attn_kernel<D>, grid, PTC_THREADS, SA_SMEM<D>, stream, map, p);
   if (grid > 8 * units) VB_LAUNCH_PDL((shared_join_kernel<D, SJ_WARPS>), dim3(units, m), 32 * SJ_WARPS, 0, stream, p);
   else VB_LAUNCH_PDL((shared_join_kernel<D, 1>), dim3(units, (m + SJ_WARPS - 1) / SJ_WARPS), 32 * SJ_WARPS, 0, stream, p);
   return 0;
@@ -537,7 +659,7 @@ static int check_shared(const char* who, const VbSharedPlan* s) {
 
 struct SharedLayout {
   int sub, subs, groups, cap, mpad;
-  size_t segments, acc, stat, ints, bytes;      // entries first
+  size_t parts, acc, stat, blocks_of, ints, bytes;      // entries first
 };
 static SharedLayout shared_layout(const VbSharedPlan* s) {
   SharedLayout l;
@@ -548,11 +670,12 @@ static SharedLayout shared_layout(const VbSharedPlan* s) {
   l.cap = l.sub * s->columns * (s->page_size / sa_piece(s->page_size));
   l.mpad = (l.sub * G + 15) / 16 * 16;
   const size_t units = static_cast<size_t>(l.groups) * s->n_kv, segments = s->grid + units;
-  l.segments = 16ull * l.groups * l.cap;
-  l.acc = l.segments + 16ull * segments;
+  l.parts = 16ull * l.groups * l.cap;
+  l.acc = l.parts + 32ull * s->grid;
   l.stat = l.acc + 4ull * segments * l.mpad * s->head_dim;
-  l.ints = l.stat + 8ull * segments * l.mpad;
-  l.bytes = l.ints + 4ull * (2ull * l.groups + units + 1 + s->rows);
+  l.blocks_of = l.stat + 8ull * segments * l.mpad;
+  l.ints = l.blocks_of + 8ull * units;
+  l.bytes = l.ints + 4ull * (3ull * l.groups + 1 + s->rows);
   return l;
 }
 
@@ -574,9 +697,10 @@ extern "C" int vb_shared_plan(const VbSharedPlan* plan, const int32_t* d_table, 
   uint8_t* at = static_cast<uint8_t*>(plan->d_buffer);
   SharedPlanParams p = {};
   p.entries = reinterpret_cast<int4*>(at);
-  p.segments = reinterpret_cast<int4*>(at + l.segments);
+  p.parts = reinterpret_cast<int4*>(at + l.parts);
   p.counts = reinterpret_cast<int32_t*>(at + l.ints);
-  p.whole = p.counts + l.groups, p.seg0 = p.whole + l.groups, p.len = p.seg0 + l.groups * plan->n_kv + 1;
+  p.whole = p.counts + l.groups, p.tile0 = p.whole + l.groups, p.len = p.tile0 + l.groups + 1;
+  p.blocks_of = reinterpret_cast<int2*>(at + l.blocks_of);
   p.table = d_table, p.tokens = d_tokens;
   p.rows = plan->rows, p.width = plan->width, p.sub = l.sub, p.subs = l.subs, p.groups = l.groups, p.cap = l.cap;
   p.columns = plan->columns, p.pages = pages, p.page_size = plan->page_size, p.piece = sa_piece(plan->page_size);
@@ -611,9 +735,10 @@ extern "C" int vb_shared_attn(void* d_out, const void* d_q, const void* d_kv, in
   uint8_t* at = static_cast<uint8_t*>(plan->d_buffer);
   SharedAttnParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(d_q), p.out = static_cast<__nv_bfloat16*>(d_out), p.kv = static_cast<const __nv_bfloat16*>(d_kv);
-  p.entries = reinterpret_cast<const int4*>(at), p.segments = reinterpret_cast<const int4*>(at + l.segments);
+  p.entries = reinterpret_cast<const int4*>(at), p.parts = reinterpret_cast<const int4*>(at + l.parts);
   p.counts = reinterpret_cast<const int32_t*>(at + l.ints);
-  p.whole = p.counts + l.groups, p.seg0 = p.whole + l.groups, p.len = p.seg0 + l.groups * H + 1;
+  p.whole = p.counts + l.groups, p.len = p.whole + 2 * l.groups + 1;
+  p.blocks_of = reinterpret_cast<const int2*>(at + l.blocks_of);
   p.acc = reinterpret_cast<float*>(at + l.acc), p.stat = reinterpret_cast<float2*>(at + l.stat);
   p.slab_base = slab_base;
   VB_CHECK_ARG(p.wait_flag = wait_flag(WK_PREFILL_ATTN), "vb_shared_attn: no mapped host memory");

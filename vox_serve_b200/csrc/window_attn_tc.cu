@@ -39,7 +39,7 @@ __device__ __forceinline__ void wtc_tma_4d(uint32_t dst, const CUtensorMap* m, u
 }
 
 struct WindowRows {
-  static constexpr bool HOLE = true, STAGED = false;
+  static constexpr bool HOLE = true, STAGED = false, CHAINED = false;
   const WindowTcParams& p;
   int n_tiles, n0, t1;           // tiles 0 .. n0 - 1 hold kept tokens, the rest start at t1
   int hole0, hole1;              // between the kept tokens and the first key that the block's first row sees
