@@ -2269,8 +2269,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, weight: Opti
             and (end_token is None or 0 <= end_token < z[1])):
         _beam_select_check(logits, scores, n, weight, ended, end_token)
     (B, W), (R, V), f32, on = s, z, dtype is F32, logits.device
-    step = BeamStep(torch.empty((B, n), dtype=F32, device=on), torch.empty((B, n), dtype=torch.int32, device=on), torch.empty((B, n), dtype=torch.int64, device=on),
-                    None if end_token is None else torch.empty((B, n), dtype=torch.bool, device=on))
+    step = BeamStep(torch.empty(B, n, dtype=F32, device=on), torch.empty(B, n, dtype=torch.int32, device=on), torch.empty(B, n, dtype=torch.int64, device=on),
+                    None if end_token is None else torch.empty(B, n, dtype=torch.bool, device=on))
     # (of the allocator's, so that calls on other streams and captured graphs have their own)
     n_ws = _beam_ws(B, W, V, n, f32)
     ws = torch.empty(n_ws // 8, dtype=torch.int64, device=on)
@@ -2305,7 +2305,7 @@ def beam_reorder(states: Sequence[torch.Tensor], parent: torch.Tensor, slots: Op
     ptrs, sizes, rows = [0] * k, [0] * k, states[0].shape[0] if k and states[0].dim() else 0
     for i, t in enumerate(states):
         n = t.nbytes
-        ok = ok and n > 0 and t.shape[0] == rows and t.get_device() == dev and t.is_contiguous()
+        ok = ok and n > 0 and t.dim() > 0 and t.shape[0] == rows and t.get_device() == dev and t.is_contiguous()
         ptrs[i], sizes[i] = t.data_ptr(), n // rows if rows else 0
     if not ok or len(set(ptrs)) != k or (k and (max(sizes) >= 1 << 32 or (slots is None and by[0] * by[1] > rows))):
         _beam_reorder_check(states, parent, slots)
@@ -2478,15 +2478,18 @@ def shared_attn(q: torch.Tensor, kv_cache: torch.Tensor, slab_base: int, plan: S
     [layers, pages, 2, page, Hkv, D] (slab_base = layer * pages) or one layer [pages, 2, page, Hkv, D] bf16, as for ``paged_attn``, whose results it has up to rounding;
     ``plan``: ``shared_plan`` of this step's tables.  out: bf16 like q, or a TiledAct.  What is not finite in a page reaches the rows that hold it and no others."""
     R, Hq, D = plan.rows, plan.n_q, plan.head_dim
-    if not (q.is_cuda and q.get_device() == plan._device == kv_cache.get_device() == _device_index()):
+    dev, s = _device_index(), kv_cache.shape
+    per, slabs = (s[-5], s[0] * (s[1] if len(s) == 6 else 1)) if len(s) in (5, 6) else (1, 0)
+    # (one comparison per fact when all of them hold)
+    if not (q.get_device() == plan._device == kv_cache.get_device() == dev and q.dtype is BF16 and q.shape == (R, Hq, D) and q.is_contiguous() and kv_cache.dtype is BF16
+            and slabs > 0 and s[-4:] == (2, plan.page_size, plan.n_kv, D) and kv_cache.is_contiguous() and plan.pages <= per and 0 <= slab_base <= slabs - per
+            and slab_base % per == 0):
         _need_here("shared_attn", q, kv_cache, plan.buf)
-    _refuse(q.dtype is not BF16 or tuple(q.shape) != (R, Hq, D) or not q.is_contiguous(), f"shared_attn: bf16 queries [{R}, {Hq}, {D}] are needed")
-    s = kv_cache.shape
-    _refuse(kv_cache.dtype is not BF16 or not kv_cache.is_contiguous() or len(s) not in (5, 6) or tuple(s[-4:]) != (2, plan.page_size, plan.n_kv, D),
-            f"shared_attn: a bf16 cache [.., pages, 2, {plan.page_size}, {plan.n_kv}, {D}] is needed, not {tuple(s)}")
-    per, slabs = s[-5], s[0] * (s[1] if len(s) == 6 else 1)
-    _refuse(plan.pages > per, f"shared_attn: the plan is of {plan.pages} pages, the cache has {per} a layer")
-    _refuse(not 0 <= slab_base <= slabs - per or slab_base % per != 0, f"shared_attn: layer at page {slab_base} of {slabs}")
+        _refuse(q.dtype is not BF16 or tuple(q.shape) != (R, Hq, D) or not q.is_contiguous(), f"shared_attn: bf16 queries [{R}, {Hq}, {D}] are needed")
+        _refuse(kv_cache.dtype is not BF16 or not kv_cache.is_contiguous() or slabs < 1 or tuple(s[-4:]) != (2, plan.page_size, plan.n_kv, D),
+                f"shared_attn: a bf16 cache [.., pages, 2, {plan.page_size}, {plan.n_kv}, {D}] is needed, not {tuple(s)}")
+        _refuse(plan.pages > per, f"shared_attn: the plan is of {plan.pages} pages, the cache has {per} a layer")
+        _refuse(not 0 <= slab_base <= slabs - per or slab_base % per != 0, f"shared_attn: layer at page {slab_base} of {slabs}")
     xt = 0
     if isinstance(out, TiledAct):
         _need_here("shared_attn", out.data)
@@ -2499,5 +2502,5 @@ def shared_attn(q: torch.Tensor, kv_cache: torch.Tensor, slab_base: int, plan: S
         _need_here("shared_attn", out)
         _refuse(out.dtype is not BF16 or out.shape != q.shape or not out.is_contiguous(), f"shared_attn: out is bf16 [{R}, {Hq}, {D}]")
     call("vb_shared_attn", to.data_ptr(), q.data_ptr(), kv_cache.data_ptr(), slabs, int(slab_base), plan._ptr, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), xt,
-         _stream())
+         _raw_stream(dev))
     return out
