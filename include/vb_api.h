@@ -971,7 +971,7 @@ typedef struct {
   int64_t slot_bytes;
   int32_t layers, parts, slots, pad;
 } VbPageCache;
-size_t vb_page_pool_scratch_bytes(int pages, int rows);
+size_t vb_page_pool_scratch_bytes(int pages);
 int vb_fork_pages(const VbPagePool* pool, const VbPagePool* out, const int32_t* d_src, int group, const int32_t* d_grow, int grow, const VbPageCache* caches,
                   int n_caches, void* stream);
 int vb_compact_pages(const VbPagePool* pool, const VbPagePool* out, const VbPageCache* caches, int n_caches, void* stream);

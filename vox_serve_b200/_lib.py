@@ -228,7 +228,7 @@ SIGNATURES = {
     "vb_beam_select_workspace_bytes": (c_size_t, [c_int, c_int, c_int, c_int, c_int]),
     "vb_beam_select": (c_int, [P, P, P, P, P, c_int64, c_int, P, P, P, c_int, c_int, c_int, c_int, c_int64, P, c_size_t, P]),
     "vb_beam_reorder": (c_int, [P, P, c_int, c_int, P, P, c_int, c_int, P]),
-    "vb_page_pool_scratch_bytes": (c_size_t, [c_int, c_int]),
+    "vb_page_pool_scratch_bytes": (c_size_t, [c_int]),
     "vb_fork_pages": (c_int, [P, P, P, c_int, P, c_int, P, c_int, P]),
     "vb_compact_pages": (c_int, [P, P, P, c_int, P]),
     "vb_shared_plan_bytes": (c_size_t, [P]),

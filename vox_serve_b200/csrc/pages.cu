@@ -13,46 +13,37 @@
 
 namespace vb {
 
-constexpr int PG_THREADS = 1024, PG_MAX_CLUSTER = 8, PG_MAX_ROWS = 4096, PG_STAGE = 8192;
+constexpr int PG_THREADS = 1024, PG_MAX_CLUSTER = 8, PG_MAX_ROWS = 4096, PG_STAGE = 8192, PG_SMEM_PAGES = 8192;
 
 // words of a pool's status
 enum { PS_MISSING = 0, PS_LONG = 1, PS_COPIES = 2, PS_USED = 3 };
 
 __device__ __forceinline__ int ldcg(const int32_t* p) { return __ldcg(p); }
 
-// exclusive prefix over the block of one number a thread; total in all threads.  `sums`: 33 words
-__device__ __forceinline__ int block_prefix(int mine, int* sums, int& total) {
+// exclusive prefix over the block of two numbers a thread; totals in all threads.  `sums`: 33 words
+__device__ __forceinline__ int2 block_prefix(int2 mine, int2* sums, int2& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  int inc = mine;
+  int2 inc = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
-    const int v = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += v;
+    const int x = __shfl_up_sync(0xffffffffu, inc.x, o), y = __shfl_up_sync(0xffffffffu, inc.y, o);
+    if (lane >= o) inc.x += x, inc.y += y;
   }
   __syncthreads();                                   // (the last call's sums have been read)
   if (lane == 31) sums[warp] = inc;
   __syncthreads();
-  if (warp == 0) {
-    int s = sums[lane], t = s;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, t, o);
-      if (lane >= o) t += v;
-    }
-    sums[lane] = t - s;
-    if (lane == 31) sums[32] = t;
-  }
-  __syncthreads();
-  total = sums[32];
-  return sums[warp] + inc - mine;
+  const int2 s = sums[lane];
+  const int2 before = make_int2(__reduce_add_sync(0xffffffffu, lane < warp ? s.x : 0), __reduce_add_sync(0xffffffffu, lane < warp ? s.y : 0));
+  total = make_int2(__reduce_add_sync(0xffffffffu, s.x), __reduce_add_sync(0xffffffffu, s.y));
+  return make_int2(before.x + inc.x - mine.x, before.y + inc.y - mine.y);
 }
 
 struct ForkParams {
   const int32_t *table, *tokens, *refs;              // the pool as it is
   int32_t *out_table, *out_tokens, *out_refs;        // as it becomes (may be the same)
-  int32_t *status, *copies, *work, *first, *base;    // scratch of the pool that is written: copies [rows][3], work / first [pages], base [rows]
+  int32_t *status, *copies, *work, *free;            // of the pool that is written: copies [rows][3]; scratch work / free [pages], where these are not in shared memory
   const int32_t *src, *grow;                         // row that every row continues (null: itself; < 0: none), tokens it gets room for (null: grow_all)
-  int rows, columns, pages, page_size, group, grow_all;
+  int rows, columns, pages, page_size, group, grow_all, in_smem;
 };
 
 // the row that row i continues; -1: none
@@ -76,146 +67,169 @@ __device__ __forceinline__ int fork_page(const ForkParams& p, int row, int col) 
   return g >= 0 && g < p.pages ? g : -1;
 }
 
+// the same place in block 0's shared memory, as an ordinary address
+template <typename T>
+__device__ __forceinline__ T* in_block0(T* p) {
+  T* r;
+  asm("mapa.u64 %0, %1, 0;" : "=l"(r) : "l"(p));
+  return r;
+}
+
+// What is known of a row stands in every block's shared memory.  A row that k rows continue adds k - 1 to the count of each of its pages, once a page and not
+// once a row that takes it over.  Counts and free pages stand in block 0's shared memory for pools of up to PG_SMEM_PAGES pages (measured, against scratch in
+// global memory: XXX), and are volatile to every block.
 __global__ void __launch_bounds__(PG_THREADS, 1) fork_pages_kernel(const __grid_constant__ ForkParams p) {
   extern __shared__ int32_t pg_smem[];
-  int32_t* s_src = pg_smem;                          // [rows]
-  int32_t* s_tok = s_src + p.rows;                   // [rows] tokens of the row it continues
-  int32_t* stage = s_tok + p.rows;                   // PG_STAGE: new values of a block of columns
-  __shared__ int sums[33];
-  __shared__ int s_ok;
-  const int tid = threadIdx.x, rank = cluster_ctarank(), blocks = cluster_nctarank();
+  int32_t* s_src = pg_smem;                          // [rows] the row that a row continues, -1: none
+  int32_t* s_grow = s_src + p.rows;                  // [rows] tokens it gets room for
+  int32_t* s_tok = s_grow + p.rows;                  // [rows] tokens before the step
+  int32_t* s_held = s_tok + p.rows;                  // [rows] ... and pages
+  int32_t* s_heirs = s_held + p.rows;                // [rows] rows that continue it
+  int32_t* s_keeper = s_heirs + p.rows;              // [rows] ... the first of them
+  int32_t* s_tail = s_keeper + p.rows;               // [rows] page that the row copies, -1: none
+  int32_t* s_base = s_tail + p.rows;                 // [rows] its first of the free pages, times two; 1: that one is for a copy
+  int32_t* stage = s_base + p.rows;                  // PG_STAGE: new values of a block of columns
+  __shared__ int2 sums[32];
+  __shared__ int s_ok, s_copies;
+  const int tid = threadIdx.x, rank = cluster_ctarank(), blocks = cluster_nctarank(), P = p.page_size;
+  const int all = blocks * PG_THREADS, mine = rank * PG_THREADS + tid;
+  volatile int32_t* work = p.in_smem ? in_block0(stage + PG_STAGE) : p.work;                // [pages] holders
+  volatile int32_t* free = p.in_smem ? in_block0(stage + PG_STAGE + p.pages) : p.free;      // [pages needed] the lowest free ones
+  volatile int32_t* base = in_block0(s_base);
   pdl_sync();
+  const int ref = mine < p.pages ? p.refs[mine] : 0;      // (all loads of the start at once)
   for (int i = tid; i < p.rows; i += PG_THREADS) {
-    const int s = fork_source(p, i);
-    s_src[i] = s;
-    s_tok[i] = s < 0 ? 0 : fork_tokens(p, s);
+    const int s = fork_source(p, i), n = fork_tokens(p, i), g = p.grow ? p.grow[i] : p.grow_all;
+    s_src[i] = s, s_grow[i] = g > 0 ? g : 0, s_tok[i] = n, s_held[i] = (n + P - 1) / P, s_heirs[i] = 0, s_keeper[i] = 0x7fffffff, s_tail[i] = -1;
   }
-  for (int g = rank * PG_THREADS + tid; g < p.pages; g += blocks * PG_THREADS) p.work[g] = p.refs[g], p.first[g] = 0x7fffffff;
+  if (tid == 0) s_copies = 0;
+  if (blocks > 1) cluster_sync_all();                // (block 0 runs: its shared memory may be written)
+  if (mine < p.pages) work[mine] = ref;
+  for (int g = mine + all; g < p.pages; g += all) work[g] = p.refs[g];
   __syncthreads();
+  for (int i = tid; i < p.rows; i += PG_THREADS)
+    if (s_src[i] >= 0) atomicAdd(s_heirs + s_src[i], 1), atomicMin(s_keeper + s_src[i], i);
   cluster_sync_all();
 
-  // holders of every page after the step, from those before it: rows that go on where they are change nothing
-  const int P = p.page_size;
-  const long long cells = static_cast<long long>(p.rows) * p.columns;
-  for (long long e = static_cast<long long>(rank) * PG_THREADS + tid; e < cells; e += static_cast<long long>(blocks) * PG_THREADS) {
-    const int i = static_cast<int>(e / p.columns), c = static_cast<int>(e - static_cast<long long>(i) * p.columns), s = s_src[i];
-    if (s == i) continue;
-    if (c < (fork_tokens(p, i) + P - 1) / P) {
-      const int g = fork_page(p, i, c);
-      if (g >= 0) atomicSub(p.work + g, 1);
-    }
-    if (s >= 0 && c < (s_tok[i] + P - 1) / P) {
+  // holders of every page after the step, from those before it
+  const int log_x = min(10, 32 - __clz(p.columns - 1)), x = 1 << log_x;      // (x neighbouring threads of the cluster a row)
+  for (int s = mine >> log_x; s < p.rows; s += all >> log_x) {
+    const int more = s_heirs[s] - 1, held = more ? s_held[s] : 0;
+#pragma unroll 4
+    for (int c = mine & (x - 1); c < held; c += x) {
       const int g = fork_page(p, s, c);
-      if (g >= 0) atomicAdd(p.work + g, 1);
+      if (g >= 0) atomicAdd(const_cast<int32_t*>(work) + g, more);
     }
   }
-  // the first row that holds a page which is not full
-  for (int i = rank * PG_THREADS + tid; i < p.rows; i += blocks * PG_THREADS) {
-    if (s_src[i] < 0 || s_tok[i] % P == 0) continue;
-    const int g = fork_page(p, s_src[i], s_tok[i] / P);
-    if (g >= 0) atomicMin(p.first + g, i);
-  }
+  if (rank == 0)
+    for (int i = tid; i < p.rows; i += PG_THREADS) {
+      const int s = s_src[i], n = s < 0 ? 0 : s_tok[s];
+      if (n % P && s_keeper[s] != i) s_tail[i] = fork_page(p, s, n / P);
+    }
   cluster_sync_all();
 
+  // (tokens after the step fit 32 bits: at most 2^30 and what a row may grow by)
+  auto pages_after = [&](int s, int i) { return (static_cast<uint32_t>(s_tok[s]) + static_cast<uint32_t>(s_grow[i]) + P - 1u) / static_cast<uint32_t>(P); };
   if (rank == 0) {
     // pages that every row needs: one for a copy, the others for tokens
-    int need_all = 0, copies = 0, too_long = 0;
+    int need_all = 0, too_long = 0;
     for (int i0 = 0; i0 < p.rows; i0 += PG_THREADS) {
-      const int i = i0 + tid;
-      int need = 0, copy = 0, longer = 0, tail = -1, part = 0;
-      if (i < p.rows && s_src[i] >= 0) {
-        const int n = s_tok[i], g = p.grow ? ldcg(p.grow + i) : p.grow_all;
-        const long long m = static_cast<long long>(n) + (g > 0 ? g : 0);
-        part = n % P;
-        if (part) tail = fork_page(p, s_src[i], n / P);
-        copy = tail >= 0 && ldcg(p.first + tail) != i;
-        const long long want = (m + P - 1) / P;
-        longer = want > p.columns;
-        need = longer ? 0 : copy + static_cast<int>(want) - (n + P - 1) / P;
+      const int i = i0 + tid, s = i < p.rows ? s_src[i] : -1;
+      int need = 0, longer = 0, copy = 0;
+      if (s >= 0) {
+        const uint32_t want = pages_after(s, i);
+        copy = s_tail[i] >= 0;
+        longer = want > static_cast<uint32_t>(p.columns);
+        need = longer ? 0 : copy + static_cast<int>(want) - s_held[s];
       }
-      int total, n_copies;
-      const int before = block_prefix(need, sums, total), place = block_prefix(copy, sums, n_copies);
-      if (i < p.rows) p.base[i] = (need_all + before) * 2 + copy;
-      if (copy) {
-        int32_t* c = p.copies + 3ll * (copies + place);
-        c[0] = tail, c[1] = need_all + before, c[2] = part;      // (c[1]: which of the free pages; its number follows)
-      }
-      too_long += __syncthreads_count(longer);
-      need_all += total;
-      copies += n_copies;
+      int2 total;
+      const int2 before = block_prefix(make_int2(need, longer), sums, total);
+      if (i < p.rows) s_base[i] = (need_all + before.x) * 2 + copy;
+      need_all += total.x;
+      too_long += total.y;
     }
-    // the lowest free pages; `first` has done its work and takes their numbers
+    // the lowest free pages
     int have = 0;
     for (int g0 = 0; g0 < p.pages && have < need_all; g0 += 4 * PG_THREADS) {
-      int free = 0, mine[4];
+      int n[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         const int g = g0 + 4 * tid + j;
-        mine[j] = g < p.pages && ldcg(p.work + g) == 0;
-        free += mine[j];
+        n[j] = g < p.pages ? work[g] : 1;
       }
-      int total, at = have + block_prefix(free, sums, total);
+      int2 total;
+      int at = have + block_prefix(make_int2((n[0] == 0) + (n[1] == 0) + (n[2] == 0) + (n[3] == 0), 0), sums, total).x;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
-        if (mine[j]) {
-          if (at < need_all) p.first[at] = g0 + 4 * tid + j;
+        if (n[j] == 0) {
+          if (at < need_all) free[at] = g0 + 4 * tid + j;
           ++at;
         }
-      have += total;
+      have += total.x;
     }
     const bool ok = have >= need_all && too_long == 0;
     __syncthreads();
     if (ok) {
-      for (int k = tid; k < need_all; k += PG_THREADS) p.work[p.first[k]] = 1;
-      for (int k = tid; k < copies; k += PG_THREADS) {
-        int32_t* c = p.copies + 3ll * k;
-        c[1] = p.first[c[1]];
-        atomicSub(p.work + c[0], 1);
-      }
+      for (int k = tid; k < need_all; k += PG_THREADS) work[free[k]] = 1;
+      for (int i = tid; i < p.rows; i += PG_THREADS)
+        if (s_tail[i] >= 0) {
+          int32_t* c = p.copies + 3ll * atomicAdd(&s_copies, 1);
+          c[0] = s_tail[i], c[1] = free[s_base[i] >> 1], c[2] = s_tok[s_src[i]] % P;
+          atomicSub(const_cast<int32_t*>(work) + s_tail[i], 1);
+        }
+      __syncthreads();
     }
     if (tid == 0) {
+      s_ok = ok;
       p.status[PS_MISSING] = have >= need_all ? 0 : need_all - have;
       p.status[PS_LONG] = too_long;
-      p.status[PS_COPIES] = ok ? copies : 0;
+      p.status[PS_COPIES] = ok ? s_copies : 0;
     }
   }
   cluster_sync_all();
 
-  if (tid == 0) s_ok = ldcg(p.status + PS_MISSING) == 0 && ldcg(p.status + PS_LONG) == 0;
+  const bool ok = *static_cast<volatile int*>(in_block0(&s_ok)) != 0;
+  int32_t* s_want = s_keeper;                        // [rows] pages after the step
+  for (int i = tid; i < p.rows; i += PG_THREADS) {
+    if (rank != 0) s_base[i] = base[i];
+    s_want[i] = s_src[i] < 0 ? 0 : static_cast<int>(min(pages_after(s_src[i], i), static_cast<uint32_t>(p.columns)));
+  }
   __syncthreads();
-  const bool ok = s_ok;
-  if (!ok && p.out_table == p.table) return;        // in place: nothing has been written
-  for (int g = rank * PG_THREADS + tid; g < p.pages; g += blocks * PG_THREADS) p.out_refs[g] = ok ? ldcg(p.work + g) : ldcg(p.refs + g);
-  // A block of columns in all rows at a time, read before it is written: rows may take over one another's pages in place
-  const int wide = min(p.columns, max(1, PG_STAGE / p.rows));
-  for (int c0 = rank * wide; c0 < p.columns; c0 += blocks * wide) {
-    const int w = min(wide, p.columns - c0);
-    for (int e = tid; e < p.rows * w; e += PG_THREADS) {
-      const int i = e / w, c = c0 + e - i * w;
-      int v = -1;
-      if (!ok) {
-        v = ldcg(p.table + static_cast<long long>(i) * p.columns + c);
-      } else if (s_src[i] >= 0) {
-        const int n = s_tok[i], b = ldcg(p.base + i), copy = b & 1, at = b >> 1, held = (n + P - 1) / P;
-        const int g = p.grow ? ldcg(p.grow + i) : p.grow_all, want = static_cast<int>((static_cast<long long>(n) + (g > 0 ? g : 0) + P - 1) / P);
-        if (copy && c == n / P) v = ldcg(p.first + at);
-        else if (c < held) v = ldcg(p.table + static_cast<long long>(s_src[i]) * p.columns + c);
-        else if (c < want) v = ldcg(p.first + at + copy + c - held);
+  if (ok || p.out_table != p.table) {               // (in place, not ok: nothing has been written)
+    for (int g = mine; g < p.pages; g += all) p.out_refs[g] = ok ? work[g] : ldcg(p.refs + g);
+    // A block of columns in all rows at a time, read before it is written: rows may take over one another's pages in place.  `across` neighbouring threads a
+    // row, without a division an entry.
+    const int wide = min((p.columns + blocks - 1) / blocks, max(1, PG_STAGE / p.rows));
+    const int log_across = min(10, 32 - __clz(wide - 1)), across = 1 << log_across, tx = tid & (across - 1), ty = tid >> log_across, down = PG_THREADS >> log_across;
+    for (int c0 = rank * wide; c0 < p.columns; c0 += blocks * wide) {
+      const int w = min(wide, p.columns - c0);
+      for (int k = tx; k < w; k += across) {
+        const int c = c0 + k;
+#pragma unroll 4
+        for (int i = ty; i < p.rows; i += down) {
+          const int s = ok ? s_src[i] : i;
+          int v = -1;
+          if (s >= 0) {
+            const int held = ok ? s_held[s] : p.columns, b = ok ? s_base[i] : 0, copy = b & 1;
+            if (c < held - copy) v = ldcg(p.table + static_cast<long long>(s) * p.columns + c);
+            else if (c < (ok ? s_want[i] : 0)) v = free[(b >> 1) + (c < held ? 0 : copy + c - held)];
+          }
+          stage[i * w + k] = v;
+        }
       }
-      stage[e] = v;
+      __syncthreads();
+      for (int k = tx; k < w; k += across)
+#pragma unroll 4
+        for (int i = ty; i < p.rows; i += down) p.out_table[static_cast<long long>(i) * p.columns + c0 + k] = stage[i * w + k];
+      __syncthreads();
     }
-    __syncthreads();
-    for (int e = tid; e < p.rows * w; e += PG_THREADS) {
-      const int i = e / w;
-      p.out_table[static_cast<long long>(i) * p.columns + c0 + e - i * w] = stage[e];
+    // (tokens last: every block has read what it needs of them only at the start)
+    for (int i = mine; i < p.rows; i += all) {
+      const int s = s_src[i];
+      p.out_tokens[i] = !ok ? ldcg(p.tokens + i) : s < 0 ? 0 : s_tok[s] + s_grow[i];
     }
-    __syncthreads();
   }
-  // (tokens last: every block has read what it needs of them only at the start)
-  for (int i = rank * PG_THREADS + tid; i < p.rows; i += blocks * PG_THREADS) {
-    const int g = p.grow ? ldcg(p.grow + i) : p.grow_all;
-    p.out_tokens[i] = !ok ? ldcg(p.tokens + i) : s_src[i] < 0 ? 0 : s_tok[i] + (g > 0 ? g : 0);
-  }
+  if (blocks > 1) cluster_sync_all();                // (block 0's shared memory is read to the end)
 }
 
 struct CompactParams {
@@ -229,7 +243,7 @@ struct CompactParams {
 
 // The pages in use that stand behind as many places as there are pages in use move into the holes in front, in their order.
 __global__ void __launch_bounds__(PG_THREADS, 1) compact_pages_kernel(const __grid_constant__ CompactParams p) {
-  __shared__ int sums[33];
+  __shared__ int2 sums[32];
   const int tid = threadIdx.x, rank = cluster_ctarank(), blocks = cluster_nctarank();
   pdl_sync();
   if (rank == 0) {
@@ -241,9 +255,9 @@ __global__ void __launch_bounds__(PG_THREADS, 1) compact_pages_kernel(const __gr
         const int g = g0 + 4 * tid + j;
         mine += g < p.pages && p.refs[g] > 0;
       }
-      int total;
-      block_prefix(mine, sums, total);
-      used += total;
+      int2 total;
+      block_prefix(make_int2(mine, 0), sums, total);
+      used += total.x;
     }
     int holes = 0, movers = 0;
     for (int g0 = 0; g0 < p.pages; g0 += 4 * PG_THREADS) {
@@ -256,15 +270,16 @@ __global__ void __launch_bounds__(PG_THREADS, 1) compact_pages_kernel(const __gr
         if (what[j] >= 0) ++n[what[j]];
         if (g < p.pages) p.moved[g] = in && g < used ? g : -1;
       }
-      int th, tm;
-      int h = holes + block_prefix(n[0], sums, th), m = movers + block_prefix(n[1], sums, tm);
+      int2 total;
+      const int2 before = block_prefix(make_int2(n[0], n[1]), sums, total);
+      int h = holes + before.x, m = movers + before.y;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (what[j] == 0) p.to[h++] = g0 + 4 * tid + j;
         if (what[j] == 1) p.from[m++] = g0 + 4 * tid + j;
       }
-      holes += th;
-      movers += tm;
+      holes += total.x;
+      movers += total.y;
     }
     __syncthreads();
     for (int k = tid; k < movers; k += PG_THREADS) {      // (as many holes as movers)
@@ -388,9 +403,9 @@ static int check_caches(const char* who, const VbPageCache* caches, int n) {
 
 using namespace vb;
 
-extern "C" size_t vb_page_pool_scratch_bytes(int pages, int rows) {
-  if (pages <= 0 || rows <= 0) return 0;
-  return 4ull * (2ull * pages + rows);
+extern "C" size_t vb_page_pool_scratch_bytes(int pages) {
+  if (pages <= 0) return 0;
+  return 8ull * pages;
 }
 
 extern "C" int vb_fork_pages(const VbPagePool* pool, const VbPagePool* out, const int32_t* d_src, int group, const int32_t* d_grow, int grow, const VbPageCache* caches,
@@ -403,13 +418,13 @@ extern "C" int vb_fork_pages(const VbPagePool* pool, const VbPagePool* out, cons
   p.table = pool->d_table, p.tokens = pool->d_tokens, p.refs = pool->d_refs;
   p.out_table = out->d_table, p.out_tokens = out->d_tokens, p.out_refs = out->d_refs;
   p.status = out->d_status, p.copies = out->d_copies;
-  p.work = out->d_scratch, p.first = p.work + pool->pages, p.base = p.first + pool->pages;
+  p.work = out->d_scratch, p.free = p.work + pool->pages, p.in_smem = pool->pages <= PG_SMEM_PAGES;
   p.src = d_src, p.grow = d_grow, p.grow_all = grow;
   p.rows = pool->rows, p.columns = pool->columns, p.pages = pool->pages, p.page_size = pool->page_size, p.group = group;
   const long long cells = static_cast<long long>(p.rows) * p.columns, share = (cells + 4 * PG_THREADS - 1) / (4 * PG_THREADS);
   const int cluster = share >= PG_MAX_CLUSTER ? PG_MAX_CLUSTER : share > 2 ? 4 : static_cast<int>(share);
-  VB_CHECK_CUDA(rm_smem<fork_pages_kernel>((2 * PG_MAX_ROWS + PG_STAGE) * 4));
-  VB_LAUNCH_PDL_CLUSTER(fork_pages_kernel, cluster, PG_THREADS, (2 * p.rows + PG_STAGE) * 4, stream, cluster, p);
+  VB_CHECK_CUDA(rm_smem<fork_pages_kernel>((8 * PG_MAX_ROWS + PG_STAGE + 2 * PG_SMEM_PAGES) * 4));
+  VB_LAUNCH_PDL_CLUSTER(fork_pages_kernel, cluster, PG_THREADS, (8 * p.rows + PG_STAGE + (p.in_smem ? 2 * p.pages : 0)) * 4, stream, cluster, p);
   return copy_listed(caches, n_caches, pool, out->d_copies, out->d_status, stream);
 }
 

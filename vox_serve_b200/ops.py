@@ -2328,7 +2328,7 @@ class PagePool:
         _refuse(pages < 1 or page_size < 1 or not 1 <= rows <= 4096 or columns < 1 or columns * page_size > 0x3fffffff or (columns + 1) * rows > 0x3fffffff,
                 f"PagePool: {pages} pages of {page_size} tokens, {rows} rows (1 to 4096) of {columns} columns")
         self.pages, self.page_size, self.rows, self.columns = int(pages), int(page_size), int(rows), int(columns)
-        n = [rows * columns, rows, pages, 4, 3 * max(rows, pages), pages, 2 * pages + rows]
+        n = [rows * columns, rows, pages, 4, 3 * max(rows, pages), pages, 2 * pages]
         self._buf = torch.zeros(sum((k + 3) // 4 * 4 for k in n), dtype=torch.int32, device=device)
         parts, at = [], 0
         for k in n:
