@@ -1,0 +1,191 @@
+"""A beam search on a decoder stack, as a program runs it: prompts once, then steps of beam_select, fork_pages, beam_reorder of what else belongs to a row (here its tokens),
+shared_plan and LlamaEngine.forward(shared=), without the host between them.
+
+Tolerances: the engine rounds to bf16 behind every projection, norm, rotation and attention; that of its own tests holds (logits within 2e-2 of the largest)."""
+import pytest
+import torch
+
+from oracle import orpheus as oorph
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, I32 = torch.bfloat16, torch.float32, torch.int32
+PAGE, PAGES, COLS, WIDTH = 16, 96, 8, 4
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=I32, device="cuda")
+
+
+class Search:
+    """two requests of four beams"""
+
+    def __init__(self, mode="unfused", dims=None, end_token=None, weighted=False):
+        from vox_serve_b200 import ops
+        from vox_serve_b200.engine import LlamaDims, LlamaEngine, LlamaWeights
+        self.ops = ops
+        self.d = d = dims or oorph.OrpheusDims.tiny()
+        ld = LlamaDims(d.hidden_size, d.num_hidden_layers, d.num_attention_heads, d.num_key_value_heads, d.head_dim, d.intermediate_size, d.vocab_size, d.rms_norm_eps,
+                       d.rope_theta, d.rope_factor, d.low_freq_factor, d.high_freq_factor, d.old_context_len)
+        self.weights = LlamaWeights.from_state_dict(oorph.synth_weights(d, seed=7), ld)
+        self.kv = torch.zeros(d.num_hidden_layers, PAGES, 2, PAGE, d.num_key_value_heads, d.head_dim, dtype=BF16, device="cuda")
+        self.eng = LlamaEngine(self.weights, self.kv, PAGE, max_rows=128)
+        self.eng.force_unfused = mode == "unfused"
+        self.teacher = LlamaEngine(self.weights, torch.zeros_like(self.kv), PAGE, max_rows=128)
+        g = torch.Generator().manual_seed(3)
+        self.prompts = [torch.randint(10, d.vocab_size, (n,), generator=g).tolist() for n in (37, 21)]
+        self.rows = len(self.prompts) * WIDTH
+        self.pool = ops.PagePool(PAGES, PAGE, self.rows, COLS)
+        self.plan = ops.SharedPlan(self.rows, WIDTH, COLS, PAGE, d.num_attention_heads, d.num_key_value_heads, d.head_dim)
+        self.history = torch.zeros(self.rows, 32, dtype=I32, device="cuda")
+        self.scores = torch.full((2, WIDTH), -float("inf"), device="cuda")
+        self.ended = torch.zeros(2, WIDTH, dtype=torch.bool, device="cuda") if end_token is not None else None
+        self.end_token, self.weighted, self.t = end_token, weighted, 0
+        self.weight = torch.ones(2, WIDTH, device="cuda") if weighted else None
+        self.ids = torch.zeros(self.rows, dtype=I32, device="cuda")
+        self.at = torch.zeros(1, dtype=torch.int64, device="cuda")      # the history's next place
+
+    def prompt_logits(self, eng, tables, tokens, rows):
+        """logits of the last token of every prompt in ``tokens``; its pages: a row of ``tables``"""
+        ops = self.ops
+        qo = [0]
+        for t in tokens:
+            qo.append(qo[-1] + len(t))
+        ops.plan_rows(eng.plan, _i32(qo), _i32([r * tables.shape[1] for r in rows] + [tables.numel()]), tables.view(-1), None, len(tokens), qo[-1], PAGE, eng.chunk,
+                      kv_len=_i32([len(t) for t in tokens]))
+        pos = torch.cat([torch.arange(len(t), dtype=I32) for t in tokens]).cuda()
+        return eng.forward(_i32([x for t in tokens for x in t]), pos, qo[-1], last_rows=_i32([q - 1 for q in qo[1:]])).clone()
+
+    def start(self):
+        self.ops.fork_pages(self.pool, grow=_i32([37, 0, 0, 0, 21, 0, 0, 0]))
+        self.pool.check()
+        logits = self.prompt_logits(self.eng, self.pool.table, self.prompts, [0, WIDTH])
+        self.scores[:, 0] = 0.0
+        self.choose(logits.repeat_interleave(WIDTH, 0))
+
+    def choose(self, logits):
+        ops = self.ops
+        step = ops.beam_select(logits, self.scores, WIDTH, weight=self.weight, ended=self.ended, end_token=self.end_token)
+        ops.beam_reorder([self.history], step.parent)
+        self.history.index_copy_(1, self.at, step.token.to(I32).view(-1, 1))
+        self.at += 1
+        ops.fork_pages(self.pool, step.parent, 1, [self.kv])
+        self.scores.copy_(step.scores)
+        if self.ended is not None:
+            self.ended.copy_(step.ended)
+        self.ids.copy_(step.token.view(-1))
+
+    def forward(self, shared=True):
+        ops = self.ops
+        ops.plan_rows(self.eng.plan, None, self.pool.indptr, self.pool.table.view(-1), None, self.rows, self.rows, PAGE, self.eng.chunk, kv_len=self.pool.tokens)
+        if shared:
+            ops.shared_plan(self.plan, self.pool.table, self.pool.tokens, PAGES)
+        return self.eng.forward(self.ids, self.pool.tokens - 1, self.rows, shared=self.plan if shared else None)
+
+    def step(self):
+        self.choose(self.forward())
+
+    def sequences(self):
+        n = int(self.at)
+        return [self.prompts[r // WIDTH] + self.history[r, :n].tolist() for r in range(self.rows)]
+
+    def taught(self):
+        """logits behind every row's whole sequence, each read as one prompt"""
+        seq = self.sequences()
+        tables = torch.arange(4 * 8, dtype=I32, device="cuda").view(4, 8)
+        return torch.cat([self.prompt_logits(self.teacher, tables[:1], [s], [0]) for s in seq])
+
+
+@pytest.mark.parametrize("mode", ["unfused", "fused"])
+def test_rows_know_their_own_sequences(mode):
+    """every step's logits are those of the row's sequence read from its start, and those of one stream a row on the same tables"""
+    s = Search(mode)
+    s.start()
+    held = []
+    for _ in range(18):
+        want = s.taught()
+        got = s.forward().clone()
+        alone = s.forward(shared=False).clone()
+        tol = 2e-2 * want.float().abs().max()
+        assert bool(((got.float() - want.float()).abs() <= tol).all())
+        assert bool(((got.float() - alone.float()).abs() <= tol).all())
+        s.pool.check()
+        held.append(int((s.pool.refs > 0).sum()))
+        s.choose(got)
+    # shared pages of prompts are held once, pages of beams that died come back
+    refs = s.pool.refs.tolist()
+    counted = [0] * PAGES
+    for row in s.pool.table.tolist():
+        for p in row:
+            if p >= 0:
+                counted[p] += 1
+    assert refs == counted and s.pool.tokens.tolist() == [37 + 19] * 4 + [21 + 19] * 4
+    assert max(held) < sum(-(-n // PAGE) for n in s.pool.tokens.tolist())
+    # scores are in order, and the sum of what the steps gave
+    assert bool((s.scores[:, :-1] >= s.scores[:, 1:]).all())
+    # moved to the front of the cache, the same rows see the same
+    before = s.forward().clone()
+    s.ops.compact_pages(s.pool, [s.kv])
+    assert s.pool.refs[:int(s.pool.status[3])].min() > 0 and not bool(s.pool.refs[int(s.pool.status[3]):].any())
+    assert torch.equal(s.forward(), before)
+
+
+def test_beams_that_end_and_die():
+    """an end token that is likely: beams end and keep their place by their weighted scores; nothing is missing or left over"""
+    s = Search(end_token=11, weighted=True)
+    s.start()
+    total = s.scores.clone()
+    for k in range(12):
+        s.weight.copy_(torch.where(s.ended, s.weight, torch.full_like(s.weight, (k + 2) ** -0.7)))
+        logits = s.forward().clone()
+        logits[:, 11] += 4.0
+        was, old = s.ended.clone(), s.scores.clone()
+        s.choose(logits)
+        s.pool.check()
+        for b in range(2):
+            for w in range(WIDTH):
+                if bool(was[b, w]):                        # an ended beam's score comes back as it was, if it comes back
+                    same = (s.scores[b] == old[b, w]) & s.ended[b]
+                    assert int(same.sum()) <= int((old[b] == old[b, w]).sum())
+        total = s.scores
+    assert bool(s.ended.any()) and bool(torch.isfinite(total).all())
+
+
+def test_a_captured_step():
+    """the whole step as one graph: the same bits as step by step"""
+    runs = []
+    for captured in (False, True):
+        s = Search()
+        s.start()
+        s.step()
+        if captured:
+            state = [s.kv, s.pool._buf, s.history, s.scores, s.ids, s.at]
+            kept = [t.clone() for t in state]
+            g = torch.cuda.CUDAGraph()
+            s.step()
+            torch.cuda.synchronize()
+            with torch.cuda.graph(g):
+                s.step()
+            for t, k in zip(state, kept):
+                t.copy_(k)
+        for _ in range(10):
+            g.replay() if captured else s.step()
+        torch.cuda.synchronize()
+        s.pool.check()
+        runs.append((s.sequences(), s.scores.clone(), s.pool.table.clone(), s.pool.refs.clone(), s.kv.clone()))
+    assert runs[0][0] == runs[1][0]
+    assert all(torch.equal(a, b) for a, b in zip(runs[0][1:], runs[1][1:]))
+
+
+def test_plans_of_other_steps_are_refused():
+    s = Search()
+    s.start()
+    ops, d = s.ops, s.d
+    s.ops.plan_rows(s.eng.plan, None, s.pool.indptr, s.pool.table.view(-1), None, 8, 8, PAGE, s.eng.chunk, kv_len=s.pool.tokens)
+    for other in (ops.SharedPlan(4, 4, COLS, PAGE, d.num_attention_heads, d.num_key_value_heads, d.head_dim), ops.SharedPlan(8, 4, COLS, 32, d.num_attention_heads, d.num_key_value_heads, d.head_dim),
+                  ops.SharedPlan(8, 4, COLS, PAGE, 2 * d.num_attention_heads, d.num_key_value_heads, d.head_dim), ops.SharedPlan(8, 4, COLS, PAGE, d.num_attention_heads, d.num_key_value_heads, 64)):
+        with pytest.raises(ops.VoxB200Error):
+            s.eng.forward(s.ids, s.pool.tokens - 1, 8, shared=other)
+    ops.plan_rows(s.eng.plan, _i32([0, 4, 8]), s.pool.indptr, s.pool.table.view(-1), None, 2, 8, PAGE, s.eng.chunk, kv_len=s.pool.tokens)
+    with pytest.raises(ops.VoxB200Error, match="decode steps"):
+        s.eng.forward(s.ids, s.pool.tokens - 1, 8, shared=s.plan)

@@ -340,7 +340,7 @@ class LlamaEngine:
     def forward(self, input_ids: Optional[torch.Tensor], position_ids: torch.Tensor, n_rows: int,
                 last_rows: Optional[torch.Tensor] = None, n_out: Optional[int] = None,
                 plan: Optional[ops.RowPlan] = None, last_rows_offset: int = 0, head=None, want_hidden: bool = False,
-                adapters: Optional[ops.LoraPlan] = None):
+                adapters: Optional[ops.LoraPlan] = None, shared: Optional[ops.SharedPlan] = None):
         """input_ids / position_ids int32 [n_rows] on the device; self.plan must hold the step's row plan
         (ops.plan_rows).  Returns logits [n_out or n_rows, vocab] bf16 (a view of the static buffer).
         last_rows (int32 [n_out]) selects the rows whose logits are needed (prefill: qo_indptr[1:] - 1).
@@ -350,8 +350,16 @@ class LlamaEngine:
         return the final-normed rows [n_out or n_rows, hidden] bf16, row-major (the backbone state a depth decoder
         starts from, csm.py:290-300).  ``adapters``: the plan of the rows' adapters (ops.lora_plan; ``set_adapters`` first).  Such a
         step runs every row, those without an adapter too, on row-major activations and planes of gate | up: their results are
-        those of a step without adapters up to bf16 rounding, not to the bit."""
+        those of a step without adapters up to bf16 rounding, not to the bit.  ``shared``: a decode step whose requests have several rows that share
+        pages (ops.shared_plan of the tables that ``plan`` was made from, the step's tokens counted): a page is read once for all of them."""
         d, w, R = self.dims, self.w, n_rows
+        if shared is not None:
+            dims = (shared.rows, shared.n_q, shared.n_kv, shared.head_dim, shared.page_size)
+            if dims != (R, d.num_attention_heads, d.num_key_value_heads, d.head_dim, self.page_size):
+                raise VoxB200Error(f"forward: the plan of shared pages is of {dims} rows, heads, key heads, head size and page, the step of "
+                                   f"{(R, d.num_attention_heads, d.num_key_value_heads, d.head_dim, self.page_size)}")
+            if (self.plan if plan is None else plan).qo_indptr is not None:
+                raise VoxB200Error("forward: shared pages are read by decode steps, one row of every table")
         if adapters is not None:                   # (before anything is written)
             if self.adapters is None:
                 raise VoxB200Error("forward: the engine has no adapters (set_adapters)")
@@ -367,12 +375,12 @@ class LlamaEngine:
             ops.embedding(w.embed, input_ids, out=hidden)
         x_final = normed
         if fused:
-            self._layers_fused(position_ids, R, plan)
+            self._layers_fused(position_ids, R, plan, shared)
             if last_rows is None and self.tiled_acts:
                 x_final = self.normed_t.view_rows(R)
             ops.rmsnorm(hidden, w.norm, d.rms_norm_eps, out=x_final)
         else:
-            x_final = self._layers_unfused(position_ids, R, plan, first, adapters)
+            x_final = self._layers_unfused(position_ids, R, plan, first, adapters, shared)
         if last_rows is not None:
             n_out = last_rows.numel() if n_out is None else n_out
             if isinstance(x_final, ops.TiledAct):      # a gather needs rows: those of the stream, then their norm
@@ -399,7 +407,14 @@ class LlamaEngine:
     # removed.  The fused projections stay as parity-tested C-ABI operators.
     force_unfused = os.environ.get("VB_DECODE_MODE", "unfused") == "unfused"
 
-    def _layers_fused(self, position_ids: torch.Tensor, R: int, plan: ops.RowPlan) -> None:
+    def _attend(self, layer: int, q: torch.Tensor, out, plan: ops.RowPlan, R: int, shared: Optional[ops.SharedPlan]) -> None:
+        if shared is not None:
+            ops.shared_attn(q, self.kv_map, layer * self.pages_per_layer, shared, out=out)
+        else:
+            ops.paged_attn(q, self.kv_map, layer * self.pages_per_layer, plan, R, self.dims.num_key_value_heads, self.page_size, self.chunk, self.attn_ws, out=out,
+                           grid_ctas=self.attn_grid)
+
+    def _layers_fused(self, position_ids: torch.Tensor, R: int, plan: ops.RowPlan, shared: Optional[ops.SharedPlan] = None) -> None:
         """hidden is updated in place, the RMSNorm statistics travel as per-tile sums of squares written by the
         residual projections (ssq[parts][R]).  Per layer: norm + QKV + RoPE + append, paged attention, O + residual,
         norm + gate/up + SiLU, down + residual: one launch per fused projection (5 per layer)."""
@@ -421,8 +436,7 @@ class LlamaEngine:
             ops.proj_norm_qkv_rope_append(hidden if (i == 0 or not tiled) else hidden_t, ssq, 1 if i == 0 else tiles_h,
                                           L["ln1"], eps, L["qkv"], self.kv_cache[i], cs, plan, hq, hkv, D,
                                           self.fsplit_qkv, q_out=q)
-            ops.paged_attn(q, self.kv_map, i * self.pages_per_layer, plan, R, hkv, self.page_size, self.chunk,
-                           self.attn_ws, out=attn_x_out, grid_ctas=self.attn_grid)
+            self._attend(i, q, attn_x_out, plan, R, shared)
             ops.proj_residual(attn_x, L["o"], hidden, self.fsplit_o, hidden_out=hidden, ssq_out=ssq,
                               hidden_tiles_out=hidden_t)
             ops.proj_norm_gateup_silu(hidden_t if tiled else hidden, ssq, tiles_h, L["ln2"], eps, L["gu"], self.gu_half,
@@ -431,7 +445,7 @@ class LlamaEngine:
                               hidden_tiles_out=hidden_t)
 
     def _layers_unfused(self, position_ids: torch.Tensor, R: int, plan: ops.RowPlan, input_ids: Optional[torch.Tensor] = None,
-                         adapters: Optional[ops.LoraPlan] = None):
+                         adapters: Optional[ops.LoraPlan] = None, shared: Optional[ops.SharedPlan] = None):
         """8 launches per layer.  Activations travel between kernels in the tiled layout (the attention output only in
         decode-sized steps and only with VB_ATTN_TILED=1); returns what holds the final normed rows (a TiledAct then,
         else self.normed[:R]).  input_ids: the embedding rows are still to be fetched."""
@@ -458,8 +472,7 @@ class LlamaEngine:
             ops.qkv_rope_append(p, self.kv_cache[i], position_ids, self.freq, plan, hq, hkv, D, q_out=q,
                                 interleave=d.rope_interleave, q_norm=L.get("qn"), k_norm=L.get("kn"),
                                 norm_eps=d.rms_norm_eps, qkv_bias=L.get("qkv_b"))
-            ops.paged_attn(q, self.kv_map, i * self.pages_per_layer, plan, R, hkv, self.page_size, self.chunk,
-                           self.attn_ws, out=attn_o, grid_ctas=self.attn_grid)
+            self._attend(i, q, attn_o, plan, R, shared)
             if adapters is None:
                 p = ops.gemm(attn_o if attn_tiled else attn_o.view(R, hq * D), L["o"], mode=1, split_k=s_o,
                              out=self._partials(s_o, R, H))
