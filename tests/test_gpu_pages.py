@@ -187,7 +187,7 @@ def test_short_of_pages_changes_nothing():
     plain.same_as(pool, caches)
 
 
-@pytest.mark.parametrize("rows,columns,P", [(64, 700, 16), (300, 90, 2), (4096, 3, 4), (2, 5000, 1)])
+@pytest.mark.parametrize("rows,columns,P", [(64, 700, 16), (300, 90, 2), (4096, 3, 4), (4096, 2, 7), (4096, 1, 9), (2, 5000, 1), (1, 8000, 3), (33, 33, 64)])
 def test_large_tables(rows, columns, P):
     """tables that several blocks share, pools that are searched in steps"""
     rng = random.Random(rows)
@@ -199,7 +199,7 @@ def test_large_tables(rows, columns, P):
     plain.same_as(pool, caches)
     for _ in range(3):
         src = [rng.randrange(-1, rows) for _ in range(rows)]
-        grow = [rng.randrange(0, P // 2 + 1) for _ in range(rows)]
+        grow = [rng.randrange(0, max(1, columns * P // 10) + 1) for _ in range(rows)]
         assert plain.step(src, grow)
         ops.fork_pages(pool, _i32(src), _i32(grow))
         pool.check()

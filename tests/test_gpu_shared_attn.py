@@ -172,6 +172,21 @@ def test_tables_that_name_no_pages():
     _check(out, q, kv[0], t2, torch.tensor([24, 16], dtype=I32, device="cuda"))
 
 
+def test_pages_behind_the_cache_are_zeros():
+    """a plan that was made for any cache, a table that names a page this one has not: keys and values of zero, also where values are looked over again"""
+    P = 16
+    kv, q = _data(4, P, 2, 2, 2, 64, seed=6)
+    table = torch.tensor([[1, 1 << 20], [1, 2]], dtype=I32, device="cuda")
+    tokens = torch.tensor([30, 20], dtype=I32, device="cuda")
+    plan = ops.SharedPlan(2, 2, 2, P, 2, 2, 64)
+    padded = torch.cat([kv[0], torch.zeros_like(kv[0, :1])])
+    for bad in (0.0, NAN):
+        kv[0, 2, 1, 3] += bad                                # (row 1's)
+        out = ops.shared_attn(q, kv, 0, ops.shared_plan(plan, table, tokens))
+        _check(out[:1], q[:1], padded, torch.tensor([[1, 4]], dtype=I32, device="cuda"), tokens[:1])
+    assert not bool(torch.isfinite(out[1]).any())
+
+
 def test_layers_and_one_layer():
     table, tokens, pages = _tree(2, 3, 90, 9, 16, seed=8)
     kv, q = _data(pages, 16, 6, 6, 3, 64, seed=9, layers=3)

@@ -277,7 +277,7 @@ struct SharedAttnParams {
   const int2* blocks_of;         // [units]
   float* acc;                    // [blocks + units][mpad][D]: the segment of block b on unit u stands at b + u
   float2* stat;                  // [blocks + units][mpad] maximum (base 2), denominator against it
-  long long slab_base;
+  long long slab_base, slabs;
   unsigned char* wait_flag;
   int rows, width, sub, subs, groups, cap, page_size, piece, tile_pieces, n_q, heads, G, mpad, xt_tile;
   float scale_log2;
@@ -331,6 +331,7 @@ __device__ __noinline__ void shared_give_back(const SharedAttnParams& p, const i
     for (int k = 0; k < PTC_KT; ++k) {
       if (!(m >> k & 1ull)) continue;
       const int tok = entries[first + k / p.piece].x + k % p.piece, page = tok / p.page_size, slot = tok - page * p.page_size;
+      if (p.slab_base + page >= p.slabs) continue;               // (behind the cache: the copies brought zeros)
       const uint32_t* src = reinterpret_cast<const uint32_t*>(p.kv + ((((p.slab_base + page) * 2 + 1) * p.page_size + slot) * p.heads + head) * D + c0);
       for (int i = 0; i < 16; ++i) {
         const uint32_t w = src[i];
@@ -747,7 +748,7 @@ extern "C" int vb_shared_attn(void* d_out, const void* d_q, const void* d_kv, in
   p.whole = p.counts + l.groups, p.len = p.whole + 2 * l.groups + 1;
   p.blocks_of = reinterpret_cast<const int2*>(at + l.blocks_of);
   p.acc = reinterpret_cast<float*>(at + l.acc), p.stat = reinterpret_cast<float2*>(at + l.stat);
-  p.slab_base = slab_base;
+  p.slab_base = slab_base, p.slabs = slabs;
   VB_CHECK_ARG(p.wait_flag = wait_flag(WK_PREFILL_ATTN), "vb_shared_attn: no mapped host memory");
   p.rows = plan->rows, p.width = plan->width, p.sub = l.sub, p.subs = l.subs, p.groups = l.groups, p.cap = l.cap, p.page_size = P, p.piece = piece;
   p.tile_pieces = PTC_KT / piece, p.n_q = plan->n_q, p.heads = H, p.G = plan->n_q / H, p.mpad = l.mpad, p.xt_tile = out_xt_tile;

@@ -2265,7 +2265,9 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, weight: Opti
     dtype = logits.dtype
     # (one comparison per fact when all of them hold; what does not says so in the check)
     if not (len(s) == len(z) == 2 and (dtype is BF16 or dtype is F32) and scores.dtype is F32 and logits.get_device() == scores.get_device() == dev and z[0] == s[0] * s[1] > 0
-            and s[1] <= BEAM_MAX_WIDTH and 1 <= n <= BEAM_MAX_N and 1 <= z[1] <= 1 << 24 and logits.stride(1) == 1 and scores.is_contiguous() and weight is None and ended is None
+            and s[1] <= BEAM_MAX_WIDTH and 1 <= n <= BEAM_MAX_N and 1 <= z[1] <= 1 << 24 and logits.stride(1) == 1 and scores.is_contiguous()
+            and (weight is None or (weight.get_device() == dev and weight.dtype is F32 and weight.shape == s and weight.is_contiguous()))
+            and (ended is None or (end_token is not None and ended.get_device() == dev and ended.dtype is torch.bool and ended.shape == s and ended.is_contiguous()))
             and (end_token is None or 0 <= end_token < z[1])):
         _beam_select_check(logits, scores, n, weight, ended, end_token)
     (B, W), (R, V), f32, on = s, z, dtype is F32, logits.device
@@ -2297,7 +2299,7 @@ def _beam_reorder_check(states, parent, slots) -> None:
 def beam_reorder(states: Sequence[torch.Tensor], parent: torch.Tensor, slots: Optional[torch.Tensor] = None) -> Sequence[torch.Tensor]:
     """Rows of recurrent states follow their beams, in place: with parent int32 [requests, width] row slots[b, i] of every state becomes what row
     slots[b, parent[b, i]] was; parent -1 (or outside the request): the row stays as it is.  states: contiguous tensors [slots, ...] of any types, all of one number of slots
-    (of a stack of layers: one each).  slots int32 [requests, width] (None: b * width + i); a slot belongs to one beam: one that is named twice receives either row; one outside
+    (of a stack of layers: one each), none of which overlaps another.  slots int32 [requests, width] (None: b * width + i); a slot belongs to one beam: one that is named twice receives either row; one outside
     the states is skipped.  Returns ``states``."""
     dev, by, k = _device_index(), parent.shape, len(states)
     ok = (parent.get_device() == dev and parent.dtype is torch.int32 and len(by) == 2 and parent.is_contiguous() and 0 < by[0] <= 65535 and 0 < by[1] <= BEAM_MAX_WIDTH
@@ -2322,7 +2324,7 @@ class PagePool:
     page, 0: free.  All rows are empty and all pages free at first.  ``fork_pages`` and ``compact_pages`` work on it without the host; ``check`` asks how the last one went.
 
     For ``plan_rows`` a pool is a page table of ``columns`` pages a row: kv_indptr = ``indptr``, kv_indices = ``table`` in one dimension, kv_len = ``tokens``.  A
-    page that is not full belongs to one row; whoever writes the tables himself (``load``) keeps to that."""
+    page that is not full belongs to one row; a program that writes the tables itself (``load``) keeps to that.  A pool belongs to one stream at a time."""
 
     def __init__(self, pages: int, page_size: int, rows: int, columns: int, device="cuda"):
         _refuse(pages < 1 or page_size < 1 or not 1 <= rows <= 4096 or columns < 1 or columns * page_size > 0x3fffffff or (columns + 1) * rows > 0x3fffffff,
