@@ -128,33 +128,27 @@ struct Held {
   }
 };
 
-// The n largest keys of the list's first c, in order, to its front.  (They differ: a key's place is the number of larger ones.)
-__device__ __forceinline__ void keep_largest(uint64_t* list, int c, int n) {
-  uint64_t key[BS_CAP / BS_THREADS];
-  int rank[BS_CAP / BS_THREADS];
-#pragma unroll
-  for (int e = 0; e < BS_CAP / BS_THREADS; ++e) {
-    const int i = threadIdx.x + e * BS_THREADS;
-    rank[e] = n;
-    if (i < c) {
-      key[e] = list[i];
-      int r = 0;
-#pragma unroll 8
-      for (int j = 0; j < c; ++j) r += list[j] > key[e] ? 1 : 0;
-      rank[e] = r;
-    }
+// The n largest keys of the list's first c, in order, to its front.  (They differ: a key's place is the number of larger ones, which four neighbours count.)
+__device__ __forceinline__ void keep_largest(uint64_t* list, uint64_t* sorted, int c, int n) {
+  const uint32_t quad = 0xfu << (threadIdx.x & 28);
+  for (int i = threadIdx.x >> 2; i < c; i += BS_THREADS / 4) {
+    const uint64_t key = list[i];
+    int r = 0;
+#pragma unroll 4
+    for (int j = threadIdx.x & 3; j < c; j += 4) r += list[j] > key ? 1 : 0;
+    r += __shfl_xor_sync(quad, r, 1);
+    r += __shfl_xor_sync(quad, r, 2);
+    if ((threadIdx.x & 3) == 0 && r < n) sorted[r] = key;
   }
   __syncthreads();
-#pragma unroll
-  for (int e = 0; e < BS_CAP / BS_THREADS; ++e)
-    if (rank[e] < n) list[rank[e]] = key[e];
+  if (threadIdx.x < min(c, n)) list[threadIdx.x] = sorted[threadIdx.x];
   __syncthreads();
 }
 
 constexpr int BS_SPAN = 32 * BS_VECS, BS_SLOT = (BS_SPAN + 1) * 16;      // vectors of a chunk that a warp reads, and bytes of the aligned ones that hold them
 struct PartShared {
   uint8_t ring[BS_STAGES][BS_THREADS / 32][BS_SLOT];
-  uint64_t list[BS_CAP];
+  uint64_t list[BS_CAP], sorted[BS_MAX_N];
   uint32_t box[3], count, tops[8];
   float part_m[8], part_s[8];
 };
@@ -345,7 +339,7 @@ __device__ __forceinline__ void beam_part(PartShared& sh, BeamStats* stats, uint
       __syncthreads();
       c = static_cast<int>(count);
     }
-    keep_largest(list, c, n);
+    keep_largest(list, sh.sorted, c, n);
     if (tid == 0) count = min(c, n);
     if (c >= n) above = unorder_f32(static_cast<uint32_t>(list[n - 1] >> 32)), low_cut = false;
     __syncthreads();
@@ -363,7 +357,7 @@ __device__ __forceinline__ void beam_part(PartShared& sh, BeamStats* stats, uint
     if (lane == 0) *stats = {top, top == -INFINITY ? 0.f : sum};
   }
   const int c = static_cast<int>(count);
-  keep_largest(list, c, n);
+  keep_largest(list, sh.sorted, c, n);
   if (tid < n) best[tid] = tid < c ? list[tid] : 0ull;
 }
 
@@ -546,12 +540,18 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(float* __restrict
     list_key[o] = key, list_at[o] = at, list_total[o] = total_of(w, e);
   }
   __syncthreads();
-  for (int i = tid; i < found; i += BJ_THREADS) {
+  const uint32_t quad = 0xfu << (lane & 28);
+  for (int i = tid >> 2; i < found; i += BJ_THREADS / 4) {
     const uint64_t k = list_key[i], at = list_at[i];
     int rank = 0;
-#pragma unroll 8
-    for (int j = 0; j < found; ++j) rank += list_key[j] > k || (list_key[j] == k && list_at[j] < at) ? 1 : 0;
-    if (rank < n) {
+#pragma unroll 4
+    for (int j = tid & 3; j < found; j += 4) {
+      const uint64_t kj = list_key[j], aj = list_at[j];
+      rank += (kj > k) | ((kj == k) & (aj < at));
+    }
+    rank += __shfl_xor_sync(quad, rank, 1);
+    rank += __shfl_xor_sync(quad, rank, 2);
+    if ((tid & 3) == 0 && rank < n) {
       const int w = static_cast<int>(at >> 32), o = b * n + rank;
       const uint32_t v = static_cast<uint32_t>(at);
       out_score[o] = static_cast<float>(list_total[i]);
