@@ -76,8 +76,8 @@ __device__ __forceinline__ T* in_block0(T* p) {
 }
 
 // What is known of a row stands in every block's shared memory.  A row that k rows continue adds k - 1 to the count of each of its pages, once a page and not
-// once a row that takes it over.  Counts and free pages stand in block 0's shared memory for pools of up to PG_SMEM_PAGES pages (measured, against scratch in
-// global memory: XXX), and are volatile to every block.
+// once a row that takes it over.  Counts and free pages stand in block 0's shared memory for pools of up to PG_SMEM_PAGES pages (scratch in global memory
+// beyond: a step of 64 rows took 13.0 us with it, 11.4 without, each launch by itself), and are volatile to every block.
 __global__ void __launch_bounds__(PG_THREADS, 1) fork_pages_kernel(const __grid_constant__ ForkParams p) {
   extern __shared__ int32_t pg_smem[];
   int32_t* s_src = pg_smem;                          // [rows] the row that a row continues, -1: none
@@ -352,7 +352,10 @@ __global__ void __launch_bounds__(PC_THREADS) copy_listed_pages_kernel(const __g
   }
 }
 
-static int copy_listed(const VbPageCache* caches, int n_caches, const VbPagePool* pool, const int32_t* copies, const int32_t* status, void* stream) {
+// Blocks of 256 threads an SM: whole pages move best with three (587 MB: 97.7 us; four 106.8, six 107.0, eight 109.5, two 110.9), the few tokens of a step's tails
+// with six (57 MB: 19.6 us the whole step; three 21.3, eight 19.7).
+constexpr int PC_WHOLE = 3, PC_TAILS = 6;
+static int copy_listed(const VbPageCache* caches, int n_caches, const VbPagePool* pool, const int32_t* copies, const int32_t* status, int blocks, void* stream) {
   for (int c0 = 0; c0 < n_caches; c0 += PC_CACHES) {
     CopyCaches t = {};
     t.n = n_caches - c0 < PC_CACHES ? n_caches - c0 : PC_CACHES;
@@ -368,7 +371,7 @@ static int copy_listed(const VbPageCache* caches, int n_caches, const VbPagePool
       t.units[c] = static_cast<int>((t.part[c] + PC_UNIT - 1) / PC_UNIT);
       t.first[c + 1] = t.first[c] + static_cast<long long>(s.layers) * s.parts * t.units[c];
     }
-    VB_LAUNCH_PDL(copy_listed_pages_kernel, sm_count() * 8, PC_THREADS, 0, stream, t, copies, status);
+    VB_LAUNCH_PDL(copy_listed_pages_kernel, sm_count() * blocks, PC_THREADS, 0, stream, t, copies, status);
   }
   return 0;
 }
@@ -425,7 +428,7 @@ extern "C" int vb_fork_pages(const VbPagePool* pool, const VbPagePool* out, cons
   const int cluster = share >= PG_MAX_CLUSTER ? PG_MAX_CLUSTER : share > 2 ? 4 : static_cast<int>(share);
   VB_CHECK_CUDA(rm_smem<fork_pages_kernel>((8 * PG_MAX_ROWS + PG_STAGE + 2 * PG_SMEM_PAGES) * 4));
   VB_LAUNCH_PDL_CLUSTER(fork_pages_kernel, cluster, PG_THREADS, (8 * p.rows + PG_STAGE + (p.in_smem ? 2 * p.pages : 0)) * 4, stream, cluster, p);
-  return copy_listed(caches, n_caches, pool, out->d_copies, out->d_status, stream);
+  return copy_listed(caches, n_caches, pool, out->d_copies, out->d_status, PC_TAILS, stream);
 }
 
 extern "C" int vb_compact_pages(const VbPagePool* pool, const VbPagePool* out, const VbPageCache* caches, int n_caches, void* stream) {
@@ -441,5 +444,5 @@ extern "C" int vb_compact_pages(const VbPagePool* pool, const VbPagePool* out, c
   const long long share = (p.cells + 4 * PG_THREADS - 1) / (4 * PG_THREADS);
   const int cluster = share >= PG_MAX_CLUSTER ? PG_MAX_CLUSTER : share > 2 ? 4 : static_cast<int>(share);
   VB_LAUNCH_PDL_CLUSTER(compact_pages_kernel, cluster, PG_THREADS, 0, stream, cluster, p);
-  return copy_listed(caches, n_caches, pool, out->d_copies, out->d_status, stream);
+  return copy_listed(caches, n_caches, pool, out->d_copies, out->d_status, PC_WHOLE, stream);
 }
