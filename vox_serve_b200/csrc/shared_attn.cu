@@ -42,7 +42,24 @@ struct SharedPlanParams {
   int rows, width, sub, subs, groups, cap, columns, pages, page_size, piece, tile_pieces, heads, grid;
 };
 
-constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32, SP_MAX_COLUMNS = 16384, SP_CLUSTER = 8;
+constexpr int SP_THREADS = 1024, SP_WARPS = SP_THREADS / 32, SP_CHUNK = 4 * SP_WARPS, SP_MAX_COLUMNS = 16384, SP_CLUSTER = 8;
+
+// exclusive prefix over a block of 1024 of what its threads have, and the total; `sums`: 32 words
+__device__ __forceinline__ int sp_prefix(int mine, int* sums, int& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int inc = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, inc, o);
+    if (lane >= o) inc += v;
+  }
+  __syncthreads();                                     // (the last call's sums have been read)
+  if (lane == 31) sums[warp] = inc;
+  __syncthreads();
+  const int all = sums[lane], before = __reduce_add_sync(0xffffffffu, lane < warp ? all : 0);
+  total = __reduce_add_sync(0xffffffffu, all);
+  return before + inc - mine;
+}
 
 __device__ __forceinline__ int shared_first_row(const SharedPlanParams& p, int g, int& n) {
   const int in = g % p.subs * p.sub;
@@ -75,175 +92,174 @@ __device__ __forceinline__ SharedColumn shared_column(const SharedPlanParams& p,
   return c;
 }
 
-// A cluster a group, its columns dealt out to the blocks in turn stretches.  Counted first, then written behind what stands in front.
+// A cluster a group, the columns in chunks of SP_CHUNK to its blocks in turn, four to a warp.  Counted first, then written behind what stands in front (block
+// after block).  The first chunk's pages are asked for together with the tokens and kept for the second look.
 __global__ void __launch_bounds__(SP_THREADS) shared_list_kernel(const __grid_constant__ SharedPlanParams p) {
-  extern __shared__ int2 sp_first[];                   // whole pieces and others in front of a column, within the block
-  __shared__ int2 sums[SP_WARPS], carry;
+  extern __shared__ int sp_first[];                    // [2][columns of the block] whole pieces in front of a column, others, within the block
+  __shared__ int sums[SP_WARPS];
   __shared__ float totals[2];                          // (ints, read by the other blocks)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = cluster_ctarank(), blocks = cluster_nctarank(), g = blockIdx.x / blocks;
   pdl_sync();
   int n;
   const int r0 = shared_first_row(p, g, n);
+  const int32_t* row = p.table + static_cast<long long>(r0 + (lane < n ? lane : 0)) * p.columns;
+  auto column = [&](int i) { return (i / SP_CHUNK * blocks + rank) * SP_CHUNK + i % SP_CHUNK; };
+  int kept[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) kept[j] = lane < n && column(warp * 4 + j) < p.columns ? row[column(warp * 4 + j)] : -1;
   int len = 0;
   if (lane < n) {
     len = p.tokens[r0 + lane];
     len = len < 0 ? 0 : min(len, p.columns * p.page_size);
     if (rank == 0 && warp == 0) p.len[r0 + lane] = len;
   }
-  const int32_t* row = p.table + static_cast<long long>(r0 + (lane < n ? lane : 0)) * p.columns;
   const uint32_t alive = __ballot_sync(0xffffffffu, len > 0);
   const int longest = __reduce_max_sync(0xffffffffu, len), columns = (longest + p.page_size - 1) / p.page_size;
-  const int each = (columns + blocks - 1) / blocks, c_lo = min(columns, rank * each), here = min(columns, c_lo + each) - c_lo;
-  auto page_at = [&](int c) { return c * p.page_size < len ? row[c] : -1; };
-  for (int c0 = warp * 4; c0 < here; c0 += SP_WARPS * 4) {
+  const int here = (columns + blocks * SP_CHUNK - 1) / (blocks * SP_CHUNK) * SP_CHUNK;      // (with places behind the last column)
+  int *first_w = sp_first, *first_o = sp_first + here;
+  auto pages_at = [&](int c0, int (&page)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) page[j] = c0 < SP_CHUNK ? kept[j] : column(c0 + j) * p.page_size < len ? row[column(c0 + j)] : -1;
+  };
+  for (int c0 = warp * 4; c0 < here; c0 += SP_CHUNK) {
     int page[4];
+    pages_at(c0, page);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) page[j] = c0 + j < here ? page_at(c_lo + c0 + j) : -1;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c0 + j < here) {
-        const SharedColumn c = shared_column(p, page[j], len - (c_lo + c0 + j) * p.page_size, alive);
-        const int all = __reduce_add_sync(0xffffffffu, c.pieces), whole = __reduce_add_sync(0xffffffffu, c.whole);
-        if (lane == 0) sp_first[c0 + j] = make_int2(whole, all - whole);
+    for (int j = 0; j < 4; ++j) {
+      const int col = column(c0 + j);
+      int all = 0, whole = 0;
+      if (col < columns) {
+        const SharedColumn c = shared_column(p, page[j], len - col * p.page_size, alive);
+        all = __reduce_add_sync(0xffffffffu, c.pieces), whole = __reduce_add_sync(0xffffffffu, c.whole);
       }
+      if (lane == 0) first_w[c0 + j] = whole, first_o[c0 + j] = all - whole;
+    }
   }
-  if (tid == 0) carry = make_int2(0, 0);
   __syncthreads();
+  int carry_w = 0, carry_o = 0;
   for (int c0 = 0; c0 < here; c0 += SP_THREADS) {       // exclusive prefix over the block's columns
     const int c = c0 + tid;
-    const int2 mine = c < here ? sp_first[c] : make_int2(0, 0);
-    int2 inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int x = __shfl_up_sync(0xffffffffu, inc.x, o), y = __shfl_up_sync(0xffffffffu, inc.y, o);
-      if (lane >= o) inc.x += x, inc.y += y;
-    }
-    if (lane == 31) sums[warp] = inc;
-    __syncthreads();
-    int2 before = carry, all = carry;
-#pragma unroll
-    for (int w = 0; w < SP_WARPS; ++w) {
-      if (w < warp) before.x += sums[w].x, before.y += sums[w].y;
-      all.x += sums[w].x, all.y += sums[w].y;
-    }
-    if (c < here) sp_first[c] = make_int2(before.x + inc.x - mine.x, before.y + inc.y - mine.y);
-    __syncthreads();
-    if (tid == 0) carry = all;
-    __syncthreads();
+    int all_w, all_o;
+    const int w = sp_prefix(c < here ? first_w[c] : 0, sums, all_w), o = sp_prefix(c < here ? first_o[c] : 0, sums, all_o);
+    if (c < here) first_w[c] = carry_w + w, first_o[c] = carry_o + o;
+    carry_w += all_w, carry_o += all_o;
   }
-  if (tid == 0) totals[0] = __int_as_float(carry.x), totals[1] = __int_as_float(carry.y);
-  cluster_sync_all();
-  int w0 = 0, o0 = 0, all_w = 0, all_o = 0;             // pieces of the blocks in front, of all
-  for (int b = 0; b < blocks; ++b) {
-    const int w = __float_as_int(ld_dsmem_f32(&totals[0], b)), o = __float_as_int(ld_dsmem_f32(&totals[1], b));
-    if (b < rank) w0 += w, o0 += o;
-    all_w += w, all_o += o;
+  if (tid == 0) totals[0] = __int_as_float(carry_w), totals[1] = __int_as_float(carry_o);
+  __syncthreads();
+  int w0 = 0, o0 = 0, all_w = carry_w, all_o = carry_o; // pieces of the blocks in front, of all
+  if (blocks > 1) {
+    cluster_sync_all();
+    all_w = all_o = 0;
+    for (int b = 0; b < blocks; ++b) {
+      const int w = __float_as_int(ld_dsmem_f32(&totals[0], b)), o = __float_as_int(ld_dsmem_f32(&totals[1], b));
+      if (b < rank) w0 += w, o0 += o;
+      all_w += w, all_o += o;
+    }
   }
   const int tiles_w = all_w / p.tile_pieces;            // (what is left of the whole ones fills the first of the others)
   if (rank == 0 && tid == 0) p.counts[g] = all_w + all_o, p.whole[g] = tiles_w;
   int4* out = p.entries + static_cast<long long>(g) * p.cap;
-  for (int c0 = warp * 4; c0 < here; c0 += SP_WARPS * 4) {
+  for (int c0 = warp * 4; c0 < here; c0 += SP_CHUNK) {
     int page[4];
+    pages_at(c0, page);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) page[j] = c0 + j < here ? page_at(c_lo + c0 + j) : -1;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (c0 + j < here) {
-        const int col = c_lo + c0 + j;
-        const SharedColumn c = shared_column(p, page[j], len - col * p.page_size, alive);
-        int2 inc = make_int2(c.whole, c.pieces - c.whole);
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const int x = __shfl_up_sync(0xffffffffu, inc.x, o), y = __shfl_up_sync(0xffffffffu, inc.y, o);
-          if (lane >= o) inc.x += x, inc.y += y;
-        }
-        const int2 first = sp_first[c0 + j];
-        int at_w = w0 + first.x + inc.x - c.whole, at_o = all_w + o0 + first.y + inc.y - (c.pieces - c.whole);
-        for (int i = 0; i < c.pieces; ++i) {
-          const int off = i * p.piece;
-          out[i < c.whole ? at_w++ : at_o++] = make_int4(c.page * p.page_size + off, col * p.page_size + off, static_cast<int>(c.same), min(p.piece, c.tokens - off));
-        }
-      }
-  }
-  cluster_sync_all();                                   // (totals have been read)
-}
-
-__global__ void __launch_bounds__(1024) shared_deal_kernel(const __grid_constant__ SharedPlanParams p) {
-  __shared__ int sums[32];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  pdl_sync();
-  int carry = 0;
-  for (int g0 = 0; g0 < p.groups; g0 += 1024) {
-    const int g = g0 + tid, mine = g < p.groups ? (__ldcg(p.counts + g) + p.tile_pieces - 1) / p.tile_pieces : 0;
-    int inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += v;
-    }
-    __syncthreads();
-    if (lane == 31) sums[warp] = inc;
-    __syncthreads();
-    int all = sums[lane], before = lane < warp ? all : 0;
-    all = __reduce_add_sync(0xffffffffu, all), before = __reduce_add_sync(0xffffffffu, before);
-    if (g < p.groups) p.tile0[g] = carry + before + inc - mine;
-    carry += all;
-  }
-  const int total = carry, units = p.groups * p.heads;
-  const long long work = static_cast<long long>(total) * p.heads;
-  if (tid == 0) p.tile0[p.groups] = total;
-  __syncthreads();
-  auto tile0 = [&](int g) { return __ldcg(p.tile0 + g); };
-  auto sum_of = [&](int v) {
-    v = __reduce_add_sync(0xffffffffu, v);
-    __syncthreads();
-    if (lane == 0) sums[warp] = v;
-    __syncthreads();
-    return __reduce_add_sync(0xffffffffu, sums[lane]);
-  };
-  if (units <= p.grid) {
-    // Blocks of their own for every unit (one that goes on to another unit waits for it: 5 us): equal segments of at most q tiles, q the smallest with which
-    // the blocks are enough.
-    int lo = static_cast<int>(max(1ll, (work + p.grid - 1) / p.grid)), hi = max(lo, total);
-    while (lo < hi) {
-      const int q = (lo + hi) >> 1;
-      int mine = 0;
-      for (int g = tid; g < p.groups; g += 1024) mine += (tile0(g + 1) - tile0(g) + q - 1) / q;
-      if (sum_of(mine) * p.heads <= p.grid) hi = q;
-      else lo = q + 1;
-    }
-    int used = 0;
-    for (int u0 = 0; u0 < units; u0 += 1024) {
-      const int u = u0 + tid, g = u / p.heads, tiles = u < units ? tile0(g + 1) - tile0(g) : 0, n = (tiles + lo - 1) / lo;
-      int inc = n;
+    for (int j = 0; j < 4; ++j) {
+      const int col = column(c0 + j);
+      if (col >= columns) break;
+      const SharedColumn c = shared_column(p, page[j], len - col * p.page_size, alive);
+      int inc_w = c.whole, inc_o = c.pieces - c.whole;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += v;
+        const int x = __shfl_up_sync(0xffffffffu, inc_w, o), y = __shfl_up_sync(0xffffffffu, inc_o, o);
+        if (lane >= o) inc_w += x, inc_o += y;
       }
+      int at_w = w0 + first_w[c0 + j] + inc_w - c.whole, at_o = all_w + o0 + first_o[c0 + j] + inc_o - (c.pieces - c.whole);
+      for (int i = 0; i < c.pieces; ++i) {
+        const int off = i * p.piece;
+        out[i < c.whole ? at_w++ : at_o++] = make_int4(c.page * p.page_size + off, col * p.page_size + off, static_cast<int>(c.same), min(p.piece, c.tokens - off));
+      }
+    }
+  }
+  if (blocks > 1) cluster_sync_all();                   // (totals have been read)
+}
+
+constexpr int SD_MAX_GROUPS = 4096;
+__global__ void __launch_bounds__(SP_THREADS) shared_deal_kernel(const __grid_constant__ SharedPlanParams p) {
+  __shared__ int sums[SP_WARPS], tiles_s[SD_MAX_GROUPS], first_s[SD_MAX_GROUPS];      // tiles of a group, its first block
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_sync();
+  const int units = p.groups * p.heads;
+  int total = 0;
+  for (int g0 = 0; g0 < p.groups; g0 += SP_THREADS) {
+    const int g = g0 + tid, mine = g < p.groups ? (__ldcg(p.counts + g) + p.tile_pieces - 1) / p.tile_pieces : 0;
+    int all;
+    const int before = sp_prefix(mine, sums, all);
+    if (units <= p.grid) {
+      if (g < p.groups) tiles_s[g] = mine;
+    } else if (g < p.groups) {
+      p.tile0[g] = total + before;
+    }
+    total += all;
+  }
+  const long long work = static_cast<long long>(total) * p.heads;
+  __syncthreads();
+  if (units <= p.grid) {
+    // Blocks of their own for every unit (one that goes on to another unit waits for it: 5 us): equal segments of at most q tiles, q the smallest with which
+    // the blocks are enough: a unit of t tiles takes at most t / q + 1 of them, which bounds it from above.  A warp tries one, 32 at once.
+    int lo = static_cast<int>(max(1ll, (work + p.grid - 1) / p.grid)), hi = max(lo, total);
+    if (units < p.grid) hi = max(lo, min(hi, static_cast<int>((work + p.grid - units - 1) / (p.grid - units))));
+    while (lo < hi) {
+      const int step = (hi - lo + SP_WARPS - 1) / SP_WARPS, q = min(lo + warp * step, hi);
+      int mine = 0;
+      for (int g = lane; g < p.groups; g += 32) mine += (tiles_s[g] + q - 1) / q;
+      mine = __reduce_add_sync(0xffffffffu, mine);
+      if (lane == 0) sums[warp] = mine * p.heads <= p.grid;
       __syncthreads();
-      if (lane == 31) sums[warp] = inc;
+      const uint32_t enough = __ballot_sync(0xffffffffu, sums[lane] != 0);
       __syncthreads();
-      int all = sums[lane], before = lane < warp ? all : 0;
-      all = __reduce_add_sync(0xffffffffu, all), before = __reduce_add_sync(0xffffffffu, before);
-      const int at = used + before + inc - n;
-      if (u < units) {
-        p.blocks_of[u] = make_int2(at, at + n - 1);
-        const int4 of = make_int4(__ldcg(p.counts + g), __ldcg(p.whole + g), 0, 0);
-        for (int i = 0; i < n; ++i) {
-          const int from = static_cast<int>(static_cast<long long>(tiles) * i / n), to = static_cast<int>(static_cast<long long>(tiles) * (i + 1) / n);
-          p.parts[2 * (at + i)] = make_int4(g, u - g * p.heads, from, to - from), p.parts[2 * (at + i) + 1] = of;
-        }
+      const int i = enough ? __ffs(enough) - 1 : SP_WARPS;      // the first that is enough
+      const int up = i < SP_WARPS ? min(lo + i * step, hi) : hi;
+      if (i > 0) lo = min(lo + (i - 1) * step, hi) + 1;
+      hi = max(lo, up);
+    }
+    const int q = lo;
+    int used = 0;
+    for (int g0 = 0; g0 < p.groups; g0 += SP_THREADS) {
+      const int g = g0 + tid, n = g < p.groups ? (tiles_s[g] + q - 1) / q : 0;
+      int all;
+      const int before = sp_prefix(n * p.heads, sums, all);
+      if (g < p.groups) {
+        first_s[g] = used + before;
+        for (int h = 0; h < p.heads; ++h) p.blocks_of[g * p.heads + h] = make_int2(used + before + h * n, used + before + h * n + n - 1);
       }
       used += all;
     }
-    for (int i = used + tid; i < p.grid; i += 1024) p.parts[2 * i] = make_int4(0, 0, 0, 0);
+    __syncthreads();
+    for (int i = tid; i < p.grid; i += SP_THREADS) {
+      int4 part = make_int4(0, 0, 0, 0), of = part;
+      if (i < used) {
+        int g = 0, last = p.groups - 1;                  // the last group that begins at or before this block (of several the others are empty)
+        while (g < last) {
+          const int mid = (g + last + 1) >> 1;
+          if (first_s[mid] <= i) g = mid;
+          else last = mid - 1;
+        }
+        const int tiles = tiles_s[g], n = (tiles + q - 1) / q, h = (i - first_s[g]) / n, k = (i - first_s[g]) - h * n;
+        const int from = static_cast<int>(static_cast<long long>(tiles) * k / n), to = static_cast<int>(static_cast<long long>(tiles) * (k + 1) / n);
+        part = make_int4(g, h, from, to - from);
+        of = make_int4(__ldcg(p.counts + g), __ldcg(p.whole + g), 0, 0);
+      }
+      p.parts[2 * i] = part, p.parts[2 * i + 1] = of;
+    }
     return;
   }
+  if (tid == 0) p.tile0[p.groups] = total;
+  __syncthreads();
+  auto tile0 = [&](int g) { return __ldcg(p.tile0 + g); };
   // More units than blocks: equal stretches of all their tiles in a line
   const long long blocks = min(work, static_cast<long long>(p.grid));      // (none without a tile: the join counts on it)
-  for (int i = tid; i < p.grid; i += 1024) {
+  for (int i = tid; i < p.grid; i += SP_THREADS) {
     int4 part = make_int4(0, 0, 0, 0), of = part;
     if (i < blocks) {
       const long long start = work * i / blocks;
@@ -259,7 +275,7 @@ __global__ void __launch_bounds__(1024) shared_deal_kernel(const __grid_constant
     }
     p.parts[2 * i] = part, p.parts[2 * i + 1] = of;
   }
-  for (int u = tid; u < units; u += 1024) {
+  for (int u = tid; u < units; u += SP_THREADS) {
     const int g = u / p.heads, t0 = tile0(g), tiles = tile0(g + 1) - t0;
     const long long first = static_cast<long long>(t0) * p.heads + static_cast<long long>(u - g * p.heads) * tiles;
     // (whose stretch holds a tile)
@@ -713,10 +729,9 @@ extern "C" int vb_shared_plan(const VbSharedPlan* plan, const int32_t* d_table, 
   p.rows = plan->rows, p.width = plan->width, p.sub = l.sub, p.subs = l.subs, p.groups = l.groups, p.cap = l.cap;
   p.columns = plan->columns, p.pages = pages, p.page_size = plan->page_size, p.piece = sa_piece(plan->page_size);
   p.tile_pieces = PTC_KT / p.piece, p.heads = plan->n_kv, p.grid = plan->grid;
-  const int cluster = plan->columns > 256 ? SP_CLUSTER : plan->columns > 64 ? 4 : plan->columns > 16 ? 2 : 1;
-  VB_CHECK_CUDA(rm_smem<shared_list_kernel>(SP_MAX_COLUMNS * 8));
-  VB_LAUNCH_PDL_CLUSTER(shared_list_kernel, l.groups * cluster, SP_THREADS, (plan->columns + cluster - 1) / cluster * 8, stream, cluster, p);
-  VB_LAUNCH_PDL(shared_deal_kernel, 1, 1024, 0, stream, p);
+  const int chunks = (plan->columns + SP_CHUNK - 1) / SP_CHUNK, cluster = chunks > 4 ? SP_CLUSTER : chunks > 2 ? 4 : chunks;      // (a chunk a block, as far as they go)
+  VB_LAUNCH_PDL_CLUSTER(shared_list_kernel, l.groups * cluster, SP_THREADS, (chunks + cluster - 1) / cluster * SP_CHUNK * 8, stream, cluster, p);
+  VB_LAUNCH_PDL(shared_deal_kernel, 1, SP_THREADS, 0, stream, p);
   return 0;
 }
 
