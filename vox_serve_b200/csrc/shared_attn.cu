@@ -42,9 +42,10 @@ struct SharedPlanParams {
   int rows, width, sub, subs, groups, cap, columns, pages, page_size, piece, tile_pieces, heads, grid;
 };
 
-constexpr int SP_THREADS = 1024, SP_WARPS = SP_THREADS / 32, SP_CHUNK = 4 * SP_WARPS, SP_MAX_COLUMNS = 16384, SP_CLUSTER = 8;
+constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32, SP_CHUNK = 128, SP_MAX_COLUMNS = 16384, SP_CLUSTER = 8;
 
-// exclusive prefix over a block of 1024 of what its threads have, and the total; `sums`: 32 words
+// exclusive prefix over a block of WARPS warps of what its threads have, and the total; `sums`: a word a warp
+template <int WARPS>
 __device__ __forceinline__ int sp_prefix(int mine, int* sums, int& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int inc = mine;
@@ -56,7 +57,7 @@ __device__ __forceinline__ int sp_prefix(int mine, int* sums, int& total) {
   __syncthreads();                                     // (the last call's sums have been read)
   if (lane == 31) sums[warp] = inc;
   __syncthreads();
-  const int all = sums[lane], before = __reduce_add_sync(0xffffffffu, lane < warp ? all : 0);
+  const int all = WARPS == 32 || lane < WARPS ? sums[lane] : 0, before = __reduce_add_sync(0xffffffffu, lane < warp ? all : 0);
   total = __reduce_add_sync(0xffffffffu, all);
   return before + inc - mine;
 }
@@ -92,22 +93,33 @@ __device__ __forceinline__ SharedColumn shared_column(const SharedPlanParams& p,
   return c;
 }
 
-// A cluster a group, the columns in chunks of SP_CHUNK to its blocks in turn, four to a warp.  Counted first, then written behind what stands in front (block
-// after block).  The first chunk's pages are asked for together with the tokens and kept for the second look.
+// A cluster a group, its columns in chunks to the blocks in turn.  A column of which all living rows see one whole page is known by its largest and least page
+// number: threads side by side read columns side by side, four of them the rows of one.  The others, where rows have parted, take a warp each, a lane a row.
+// Counted first, then written behind what stands in front, block after block.  What bounds it is latency: the tables' and the code's own, which runs once; so no
+// loop is unrolled but those of loads, and blocks have no more warps than load.  Both launches, one after the other in a graph (the first columns of the table in
+// brackets): 2 requests of 5 rows [1273] 12.3 us, 8 of 8 [34] 11.5, one of 4 [11] 11.2; every column with a warp, four unrolled, took 36.5, 18.1 and 12.7.
 __global__ void __launch_bounds__(SP_THREADS) shared_list_kernel(const __grid_constant__ SharedPlanParams p) {
-  extern __shared__ int sp_first[];                    // [2][columns of the block] whole pieces in front of a column, others, within the block
-  __shared__ int sums[SP_WARPS];
+  extern __shared__ int sp_smem[];                     // of the block's columns: whole pieces in front, others in front, the page that all see, those that have parted
+  __shared__ int sums[SP_WARPS], n_parted;
+  __shared__ int2 seen[SP_THREADS];
   __shared__ float totals[2];                          // (ints, read by the other blocks)
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = cluster_ctarank(), blocks = cluster_nctarank(), g = blockIdx.x / blocks;
+  const int at_c = tid % SP_CHUNK, at_r = tid / SP_CHUNK;
+  constexpr int ACROSS = SP_THREADS / SP_CHUNK;
+  if (tid == 0) n_parted = 0;
   pdl_sync();
   int n;
   const int r0 = shared_first_row(p, g, n);
-  const int32_t* row = p.table + static_cast<long long>(r0 + (lane < n ? lane : 0)) * p.columns;
+  const int32_t* table = p.table + static_cast<long long>(r0) * p.columns;
   auto column = [&](int i) { return (i / SP_CHUNK * blocks + rank) * SP_CHUNK + i % SP_CHUNK; };
-  int kept[4];
+  int v[32 / ACROSS];
+  auto ask = [&](int c) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) kept[j] = lane < n && column(warp * 4 + j) < p.columns ? row[column(warp * 4 + j)] : -1;
+    for (int j = 0; j < 32 / ACROSS; ++j)
+      if (at_r + j * ACROSS < n && c < p.columns) v[j] = table[static_cast<long long>(at_r + j * ACROSS) * p.columns + c];
+  };
+  ask(column(at_c));                                   // (on its way together with the tokens)
   int len = 0;
   if (lane < n) {
     len = p.tokens[r0 + lane];
@@ -115,33 +127,45 @@ __global__ void __launch_bounds__(SP_THREADS) shared_list_kernel(const __grid_co
     if (rank == 0 && warp == 0) p.len[r0 + lane] = len;
   }
   const uint32_t alive = __ballot_sync(0xffffffffu, len > 0);
-  const int longest = __reduce_max_sync(0xffffffffu, len), columns = (longest + p.page_size - 1) / p.page_size;
+  const int longest = __reduce_max_sync(0xffffffffu, len), shortest = __reduce_min_sync(0xffffffffu, len > 0 ? len : 0x7fffffff);
+  const int columns = (longest + p.page_size - 1) / p.page_size, per_page = p.page_size / p.piece;
   const int here = (columns + blocks * SP_CHUNK - 1) / (blocks * SP_CHUNK) * SP_CHUNK;      // (with places behind the last column)
-  int *first_w = sp_first, *first_o = sp_first + here;
-  auto pages_at = [&](int c0, int (&page)[4]) {
+  int *first_w = sp_smem, *first_o = first_w + here, *one = first_o + here, *parted = one + here;
+  for (int c0 = 0; c0 < here; c0 += SP_CHUNK) {
+    const int i = c0 + at_c, c = column(i);
+    if (c0 > 0) ask(c);
+    int2 m = make_int2(-1, 0x7fffffff);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) page[j] = c0 < SP_CHUNK ? kept[j] : column(c0 + j) * p.page_size < len ? row[column(c0 + j)] : -1;
-  };
-  for (int c0 = warp * 4; c0 < here; c0 += SP_CHUNK) {
-    int page[4];
-    pages_at(c0, page);
+    for (int j = 0; j < 32 / ACROSS; ++j)
+      if (at_r + j * ACROSS < n && c < columns && (alive >> (at_r + j * ACROSS) & 1u)) m = make_int2(max(m.x, v[j]), min(m.y, v[j]));
+    seen[tid] = m;
+    __syncthreads();
+    if (at_r == 0) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int col = column(c0 + j);
-      int all = 0, whole = 0;
-      if (col < columns) {
-        const SharedColumn c = shared_column(p, page[j], len - col * p.page_size, alive);
-        all = __reduce_add_sync(0xffffffffu, c.pieces), whole = __reduce_add_sync(0xffffffffu, c.whole);
-      }
-      if (lane == 0) first_w[c0 + j] = whole, first_o[c0 + j] = all - whole;
+      for (int k = 1; k < ACROSS; ++k) m = make_int2(max(m.x, seen[at_c + k * SP_CHUNK].x), min(m.y, seen[at_c + k * SP_CHUNK].y));
+      const bool same = c < columns && (c + 1) * p.page_size <= shortest && m.x == m.y && m.x >= 0 && m.x < p.pages;
+      first_w[i] = same ? per_page : 0, first_o[i] = 0, one[i] = same ? m.x : -1;
+      if (!same && c < columns) parted[atomicAdd(&n_parted, 1)] = i;
     }
+    __syncthreads();
+  }
+  const int n_warp = n_parted;
+  auto parted_column = [&](int i) {
+    const int c = column(i);
+    return shared_column(p, c * p.page_size < len ? table[static_cast<long long>(lane) * p.columns + c] : -1, len - c * p.page_size, alive);
+  };
+#pragma unroll 1
+  for (int k = warp; k < n_warp; k += SP_WARPS) {
+    const SharedColumn c = parted_column(parted[k]);
+    const int all = __reduce_add_sync(0xffffffffu, c.pieces), whole = __reduce_add_sync(0xffffffffu, c.whole);
+    if (lane == 0) first_w[parted[k]] = whole, first_o[parted[k]] = all - whole;
   }
   __syncthreads();
   int carry_w = 0, carry_o = 0;
   for (int c0 = 0; c0 < here; c0 += SP_THREADS) {       // exclusive prefix over the block's columns
     const int c = c0 + tid;
     int all_w, all_o;
-    const int w = sp_prefix(c < here ? first_w[c] : 0, sums, all_w), o = sp_prefix(c < here ? first_o[c] : 0, sums, all_o);
+    const int w = sp_prefix<SP_WARPS>(c < here ? first_w[c] : 0, sums, all_w), o = sp_prefix<SP_WARPS>(c < here ? first_o[c] : 0, sums, all_o);
     if (c < here) first_w[c] = carry_w + w, first_o[c] = carry_o + o;
     carry_w += all_w, carry_o += all_o;
   }
@@ -160,41 +184,42 @@ __global__ void __launch_bounds__(SP_THREADS) shared_list_kernel(const __grid_co
   const int tiles_w = all_w / p.tile_pieces;            // (what is left of the whole ones fills the first of the others)
   if (rank == 0 && tid == 0) p.counts[g] = all_w + all_o, p.whole[g] = tiles_w;
   int4* out = p.entries + static_cast<long long>(g) * p.cap;
-  for (int c0 = warp * 4; c0 < here; c0 += SP_CHUNK) {
-    int page[4];
-    pages_at(c0, page);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int col = column(c0 + j);
-      if (col >= columns) break;
-      const SharedColumn c = shared_column(p, page[j], len - col * p.page_size, alive);
-      int inc_w = c.whole, inc_o = c.pieces - c.whole;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int x = __shfl_up_sync(0xffffffffu, inc_w, o), y = __shfl_up_sync(0xffffffffu, inc_o, o);
-        if (lane >= o) inc_w += x, inc_o += y;
-      }
-      int at_w = w0 + first_w[c0 + j] + inc_w - c.whole, at_o = all_w + o0 + first_o[c0 + j] + inc_o - (c.pieces - c.whole);
-      for (int i = 0; i < c.pieces; ++i) {
-        const int off = i * p.piece;
-        out[i < c.whole ? at_w++ : at_o++] = make_int4(c.page * p.page_size + off, col * p.page_size + off, static_cast<int>(c.same), min(p.piece, c.tokens - off));
-      }
+#pragma unroll 1
+  for (int k = warp; k < n_warp; k += SP_WARPS) {
+    const int at = parted[k], col = column(at);
+    const SharedColumn c = parted_column(at);
+    int inc_w = c.whole, inc_o = c.pieces - c.whole;
+#pragma unroll 1
+    for (int o = 1; o < 32; o <<= 1) {
+      const int x = __shfl_up_sync(0xffffffffu, inc_w, o), y = __shfl_up_sync(0xffffffffu, inc_o, o);
+      if (lane >= o) inc_w += x, inc_o += y;
+    }
+    int at_w = w0 + first_w[at] + inc_w - c.whole, at_o = all_w + o0 + first_o[at] + inc_o - (c.pieces - c.whole);
+#pragma unroll 1
+    for (int i = 0; i < c.pieces; ++i) {
+      const int off = i * p.piece;
+      out[i < c.whole ? at_w++ : at_o++] = make_int4(c.page * p.page_size + off, col * p.page_size + off, static_cast<int>(c.same), min(p.piece, c.tokens - off));
     }
   }
+#pragma unroll 1
+  for (int i = at_c; i < here; i += SP_CHUNK)
+    if (one[i] >= 0)
+      for (int k = at_r; k < per_page; k += ACROSS)
+        out[w0 + first_w[i] + k] = make_int4(one[i] * p.page_size + k * p.piece, column(i) * p.page_size + k * p.piece, static_cast<int>(alive), p.piece);
   if (blocks > 1) cluster_sync_all();                   // (totals have been read)
 }
 
-constexpr int SD_MAX_GROUPS = 4096;
-__global__ void __launch_bounds__(SP_THREADS) shared_deal_kernel(const __grid_constant__ SharedPlanParams p) {
-  __shared__ int sums[SP_WARPS], tiles_s[SD_MAX_GROUPS], first_s[SD_MAX_GROUPS];      // tiles of a group, its first block
+constexpr int SD_THREADS = 1024, SD_WARPS = SD_THREADS / 32, SD_MAX_GROUPS = 4096;
+__global__ void __launch_bounds__(SD_THREADS) shared_deal_kernel(const __grid_constant__ SharedPlanParams p) {
+  __shared__ int sums[SD_WARPS], tiles_s[SD_MAX_GROUPS], first_s[SD_MAX_GROUPS];      // tiles of a group, its first block
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_sync();
   const int units = p.groups * p.heads;
   int total = 0;
-  for (int g0 = 0; g0 < p.groups; g0 += SP_THREADS) {
+  for (int g0 = 0; g0 < p.groups; g0 += SD_THREADS) {
     const int g = g0 + tid, mine = g < p.groups ? (__ldcg(p.counts + g) + p.tile_pieces - 1) / p.tile_pieces : 0;
     int all;
-    const int before = sp_prefix(mine, sums, all);
+    const int before = sp_prefix<SD_WARPS>(mine, sums, all);
     if (units <= p.grid) {
       if (g < p.groups) tiles_s[g] = mine;
     } else if (g < p.groups) {
@@ -210,7 +235,7 @@ __global__ void __launch_bounds__(SP_THREADS) shared_deal_kernel(const __grid_co
     int lo = static_cast<int>(max(1ll, (work + p.grid - 1) / p.grid)), hi = max(lo, total);
     if (units < p.grid) hi = max(lo, min(hi, static_cast<int>((work + p.grid - units - 1) / (p.grid - units))));
     while (lo < hi) {
-      const int step = (hi - lo + SP_WARPS - 1) / SP_WARPS, q = min(lo + warp * step, hi);
+      const int step = (hi - lo + SD_WARPS - 1) / SD_WARPS, q = min(lo + warp * step, hi);
       int mine = 0;
       for (int g = lane; g < p.groups; g += 32) mine += (tiles_s[g] + q - 1) / q;
       mine = __reduce_add_sync(0xffffffffu, mine);
@@ -218,17 +243,17 @@ __global__ void __launch_bounds__(SP_THREADS) shared_deal_kernel(const __grid_co
       __syncthreads();
       const uint32_t enough = __ballot_sync(0xffffffffu, sums[lane] != 0);
       __syncthreads();
-      const int i = enough ? __ffs(enough) - 1 : SP_WARPS;      // the first that is enough
-      const int up = i < SP_WARPS ? min(lo + i * step, hi) : hi;
+      const int i = enough ? __ffs(enough) - 1 : SD_WARPS;      // the first that is enough
+      const int up = i < SD_WARPS ? min(lo + i * step, hi) : hi;
       if (i > 0) lo = min(lo + (i - 1) * step, hi) + 1;
       hi = max(lo, up);
     }
     const int q = lo;
     int used = 0;
-    for (int g0 = 0; g0 < p.groups; g0 += SP_THREADS) {
+    for (int g0 = 0; g0 < p.groups; g0 += SD_THREADS) {
       const int g = g0 + tid, n = g < p.groups ? (tiles_s[g] + q - 1) / q : 0;
       int all;
-      const int before = sp_prefix(n * p.heads, sums, all);
+      const int before = sp_prefix<SD_WARPS>(n * p.heads, sums, all);
       if (g < p.groups) {
         first_s[g] = used + before;
         for (int h = 0; h < p.heads; ++h) p.blocks_of[g * p.heads + h] = make_int2(used + before + h * n, used + before + h * n + n - 1);
@@ -236,7 +261,7 @@ __global__ void __launch_bounds__(SP_THREADS) shared_deal_kernel(const __grid_co
       used += all;
     }
     __syncthreads();
-    for (int i = tid; i < p.grid; i += SP_THREADS) {
+    for (int i = tid; i < p.grid; i += SD_THREADS) {
       int4 part = make_int4(0, 0, 0, 0), of = part;
       if (i < used) {
         int g = 0, last = p.groups - 1;                  // the last group that begins at or before this block (of several the others are empty)
@@ -259,7 +284,7 @@ __global__ void __launch_bounds__(SP_THREADS) shared_deal_kernel(const __grid_co
   auto tile0 = [&](int g) { return __ldcg(p.tile0 + g); };
   // More units than blocks: equal stretches of all their tiles in a line
   const long long blocks = min(work, static_cast<long long>(p.grid));      // (none without a tile: the join counts on it)
-  for (int i = tid; i < p.grid; i += SP_THREADS) {
+  for (int i = tid; i < p.grid; i += SD_THREADS) {
     int4 part = make_int4(0, 0, 0, 0), of = part;
     if (i < blocks) {
       const long long start = work * i / blocks;
@@ -275,7 +300,7 @@ __global__ void __launch_bounds__(SP_THREADS) shared_deal_kernel(const __grid_co
     }
     p.parts[2 * i] = part, p.parts[2 * i + 1] = of;
   }
-  for (int u = tid; u < units; u += SP_THREADS) {
+  for (int u = tid; u < units; u += SD_THREADS) {
     const int g = u / p.heads, t0 = tile0(g), tiles = tile0(g + 1) - t0;
     const long long first = static_cast<long long>(t0) * p.heads + static_cast<long long>(u - g * p.heads) * tiles;
     // (whose stretch holds a tile)
@@ -730,8 +755,8 @@ extern "C" int vb_shared_plan(const VbSharedPlan* plan, const int32_t* d_table, 
   p.columns = plan->columns, p.pages = pages, p.page_size = plan->page_size, p.piece = sa_piece(plan->page_size);
   p.tile_pieces = PTC_KT / p.piece, p.heads = plan->n_kv, p.grid = plan->grid;
   const int chunks = (plan->columns + SP_CHUNK - 1) / SP_CHUNK, cluster = chunks > 4 ? SP_CLUSTER : chunks > 2 ? 4 : chunks;      // (a chunk a block, as far as they go)
-  VB_LAUNCH_PDL_CLUSTER(shared_list_kernel, l.groups * cluster, SP_THREADS, (chunks + cluster - 1) / cluster * SP_CHUNK * 8, stream, cluster, p);
-  VB_LAUNCH_PDL(shared_deal_kernel, 1, SP_THREADS, 0, stream, p);
+  VB_LAUNCH_PDL_CLUSTER(shared_list_kernel, l.groups * cluster, SP_THREADS, (chunks + cluster - 1) / cluster * SP_CHUNK * 16, stream, cluster, p);
+  VB_LAUNCH_PDL(shared_deal_kernel, 1, SD_THREADS, 0, stream, p);
   return 0;
 }
 
