@@ -32,9 +32,10 @@ constexpr int SA_SMEM = SA_OUT<D> + 128 * 64 + 1024;
 inline int sa_piece(int page_size) { return page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : 16; }
 
 // ---- the plan -------------------------------------------------------------------------------------------------------------------
+constexpr int SD_PART = 8;       // words of 16 bytes, a line: a block knows what to fetch first with one load
 struct SharedPlanParams {
   int4* entries;                 // [groups][cap]: {token's place in a layer's pages, its position, rows that hold it, tokens}
-  int4* parts;                   // [grid][2] {group, head, first tile, tiles}, {pieces of the group, its tiles that are seen whole}
+  int4* parts;                   // [grid][SD_PART]: {group, head, first tile, tiles}, {pieces of the group, its tiles that are seen whole}, the first tile's pieces
   int32_t *counts, *whole, *len; // [groups] pieces and tiles that are seen whole, [rows]
   int32_t* tile0;                // [groups + 1] tiles in front of a group
   int2* blocks_of;               // [units] first and last block of a unit
@@ -215,6 +216,16 @@ __global__ void __launch_bounds__(SD_THREADS) shared_deal_kernel(const __grid_co
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_sync();
   const int units = p.groups * p.heads;
+  auto write_part = [&](int i, const int4& part, const int4& of) {
+    int4 *to = p.parts + i * SD_PART, e[4];
+    const int first = part.z * p.tile_pieces;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      e[k] = k < p.tile_pieces && part.w > 0 && first + k < of.x ? __ldcg(p.entries + static_cast<long long>(part.x) * p.cap + first + k) : make_int4(0, 0, 0, 0);
+    to[0] = part, to[1] = of;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) to[2 + k] = e[k];
+  };
   int total = 0;
   for (int g0 = 0; g0 < p.groups; g0 += SD_THREADS) {
     const int g = g0 + tid, mine = g < p.groups ? (__ldcg(p.counts + g) + p.tile_pieces - 1) / p.tile_pieces : 0;
@@ -275,7 +286,7 @@ __global__ void __launch_bounds__(SD_THREADS) shared_deal_kernel(const __grid_co
         part = make_int4(g, h, from, to - from);
         of = make_int4(__ldcg(p.counts + g), __ldcg(p.whole + g), 0, 0);
       }
-      p.parts[2 * i] = part, p.parts[2 * i + 1] = of;
+      write_part(i, part, of);
     }
     return;
   }
@@ -298,7 +309,7 @@ __global__ void __launch_bounds__(SD_THREADS) shared_deal_kernel(const __grid_co
       part = make_int4(lo, in / tiles, in % tiles, static_cast<int>(work * (i + 1) / blocks - start));
       of = make_int4(__ldcg(p.counts + lo), __ldcg(p.whole + lo), 0, 0);
     }
-    p.parts[2 * i] = part, p.parts[2 * i + 1] = of;
+    write_part(i, part, of);
   }
   for (int u = tid; u < units; u += SD_THREADS) {
     const int g = u / p.heads, t0 = tile0(g), tiles = tile0(g + 1) - t0;
@@ -516,7 +527,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 2) shared_attn_kernel(const __gri
   const uint32_t tmem_base = sh->tmem;
   if (tid == 0) sh2->tmem = tmem_base;
   pdl_wait();
-  const int4 part = p.parts[2 * blockIdx.x], of = p.parts[2 * blockIdx.x + 1];
+  const int4 part = p.parts[SD_PART * blockIdx.x], of = p.parts[SD_PART * blockIdx.x + 1], head_piece = p.parts[SD_PART * blockIdx.x + 2 + (lane & 3)];
   pdl_trigger();
 #pragma unroll 1
   for (int pass = 0; part.w > 0; ++pass) {
@@ -554,7 +565,7 @@ __global__ void __launch_bounds__(PTC_THREADS, 2) shared_attn_kernel(const __gri
         const int i = w.t * p.tile_pieces + lane;
         return lane < p.tile_pieces && w.left > 0 && i < w.count ? p.entries[static_cast<long long>(w.g) * p.cap + i] : make_int4(0, 0, 0, 0);
       };
-      int4 next = find();
+      int4 next = lane < p.tile_pieces ? head_piece : make_int4(0, 0, 0, 0);      // (the first tile's)
       uint32_t turn = 0;                                      // bit s: parity of stage s's next tile that is changed
       bool pending = false;                                   // the tile in front, if its values are still to be changed
       for (int j = 0; j <= part.w; ++j) {
@@ -623,7 +634,7 @@ constexpr int SJ_WARPS = 8;
 template <int D, int WPR>
 __global__ void __launch_bounds__(32 * SJ_WARPS) shared_join_kernel(const __grid_constant__ SharedAttnParams p) {
   constexpr int E = D / 32;
-  __shared__ float part[SJ_WARPS][32][E + 1];
+  __shared__ float part[SJ_WARPS][32][E + 1], tops[SJ_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, unit = blockIdx.x, g = unit / p.heads, h = unit - g * p.heads;
   const int m = blockIdx.y * (SJ_WARPS / WPR) + warp / WPR, sub = warp % WPR;
   pdl_sync();
@@ -631,40 +642,60 @@ __global__ void __launch_bounds__(32 * SJ_WARPS) shared_join_kernel(const __grid
   const int r0 = shared_group(p, g, n_rows);
   const bool on = m < n_rows * p.G;
   const int row = r0 + (on ? m / p.G : 0), k = (h * p.G + (on ? m % p.G : 0)) * D + lane * E;
-  float acc[E], total = 0.f;
+  const int2 blocks = p.blocks_of[unit];
+  float acc[E], total = 0.f, top = -INFINITY;                   // against the largest maximum so far
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
   if (on && p.len[row] > 0) {
-    const int2 blocks = p.blocks_of[unit];
     const int s0 = blocks.x + unit, s1 = blocks.y + unit + 1;
-    float top = -INFINITY;
-    for (int s = s0 + lane; s < s1; s += 32) top = fmaxf(top, p.stat[static_cast<long long>(s) * p.mpad + m].x);
-    top = warp_max(top);
-    if (top == -INFINITY) top = 0.f;                            // (scores that are all NaN: the sums below say so)
-#pragma unroll 8
-    for (int s = s0 + sub; s < s1; s += WPR) {
-      const long long at = static_cast<long long>(s) * p.mpad + m;
-      const float2 st = p.stat[at];
-      const float f = st.x == -INFINITY ? (st.y == 0.f ? 0.f : 1.f) : ptc_ex2(st.x - top);      // (nothing seen; scores that are NaN)
-      float v[E];
-      if (E == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(p.acc + at * D + lane * E);
-      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(p.acc + at * D + lane * E);
-      total += st.y * f;
+    for (int s = s0 + sub; s < s1; s += 8 * WPR) {              // eight segments' maxima and outputs at once
+      float2 st[8];
+      float v[8][E];
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] += v[e] * f;
+      for (int i = 0; i < 8; ++i) {
+        const long long at = static_cast<long long>(s + i * WPR) * p.mpad + m;
+        const bool in = s + i * WPR < s1;
+        st[i] = in ? p.stat[at] : make_float2(-INFINITY, 0.f);
+        if (E == 4) *reinterpret_cast<float4*>(v[i]) = in ? *reinterpret_cast<const float4*>(p.acc + at * D + lane * E) : make_float4(0.f, 0.f, 0.f, 0.f);
+        else *reinterpret_cast<float2*>(v[i]) = in ? *reinterpret_cast<const float2*>(p.acc + at * D + lane * E) : make_float2(0.f, 0.f);
+      }
+      float most = top;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = fmaxf(most, st[i].x);
+      const float keep = top == -INFINITY ? 1.f : ptc_ex2(top - most);      // (nothing yet, or what is not a number)
+      total *= keep;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= keep;
+      top = most;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float f = st[i].x == -INFINITY ? (st[i].y == 0.f ? 0.f : 1.f) : ptc_ex2(st[i].x - top);      // (nothing seen; scores that are NaN)
+        total += st[i].y * f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) acc[e] += v[i][e] * f;
+      }
     }
   }
   if (WPR > 1) {
 #pragma unroll
     for (int e = 0; e < E; ++e) part[warp][lane][e] = acc[e];
     part[warp][lane][E] = total;
+    if (lane == 0) tops[warp] = top;
     __syncthreads();
     if (sub == 0) {
+      float most = top;
+#pragma unroll
+      for (int w = 1; w < WPR; ++w) most = fmaxf(most, tops[warp + w]);
+      const float keep = top == -INFINITY ? 1.f : ptc_ex2(top - most);
+      total *= keep;
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] *= keep;
 #pragma unroll
       for (int w = 1; w < WPR; ++w) {
+        const float f = tops[warp + w] == -INFINITY ? 1.f : ptc_ex2(tops[warp + w] - most);
 #pragma unroll
-        for (int e = 0; e < E; ++e) acc[e] += part[warp + w][lane][e];
-        total += part[warp + w][lane][E];
+        for (int e = 0; e < E; ++e) acc[e] += part[warp + w][lane][e] * f;
+        total += part[warp + w][lane][E] * f;
       }
     }
   }
@@ -720,7 +751,7 @@ static SharedLayout shared_layout(const VbSharedPlan* s) {
   l.mpad = (l.sub * G + 15) / 16 * 16;
   const size_t units = static_cast<size_t>(l.groups) * s->n_kv, segments = s->grid + units;
   l.parts = 16ull * l.groups * l.cap;
-  l.acc = l.parts + 32ull * s->grid;
+  l.acc = l.parts + 16ull * SD_PART * s->grid;
   l.stat = l.acc + 4ull * segments * l.mpad * s->head_dim;
   l.blocks_of = l.stat + 8ull * segments * l.mpad;
   l.ints = l.blocks_of + 8ull * units;
