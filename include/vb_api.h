@@ -75,7 +75,7 @@ int vb_rope(void* d_q_out, void* d_k_out, const void* d_q, const void* d_k, cons
  * qo_indptr == NULL means decode (one row per request).  d_kv_len (optional, [B]) gives each request's kv
  * length explicitly -- then the page table may hold pre-allocated pages beyond it and last_page_len is
  * ignored (device-resident decode loop; the reference derives the length from the table, :96-97).  Rows >= n_rows_valid up to n_rows_padded get
- * page = -1 (their K/V append is skipped; the reference scatters them into page -1).
+ * page = -1 (their K/V append is skipped; the reference scatters them into page -1).  So has the row of a request of no tokens (d_kv_len 0).
  * Outputs (device int32): row_req[R], row_kvlen[R], row_page[R], row_slot[R], row_chunk_start[R+1] (exclusive
  * prefix of ceil(kvlen / chunk_tokens): the attention kernel's work list), row_pagebase[R] (= kv_indptr of the
  * row's request, so the attention kernel resolves a tile's page with one load) and row_old[R] (tokens of the

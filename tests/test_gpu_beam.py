@@ -295,3 +295,28 @@ def test_reorder_of_a_large_state():
     t[:, 0] = 100 + torch.arange(12, device="cuda", dtype=torch.int32)
     ops.beam_reorder([t], torch.tensor([[3, 0, 1, 2]], dtype=I32, device="cuda"), torch.tensor([[11, 10, 1, 0]], dtype=I32, device="cuda"))
     assert t[:, -1].tolist() == [1, 10, 2, 3, 4, 5, 6, 7, 8, 9, 11, 0] and t[:, 0].tolist() == [101, 110, 102, 103, 104, 105, 106, 107, 108, 109, 111, 100]
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_the_largest_vocabulary(dtype):
+    z, s = _inputs(1, 1, 1 << 24, dtype)
+    _check(ops.beam_select(z, s, 3), z, s, 3)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("V", [9, 40, 12345])
+def test_everything_at_once(V, dtype):
+    """weights, beams that ended, dead ones, masks, rows apart, requests with fewer candidates than are asked for, one with none"""
+    B, W, n, end = 4, 6, 50, 3
+    z, s = _inputs(B, W, V + 5, dtype, seed=3)
+    z = z[:, 2:2 + V]
+    weight = torch.rand(B, W, device="cuda") + 0.2
+    ended = torch.zeros(B, W, dtype=torch.bool, device="cuda")
+    ended[0, 1] = ended[1, 2] = ended[1, 5] = True
+    s[0, 3], s[2, 1:], s[3, :] = -INF, -INF, -INF
+    ended[2, 4] = True                                       # (dead: its ended bit does not wake it)
+    weight[1, 0], weight[0, 5] = 0.0, NAN
+    z[W + 3] = -INF
+    z[::2, V // 2:] = torch.finfo(dtype).min
+    z[1::2, :V // 3] = -INF
+    _check(ops.beam_select(z, s, n, weight=weight, ended=ended, end_token=end), z, s, n, weight, ended, end)

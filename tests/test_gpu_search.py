@@ -189,3 +189,63 @@ def test_plans_of_other_steps_are_refused():
     ops.plan_rows(s.eng.plan, _i32([0, 4, 8]), s.pool.indptr, s.pool.table.view(-1), None, 2, 8, PAGE, s.eng.chunk, kv_len=s.pool.tokens)
     with pytest.raises(ops.VoxB200Error, match="decode steps"):
         s.eng.forward(s.ids, s.pool.tokens - 1, 8, shared=s.plan)
+
+
+@pytest.mark.parametrize("mode", ["unfused", "fused"])
+def test_a_request_that_leaves(mode):
+    """its rows stay in the step without a token: positions of -1, token -1, no page is written for them, and the others' logits are those of their sequences"""
+    s = Search(mode)
+    s.start()
+    for _ in range(3):
+        s.step()
+    s.ops.fork_pages(s.pool, _i32([0, 1, 2, 3, -1, -1, -1, -1]))
+    s.pool.check()
+    assert s.pool.tokens.tolist() == [37 + 4] * 4 + [0] * 4
+    s.ids[4:] = -1
+    for shared in (True, False):
+        before = s.kv.clone()
+        got = s.forward(shared).clone()
+        want = s.taught()
+        assert bool(((got[:4].float() - want[:4].float()).abs() <= 2e-2 * want.float().abs().max()).all())
+        own = s.pool.refs > 0
+        assert torch.equal(before[:, ~own], s.kv[:, ~own])
+
+
+def test_rows_without_a_token_have_no_place():
+    """plan_rows of kv_len 0: no page, whatever the table holds, and the row in front is not looked at"""
+    from vox_serve_b200 import ops
+    for page in (1, 16):
+        plan = ops.RowPlan(4, "cuda")
+        table = _i32([7, 3, 5, 2, 9, 9, 9, 9])
+        ops.plan_rows(plan, None, _i32([0, 2, 4, 6, 8]), table, None, 4, 4, page, page, kv_len=_i32([0, 1, 0, 2]))
+        assert plan.row_page[:4].tolist() == [-1, 5, -1, 9] and plan.row_kvlen[:4].tolist() == [0, 1, 0, 2]
+        assert plan.row_slot[:4].tolist() == [0, 0, 0, 1 % page]
+
+
+def test_with_adapters():
+    """rows with adapters of their own read shared pages as others do"""
+    from vox_serve_b200.engine import LlamaAdapters
+    s = Search()
+    s.start()
+    for _ in range(2):
+        s.step()
+    bank = LlamaAdapters(s.weights.dims, 2, 8)
+    g = torch.Generator().manual_seed(1)
+    state = {}
+    for i in range(s.d.num_hidden_layers):
+        for short, module in (("q", "self_attn.q_proj"), ("o", "self_attn.o_proj"), ("down", "mlp.down_proj")):
+            n, k = oorph.synth_weights(s.d, seed=7)[oorph.layer_names(i)[short]].shape
+            state[f"model.layers.{i}.{module}.lora_A.weight"] = (torch.randn(4, k, generator=g) / k ** 0.5).to(BF16)
+            state[f"model.layers.{i}.{module}.lora_B.weight"] = (torch.randn(n, 4, generator=g) * 0.1).to(BF16)
+    bank.load(1, state, 2.0)
+    s.eng.set_adapters(bank)
+    plan = s.ops.LoraPlan(s.rows, 2)
+    s.ops.lora_plan(plan, _i32([1, -1, 1, 0, -1, 1, 1, -1]))
+    logits = []
+    for shared in (True, False):
+        s.ops.plan_rows(s.eng.plan, None, s.pool.indptr, s.pool.table.view(-1), None, s.rows, s.rows, PAGE, s.eng.chunk, kv_len=s.pool.tokens)
+        s.ops.shared_plan(s.plan, s.pool.table, s.pool.tokens, PAGES)
+        logits.append(s.eng.forward(s.ids, s.pool.tokens - 1, s.rows, adapters=plan, shared=s.plan if shared else None).float().clone())
+    assert bool(((logits[0] - logits[1]).abs() <= 2e-2 * logits[1].abs().max()).all())
+    bare = s.forward().float()
+    assert float((bare[0] - logits[0][0]).abs().max()) > float((bare[1] - logits[0][1]).abs().max())      # (the adapter of row 0 is there)

@@ -262,3 +262,53 @@ def test_captured_with_its_plan_and_on_two_streams():
         torch.cuda.synchronize()
         for _, q, kv, table, tokens, out, _ in steps:
             _check(out, q, kv[0], table, tokens)
+
+
+@pytest.mark.parametrize("bad", [NAN, INF])
+def test_what_is_not_finite_where_blocks_walk_on(bad):
+    """more groups and heads than blocks: a block goes on from one to the next, a second time where values are not finite"""
+    B, W, G, H, P, D = 41, 2, 2, 8, 16, 64
+    table, tokens, pages = _tree(B, W, 330, 25, P, seed=17)
+    tokens[10:12] = 0
+    kv, q = _data(pages, P, B * W, G * H, H, D, seed=18)
+    clean = _run(q, kv, 0, table, tokens, W).clone()
+    _check(clean, q, kv[0], table, tokens)
+    on = torch.zeros(pages, P, dtype=torch.bool)
+    for r, n in enumerate(tokens.tolist()):
+        for t in range(n):
+            on[int(table[r, t // P]), t % P] = True
+    dirty = torch.where(on.cuda()[None, :, None, :, None, None], kv, torch.full_like(kv, bad))
+    assert torch.equal(_run(q, dirty, 0, table, tokens, W), clean)
+    own = []
+    for r in (1, 30, 67):                                   # one value of a row's last token, in one head
+        dirty[0, table[r, (int(tokens[r]) - 1) // P].long(), 1, (int(tokens[r]) - 1) % P, r % H, 7] = bad
+        own += [i for i in range(B * W) if int(table[r, (int(tokens[r]) - 1) // P]) in table[i, :-(-int(tokens[i]) // P)].tolist()]
+    out = _run(q, dirty, 0, table, tokens, W)
+    rest = [i for i in range(B * W) if i not in own]
+    assert torch.equal(out[rest], clean[rest])
+    for r in (1, 30, 67):
+        hit = out[r, r % H * G:(r % H + 1) * G]
+        assert not bool(torch.isfinite(hit[:, 7]).any()) and bool(torch.isfinite(out[r].view(H, G, D)[[h for h in range(H) if h != r % H]]).all())
+
+
+@pytest.mark.parametrize("rows,columns", [(8, 300), (3, 1100), (32, 140)])
+def test_rows_that_share_nothing_in_their_columns(rows, columns):
+    """every row its own pages, and pages that stand in several columns, of one row or of several"""
+    P, D = 16, 64
+    g = torch.Generator().manual_seed(rows)
+    table = torch.randperm(rows * columns, generator=g).to(I32).view(rows, columns)
+    table[0, 5:9] = table[0, 3]
+    table[1] = table[0].roll(1)
+    table[2, ::2] = table[1, ::2]
+    table = table.cuda()
+    tokens = torch.randint(columns * P // 2, columns * P + 1, (rows,), generator=g).to(I32).cuda()
+    tokens[0] = columns * P
+    kv, q = _data(rows * columns, P, rows, 2, 1, D, seed=3)
+    _check(_run(q, kv, 0, table, tokens, rows), q, kv[0], table, tokens)
+
+
+def test_output_over_the_queries():
+    table, tokens, pages = _tree(2, 3, 200, 30, 16, seed=9)
+    kv, q = _data(pages, 16, 6, 6, 3, 128, seed=10)
+    want = _run(q, kv, 0, table, tokens, 3).clone()
+    assert torch.equal(_run(q, kv, 0, table, tokens, 3, out=q), want)

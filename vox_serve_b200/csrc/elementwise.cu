@@ -233,8 +233,9 @@ __global__ void __launch_bounds__(1024) plan_rows_kernel(const int32_t* __restri
       row_pagebase[row] = p0;
       row_old[row] = kv_len - n_new;
       row_kvlen[row] = g + 1;
-      row_page[row] = kv_indices[p0 + g / page_size];
-      row_slot[row] = g % page_size;
+      // (a request of no tokens, the row of a search that has left: nothing is appended, nothing attended to)
+      row_page[row] = g >= 0 ? kv_indices[p0 + g / page_size] : -1;
+      row_slot[row] = g >= 0 ? g % page_size : 0;
     }
   }
   if (tid == 0) carry = 0;
