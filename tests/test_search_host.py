@@ -182,7 +182,7 @@ def test_plan_cuts_requests_evenly():
 
     def expect(rows, sub, groups, mpad):
         segments = 1 + groups
-        return 16 * groups * sub + 32 + segments * mpad * (64 * 4 + 8) + 8 * groups + 4 * (3 * groups + 1 + rows)
+        return 16 * groups * sub + 128 + segments * mpad * (64 * 4 + 8) + 8 * groups + 4 * (3 * groups + 1 + rows)
     assert size(9, 16) == expect(9, 5, 2, 80)          # 8 rows would fit: 5 and 4
     assert size(16, 8) == expect(16, 16, 1, 128)
     assert size(17, 8) == expect(17, 9, 2, 80)
@@ -194,7 +194,7 @@ def test_plan_cuts_requests_evenly():
 def test_entry_points_check_by_themselves():
     """the C ABI refuses without a device what it would not survive"""
     lib = _lib.load()
-    assert lib.vb_beam_select_workspace_bytes(2, 3, 8193, 4, 0) == 2 * 3 * 2 * (8 + 32)
+    assert lib.vb_beam_select_workspace_bytes(2, 5, 8193, 4, 0) == 2 * 5 * 2 * (8 + 32) and lib.vb_beam_select_workspace_bytes(2, 4, 8193, 4, 0) == 0
     assert lib.vb_beam_select(None, None, None, None, None, 0, 0, None, None, None, 1, 1, 8, 1, -1, None, 0, None) != 0 and b"null" in lib.vb_last_error()
     buf = ctypes.create_string_buffer(4096)
     at = (ctypes.addressof(buf) + 15) // 16 * 16

@@ -357,7 +357,7 @@ LAUNCHES = {"vb_set_pdl": 0, "vb_set_trace": 0, "vb_weight_tiles_bytes": 0, "vb_
             "vb_short_conv": 2, "vb_selective_scan_tiled": 3, "vb_selective_scan_piece_rows": 0,
             "vb_selective_scan_scratch_floats": 0, "vb_sigmoid_attn": 1, "vb_ssd_tiled": 3, "vb_ssd_tile_rows": 0,
             "vb_ssd_scratch_floats": 0, "vb_lora_plan_bytes": 0, "vb_lora_workspace_bytes": 0, "vb_moe_layer_max_rows": 0,
-            "vb_moe_layer_workspace_bytes": 0, "vb_moe_layer": 2, "vb_beam_select_workspace_bytes": 0, "vb_beam_select": 2, "vb_page_pool_scratch_bytes": 0,
+            "vb_moe_layer_workspace_bytes": 0, "vb_moe_layer": 2, "vb_beam_select_workspace_bytes": 0, "vb_page_pool_scratch_bytes": 0,
             "vb_shared_plan_bytes": 0, "vb_shared_plan": 2, "vb_shared_attn": 2}
 launch_counter = [0]
 

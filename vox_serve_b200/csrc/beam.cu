@@ -17,6 +17,8 @@ constexpr int BS_THREADS = 256, BS_VECS = 4, BS_STAGES = 2;     // a chunk: four
 constexpr int BS_CAP = 1024;                                   // candidates that a block keeps
 constexpr int BS_BLOCKS = 4;                                    // blocks an SM holds
 constexpr int BS_MAX_N = 64, BS_MAX_W = 32;
+constexpr int BS_CLUSTER = 8;                                   // blocks of a request that join in the same launch
+static_assert(BS_CLUSTER * BS_MAX_N * 16 <= 16384, "the join's candidates stand where the ring stood");
 constexpr int BJ_BINS = 1024;                                   // 16 to a doubling, from 2^-23 to 2^41
 constexpr int BJ_THREADS = 512, BJ_ALL = 8192;                  // candidates of a request: 128 KB of ranks and values
 
@@ -361,59 +363,88 @@ __device__ __forceinline__ void beam_part(PartShared& sh, BeamStats* stats, uint
   if (tid < n) best[tid] = tid < c ? list[tid] : 0ull;
 }
 
+// the same place in the shared memory of the cluster's first block, as an ordinary address
 template <typename T>
-__global__ void __launch_bounds__(BS_THREADS, BS_BLOCKS) beam_part_kernel(BeamStats* __restrict__ stats, uint64_t* __restrict__ best, const T* __restrict__ logits,
-                                                                          long long stride, int V, int parts, const float* score, const float* weight,
-                                                                          const uint8_t* ended, int n) {
-  extern __shared__ __align__(16) uint8_t bs_raw[];
-  PartShared& sh = *reinterpret_cast<PartShared*>(bs_raw);
-  const int row = blockIdx.x / parts, part = blockIdx.x - row * parts;
+__device__ __forceinline__ T* in_first_block(T* at) {
+  T* r;
+  asm("mapa.u64 %0, %1, 0;" : "=l"(r) : "l"(at));
+  return r;
+}
+
+struct BeamCall {
+  BeamStats* stats;              // [rows * parts]
+  uint64_t* best;                // [rows * parts][n]
+  const void* logits;
+  long long stride;
+  const float *score, *weight;
+  const uint8_t* ended;
+  float* out_score;
+  int32_t* out_parent;
+  int64_t* out_token;
+  uint8_t* out_ended;
+  int V, parts, W, n;
+  long long end_token;
+};
+
+template <typename T>
+__device__ __forceinline__ void beam_one_part(PartShared& sh, const BeamCall& p, BeamStats* st, uint64_t* out) {      // (where its statistics and its best go)
+  const int row = blockIdx.x / p.parts, part = blockIdx.x - row * p.parts;
   if (threadIdx.x == 0) sh.box[0] = sh.box[1] = sh.box[2] = sh.count = 0u;
   pdl_sync();
-  if (!beam_reads(score, weight, ended, row)) return;       // (the second kernel does not look at this row either)
+  if (!beam_reads(p.score, p.weight, p.ended, row)) return;       // (the join does not look at this row either)
   __syncthreads();
-  const uint8_t* at = reinterpret_cast<const uint8_t*>(logits + static_cast<long long>(row) * stride);
+  const uint8_t* at = static_cast<const uint8_t*>(p.logits) + static_cast<long long>(row) * p.stride * static_cast<long long>(sizeof(T));
   const int by = static_cast<int>(reinterpret_cast<uintptr_t>(at) & 15);
-  BeamStats* st = stats + blockIdx.x;
-  uint64_t* out = best + static_cast<long long>(blockIdx.x) * n;
-  if (by == 0) beam_part<T, 16>(sh, st, out, at, V, part, parts, n);
-  else if (by == 8) beam_part<T, 8>(sh, st, out, at, V, part, parts, n);
-  else if (sizeof(T) == 4 || by % 4 == 0) beam_part<T, 4>(sh, st, out, at, V, part, parts, n);
-  else beam_part<T, sizeof(T)>(sh, st, out, at, V, part, parts, n);
+  if (by == 0) beam_part<T, 16>(sh, st, out, at, p.V, part, p.parts, p.n);
+  else if (by == 8) beam_part<T, 8>(sh, st, out, at, p.V, part, p.parts, p.n);
+  else if (sizeof(T) == 4 || by % 4 == 0) beam_part<T, 4>(sh, st, out, at, p.V, part, p.parts, p.n);
+  else beam_part<T, sizeof(T)>(sh, st, out, at, p.V, part, p.parts, p.n);
+}
+
+template <typename T>
+__global__ void __launch_bounds__(BS_THREADS, BS_BLOCKS) beam_part_kernel(const __grid_constant__ BeamCall p) {
+  extern __shared__ __align__(16) uint8_t bs_raw[];
+  beam_one_part<T>(*reinterpret_cast<PartShared*>(bs_raw), p, p.stats + blockIdx.x, p.best + static_cast<long long>(blockIdx.x) * p.n);
 }
 
 // The n best of one request.  Candidate c of its W * parts * n: beam, part, place; its rank stands in shared memory (in registers, unrolled, the code took longer
 // to arrive than to run).
-__global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(float* __restrict__ out_score, int32_t* __restrict__ out_parent, int64_t* __restrict__ out_token,
-                                                               uint8_t* __restrict__ out_ended, const BeamStats* __restrict__ stats,
-                                                               const uint64_t* __restrict__ best, const float* score, const float* weight,
-                                                               const uint8_t* ended, int W, int parts, int n, long long end_token) {
-  constexpr int CAP = BS_MAX_N + 32;
-  extern __shared__ uint64_t bj_key[];                 // [W * parts * n] ranks as ordered numbers, 0: none; behind them the candidates
+template <int THREADS>
+struct JoinShared {
+  static constexpr int CAP = BS_MAX_N + 32;
   // total = (x - top) + base: a row may hold nothing but lowest values; base of an ended beam: its score
-  __shared__ double base[BS_MAX_W], tops[BS_MAX_W];
-  __shared__ uint8_t kind[BS_MAX_W];                   // 0: no candidates, 1: logits, 2: ended
-  __shared__ uint64_t list_key[CAP], list_at[CAP], warp_most[BJ_THREADS / 32];      // rank, (beam, token)
-  __shared__ double list_total[CAP];
-  __shared__ uint32_t box[3], count;
-  __shared__ int bins[BJ_BINS], warp_sum_s[BJ_THREADS / 32], box_bin, box_upto;
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, b = blockIdx.x;
+  double base[BS_MAX_W], tops[BS_MAX_W];
+  uint64_t list_key[CAP], list_at[CAP], warp_most[THREADS / 32];      // rank, (beam, token)
+  double list_total[CAP];
+  uint32_t box[3], count;
+  int bins[BJ_BINS], warp_sum_s[THREADS / 32], box_bin, box_upto;
+  uint8_t kind[BS_MAX_W];                              // 0: no candidates, 1: logits, 2: ended
+};
+template <int THREADS>
+__device__ __forceinline__ void beam_join(JoinShared<THREADS>& sh, uint64_t* bj_key, const BeamCall& p, int b, const BeamStats* stats, const uint64_t* mine_of) {      // (of the request)
+  double *base = sh.base, *tops = sh.tops, *list_total = sh.list_total;
+  uint64_t *list_key = sh.list_key, *list_at = sh.list_at, *warp_most = sh.warp_most;
+  uint32_t *box = sh.box, &count = sh.count;
+  int *bins = sh.bins, *warp_sum_s = sh.warp_sum_s, &box_bin = sh.box_bin, &box_upto = sh.box_upto;
+  uint8_t* kind = sh.kind;
+  const float *score = p.score, *weight = p.weight;
+  const uint8_t* ended = p.ended;
+  const int W = p.W, parts = p.parts, n = p.n;
+  const long long end_token = p.end_token;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int per_row = parts * n, all = W * per_row;
   uint64_t* bj_e = bj_key + all;
-  const uint64_t* mine_of = best + static_cast<long long>(b) * all;
-  if (tid == 0) box[0] = box[1] = box[2] = count = 0u;
-  pdl_sync();
   auto total_of = [&](int w, uint64_t e) { return kind[w] == 2 ? base[w] : (static_cast<double>(unorder_f32(static_cast<uint32_t>(e >> 32))) - tops[w]) + base[w]; };
   auto place_of = [&](int w, uint64_t e) {
     return static_cast<uint64_t>(w) << 32 | (kind[w] == 2 ? static_cast<uint32_t>(end_token) : 0xffffffffu - static_cast<uint32_t>(e));
   };
   uint64_t most = 0ull;
   int mine = 0;
-  for (int w = warp; w < W; w += BJ_THREADS / 32) {    // a warp a beam
+  for (int w = warp; w < W; w += THREADS / 32) {    // a warp a beam
     const int row = b * W + w;
     const float s = score[row], f = weight ? weight[row] : 1.f;
     const bool over = ended && ended[row];
-    const BeamStats t0 = lane < parts ? stats[row * parts + lane] : BeamStats{-INFINITY, 0.f};      // (of a row that was not read: anything)
+    const BeamStats t0 = lane < parts ? stats[w * parts + lane] : BeamStats{-INFINITY, 0.f};      // (of a row that was not read: anything)
     int k = !isfinite(s) || !isfinite(f) || !(f > 0.f) ? 0 : over ? 2 : 1;
     uint64_t e[4] = {0ull, 0ull, 0ull, 0ull};          // (the first of its candidates, on their way meanwhile)
 #pragma unroll
@@ -422,11 +453,11 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(float* __restrict
     double log_sum = 0.0, peak = 0.0;
     if (k == 1) {
       float top = t0.m;
-      for (int i = lane + 32; i < parts; i += 32) top = fmaxf(top, stats[row * parts + i].m);
+      for (int i = lane + 32; i < parts; i += 32) top = fmaxf(top, stats[w * parts + i].m);
       top = warp_max(top);
       double sum = t0.m == -INFINITY ? 0.0 : static_cast<double>(t0.s) * exp(static_cast<double>(t0.m) - static_cast<double>(top));
       for (int i = lane + 32; i < parts; i += 32) {
-        const BeamStats t = stats[row * parts + i];
+        const BeamStats t = stats[w * parts + i];
         if (t.m != -INFINITY) sum += static_cast<double>(t.s) * exp(static_cast<double>(t.m) - static_cast<double>(top));
       }
 #pragma unroll
@@ -456,23 +487,26 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(float* __restrict
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, o));
     if (lane == 0) warp_most[warp] = most;
-    for (int i = tid; i < BJ_BINS; i += BJ_THREADS) bins[i] = 0;
+    for (int i = tid; i < BJ_BINS; i += THREADS) bins[i] = 0;
     __syncthreads();
     uint64_t top = 0ull;
 #pragma unroll
-    for (int i = 0; i < BJ_THREADS / 32; ++i) top = max(top, warp_most[i]);
+    for (int i = 0; i < THREADS / 32; ++i) top = max(top, warp_most[i]);
     const double best_rank = unorder_f64(top);
     auto bin_of = [&](uint64_t key) {                       // (monotone: the same subtraction and conversion for all)
       const int i = static_cast<int>(__float_as_uint(static_cast<float>(best_rank - unorder_f64(key))) >> 19) - (104 << 4);
       return i < 0 ? 0 : i < BJ_BINS ? i : BJ_BINS - 1;
     };
 #pragma unroll 2
-    for (int c = tid; c < all; c += BJ_THREADS)
+    for (int c = tid; c < all; c += THREADS)
       if (bj_key[c]) atomicAdd(&bins[bin_of(bj_key[c])], 1);
     __syncthreads();
-    // the bin in which the n-th is: two bins a thread
-    const int b0 = bins[2 * tid], b1 = bins[2 * tid + 1];
-    int upto = b0 + b1;
+    // the bin in which the n-th is
+    constexpr int OWN = BJ_BINS / THREADS;
+    int upto = 0;
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) upto += bins[OWN * tid + i];
+    const int own = upto;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -481,11 +515,12 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(float* __restrict
     if (lane == 31) warp_sum_s[warp] = upto;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < BJ_THREADS / 32; ++i)
+    for (int i = 0; i < THREADS / 32; ++i)
       if (i < warp) upto += warp_sum_s[i];
-    if (upto >= n && upto - b0 - b1 < n) {                  // (one thread)
-      const bool second = upto - b1 < n;
-      box_bin = 2 * tid + second, box_upto = second ? upto : upto - b1;
+    if (upto >= n && upto - own < n) {                      // (one thread)
+      int bin = OWN * tid, sum = upto - own + bins[bin];
+      while (sum < n) sum += bins[++bin];
+      box_bin = bin, box_upto = sum;
     }
     __syncthreads();
     const int last = box_bin;
@@ -494,7 +529,7 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(float* __restrict
       // the lowest rank of the bins that count: what is below stays out
       uint64_t least = ~0ull;
 #pragma unroll 2
-      for (int c = tid; c < all; c += BJ_THREADS)
+      for (int c = tid; c < all; c += THREADS)
         if (bj_key[c] && bin_of(bj_key[c]) <= last) least = min(least, bj_key[c]);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) least = min(least, __shfl_xor_sync(0xffffffffu, least, o));
@@ -502,12 +537,12 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(float* __restrict
       __syncthreads();
       cut = ~0ull;
 #pragma unroll
-      for (int i = 0; i < BJ_THREADS / 32; ++i) cut = min(cut, warp_most[i]);
+      for (int i = 0; i < THREADS / 32; ++i) cut = min(cut, warp_most[i]);
     }
     auto count_from = [&](uint64_t from) {
       int m = 0;
 #pragma unroll 4
-      for (int c = tid; c < all; c += BJ_THREADS) m += bj_key[c] >= from;
+      for (int c = tid; c < all; c += THREADS) m += bj_key[c] >= from;
       return block_count(m, box, turn);
     };
     uint64_t lo = cut, hi = top + 1ull;
@@ -523,14 +558,14 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(float* __restrict
       const uint64_t mid = below + ((tie - below) >> 1);
       mine = 0;
 #pragma unroll 1
-      for (int c = tid; c < all; c += BJ_THREADS) mine += bj_key[c] > cut || (bj_key[c] == cut && place_of(c / per_row, bj_e[c]) <= mid);
+      for (int c = tid; c < all; c += THREADS) mine += bj_key[c] > cut || (bj_key[c] == cut && place_of(c / per_row, bj_e[c]) <= mid);
       const int c = block_count(mine, box, turn);
       if (c >= n) tie = mid, found = c;
       else below = mid + 1ull;
     }
   }
 #pragma unroll 1
-  for (int c = tid; c < all; c += BJ_THREADS) {
+  for (int c = tid; c < all; c += THREADS) {
     const uint64_t key = bj_key[c];
     if (key < cut) continue;
     const int w = c / per_row;
@@ -541,7 +576,7 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(float* __restrict
   }
   __syncthreads();
   const uint32_t quad = 0xfu << (lane & 28);
-  for (int i = tid >> 2; i < found; i += BJ_THREADS / 4) {
+  for (int i = tid >> 2; i < found; i += THREADS / 4) {
     const uint64_t k = list_key[i], at = list_at[i];
     int rank = 0;
 #pragma unroll 4
@@ -554,18 +589,43 @@ __global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(float* __restrict
     if ((tid & 3) == 0 && rank < n) {
       const int w = static_cast<int>(at >> 32), o = b * n + rank;
       const uint32_t v = static_cast<uint32_t>(at);
-      out_score[o] = static_cast<float>(list_total[i]);
-      out_parent[o] = w;
-      out_token[o] = v;
-      if (out_ended) out_ended[o] = kind[w] == 2 || static_cast<long long>(v) == end_token;
+      p.out_score[o] = static_cast<float>(list_total[i]);
+      p.out_parent[o] = w;
+      p.out_token[o] = v;
+      if (p.out_ended) p.out_ended[o] = kind[w] == 2 || static_cast<long long>(v) == end_token;
     }
   }
-  for (int i = found + tid; i < n; i += BJ_THREADS) {
-    out_score[b * n + i] = -INFINITY;
-    out_parent[b * n + i] = -1;
-    out_token[b * n + i] = -1;
-    if (out_ended) out_ended[b * n + i] = 1;
+  for (int i = found + tid; i < n; i += THREADS) {
+    p.out_score[b * n + i] = -INFINITY;
+    p.out_parent[b * n + i] = -1;
+    p.out_token[b * n + i] = -1;
+    if (p.out_ended) p.out_ended[b * n + i] = 1;
   }
+}
+
+__global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_constant__ BeamCall p) {
+  extern __shared__ uint64_t bj_key[];                 // [W * parts * n] ranks as ordered numbers, 0: none; behind them the candidates
+  __shared__ JoinShared<BJ_THREADS> sh;
+  if (threadIdx.x == 0) sh.box[0] = sh.box[1] = sh.box[2] = sh.count = 0u;
+  pdl_sync();
+  const long long first = static_cast<long long>(blockIdx.x) * p.W * p.parts;
+  beam_join<BJ_THREADS>(sh, bj_key, p, blockIdx.x, p.stats + first, p.best + first * p.n);
+}
+
+// Both in one launch where a request's parts are few: a cluster a request, whose blocks leave what they found in the first one's shared memory.  (One beam of two
+// over 2051 tokens: 6.45 -> 5.9 us in a graph, the call 16.1 -> 13.6.)
+template <typename T>
+__global__ void __launch_bounds__(BS_THREADS) beam_small_kernel(const __grid_constant__ BeamCall p) {
+  extern __shared__ __align__(16) uint8_t bs_raw[];
+  __shared__ JoinShared<BS_THREADS> sh;
+  __shared__ BeamStats stats[BS_CLUSTER];
+  __shared__ uint64_t best[BS_CLUSTER * BS_MAX_N];
+  if (threadIdx.x == 0) sh.box[0] = sh.box[1] = sh.box[2] = sh.count = 0u;
+  cluster_sync_all();                                  // (the first block runs)
+  const int rank = cluster_ctarank();
+  beam_one_part<T>(*reinterpret_cast<PartShared*>(bs_raw), p, in_first_block(stats + rank), in_first_block(best + rank * p.n));
+  cluster_sync_all();
+  if (rank == 0) beam_join<BS_THREADS>(sh, reinterpret_cast<uint64_t*>(bs_raw), p, blockIdx.x / (p.W * p.parts), stats, best);
 }
 
 // ---- states that follow their beams ----------------------------------------------------------------------------------------------
@@ -646,13 +706,14 @@ using namespace vb;
 
 extern "C" size_t vb_beam_select_workspace_bytes(int requests, int width, int vocab, int n, int logits_f32) {
   if (requests <= 0 || width <= 0 || width > BS_MAX_W || vocab <= 0 || n <= 0 || n > BS_MAX_N) return 0;
-  return static_cast<size_t>(requests) * width * beam_parts(requests, width, vocab, n, logits_f32 ? 4 : 2) * (sizeof(BeamStats) + 8ull * n);
+  const int parts = beam_parts(requests, width, vocab, n, logits_f32 ? 4 : 2);
+  return width * parts <= BS_CLUSTER ? 0 : static_cast<size_t>(requests) * width * parts * (sizeof(BeamStats) + 8ull * n);
 }
 
 extern "C" int vb_beam_select(float* d_score, int32_t* d_parent, int64_t* d_token, uint8_t* d_out_ended, const void* d_logits, int64_t row_stride, int logits_f32,
                               const float* d_beam_score, const float* d_weight, const uint8_t* d_ended, int requests, int width, int vocab, int n, int64_t end_token,
                               void* d_workspace, size_t workspace_bytes, void* stream) {
-  VB_CHECK_ARG(d_score && d_parent && d_token && d_logits && d_beam_score && d_workspace, "vb_beam_select: null pointer");
+  VB_CHECK_ARG(d_score && d_parent && d_token && d_logits && d_beam_score, "vb_beam_select: null pointer");
   VB_CHECK_ARG(requests > 0 && width > 0 && width <= BS_MAX_W && n > 0 && n <= BS_MAX_N, "vb_beam_select: %d requests of %d beams (1 to %d), the best %d (1 to %d)", requests,
                width, BS_MAX_W, n, BS_MAX_N);
   VB_CHECK_ARG(vocab > 0 && vocab <= (1 << 24), "vb_beam_select: vocabulary of %d (1 to 2^24)", vocab);
@@ -663,20 +724,24 @@ extern "C" int vb_beam_select(float* d_score, int32_t* d_parent, int64_t* d_toke
   const int parts = beam_parts(requests, width, vocab, n, logits_f32 ? 4 : 2);
   const long long blocks = static_cast<long long>(requests) * width * parts;
   VB_CHECK_ARG(blocks <= 0x7fffffffll && static_cast<long long>(requests) * n <= 0x7fffffffll, "vb_beam_select: %lld parts of rows", blocks);
-  VB_CHECK_ARG(workspace_bytes >= vb_beam_select_workspace_bytes(requests, width, vocab, n, logits_f32) && reinterpret_cast<uintptr_t>(d_workspace) % 8 == 0,
-               "vb_beam_select: workspace of %zu bytes", workspace_bytes);
+  const size_t need = vb_beam_select_workspace_bytes(requests, width, vocab, n, logits_f32);
+  VB_CHECK_ARG(need == 0 || (d_workspace && workspace_bytes >= need && reinterpret_cast<uintptr_t>(d_workspace) % 8 == 0), "vb_beam_select: workspace of %zu bytes, not %zu",
+               workspace_bytes, need);
   uint64_t* best = static_cast<uint64_t*>(d_workspace);
-  BeamStats* stats = reinterpret_cast<BeamStats*>(best + blocks * n);
+  BeamStats* stats = need ? reinterpret_cast<BeamStats*>(best + blocks * n) : nullptr;
+  BeamCall p = {stats, best, d_logits, static_cast<long long>(row_stride), d_beam_score, d_weight, d_ended, d_score, d_parent, d_token, d_out_ended,
+                vocab, parts, width, n, static_cast<long long>(end_token)};
+  if (width * parts <= BS_CLUSTER) {
+    VB_CHECK_CUDA(logits_f32 ? rm_smem<beam_small_kernel<float>>(sizeof(PartShared)) : rm_smem<beam_small_kernel<__nv_bfloat16>>(sizeof(PartShared)));
+    if (logits_f32) VB_LAUNCH_PDL_CLUSTER(beam_small_kernel<float>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, width * parts, p);
+    else VB_LAUNCH_PDL_CLUSTER(beam_small_kernel<__nv_bfloat16>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, width * parts, p);
+    return 0;
+  }
   VB_CHECK_CUDA(logits_f32 ? rm_smem<beam_part_kernel<float>>(sizeof(PartShared)) : rm_smem<beam_part_kernel<__nv_bfloat16>>(sizeof(PartShared)));
-  if (logits_f32)
-    VB_LAUNCH_PDL(beam_part_kernel<float>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, stats, best, static_cast<const float*>(d_logits),
-                  static_cast<long long>(row_stride), vocab, parts, d_beam_score, d_weight, d_ended, n);
-  else
-    VB_LAUNCH_PDL(beam_part_kernel<__nv_bfloat16>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, stats, best, static_cast<const __nv_bfloat16*>(d_logits),
-                  static_cast<long long>(row_stride), vocab, parts, d_beam_score, d_weight, d_ended, n);
+  if (logits_f32) VB_LAUNCH_PDL(beam_part_kernel<float>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, p);
+  else VB_LAUNCH_PDL(beam_part_kernel<__nv_bfloat16>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, p);
   VB_CHECK_CUDA(rm_smem<beam_join_kernel>(BJ_ALL * 16));
-  VB_LAUNCH_PDL(beam_join_kernel, static_cast<unsigned>(requests), BJ_THREADS, static_cast<size_t>(width) * parts * n * 16, stream, d_score, d_parent, d_token, d_out_ended, stats, best, d_beam_score, d_weight,
-                d_ended, width, parts, n, static_cast<long long>(end_token));
+  VB_LAUNCH_PDL(beam_join_kernel, static_cast<unsigned>(requests), BJ_THREADS, static_cast<size_t>(width) * parts * n * 16, stream, p);
   return 0;
 }
 

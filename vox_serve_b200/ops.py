@@ -2273,11 +2273,12 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, weight: Opti
     (B, W), (R, V), f32, on = s, z, dtype is F32, logits.device
     step = BeamStep(torch.empty(B, n, dtype=F32, device=on), torch.empty(B, n, dtype=torch.int32, device=on), torch.empty(B, n, dtype=torch.int64, device=on),
                     None if end_token is None else torch.empty(B, n, dtype=torch.bool, device=on))
-    # (of the allocator's, so that calls on other streams and captured graphs have their own)
-    n_ws = _beam_ws(B, W, V, n, f32)
-    ws = torch.empty(n_ws // 8, dtype=torch.int64, device=on)
+    n_ws, ws = _beam_ws(B, W, V, n, f32), None
+    if n_ws:                                           # (of the allocator's, so that calls on other streams and captured graphs have their own)
+        ws = torch.empty(n_ws // 8, dtype=torch.int64, device=on)
+        _lib.launch_counter[0] += 1
     call("vb_beam_select", step.scores.data_ptr(), step.parent.data_ptr(), step.token.data_ptr(), None if end_token is None else step.ended.data_ptr(), logits.data_ptr(),
-         logits.stride(0) if R > 1 else V, f32, scores.data_ptr(), _p(weight), _p(ended), B, W, V, n, -1 if end_token is None else end_token, ws.data_ptr(), n_ws, _raw_stream(dev))
+         logits.stride(0) if R > 1 else V, f32, scores.data_ptr(), _p(weight), _p(ended), B, W, V, n, -1 if end_token is None else end_token, ws.data_ptr() if n_ws else None, n_ws, _raw_stream(dev))
     return step
 
 
