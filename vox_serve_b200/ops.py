@@ -9,6 +9,7 @@ from __future__ import annotations
 import ctypes
 import math
 import os
+from array import array
 from functools import lru_cache
 from typing import Dict, NamedTuple, Optional, Sequence, Tuple, Union
 
@@ -2314,7 +2315,8 @@ def beam_reorder(states: Sequence[torch.Tensor], parent: torch.Tensor, slots: Op
         _beam_reorder_check(states, parent, slots)
     if not k:
         return states
-    call("vb_beam_reorder", (ctypes.c_void_p * k)(*ptrs), (ctypes.c_int64 * k)(*sizes), k, rows, parent.data_ptr(), _p(slots), by[0], by[1], _raw_stream(dev))
+    ptrs, sizes = array("Q", ptrs), array("q", sizes)
+    call("vb_beam_reorder", ptrs.buffer_info()[0], sizes.buffer_info()[0], k, rows, parent.data_ptr(), _p(slots), by[0], by[1], _raw_stream(dev))
     if k > 64:
         _lib.launch_counter[0] += (k - 1) // 64
     return states
