@@ -6,7 +6,7 @@
 // once, with the set of rows that hold it, instead of once for every row.  A group's rows times the query heads of a key head, up to 128, are the accumulator
 // rows of the tcgen05 core (attn_tc.cuh): a tile of 64 keys meets all of them while it is on chip.
 //
-//   plan (once a step)   a cluster a group lists its different pages in pieces of 16 to 64 tokens {place in the cache, position, rows, tokens}: first the tiles
+//   plan (once a step)   a cluster a group lists its different pages in pieces of 16 tokens {place in the cache, position, rows, tokens}: first the tiles
 //                        that all living rows see whole, then the rest; the tiles of every group and key head are cut into equal segments, as many as there are
 //                        blocks (two an SM); where there are more groups and heads than blocks, a block gets an equal stretch of all of them
 //   attention            a block walks its segments: maximum, denominator and unnormalised output of each one's rows
@@ -29,7 +29,9 @@ template <int D>
 constexpr int SA_OUT = PtcLayout<D>::BAR + 768;
 template <int D>
 constexpr int SA_SMEM = SA_OUT<D> + 128 * 64 + 1024;
-inline int sa_piece(int page_size) { return page_size % 64 == 0 ? 64 : page_size % 32 == 0 ? 32 : 16; }
+// Pages are listed in pieces of 16 tokens, four to a tile.  Pieces of a tile that are neighbours in a page come with one copy of as many rows: one of 64 for most
+// tiles of pages of 64 and more.
+constexpr int SA_PIECE = 16, SA_TILE_PIECES = PTC_KT / SA_PIECE;
 
 // ---- the plan -------------------------------------------------------------------------------------------------------------------
 constexpr int SD_PART = 8;       // words of 16 bytes, a line: a block knows what to fetch first with one load
@@ -40,7 +42,7 @@ struct SharedPlanParams {
   int32_t* tile0;                // [groups + 1] tiles in front of a group
   int2* blocks_of;               // [units] first and last block of a unit
   const int32_t *table, *tokens;
-  int rows, width, sub, subs, groups, cap, columns, pages, page_size, piece, tile_pieces, heads, grid;
+  int rows, width, sub, subs, groups, cap, columns, pages, page_size, heads, grid;
 };
 
 constexpr int SP_THREADS = 512, SP_WARPS = SP_THREADS / 32, SP_CHUNK = 128, SP_MAX_COLUMNS = 16384, SP_CLUSTER = 8;
@@ -89,8 +91,8 @@ __device__ __forceinline__ SharedColumn shared_column(const SharedPlanParams& p,
   }
   const bool leads = c.page >= 0 && static_cast<int>(threadIdx.x & 31) == __ffs(c.same) - 1;
   c.tokens = most = min(most, p.page_size);
-  c.pieces = leads ? (most + p.piece - 1) / p.piece : 0;
-  c.whole = leads && (c.same & alive) == alive ? min(least, p.page_size) / p.piece : 0;
+  c.pieces = leads ? (most + SA_PIECE - 1) / SA_PIECE : 0;
+  c.whole = leads && (c.same & alive) == alive ? min(least, p.page_size) / SA_PIECE : 0;
   return c;
 }
 
@@ -129,7 +131,7 @@ __global__ void __launch_bounds__(SP_THREADS) shared_list_kernel(const __grid_co
   }
   const uint32_t alive = __ballot_sync(0xffffffffu, len > 0);
   const int longest = __reduce_max_sync(0xffffffffu, len), shortest = __reduce_min_sync(0xffffffffu, len > 0 ? len : 0x7fffffff);
-  const int columns = (longest + p.page_size - 1) / p.page_size, per_page = p.page_size / p.piece;
+  const int columns = (longest + p.page_size - 1) / p.page_size, per_page = p.page_size / SA_PIECE;
   const int here = (columns + blocks * SP_CHUNK - 1) / (blocks * SP_CHUNK) * SP_CHUNK;      // (with places behind the last column)
   int *first_w = sp_smem, *first_o = first_w + here, *one = first_o + here, *parted = one + here;
   for (int c0 = 0; c0 < here; c0 += SP_CHUNK) {
@@ -182,7 +184,7 @@ __global__ void __launch_bounds__(SP_THREADS) shared_list_kernel(const __grid_co
       all_w += w, all_o += o;
     }
   }
-  const int tiles_w = all_w / p.tile_pieces;            // (what is left of the whole ones fills the first of the others)
+  const int tiles_w = all_w / SA_TILE_PIECES;            // (what is left of the whole ones fills the first of the others)
   if (rank == 0 && tid == 0) p.counts[g] = all_w + all_o, p.whole[g] = tiles_w;
   int4* out = p.entries + static_cast<long long>(g) * p.cap;
 #pragma unroll 1
@@ -198,15 +200,15 @@ __global__ void __launch_bounds__(SP_THREADS) shared_list_kernel(const __grid_co
     int at_w = w0 + first_w[at] + inc_w - c.whole, at_o = all_w + o0 + first_o[at] + inc_o - (c.pieces - c.whole);
 #pragma unroll 1
     for (int i = 0; i < c.pieces; ++i) {
-      const int off = i * p.piece;
-      out[i < c.whole ? at_w++ : at_o++] = make_int4(c.page * p.page_size + off, col * p.page_size + off, static_cast<int>(c.same), min(p.piece, c.tokens - off));
+      const int off = i * SA_PIECE;
+      out[i < c.whole ? at_w++ : at_o++] = make_int4(c.page * p.page_size + off, col * p.page_size + off, static_cast<int>(c.same), min(SA_PIECE, c.tokens - off));
     }
   }
 #pragma unroll 1
   for (int i = at_c; i < here; i += SP_CHUNK)
     if (one[i] >= 0)
       for (int k = at_r; k < per_page; k += ACROSS)
-        out[w0 + first_w[i] + k] = make_int4(one[i] * p.page_size + k * p.piece, column(i) * p.page_size + k * p.piece, static_cast<int>(alive), p.piece);
+        out[w0 + first_w[i] + k] = make_int4(one[i] * p.page_size + k * SA_PIECE, column(i) * p.page_size + k * SA_PIECE, static_cast<int>(alive), SA_PIECE);
   if (blocks > 1) cluster_sync_all();                   // (totals have been read)
 }
 
@@ -218,17 +220,17 @@ __global__ void __launch_bounds__(SD_THREADS) shared_deal_kernel(const __grid_co
   const int units = p.groups * p.heads;
   auto write_part = [&](int i, const int4& part, const int4& of) {
     int4 *to = p.parts + i * SD_PART, e[4];
-    const int first = part.z * p.tile_pieces;
+    const int first = part.z * SA_TILE_PIECES;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
-      e[k] = k < p.tile_pieces && part.w > 0 && first + k < of.x ? __ldcg(p.entries + static_cast<long long>(part.x) * p.cap + first + k) : make_int4(0, 0, 0, 0);
+      e[k] = k < SA_TILE_PIECES && part.w > 0 && first + k < of.x ? __ldcg(p.entries + static_cast<long long>(part.x) * p.cap + first + k) : make_int4(0, 0, 0, 0);
     to[0] = part, to[1] = of;
 #pragma unroll
     for (int k = 0; k < 4; ++k) to[2 + k] = e[k];
   };
   int total = 0;
   for (int g0 = 0; g0 < p.groups; g0 += SD_THREADS) {
-    const int g = g0 + tid, mine = g < p.groups ? (__ldcg(p.counts + g) + p.tile_pieces - 1) / p.tile_pieces : 0;
+    const int g = g0 + tid, mine = g < p.groups ? (__ldcg(p.counts + g) + SA_TILE_PIECES - 1) / SA_TILE_PIECES : 0;
     int all;
     const int before = sp_prefix<SD_WARPS>(mine, sums, all);
     if (units <= p.grid) {
@@ -331,7 +333,7 @@ struct SharedAttnParams {
   float2* stat;                  // [blocks + units][mpad] maximum (base 2), denominator against it
   long long slab_base, slabs;
   unsigned char* wait_flag;
-  int rows, width, sub, subs, groups, cap, page_size, piece, tile_pieces, n_q, heads, G, mpad, xt_tile;
+  int rows, width, sub, subs, groups, cap, page_size, n_q, heads, G, mpad, xt_tile;
   float scale_log2;
 };
 
@@ -347,7 +349,7 @@ struct SharedWalk {
   int g, h, t, left;             // group, key head, first tile; tiles of the stretch from here on
   int count, whole, tiles;       // of the group
   __device__ __forceinline__ SharedWalk(const SharedAttnParams& p_, const int4& part, const int4& of)
-      : p(p_), g(part.x), h(part.y), t(part.z), left(part.w), count(of.x), whole(of.y), tiles((of.x + p_.tile_pieces - 1) / p_.tile_pieces) {}
+      : p(p_), g(part.x), h(part.y), t(part.z), left(part.w), count(of.x), whole(of.y), tiles((of.x + SA_TILE_PIECES - 1) / SA_TILE_PIECES) {}
   __device__ __forceinline__ int here() const { return min(left, tiles - t); }      // tiles of the segment
   __device__ __forceinline__ void step(int n) {                                     // n tiles on, within the segment
     t += n, left -= n;
@@ -359,17 +361,19 @@ struct SharedWalk {
       ++g;
       count = p.counts[g];
     } while (count == 0);        // (tiles are left, so there is one)
-    whole = p.whole[g], tiles = (count + p.tile_pieces - 1) / p.tile_pieces;
+    whole = p.whole[g], tiles = (count + SA_TILE_PIECES - 1) / SA_TILE_PIECES;
   }
 };
 
 // Tokens of a tile that a row sees: it holds the page, and the token is not behind its last
-__device__ __forceinline__ uint64_t shared_mask(const int4* pieces, int n_pieces, int piece, int bit, int len) {
+__device__ __forceinline__ uint64_t shared_mask(const int4* pieces, int n_pieces, int bit, int len) {
   uint64_t m = 0ull;
-  for (int i = 0; i < n_pieces; ++i) {
+#pragma unroll
+  for (int i = 0; i < SA_TILE_PIECES; ++i) {
+    if (i >= n_pieces) break;
     const int4 e = pieces[i];
     const int n = (static_cast<uint32_t>(e.z) >> bit & 1u) ? min(len - e.y, e.w) : 0;
-    if (n > 0) m |= (n < 64 ? (1ull << n) - 1ull : ~0ull) << (i * piece);
+    if (n > 0) m |= ((1ull << n) - 1ull) << (i * SA_PIECE);
   }
   return m;
 }
@@ -378,11 +382,11 @@ __device__ __forceinline__ uint64_t shared_mask(const int4* pieces, int n_pieces
 template <int D>
 __device__ __noinline__ void shared_give_back(const SharedAttnParams& p, const int4* entries, int count, int from, int to, int head, int bit, int len, int c0, float* v) {
   for (int t = from; t < to; ++t) {
-    const int first = t * p.tile_pieces;
-    const uint64_t m = shared_mask(entries + first, min(p.tile_pieces, count - first), p.piece, bit, len);
+    const int first = t * SA_TILE_PIECES;
+    const uint64_t m = shared_mask(entries + first, min(SA_TILE_PIECES, count - first), bit, len);
     for (int k = 0; k < PTC_KT; ++k) {
       if (!(m >> k & 1ull)) continue;
-      const int tok = entries[first + k / p.piece].x + k % p.piece, page = tok / p.page_size, slot = tok - page * p.page_size;
+      const int tok = entries[first + k / SA_PIECE].x + k % SA_PIECE, page = tok / p.page_size, slot = tok - page * p.page_size;
       if (p.slab_base + page >= p.slabs) continue;               // (behind the cache: the copies brought zeros)
       const uint32_t* src = reinterpret_cast<const uint32_t*>(p.kv + ((((p.slab_base + page) * 2 + 1) * p.page_size + slot) * p.heads + head) * D + c0);
       for (int i = 0; i < 16; ++i) {
@@ -419,7 +423,7 @@ struct SharedRows {
   __device__ __forceinline__ bool full(int tok0) const {
     seen = ~0ull;
     const int t = tok0 / PTC_KT;
-    if (t >= whole && ok) seen = shared_mask(meta + (base + t - t0 & 3) * 4, p.tile_pieces, p.piece, bit, len);      // (a row that is none may have anything)
+    if (t >= whole && ok) seen = shared_mask(meta + (base + t - t0 & 3) * 4, SA_TILE_PIECES, bit, len);      // (a row that is none may have anything)
     return seen == ~0ull;
   }
   __device__ __forceinline__ bool visible(int kj) const { return seen >> (kj & (PTC_KT - 1)) & 1ull; }
@@ -485,25 +489,31 @@ struct SharedRows {
   }
 };
 
-// A lane a piece of the tile: its boxes, K or V.  A place without a piece gets the first one again: what stands there is multiplied by probability 0, and what
-// an earlier kernel left in shared memory need not be finite.
+// A lane a piece of the tile: the first of every run of neighbours copies them, K or V.  A place without a piece gets the tile's first one again: what stands there is
+// multiplied by probability 0, and what an earlier kernel left in shared memory need not be finite.
+struct SharedMaps {
+  CUtensorMap rows[SA_TILE_PIECES];      // boxes of 16, 32, 48, 64 rows (as far as a page has so many)
+};
 template <int D>
-__device__ __forceinline__ void shared_fetch(const SharedAttnParams& p, const CUtensorMap* map, const int4& e, int part, int head, uint32_t dst, uint64_t* bar) {
+__device__ __forceinline__ void shared_fetch(const SharedAttnParams& p, const SharedMaps& maps, const int4& e, int part, int head, uint32_t dst, uint64_t* bar) {
   const int lane = threadIdx.x & 31;
-  const int first = __shfl_sync(0xffffffffu, e.x, 0), at = e.w > 0 ? e.x : first;
+  const int first = __shfl_sync(0xffffffffu, e.x, 0), at = e.w > 0 ? e.x : first, before = __shfl_up_sync(0xffffffffu, at, 1);
+  const int page = at / p.page_size, slot = at - page * p.page_size;
+  const uint32_t starts = __ballot_sync(0xffffffffu, lane == 0 || at != before + SA_PIECE || slot == 0);
   if (lane == 0) mbar_arrive_expect_tx(bar, PTC_KT * D * 2);
   __syncwarp();
-  if (lane < p.tile_pieces) {
-    const int page = at / p.page_size, slot = at - page * p.page_size;
+  if (lane < SA_TILE_PIECES && (starts >> lane & 1u)) {
+    const uint32_t behind = (starts | 1u << SA_TILE_PIECES) & ~((2u << lane) - 1u);
+    const CUtensorMap* map = &maps.rows[__ffs(behind) - 2 - lane];
 #pragma unroll
     for (int kb = 0; kb < D / 64; ++kb)
-      ptc_tma_5d(dst + kb * (PTC_KT * 128) + lane * p.piece * 128, map, smem_u32(bar), kb * 64, slot, head, part, static_cast<int>(p.slab_base + page));
+      ptc_tma_5d(dst + kb * (PTC_KT * 128) + lane * SA_PIECE * 128, map, smem_u32(bar), kb * 64, slot, head, part, static_cast<int>(p.slab_base + page));
   }
   __syncwarp();
 }
 
 template <int D>
-__global__ void __launch_bounds__(PTC_THREADS, 2) shared_attn_kernel(const __grid_constant__ CUtensorMap map, const __grid_constant__ SharedAttnParams p) {
+__global__ void __launch_bounds__(PTC_THREADS, 2) shared_attn_kernel(const __grid_constant__ SharedMaps maps, const __grid_constant__ SharedAttnParams p) {
   using L = PtcLayout<D>;
   extern __shared__ uint8_t sa_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(sa_raw) + 1023) & ~static_cast<uintptr_t>(1023));
@@ -515,7 +525,8 @@ __global__ void __launch_bounds__(PTC_THREADS, 2) shared_attn_kernel(const __gri
   if (tid == 0) {
     ptc_init(sh, 1);
     ptc_init(sh2, 1);
-    prefetch_tmap(&map);
+    prefetch_tmap(&maps.rows[0]);
+    prefetch_tmap(&maps.rows[SA_TILE_PIECES - 1]);
   }
   if (warp == 4) {
     tmem_alloc(&sh->tmem, 256);
@@ -562,10 +573,10 @@ __global__ void __launch_bounds__(PTC_THREADS, 2) shared_attn_kernel(const __gri
       uint64_t *full = values ? sh->v_full : sh->k_full, *empty = values ? sh->v_empty : sh->k_empty;
       const uint32_t ring = smem_u32(smem + (values ? L::V : L::K));
       auto find = [&]() {                                     // a lane a piece of the tile
-        const int i = w.t * p.tile_pieces + lane;
-        return lane < p.tile_pieces && w.left > 0 && i < w.count ? p.entries[static_cast<long long>(w.g) * p.cap + i] : make_int4(0, 0, 0, 0);
+        const int i = w.t * SA_TILE_PIECES + lane;
+        return lane < SA_TILE_PIECES && w.left > 0 && i < w.count ? p.entries[static_cast<long long>(w.g) * p.cap + i] : make_int4(0, 0, 0, 0);
       };
-      int4 next = lane < p.tile_pieces ? head_piece : make_int4(0, 0, 0, 0);      // (the first tile's)
+      int4 next = lane < SA_TILE_PIECES ? head_piece : make_int4(0, 0, 0, 0);      // (the first tile's)
       uint32_t turn = 0;                                      // bit s: parity of stage s's next tile that is changed
       bool pending = false;                                   // the tile in front, if its values are still to be changed
       for (int j = 0; j <= part.w; ++j) {
@@ -583,9 +594,9 @@ __global__ void __launch_bounds__(PTC_THREADS, 2) shared_attn_kernel(const __gri
             break;
           }
           // (tile j + 4's stands where tile j's was: its stage was empty, so tile j + 2's scores have been multiplied, and tile j's output with them)
-          if (!values && masked && lane < p.tile_pieces) meta[(j & 3) * 4 + lane] = e;
+          if (!values && masked && lane < SA_TILE_PIECES) meta[(j & 3) * 4 + lane] = e;
           change = values && masked && careful;
-          shared_fetch<D>(p, &map, e, values ? 1 : 0, head, ring + s * L::TILE, change ? &sh->v_part[s] : &full[s]);
+          shared_fetch<D>(p, maps, e, values ? 1 : 0, head, ring + s * L::TILE, change ? &sh->v_part[s] : &full[s]);
         }
         if (pending) {                                        // (behind the next tile's copies, which are on their way meanwhile)
           const int o = s ^ 1;
@@ -707,10 +718,10 @@ __global__ void __launch_bounds__(32 * SJ_WARPS) shared_join_kernel(const __grid
 }
 
 template <int D>
-static int launch_shared(const CUtensorMap& map, const SharedAttnParams& p, int grid, void* stream) {
+static int launch_shared(const SharedMaps& maps, const SharedAttnParams& p, int grid, void* stream) {
   const int units = p.groups * p.heads, m = p.sub * p.G;
   VB_CHECK_CUDA(rm_smem<shared_attn_kernel<D>>(SA_SMEM<D>));
-  VB_LAUNCH_PDL(shared_attn_kernel<D>, grid, PTC_THREADS, SA_SMEM<D>, stream, map, p);
+  VB_LAUNCH_PDL(shared_attn_kernel<D>, grid, PTC_THREADS, SA_SMEM<D>, stream, maps, p);
   if (grid > 8 * units) VB_LAUNCH_PDL((shared_join_kernel<D, SJ_WARPS>), dim3(units, m), 32 * SJ_WARPS, 0, stream, p);
   else VB_LAUNCH_PDL((shared_join_kernel<D, 1>), dim3(units, (m + SJ_WARPS - 1) / SJ_WARPS), 32 * SJ_WARPS, 0, stream, p);
   return 0;
@@ -732,7 +743,7 @@ static int check_shared(const char* who, const VbSharedPlan* s) {
   VB_CHECK_ARG(s->columns > 0 && s->columns <= SP_MAX_COLUMNS && static_cast<int64_t>(s->columns) * s->page_size <= 0x3fffffff, "%s: %d pages a row (1 to %d)", who, s->columns,
                SP_MAX_COLUMNS);
   VB_CHECK_ARG(s->grid > 0 && s->grid <= 4096, "%s: %d blocks", who, s->grid);
-  const int64_t pieces = static_cast<int64_t>(s->rows) * s->columns * (s->page_size / sa_piece(s->page_size));
+  const int64_t pieces = static_cast<int64_t>(s->rows) * s->columns * (s->page_size / SA_PIECE);
   VB_CHECK_ARG(pieces * s->n_kv <= 0x3fffffff, "%s: %d rows of %d pages on %d heads", who, s->rows, s->columns, s->n_kv);
   return 0;
 }
@@ -747,7 +758,7 @@ static SharedLayout shared_layout(const VbSharedPlan* s) {
   l.sub = shared_sub(s->width, G);
   l.subs = (s->width + l.sub - 1) / l.sub;
   l.groups = s->rows / s->width * l.subs;
-  l.cap = l.sub * s->columns * (s->page_size / sa_piece(s->page_size));
+  l.cap = l.sub * s->columns * (s->page_size / SA_PIECE);
   l.mpad = (l.sub * G + 15) / 16 * 16;
   const size_t units = static_cast<size_t>(l.groups) * s->n_kv, segments = s->grid + units;
   l.parts = 16ull * l.groups * l.cap;
@@ -783,8 +794,7 @@ extern "C" int vb_shared_plan(const VbSharedPlan* plan, const int32_t* d_table, 
   p.blocks_of = reinterpret_cast<int2*>(at + l.blocks_of);
   p.table = d_table, p.tokens = d_tokens;
   p.rows = plan->rows, p.width = plan->width, p.sub = l.sub, p.subs = l.subs, p.groups = l.groups, p.cap = l.cap;
-  p.columns = plan->columns, p.pages = pages, p.page_size = plan->page_size, p.piece = sa_piece(plan->page_size);
-  p.tile_pieces = PTC_KT / p.piece, p.heads = plan->n_kv, p.grid = plan->grid;
+  p.columns = plan->columns, p.pages = pages, p.page_size = plan->page_size, p.heads = plan->n_kv, p.grid = plan->grid;
   const int chunks = (plan->columns + SP_CHUNK - 1) / SP_CHUNK, cluster = chunks > 4 ? SP_CLUSTER : chunks > 2 ? 4 : chunks;      // (a chunk a block, as far as they go)
   VB_LAUNCH_PDL_CLUSTER(shared_list_kernel, l.groups * cluster, SP_THREADS, (chunks + cluster - 1) / cluster * SP_CHUNK * 16, stream, cluster, p);
   VB_LAUNCH_PDL(shared_deal_kernel, 1, SD_THREADS, 0, stream, p);
@@ -800,17 +810,24 @@ extern "C" int vb_shared_attn(void* d_out, const void* d_q, const void* d_kv, in
   VB_CHECK_ARG(reinterpret_cast<uintptr_t>(d_kv) % 16 == 0 && reinterpret_cast<uintptr_t>(d_q) % 16 == 0 && reinterpret_cast<uintptr_t>(d_out) % 16 == 0,
                "vb_shared_attn: unaligned tensors");
   const SharedLayout l = shared_layout(plan);
-  const int D = plan->head_dim, H = plan->n_kv, P = plan->page_size, piece = sa_piece(P);
+  const int D = plan->head_dim, H = plan->n_kv, P = plan->page_size;
   auto fn = encode_fn();
   VB_CHECK_ARG(fn, "vb_shared_attn: cuTensorMapEncodeTiled not available (no CUDA driver?)");
-  CUtensorMap map;
+  SharedMaps maps;
   const cuuint64_t dims[5] = {static_cast<cuuint64_t>(D), static_cast<cuuint64_t>(P), static_cast<cuuint64_t>(H), 2, static_cast<cuuint64_t>(slabs)};
   const cuuint64_t row = 2ull * H * D;
   const cuuint64_t strides[4] = {row, 2ull * D, row * P, 2 * row * P};
-  const cuuint32_t box[5] = {64, static_cast<cuuint32_t>(piece), 1, 1, 1}, estr[5] = {1, 1, 1, 1, 1};
-  const CUresult r = fn(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(d_kv), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  VB_CHECK_ARG(r == CUDA_SUCCESS, "vb_shared_attn: cuTensorMapEncodeTiled failed: CUresult %d", static_cast<int>(r));
+  const cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  for (int i = 0; i < SA_TILE_PIECES; ++i) {
+    if ((i + 1) * SA_PIECE > P) {                        // (no run of so many)
+      maps.rows[i] = maps.rows[0];
+      continue;
+    }
+    const cuuint32_t box[5] = {64, static_cast<cuuint32_t>((i + 1) * SA_PIECE), 1, 1, 1};
+    const CUresult r = fn(&maps.rows[i], CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 5, const_cast<void*>(d_kv), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    VB_CHECK_ARG(r == CUDA_SUCCESS, "vb_shared_attn: cuTensorMapEncodeTiled failed: CUresult %d", static_cast<int>(r));
+  }
   uint8_t* at = static_cast<uint8_t*>(plan->d_buffer);
   SharedAttnParams p = {};
   p.q = static_cast<const __nv_bfloat16*>(d_q), p.out = static_cast<__nv_bfloat16*>(d_out), p.kv = static_cast<const __nv_bfloat16*>(d_kv);
@@ -821,8 +838,8 @@ extern "C" int vb_shared_attn(void* d_out, const void* d_q, const void* d_kv, in
   p.acc = reinterpret_cast<float*>(at + l.acc), p.stat = reinterpret_cast<float2*>(at + l.stat);
   p.slab_base = slab_base, p.slabs = slabs;
   VB_CHECK_ARG(p.wait_flag = wait_flag(WK_PREFILL_ATTN), "vb_shared_attn: no mapped host memory");
-  p.rows = plan->rows, p.width = plan->width, p.sub = l.sub, p.subs = l.subs, p.groups = l.groups, p.cap = l.cap, p.page_size = P, p.piece = piece;
-  p.tile_pieces = PTC_KT / piece, p.n_q = plan->n_q, p.heads = H, p.G = plan->n_q / H, p.mpad = l.mpad, p.xt_tile = out_xt_tile;
+  p.rows = plan->rows, p.width = plan->width, p.sub = l.sub, p.subs = l.subs, p.groups = l.groups, p.cap = l.cap, p.page_size = P;
+  p.n_q = plan->n_q, p.heads = H, p.G = plan->n_q / H, p.mpad = l.mpad, p.xt_tile = out_xt_tile;
   p.scale_log2 = sm_scale * 1.44269504088896f;
-  return D == 64 ? launch_shared<64>(map, p, plan->grid, stream) : launch_shared<128>(map, p, plan->grid, stream);
+  return D == 64 ? launch_shared<64>(maps, p, plan->grid, stream) : launch_shared<128>(maps, p, plan->grid, stream);
 }
