@@ -4,9 +4,18 @@
 //   the n candidates of largest weight[w] * total[w][v]; equal ones in the order of (w, v)
 //   a beam that has ended has one candidate, its end token at its own score
 //
-// Two launches.  The first reads the logits once: a block streams a part of a row through registers in chunks, the next one in flight, and leaves the part's
-// maximum, its sum of exponentials and its n largest in order.  The second, a block a request, adds the sums up, ranks the n largest of every part by their totals
-// and writes the n best.  What orders candidates is computed in 64 bits from the parts' sums; a sum's terms carry 2^-22 each and no common error.
+// Two kernels.  The first reads the logits once: a block takes a part of a row in chunks, by asynchronous copies into shared memory with the next one on its way,
+// and leaves the part's maximum, its sum of exponentials and its n largest in order.  The second, a block a request, adds the sums up, ranks the n largest of every
+// part by their totals and writes the n best.  Where a request has at most eight parts both are one launch, a cluster a request.
+//
+// What orders candidates is computed in 64 bits from the parts' sums.  A sum's terms carry the special function unit's 2^-22 and, from one fp32 constant for log2 e,
+// 1.3e-8 of the distance from the maximum: below 2^-20 of a term that counts (distance up to 40).  Sums of parts meet through log2 e in two constants.
+//
+// Measured (a captured chain of calls, the parts alone in brackets): 16 requests of 16 beams over 156940 bf16 tokens, n 32, 31 us [23]; its 80 MB are 12.4 us of
+// HBM, and what is above that is the unevenness of 512 blocks on 148 SMs (three or four each: they end after 9 to 23 us), a meeting of the block for every chunk,
+// and the join (5: latencies).  16 of 5 over 32003 fp32 tokens, n 10: 12.5 us.  One of two over 2051: 5.9, most of it the launch.
+// Four blocks an SM with two chunks in shared memory: 31.2 us; three with three 33.3, with four 32.6; four with three 34.4 (a list of 512); five with two 31.6.  Parts so
+// that all blocks run at once: more of them pay the first cut and the last order again, fewer leave SMs idle.
 #include "../../include/vb_api.h"
 #define VB_PDL_FAMILY 16
 #include "rowmma.cuh"
@@ -630,7 +639,8 @@ __global__ void __launch_bounds__(BS_THREADS) beam_small_kernel(const __grid_con
 
 // ---- states that follow their beams ----------------------------------------------------------------------------------------------
 // state[slot[b][i]] = what state[slot[b][parent[b][i]]] was.  A thread owns a vector's place in all W rows of a request: it reads what moves there, then
-// writes, so that rows may change places without a second copy of the state.
+// writes, so that rows may change places without a second copy of the state.  All states in one launch (64 a launch).  Bound by HBM: 8 requests of 8 beams,
+// 413 MB read and 413 written, 131 us, 98 % of a copy's rate; one small request 2.0 us, the launch.
 constexpr int BR_TENSORS = 64, BR_THREADS = 256;
 struct ReorderTensors {
   void* at[BR_TENSORS];

@@ -7,6 +7,10 @@
 //
 // Free pages are given out lowest number first, to rows in their order, to a row first the page for a copy.  All or nothing: if pages or columns run short
 // nothing changes and the status says so.
+//
+// What bounds it: the tables a chain of dependent loads and meetings (a step of 64 rows 7 us, a chain of such steps; 16 continuations of a prompt of 8000 tokens 9),
+// the contents HBM: tails of a step, 57 MB, 10 us beside a floor of 8.9; 140 pages of 2.1 MB
+// that move, 587 MB read and written, 91 of 97.5 us in all (6.4 TB/s).
 #include "../../include/vb_api.h"
 #define VB_PDL_FAMILY 4
 #include "rowmma.cuh"

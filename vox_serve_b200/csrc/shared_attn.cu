@@ -16,6 +16,14 @@
 // whose results are not finite, and that had such tiles, walks its segments again: values that are not finite are taken out on the way, and the rows that see
 // them get them back at the end.  Caches that hold finite numbers everywhere, behind a row's last token too, never go there.
 // Probabilities enter the second product as two bf16 parts (2^-17).
+//
+// What bounds it now: HBM while tiles arrive (6 to 7.6 TB/s), and around that 2.5 us to the first copy, 3 to 5 from a block's last scores to its results in memory,
+// 4 for the join.  Measured, a call in a captured chain: 8 requests of 8 rows (7 alive) on prompts of 4050 tokens and 300 more, 16 heads on 8 of 128, pages of 128:
+// 157 MB in 37.4 us (24.4 of HBM; blocks of a group and head end unevenly, up to 4 us); 2 of 5 on 61007 tokens, 32 heads on 2, pages of 48: 110 MB in 34.7 us (17.1;
+// 80 rows of products put out 12 MB of partial results); 4 rows of 171 tokens, pages of 16: 7.7 us.  Read once for every row (paged_attn) the same take 112, 322 and 13.4.
+// Against paged_attn without anything to share: 8 rows of 1100 tokens 15.2 us beside 18.0, 32 rows of 600 21.0 beside 17.4: a row alone keeps 126 of 128 accumulator
+// rows idle, and that one fetches while the kernel in front still runs.
+// mma.sync instead of the tcgen05 core took 104 us for the second case.  Three to six blocks' worth of segments an SM instead of two: 54 to 58 for the first (43 then).
 #include "../../include/vb_api.h"
 #define VB_PDL_FAMILY 1
 #include "attn_tc.cuh"
