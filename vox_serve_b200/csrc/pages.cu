@@ -8,7 +8,7 @@
 // Free pages are given out lowest number first, to rows in their order, to a row first the page for a copy.  All or nothing: if pages or columns run short
 // nothing changes and the status says so.
 //
-// What bounds it: the tables a chain of dependent loads and meetings (a step of 64 rows 7 us, a chain of such steps; 16 continuations of a prompt of 8000 tokens 9),
+// What bounds it: the tables a chain of dependent loads and meetings (a step of 64 rows 7 us, a chain of such steps; 16 continuations of a prompt of 8000 tokens 8),
 // the contents HBM: tails of a step, 57 MB, 10 us beside a floor of 8.9; 140 pages of 2.1 MB
 // that move, 587 MB read and written, 91 of 97.5 us in all (6.4 TB/s).
 #include "../../include/vb_api.h"
@@ -17,7 +17,7 @@
 
 namespace vb {
 
-constexpr int PG_THREADS = 1024, PG_MAX_CLUSTER = 8, PG_MAX_ROWS = 4096, PG_STAGE = 8192, PG_SMEM_PAGES = 8192;
+constexpr int PG_THREADS = 1024, PG_FEW_THREADS = 512, PG_FEW_CELLS = 16384, PG_MAX_CLUSTER = 8, PG_MAX_ROWS = 4096, PG_STAGE = 8192, PG_SMEM_PAGES = 8192;
 
 // words of a pool's status
 enum { PS_MISSING = 0, PS_LONG = 1, PS_COPIES = 2, PS_USED = 3 };
@@ -25,6 +25,7 @@ enum { PS_MISSING = 0, PS_LONG = 1, PS_COPIES = 2, PS_USED = 3 };
 __device__ __forceinline__ int ldcg(const int32_t* p) { return __ldcg(p); }
 
 // exclusive prefix over the block of two numbers a thread; totals in all threads.  `sums`: 33 words
+template <int THREADS>
 __device__ __forceinline__ int2 block_prefix(int2 mine, int2* sums, int2& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int2 inc = mine;
@@ -36,7 +37,7 @@ __device__ __forceinline__ int2 block_prefix(int2 mine, int2* sums, int2& total)
   __syncthreads();                                   // (the last call's sums have been read)
   if (lane == 31) sums[warp] = inc;
   __syncthreads();
-  const int2 s = sums[lane];
+  const int2 s = THREADS == 1024 || lane < THREADS / 32 ? sums[lane] : make_int2(0, 0);
   const int2 before = make_int2(__reduce_add_sync(0xffffffffu, lane < warp ? s.x : 0), __reduce_add_sync(0xffffffffu, lane < warp ? s.y : 0));
   total = make_int2(__reduce_add_sync(0xffffffffu, s.x), __reduce_add_sync(0xffffffffu, s.y));
   return make_int2(before.x + inc.x - mine.x, before.y + inc.y - mine.y);
@@ -82,7 +83,10 @@ __device__ __forceinline__ T* in_block0(T* p) {
 // What is known of a row stands in every block's shared memory.  A row that k rows continue adds k - 1 to the count of each of its pages, once a page and not
 // once a row that takes it over.  Counts and free pages stand in block 0's shared memory for pools of up to PG_SMEM_PAGES pages (scratch in global memory
 // beyond: a step of 64 rows took 13.0 us with it, 11.4 without, each launch by itself), and are volatile to every block.
-__global__ void __launch_bounds__(PG_THREADS, 1) fork_pages_kernel(const __grid_constant__ ForkParams p) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1) fork_pages_kernel(const __grid_constant__ ForkParams p) {
+  constexpr int LOG_THREADS = THREADS == 1024 ? 10 : 9;
+  static_assert(THREADS == 1 << LOG_THREADS, "rows of the cluster's threads are powers of two");
   extern __shared__ int32_t pg_smem[];
   int32_t* s_src = pg_smem;                          // [rows] the row that a row continues, -1: none
   int32_t* s_grow = s_src + p.rows;                  // [rows] tokens it gets room for
@@ -96,13 +100,13 @@ __global__ void __launch_bounds__(PG_THREADS, 1) fork_pages_kernel(const __grid_
   __shared__ int2 sums[32];
   __shared__ int s_ok, s_copies;
   const int tid = threadIdx.x, rank = cluster_ctarank(), blocks = cluster_nctarank(), P = p.page_size;
-  const int all = blocks * PG_THREADS, mine = rank * PG_THREADS + tid;
+  const int all = blocks * THREADS, mine = rank * THREADS + tid;
   volatile int32_t* work = p.in_smem ? in_block0(stage + PG_STAGE) : p.work;                // [pages] holders
   volatile int32_t* free = p.in_smem ? in_block0(stage + PG_STAGE + p.pages) : p.free;      // [pages needed] the lowest free ones
   volatile int32_t* base = in_block0(s_base);
   pdl_sync();
   const int ref = mine < p.pages ? p.refs[mine] : 0;      // (all loads of the start at once)
-  for (int i = tid; i < p.rows; i += PG_THREADS) {
+  for (int i = tid; i < p.rows; i += THREADS) {
     const int s = fork_source(p, i), n = fork_tokens(p, i), g = p.grow ? p.grow[i] : p.grow_all;
     s_src[i] = s, s_grow[i] = g > 0 ? g : 0, s_tok[i] = n, s_held[i] = (n + P - 1) / P, s_heirs[i] = 0, s_keeper[i] = 0x7fffffff, s_tail[i] = -1;
   }
@@ -111,22 +115,22 @@ __global__ void __launch_bounds__(PG_THREADS, 1) fork_pages_kernel(const __grid_
   if (mine < p.pages) work[mine] = ref;
   for (int g = mine + all; g < p.pages; g += all) work[g] = p.refs[g];
   __syncthreads();
-  for (int i = tid; i < p.rows; i += PG_THREADS)
+  for (int i = tid; i < p.rows; i += THREADS)
     if (s_src[i] >= 0) atomicAdd(s_heirs + s_src[i], 1), atomicMin(s_keeper + s_src[i], i);
   cluster_sync_all();
 
   // holders of every page after the step, from those before it
-  const int log_x = min(10, 32 - __clz(p.columns - 1)), x = 1 << log_x;      // (x neighbouring threads of the cluster a row)
+  const int log_x = min(LOG_THREADS, 32 - __clz(p.columns - 1)), x = 1 << log_x;      // (x neighbouring threads of the cluster a row)
   for (int s = mine >> log_x; s < p.rows; s += all >> log_x) {
     const int more = s_heirs[s] - 1, held = more ? s_held[s] : 0;
-#pragma unroll 4
+#pragma unroll 1
     for (int c = mine & (x - 1); c < held; c += x) {
       const int g = fork_page(p, s, c);
       if (g >= 0) atomicAdd(const_cast<int32_t*>(work) + g, more);
     }
   }
   if (rank == 0)
-    for (int i = tid; i < p.rows; i += PG_THREADS) {
+    for (int i = tid; i < p.rows; i += THREADS) {
       const int s = s_src[i], n = s < 0 ? 0 : s_tok[s];
       if (n % P && s_keeper[s] != i) s_tail[i] = fork_page(p, s, n / P);
     }
@@ -137,7 +141,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) fork_pages_kernel(const __grid_
   if (rank == 0) {
     // pages that every row needs: one for a copy, the others for tokens
     int need_all = 0, too_long = 0;
-    for (int i0 = 0; i0 < p.rows; i0 += PG_THREADS) {
+    for (int i0 = 0; i0 < p.rows; i0 += THREADS) {
       const int i = i0 + tid, s = i < p.rows ? s_src[i] : -1;
       int need = 0, longer = 0, copy = 0;
       if (s >= 0) {
@@ -147,14 +151,14 @@ __global__ void __launch_bounds__(PG_THREADS, 1) fork_pages_kernel(const __grid_
         need = longer ? 0 : copy + static_cast<int>(want) - s_held[s];
       }
       int2 total;
-      const int2 before = block_prefix(make_int2(need, longer), sums, total);
+      const int2 before = block_prefix<THREADS>(make_int2(need, longer), sums, total);
       if (i < p.rows) s_base[i] = (need_all + before.x) * 2 + copy;
       need_all += total.x;
       too_long += total.y;
     }
     // the lowest free pages
     int have = 0;
-    for (int g0 = 0; g0 < p.pages && have < need_all; g0 += 4 * PG_THREADS) {
+    for (int g0 = 0; g0 < p.pages && have < need_all; g0 += 4 * THREADS) {
       int n[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -162,7 +166,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) fork_pages_kernel(const __grid_
         n[j] = g < p.pages ? work[g] : 1;
       }
       int2 total;
-      int at = have + block_prefix(make_int2((n[0] == 0) + (n[1] == 0) + (n[2] == 0) + (n[3] == 0), 0), sums, total).x;
+      int at = have + block_prefix<THREADS>(make_int2((n[0] == 0) + (n[1] == 0) + (n[2] == 0) + (n[3] == 0), 0), sums, total).x;
 #pragma unroll
       for (int j = 0; j < 4; ++j)
         if (n[j] == 0) {
@@ -174,8 +178,8 @@ __global__ void __launch_bounds__(PG_THREADS, 1) fork_pages_kernel(const __grid_
     const bool ok = have >= need_all && too_long == 0;
     __syncthreads();
     if (ok) {
-      for (int k = tid; k < need_all; k += PG_THREADS) work[free[k]] = 1;
-      for (int i = tid; i < p.rows; i += PG_THREADS)
+      for (int k = tid; k < need_all; k += THREADS) work[free[k]] = 1;
+      for (int i = tid; i < p.rows; i += THREADS)
         if (s_tail[i] >= 0) {
           int32_t* c = p.copies + 3ll * atomicAdd(&s_copies, 1);
           c[0] = s_tail[i], c[1] = free[s_base[i] >> 1], c[2] = s_tok[s_src[i]] % P;
@@ -194,7 +198,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) fork_pages_kernel(const __grid_
 
   const bool ok = *static_cast<volatile int*>(in_block0(&s_ok)) != 0;
   int32_t* s_want = s_keeper;                        // [rows] pages after the step
-  for (int i = tid; i < p.rows; i += PG_THREADS) {
+  for (int i = tid; i < p.rows; i += THREADS) {
     if (rank != 0) s_base[i] = base[i];
     s_want[i] = s_src[i] < 0 ? 0 : static_cast<int>(min(pages_after(s_src[i], i), static_cast<uint32_t>(p.columns)));
   }
@@ -204,7 +208,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) fork_pages_kernel(const __grid_
     // A block of columns in all rows at a time, read before it is written: rows may take over one another's pages in place.  `across` neighbouring threads a
     // row, without a division an entry.
     const int wide = min((p.columns + blocks - 1) / blocks, max(1, PG_STAGE / p.rows));
-    const int log_across = min(10, 32 - __clz(wide - 1)), across = 1 << log_across, tx = tid & (across - 1), ty = tid >> log_across, down = PG_THREADS >> log_across;
+    const int log_across = min(LOG_THREADS, 32 - __clz(wide - 1)), across = 1 << log_across, tx = tid & (across - 1), ty = tid >> log_across, down = THREADS >> log_across;
     for (int c0 = rank * wide; c0 < p.columns; c0 += blocks * wide) {
       const int w = min(wide, p.columns - c0);
       for (int k = tx; k < w; k += across) {
@@ -246,13 +250,14 @@ struct CompactParams {
 };
 
 // The pages in use that stand behind as many places as there are pages in use move into the holes in front, in their order.
-__global__ void __launch_bounds__(PG_THREADS, 1) compact_pages_kernel(const __grid_constant__ CompactParams p) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS, 1) compact_pages_kernel(const __grid_constant__ CompactParams p) {
   __shared__ int2 sums[32];
   const int tid = threadIdx.x, rank = cluster_ctarank(), blocks = cluster_nctarank();
   pdl_sync();
   if (rank == 0) {
     int used = 0;
-    for (int g0 = 0; g0 < p.pages; g0 += 4 * PG_THREADS) {
+    for (int g0 = 0; g0 < p.pages; g0 += 4 * THREADS) {
       int mine = 0;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -260,11 +265,11 @@ __global__ void __launch_bounds__(PG_THREADS, 1) compact_pages_kernel(const __gr
         mine += g < p.pages && p.refs[g] > 0;
       }
       int2 total;
-      block_prefix(make_int2(mine, 0), sums, total);
+      block_prefix<THREADS>(make_int2(mine, 0), sums, total);
       used += total.x;
     }
     int holes = 0, movers = 0;
-    for (int g0 = 0; g0 < p.pages; g0 += 4 * PG_THREADS) {
+    for (int g0 = 0; g0 < p.pages; g0 += 4 * THREADS) {
       int n[2] = {0, 0}, what[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -275,7 +280,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) compact_pages_kernel(const __gr
         if (g < p.pages) p.moved[g] = in && g < used ? g : -1;
       }
       int2 total;
-      const int2 before = block_prefix(make_int2(n[0], n[1]), sums, total);
+      const int2 before = block_prefix<THREADS>(make_int2(n[0], n[1]), sums, total);
       int h = holes + before.x, m = movers + before.y;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -286,7 +291,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) compact_pages_kernel(const __gr
       movers += total.y;
     }
     __syncthreads();
-    for (int k = tid; k < movers; k += PG_THREADS) {      // (as many holes as movers)
+    for (int k = tid; k < movers; k += THREADS) {      // (as many holes as movers)
       const int from = p.from[k], to = p.to[k];
       p.moved[from] = to;
       int32_t* c = p.copies + 3ll * k;
@@ -295,7 +300,7 @@ __global__ void __launch_bounds__(PG_THREADS, 1) compact_pages_kernel(const __gr
     if (tid == 0) p.status[PS_MISSING] = p.status[PS_LONG] = 0, p.status[PS_COPIES] = movers, p.status[PS_USED] = used;
   }
   cluster_sync_all();
-  const long long at = static_cast<long long>(rank) * PG_THREADS + tid, step = static_cast<long long>(blocks) * PG_THREADS;
+  const long long at = static_cast<long long>(rank) * THREADS + tid, step = static_cast<long long>(blocks) * THREADS;
   for (long long e = at; e < p.cells; e += step) {
     const int g = p.table[e];
     p.out_table[e] = g >= 0 && g < p.pages ? ldcg(p.moved + g) : g;
@@ -380,6 +385,13 @@ static int copy_listed(const VbPageCache* caches, int n_caches, const VbPagePool
   return 0;
 }
 
+// Small tables take half as many threads a block: what is done once costs its instructions and meetings.  A step, 512 / 1024 threads: 44 cells 6.5 / 7.4 us, 8000 11.6 /
+// 12.9, 16000 17.1 / 17.3, 34000 26.4 / 21.4, 130000 33.4 / 27.3.
+static bool pg_few(long long cells, int pages) { return cells <= PG_FEW_CELLS && pages <= PG_SMEM_PAGES; }
+static int pg_cluster(long long cells, bool few) {
+  const long long per = 4 * (few ? PG_FEW_THREADS : PG_THREADS), share = (cells + per - 1) / per;
+  return share >= PG_MAX_CLUSTER ? PG_MAX_CLUSTER : share > 2 ? 4 : static_cast<int>(share);
+}
 static int check_pool(const char* who, const VbPagePool* a, const VbPagePool* out) {
   VB_CHECK_ARG(a && out, "%s: null pool", who);
   for (const VbPagePool* p : {a, out})
@@ -428,10 +440,12 @@ extern "C" int vb_fork_pages(const VbPagePool* pool, const VbPagePool* out, cons
   p.work = out->d_scratch, p.free = p.work + pool->pages, p.in_smem = pool->pages <= PG_SMEM_PAGES;
   p.src = d_src, p.grow = d_grow, p.grow_all = grow;
   p.rows = pool->rows, p.columns = pool->columns, p.pages = pool->pages, p.page_size = pool->page_size, p.group = group;
-  const long long cells = static_cast<long long>(p.rows) * p.columns, share = (cells + 4 * PG_THREADS - 1) / (4 * PG_THREADS);
-  const int cluster = share >= PG_MAX_CLUSTER ? PG_MAX_CLUSTER : share > 2 ? 4 : static_cast<int>(share);
-  VB_CHECK_CUDA(rm_smem<fork_pages_kernel>((8 * PG_MAX_ROWS + PG_STAGE + 2 * PG_SMEM_PAGES) * 4));
-  VB_LAUNCH_PDL_CLUSTER(fork_pages_kernel, cluster, PG_THREADS, (8 * p.rows + PG_STAGE + (p.in_smem ? 2 * p.pages : 0)) * 4, stream, cluster, p);
+  const bool few = pg_few(static_cast<long long>(p.rows) * p.columns, p.pages);
+  const int cluster = pg_cluster(static_cast<long long>(p.rows) * p.columns, few), most = (8 * PG_MAX_ROWS + PG_STAGE + 2 * PG_SMEM_PAGES) * 4;
+  const int smem = (8 * p.rows + PG_STAGE + (p.in_smem ? 2 * p.pages : 0)) * 4;
+  VB_CHECK_CUDA(few ? rm_smem<fork_pages_kernel<PG_FEW_THREADS>>(most) : rm_smem<fork_pages_kernel<PG_THREADS>>(most));
+  if (few) VB_LAUNCH_PDL_CLUSTER(fork_pages_kernel<PG_FEW_THREADS>, cluster, PG_FEW_THREADS, smem, stream, cluster, p);
+  else VB_LAUNCH_PDL_CLUSTER(fork_pages_kernel<PG_THREADS>, cluster, PG_THREADS, smem, stream, cluster, p);
   return copy_listed(caches, n_caches, pool, out->d_copies, out->d_status, PC_TAILS, stream);
 }
 
@@ -445,8 +459,9 @@ extern "C" int vb_compact_pages(const VbPagePool* pool, const VbPagePool* out, c
   p.from = out->d_scratch, p.to = p.from + pool->pages;
   p.rows = pool->rows, p.pages = pool->pages, p.page_size = pool->page_size;
   p.cells = static_cast<long long>(pool->rows) * pool->columns;
-  const long long share = (p.cells + 4 * PG_THREADS - 1) / (4 * PG_THREADS);
-  const int cluster = share >= PG_MAX_CLUSTER ? PG_MAX_CLUSTER : share > 2 ? 4 : static_cast<int>(share);
-  VB_LAUNCH_PDL_CLUSTER(compact_pages_kernel, cluster, PG_THREADS, 0, stream, cluster, p);
+  const bool few = pg_few(p.cells, p.pages);
+  const int cluster = pg_cluster(p.cells, few);
+  if (few) VB_LAUNCH_PDL_CLUSTER(compact_pages_kernel<PG_FEW_THREADS>, cluster, PG_FEW_THREADS, 0, stream, cluster, p);
+  else VB_LAUNCH_PDL_CLUSTER(compact_pages_kernel<PG_THREADS>, cluster, PG_THREADS, 0, stream, cluster, p);
   return copy_listed(caches, n_caches, pool, out->d_copies, out->d_status, PC_WHOLE, stream);
 }
