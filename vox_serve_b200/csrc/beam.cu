@@ -29,6 +29,7 @@ constexpr int BS_MAX_N = 64, BS_MAX_W = 32;
 constexpr int BS_CLUSTER = 8;                                   // blocks of a request that join in the same launch
 static_assert(BS_CLUSTER * BS_MAX_N * 16 <= 16384, "the join's candidates stand where the ring stood");
 constexpr int BJ_BINS = 1024;                                   // 16 to a doubling, from 2^-23 to 2^41
+constexpr int BJ_FEW = 1024;
 constexpr int BJ_THREADS = 512, BJ_ALL = 8192;                  // candidates of a request: 128 KB of ranks and values
 
 struct BeamStats {
@@ -612,13 +613,14 @@ __device__ __forceinline__ void beam_join(JoinShared<THREADS>& sh, uint64_t* bj_
   }
 }
 
-__global__ void __launch_bounds__(BJ_THREADS) beam_join_kernel(const __grid_constant__ BeamCall p) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) beam_join_kernel(const __grid_constant__ BeamCall p) {
   extern __shared__ uint64_t bj_key[];                 // [W * parts * n] ranks as ordered numbers, 0: none; behind them the candidates
-  __shared__ JoinShared<BJ_THREADS> sh;
+  __shared__ JoinShared<THREADS> sh;
   if (threadIdx.x == 0) sh.box[0] = sh.box[1] = sh.box[2] = sh.count = 0u;
   pdl_sync();
   const long long first = static_cast<long long>(blockIdx.x) * p.W * p.parts;
-  beam_join<BJ_THREADS>(sh, bj_key, p, blockIdx.x, p.stats + first, p.best + first * p.n);
+  beam_join<THREADS>(sh, bj_key, p, blockIdx.x, p.stats + first, p.best + first * p.n);
 }
 
 // Both in one launch where a request's parts are few: a cluster a request, whose blocks leave what they found in the first one's shared memory.  (One beam of two
@@ -750,8 +752,13 @@ extern "C" int vb_beam_select(float* d_score, int32_t* d_parent, int64_t* d_toke
   VB_CHECK_CUDA(logits_f32 ? rm_smem<beam_part_kernel<float>>(sizeof(PartShared)) : rm_smem<beam_part_kernel<__nv_bfloat16>>(sizeof(PartShared)));
   if (logits_f32) VB_LAUNCH_PDL(beam_part_kernel<float>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, p);
   else VB_LAUNCH_PDL(beam_part_kernel<__nv_bfloat16>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, p);
-  VB_CHECK_CUDA(rm_smem<beam_join_kernel>(BJ_ALL * 16));
-  VB_LAUNCH_PDL(beam_join_kernel, static_cast<unsigned>(requests), BJ_THREADS, static_cast<size_t>(width) * parts * n * 16, stream, p);
+  const size_t all = static_cast<size_t>(width) * parts * n;
+  if (all <= BJ_FEW) {
+    VB_LAUNCH_PDL(beam_join_kernel<BS_THREADS>, static_cast<unsigned>(requests), BS_THREADS, all * 16, stream, p);
+    return 0;
+  }
+  VB_CHECK_CUDA(rm_smem<beam_join_kernel<BJ_THREADS>>(BJ_ALL * 16));
+  VB_LAUNCH_PDL(beam_join_kernel<BJ_THREADS>, static_cast<unsigned>(requests), BJ_THREADS, all * 16, stream, p);
   return 0;
 }
 
