@@ -197,6 +197,7 @@ __device__ __forceinline__ void beam_part(PartShared& sh, BeamStats* stats, uint
   // Candidates are above this.  Once the list holds n that is the last one's value: of equal ones the lower tokens came first.
   float above = -INFINITY;
   bool low_cut = true;
+  const uint32_t enough = max(2 * n, 32);
   for (int v0 = first; v0 - warp * BS_SPAN < vecs; v0 += step) {      // (as often in every warp: they meet)
     asm volatile("cp.async.wait_group %0;" ::"n"(BS_STAGES - 2) : "memory");
     __syncwarp();
@@ -295,47 +296,35 @@ __device__ __forceinline__ void beam_part(PartShared& sh, BeamStats* stats, uint
       uint32_t i = atomicAdd(&count, static_cast<uint32_t>(__popc(hits)));
       for (; hits; hits &= hits - 1u, ++i) {
         if (i < BS_CAP) list[i] = keyed(__ffs(hits) - 1);
-        full |= i >= BS_CAP / 4;
+        full |= i >= (more ? enough : BS_CAP);
       }
     }
     if (!__syncthreads_or(full)) continue;
     int c = static_cast<int>(count);
     if (c > BS_CAP) {      // many equal or rising values: of the list and this chunk together those above a cut that leaves at least n, found by halving
-      uint64_t mine_l[BS_CAP / BS_THREADS];
       const uint32_t start = 0xffffffffu - static_cast<uint32_t>(v0 - warp * BS_SPAN) * EV;
-#pragma unroll
-      for (int e = 0; e < BS_CAP / BS_THREADS; ++e) {
+      auto earlier = [&](int e) {                            // (of earlier chunks: this one's are looked at where they came from)
         const uint64_t key = list[tid + e * BS_THREADS];
-        mine_l[e] = static_cast<uint32_t>(key) > start ? key : 0ull;      // (of earlier chunks)
-      }
+        return static_cast<uint32_t>(key) > start ? key : 0ull;
+      };
       int turn = 0, found = c;
-      // by values
-      uint32_t lo = above == -INFINITY ? 1u : order_f32(above) + 1u, hi = ~0u;      // at least n are >= lo, fewer than n are >= hi
-      while (found > BS_CAP / 4 && hi - lo > 1u) {
-        const uint32_t mid = lo + ((hi - lo) >> 1);
-        const float f = unorder_f32(mid);                      // (NaN and infinity above the largest value: none reaches them)
-        int mine = 0;
-#pragma unroll
-        for (int k = 0; k < N; ++k) mine += x.at(k) >= f && x.at(k) != INFINITY ? 1 : 0;
-#pragma unroll
-        for (int e = 0; e < BS_CAP / BS_THREADS; ++e) mine += static_cast<uint32_t>(mine_l[e] >> 32) >= mid ? 1 : 0;
-        const int got = block_count(mine, box, turn);
-        if (got >= n) lo = mid, found = got;
-        else hi = mid;
-      }
-      // equal values by tokens
-      uint64_t cut = static_cast<uint64_t>(lo) << 32, end = static_cast<uint64_t>(lo + 1u) << 32;
+      // (values first, then tokens; at least n are >= cut, fewer than n are >= end)
+      uint64_t cut = static_cast<uint64_t>(above == -INFINITY ? 1u : order_f32(above) + 1u) << 32, end = ~0ull;
+#pragma unroll 1
       while (found > BS_CAP / 4) {
         const uint64_t mid = cut + ((end - cut) >> 1);
         int mine = 0;
-#pragma unroll 4
+#pragma unroll 1
         for (int k = 0; k < N; ++k) mine += keyed(k) >= mid ? 1 : 0;
-#pragma unroll
-        for (int e = 0; e < BS_CAP / BS_THREADS; ++e) mine += mine_l[e] >= mid ? 1 : 0;
+#pragma unroll 1
+        for (int e = 0; e < BS_CAP / BS_THREADS; ++e) mine += earlier(e) >= mid ? 1 : 0;
         const int got = block_count(mine, box, turn);
         if (got >= n) cut = mid, found = got;
         else end = mid;
       }
+      uint64_t kept[BS_CAP / BS_THREADS];
+#pragma unroll
+      for (int e = 0; e < BS_CAP / BS_THREADS; ++e) kept[e] = earlier(e);
       __syncthreads();
       if (tid == 0) count = 0u;
       __syncthreads();
@@ -346,7 +335,7 @@ __device__ __forceinline__ void beam_part(PartShared& sh, BeamStats* stats, uint
       }
 #pragma unroll
       for (int e = 0; e < BS_CAP / BS_THREADS; ++e)
-        if (mine_l[e] >= cut) list[atomicAdd(&count, 1u)] = mine_l[e];
+        if (kept[e] >= cut) list[atomicAdd(&count, 1u)] = kept[e];
       if (tid < 3) box[tid] = 0u;
       __syncthreads();
       c = static_cast<int>(count);
@@ -424,6 +413,7 @@ struct JoinShared {
   static constexpr int CAP = BS_MAX_N + 32;
   // total = (x - top) + base: a row may hold nothing but lowest values; base of an ended beam: its score
   double base[BS_MAX_W], tops[BS_MAX_W];
+  float factor[BS_MAX_W];
   uint64_t list_key[CAP], list_at[CAP], warp_most[THREADS / 32];      // rank, (beam, token)
   double list_total[CAP];
   uint32_t box[3], count;
@@ -448,18 +438,15 @@ __device__ __forceinline__ void beam_join(JoinShared<THREADS>& sh, uint64_t* bj_
   auto place_of = [&](int w, uint64_t e) {
     return static_cast<uint64_t>(w) << 32 | (kind[w] == 2 ? static_cast<uint32_t>(end_token) : 0xffffffffu - static_cast<uint32_t>(e));
   };
-  uint64_t most = 0ull;
-  int mine = 0;
-  for (int w = warp; w < W; w += THREADS / 32) {    // a warp a beam
+  uint64_t e[4];                                       // (the first of a thread's candidates, on their way while the sums are added up)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) e[i] = tid + i * THREADS < all ? mine_of[tid + i * THREADS] : 0ull;
+  for (int w = warp; w < W; w += THREADS / 32) {       // a warp a beam
     const int row = b * W + w;
     const float s = score[row], f = weight ? weight[row] : 1.f;
     const bool over = ended && ended[row];
     const BeamStats t0 = lane < parts ? stats[w * parts + lane] : BeamStats{-INFINITY, 0.f};      // (of a row that was not read: anything)
     int k = !isfinite(s) || !isfinite(f) || !(f > 0.f) ? 0 : over ? 2 : 1;
-    uint64_t e[4] = {0ull, 0ull, 0ull, 0ull};          // (the first of its candidates, on their way meanwhile)
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-      if (lane + 32 * i < per_row) e[i] = mine_of[w * per_row + lane + 32 * i];
     double log_sum = 0.0, peak = 0.0;
     if (k == 1) {
       float top = t0.m;
@@ -475,18 +462,20 @@ __device__ __forceinline__ void beam_join(JoinShared<THREADS>& sh, uint64_t* bj_
       if (top == -INFINITY) k = 0;                       // everything masked: nothing to go on with
       else peak = top, log_sum = log(sum);
     }
-    if (lane == 0) base[w] = static_cast<double>(s) - log_sum, tops[w] = peak, kind[w] = k;
-    __syncwarp();
-    for (int j = lane, i = 0; j < per_row; j += 32, ++i) {
-      uint64_t c = 0ull, key = 0ull;
-      if (k == 1) c = i == 0 ? e[0] : i == 1 ? e[1] : i == 2 ? e[2] : i == 3 ? e[3] : mine_of[w * per_row + j];
-      // (an ended beam's one candidate stands in its first place; what the memory holds there is not looked at)
-      if (k == 2 ? j == 0 : c != 0ull) key = order_f64(total_of(w, c) * static_cast<double>(f));
-      bj_key[w * per_row + j] = key;
-      bj_e[w * per_row + j] = c;
-      mine += key != 0ull;
-      most = max(most, key);
-    }
+    if (lane == 0) base[w] = static_cast<double>(s) - log_sum, tops[w] = peak, sh.factor[w] = f, kind[w] = k;
+  }
+  __syncthreads();
+  uint64_t most = 0ull;
+  int mine = 0;
+#pragma unroll 1
+  for (int c = tid, i = 0; c < all; c += THREADS, ++i) {
+    const int w = c / per_row, k = kind[w];
+    const uint64_t x = k != 1 ? 0ull : i == 0 ? e[0] : i == 1 ? e[1] : i == 2 ? e[2] : i == 3 ? e[3] : mine_of[c];
+    // (an ended beam's one candidate stands in its first place; what the memory holds there is not looked at)
+    const uint64_t key = (k == 2 ? c == w * per_row : x != 0ull) ? order_f64(total_of(w, x) * static_cast<double>(sh.factor[w])) : 0ull;
+    bj_key[c] = key, bj_e[c] = x;
+    mine += key != 0ull;
+    most = max(most, key);
   }
   // All candidates if the list holds them, else those above a cut that leaves at least n.  Candidates are counted by their distance from the largest, 16 bins
   // to every doubling of it; what a bin holds too much of (equal or nearly equal ranks) is found by halving, first of ranks, then of places.
