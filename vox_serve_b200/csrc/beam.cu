@@ -126,6 +126,21 @@ struct Held {
     if (sizeof(T) == 4) w[k] = 0xff800000u;
     else w[k >> 1] = (k & 1) ? (w[k >> 1] & 0xffffu) | 0xff800000u : (w[k >> 1] & 0xffff0000u) | 0xff80u;
   }
+  // a bit for every value above `cut`, and whose bit it is (bf16 two at a time: the cut as the next bf16 value that is not above it)
+  static __device__ __forceinline__ int place(int bit) { return sizeof(T) == 4 ? bit : (bit & 15) * 2 + (bit >> 4); }
+  __device__ __forceinline__ uint32_t over(float cut) const {
+    static_assert(sizeof(T) == 4 || N == 32, "sixteen words of two");
+    uint32_t hits = 0u;
+    if (sizeof(T) == 4) {
+#pragma unroll
+      for (int k = 0; k < N; ++k) hits |= at(k) > cut ? 1u << k : 0u;
+    } else {
+      const __nv_bfloat162 c = __bfloat162bfloat162(__float2bfloat16_rd(cut));
+#pragma unroll
+      for (int j = 0; j < 4 * BS_VECS; ++j) hits |= __hgt2_mask(*reinterpret_cast<const __nv_bfloat162*>(&w[j]), c) & (0x10001u << j);
+    }
+    return hits;
+  }
   __device__ __forceinline__ float max() const {            // (NaN only where there is nothing else)
     if (sizeof(T) == 4) {
       float m = at(0);
@@ -290,12 +305,10 @@ __device__ __forceinline__ void beam_part(PartShared& sh, BeamStats* stats, uint
     };
     bool full = low_cut && more;
     if (cm > above) {
-      uint32_t hits = 0u;
-#pragma unroll
-      for (int k = 0; k < N; ++k) hits |= x.at(k) > above ? 1u << k : 0u;
+      uint32_t hits = x.over(above);
       uint32_t i = atomicAdd(&count, static_cast<uint32_t>(__popc(hits)));
       for (; hits; hits &= hits - 1u, ++i) {
-        if (i < BS_CAP) list[i] = keyed(__ffs(hits) - 1);
+        if (i < BS_CAP) list[i] = keyed(Held<T>::place(__ffs(hits) - 1));
         full |= i >= (more ? enough : BS_CAP);
       }
     }
