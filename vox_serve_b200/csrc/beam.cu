@@ -11,11 +11,13 @@
 // What orders candidates is computed in 64 bits from the parts' sums.  A sum's terms carry the special function unit's 2^-22 and, from one fp32 constant for log2 e,
 // 1.3e-8 of the distance from the maximum: below 2^-20 of a term that counts (distance up to 40).  Sums of parts meet through log2 e in two constants.
 //
-// Measured (a captured chain of calls, the parts alone in brackets): 16 requests of 16 beams over 156940 bf16 tokens, n 32, 31 us [23]; its 80 MB are 12.4 us of
-// HBM, and what is above that is the unevenness of 512 blocks on 148 SMs (three or four each: they end after 9 to 23 us), a meeting of the block for every chunk,
-// and the join (5: latencies).  16 of 5 over 32003 fp32 tokens, n 10: 12.5 us.  One of two over 2051: 5.9, most of it the launch.
+// Measured (a captured chain of calls): 16 requests of 16 beams over 156940 bf16 tokens, n 32, four fifths of them masked, 32 us, all of them open 41; the 80 MB are 12.4 us
+// of HBM.  What is above that: 512 blocks on 148 SMs, three or four each; 2.2 us a chunk of four blocks of an SM (its 64 KB are 1.3 of HBM, its exponentials 0.9 of the
+// special function unit; the rest are instructions and a meeting of the block), 8 to 13 of cuts, orders, launches and the join.  16 of 5 over 32003 fp32 tokens, n 10: 12.1 us.
+// One of two over 2051: 5.7, most of it the launch.
 // Four blocks an SM with two chunks in shared memory: 31.2 us; three with three 33.3, with four 32.6; four with three 34.4 (a list of 512); five with two 31.6.  Parts so
-// that all blocks run at once: more of them pay the first cut and the last order again, fewer leave SMs idle.
+// that all blocks run at once: more of them pay the first cut and the last order again, fewer leave SMs idle.  Lists are cut back once they hold twice what is wanted: open
+// rows 45.7 us, three times 46.6, four 47.2, at 256 53.7 (masked ones 32.6, 32.2, 32.1, 32.0).
 #include "../../include/vb_api.h"
 #define VB_PDL_FAMILY 16
 #include "rowmma.cuh"
@@ -29,8 +31,7 @@ constexpr int BS_MAX_N = 64, BS_MAX_W = 32;
 constexpr int BS_CLUSTER = 8;                                   // blocks of a request that join in the same launch
 static_assert(BS_CLUSTER * BS_MAX_N * 16 <= 16384, "the join's candidates stand where the ring stood");
 constexpr int BJ_BINS = 1024;                                   // 16 to a doubling, from 2^-23 to 2^41
-constexpr int BJ_FEW = 1024;
-constexpr int BJ_THREADS = 512, BJ_ALL = 8192;                  // candidates of a request: 128 KB of ranks and values
+constexpr int BJ_FEW = 512, BJ_ALL = 8192;                  // candidates of a request: 128 KB of ranks and values
 
 struct BeamStats {
   float m, s;
@@ -755,12 +756,14 @@ extern "C" int vb_beam_select(float* d_score, int32_t* d_parent, int64_t* d_toke
   if (logits_f32) VB_LAUNCH_PDL(beam_part_kernel<float>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, p);
   else VB_LAUNCH_PDL(beam_part_kernel<__nv_bfloat16>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, p);
   const size_t all = static_cast<size_t>(width) * parts * n;
+  // Fewer threads meet sooner, more get through longer lists.  256 / 512 threads: 80 to 320 candidates a request 8.2 / 8.9 and 12.1 / 12.8 us, 1024 42.2 / 41.1, 2560 14.7 /
+  // 12.8, 8192 30.1 / 22.5 (1024 threads: 14.3 for 2560, 22.3 for 8192).
   if (all <= BJ_FEW) {
-    VB_LAUNCH_PDL(beam_join_kernel<BS_THREADS>, static_cast<unsigned>(requests), BS_THREADS, all * 16, stream, p);
-    return 0;
+    VB_LAUNCH_PDL(beam_join_kernel<256>, static_cast<unsigned>(requests), 256, all * 16, stream, p);
+  } else {
+    VB_CHECK_CUDA(rm_smem<beam_join_kernel<512>>(BJ_ALL * 16));
+    VB_LAUNCH_PDL(beam_join_kernel<512>, static_cast<unsigned>(requests), 512, all * 16, stream, p);
   }
-  VB_CHECK_CUDA(rm_smem<beam_join_kernel<BJ_THREADS>>(BJ_ALL * 16));
-  VB_LAUNCH_PDL(beam_join_kernel<BJ_THREADS>, static_cast<unsigned>(requests), BJ_THREADS, all * 16, stream, p);
   return 0;
 }
 
@@ -792,6 +795,8 @@ extern "C" int vb_beam_reorder(void* const* states, const int64_t* row_bytes, in
     t.first[t.n] = static_cast<uint32_t>(blocks);
     VB_CHECK_ARG(blocks <= 0x7fffffffll, "vb_beam_reorder: %lld blocks", blocks);
     const dim3 grid(static_cast<unsigned>(blocks), requests);
+    // (a thread's registers hold its vector of every row: 8 requests of 8 rows 131 us, with room for 32 rows 503.  2 of 32 rows of 1 MB, 16 bytes a row at a time: 133;
+    // 8 bytes 166, 4 bytes 162.)
     if (width <= 4) VB_LAUNCH_PDL(beam_reorder_kernel<4>, grid, BR_THREADS, 0, stream, t, d_parent, d_slots, width);
     else if (width <= 8) VB_LAUNCH_PDL(beam_reorder_kernel<8>, grid, BR_THREADS, 0, stream, t, d_parent, d_slots, width);
     else if (width <= 16) VB_LAUNCH_PDL(beam_reorder_kernel<16>, grid, BR_THREADS, 0, stream, t, d_parent, d_slots, width);

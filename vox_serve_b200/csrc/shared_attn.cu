@@ -730,6 +730,7 @@ static int launch_shared(const SharedMaps& maps, const SharedAttnParams& p, int 
   const int units = p.groups * p.heads, m = p.sub * p.G;
   VB_CHECK_CUDA(rm_smem<shared_attn_kernel<D>>(SA_SMEM<D>));
   VB_LAUNCH_PDL(shared_attn_kernel<D>, grid, PTC_THREADS, SA_SMEM<D>, stream, maps, p);
+  // (eight warps a row where a unit has more than eight segments; one / eight warps: 4 units 51.2 / 35.5 us, 8 units 15.4 / 12.6, 64 38.5 / 40.5, 256 20.8 / 23.5)
   if (grid > 8 * units) VB_LAUNCH_PDL((shared_join_kernel<D, SJ_WARPS>), dim3(units, m), 32 * SJ_WARPS, 0, stream, p);
   else VB_LAUNCH_PDL((shared_join_kernel<D, 1>), dim3(units, (m + SJ_WARPS - 1) / SJ_WARPS), 32 * SJ_WARPS, 0, stream, p);
   return 0;
