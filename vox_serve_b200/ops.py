@@ -2256,7 +2256,8 @@ def _beam_select_check(logits, scores, n, weight, ended, end_token) -> None:
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, weight: Optional[torch.Tensor] = None, ended: Optional[torch.Tensor] = None,
                 end_token: Optional[int] = None) -> BeamStep:
     """One step of a beam search.  logits [requests * width, vocab] bf16 or fp32 (rows apart by any stride), scores fp32 [requests, width]: the beams' log probabilities so
-    far.  Of all continuations of a request's beams, total[w, v] = scores[w] + log_softmax(logits[w])[v], the n best in order, equal ones by (w, v).
+    far.  Of all continuations of a request's beams, total[w, v] = scores[w] + log_softmax(logits[w])[v], the n best in order, equal ones by (w, v).  Totals are 64-bit numbers;
+    where those do not tell a beam's candidates apart (scores or logits beyond 2^50), they are n of its largest logits.
 
     Logits that are not finite are masked: they are no candidates and have no part in the softmax.  A beam whose score is not finite (-inf: not alive yet, or dead), or that
     has no logit left, has no candidates.  ``weight`` fp32 [requests, width]: candidates are ranked by weight * total (length to the power -alpha, say; totals come back
