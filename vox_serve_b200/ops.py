@@ -2368,30 +2368,41 @@ class PagePool:
         _refuse(longer > 0, f"fork_pages: {longer} rows grew past {self.columns} pages")
 
 
+def _page_cache_check(who: str, t, pool: PagePool) -> None:
+    """raises if a cache does not fit the pool"""
+    _need_here(who, t)
+    s, P, n = t.shape, pool.page_size, pool.pages
+    _refuse(not t.is_contiguous() or t.numel() == 0, f"{who}: contiguous caches are needed, not {tuple(s)}")
+    whole = t.dim() == 6 and s[1] == n and s[2] == 2 and s[3] == P
+    _refuse(not whole and (t.dim() < 2 or s[0] != n), f"{who}: a cache of {n} pages of {P} tokens is needed: [layers, pages, 2, page, ...], [pages, 2, page, ...] or [pages, n, ...], not {tuple(s)}")
+    slot = t.nbytes // (s[0] * n * 2 * P if whole else n * 2 * P if t.dim() == 5 and s[1] == 2 and s[2] == P else n * s[1])
+    _refuse(slot % 16 != 0 or t.data_ptr() % 16 != 0, f"{who}: {slot} bytes a token of a cache (a multiple of 16, aligned to 16)")
+
+
 def _page_caches(who: str, caches, pool: PagePool):
     """VbPageCache of every cache: [layers, pages, 2, page, ...] or, of one layer, [pages, page, ...]; per page anything else [pages, n, ...] goes as a whole"""
-    out, seen = [], set()
+    P, n, dev, words, k = pool.page_size, pool.pages, pool._device, [], 0
     for t in caches:
-        _need_here(who, t)
-        s, P, n = t.shape, pool.page_size, pool.pages
-        _refuse(not t.is_contiguous() or t.numel() == 0, f"{who}: contiguous caches are needed, not {tuple(s)}")
-        if t.data_ptr() in seen:                       # (a cache that is both keys and values is one)
-            continue
-        seen.add(t.data_ptr())
-        if t.dim() == 6 and s[1] == n and s[2] == 2 and s[3] == P:
+        s, at, size, layers, parts, slots = t.shape, t.data_ptr(), t.nbytes, 1, 1, 0
+        d = len(s)
+        if d == 6 and s[1] == n and s[2] == 2 and s[3] == P:
             layers, parts, slots = s[0], 2, P
-        elif t.dim() == 5 and s[0] == n and s[1] == 2 and s[2] == P:
-            layers, parts, slots = 1, 2, P
-        else:
-            _refuse(t.dim() < 2 or s[0] != n, f"{who}: a cache of {n} pages of {P} tokens is needed: [layers, pages, 2, page, ...], [pages, 2, page, ...] or [pages, n, ...], not {tuple(s)}")
-            layers, parts, slots = 1, 1, s[1]
-        slot = t.numel() // (layers * n * parts * slots) * t.element_size()
-        _refuse(slot % 16 != 0 or t.data_ptr() % 16 != 0, f"{who}: {slot} bytes a token of a cache (a multiple of 16, aligned to 16)")
-        out.append((t.data_ptr(), slot, layers, parts, slots, 0))
-    return (_lib.PageCacheStruct * max(1, len(out)))(*out), len(out)
+        elif d == 5 and s[0] == n and s[1] == 2 and s[2] == P:
+            parts, slots = 2, P
+        elif d > 1 and s[0] == n:
+            slots = s[1]
+        slot = size // (layers * n * parts * slots) if size and slots else 0
+        if slot == 0 or slot % 16 or at % 16 or t.get_device() != dev or not t.is_contiguous():
+            _page_cache_check(who, t, pool)
+        if at not in words[::4]:                       # (a cache that is both keys and values is one)
+            words += (at, slot, layers | parts << 32, slots)
+            k += 1
+    return (_lib.PageCacheStruct * max(1, k)).from_buffer(array("q", words or (0, 0, 0, 0))), k
 
 
 def _pool_check(who: str, pool: PagePool, out: Optional[PagePool]) -> PagePool:
+    if out is None and pool._device == _device_index():
+        return pool
     out = pool if out is None else out
     _refuse(pool._device < 0 or pool._device != _device_index() or out._device != pool._device, f"{who}: pools on the current device are needed")
     _refuse((pool.pages, pool.page_size, pool.rows, pool.columns) != (out.pages, out.page_size, out.rows, out.columns), f"{who}: out is a pool of another size")
@@ -2412,23 +2423,26 @@ def fork_pages(pool: PagePool, src: Optional[torch.Tensor] = None, grow: Union[i
     left out loses those tokens for the copies.  Free pages are given out lowest number first.  If pages or columns run short nothing changes, and ``check`` of the pool
     that was written raises.  ``out``: a pool of the same size that is written instead (it has tables of its own; the caches are one)."""
     out = _pool_check("fork_pages", pool, out)
-    by, g_ptr, g_all = 0, None, 0
+    by, g_ptr, g_all, rows = 0, None, 0, pool.rows
     if src is not None:
-        _need_here("fork_pages", src)
-        _refuse(src.dtype is not torch.int32 or not src.is_contiguous() or src.numel() != pool.rows or src.dim() not in (1, 2), f"fork_pages: int32 sources of {pool.rows} rows are needed")
-        by = src.shape[1] if src.dim() == 2 else 0
+        z = src.shape
+        by = z[1] if len(z) == 2 else 0
+        if not (src.get_device() == pool._device and src.dtype is torch.int32 and src.is_contiguous() and (z[0] * by if by else len(z) == 1 and z[0]) == rows):
+            _need_here("fork_pages", src)
+            _refuse(src.dtype is not torch.int32 or not src.is_contiguous() or src.numel() != rows or src.dim() not in (1, 2), f"fork_pages: int32 sources of {rows} rows are needed")
     if group is not None:
-        _refuse(group < 1 or pool.rows % group != 0 or by not in (0, group), f"fork_pages: {pool.rows} rows in groups of {group}")
+        _refuse(group < 1 or rows % group != 0 or by not in (0, group), f"fork_pages: {rows} rows in groups of {group}")
         by = group
     if isinstance(grow, torch.Tensor):
         _need_here("fork_pages", grow)
-        _refuse(grow.dtype is not torch.int32 or tuple(grow.shape) != (pool.rows,) or not grow.is_contiguous(), f"fork_pages: room is a number or int32 [{pool.rows}]")
+        _refuse(grow.dtype is not torch.int32 or tuple(grow.shape) != (rows,) or not grow.is_contiguous(), f"fork_pages: room is a number or int32 [{rows}]")
         g_ptr = grow.data_ptr()
     else:
         g_all = int(grow)
-        _refuse(not 0 <= g_all <= 0x3fffffff, f"fork_pages: room for {g_all} more tokens")
+        if not 0 <= g_all <= 0x3fffffff:
+            _refuse(True, f"fork_pages: room for {g_all} more tokens")
     c, n = _page_caches("fork_pages", caches, pool)
-    call("vb_fork_pages", pool._ptr, out._ptr, _p(src), by, g_ptr, g_all, ctypes.addressof(c), n, _stream())
+    call("vb_fork_pages", pool._ptr, out._ptr, None if src is None else src.data_ptr(), by, g_ptr, g_all, ctypes.addressof(c), n, _raw_stream(pool._device))
     _lib.launch_counter[0] += (n + 31) // 32
     return out
 
@@ -2438,7 +2452,7 @@ def compact_pages(pool: PagePool, caches: Sequence[torch.Tensor] = (), out: Opti
     ``fork_pages``), tables and counts.  ``moved`` int32 [pages] of the pool that is written: a page's new number, -1 where it was free; ``status[3]``: U."""
     out = _pool_check("compact_pages", pool, out)
     c, n = _page_caches("compact_pages", caches, pool)
-    call("vb_compact_pages", pool._ptr, out._ptr, ctypes.addressof(c), n, _stream())
+    call("vb_compact_pages", pool._ptr, out._ptr, ctypes.addressof(c), n, _raw_stream(pool._device))
     _lib.launch_counter[0] += (n + 31) // 32
     return out
 
