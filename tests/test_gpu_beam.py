@@ -320,3 +320,49 @@ def test_everything_at_once(V, dtype):
     z[::2, V // 2:] = torch.finfo(dtype).min
     z[1::2, :V // 3] = -INF
     _check(ops.beam_select(z, s, n, weight=weight, ended=ended, end_token=end), z, s, n, weight, ended, end)
+
+
+def _row_of_top(top, V, dtype, kind):
+    """fp32 row whose largest value is ``top``: alone in its thread's share of the row, everywhere, or above values that 64 bits tell apart beside it"""
+    t = torch.tensor(top, dtype=F32, device="cuda")
+    if kind == "alone":
+        z = torch.full((V,), -INF, device="cuda")
+        z[V // 3] = t
+    elif kind == "equal":
+        z = torch.full((V,), top, device="cuda")
+    else:
+        z = t - t.abs() * (torch.arange(V, device="cuda").roll(V // 2) % 977) / 1024
+    return z.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("kind", ["alone", "equal", "lower"])
+def test_large_logits(kind, dtype):
+    """a maximum whose product with log2 e is rounded by up to 2^127: no term is lost, of either sign, at any size"""
+    V, n = 2500, 12
+    tops = [1600008448.0, 2000003840.0, 2500027136.0, 4000063488.0, 1073741760.0, 1073741824.0, 1488522240.0, 1.4e9] + [float(10 ** k) for k in range(3, 37)]
+    tops = [x for t in tops for x in (t, -t)]
+    z = torch.stack([_row_of_top(t, V, dtype, kind) for t in tops])
+    s = torch.full((len(tops) // 2, 2), -1.5, device="cuda")
+    s[:, 1] = -2.0
+    step = ops.beam_select(z, s, n)
+    _check(step, z, s, n)
+    one = s.view(-1, 1)                                     # each row as a request of its own
+    step = ops.beam_select(z, one, n)
+    _check(step, z, one, n)
+    assert bool((step.parent[:, 0] == 0).all())
+
+
+def test_every_size_of_a_single_logit():
+    """one open token a row: its total is the row's score, whatever the logit"""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    e = torch.rand(20000, generator=g, device="cuda", dtype=F64) * 126 * (1 - 2 * (torch.arange(20000, device="cuda") % 2))
+    x = torch.exp2(e).to(F32) * torch.where(torch.rand(20000, generator=g, device="cuda") < 0.5, -1.0, 1.0)
+    near = torch.exp2(29.5 + 5.0 * torch.rand(20000, generator=g, device="cuda", dtype=F64)).to(F32)
+    x = torch.cat([x, near, -near])
+    s = -40.0 * torch.rand(x.numel(), 1, generator=g, device="cuda")
+    z = torch.full((x.numel(), 9), -INF, device="cuda")
+    z[:, 4] = x
+    step = ops.beam_select(z, s, 1)
+    assert bool((step.token == 4).all()) and bool((step.parent == 0).all())
+    assert bool(((step.scores - s).abs() <= 2.0 ** -18 + 2.0 ** -23 * s.abs()).all())

@@ -55,6 +55,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
   asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}" : "=f"(d.x), "=f"(d.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
   return d;
 }
+constexpr float BS_SHORT = 1073741824.f;                        // maxima up to which a thread's sum takes the short way
 constexpr float LOG2E = 1.44269502f, LOG2E_REST = 1.92596303e-8f;
 // e^d, d <= 0: log2 e in two parts, so that the product's rounding (2^-24 of the exponent) is the only error and has no common sign
 __device__ __forceinline__ float exp_down(float d) { return ex2(fmaf(d, LOG2E, d * LOG2E_REST)); }
@@ -233,7 +234,8 @@ __device__ __forceinline__ void beam_part(PartShared& sh, BeamStats* stats, uint
         if (token(k) >= static_cast<uint32_t>(V)) x.mask(k);
     }
     // Maximum and sum of exponentials of what the thread holds.  One product and sum an element: 2^(x log2 e - c) with c the rounded m log2 e, and what the
-    // rounding took is put back into the sum.  What is not finite shows up in the maximum or the sum and is masked then; huge values take the longer way.
+    // rounding took is put back into the sum.  That is at most half a step of c, 64 below |m| = 2^30 (c < 2^31): neither factor is flushed there.  From 2^30 on (fp32 logits
+    // lost their whole sum from 1.49e9 on) the longer way.  What is not finite shows up in the maximum or the sum and is masked on that way.
     float cm = x.max(), cs = 0.f;
     if (!(cm >= -INFINITY)) cm = -INFINITY;                  // (NaN alone)
     if (cm != -INFINITY) {
@@ -245,7 +247,7 @@ __device__ __forceinline__ void beam_part(PartShared& sh, BeamStats* stats, uint
         t[(k >> 1) & 1] = add2(t[(k >> 1) & 1], make_float2(ex2(y.x), ex2(y.y)));
       }
       cs = ((t[0].x + t[0].y) + (t[1].x + t[1].y)) * ex2(fmaf(-cm, LOG2E, c));
-      if (!(cs < INFINITY) || !(fabsf(cm) < 1e37f)) {
+      if (!(cs < INFINITY) || !(fabsf(cm) < BS_SHORT)) {
 #pragma unroll
         for (int k = 0; k < N; ++k)
           if (!isfinite(x.at(k))) x.mask(k);
