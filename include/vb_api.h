@@ -955,17 +955,20 @@ int vb_beam_reorder(void* const* states, const int64_t* row_bytes, int n_states,
                     void* stream);
 /* Page tables on the device (csrc/pages.cu).  VbPagePool (HOST struct): table [rows][columns] page numbers (-1 behind a row's last), tokens [rows], refs [pages] rows
  *   that hold a page, status [4] {pages that were missing, rows that grew past their columns, copies, pages in use}, copies [max(rows, pages)][3] {page, page,
- *   tokens}, moved [pages], scratch of vb_page_pool_scratch_bytes.  A page that is not full belongs to one row.
+ *   tokens}, moved [pages], scratch of vb_page_pool_scratch_bytes, live [rows] (or NULL) what a step may see of its rows: tokens, or 0 for all of them while a
+ *   shortage stands.  A page that is not full belongs to one row.  All zero at first, the table -1.
  * VbPageCache (HOST struct): data [layers][pages][parts][slots][slot_bytes], 16-byte aligned, slot_bytes a multiple of 16.
  * vb_fork_pages: row i of `out` continues row src[i] of `pool` (NULL: itself; < 0: none, its pages are given back; group > 0: counted within the row's group of so
  *   many rows) and gets room for grow[i] (NULL: grow) more tokens.  Of the rows that take over a page that is not full the first keeps it, the others get copies
  *   of its tokens in all caches.  Free pages: lowest number first, rows in order, a row's copy first.  If pages or columns run short, out = pool and status says how
- *   many.  out may be pool.  A page that falls free in the step may be given out in it.
+ *   many; while status [0] or [1] of `pool` is not 0 every call leaves the pool as it is and hands the two words on.  The caller clears them.  out may be pool.  A page that
+ *   falls free in the step may be given out in it.
  * vb_compact_pages: with U pages in use those numbered U and above move to the free ones below U, in order, contents and all; moved[page] is a page's new number, -1
- *   where it was free. */
+ *   where it was free.  A shortage stands on. */
 typedef struct {
   int32_t *d_table, *d_tokens, *d_refs, *d_status, *d_copies, *d_moved, *d_scratch;
   int32_t pages, page_size, rows, columns;
+  int32_t* d_live;
 } VbPagePool;
 typedef struct {
   void* data;

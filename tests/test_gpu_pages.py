@@ -290,3 +290,79 @@ def test_captured_steps():
             torch.cuda.synchronize()
             assert plain.step(s, n)
             plain.same_as(pool, caches)
+
+
+@pytest.mark.parametrize("apart", [False, True])
+def test_a_shortage_stays_until_it_is_asked_for(apart):
+    """steps behind one that ran short change nothing, though they could go on; rows have no tokens to see meanwhile; compacting does not forget it"""
+    plain, pool, caches = _make(10, 16, 4, 8)
+    other = ops.PagePool(10, 16, 4, 8)
+
+    def turn(f):
+        nonlocal pool, other
+        out = f(pool, other if apart else pool)
+        if apart:
+            pool, other = other, pool
+        return out
+    assert plain.step([0, 1, 2, 3], [20, 32, 5, 0])
+    turn(lambda a, out: ops.fork_pages(a, grow=_i32([20, 32, 5, 0]), out=out))
+    assert torch.equal(pool.live, pool.tokens)
+    for src, grow in (([0, 0, 0, 0], [40] * 4), ([0, 1, 2, 3], [1] * 4), ([0, 1, -1, -1], [0] * 4), ([0, 1, 2, 3], [8 * 16 + 1, 0, 0, 0])):
+        turn(lambda a, out: ops.fork_pages(a, _i32(src), _i32(grow), caches=caches, out=out))
+        plain.same_as(pool, caches)
+        assert pool.status[:3].tolist() == [3, 0, 0] and not bool(pool.live.any())      # 3 copies and 8 pages, of which 8 are free
+    plain.compact()
+    turn(lambda a, out: ops.compact_pages(a, caches, out=out))
+    plain.same_as(pool, caches)
+    assert not bool(pool.live.any())
+    with pytest.raises(VoxB200Error, match="3 pages are missing"):
+        pool.check()
+    assert torch.equal(pool.live, pool.tokens)
+    pool.check()
+    assert plain.step([0, 1, 1, -1], [1] * 4)
+    turn(lambda a, out: ops.fork_pages(a, _i32([0, 1, 1, -1]), 1, caches=caches, out=out))
+    pool.check()
+    plain.same_as(pool, caches)
+    assert torch.equal(pool.live, pool.tokens)
+    # rows that outgrow their columns stay said too
+    turn(lambda a, out: ops.fork_pages(a, grow=_i32([0, 8 * 16, 0, 0]), out=out))
+    turn(lambda a, out: ops.fork_pages(a, grow=_i32([0, 0, 0, 0]), out=out))
+    with pytest.raises(VoxB200Error, match="1 rows grew past 8 pages"):
+        pool.check()
+    plain.same_as(pool, caches)
+    # other tables begin anew
+    turn(lambda a, out: ops.fork_pages(a, grow=4000, out=out))
+    pool.load(pool.table.clone(), pool.tokens.clone())
+    pool.check()
+    assert torch.equal(pool.live, pool.tokens)
+
+
+@pytest.mark.parametrize("rows,columns,pages", [(64, 700, 9000), (300, 90, 400)])
+def test_live_rows_of_large_tables(rows, columns, pages):
+    """several blocks, counts in shared memory and not: live is tokens, and 0 everywhere once a step has run short"""
+    plain, pool, caches = _make(pages, 2, rows, columns, kinds=())
+    grow = [(i * 7) % 3 for i in range(rows)]
+    assert plain.step(list(range(rows)), grow)
+    ops.fork_pages(pool, grow=_i32(grow))
+    assert pool.live.tolist() == plain.tokens
+    ops.fork_pages(pool, grow=columns * 2)
+    ops.fork_pages(pool, grow=0)
+    plain.same_as(pool, caches)
+    assert not bool(pool.live.any())
+    with pytest.raises(VoxB200Error):
+        pool.check()
+
+
+def test_pools_of_a_c_caller_without_live_rows():
+    import ctypes
+
+    from vox_serve_b200 import _lib
+    plain, pool, caches = _make(10, 16, 4, 8, kinds=())
+    s = _lib.PagePoolStruct.from_buffer_copy(pool._struct)
+    s.d_live = None
+    pool.live.fill_(77)
+    ops.call("vb_fork_pages", ctypes.addressof(s), ctypes.addressof(s), None, 0, None, 5, None, 0, torch.cuda.current_stream().cuda_stream)
+    ops.call("vb_compact_pages", ctypes.addressof(s), ctypes.addressof(s), None, 0, torch.cuda.current_stream().cuda_stream)
+    assert plain.step([0, 1, 2, 3], [5] * 4)
+    plain.same_as(pool, caches)
+    assert bool((pool.live == 77).all())

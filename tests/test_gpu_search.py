@@ -249,3 +249,49 @@ def test_with_adapters():
     assert bool(((logits[0] - logits[1]).abs() <= 2e-2 * logits[1].abs().max()).all())
     bare = s.forward().float()
     assert float((bare[0] - logits[0][0]).abs().max()) > float((bare[1] - logits[0][1]).abs().max())      # (the adapter of row 0 is there)
+
+
+class LiveSearch(Search):
+    """lengths of a step from the pool's live rows"""
+
+    def forward(self, shared=True):
+        ops, live = self.ops, self.pool.live
+        ops.plan_rows(self.eng.plan, None, self.pool.indptr, self.pool.table.view(-1), None, self.rows, self.rows, PAGE, self.eng.chunk, kv_len=live)
+        if shared:
+            ops.shared_plan(self.plan, self.pool.table, live, PAGES)
+        return self.eng.forward(self.ids, live - 1, self.rows, shared=self.plan if shared else None)
+
+
+@pytest.mark.parametrize("shared", [True, False])
+def test_a_captured_loop_that_runs_short_in_the_middle(shared):
+    """from the step on that found too few pages, tables and cache hold what they held, though pages come free again behind it; and it is said at the end"""
+    s = LiveSearch()
+    s.start()
+    s.choose(s.forward(shared))
+    g = torch.cuda.CUDAGraph()
+    s.choose(s.forward(shared))
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        s.choose(s.forward(shared))
+    s.pool.check()
+    others = s.pool.refs == 0
+    others[torch.nonzero(others)[:3].view(-1)] = False      # three pages are left, the others somebody else's
+    s.pool.refs[others] = 1
+    kept = None
+    for k in range(26):
+        g.replay()
+        torch.cuda.synchronize()
+        if kept is None and bool(s.pool.status[:2].any()):
+            kept = [t.clone() for t in (s.kv, s.pool.table, s.pool.tokens)]
+            s.pool.refs[others] = 0                          # (pages come free: the next step would find enough)
+            assert 2 < k < 20
+    assert kept is not None and not bool(s.pool.live.any())
+    for t, was in zip((s.kv, s.pool.table, s.pool.tokens), kept):
+        assert torch.equal(t, was)
+    with pytest.raises(s.ops.VoxB200Error, match="pages are missing"):
+        s.pool.check()
+    s.ops.check_waits()
+    g.replay()                                               # (asked for: it goes on)
+    torch.cuda.synchronize()
+    s.pool.check()
+    assert torch.equal(s.pool.tokens, kept[2] + 1) and torch.equal(s.pool.live, s.pool.tokens)

@@ -213,3 +213,19 @@ def test_entry_points_check_by_themselves():
     assert lib.vb_fork_pages(p, p, None, 3, None, 0, None, 0, None) != 0
     shared = _lib.PagePoolStruct(at, at + 64, at, at, at, at, at, 4, 16, 2, 2)
     assert lib.vb_fork_pages(p, ctypes.addressof(shared), None, 0, None, 0, None, 0, None) != 0 and b"share" in lib.vb_last_error()
+
+
+def test_a_shortage_is_said_once():
+    pool = ops.PagePool(6, 4, 3, 3, device="cpu")
+    assert pool.live.shape == (3,) and not bool(pool.live.any())
+    pool.load(torch.tensor([[5, 1, -1], [2, -1, -1], [-1, -1, -1]], dtype=I32), torch.tensor([5, 4, 0], dtype=I32))
+    assert pool.live.tolist() == [5, 4, 0]
+    pool.status[0], pool.status[2] = 2, 7
+    pool.live.zero_()
+    with pytest.raises(VoxB200Error, match="2 pages are missing"):
+        pool.check()
+    assert pool.status.tolist() == [0, 0, 7, 0] and pool.live.tolist() == [5, 4, 0]
+    pool.check()
+    pool.status[1] = 1
+    pool.load(pool.table.clone(), pool.tokens.clone())
+    pool.check()

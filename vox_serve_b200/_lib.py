@@ -254,7 +254,7 @@ class MoeRouterStruct(C.Structure):
 
 class PagePoolStruct(C.Structure):
     """VbPagePool"""
-    _fields_ = [(n, P) for n in ("d_table", "d_tokens", "d_refs", "d_status", "d_copies", "d_moved", "d_scratch")] + [(n, C.c_int32) for n in ("pages", "page_size", "rows", "columns")]
+    _fields_ = [(n, P) for n in ("d_table", "d_tokens", "d_refs", "d_status", "d_copies", "d_moved", "d_scratch")] + [(n, C.c_int32) for n in ("pages", "page_size", "rows", "columns")] + [("d_live", P)]
 
 
 class PageCacheStruct(C.Structure):

@@ -6,7 +6,8 @@
 // kernel that copies what it listed, in all layers of all caches.
 //
 // Free pages are given out lowest number first, to rows in their order, to a row first the page for a copy.  All or nothing: if pages or columns run short
-// nothing changes and the status says so.
+// nothing changes and the status says so: that stays, and the pool as it is, until the caller has cleared those words, so that a loop that never asks cannot lose
+// it.  Meanwhile `live` tells the kernels behind a step that its rows have no tokens: nothing is appended, nothing read.
 //
 // What bounds it: the tables a chain of dependent loads and meetings (a step of 64 rows 7 us, a chain of such steps; 16 continuations of a prompt of 8000 tokens 8),
 // the contents HBM: tails of a step, 57 MB, 10 us beside a floor of 8.9; 140 pages of 2.1 MB
@@ -47,6 +48,8 @@ struct ForkParams {
   const int32_t *table, *tokens, *refs;              // the pool as it is
   int32_t *out_table, *out_tokens, *out_refs;        // as it becomes (may be the same)
   int32_t *status, *copies, *work, *free;            // of the pool that is written: copies [rows][3]; scratch work / free [pages], where these are not in shared memory
+  const int32_t* was;                                // status of the pool as it is
+  int32_t* live;                                     // of the pool that is written, or null: tokens, 0 while it is short
   const int32_t *src, *grow;                         // row that every row continues (null: itself; < 0: none), tokens it gets room for (null: grow_all)
   int rows, columns, pages, page_size, group, grow_all, in_smem;
 };
@@ -106,6 +109,7 @@ __global__ void __launch_bounds__(THREADS, 1) fork_pages_kernel(const __grid_con
   volatile int32_t* base = in_block0(s_base);
   pdl_sync();
   const int ref = mine < p.pages ? p.refs[mine] : 0;      // (all loads of the start at once)
+  const int was_missing = p.was[PS_MISSING], was_long = p.was[PS_LONG];      // an earlier step's: the pool has stood still since
   for (int i = tid; i < p.rows; i += THREADS) {
     const int s = fork_source(p, i), n = fork_tokens(p, i), g = p.grow ? p.grow[i] : p.grow_all;
     s_src[i] = s, s_grow[i] = g > 0 ? g : 0, s_tok[i] = n, s_held[i] = (n + P - 1) / P, s_heirs[i] = 0, s_keeper[i] = 0x7fffffff, s_tail[i] = -1;
@@ -175,7 +179,7 @@ __global__ void __launch_bounds__(THREADS, 1) fork_pages_kernel(const __grid_con
         }
       have += total.x;
     }
-    const bool ok = have >= need_all && too_long == 0;
+    const bool stands = was_missing != 0 || was_long != 0, ok = !stands && have >= need_all && too_long == 0;
     __syncthreads();
     if (ok) {
       for (int k = tid; k < need_all; k += THREADS) work[free[k]] = 1;
@@ -189,8 +193,8 @@ __global__ void __launch_bounds__(THREADS, 1) fork_pages_kernel(const __grid_con
     }
     if (tid == 0) {
       s_ok = ok;
-      p.status[PS_MISSING] = have >= need_all ? 0 : need_all - have;
-      p.status[PS_LONG] = too_long;
+      p.status[PS_MISSING] = stands ? was_missing : have >= need_all ? 0 : need_all - have;
+      p.status[PS_LONG] = stands ? was_long : too_long;
       p.status[PS_COPIES] = ok ? s_copies : 0;
     }
   }
@@ -237,6 +241,11 @@ __global__ void __launch_bounds__(THREADS, 1) fork_pages_kernel(const __grid_con
       p.out_tokens[i] = !ok ? ldcg(p.tokens + i) : s < 0 ? 0 : s_tok[s] + s_grow[i];
     }
   }
+  if (p.live)
+    for (int i = mine; i < p.rows; i += all) {
+      const int s = ok ? s_src[i] : -1;
+      p.live[i] = s < 0 ? 0 : s_tok[s] + s_grow[i];
+    }
   if (blocks > 1) cluster_sync_all();                // (block 0's shared memory is read to the end)
 }
 
@@ -244,6 +253,8 @@ struct CompactParams {
   const int32_t *table, *tokens, *refs;
   int32_t *out_table, *out_tokens, *out_refs, *moved;        // moved [pages]: a page's new number, -1: not in use
   int32_t *status, *copies;                                  // copies [pages][3]
+  const int32_t* was;                                        // status of the pool as it is
+  int32_t* live;                                             // (as for ForkParams)
   int32_t *from, *to;                                        // scratch [pages]
   long long cells;
   int rows, pages, page_size;
@@ -297,7 +308,7 @@ __global__ void __launch_bounds__(THREADS, 1) compact_pages_kernel(const __grid_
       int32_t* c = p.copies + 3ll * k;
       c[0] = from, c[1] = to, c[2] = p.page_size;
     }
-    if (tid == 0) p.status[PS_MISSING] = p.status[PS_LONG] = 0, p.status[PS_COPIES] = movers, p.status[PS_USED] = used;
+    if (tid == 0) p.status[PS_COPIES] = movers, p.status[PS_USED] = used;
   }
   cluster_sync_all();
   const long long at = static_cast<long long>(rank) * THREADS + tid, step = static_cast<long long>(blocks) * THREADS;
@@ -305,7 +316,13 @@ __global__ void __launch_bounds__(THREADS, 1) compact_pages_kernel(const __grid_
     const int g = p.table[e];
     p.out_table[e] = g >= 0 && g < p.pages ? ldcg(p.moved + g) : g;
   }
-  for (long long i = at; i < p.rows; i += step) p.out_tokens[i] = p.tokens[i];
+  const int was_missing = p.was[PS_MISSING], was_long = p.was[PS_LONG];
+  if (at == 0 && p.status != p.was) p.status[PS_MISSING] = was_missing, p.status[PS_LONG] = was_long;      // (a shortage stands until it is cleared)
+  for (long long i = at; i < p.rows; i += step) {
+    const int n = p.tokens[i];
+    p.out_tokens[i] = n;
+    if (p.live) p.live[i] = was_missing != 0 || was_long != 0 ? 0 : n;
+  }
   const int movers = ldcg(p.status + PS_COPIES), used = ldcg(p.status + PS_USED);
   if (p.out_refs != p.refs)
     for (long long g = at; g < p.pages; g += step)
@@ -436,7 +453,7 @@ extern "C" int vb_fork_pages(const VbPagePool* pool, const VbPagePool* out, cons
   ForkParams p = {};
   p.table = pool->d_table, p.tokens = pool->d_tokens, p.refs = pool->d_refs;
   p.out_table = out->d_table, p.out_tokens = out->d_tokens, p.out_refs = out->d_refs;
-  p.status = out->d_status, p.copies = out->d_copies;
+  p.status = out->d_status, p.copies = out->d_copies, p.was = pool->d_status, p.live = out->d_live;
   p.work = out->d_scratch, p.free = p.work + pool->pages, p.in_smem = pool->pages <= PG_SMEM_PAGES;
   p.src = d_src, p.grow = d_grow, p.grow_all = grow;
   p.rows = pool->rows, p.columns = pool->columns, p.pages = pool->pages, p.page_size = pool->page_size, p.group = group;
@@ -455,7 +472,7 @@ extern "C" int vb_compact_pages(const VbPagePool* pool, const VbPagePool* out, c
   CompactParams p = {};
   p.table = pool->d_table, p.tokens = pool->d_tokens, p.refs = pool->d_refs;
   p.out_table = out->d_table, p.out_tokens = out->d_tokens, p.out_refs = out->d_refs, p.moved = out->d_moved;
-  p.status = out->d_status, p.copies = out->d_copies;
+  p.status = out->d_status, p.copies = out->d_copies, p.was = pool->d_status, p.live = out->d_live;
   p.from = out->d_scratch, p.to = p.from + pool->pages;
   p.rows = pool->rows, p.pages = pool->pages, p.page_size = pool->page_size;
   p.cells = static_cast<long long>(pool->rows) * pool->columns;

@@ -2325,31 +2325,32 @@ def beam_reorder(states: Sequence[torch.Tensor], parent: torch.Tensor, slots: Op
 
 class PagePool:
     """Page tables of a paged cache on the device: ``table`` int32 [rows, columns] (-1 behind a row's last page), ``tokens`` int32 [rows], ``refs`` int32 [pages]: how many rows hold a
-    page, 0: free.  All rows are empty and all pages free at first.  ``fork_pages`` and ``compact_pages`` work on it without the host; ``check`` asks how the last one went.
+    page, 0: free.  All rows are empty and all pages free at first.  ``fork_pages`` and ``compact_pages`` work on it without the host; ``check`` asks whether pages ran short.
 
-    For ``plan_rows`` a pool is a page table of ``columns`` pages a row: kv_indptr = ``indptr``, kv_indices = ``table`` in one dimension, kv_len = ``tokens``.  A
-    page that is not full belongs to one row; a program that writes the tables itself (``load``) keeps to that.  A pool belongs to one stream at a time."""
+    For ``plan_rows`` a pool is a page table of ``columns`` pages a row: kv_indptr = ``indptr``, kv_indices = ``table`` in one dimension, kv_len = ``live``.  ``live`` int32 [rows] is
+    ``tokens``, or 0 for every row from a step that ran short on until ``check`` has said so: what reads lengths from it then appends nothing and attends to nothing, and the
+    cache stays as it was.  A page that is not full belongs to one row; a program that writes the tables itself (``load``) keeps to that.  A pool belongs to one stream at a time."""
 
     def __init__(self, pages: int, page_size: int, rows: int, columns: int, device="cuda"):
         _refuse(pages < 1 or page_size < 1 or not 1 <= rows <= 4096 or columns < 1 or columns * page_size > 0x3fffffff or (columns + 1) * rows > 0x3fffffff,
                 f"PagePool: {pages} pages of {page_size} tokens, {rows} rows (1 to 4096) of {columns} columns")
         self.pages, self.page_size, self.rows, self.columns = int(pages), int(page_size), int(rows), int(columns)
-        n = [rows * columns, rows, pages, 4, 3 * max(rows, pages), pages, 2 * pages]
+        n = [rows * columns, rows, pages, 4, 3 * max(rows, pages), pages, 2 * pages, rows]
         self._buf = torch.zeros(sum((k + 3) // 4 * 4 for k in n), dtype=torch.int32, device=device)
         parts, at = [], 0
         for k in n:
             parts.append(self._buf[at:at + k])
             at += (k + 3) // 4 * 4
-        self.table, self.tokens, self.refs, self.status, self.copies, self.moved, scratch = parts
+        self.table, self.tokens, self.refs, self.status, self.copies, self.moved, scratch, self.live = parts
         self.table = self.table.view(rows, columns)
         self.table.fill_(-1)
         self.indptr = torch.arange(0, (rows + 1) * columns, columns, dtype=torch.int32, device=device)
         self._struct = _lib.PagePoolStruct(*(t.data_ptr() for t in (self.table, self.tokens, self.refs, self.status, self.copies, self.moved, scratch)),
-                                           self.pages, self.page_size, self.rows, self.columns)
+                                           self.pages, self.page_size, self.rows, self.columns, self.live.data_ptr())
         self._ptr, self._device = ctypes.addressof(self._struct), self._buf.get_device()
 
     def load(self, table: torch.Tensor, tokens: torch.Tensor) -> "PagePool":
-        """tables that exist already: int32 [rows, columns] and [rows]; ``refs`` is counted from them"""
+        """tables that exist already: int32 [rows, columns] and [rows]; ``refs`` is counted from them, a shortage of the tables before is over"""
         _refuse(tuple(table.shape) != (self.rows, self.columns) or tuple(tokens.shape) != (self.rows,), f"PagePool.load: a table [{self.rows}, {self.columns}] is needed")
         self.table.copy_(table)
         self.tokens.copy_(tokens)
@@ -2359,11 +2360,17 @@ class PagePool:
         count = torch.zeros(self.pages + 1, dtype=torch.int32, device=self.table.device).index_add_(0, at, torch.ones_like(at, dtype=torch.int32))
         self.refs.copy_(count[:self.pages])
         self.table.masked_fill_(~on, -1)
+        self.status[:2].zero_()
+        self.live.copy_(self.tokens)
         return self
 
     def check(self) -> None:
-        """Raises if the last ``fork_pages`` found too few pages or columns (it changed nothing then).  Waits for it."""
+        """Raises if a ``fork_pages`` found too few pages or columns since the last ``check``: the tables are those before that step (it and all behind it changed nothing),
+        and go on from there.  Waits for the last one."""
         missing, longer = self.status[:2].tolist()
+        if missing or longer:
+            self.status[:2].zero_()
+            self.live.copy_(self.tokens)
         _refuse(missing > 0, f"fork_pages: {missing} pages are missing (of {self.pages})")
         _refuse(longer > 0, f"fork_pages: {longer} rows grew past {self.columns} pages")
 
@@ -2420,8 +2427,9 @@ def fork_pages(pool: PagePool, src: Optional[torch.Tensor] = None, grow: Union[i
 
     Pages are shared, not copied, but for one that is not full yet: of the rows that take it over the first keeps it, the others get copies of the tokens in it, in every one of
     ``caches``: [layers, pages, 2, page, ...], [pages, 2, page, ...], or of one layer [pages, page, ...]; [pages, n, ...] with another n goes as a whole page.  A cache that is
-    left out loses those tokens for the copies.  Free pages are given out lowest number first.  If pages or columns run short nothing changes, and ``check`` of the pool
-    that was written raises.  ``out``: a pool of the same size that is written instead (it has tables of its own; the caches are one)."""
+    left out loses those tokens for the copies.  Free pages are given out lowest number first.  If pages or columns run short nothing changes, in this call and in all behind it,
+    until ``check`` of the pool that was written has raised; ``live`` is 0 meanwhile.  What else followed the step (``beam_reorder``, scores) has moved on: a program that means to
+    go on calls ``check`` in front of that.  ``out``: a pool of the same size that is written instead (it has tables of its own; the caches are one)."""
     out = _pool_check("fork_pages", pool, out)
     by, g_ptr, g_all, rows = 0, None, 0, pool.rows
     if src is not None:
