@@ -366,3 +366,20 @@ def test_pools_of_a_c_caller_without_live_rows():
     assert plain.step([0, 1, 2, 3], [5] * 4)
     plain.same_as(pool, caches)
     assert bool((pool.live == 77).all())
+
+
+@pytest.mark.parametrize("first", [0, 1])
+def test_a_layer_beside_the_stack_it_begins(first):
+    """all layers follow, whichever of the two stands in front"""
+    plain, pool, caches = _make(20, 16, 4, 3, kinds=("kv",))
+    both = [caches[0], caches[0][0]] if first else [caches[0][0], caches[0]]
+    assert plain.step([0, 1, 2, 3], [21, 3, 0, 40])
+    ops.fork_pages(pool, grow=_i32([21, 3, 0, 40]))
+    assert plain.step([0, 0, 1, -1], [1] * 4)
+    ops.fork_pages(pool, _i32([0, 0, 1, -1]), 1, caches=both)
+    plain.same_as(pool, caches)
+    assert plain.step([-1, 1, 2, -1], [0] * 4)
+    ops.fork_pages(pool, _i32([-1, 1, 2, -1]), 0, caches=both)
+    plain.compact()
+    ops.compact_pages(pool, caches=both)
+    plain.same_as(pool, caches)

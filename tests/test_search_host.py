@@ -229,3 +229,14 @@ def test_a_shortage_is_said_once():
     pool.status[1] = 1
     pool.load(pool.table.clone(), pool.tokens.clone())
     pool.check()
+
+
+def test_caches_that_begin_at_one_address(launched):
+    """the same cache twice is one; one that is longer, or has other slots, is another, whichever comes first"""
+    pool = _pool()
+    kv = torch.zeros(3, 6, 2, 16, 2, 8, dtype=BF16)
+    flat = kv.view(3, 6, 32, 16)[0]
+    for caches in ([kv, kv[0], flat], [flat, kv[0], kv], [kv[0], kv, flat, kv, kv[0], flat]):
+        c, n = ops._page_caches("compact_pages", caches, pool)
+        got = [(s.data, s.slot_bytes, s.layers, s.parts, s.slots) for s in c[:n]]
+        assert n == 3 and set(got) == {(kv.data_ptr(), 32, 3, 2, 16), (kv.data_ptr(), 32, 1, 2, 16), (kv.data_ptr(), 32, 1, 1, 32)}

@@ -2388,7 +2388,7 @@ def _page_cache_check(who: str, t, pool: PagePool) -> None:
 
 def _page_caches(who: str, caches, pool: PagePool):
     """VbPageCache of every cache: [layers, pages, 2, page, ...] or, of one layer, [pages, page, ...]; per page anything else [pages, n, ...] goes as a whole"""
-    P, n, dev, words, k = pool.page_size, pool.pages, pool._device, [], 0
+    P, n, dev, words, seen = pool.page_size, pool.pages, pool._device, [], set()
     for t in caches:
         s, at, size, layers, parts, slots = t.shape, t.data_ptr(), t.nbytes, 1, 1, 0
         d = len(s)
@@ -2401,9 +2401,11 @@ def _page_caches(who: str, caches, pool: PagePool):
         slot = size // (layers * n * parts * slots) if size and slots else 0
         if slot == 0 or slot % 16 or at % 16 or t.get_device() != dev or not t.is_contiguous():
             _page_cache_check(who, t, pool)
-        if at not in words[::4]:                       # (a cache that is both keys and values is one)
-            words += (at, slot, layers | parts << 32, slots)
-            k += 1
+        one = (at, slot, layers | parts << 32, slots)
+        if one not in seen:                            # (a cache that is both keys and values is one; a layer beside the stack that it begins is not)
+            seen.add(one)
+            words += one
+    k = len(seen)
     return (_lib.PageCacheStruct * max(1, k)).from_buffer(array("q", words or (0, 0, 0, 0))), k
 
 
