@@ -295,3 +295,51 @@ def test_a_captured_loop_that_runs_short_in_the_middle(shared):
     torch.cuda.synchronize()
     s.pool.check()
     assert torch.equal(s.pool.tokens, kept[2] + 1) and torch.equal(s.pool.live, s.pool.tokens)
+
+
+class KeptSearch(Search):
+    """keeps what a step chose"""
+
+    def choose(self, logits):
+        ops = self.ops
+        self.last = step = ops.beam_select(logits, self.scores, WIDTH, weight=self.weight, ended=self.ended, end_token=self.end_token)
+        ops.fork_pages(self.pool, step.parent, 1, [self.kv])
+        ops.beam_reorder([self.history], step.parent)
+        self.history.index_copy_(1, self.at, step.token.to(I32).view(-1, 1))
+        self.at += 1
+        self.scores.copy_(step.scores)
+        self.ended.copy_(step.ended)
+        self.ids.copy_(step.token.view(-1))
+
+
+def test_ended_beams_keep_their_scores():
+    """an ended beam comes back once at most, under its end token and at its own score to the bit; it is there wherever its rank is above the last chosen one by more than a
+    sum's error (2^-18 of a total, both sides); every total of a step is a number"""
+    s = KeptSearch(end_token=11, weighted=True)
+    s.start()
+    carried = 0
+    for k in range(14):
+        s.weight.copy_(torch.where(s.ended, s.weight, torch.full_like(s.weight, (k + 2) ** -0.7)))
+        logits = s.forward().clone()
+        logits[:, 11] += 4.0
+        was, old, weight = s.ended.cpu(), s.scores.cpu(), s.weight.cpu()
+        s.choose(logits)
+        s.pool.check()
+        parent, token, score, over = (t.cpu() for t in (s.last.parent, s.last.token, s.last.scores, s.last.ended))
+        assert bool(torch.isfinite(score).all()) and bool((parent >= 0).all())
+        for b in range(2):
+            ranks = [float(score[b, i].double() * weight[b, parent[b, i]].double()) for i in range(WIDTH)]
+            slack = 4 * 2.0 ** -18 * float(weight[b].max()) + 2.0 ** -22 * max(abs(r) for r in ranks)
+            assert all(x >= y - slack for x, y in zip(ranks, ranks[1:]))
+            for w in range(WIDTH):
+                mine = torch.nonzero(parent[b] == w).view(-1).tolist()
+                if not bool(was[b, w]):
+                    assert all(bool(over[b, i]) == (int(token[b, i]) == 11) for i in mine)
+                    continue
+                assert len(mine) <= 1
+                for i in mine:
+                    assert float(score[b, i]) == float(old[b, w]) and int(token[b, i]) == 11 and bool(over[b, i])
+                    carried += 1
+                if not mine:
+                    assert float(old[b, w].double() * weight[b, w].double()) <= ranks[-1] + slack
+    assert carried > 0
