@@ -312,3 +312,22 @@ def test_output_over_the_queries():
     kv, q = _data(pages, 16, 6, 6, 3, 128, seed=10)
     want = _run(q, kv, 0, table, tokens, 3).clone()
     assert torch.equal(_run(q, kv, 0, table, tokens, 3, out=q), want)
+
+
+@pytest.mark.parametrize("G", [2, 16])
+def test_masked_tiles_one_behind_the_other(G):
+    """every tile has its own pieces and masks, which one warp writes and four read while the next tiles are fetched: the same bits on every run, in line with 64 bits"""
+    B, W, H, P, D, cols = 3, 8, 2, 16, 128, 90
+    g = torch.Generator().manual_seed(2)
+    table = torch.randperm(B * W * cols, generator=g).to(I32).view(B * W, cols)
+    for b in range(B):                                       # every other page is held by a changing half of the rows
+        for c in range(0, cols, 2):
+            half = torch.randperm(W, generator=g)[:W // 2] + b * W
+            table[half, c] = table[b * W, c].clone()
+    table = table.cuda()
+    tokens = torch.randint(cols * P - 300, cols * P + 1, (B * W,), generator=g).to(I32).cuda()
+    kv, q = _data(B * W * cols, P, B * W, G * H, H, D, seed=13)
+    a = _run(q, kv, 0, table, tokens, W)
+    _check(a, q, kv[0], table, tokens)
+    for _ in range(40):
+        assert torch.equal(a, _run(q, kv, 0, table, tokens, W))

@@ -508,6 +508,7 @@ __device__ __forceinline__ void shared_fetch(const SharedAttnParams& p, const Sh
   const int first = __shfl_sync(0xffffffffu, e.x, 0), at = e.w > 0 ? e.x : first, before = __shfl_up_sync(0xffffffffu, at, 1);
   const int page = at / p.page_size, slot = at - page * p.page_size;
   const uint32_t starts = __ballot_sync(0xffffffffu, lane == 0 || at != before + SA_PIECE || slot == 0);
+  __syncwarp();                          // (what the other lanes wrote of the tile's pieces is released by lane 0's arrival; shuffles order no memory)
   if (lane == 0) mbar_arrive_expect_tx(bar, PTC_KT * D * 2);
   __syncwarp();
   if (lane < SA_TILE_PIECES && (starts >> lane & 1u)) {
