@@ -944,7 +944,7 @@ int vb_moe_layer(float* d_y, long long ldy, const void* d_h, long long ldh, cons
  *   is not a finite number > 0 has none.  Logits [requests * width] rows of vocab (1 .. 2^24), bf16 or fp32, row_stride elements apart, at any element.
  *   Outputs [requests][n] (n 1 .. 64, width 1 .. 32): score fp32, parent int32 (beam of the request), token int64, d_out_ended (NULL: not wanted): the parent has
  *   ended or the token is end_token.  Fewer than n candidates: -infinity, -1, -1, 1 behind them.  end_token < 0 where no beam ends (d_ended, d_out_ended NULL).
- *   Workspace: vb_beam_select_workspace_bytes (0 where a request is a cluster's work: d_workspace may be NULL), one per call in flight.
+ *   Workspace: vb_beam_select_workspace_bytes (0 where the requests are clusters' work and all run at once: d_workspace may be NULL; asked for on the device of the call), one per call in flight.
  * vb_beam_reorder: row slot[b][i] of every state becomes what row slot[b][parent[b][i]] was, in place (d_slots NULL: b * width + i).  parent < 0, or one outside the
  *   request: the row stays.  states / row_bytes: HOST arrays, n_states tensors of n_slots rows; a slot stands in d_slots once. */
 size_t vb_beam_select_workspace_bytes(int requests, int width, int vocab, int n, int logits_f32);

@@ -366,3 +366,28 @@ def test_every_size_of_a_single_logit():
     step = ops.beam_select(z, s, 1)
     assert bool((step.token == 4).all()) and bool((step.parent == 0).all())
     assert bool(((step.scores - s).abs() <= 2.0 ** -18 + 2.0 ** -23 * s.abs()).all())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("B,W,V,n", [(64, 4, 32003, 8), (74, 8, 2051, 16), (300, 8, 515, 5), (148, 1, 20000, 2), (700, 1, 33, 3), (222, 2, 9000, 4), (5000, 2, 12, 4)])
+def test_many_requests(B, W, V, n, dtype):
+    """more requests than run at once as clusters, and as many as do: a workspace in the first case, none in the second, the same choices"""
+    z, s = _inputs(B, W, V, dtype)
+    s[::3, W - 1] = -INF
+    _check(ops.beam_select(z, s, n), z, s, n)
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_one_launch_only_where_all_requests_run_at_once(dtype):
+    """the workspace grows from none to some with the requests, and never back; one request is one launch up to eight parts"""
+    f32 = dtype is F32
+    for W, V in ((1, 2051), (2, 2051), (4, 2051), (8, 2051), (3, 500)):
+        none = [ops._beam_ws(B, W, V, 4, f32) == 0 for B in (1, 2, 8, 32, 60, 200, 400, 800, 2000)]
+        assert none[0] and not none[-1] and none == sorted(none, reverse=True)
+    z, s = _inputs(3, 4, 700, dtype)
+    for B, launches in ((3, 1), (900, 2)):
+        zz, ss = z.repeat(B // 3, 1), s.repeat(B // 3, 1)
+        before = ops.launch_count()
+        step = ops.beam_select(zz, ss, 5)
+        assert ops.launch_count() - before == launches
+        _check(step, zz, ss, 5)

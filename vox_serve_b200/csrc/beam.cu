@@ -6,7 +6,7 @@
 //
 // Two kernels.  The first reads the logits once: a block takes a part of a row in chunks, by asynchronous copies into shared memory with the next one on its way,
 // and leaves the part's maximum, its sum of exponentials and its n largest in order.  The second, a block a request, adds the sums up, ranks the n largest of every
-// part by their totals and writes the n best.  Where a request has at most eight parts both are one launch, a cluster a request.
+// part by their totals and writes the n best.  Where a request has at most eight parts and all requests run at once both are one launch, a cluster a request.
 //
 // What orders candidates is computed in 64 bits from the parts' sums.  A sum's terms carry the special function unit's 2^-22 and, from one fp32 constant for log2 e,
 // 1.3e-8 of the distance from the maximum: below 2^-20 of a term that counts (distance up to 40).  Sums of parts meet through log2 e in two constants.
@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const __grid_constan
   beam_join<THREADS>(sh, bj_key, p, blockIdx.x, p.stats + first, p.best + first * p.n);
 }
 
-// Both in one launch where a request's parts are few: a cluster a request, whose blocks leave what they found in the first one's shared memory.  (One beam of two
+// Both in one launch where a request's parts are few and all requests run at once (beam_one_launch): a cluster a request, whose blocks leave what they found in the first one's shared memory.  (One beam of two
 // over 2051 tokens: 6.45 -> 5.9 us in a graph, the call 16.1 -> 13.6.)
 template <typename T>
 __global__ void __launch_bounds__(BS_THREADS) beam_small_kernel(const __grid_constant__ BeamCall p) {
@@ -717,6 +717,24 @@ static int beam_parts(int requests, int width, int vocab, int n, int elem) {
   return (chunks + each - 1) / each;
 }
 
+// One launch where a request's parts are a cluster's work and all clusters run at once, by the device's own count: its blocks take more registers (bf16: three an SM, not
+// four) and stay until their request has been joined, so a second wave of them costs more than a second launch.  One / two launches, bf16, where all run at once: 1 x 2 rows of
+// 2051 6.2 / 6.7 us, 100 x 1 of 32003 7.7 / 9.5, 64 x 4 of 8192 7.5 / 7.7, 111 x 3 of 156940 39.8 / 46.1; where they do not: 64 x 4 of 32003 18.3 / 14.8, of 156940 42.0 / 33.0, 74 x 8 of
+// 2051 14.7 / 12.8, 300 x 8 of 8192 42.6 / 26.5.  fp32: 128 x 2 of 32003 14.4 / 15.7, 296 x 2 of 8192 9.7 / 10.2; 74 x 4 of 8192 12.8 / 9.3, 74 x 8 of 156940 97 / 69.  (fp32
+// clusters of eight all run at once but unevenly over the SMs: 40 x 8 of 156940 61.3 / 52.4, 64 x 4 of 8192 10.7 / 9.2 stay one.)
+template <auto Kernel>
+static bool beam_fits(int requests, int cluster) {
+  if (rm_smem<Kernel>(sizeof(PartShared)) != cudaSuccess) {      // (no device: sizes are asked for, nothing runs)
+    cudaGetLastError();
+    return true;
+  }
+  return requests <= rm_clusters<Kernel>(cluster, BS_THREADS, sizeof(PartShared));
+}
+static bool beam_one_launch(int requests, int width, int parts, bool f32) {
+  if (width * parts > BS_CLUSTER) return false;
+  return f32 ? beam_fits<beam_small_kernel<float>>(requests, width * parts) : beam_fits<beam_small_kernel<__nv_bfloat16>>(requests, width * parts);
+}
+
 }  // namespace vb
 
 using namespace vb;
@@ -724,7 +742,7 @@ using namespace vb;
 extern "C" size_t vb_beam_select_workspace_bytes(int requests, int width, int vocab, int n, int logits_f32) {
   if (requests <= 0 || width <= 0 || width > BS_MAX_W || vocab <= 0 || n <= 0 || n > BS_MAX_N) return 0;
   const int parts = beam_parts(requests, width, vocab, n, logits_f32 ? 4 : 2);
-  return width * parts <= BS_CLUSTER ? 0 : static_cast<size_t>(requests) * width * parts * (sizeof(BeamStats) + 8ull * n);
+  return beam_one_launch(requests, width, parts, logits_f32) ? 0 : static_cast<size_t>(requests) * width * parts * (sizeof(BeamStats) + 8ull * n);
 }
 
 extern "C" int vb_beam_select(float* d_score, int32_t* d_parent, int64_t* d_token, uint8_t* d_out_ended, const void* d_logits, int64_t row_stride, int logits_f32,
@@ -748,8 +766,7 @@ extern "C" int vb_beam_select(float* d_score, int32_t* d_parent, int64_t* d_toke
   BeamStats* stats = need ? reinterpret_cast<BeamStats*>(best + blocks * n) : nullptr;
   BeamCall p = {stats, best, d_logits, static_cast<long long>(row_stride), d_beam_score, d_weight, d_ended, d_score, d_parent, d_token, d_out_ended,
                 vocab, parts, width, n, static_cast<long long>(end_token)};
-  if (width * parts <= BS_CLUSTER) {
-    VB_CHECK_CUDA(logits_f32 ? rm_smem<beam_small_kernel<float>>(sizeof(PartShared)) : rm_smem<beam_small_kernel<__nv_bfloat16>>(sizeof(PartShared)));
+  if (need == 0) {                                     // (beam_fits has asked for their shared memory)
     if (logits_f32) VB_LAUNCH_PDL_CLUSTER(beam_small_kernel<float>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, width * parts, p);
     else VB_LAUNCH_PDL_CLUSTER(beam_small_kernel<__nv_bfloat16>, static_cast<unsigned>(blocks), BS_THREADS, sizeof(PartShared), stream, width * parts, p);
     return 0;
