@@ -497,7 +497,7 @@ int vb_gemm_bf16_grouped_glu(void* d_y, const void* d_w_tiles, const void* x_map
  * synchronises the device).
  * vb_wait_flags: eight bytes of host memory, one flag per kind of kernel whose waits give up after two seconds -- 0 prompt projections, 1
  * vocoder convolutions, 2 prompt attention and attention over shared pages, 3 window attention of prompts, 4 vb_wait_check, 5 experts of a decode step, 6 adapters of a step.  A kernel whose
- * wait ran out sets its flag and leaves its output incomplete (7 without a wait: adapters, a plan of other rows or slots than the call's): look at them after synchronising, before results are used, and clear them (NULL: no device).
+ * wait ran out sets its flag and leaves its output incomplete (7 without a wait: adapters, a plan of other rows or slots than the call's; shared pages, one of other lengths): look at them after synchronising, before results are used, and clear them (NULL: no device).
  * vb_wait_check: one kernel that waits on a barrier at most limit_us from the moment a second warp opens it, pause_us after the start (both warps
  * then agree on whether it ran out: the flag is 3);
  * that warp then completes the barrier, or with complete = 0 does not (flag 4). */
@@ -983,10 +983,11 @@ int vb_compact_pages(const VbPagePool* pool, const VbPagePool* out, const VbPage
  *   request hold in the same column is read once for (up to 32, and up to 128 / (n_q / n_kv)) of them.  d_buffer: vb_shared_plan_bytes (0: sizes that are refused), 16-byte aligned,
  *   written by vb_shared_plan once a step and by every vb_shared_attn (one stream at a time).  head_dim 64 or 128, page_size a multiple of 16, grid: blocks that run at once (two an SM).
  * vb_shared_plan: d_table [rows][columns], d_tokens [rows] (0: a row without tokens, its output is zero); entries that are no page are skipped.
- * vb_shared_attn: q / out [rows][n_q][head_dim] bf16 (out_xt_tile > 0: the tiled layout), d_kv [slabs][2][page_size][n_kv][head_dim] bf16, slab_base = layer * pages. */
+ * vb_shared_attn: d_row_tokens (or NULL) [rows]: what the rows of the calling step hold; where the plan's differ zeros come out and flag 7 of vb_wait_flags is set.  q / out [rows][n_q][head_dim] bf16 (out_xt_tile > 0: the tiled layout), d_kv [slabs][2][page_size][n_kv][head_dim] bf16, slab_base = layer * pages. */
 typedef struct {
   void* d_buffer;
   int32_t rows, width, columns, page_size, n_q, n_kv, head_dim, grid;
+  const int32_t* d_row_tokens;
 } VbSharedPlan;
 size_t vb_shared_plan_bytes(const VbSharedPlan* plan);
 int vb_shared_plan(const VbSharedPlan* plan, const int32_t* d_table, const int32_t* d_tokens, int pages, void* stream);

@@ -343,3 +343,35 @@ def test_ended_beams_keep_their_scores():
                 if not mine:
                     assert float(old[b, w].double() * weight[b, w].double()) <= ranks[-1] + slack
     assert carried > 0
+
+
+@pytest.mark.parametrize("mode", ["unfused", "fused"])
+def test_a_plan_that_is_not_the_steps(mode):
+    """one that was never made is refused before anything is written; one of the step before gives no logits that go unnoticed"""
+    s = Search(mode)
+    s.start()
+    ops = s.ops
+
+    def rows():
+        ops.plan_rows(s.eng.plan, None, s.pool.indptr, s.pool.table.view(-1), None, s.rows, s.rows, PAGE, s.eng.chunk, kv_len=s.pool.tokens)
+    rows()
+    before = s.kv.clone()
+    with pytest.raises(ops.VoxB200Error, match="never made"):
+        s.eng.forward(s.ids, s.pool.tokens - 1, s.rows, shared=s.plan)
+    assert torch.equal(s.kv, before)
+    s.choose(s.forward())
+    torch.cuda.synchronize()
+    ops.check_waits()
+    rows()
+    with pytest.raises(ops.VoxB200Error, match="shared pages"):      # (by a launch of a later layer, or at the end)
+        s.eng.forward(s.ids, s.pool.tokens - 1, s.rows, shared=s.plan)
+        torch.cuda.synchronize()
+        ops.check_waits()
+    torch.cuda.synchronize()
+    try:                                                     # (layers that were on their way when the first one raised)
+        ops.check_waits()
+    except ops.VoxB200Error:
+        pass
+    assert bool(torch.isfinite(s.forward()).all())
+    torch.cuda.synchronize()
+    ops.check_waits()

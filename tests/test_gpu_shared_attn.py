@@ -331,3 +331,38 @@ def test_masked_tiles_one_behind_the_other(G):
     _check(a, q, kv[0], table, tokens)
     for _ in range(40):
         assert torch.equal(a, _run(q, kv, 0, table, tokens, W))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("B,W", [(1, 4), (3, 4), (70, 2)])
+def test_a_plan_of_other_lengths(B, W, D):
+    """rows for which the plan has other lengths than the step come out as zeros and the host is told; the others' bits are what they are without lengths"""
+    table, tokens, pages = _tree(B, W, 200, 30, 16, seed=51)
+    R = B * W
+    kv, q = _data(pages, 16, R, 8, 4, D, seed=52)
+    tokens[1] = -2
+    plan = ops.SharedPlan(R, W, table.shape[1], 16, 8, 4, D)
+    ops.shared_plan(plan, table, tokens, pages)
+    want = ops.shared_attn(q, kv, 0, plan)
+    assert torch.equal(ops.shared_attn(q, kv, 0, plan, tokens=tokens), want)
+    torch.cuda.synchronize()
+    ops.check_waits()
+    step = tokens.clone()
+    step[0] += 1
+    step[1] = 0                                              # (none, as -2 is)
+    step[R - 1] = 0
+    out = ops.shared_attn(q, kv, 0, plan, tokens=step, out=torch.full_like(q, NAN))
+    torch.cuda.synchronize()
+    with pytest.raises(ops.VoxB200Error, match="shared pages"):
+        ops.check_waits()
+    ops.check_waits()
+    assert not bool(out[[0, R - 1]].any()) and torch.equal(out[1:R - 1], want[1:R - 1])
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.shared_plan(plan, table, step, pages)
+        ops.shared_attn(q, kv, 0, plan, tokens=step, out=out)
+    step.copy_(tokens)
+    g.replay()
+    torch.cuda.synchronize()
+    ops.check_waits()
+    assert torch.equal(out, want)

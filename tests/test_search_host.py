@@ -240,3 +240,25 @@ def test_caches_that_begin_at_one_address(launched):
         c, n = ops._page_caches("compact_pages", caches, pool)
         got = [(s.data, s.slot_bytes, s.layers, s.parts, s.slots) for s in c[:n]]
         assert n == 3 and set(got) == {(kv.data_ptr(), 32, 3, 2, 16), (kv.data_ptr(), 32, 1, 2, 16), (kv.data_ptr(), 32, 1, 1, 32)}
+
+
+def test_attn_needs_a_plan_that_was_made(launched):
+    plan = ops.SharedPlan(6, 3, 4, 16, 4, 2, 64, device="cpu")
+    plan._device = -1
+    q, kv = torch.zeros(6, 4, 64, dtype=BF16), torch.zeros(5, 2, 16, 2, 64, dtype=BF16)
+    table, tokens = torch.zeros(6, 4, dtype=I32), torch.zeros(6, dtype=I32)
+    with pytest.raises(VoxB200Error, match="never made"):
+        ops.shared_attn(q, kv, 0, plan)
+    assert launched == []
+    ops.shared_plan(plan, table, tokens, 5)
+    ops.shared_attn(q, kv, 0, plan)
+    assert not plan._struct.d_row_tokens
+    ops.shared_attn(q, kv, 0, plan, tokens=tokens)
+    assert plan._struct.d_row_tokens == tokens.data_ptr()
+    ops.shared_attn(q, kv, 0, plan)
+    assert not plan._struct.d_row_tokens
+    n = len(launched)
+    for bad in (tokens.long(), tokens[:5], tokens.view(2, 3), torch.zeros(12, dtype=I32)[::2]):
+        with pytest.raises(VoxB200Error, match="int32 tokens"):
+            ops.shared_attn(q, kv, 0, plan, tokens=bad)
+    assert len(launched) == n

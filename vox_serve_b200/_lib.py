@@ -264,16 +264,16 @@ class PageCacheStruct(C.Structure):
 
 class SharedPlanStruct(C.Structure):
     """VbSharedPlan"""
-    _fields_ = [("d_buffer", P)] + [(n, C.c_int32) for n in ("rows", "width", "columns", "page_size", "n_q", "n_kv", "head_dim", "grid")]
+    _fields_ = [("d_buffer", P)] + [(n, C.c_int32) for n in ("rows", "width", "columns", "page_size", "n_q", "n_kv", "head_dim", "grid")] + [("d_row_tokens", P)]
 
 
 _lock = threading.Lock()
 _lib = None
 # flags in mapped host memory, one byte per kind of kernel whose waits give up (csrc/common.cuh, BoundedWait); the last one: a kernel that met a table of
-# another step's (csrc/lora.cu)
+# another step's (csrc/lora.cu, csrc/shared_attn.cu)
 _wait_flags = None
 WAIT_KINDS = ("a projection of a prompt step", "a vocoder convolution", "prompt attention or attention over shared pages", "window attention of a prompt", "vb_wait_check", "experts of a decode step", "adapters of a step",
-              "a plan of adapters")
+              "a plan of adapters or of shared pages")
 
 
 class VoxB200Error(RuntimeError):
@@ -344,7 +344,7 @@ def check_waits():
         kinds = [name for i, name in enumerate(WAIT_KINDS) if bits >> (8 * i) & 0xff] or ["a kernel"]
         why = []
         if kinds[-1] == WAIT_KINDS[-1]:
-            why.append(f"{kinds.pop()} of other rows or slots than the step's was read (a captured step behind another step's plan?)")
+            why.append(f"{kinds.pop()} of other rows, slots or lengths than the step's was read (a captured step behind another step's plan?)")
         if kinds:
             why.append(f"a wait inside {' and '.join(kinds)} ran out")
         raise VoxB200Error(f"{'; '.join(why)}: results since then are incomplete")

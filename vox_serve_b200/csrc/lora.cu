@@ -979,7 +979,7 @@ static int lora_setup(const char* who, LoraParams& p, const void* d_x, long long
   VB_CHECK_ARG(reinterpret_cast<uintptr_t>(d_tiles) % 16 == 0, "%s: the plan must be 16-byte aligned", who);
   VB_CHECK_ARG(T <= LORA_MAX_ROWS, "%s: %d rows; at most %d", who, T, LORA_MAX_ROWS);
   VB_CHECK_ARG(ldx % 8 == 0 && ldx >= p.K && reinterpret_cast<uintptr_t>(d_x) % 16 == 0, "%s: rows of x must be 16-byte aligned (K %d, row stride %lld)", who, p.K, ldx);
-  VB_CHECK_ARG(p.plan_flag = wait_flag(WK_LORA_PLAN), "%s: no mapped host memory", who);
+  VB_CHECK_ARG(p.plan_flag = wait_flag(WK_PLAN), "%s: no mapped host memory", who);
   p.slots = bank->slots;
   p.tiles = static_cast<const int32_t*>(d_tiles) + LORA_PLAN_HEAD;
   p.groups = reinterpret_cast<const int4*>(p.tiles + static_cast<long long>(lora_max_tiles(T, bank->slots)) * (4 + p.tile_rows));

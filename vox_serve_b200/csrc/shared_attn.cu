@@ -340,7 +340,8 @@ struct SharedAttnParams {
   float* acc;                    // [blocks + units][mpad][D]: the segment of block b on unit u stands at b + u
   float2* stat;                  // [blocks + units][mpad] maximum (base 2), denominator against it
   long long slab_base, slabs;
-  unsigned char* wait_flag;
+  unsigned char *wait_flag, *plan_flag;
+  const int32_t* expect;         // tokens of the rows in the step that calls, or null: a plan of other ones is another step's
   int rows, width, sub, subs, groups, cap, page_size, n_q, heads, G, mpad, xt_tile;
   float scale_log2;
 };
@@ -663,10 +664,16 @@ __global__ void __launch_bounds__(32 * SJ_WARPS) shared_join_kernel(const __grid
   const bool on = m < n_rows * p.G;
   const int row = r0 + (on ? m / p.G : 0), k = (h * p.G + (on ? m % p.G : 0)) * D + lane * E;
   const int2 blocks = p.blocks_of[unit];
+  const int len = p.len[row];
+  const bool other = p.expect && max(0, p.expect[row]) != len;  // (zeros come out, and the host is told)
+  if (other && on && lane == 0) {
+    *reinterpret_cast<volatile unsigned char*>(p.plan_flag) = 1;
+    __threadfence_system();
+  }
   float acc[E], total = 0.f, top = -INFINITY;                   // against the largest maximum so far
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.f;
-  if (on && p.len[row] > 0) {
+  if (on && len > 0 && !other) {
     const int s0 = blocks.x + unit, s1 = blocks.y + unit + 1;
     for (int s = s0 + sub; s < s1; s += 8 * WPR) {              // eight segments' maxima and outputs at once
       float2 st[8];
@@ -847,7 +854,8 @@ extern "C" int vb_shared_attn(void* d_out, const void* d_q, const void* d_kv, in
   p.blocks_of = reinterpret_cast<const int2*>(at + l.blocks_of);
   p.acc = reinterpret_cast<float*>(at + l.acc), p.stat = reinterpret_cast<float2*>(at + l.stat);
   p.slab_base = slab_base, p.slabs = slabs;
-  VB_CHECK_ARG(p.wait_flag = wait_flag(WK_PREFILL_ATTN), "vb_shared_attn: no mapped host memory");
+  VB_CHECK_ARG((p.wait_flag = wait_flag(WK_PREFILL_ATTN)) && (p.plan_flag = wait_flag(WK_PLAN)), "vb_shared_attn: no mapped host memory");
+  p.expect = plan->d_row_tokens;
   p.rows = plan->rows, p.width = plan->width, p.sub = l.sub, p.subs = l.subs, p.groups = l.groups, p.cap = l.cap, p.page_size = P;
   p.n_q = plan->n_q, p.heads = H, p.G = plan->n_q / H, p.mpad = l.mpad, p.xt_tile = out_xt_tile;
   p.scale_log2 = sm_scale * 1.44269504088896f;

@@ -351,7 +351,8 @@ class LlamaEngine:
         starts from, csm.py:290-300).  ``adapters``: the plan of the rows' adapters (ops.lora_plan; ``set_adapters`` first).  Such a
         step runs every row, those without an adapter too, on row-major activations and planes of gate | up: their results are
         those of a step without adapters up to bf16 rounding, not to the bit.  ``shared``: a decode step whose requests have several rows that share
-        pages (ops.shared_plan of the tables that ``plan`` was made from, the step's tokens counted): a page is read once for all of them."""
+        pages (ops.shared_plan of the tables that ``plan`` was made from, the step's tokens counted): a page is read once for all of them.  One that was never made is
+        refused; one whose lengths are not the step's (another step's) gives no attention, and the next call or ``ops.check_waits`` raises."""
         d, w, R = self.dims, self.w, n_rows
         if shared is not None:
             dims = (shared.rows, shared.n_q, shared.n_kv, shared.head_dim, shared.page_size)
@@ -360,12 +361,16 @@ class LlamaEngine:
                                    f"{(R, d.num_attention_heads, d.num_key_value_heads, d.head_dim, self.page_size)}")
             if (self.plan if plan is None else plan).qo_indptr is not None:
                 raise VoxB200Error("forward: shared pages are read by decode steps, one row of every table")
+            if not shared.made:
+                raise VoxB200Error("forward: the plan of shared pages was never made (ops.shared_plan)")
         if adapters is not None:                   # (before anything is written)
             if self.adapters is None:
                 raise VoxB200Error("forward: the engine has no adapters (set_adapters)")
             if (adapters.n_rows, adapters.slots) != (R, self.adapters.slots):
                 raise VoxB200Error(f"forward: the plan of adapters is of {adapters.n_rows} rows and {adapters.slots} slots, the step of {R} and {self.adapters.slots}")
         plan = self.plan if plan is None else plan
+        if shared is not None:                     # (with the lengths that it has to have been made for)
+            shared = (shared, plan.row_kvlen[:R])
         if R > self.max_rows:
             raise VoxB200Error(f"{R} rows exceed the engine's max_rows {self.max_rows}")
         hidden, normed = self.hidden[:R], self.normed[:R]
@@ -407,14 +412,14 @@ class LlamaEngine:
     # removed.  The fused projections stay as parity-tested C-ABI operators.
     force_unfused = os.environ.get("VB_DECODE_MODE", "unfused") == "unfused"
 
-    def _attend(self, layer: int, q: torch.Tensor, out, plan: ops.RowPlan, R: int, shared: Optional[ops.SharedPlan]) -> None:
+    def _attend(self, layer: int, q: torch.Tensor, out, plan: ops.RowPlan, R: int, shared: Optional[Tuple[ops.SharedPlan, torch.Tensor]]) -> None:
         if shared is not None:
-            ops.shared_attn(q, self.kv_map, layer * self.pages_per_layer, shared, out=out)
+            ops.shared_attn(q, self.kv_map, layer * self.pages_per_layer, shared[0], out=out, tokens=shared[1])
         else:
             ops.paged_attn(q, self.kv_map, layer * self.pages_per_layer, plan, R, self.dims.num_key_value_heads, self.page_size, self.chunk, self.attn_ws, out=out,
                            grid_ctas=self.attn_grid)
 
-    def _layers_fused(self, position_ids: torch.Tensor, R: int, plan: ops.RowPlan, shared: Optional[ops.SharedPlan] = None) -> None:
+    def _layers_fused(self, position_ids: torch.Tensor, R: int, plan: ops.RowPlan, shared: Optional[Tuple[ops.SharedPlan, torch.Tensor]] = None) -> None:
         """hidden is updated in place, the RMSNorm statistics travel as per-tile sums of squares written by the
         residual projections (ssq[parts][R]).  Per layer: norm + QKV + RoPE + append, paged attention, O + residual,
         norm + gate/up + SiLU, down + residual: one launch per fused projection (5 per layer)."""
@@ -445,7 +450,7 @@ class LlamaEngine:
                               hidden_tiles_out=hidden_t)
 
     def _layers_unfused(self, position_ids: torch.Tensor, R: int, plan: ops.RowPlan, input_ids: Optional[torch.Tensor] = None,
-                         adapters: Optional[ops.LoraPlan] = None, shared: Optional[ops.SharedPlan] = None):
+                         adapters: Optional[ops.LoraPlan] = None, shared: Optional[Tuple[ops.SharedPlan, torch.Tensor]] = None):
         """8 launches per layer.  Activations travel between kernels in the tiled layout (the attention output only in
         decode-sized steps and only with VB_ATTN_TILED=1); returns what holds the final normed rows (a TiledAct then,
         else self.normed[:R]).  input_ids: the embedding rows are still to be fetched."""

@@ -2478,7 +2478,8 @@ class SharedPlan:
         _refuse(page_size < 16 or page_size % 16 != 0 or page_size > 4096, f"SharedPlan: pages of {page_size} tokens (a multiple of 16, at most 4096)")
         _refuse(not 1 <= columns <= 16384, f"SharedPlan: {columns} pages a row (1 to 16384)")
         self.rows, self.width, self.columns, self.page_size, self.n_q, self.n_kv, self.head_dim = (int(v) for v in (rows, width, columns, page_size, n_q, n_kv, head_dim))
-        self.pages = 0                                 # of the cache that the plan was made for
+        self.pages, self.made = 0, False               # pages of the cache that the plan was made for; whether shared_plan has been called on it
+        self._tokens = None                            # what d_row_tokens says
         grid = 2 * (attn_grid_ctas() if torch.device(device).type == "cuda" else 148)      # two blocks an SM
         self._struct = _lib.SharedPlanStruct(None, self.rows, self.width, self.columns, self.page_size, self.n_q, self.n_kv, self.head_dim, grid)
         self._ptr = ctypes.addressof(self._struct)
@@ -2499,22 +2500,27 @@ def shared_plan(plan: SharedPlan, table: torch.Tensor, tokens: torch.Tensor, pag
     most = 0x7fffffff // plan.page_size
     _refuse(not 0 <= pages <= most, f"shared_plan: {pages} pages of {plan.page_size} tokens")
     call("vb_shared_plan", plan._ptr, table.data_ptr(), tokens.data_ptr(), pages or most, _stream())
-    plan.pages = int(pages)
+    plan.pages, plan.made = int(pages), True
     return plan
 
 
-def shared_attn(q: torch.Tensor, kv_cache: torch.Tensor, slab_base: int, plan: SharedPlan, sm_scale: Optional[float] = None, out=None):
+def shared_attn(q: torch.Tensor, kv_cache: torch.Tensor, slab_base: int, plan: SharedPlan, sm_scale: Optional[float] = None, out=None, tokens: Optional[torch.Tensor] = None):
     """Attention of one new token a row, every different page read once for the rows of a request that hold it: q bf16 [rows, Hq, D] -> [rows, Hq, D].  kv_cache: the whole cache
     [layers, pages, 2, page, Hkv, D] (slab_base = layer * pages) or one layer [pages, 2, page, Hkv, D] bf16, as for ``paged_attn``, whose results it has up to rounding;
-    ``plan``: ``shared_plan`` of this step's tables.  out: bf16 like q, or a TiledAct.  What is not finite in a page reaches the rows that hold it and no others."""
+    ``plan``: ``shared_plan`` of this step's tables.  out: bf16 like q, or a TiledAct.  What is not finite in a page reaches the rows that hold it and no others (as
+    infinity or NaN).  ``tokens`` int32 [rows]: what the rows of this step hold.  A plan that was made for other lengths is another step's: such rows come out as zeros, and
+    ``check_waits`` and every further call raise."""
     R, Hq, D = plan.rows, plan.n_q, plan.head_dim
     dev, s = _device_index(), kv_cache.shape
     per, slabs = (s[-5], s[0] * (s[1] if len(s) == 6 else 1)) if len(s) in (5, 6) else (1, 0)
     # (one comparison per fact when all of them hold)
     if not (q.get_device() == plan._device == kv_cache.get_device() == dev and q.dtype is BF16 and q.shape == (R, Hq, D) and q.is_contiguous() and kv_cache.dtype is BF16
             and slabs > 0 and s[-4:] == (2, plan.page_size, plan.n_kv, D) and kv_cache.is_contiguous() and plan.pages <= per and 0 <= slab_base <= slabs - per
-            and slab_base % per == 0):
-        _need_here("shared_attn", q, kv_cache, plan.buf)
+            and slab_base % per == 0 and plan.made
+            and (tokens is None or (tokens.get_device() == dev and tokens.dtype is torch.int32 and tokens.shape == (R,) and tokens.is_contiguous()))):
+        _need_here("shared_attn", q, kv_cache, plan.buf, tokens)
+        _refuse(not plan.made, "shared_attn: the plan was never made (shared_plan)")
+        _refuse(tokens is not None and (tokens.dtype is not torch.int32 or tuple(tokens.shape) != (R,) or not tokens.is_contiguous()), f"shared_attn: int32 tokens [{R}] are needed")
         _refuse(q.dtype is not BF16 or tuple(q.shape) != (R, Hq, D) or not q.is_contiguous(), f"shared_attn: bf16 queries [{R}, {Hq}, {D}] are needed")
         _refuse(kv_cache.dtype is not BF16 or not kv_cache.is_contiguous() or slabs < 1 or tuple(s[-4:]) != (2, plan.page_size, plan.n_kv, D),
                 f"shared_attn: a bf16 cache [.., pages, 2, {plan.page_size}, {plan.n_kv}, {D}] is needed, not {tuple(s)}")
@@ -2531,6 +2537,9 @@ def shared_attn(q: torch.Tensor, kv_cache: torch.Tensor, slab_base: int, plan: S
         to = out
         _need_here("shared_attn", out)
         _refuse(out.dtype is not BF16 or out.shape != q.shape or not out.is_contiguous(), f"shared_attn: out is bf16 [{R}, {Hq}, {D}]")
+    at = None if tokens is None else tokens.data_ptr()
+    if at != plan._tokens:
+        plan._tokens = plan._struct.d_row_tokens = at
     call("vb_shared_attn", to.data_ptr(), q.data_ptr(), kv_cache.data_ptr(), slabs, int(slab_base), plan._ptr, 1.0 / math.sqrt(D) if sm_scale is None else float(sm_scale), xt,
          _raw_stream(dev))
     return out
