@@ -383,3 +383,21 @@ def test_a_layer_beside_the_stack_it_begins(first):
     plain.compact()
     ops.compact_pages(pool, caches=both)
     plain.same_as(pool, caches)
+
+
+def test_load_refuses_shared_partial_pages_and_is_captured():
+    pool = ops.PagePool(6, 4, 3, 3)
+    table, tokens = _i32([[5, 1, -1], [5, 2, -1], [-1, -1, -1]]), _i32([5, 7, 0])
+    pool.load(table, tokens)
+    with pytest.raises(VoxB200Error, match="2 rows share a page"):
+        pool.load(_i32([[5, 1, -1], [5, 1, -1], [-1, -1, -1]]), tokens)
+    assert pool.refs.tolist() == [0, 1, 1, 0, 0, 2]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        pool.load(table, tokens)
+        ops.fork_pages(pool, torch.zeros(3, dtype=I32, device="cuda"), 1)
+    table.copy_(_i32([[0, 3, -1], [0, 4, -1], [0, -1, -1]]))
+    tokens.copy_(_i32([6, 8, 4]))
+    g.replay()
+    pool.check()
+    assert pool.tokens.tolist() == [7, 7, 7] and pool.table.tolist() == [[0, 3, -1], [0, 1, -1], [0, 2, -1]] and pool.refs.tolist() == [3, 1, 1, 1, 0, 0]

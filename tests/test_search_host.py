@@ -262,3 +262,26 @@ def test_attn_needs_a_plan_that_was_made(launched):
         with pytest.raises(VoxB200Error, match="int32 tokens"):
             ops.shared_attn(q, kv, 0, plan, tokens=bad)
     assert len(launched) == n
+
+
+@pytest.mark.parametrize("table,tokens,rows", [
+    ([[5, 1, -1], [5, 1, -1], [-1, -1, -1]], [5, 5, 0], 2),       # both go on in page 1
+    ([[5, 1, -1], [5, 1, -1], [-1, -1, -1]], [5, 8, 0], 1),       # row 1 has filled it, row 0 would write over it
+    ([[5, 1, -1], [0, 2, 1], [3, 4, -1]], [6, 9, 8], 2),
+    ([[1, 1, -1], [-1, -1, -1], [-1, -1, -1]], [5, 0, 0], 1)])    # a row that holds it twice
+def test_tables_that_share_a_page_that_is_not_full(table, tokens, rows):
+    pool = ops.PagePool(6, 4, 3, 3, device="cpu")
+    pool.load(torch.tensor([[0, 1, 2], [0, 3, -1], [-1, -1, -1]], dtype=I32), torch.tensor([12, 8, 0], dtype=I32))
+    before = pool._buf.clone()
+    with pytest.raises(VoxB200Error, match=f"{rows} rows share a page"):
+        pool.load(torch.tensor(table, dtype=I32), torch.tensor(tokens, dtype=I32))
+    assert torch.equal(pool._buf, before)
+
+
+def test_tables_that_may_be_loaded():
+    """full pages are shared, partial ones are not; what stands behind a row's tokens, numbers that are no page, rows longer than their columns and rows of less than none are passed over"""
+    pool = ops.PagePool(6, 4, 3, 3, device="cpu")
+    for table, tokens, refs in (([[5, 1, -1], [5, 2, 1], [5, 0, -1]], [7, 8, 4], [0, 1, 1, 0, 0, 3]), ([[5, 9, 0], [5, 9, 0], [9, 9, -3]], [6, 6, 3], [0, 0, 0, 0, 0, 2]),
+                                ([[0, 1, 2], [0, 1, 2], [0, -1, -1]], [13, 12, -3], [2, 2, 2, 0, 0, 0]), ([[0, 1, 2], [3, 3, 3], [4, 0, 0]], [9, 0, 1], [1, 1, 1, 0, 1, 0])):
+        pool.load(torch.tensor(table), torch.tensor(tokens))
+        assert pool.refs.tolist() == refs and pool.tokens.tolist() == tokens

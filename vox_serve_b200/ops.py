@@ -2350,16 +2350,24 @@ class PagePool:
         self._ptr, self._device = ctypes.addressof(self._struct), self._buf.get_device()
 
     def load(self, table: torch.Tensor, tokens: torch.Tensor) -> "PagePool":
-        """tables that exist already: int32 [rows, columns] and [rows]; ``refs`` is counted from them, a shortage of the tables before is over"""
+        """Tables that exist already: int32 [rows, columns] and [rows]; ``refs`` is counted from them, a shortage of the tables before is over.  A page that a row holds and has not
+        filled must be that row's alone (both would append to it): raises otherwise, and nothing is taken over.  Waits for the tables; in a capture nothing can, and it is not
+        looked at."""
         _refuse(tuple(table.shape) != (self.rows, self.columns) or tuple(tokens.shape) != (self.rows,), f"PagePool.load: a table [{self.rows}, {self.columns}] is needed")
-        self.table.copy_(table)
+        to, P = self.table.device, self.page_size
+        table, tokens = table.to(to, torch.int32), tokens.to(to, torch.int32)
+        held = (tokens + P - 1) // P
+        on = (torch.arange(self.columns, device=to)[None] < held[:, None]) & (table >= 0) & (table < self.pages)
+        at = torch.where(on, table, torch.full_like(table, self.pages)).long()
+        count = torch.zeros(self.pages + 1, dtype=torch.int32, device=to).index_add_(0, at.view(-1), torch.ones_like(at.view(-1), dtype=torch.int32))
+        count[self.pages:].zero_()                     # (no page)
+        if not (table.is_cuda and torch.cuda.is_current_stream_capturing()):
+            last = at.gather(1, (tokens // P).clamp(0, self.columns - 1).long()[:, None])[:, 0]
+            shared = int(((tokens > 0) & (tokens % P != 0) & (tokens < self.columns * P) & (count[last] > 1)).sum())
+            _refuse(shared > 0, f"PagePool.load: {shared} rows share a page that they have not filled")
+        self.table.copy_(table.masked_fill(~on, -1))
         self.tokens.copy_(tokens)
-        held = (self.tokens + self.page_size - 1) // self.page_size
-        on = (torch.arange(self.columns, device=self.table.device)[None] < held[:, None]) & (self.table >= 0) & (self.table < self.pages)
-        at = torch.where(on, self.table, torch.full_like(self.table, self.pages)).view(-1).long()
-        count = torch.zeros(self.pages + 1, dtype=torch.int32, device=self.table.device).index_add_(0, at, torch.ones_like(at, dtype=torch.int32))
         self.refs.copy_(count[:self.pages])
-        self.table.masked_fill_(~on, -1)
         self.status[:2].zero_()
         self.live.copy_(self.tokens)
         return self
