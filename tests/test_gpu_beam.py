@@ -391,3 +391,12 @@ def test_one_launch_only_where_all_requests_run_at_once(dtype):
         step = ops.beam_select(zz, ss, 5)
         assert ops.launch_count() - before == launches
         _check(step, zz, ss, 5)
+
+
+def test_reorder_of_a_slot_named_twice():
+    """in a request: the last of its beams that move, in every column"""
+    t = torch.arange(6.0, device="cuda")[:, None].repeat(1, 5000).contiguous()
+    ops.beam_reorder([t], torch.tensor([[2, 3, 2, 3]], dtype=I32, device="cuda"), torch.tensor([[4, 4, 1, 0]], dtype=I32, device="cuda"))
+    assert bool((t[4] == 0).all()) and bool((t[[0, 1, 2, 3, 5]] == torch.tensor([0.0, 1, 2, 3, 5], device="cuda")[:, None]).all())
+    ops.beam_reorder([t], torch.tensor([[2, 1, 2, 3]], dtype=I32, device="cuda"), torch.tensor([[4, 4, 1, 0]], dtype=I32, device="cuda"))
+    assert bool((t[4] == 1).all())

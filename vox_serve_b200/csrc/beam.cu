@@ -15,7 +15,7 @@
 // of HBM.  What is above that: 512 blocks on 148 SMs, three or four each; 2.2 us a chunk of four blocks of an SM (its 64 KB are 1.3 of HBM, its exponentials 0.9 of the
 // special function unit; the rest are instructions and a meeting of the block), 8 to 13 of cuts, orders, launches and the join.  16 of 5 over 32003 fp32 tokens, n 10: 12.1 us.
 // One of two over 2051: 5.7, most of it the launch.
-// Four blocks an SM with two chunks in shared memory: 31.2 us; three with three 33.3, with four 32.6; four with three 34.4 (a list of 512); five with two 31.6.  Parts so
+// The bf16 form is held at 64 registers for four blocks an SM and spills 148 bytes a thread in its stream.  Four blocks an SM with two chunks in shared memory: 31.2 us; three with three 33.3, with four 32.6; four with three 34.4 (a list of 512); five with two 31.6.  Parts so
 // that all blocks run at once: more of them pay the first cut and the last order again, fewer leave SMs idle.  Lists are cut back once they hold twice what is wanted: open
 // rows 45.7 us, three times 46.6, four 47.2, at 256 53.7 (masked ones 32.6, 32.2, 32.1, 32.0).
 #include "../../include/vb_api.h"

@@ -2256,8 +2256,11 @@ def _beam_select_check(logits, scores, n, weight, ended, end_token) -> None:
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, weight: Optional[torch.Tensor] = None, ended: Optional[torch.Tensor] = None,
                 end_token: Optional[int] = None) -> BeamStep:
     """One step of a beam search.  logits [requests * width, vocab] bf16 or fp32 (rows apart by any stride), scores fp32 [requests, width]: the beams' log probabilities so
-    far.  Of all continuations of a request's beams, total[w, v] = scores[w] + log_softmax(logits[w])[v], the n best in order, equal ones by (w, v).  Totals are 64-bit numbers;
-    where those do not tell a beam's candidates apart (scores or logits beyond 2^50), they are n of its largest logits.
+    far.  Of all continuations of a request's beams, total[w, v] = scores[w] + log_softmax(logits[w])[v], the n best in order, equal ones by (w, v).
+
+    Totals are formed and ranked in 64 bits, from sums of exponentials whose terms carry 2^-22 and their distance from the maximum 1.3e-8 of itself (a total is off by less than
+    2^-18): within a beam the order is that of its logits; of two beams whose totals are closer than that either may come first.  Where 64 bits do not tell a beam's totals apart
+    (logits whose difference is below 2^-53 of the score or the largest logit), they are n of its largest logits.  Scores come back in fp32; a total below its range as -inf.
 
     Logits that are not finite are masked: they are no candidates and have no part in the softmax.  A beam whose score is not finite (-inf: not alive yet, or dead), or that
     has no logit left, has no candidates.  ``weight`` fp32 [requests, width]: candidates are ranked by weight * total (length to the power -alpha, say; totals come back
@@ -2302,8 +2305,8 @@ def _beam_reorder_check(states, parent, slots) -> None:
 def beam_reorder(states: Sequence[torch.Tensor], parent: torch.Tensor, slots: Optional[torch.Tensor] = None) -> Sequence[torch.Tensor]:
     """Rows of recurrent states follow their beams, in place: with parent int32 [requests, width] row slots[b, i] of every state becomes what row
     slots[b, parent[b, i]] was; parent -1 (or outside the request): the row stays as it is.  states: contiguous tensors [slots, ...] of any types, all of one number of slots
-    (of a stack of layers: one each), none of which overlaps another.  slots int32 [requests, width] (None: b * width + i); a slot belongs to one beam: one that is named twice receives either row; one outside
-    the states is skipped.  Returns ``states``."""
+    (of a stack of layers: one each), none of which overlaps another.  slots int32 [requests, width] (None: b * width + i); a slot belongs to one beam: one that a request names twice receives the row of the last of its beams that move,
+    one that two requests name parts of either's; one outside the states is skipped.  Returns ``states``."""
     dev, by, k = _device_index(), parent.shape, len(states)
     ok = (parent.get_device() == dev and parent.dtype is torch.int32 and len(by) == 2 and parent.is_contiguous() and 0 < by[0] <= 65535 and 0 < by[1] <= BEAM_MAX_WIDTH
           and (slots is None or (slots.get_device() == dev and slots.dtype is torch.int32 and slots.shape == by and slots.is_contiguous())))
