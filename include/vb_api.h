@@ -983,7 +983,8 @@ int vb_compact_pages(const VbPagePool* pool, const VbPagePool* out, const VbPage
  *   request hold in the same column is read once for (up to 32, and up to 128 / (n_q / n_kv)) of them.  d_buffer: vb_shared_plan_bytes (0: sizes that are refused), 16-byte aligned,
  *   written by vb_shared_plan once a step and by every vb_shared_attn (one stream at a time).  head_dim 64 or 128, page_size a multiple of 16, grid: blocks that run at once (two an SM).
  * vb_shared_plan: d_table [rows][columns], d_tokens [rows] (0: a row without tokens, its output is zero); entries that are no page are skipped.
- * vb_shared_attn: d_row_tokens (or NULL) [rows]: what the rows of the calling step hold; where the plan's differ zeros come out and flag 7 of vb_wait_flags is set.  q / out [rows][n_q][head_dim] bf16 (out_xt_tile > 0: the tiled layout), d_kv [slabs][2][page_size][n_kv][head_dim] bf16, slab_base = layer * pages. */
+ *   d_row_tokens (or NULL) [rows]: what the rows of the calling step hold; where the plan's differ zeros come out and flag 7 of vb_wait_flags is set.
+ * vb_shared_attn: q / out [rows][n_q][head_dim] bf16 (out_xt_tile > 0: the tiled layout), d_kv [slabs][2][page_size][n_kv][head_dim] bf16, slab_base = layer * pages. */
 typedef struct {
   void* d_buffer;
   int32_t rows, width, columns, page_size, n_q, n_kv, head_dim, grid;

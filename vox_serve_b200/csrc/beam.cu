@@ -15,9 +15,10 @@
 // of HBM.  What is above that: 512 blocks on 148 SMs, three or four each; 2.2 us a chunk of four blocks of an SM (its 64 KB are 1.3 of HBM, its exponentials 0.9 of the
 // special function unit; the rest are instructions and a meeting of the block), 8 to 13 of cuts, orders, launches and the join.  16 of 5 over 32003 fp32 tokens, n 10: 12.1 us.
 // One of two over 2051: 5.7, most of it the launch.
-// The bf16 form is held at 64 registers for four blocks an SM and spills 148 bytes a thread in its stream.  Four blocks an SM with two chunks in shared memory: 31.2 us; three with three 33.3, with four 32.6; four with three 34.4 (a list of 512); five with two 31.6.  Parts so
-// that all blocks run at once: more of them pay the first cut and the last order again, fewer leave SMs idle.  Lists are cut back once they hold twice what is wanted: open
-// rows 45.7 us, three times 46.6, four 47.2, at 256 53.7 (masked ones 32.6, 32.2, 32.1, 32.0).
+// The bf16 form is held at 64 registers for four blocks an SM and spills 148 bytes a thread in its stream.  Four blocks an SM with two chunks in shared memory: 31.2 us;
+// three with three 33.3, with four 32.6; four with three 34.4 (a list of 512); five with two 31.6.  Parts so that all blocks run at once: more of them pay the first cut and
+// the last order again, fewer leave SMs idle.  Lists are cut back once they hold twice what is wanted: open rows 45.7 us, three times 46.6, four 47.2, at 256 53.7 (masked
+// ones 32.6, 32.2, 32.1, 32.0).
 #include "../../include/vb_api.h"
 #define VB_PDL_FAMILY 16
 #include "rowmma.cuh"
@@ -628,8 +629,8 @@ __global__ void __launch_bounds__(THREADS) beam_join_kernel(const __grid_constan
   beam_join<THREADS>(sh, bj_key, p, blockIdx.x, p.stats + first, p.best + first * p.n);
 }
 
-// Both in one launch where a request's parts are few and all requests run at once (beam_one_launch): a cluster a request, whose blocks leave what they found in the first one's shared memory.  (One beam of two
-// over 2051 tokens: 6.45 -> 5.9 us in a graph, the call 16.1 -> 13.6.)
+// Both in one launch where a request's parts are few and all requests run at once (beam_one_launch): a cluster a request, whose blocks leave what they found in the
+// first one's shared memory.  (One beam of two over 2051 tokens: 6.45 -> 5.9 us in a graph, the call 16.1 -> 13.6.)
 template <typename T>
 __global__ void __launch_bounds__(BS_THREADS) beam_small_kernel(const __grid_constant__ BeamCall p) {
   extern __shared__ __align__(16) uint8_t bs_raw[];

@@ -23,7 +23,8 @@
 // 80 rows of products put out 12 MB of partial results); 4 rows of 171 tokens, pages of 16: 7.7 us.  Read once for every row (paged_attn) the same take 112, 322 and 13.4.
 // Against paged_attn without anything to share: 8 rows of 1100 tokens 15.2 us beside 18.0, 32 rows of 600 21.0 beside 17.4: a row alone keeps 126 of 128 accumulator
 // rows idle, and that one fetches while the kernel in front still runs.
-// 128 registers for two blocks an SM, of which the heads of 128 spill 96 bytes a thread, those of 64 64.  mma.sync instead of the tcgen05 core took 104 us for the second case.  Three to six blocks' worth of segments an SM instead of two: 54 to 58 for the first (43 then).
+// At 128 registers, for two blocks an SM, heads of 128 spill 96 bytes a thread, heads of 64 spill 64.  mma.sync instead of the tcgen05 core took 104 us for the second case.
+// Three to six blocks' worth of segments an SM instead of two: 54 to 58 for the first (43 then).
 #include "../../include/vb_api.h"
 #define VB_PDL_FAMILY 1
 #include "attn_tc.cuh"

@@ -2258,8 +2258,8 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, n: int, weight: Opti
     """One step of a beam search.  logits [requests * width, vocab] bf16 or fp32 (rows apart by any stride), scores fp32 [requests, width]: the beams' log probabilities so
     far.  Of all continuations of a request's beams, total[w, v] = scores[w] + log_softmax(logits[w])[v], the n best in order, equal ones by (w, v).
 
-    Totals are formed and ranked in 64 bits, from sums of exponentials whose terms carry 2^-22 and their distance from the maximum 1.3e-8 of itself (a total is off by less than
-    2^-18): within a beam the order is that of its logits; of two beams whose totals are closer than that either may come first.  Where 64 bits do not tell a beam's totals apart
+    Totals are formed and ranked in 64 bits, from fp32 sums of exponentials whose terms carry 2^-22 and 1.3e-8 of their distance from the maximum (totals were off by 2^-20 at
+    most, of up to 2^24 tokens): within a beam the order is that of its logits; of two beams whose totals are closer than that either may come first.  Where 64 bits do not tell a beam's totals apart
     (logits whose difference is below 2^-53 of the score or the largest logit), they are n of its largest logits.  Scores come back in fp32; a total below its range as -inf.
 
     Logits that are not finite are masked: they are no candidates and have no part in the softmax.  A beam whose score is not finite (-inf: not alive yet, or dead), or that
